@@ -1196,6 +1196,91 @@ int rlt_rocm_env_evaluate(rlt_rocm_device* device, const rlt_env_runner* env, in
                           const float* initial_states, int n_episodes, int step_limit, float* returns, uint32_t* episode_length, float* summary,
                           void* workspace, size_t workspace_bytes);
 
+/* ----------------------------------------- blocks over sequences (no counterpart in the reference) -- */
+
+/* Element types of the tensors below. Parameters, their gradients and states are fp32 whatever the tensors' type; every sum is held in fp32. */
+enum rlt_type {
+    RLT_TYPE_F32  = 0,
+    RLT_TYPE_BF16 = 1
+};
+
+/* A tensor [steps x rows x heads x channels]: element (t, b, h, c) is at data[t * step_stride + b * row_stride + h * head_stride + c], strides in elements, the channels
+ * of a head side by side. Step-major sequences as the GRU's are step_stride = rows * heads * channels, row_stride = heads * channels, head_stride = channels; a part of a
+ * wider tensor (queries, keys and values from one product) or another order of the axes differs in the strides alone. */
+typedef struct rlt_head_view {
+    void* data;
+    int64_t step_stride, row_stride, head_stride;
+} rlt_head_view;
+
+/* Linear attention with a decay for each head, a recurrent layer whose state is a matrix [key_dim x value_dim] per row and head:
+ *     S_t = a_t S_{t-1} + k_t^T v_t,   output_t = scale * q_t S_t,   a_t = exp(log_decay[head]), or nothing at a reset.
+ * Query head h reads key / value head h / (heads / kv_heads); every query head has its own decay and state. key_dim and value_dim up to 128. */
+typedef struct rlt_linear_attention {
+    const float* log_decay;      /* [heads], <= 0 for a state that forgets (-infinity: only the step itself) */
+    float scale;
+    int32_t type;                /* enum rlt_type of q, k, v, the output and their gradients */
+    int32_t batch;               /* rows */
+    int32_t heads, kv_heads;     /* kv_heads divides heads */
+    int32_t key_dim, value_dim;
+    int32_t reserved;
+} rlt_linear_attention;
+
+/* Scratch memory of a forward (backward = 0) or backward (1) call over `steps` steps; depends on the shapes alone. A workspace belongs to one call at a time. */
+size_t rlt_rocm_linear_attention_workspace_bytes(const rlt_linear_attention* layer, int steps, int backward);
+/* All steps of a sequence. initial_state, final_state [batch x heads x key_dim x value_dim] (NULL: zeros / not wanted; they may be the same buffer); reset [steps x batch] (NULL: none): a row whose
+ * flag is set at step t forgets its state (the initial one too) before that step; lengths [batch] (NULL: all of them): row b has lengths[b] steps (clamped to 0 ... steps), its
+ * output beyond them is zero, its state stays, and what its inputs hold there is not looked at. Within a sequence a NaN or an infinity in an input may reach the outputs of up to 63 steps
+ * before it, whatever the resets say. */
+int rlt_rocm_linear_attention_forward(rlt_rocm_device* device, const rlt_linear_attention* layer, const rlt_head_view* q, const rlt_head_view* k, const rlt_head_view* v,
+                                      const rlt_head_view* output, const float* initial_state, float* final_state, const uint8_t* reset, const int32_t* lengths, int steps,
+                                      void* workspace, size_t workspace_bytes);
+/* Gradients through time, from the layer's inputs alone (the forward pass keeps nothing): d_q, d_k, d_v (zero beyond a row's length), d_initial_state (NULL: not wanted), d_log_decay [heads]
+ * (NULL: not wanted; accumulate = 0 overwrites it, 1 adds to it). d_final_state is the gradient with respect to final_state (NULL: zeros). */
+int rlt_rocm_linear_attention_backward(rlt_rocm_device* device, const rlt_linear_attention* layer, const rlt_head_view* q, const rlt_head_view* k, const rlt_head_view* v,
+                                       const rlt_head_view* d_output, const rlt_head_view* d_q, const rlt_head_view* d_k, const rlt_head_view* d_v,
+                                       const float* initial_state, const float* d_final_state, float* d_initial_state, float* d_log_decay, int accumulate,
+                                       const uint8_t* reset, const int32_t* lengths, int steps, void* workspace, size_t workspace_bytes);
+/* One step of every row, as a rollout or a served sequence takes it: next_state (which may be state itself) and the output of this step. reset [batch] (NULL: none). The views' step_stride is not read. */
+int rlt_rocm_linear_attention_step(rlt_rocm_device* device, const rlt_linear_attention* layer, const rlt_head_view* q, const rlt_head_view* k, const rlt_head_view* v,
+                                   const rlt_head_view* output, const float* state, float* next_state, const uint8_t* reset);
+
+enum rlt_norm {
+    RLT_NORM_NONE  = 0,
+    RLT_NORM_RMS   = 1,          /* x / sqrt(mean(x^2) + epsilon) */
+    RLT_NORM_LAYER = 2           /* (x - mean(x)) / sqrt(mean((x - mean(x))^2) + epsilon) */
+};
+
+/* What stands between two blocks of a residual stream, in one pass: the norm after a block, its gate and residual scale, and the norm before the next block,
+ *     y = x + residual_scale * gate_activation(gate) * (branch_norm(branch) * branch_weights + branch_biases),   h = output_norm(y) * output_weights + output_biases,
+ * row by row over dim columns (at most 8,192). Weights that are NULL are ones, biases that are NULL zeros. */
+typedef struct rlt_residual_norm {
+    int32_t type;                /* enum rlt_type of the tensors [rows x dim] */
+    int32_t dim;
+    int32_t branch_norm, output_norm;      /* enum rlt_norm */
+    int32_t gate_activation;     /* enum rlt_activation */
+    float epsilon;               /* > 0 */
+    const float* branch_weights; const float* branch_biases;      /* [dim] each */
+    const float* output_weights; const float* output_biases;
+    const float* residual_scale;
+    float* d_branch_weights; float* d_branch_biases; float* d_output_weights; float* d_output_biases; float* d_residual_scale;      /* gradients; NULL: not wanted */
+} rlt_residual_norm;
+
+/* gate NULL: no gate. branch NULL: no block before this norm, y is x (gate is not read). y or h NULL: not wanted; y may be x. h is formed from y before y is rounded to its type. */
+int rlt_rocm_residual_norm_forward(rlt_rocm_device* device, const rlt_residual_norm* layer, const void* x, int ldx, const void* branch, int ldb, const void* gate, int ldg,
+                                   void* y, int ldy, void* h, int ldh, int rows);
+size_t rlt_rocm_residual_norm_workspace_bytes(const rlt_residual_norm* layer, int rows);
+/* From the forward pass's branch, gate and y (the residual stream that it left): d_y is the gradient that reaches y from further on (NULL: none), d_h the one that reaches h (NULL: none);
+ * d_x (which may be d_y), d_branch and d_gate (each NULL: not wanted) are overwritten, the layer's d_* too where accumulate = 0; 1 adds to them. */
+int rlt_rocm_residual_norm_backward(rlt_rocm_device* device, const rlt_residual_norm* layer, const void* branch, int ldb, const void* gate, int ldg, const void* y, int ldy,
+                                    const void* d_y, int lddy, const void* d_h, int lddh, void* d_x, int lddx, void* d_branch, int lddb, void* d_gate, int lddg, int rows,
+                                    int accumulate, void* workspace, size_t workspace_bytes);
+
+/* y = residual + (kept ? x / (1 - p) : 0) (residual NULL: zeros), rows x cols; y may be x or residual. Which elements stay is a function of (seed, stream) alone and stored nowhere: element
+ * i = row * cols + column goes by 16 bits of the generator of rlt_rocm_rand_bits_u32, half i % 8 of group i / 8 (the low half of a word first), and stays where they reach
+ * 65536 p, p being `rate` (0 ... 1) rounded to a multiple of 1 / 65536. The gradient with respect to x is the same call on the output's gradient, without a residual. */
+int rlt_rocm_dropout(rlt_rocm_device* device, int type, const void* x, int ldx, const void* residual, int ldr, void* y, int ldy, int rows, int cols, float rate,
+                     uint64_t seed, uint64_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -245,6 +245,25 @@ class OnPolicyDataset(C.Structure):
                 ("terminated", C.c_void_p), ("truncated", C.c_void_p), ("all_reset", C.c_void_p), ("ld", C.c_int32), ("steps_per_env", C.c_int32)]
 
 
+TYPE = {"float32": 0, "bfloat16": 1}
+NORM = {"none": 0, "rms": 1, "layer": 2}
+
+
+class HeadView(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("step_stride", C.c_int64), ("row_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+class LinearAttention(C.Structure):
+    _fields_ = [("log_decay", C.c_void_p), ("scale", C.c_float), ("type", C.c_int32), ("batch", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32),
+                ("key_dim", C.c_int32), ("value_dim", C.c_int32), ("reserved", C.c_int32)]
+
+
+class ResidualNorm(C.Structure):
+    _fields_ = [("type", C.c_int32), ("dim", C.c_int32), ("branch_norm", C.c_int32), ("output_norm", C.c_int32), ("gate_activation", C.c_int32), ("epsilon", C.c_float),
+                ("branch_weights", C.c_void_p), ("branch_biases", C.c_void_p), ("output_weights", C.c_void_p), ("output_biases", C.c_void_p), ("residual_scale", C.c_void_p),
+                ("d_branch_weights", C.c_void_p), ("d_branch_biases", C.c_void_p), ("d_output_weights", C.c_void_p), ("d_output_biases", C.c_void_p), ("d_residual_scale", C.c_void_p)]
+
+
 I, F, P, S, U64 = C.c_int, C.c_float, C.c_void_p, C.c_size_t, C.c_uint64
 LP = C.POINTER(DenseLayer)
 # return codes of the C ABI (include/rlt_rocm.h)
@@ -380,6 +399,14 @@ ROCM_ONLY = {
     "set_update_options": ([P, I, I], I), "set_wait_limit": ([P, C.c_uint32], I),
     "graph_begin_capture": ([P], I), "graph_end_capture": ([P, C.POINTER(P)], I), "graph_launch": ([P, P], I), "graph_destroy": ([P, P], I),
     "advance_streams": ([P, U64], I), "set_stream_offset": ([P, U64], I),
+    "linear_attention_workspace_bytes": ([C.POINTER(LinearAttention), I, I], S),
+    "linear_attention_forward": ([P, C.POINTER(LinearAttention)] + [C.POINTER(HeadView)] * 4 + [P, P, P, P, I, P, S], I),
+    "linear_attention_backward": ([P, C.POINTER(LinearAttention)] + [C.POINTER(HeadView)] * 7 + [P, P, P, P, I, P, P, I, P, S], I),
+    "linear_attention_step": ([P, C.POINTER(LinearAttention)] + [C.POINTER(HeadView)] * 4 + [P, P, P], I),
+    "residual_norm_forward": ([P, C.POINTER(ResidualNorm), P, I, P, I, P, I, P, I, P, I, I], I),
+    "residual_norm_workspace_bytes": ([C.POINTER(ResidualNorm), I], S),
+    "residual_norm_backward": ([P, C.POINTER(ResidualNorm), P, I, P, I, P, I, P, I, P, I, P, I, P, I, P, I, I, I, P, S], I),
+    "dropout": ([P, I, P, I, P, I, P, I, I, I, F, U64, U64], I),
 }
 
 
