@@ -14,32 +14,89 @@ struct DropoutLaunch {
     const uint64_t* stream_offset;
 };
 
-// A thread takes groups of eight elements, what one call of the generator decides: 16 bits an element resolve a rate to 1.5e-5, and the 40 quarter-rate multiplications of a
-// call are shared by twice as many elements as with the words of rand_f32. VECTOR: groups lie in memory as they are counted (rows without a gap between them, or of a multiple of eight columns) on 16-byte
-// boundaries; otherwise element by element.
-template <typename T, bool VECTOR> __global__ __launch_bounds__(256) void dropout_kernel(DropoutLaunch a) {
+enum Layout { DENSE, ROWS, ELEMENTS };      // groups lie side by side on 16-byte boundaries; within rows of whole groups on such boundaries; anything else
+constexpr int UNROLL = 4;
+
+// A group of eight elements is what one call of the generator decides: 16 bits an element resolve a rate to 1.5e-5, and the call's twenty 32 x 32 multiplications are shared by twice as many
+// elements as with the words of rand_f32. A thread takes UNROLL groups, the workgroup's thread count apart, all of whose loads are asked for before the first draw.
+template <typename T, int LAYOUT> __global__ __launch_bounds__(256) void dropout_kernel(DropoutLaunch a) {
+    constexpr int V = 16 / sizeof(T);
     const T* x = (const T*)a.x; const T* residual = (const T*)a.residual; T* y = (T*)a.y;
     const uint64_t stream = a.stream + *a.stream_offset;
-    const size_t groups = (a.count + 7) / 8;
-    for (size_t g = (size_t)blockIdx.x * blockDim.x + threadIdx.x; g < groups; g += (size_t)gridDim.x * blockDim.x) {
-        const size_t first = g * 8;
-        const rlt_u32x4 w = rlt_philox(a.seed, stream, g);
-        const uint32_t words[4] = {w.x, w.y, w.z, w.w};
-        const int n = a.count - first < 8 ? (int)(a.count - first) : 8;
-        size_t row = first / a.cols; int col = (int)(first - row * a.cols);
-        for (int i = 0; i < n; i++) {
-            const uint32_t bits = (words[i >> 1] >> (16 * (i & 1))) & 0xffffu;
-            float v = bits >= a.threshold ? (float)x[row * a.ldx + col] * a.scale : 0.0f;
-            if (residual) v += (float)residual[row * a.ldr + col];
-            y[row * a.ldy + col] = (T)v;
-            if (++col == a.cols) { col = 0; row++; }
+    const size_t groups = (a.count + 7) / 8, whole = a.count / 8, first = (size_t)blockIdx.x * (256 * UNROLL) + threadIdx.x;
+    if constexpr (LAYOUT != ELEMENTS) {
+        float v[UNROLL][8], r[UNROLL][8];
+        size_t ax[UNROLL], ar[UNROLL], ay[UNROLL];
+#pragma unroll
+        for (int j = 0; j < UNROLL; j++) {
+            const size_t g = first + j * 256;
+            if constexpr (LAYOUT == DENSE) ax[j] = ar[j] = ay[j] = g * 8;
+            else {
+                const uint32_t per_row = (uint32_t)a.cols / 8, row = (uint32_t)g / per_row, col = ((uint32_t)g - row * per_row) * 8;
+                ax[j] = (size_t)row * a.ldx + col; ar[j] = (size_t)row * a.ldr + col; ay[j] = (size_t)row * a.ldy + col;
+            }
+            if (g < whole) {
+#pragma unroll
+                for (int i = 0; i < 8; i += V) rlt_load<V>(x + ax[j] + i, v[j] + i);
+                if (residual) {
+#pragma unroll
+                    for (int i = 0; i < 8; i += V) rlt_load<V>(residual + ar[j] + i, r[j] + i);
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < UNROLL; j++) {
+            const size_t g = first + j * 256;
+            const rlt_u32x4 w = rlt_philox(a.seed, stream, g);
+            const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+            if (g < whole) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const uint32_t bits = (i & 1) ? words[i >> 1] >> 16 : words[i >> 1] & 0xffffu;
+                    v[j][i] = bits >= a.threshold ? v[j][i] * a.scale : 0.0f;
+                    if (residual) v[j][i] += r[j][i];
+                }
+#pragma unroll
+                for (int i = 0; i < 8; i += V) rlt_store<V>(y + ay[j] + i, v[j] + i);
+            } else if (g < groups) {      // the last group of a dense tensor
+                for (int i = 0; g * 8 + i < a.count; i++) {
+                    const uint32_t bits = (words[i >> 1] >> (16 * (i & 1))) & 0xffffu;
+                    float e = bits >= a.threshold ? (float)x[g * 8 + i] * a.scale : 0.0f;
+                    if (residual) e += (float)residual[g * 8 + i];
+                    y[g * 8 + i] = (T)e;
+                }
+            }
+        }
+    } else {
+        for (int j = 0; j < UNROLL; j++) {
+            const size_t g = first + j * 256;
+            if (g >= groups) break;
+            const rlt_u32x4 w = rlt_philox(a.seed, stream, g);
+            const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+            size_t row = g * 8 / a.cols; int col = (int)(g * 8 - row * a.cols);
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                if (g * 8 + i >= a.count) break;
+                const uint32_t bits = (i & 1) ? words[i >> 1] >> 16 : words[i >> 1] & 0xffffu;
+                float e = bits >= a.threshold ? (float)x[row * a.ldx + col] * a.scale : 0.0f;
+                if (residual) e += (float)residual[row * a.ldr + col];
+                y[row * a.ldy + col] = (T)e;
+                if (++col == a.cols) { col = 0; row++; }
+            }
         }
     }
 }
 
-template <typename T> void launch(rlt_rocm_device* device, const DropoutLaunch& a) {
-    const size_t groups = (a.count + 7) / 8, blocks = (groups + 255) / 256;
-    hipLaunchKernelGGL((dropout_kernel<T, false>), dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, device->stream, a);
+template <typename T> int launch(rlt_rocm_device* device, const DropoutLaunch& a) {
+    const size_t blocks = ((a.count + 7) / 8 + 256 * UNROLL - 1) / (256 * UNROLL);
+    if (blocks > INT32_MAX) return RLT_E_UNSUPPORTED;
+    const bool aligned = rlt_vectors<T>(a.x, 0) && rlt_vectors<T>(a.y, 0) && (!a.residual || rlt_vectors<T>(a.residual, 0));
+    const bool dense = a.ldx == a.cols && a.ldy == a.cols && (!a.residual || a.ldr == a.cols);
+    const bool rows = a.cols % 8 == 0 && rlt_vectors<T>(a.x, a.ldx) && rlt_vectors<T>(a.y, a.ldy) && (!a.residual || rlt_vectors<T>(a.residual, a.ldr)) && a.count / 8 <= UINT32_MAX;
+    if (aligned && dense) hipLaunchKernelGGL((dropout_kernel<T, DENSE>), dim3((unsigned)blocks), dim3(256), 0, device->stream, a);
+    else if (rows) hipLaunchKernelGGL((dropout_kernel<T, ROWS>), dim3((unsigned)blocks), dim3(256), 0, device->stream, a);
+    else hipLaunchKernelGGL((dropout_kernel<T, ELEMENTS>), dim3((unsigned)blocks), dim3(256), 0, device->stream, a);
+    return rlt_launch_status(device);
 }
 
 }  // namespace
@@ -51,6 +108,5 @@ extern "C" int rlt_rocm_dropout(rlt_rocm_device* device, int type, const void* x
     RLT_REQUIRE(rate >= 0.0f && rate <= 1.0f);      // not a NaN either
     DropoutLaunch a = {x, residual, y, ldx, ldr, ldy, cols, (size_t)rows * cols, (uint32_t)(rate * 65536.0f + 0.5f), 0.0f, seed, stream, device->stream_offset};
     a.scale = a.threshold < 65536u ? (float)(65536.0 / (65536.0 - a.threshold)) : 0.0f;
-    if (type == RLT_TYPE_F32) launch<float>(device, a); else launch<rlt_bf16>(device, a);
-    return rlt_launch_status(device);
+    return type == RLT_TYPE_F32 ? launch<float>(device, a) : launch<rlt_bf16>(device, a);
 }

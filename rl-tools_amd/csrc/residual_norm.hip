@@ -18,11 +18,18 @@ struct NormBackward {
     float* partial;               // [workgroups][SUMS][dim]
 };
 
-// Sums over the THREADS that share a row, every one of which receives them. Consecutive calls take turns with two halves of `lds`: a wavefront that writes one has passed the barrier
+// THREADS share a row: a part of a wavefront, a wavefront (several rows to a workgroup of 256 then, whose wavefronts do not wait for each other) or a workgroup.
+template <int THREADS> constexpr int WORKGROUP = THREADS <= 64 ? 256 : THREADS;
+
+// Sums over the threads that share a row, every one of which receives them. Consecutive calls take turns with two halves of `lds`: a wavefront that writes one has passed the barrier
 // behind which everybody had read it.
 template <int THREADS, int N> __device__ __forceinline__ void row_sums(float (&v)[N], float* lds, int& turn) {
 #pragma unroll
-    for (int i = 0; i < N; i++) v[i] = rlt_wave_sum(v[i]);
+    for (int i = 0; i < N; i++) {
+        asm volatile("" : "+v"(v[i]));      // no contraction into the first exchange: both sides of an exchange round alike (rlt_wave_sum)
+#pragma unroll
+        for (int off = (THREADS < 64 ? THREADS : 64) / 2; off > 0; off >>= 1) v[i] += __shfl_xor(v[i], off, 64);
+    }
     if constexpr (THREADS > 64) {
         constexpr int WAVES = THREADS / 64;
         float* half = lds + turn * WAVES * 4;
@@ -103,21 +110,35 @@ template <int V, int K, int THREADS> __device__ __forceinline__ float normalise(
     return 1.0f / sqrtf(s[0] * inverse_dim + epsilon);
 }
 
-// The gate's activation and its derivative. Functions as rlt_act has them; GELU as x / (1 + e^(-2 z)), which keeps its relative accuracy where 1 + tanh(z) cancels.
-__device__ __forceinline__ float gate_of(float x, int kind, float& slope) {
-    if (kind == RLT_ACT_SIGMOID || kind == RLT_ACT_GELU) {
-        const float a = 0.3989422804014327f, b = 0.044715f, z = kind == RLT_ACT_GELU ? 2.0f * a * fmaf(b * x * x, x, x) : x;
-        const float e = expf(-fabsf(z)), large = 1.0f / (1.0f + e), small = e * large, p = z >= 0.0f ? large : small, q = z >= 0.0f ? small : large;      // p + q = 1
-        if (kind == RLT_ACT_SIGMOID) { slope = p * q; return p; }
-        slope = p * fmaf(2.0f * x * q, a * fmaf(3.0f * b * x, x, 1.0f), 1.0f);
-        return x * p;
+// The gates' activations, in place, and their derivatives. One loop over a thread's gates for each function, not a choice for each gate. Functions as rlt_act has them; sigmoid and GELU, as x / (1 + e^(-2 z)),
+// keep their relative accuracy where 1 + tanh(z) cancels.
+template <int N, bool SLOPES> __device__ __forceinline__ void gates_of(float (&g)[N], float (&slope)[N], int kind) {
+    if (kind == RLT_ACT_SIGMOID) {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const float e = __expf(-fabsf(g[i])), large = __fdividef(1.0f, 1.0f + e), small = e * large;      // e in (0, 1]: both to two units
+            if (SLOPES) slope[i] = small * large;
+            g[i] = g[i] >= 0.0f ? large : small;
+        }
+    } else if (kind == RLT_ACT_IDENTITY) {
+#pragma unroll
+        for (int i = 0; i < N; i++) slope[i] = 1.0f;
+    } else if (kind == RLT_ACT_GELU) {
+        const float a = 0.3989422804014327f, b = 0.044715f;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const float x = g[i], z = 2.0f * a * fmaf(b * x * x, x, x), e = expf(-fabsf(z)), large = 1.0f / (1.0f + e), small = e * large, p = z >= 0.0f ? large : small, q = z >= 0.0f ? small : large;
+            if (SLOPES) slope[i] = p * fmaf(2.0f * x * q, a * fmaf(3.0f * b * x, x, 1.0f), 1.0f);
+            g[i] = x * p;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) { if (SLOPES) slope[i] = rlt_dact(g[i], kind); g[i] = rlt_act(g[i], kind); }
     }
-    slope = rlt_dact(x, kind);
-    return rlt_act(x, kind);
 }
 
-template <typename T, int V, int K, int THREADS> __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void norm_forward_kernel(NormForward a) {
-    constexpr int N = V * K, ROWS = THREADS < 256 ? 256 / THREADS : 1;
+template <typename T, int V, int K, int THREADS> __global__ __launch_bounds__(WORKGROUP<THREADS>) void norm_forward_kernel(NormForward a) {
+    constexpr int N = V * K, ROWS = WORKGROUP<THREADS> / THREADS;
     __shared__ float lds[THREADS > 64 ? 2 * (THREADS / 64) * 4 : 1];
     int turn = 0;
     const int dim = a.p.dim;
@@ -126,19 +147,16 @@ template <typename T, int V, int K, int THREADS> __global__ __launch_bounds__(TH
     load_parameters<V, K, THREADS>(a.p.output_weights, 1.0f, dim, ow); load_parameters<V, K, THREADS>(a.p.output_biases, 0.0f, dim, ob);
     load_parameters<V, K, THREADS>(a.p.residual_scale, 1.0f, dim, scale);
     for (int row = blockIdx.x * ROWS + threadIdx.x / THREADS; row < a.rows; row += gridDim.x * ROWS) {
-        float y[N];
+        float y[N], u[N], g[N];
+        if (a.branch) load_row<V, K, THREADS>((const T*)a.branch + (size_t)row * a.ldb, dim, u);
         load_row<V, K, THREADS>((const T*)a.x + (size_t)row * a.ldx, dim, y);
+        if (a.branch && a.gate) load_row<V, K, THREADS>((const T*)a.gate + (size_t)row * a.ldg, dim, g);
         if (a.branch) {
-            float u[N], g[N];
-            load_row<V, K, THREADS>((const T*)a.branch + (size_t)row * a.ldb, dim, u);
-            if (a.gate) load_row<V, K, THREADS>((const T*)a.gate + (size_t)row * a.ldg, dim, g);
             const float inverse = normalise<V, K, THREADS>(u, a.p.branch_norm, a.p.epsilon, dim, lds, turn);
+            float slope[N];
+            if (a.gate) gates_of<N, false>(g, slope, a.p.gate_activation);
 #pragma unroll
-            for (int i = 0; i < N; i++) {
-                const float n = fmaf(u[i] * inverse, bw[i], bb[i]);
-                float slope;
-                y[i] = fmaf(a.gate ? scale[i] * gate_of(g[i], a.p.gate_activation, slope) : scale[i], n, y[i]);
-            }
+            for (int i = 0; i < N; i++) y[i] = fmaf(a.gate ? scale[i] * g[i] : scale[i], fmaf(u[i] * inverse, bw[i], bb[i]), y[i]);
             // columns beyond dim: u, g and y are zero, a bias is too
         }
         if (a.y) store_row<V, K, THREADS>((T*)a.y + (size_t)row * a.ldy, dim, y);
@@ -169,13 +187,14 @@ template <int V, int K, int THREADS> __device__ __forceinline__ void norm_gradie
     }
 }
 
-template <typename T, int V, int K, int THREADS> __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void norm_backward_kernel(NormBackward a) {
-    constexpr int N = V * K, ROWS = THREADS < 256 ? 256 / THREADS : 1;
-    __shared__ float lds[THREADS > 64 ? 2 * (THREADS / 64) * 4 : 1];
+template <typename T, int V, int K, int THREADS, bool BIASES> __global__ __launch_bounds__(WORKGROUP<THREADS>) void norm_backward_kernel(NormBackward a) {
+    constexpr int N = V * K, ROWS = WORKGROUP<THREADS> / THREADS;
+    __shared__ float lds[THREADS > 64 ? 2 * (THREADS / 64) * 4 : ROWS * THREADS * N];
     int turn = 0;
     const int dim = a.p.dim;
     float bw[N], bb[N], ow[N], scale[N];
-    load_parameters<V, K, THREADS>(a.p.branch_weights, 1.0f, dim, bw); load_parameters<V, K, THREADS>(a.p.branch_biases, 0.0f, dim, bb);
+    load_parameters<V, K, THREADS>(a.p.branch_weights, 1.0f, dim, bw);
+    load_parameters<V, K, THREADS>(BIASES ? a.p.branch_biases : nullptr, 0.0f, dim, bb);
     load_parameters<V, K, THREADS>(a.p.output_weights, 1.0f, dim, ow); load_parameters<V, K, THREADS>(a.p.residual_scale, 1.0f, dim, scale);
     float sums[SUMS][N];
 #pragma unroll
@@ -183,19 +202,25 @@ template <typename T, int V, int K, int THREADS> __global__ __launch_bounds__(TH
 #pragma unroll
         for (int i = 0; i < N; i++) sums[j][i] = 0.0f;
     for (int row = blockIdx.x * ROWS + threadIdx.x / THREADS; row < a.rows; row += gridDim.x * ROWS) {
-        float d[N];      // the gradient that reaches the residual stream
-#pragma unroll
-        for (int i = 0; i < N; i++) d[i] = 0.0f;
-        if (a.d_y) load_row<V, K, THREADS>((const T*)a.d_y + (size_t)row * a.lddy, dim, d);
+        float d[N], e[N], y[N], u[N], g[N];      // d: the gradient that reaches the residual stream
         if (a.d_h) {
-            float e[N], y[N];
             load_row<V, K, THREADS>((const T*)a.d_h + (size_t)row * a.lddh, dim, e);
             load_row<V, K, THREADS>((const T*)a.y + (size_t)row * a.ldy, dim, y);
+        }
+        if (a.d_y) load_row<V, K, THREADS>((const T*)a.d_y + (size_t)row * a.lddy, dim, d);
+        else {
+#pragma unroll
+            for (int i = 0; i < N; i++) d[i] = 0.0f;
+        }
+        if (a.branch) load_row<V, K, THREADS>((const T*)a.branch + (size_t)row * a.ldb, dim, u);
+        if (a.branch && a.gate) load_row<V, K, THREADS>((const T*)a.gate + (size_t)row * a.ldg, dim, g);
+        if (a.d_h) {
             const float inverse = normalise<V, K, THREADS>(y, a.p.output_norm, a.p.epsilon, dim, lds, turn);
 #pragma unroll
             for (int i = 0; i < N; i++) {
                 y[i] *= inverse;
-                sums[OUTPUT_W][i] = fmaf(e[i], y[i], sums[OUTPUT_W][i]); sums[OUTPUT_B][i] += e[i];
+                sums[OUTPUT_W][i] = fmaf(e[i], y[i], sums[OUTPUT_W][i]);
+                if (BIASES) sums[OUTPUT_B][i] += e[i];
                 e[i] *= ow[i];
             }
             norm_gradient<V, K, THREADS>(e, y, inverse, a.p.output_norm, dim, lds, turn);
@@ -204,61 +229,123 @@ template <typename T, int V, int K, int THREADS> __global__ __launch_bounds__(TH
         }
         if (a.d_x) store_row<V, K, THREADS>((T*)a.d_x + (size_t)row * a.lddx, dim, d);
         if (a.branch) {
-            float u[N], g[N], e[N];
-            load_row<V, K, THREADS>((const T*)a.branch + (size_t)row * a.ldb, dim, u);
-            if (a.gate) load_row<V, K, THREADS>((const T*)a.gate + (size_t)row * a.ldg, dim, g);
             const float inverse = normalise<V, K, THREADS>(u, a.p.branch_norm, a.p.epsilon, dim, lds, turn);
+            float slope[N];
+            if (a.gate) gates_of<N, true>(g, slope, a.p.gate_activation);
 #pragma unroll
             for (int i = 0; i < N; i++) {
                 u[i] *= inverse;
-                float slope;
-                const float n = fmaf(u[i], bw[i], bb[i]), m = a.gate ? gate_of(g[i], a.p.gate_activation, slope) : 1.0f, dn = d[i] * scale[i] * m;
+                const float n = BIASES ? fmaf(u[i], bw[i], bb[i]) : u[i] * bw[i], m = a.gate ? g[i] : 1.0f, dn = d[i] * scale[i] * m;
                 sums[SCALE][i] = fmaf(d[i] * m, n, sums[SCALE][i]);
-                sums[BRANCH_W][i] = fmaf(dn, u[i], sums[BRANCH_W][i]); sums[BRANCH_B][i] += dn;
-                if (a.gate) g[i] = d[i] * scale[i] * n * slope;
+                sums[BRANCH_W][i] = fmaf(dn, u[i], sums[BRANCH_W][i]);
+                if (BIASES) sums[BRANCH_B][i] += dn;
+                if (a.gate) slope[i] *= d[i] * scale[i] * n;
                 e[i] = dn * bw[i];
             }
-            if (a.d_gate) store_row<V, K, THREADS>((T*)a.d_gate + (size_t)row * a.lddg, dim, g);
+            if (a.d_gate) store_row<V, K, THREADS>((T*)a.d_gate + (size_t)row * a.lddg, dim, slope);
             if (a.d_branch) {
                 norm_gradient<V, K, THREADS>(e, u, inverse, a.p.branch_norm, dim, lds, turn);
                 store_row<V, K, THREADS>((T*)a.d_branch + (size_t)row * a.lddb, dim, e);
             }
         }
     }
-    float* out = a.partial + ((size_t)blockIdx.x * ROWS + threadIdx.x / THREADS) * SUMS * dim;
     float* const wanted[SUMS] = {a.p.d_branch_weights, a.p.d_branch_biases, a.p.d_output_weights, a.p.d_output_biases, a.p.d_residual_scale};
+    float* out = a.partial + (size_t)blockIdx.x * SUMS * dim;
 #pragma unroll
-    for (int j = 0; j < SUMS; j++)
-        if (wanted[j]) {
+    for (int j = 0; j < SUMS; j++) {
+        if (!wanted[j]) continue;
+        if constexpr (ROWS > 1) {      // the rows' threads side by side, then column by column in their order
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < K; k++)
+#pragma unroll
+                for (int i = 0; i < V; i++) lds[(threadIdx.x / THREADS) * THREADS * N + (k * THREADS + threadIdx.x % THREADS) * V + i] = sums[j][k * V + i];
+            __syncthreads();
+            for (int c = threadIdx.x; c < dim; c += WORKGROUP<THREADS>) {
+                float s = 0.0f;
+#pragma unroll
+                for (int r = 0; r < ROWS; r++) s += lds[r * THREADS * N + c];
+                out[(size_t)j * dim + c] = s;
+            }
+        } else {
 #pragma unroll
             for (int k = 0; k < K; k++)
 #pragma unroll
                 for (int i = 0; i < V; i++) {
-                    const int c = (k * THREADS + (int)(threadIdx.x % THREADS)) * V + i;
+                    const int c = (k * THREADS + (int)threadIdx.x) * V + i;
                     if (c < dim) out[(size_t)j * dim + c] = sums[j][k * V + i];
                 }
         }
+    }
 }
 
-// adds up the workgroups' column sums, in their order: 64 columns to a workgroup, whose wavefronts take every fourth block each
-__global__ __launch_bounds__(256) void norm_sum_kernel(const float* __restrict__ partial, int blocks, int dim, rlt_residual_norm p, int accumulate) {
-    __shared__ float part[4][64];
+// adds up the workgroups' column sums, in a fixed order: 64 columns to a workgroup, whose wavefronts take every sixteenth block each
+__global__ __launch_bounds__(1024) void norm_sum_kernel(const float* __restrict__ partial, int blocks, int dim, rlt_residual_norm p, int accumulate) {
+    __shared__ float part[16][64];
     float* const to[SUMS] = {p.d_branch_weights, p.d_branch_biases, p.d_output_weights, p.d_output_biases, p.d_residual_scale};
     float* dst = to[blockIdx.y];
     if (!dst) return;
-    const int c = blockIdx.x * 64 + (threadIdx.x & 63), wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, c = blockIdx.x * 64 + lane, wave = threadIdx.x >> 6;
     float s = 0.0f;
     if (c < dim)
-        for (int b = wave; b < blocks; b += 4) s += partial[((size_t)b * SUMS + blockIdx.y) * dim + c];
-    part[wave][threadIdx.x & 63] = s;
+#pragma unroll 8
+        for (int b = wave; b < blocks; b += 16) s += partial[((size_t)b * SUMS + blockIdx.y) * dim + c];
+    part[wave][lane] = s;
     __syncthreads();
     if (wave == 0 && c < dim) {
-        s = ((part[0][threadIdx.x] + part[1][threadIdx.x]) + part[2][threadIdx.x]) + part[3][threadIdx.x];
+        s = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 16; w++) s += part[w][lane];
         dst[c] = accumulate ? dst[c] + s : s;
     }
 }
 
-int backward_blocks(const rlt_residual_norm*, int rows) { return rows < 256 ? rows : 256; }
+// threads that share a row in the backward pass, eight columns each
+int backward_threads(int dim) { return dim <= 128 ? 16 : dim <= 512 ? 64 : dim <= 1024 ? 128 : dim <= 2048 ? 256 : dim <= 4096 ? 512 : 1024; }
+int backward_blocks(const rlt_residual_norm* p, int rows) {
+    const int threads = backward_threads(p->dim), at_once = threads <= 64 ? 256 / threads : 1, blocks = (rows + at_once - 1) / at_once;
+    return blocks < 512 ? blocks : 512;
+}
+
+template <typename T, int V> void launch_forward(rlt_rocm_device* device, const NormForward& a) {
+    const int dim = a.p.dim;
+    auto go = [&](auto kernel, int threads) {
+        const int workgroup = threads <= 64 ? 256 : threads, at_once = workgroup / threads, blocks = (a.rows + at_once - 1) / at_once;
+        hipLaunchKernelGGL(kernel, dim3(blocks < 2048 ? blocks : 2048), dim3(workgroup), 0, device->stream, a);
+    };
+    if (dim <= 128) go(norm_forward_kernel<T, V, 8 / V, 16>, 16);
+    else if (dim <= 512) go(norm_forward_kernel<T, V, 8 / V, 64>, 64);
+    else if (dim <= 1024) go(norm_forward_kernel<T, V, 8 / V, 128>, 128);
+    else if (dim <= 2048) go(norm_forward_kernel<T, V, 8 / V, 256>, 256);
+    else if (dim <= 4096) go(norm_forward_kernel<T, V, 8 / V, 512>, 512);
+    else go(norm_forward_kernel<T, V, 8 / V, 1024>, 1024);
+}
+template <typename T, int V, bool BIASES> void launch_backward(rlt_rocm_device* device, const NormBackward& a) {
+    const int threads = backward_threads(a.p.dim);
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(backward_blocks(&a.p, a.rows)), dim3(threads <= 64 ? 256 : threads), 0, device->stream, a); };
+    if (threads == 16) go(norm_backward_kernel<T, V, 8 / V, 16, BIASES>);
+    else if (threads == 64) go(norm_backward_kernel<T, V, 8 / V, 64, BIASES>);
+    else if (threads == 128) go(norm_backward_kernel<T, V, 8 / V, 128, BIASES>);
+    else if (threads == 256) go(norm_backward_kernel<T, V, 8 / V, 256, BIASES>);
+    else if (threads == 512) go(norm_backward_kernel<T, V, 8 / V, 512, BIASES>);
+    else go(norm_backward_kernel<T, V, 8 / V, 1024, BIASES>);
+}
+// vectors of 16 bytes where every tensor's rows start on such boundaries and hold whole vectors
+template <typename T> void forward(rlt_rocm_device* device, const NormForward& a) {
+    constexpr int V = 16 / sizeof(T);
+    const bool vectors = a.p.dim % V == 0 && rlt_vectors<T>(a.x, a.ldx) && rlt_vectors<T>(a.branch, a.branch ? a.ldb : 0) && rlt_vectors<T>(a.gate, a.gate ? a.ldg : 0) &&
+                         rlt_vectors<T>(a.y, a.y ? a.ldy : 0) && rlt_vectors<T>(a.h, a.h ? a.ldh : 0);
+    if (vectors) launch_forward<T, V>(device, a); else launch_forward<T, 1>(device, a);
+}
+template <typename T> void backward(rlt_rocm_device* device, const NormBackward& a) {
+    constexpr int V = 16 / sizeof(T);
+    const bool vectors = a.p.dim % V == 0 && rlt_vectors<T>(a.branch, a.branch ? a.ldb : 0) && rlt_vectors<T>(a.gate, a.gate ? a.ldg : 0) && rlt_vectors<T>(a.y, a.d_h ? a.ldy : 0) &&
+                         rlt_vectors<T>(a.d_y, a.d_y ? a.lddy : 0) && rlt_vectors<T>(a.d_h, a.d_h ? a.lddh : 0) && rlt_vectors<T>(a.d_x, a.d_x ? a.lddx : 0) &&
+                         rlt_vectors<T>(a.d_branch, a.d_branch ? a.lddb : 0) && rlt_vectors<T>(a.d_gate, a.d_gate ? a.lddg : 0);
+    const bool biases = a.p.branch_biases || a.p.d_branch_biases || a.p.d_output_biases;
+    if (vectors) { if (biases) launch_backward<T, V, true>(device, a); else launch_backward<T, V, false>(device, a); }
+    else { if (biases) launch_backward<T, 1, true>(device, a); else launch_backward<T, 1, false>(device, a); }
+}
 
 bool described(const rlt_residual_norm* p) {
     return p && (p->type == RLT_TYPE_F32 || p->type == RLT_TYPE_BF16) && p->dim > 0 && p->branch_norm >= RLT_NORM_NONE && p->branch_norm <= RLT_NORM_LAYER && p->output_norm >= RLT_NORM_NONE &&
@@ -277,8 +364,7 @@ int rlt_rocm_residual_norm_forward(rlt_rocm_device* device, const rlt_residual_n
     RLT_REQUIRE(x && ldx >= dim && (!branch || ldb >= dim) && (!gate || ldg >= dim) && (!y || ldy >= dim) && (!h || ldh >= dim) && (y || h));
     if (dim > MAX_DIM) return RLT_E_UNSUPPORTED;
     const NormForward a = {*layer, x, branch, gate, y, h, ldx, ldb, ldg, ldy, ldh, rows};
-    if (layer->type == RLT_TYPE_F32) hipLaunchKernelGGL((norm_forward_kernel<float, 1, 8, 1024>), dim3(rows < 1024 ? rows : 1024), dim3(1024), 0, device->stream, a);
-    else hipLaunchKernelGGL((norm_forward_kernel<rlt_bf16, 1, 8, 1024>), dim3(rows < 1024 ? rows : 1024), dim3(1024), 0, device->stream, a);
+    if (layer->type == RLT_TYPE_F32) forward<float>(device, a); else forward<rlt_bf16>(device, a);
     return rlt_launch_status(device);
 }
 
@@ -301,12 +387,10 @@ int rlt_rocm_residual_norm_backward(rlt_rocm_device* device, const rlt_residual_
     const bool sums = layer->d_branch_weights || layer->d_branch_biases || layer->d_output_weights || layer->d_output_biases || layer->d_residual_scale;
     RLT_REQUIRE(!sums || (workspace && workspace_bytes >= rlt_rocm_residual_norm_workspace_bytes(layer, rows)));
     const NormBackward a = {*layer, branch, gate, y, d_y, d_h, d_x, d_branch, d_gate, ldb, ldg, ldy, lddy, lddh, lddx, lddb, lddg, rows, (float*)workspace};
-    const int blocks = backward_blocks(layer, rows);
-    if (layer->type == RLT_TYPE_F32) hipLaunchKernelGGL((norm_backward_kernel<float, 1, 8, 1024>), dim3(blocks), dim3(1024), 0, device->stream, a);
-    else hipLaunchKernelGGL((norm_backward_kernel<rlt_bf16, 1, 8, 1024>), dim3(blocks), dim3(1024), 0, device->stream, a);
+    if (layer->type == RLT_TYPE_F32) backward<float>(device, a); else backward<rlt_bf16>(device, a);
     int rc = rlt_launch_status(device);
     if (rc || !sums) return rc;
-    hipLaunchKernelGGL(norm_sum_kernel, dim3((dim + 63) / 64, SUMS), dim3(256), 0, device->stream, (const float*)workspace, blocks, dim, *layer, accumulate);
+    hipLaunchKernelGGL(norm_sum_kernel, dim3((dim + 63) / 64, SUMS), dim3(1024), 0, device->stream, (const float*)workspace, backward_blocks(layer, rows), dim, *layer, accumulate);
     return rlt_launch_status(device);
 }
 
