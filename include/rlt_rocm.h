@@ -1225,7 +1225,8 @@ typedef struct rlt_linear_attention {
     int32_t reserved;
 } rlt_linear_attention;
 
-/* Scratch memory of a forward (backward = 0) or backward (1) call over `steps` steps; depends on the shapes alone. A workspace belongs to one call at a time. */
+/* Scratch memory of a forward (backward = 0) or backward (1) call over `steps` steps; depends on the shapes alone. A workspace starts on
+ * a 16-byte boundary and belongs to one call at a time. */
 size_t rlt_rocm_linear_attention_workspace_bytes(const rlt_linear_attention* layer, int steps, int backward);
 /* All steps of a sequence. initial_state, final_state [batch x heads x key_dim x value_dim] (NULL: zeros / not wanted; they may be the same buffer); reset [steps x batch] (NULL: none): a row whose
  * flag is set at step t forgets its state (the initial one too) before that step; lengths [batch] (NULL: all of them): row b has lengths[b] steps (clamped to 0 ... steps), its

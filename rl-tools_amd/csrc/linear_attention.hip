@@ -3,104 +3,409 @@
 
 namespace {
 
-constexpr int MAX_WIDTH = 128;
+constexpr int MAX_WIDTH = 128, CHUNK = 64;
 
-// a tensor as the kernels see it: heads / group of it
-struct Part { const void* data; int64_t step, row, head; int group; };
+// a tensor as the kernels see it: heads / group of it; four channels side by side are one vector where `vectors` is set
+struct Part { void* data; int64_t step, row, head; int group, vectors; };
+// One direction of the layer over segments of the steps. "key" and "value" are the two factors of what is added to the state [key x value], "query" what reads it.
 struct Walk {
-    Part q, k, v;                 // what reads the state, and the two factors of what is added to it
-    Part out;                     // written
-    const float* log_decay; const float* initial; float* final;
+    Part q, k, v, out;
+    Part with;                    // SLOPE: what the output's derivative by the decay's logarithm is multiplied with
+    const float* log_decay;
+    const float* entry;           // state that a walk starts from (NULL: zeros): of row and head, or of row, head and segment where there are several
+    float* exit;                  // state that it ends with (NULL: not wanted), the same
+    const float* entry_slope; float* exit_slope;
+    const float* d_final;         // SLOPE: gradient with respect to the final state (NULL: zeros)
+    float* partial;               // SLOPE: [rows x heads x segments]
+    float2* factors;              // STATE: what a segment multiplies the state by (0: it forgets), and its steps
     const uint8_t* reset; const int32_t* lengths;
-    float scale_out, scale_added;
-    int batch, heads, steps, key, value;
+    float score_scale, read_scale, added_scale;
+    int batch, heads, steps, key, value, segments, segment_steps;
+    int state_key, state_value;   // strides of the state in memory
 };
 
 template <typename T> __device__ __forceinline__ T* at(const Part& p, int t, int b, int h) {
     return (T*)p.data + ((int64_t)t * p.step + (int64_t)b * p.row + (int64_t)(h / p.group) * p.head);
 }
 
-// One workgroup per row and head walks the steps; thread c holds column c of the state. Forward: the state decays, takes k^T v in and is read by q. REVERSE: it takes k^T v in, is read and decays.
-// TRANSPOSED: the state lies in memory as [value x key].
-template <typename T, typename O, bool REVERSE, bool TRANSPOSED> __global__ __launch_bounds__(MAX_WIDTH) void walk_kernel(Walk a) {
-    __shared__ float q[MAX_WIDTH], k[MAX_WIDTH];
-    const int h = blockIdx.x % a.heads, b = blockIdx.x / a.heads, c = threadIdx.x;
-    const float decay = expf(a.log_decay[h]);
-    const size_t base = ((size_t)b * a.heads + h) * a.key * a.value;
-    float state[MAX_WIDTH];
+// Operands of the matrix instructions: eight values a lane, lane l having row (column) l % 16 and, of 32 summands, those that its quarter l / 16 selects. bfloat16: one 16x16x32 instruction; fp32: eight
+// 16x16x4 instructions, the e-th of which takes value e of every lane. Which summands a quarter has is free as long as both operands agree.
+typedef float rlt_f32x8 __attribute__((ext_vector_type(8)));
+template <typename T> struct Operand;
+template <> struct Operand<float> { typedef rlt_f32x8 Vector; typedef rlt_f32x4 Quad; };
+template <> struct Operand<rlt_bf16> { typedef rlt_bf16x8 Vector; typedef rlt_bf16x4 Quad; };
+__device__ __forceinline__ rlt_f32x4 multiply(rlt_f32x8 a, rlt_f32x8 b, rlt_f32x4 c) {
 #pragma unroll
-    for (int i = 0; i < MAX_WIDTH; i++) state[i] = a.initial && c < a.value && i < a.key ? a.initial[base + (TRANSPOSED ? c * a.key + i : i * a.value + c)] : 0.0f;
-    const int length = a.lengths ? min(max(a.lengths[b], 0), a.steps) : a.steps;
-    for (int s = 0; s < a.steps; s++) {
-        const int t = REVERSE ? a.steps - 1 - s : s;
-        if (t >= length) {
-            if (a.out.data && c < a.value) at<O>(a.out, t, b, h)[c] = (O)0.0f;
-            continue;
-        }
-        __syncthreads();
-        q[c] = c < a.key ? (float)at<T>(a.q, t, b, h)[c] : 0.0f;
-        k[c] = c < a.key ? (float)at<T>(a.k, t, b, h)[c] * a.scale_added : 0.0f;
-        const float v = c < a.value ? (float)at<T>(a.v, t, b, h)[c] : 0.0f;
-        __syncthreads();
-        const bool forget = a.reset && a.reset[(size_t)t * a.batch + b];
-        float out = 0.0f;
+    for (int e = 0; e < 8; e++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
+    return c;
+}
+__device__ __forceinline__ rlt_f32x4 multiply(rlt_bf16x8 a, rlt_bf16x8 b, rlt_f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+
+// fp32 values as operands. For bfloat16 kernels they are cut into parts whose sum they are to 2^-16 (two) or exactly to fp32 (three): what a product adds to the state, and what a gradient that stays in fp32 is made of, take three,
+// what only goes into an output that is rounded to bfloat16 takes two.
+template <typename T, int PARTS> struct Cut {
+    rlt_bf16x8 part[PARTS];
+    __device__ __forceinline__ explicit Cut(rlt_f32x8 x) {
 #pragma unroll
-        for (int i = 0; i < MAX_WIDTH; i++) {
-            if (!REVERSE) state[i] = forget ? 0.0f : state[i] * decay;
-            state[i] = fmaf(k[i], v, state[i]);
-            out = fmaf(q[i], state[i], out);
-            if (REVERSE) state[i] = forget ? 0.0f : state[i] * decay;
+        for (int p = 0; p < PARTS; p++) {
+            part[p] = __builtin_convertvector(x, rlt_bf16x8);
+            if (p + 1 < PARTS) x -= __builtin_convertvector(part[p], rlt_f32x8);
         }
-        if (a.out.data && c < a.value) at<O>(a.out, t, b, h)[c] = (O)(out * a.scale_out);
     }
-    if (a.final)
+};
+template <int PARTS> struct Cut<float, PARTS> {
+    rlt_f32x8 part[1];
+    __device__ __forceinline__ explicit Cut(rlt_f32x8 x) { part[0] = x; }
+};
+template <typename T, int PARTS> constexpr int CUTS = sizeof(T) == 4 ? 1 : PARTS;
+
+// decay^n; n = 0 gives 1 also for a decay of zero
+__device__ __forceinline__ float power(float log2_decay, int n) { return n == 0 ? 1.0f : __builtin_amdgcn_exp2f(log2_decay * (float)n); }
+
+template <typename T, int D, bool SLOPE, bool STATE> struct Layout {
+    static constexpr bool NARROW = sizeof(T) == 2;
+    static constexpr int PAD = 16 / sizeof(T), ROW = D + PAD, COLUMN = CHUNK + PAD;      // rows start 4 (of 64) banks after each other: sixteen of them side by side in 16 bytes each meet no bank twice
+    static constexpr int PLANES = NARROW ? 2 : 1;
+    static constexpr int Q = 0, KR = Q + (STATE ? 0 : CHUNK * ROW), KT = KR + (STATE && NARROW ? 0 : CHUNK * ROW), VT = KT + (NARROW ? D * COLUMN : 0);      // narrow: keys and values also by columns
+    static constexpr int VR = VT + (NARROW ? D * COLUMN : 0), WR = VR + (!NARROW || (SLOPE && !STATE) ? CHUNK * ROW : 0), P = WR + (SLOPE && !STATE ? CHUNK * ROW : 0);
+    static constexpr int TOTAL = P + (STATE ? 0 : PLANES * CHUNK * COLUMN);
+    static constexpr size_t BYTES = TOTAL * sizeof(T);
+};
+
+// Chunks of 64 steps. With i, s the steps of a chunk (n of them within the row's length), S the state before it and a the decay:
+//     out_i = sum over s <= i of a^(i-s) (q_i k_s) v_s + a^(i+1) q_i S,     S <- a^n S + sum over s of a^(n-1-s) k_s^T v_s
+// where a reset between the two steps of a power makes it zero. REVERSE is the transposed recurrence of the gradients, from the last step to the first:
+//     out_i = sum over s >= i of a^(s-i) (q_i k_s) v_s + a^(n-1-i) q_i R,   R <- a^n R + sum over s of a^(s+1) k_s^T v_s.
+// A wavefront owns 16 of the value columns: their state stays in its accumulators from chunk to chunk, laid out as the matrix instruction leaves them, which is (with the summands in an order of their own) how the
+// product with the queries takes them. Scores of a chunk are shared out in tiles of 16 x 16, weighted, and exchanged through LDS.
+template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE> __global__ __launch_bounds__(4 * D) void walk_kernel(Walk a) {
+    typedef typename Operand<T>::Vector Vector;
+    typedef typename Operand<T>::Quad Quad;
+    typedef Layout<T, D, SLOPE, STATE> L;
+    constexpr int KEY_TILES = D / 16, KEY_BLOCKS = D / 32, WAVES = D / 16, STATE_CUTS = CUTS<T, SLOPE ? 3 : 2>, ADDED_CUTS = CUTS<T, 3>;
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds_bytes[];
+    T* const lds = (T*)lds_bytes;
+    const int pair = blockIdx.x / a.segments, segment = blockIdx.x % a.segments, b = pair / a.heads, h = pair % a.heads;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, quarter = lane >> 4;
+    const int length = a.lengths ? min(max(a.lengths[b], 0), a.steps) : a.steps;
+    const float log2_decay = a.log_decay[h] * 1.44269504088896341f;
+    const int begin = segment * a.segment_steps, end = min(begin + a.segment_steps, a.steps), chunks = (end - begin + CHUNK - 1) / CHUNK;
+
+    // state: tile k, element r of this lane is row 16 k + 4 quarter + r, column 16 wave + l
+    rlt_f32x4 state[KEY_TILES], slope[SLOPE ? KEY_TILES : 1];
+    const int column = 16 * wave + l;
+    const size_t state_base = ((size_t)pair * a.segments + segment) * a.key * a.value;
 #pragma unroll
-        for (int i = 0; i < MAX_WIDTH; i++)
-            if (c < a.value && i < a.key) a.final[base + (TRANSPOSED ? c * a.key + i : i * a.value + c)] = state[i];
+    for (int k = 0; k < KEY_TILES; k++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const int row = 16 * k + 4 * quarter + r;
+            const bool there = row < a.key && column < a.value;
+            const size_t i = state_base + (size_t)row * a.state_key + (size_t)column * a.state_value;
+            state[k][r] = !STATE && a.entry && there ? a.entry[i] : 0.0f;
+            if constexpr (SLOPE) slope[k][r] = !STATE && a.entry_slope && there ? a.entry_slope[i] : 0.0f;
+        }
+
+    // what a thread carries from memory to LDS: four steps of four channels of each tensor
+    const int channel = (threadIdx.x % (D / 4)) * 4, first = (threadIdx.x / (D / 4)) * 4;
+    Quad next_q[4], next_k[4], next_v[4], next_with[4];
+    uint8_t next_reset = 0;
+    auto fetch = [&](const Part& p, int width, int t0, Quad (&to)[4]) {
+        const T* src = at<T>(p, t0 + first, b, h) + channel;
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+#pragma unroll
+            for (int c = 0; c < 4; c++) to[r][c] = (T)0.0f;
+            if (t0 + first + r < min(length, end)) {
+                if (p.vectors) { if (channel < width) to[r] = *reinterpret_cast<const Quad*>(src + (int64_t)r * p.step); }
+                else {
+#pragma unroll
+                    for (int c = 0; c < 4; c++) if (channel + c < width) to[r][c] = src[(int64_t)r * p.step + c];
+                }
+            }
+        }
+    };
+    auto fetch_chunk = [&](int chunk) {
+        const int t0 = begin + chunk * CHUNK;
+        if constexpr (!STATE) fetch(a.q, a.key, t0, next_q);
+        fetch(a.k, a.key, t0, next_k);
+        fetch(a.v, a.value, t0, next_v);
+        if constexpr (SLOPE && !STATE) fetch(a.with, a.value, t0, next_with);
+        next_reset = a.reset && t0 + lane < min(length, end) ? a.reset[(size_t)(t0 + lane) * a.batch + b] : (uint8_t)0;
+    };
+    auto put_rows = [&](int base, const Quad (&from)[4]) {
+#pragma unroll
+        for (int r = 0; r < 4; r++) *reinterpret_cast<Quad*>(lds + base + (first + r) * L::ROW + channel) = from[r];
+    };
+    auto put_columns = [&](int base, const Quad (&from)[4]) {
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            Quad x;
+#pragma unroll
+            for (int r = 0; r < 4; r++) x[r] = from[r][c];
+            *reinterpret_cast<Quad*>(lds + base + (channel + c) * L::COLUMN + first) = x;
+        }
+    };
+    // operands: eight summands 32 block + 8 quarter ... of a row; of a row in the order of the accumulators; of a column over the steps
+    auto row_operand = [&](int base, int stride, int row, int block) { return *reinterpret_cast<const Vector*>(lds + base + row * stride + 32 * block + 8 * quarter); };
+    auto tiled_operand = [&](int base, int row, int block) {
+        const Quad x = *reinterpret_cast<const Quad*>(lds + base + row * L::ROW + 32 * block + 4 * quarter), y = *reinterpret_cast<const Quad*>(lds + base + row * L::ROW + 32 * block + 16 + 4 * quarter);
+        return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    auto column_operand = [&](int narrow_base, int rows_base, int col, int block) {
+        if constexpr (L::NARROW) return row_operand(narrow_base, L::COLUMN, col, block);
+        else {
+            Vector x;
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = lds[rows_base + (32 * block + 8 * quarter + e) * L::ROW + col];
+            return x;
+        }
+    };
+    auto state_vector = [&](const rlt_f32x4 (&s)[KEY_TILES], int block) { return __builtin_shufflevector(s[2 * block], s[2 * block + 1], 0, 1, 2, 3, 4, 5, 6, 7); };
+
+    if constexpr (!STATE) {      // score tiles that lie on the wrong side of the diagonal within a block of 32: zero for good
+        constexpr int O0 = REVERSE ? 16 : 0, S0 = REVERSE ? 0 : 16;
+        for (int i = threadIdx.x; i < L::PLANES * 2 * 16 * 16; i += 4 * D) {
+            const int plane = i / 512, which = (i / 256) % 2, row = (i / 16) % 16, col = i % 16;
+            lds[L::P + plane * CHUNK * L::COLUMN + (32 * which + O0 + row) * L::COLUMN + 32 * which + S0 + col] = (T)0.0f;
+        }
+    }
+    float total = 0.0f;                       // SLOPE
+    float added_weight[2][8];                 // of the chunk's steps in the state after it
+    int weights_of = -1;                      // the number of steps that they are for
+    int counted = 0; bool forgotten = false;  // STATE
+    if (chunks > 0) fetch_chunk(REVERSE ? chunks - 1 : 0);
+    for (int c = 0; c < chunks; c++) {
+        const int chunk = REVERSE ? chunks - 1 - c : c, t0 = begin + chunk * CHUNK, n = min(max(min(length, end) - t0, 0), CHUNK);
+        const uint64_t resets = __ballot(next_reset != 0);
+        rlt_lds_barrier();
+        if constexpr (!STATE) put_rows(L::Q, next_q);
+        if constexpr (!STATE || !L::NARROW) put_rows(L::KR, next_k);
+        if constexpr (L::NARROW) { put_columns(L::KT, next_k); put_columns(L::VT, next_v); }
+        if constexpr (!L::NARROW || (SLOPE && !STATE)) put_rows(L::VR, next_v);
+        if constexpr (SLOPE && !STATE) put_rows(L::WR, next_with);
+        rlt_lds_barrier();
+        if (c + 1 < chunks) fetch_chunk(REVERSE ? chunk - 1 : chunk + 1);
+
+        if (n != weights_of) {
+            weights_of = n;
+#pragma unroll
+            for (int block = 0; block < 2; block++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const int s = 32 * block + 8 * quarter + e;
+                    added_weight[block][e] = s < n ? power(log2_decay, REVERSE ? s : n - 1 - s) * a.added_scale : 0.0f;
+                }
+        }
+        const int last_reset = resets ? 63 - __builtin_clzll(resets) : -1, first_reset = resets ? __builtin_ctzll(resets) : CHUNK;
+        if constexpr (!STATE) {
+            // scores, by tiles on and below (REVERSE: above) the diagonal: rows are the steps that are added, columns those that read
+            for (int tile = wave; tile < 10; tile += WAVES) {
+                int ot = tile < 1 ? 0 : tile < 3 ? 1 : tile < 6 ? 2 : 3, st = tile - ot * (ot + 1) / 2;
+                if (REVERSE) { ot = 3 - ot; st = 3 - st; }
+                rlt_f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f}, y = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int block = 0; block < KEY_BLOCKS; block++) x = multiply(row_operand(L::KR, L::ROW, 16 * st + l, block), row_operand(L::Q, L::ROW, 16 * ot + l, block), x);
+                if constexpr (SLOPE) {
+#pragma unroll
+                    for (int block = 0; block < KEY_BLOCKS; block++) y = multiply(row_operand(L::VR, L::ROW, 16 * st + l, block), row_operand(L::WR, L::ROW, 16 * ot + l, block), y);
+                }
+                const int i = 16 * ot + l;      // the step that reads
+                const uint64_t before = resets & ((2ull << i) - 1), after = i < 63 ? resets & ~((2ull << i) - 1) : 0;
+                const int low = REVERSE ? i : before ? 63 - __builtin_clzll(before) : 0, high = REVERSE ? (after ? __builtin_ctzll(after) - 1 : 63) : i;      // steps that it sees
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int s = 16 * st + 4 * quarter + r, lag = REVERSE ? s - i : i - s;
+                    x[r] = s >= low && s <= high ? x[r] * (power(log2_decay, lag) * a.score_scale) : 0.0f;
+                    if constexpr (SLOPE) total += x[r] == 0.0f ? 0.0f : (float)lag * x[r] * y[r];
+                }
+#pragma unroll
+                for (int plane = 0; plane < L::PLANES; plane++) {
+                    const Quad part = __builtin_convertvector(x, Quad);
+                    *reinterpret_cast<Quad*>(lds + L::P + plane * CHUNK * L::COLUMN + i * L::COLUMN + 16 * st + 4 * quarter) = part;
+                    if (plane + 1 < L::PLANES) x -= __builtin_convertvector(part, rlt_f32x4);
+                }
+            }
+            // what the state before the chunk gives: columns of the result are the steps, rows the value columns
+            rlt_f32x4 out[4], out_slope[SLOPE ? 4 : 1];
+#pragma unroll
+            for (int ot = 0; ot < 4; ot++) {
+                out[ot] = rlt_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                if constexpr (SLOPE) out_slope[ot] = rlt_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            }
+#pragma unroll
+            for (int block = 0; block < KEY_BLOCKS; block++) {
+                const Cut<T, STATE_CUTS> s(state_vector(state, block));
+#pragma unroll
+                for (int ot = 0; ot < 4; ot++) {
+                    const Vector q = tiled_operand(L::Q, 16 * ot + l, block);
+#pragma unroll
+                    for (int p = 0; p < STATE_CUTS; p++) out[ot] = multiply(s.part[p], q, out[ot]);
+                }
+                if constexpr (SLOPE) {
+                    const Cut<T, STATE_CUTS> d(state_vector(slope, block));
+#pragma unroll
+                    for (int ot = 0; ot < 4; ot++) {
+                        const Vector q = tiled_operand(L::Q, 16 * ot + l, block);
+#pragma unroll
+                        for (int p = 0; p < STATE_CUTS; p++) out_slope[ot] = multiply(d.part[p], q, out_slope[ot]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int ot = 0; ot < 4; ot++) {
+                const int i = 16 * ot + l;
+                const bool sees = i < n && (REVERSE ? last_reset <= i : first_reset > i);
+                const float w = sees ? power(log2_decay, REVERSE ? n - 1 - i : i + 1) * a.read_scale : 0.0f;
+                if constexpr (SLOPE) {
+                    const Quad with = *reinterpret_cast<const Quad*>(lds + L::WR + i * L::ROW + 16 * wave + 4 * quarter);
+                    float d = 0.0f;
+#pragma unroll
+                    for (int r = 0; r < 4; r++) d = fmaf((float)with[r], fmaf((float)(i + 1), out[ot][r], out_slope[ot][r]), d);
+                    if (sees) total = fmaf(w, d, total);
+                }
+#pragma unroll
+                for (int r = 0; r < 4; r++) out[ot][r] = sees ? out[ot][r] * w : 0.0f;
+            }
+            rlt_lds_barrier();
+            // what the chunk's own steps give
+            Vector values[2];
+#pragma unroll
+            for (int block = 0; block < 2; block++) values[block] = column_operand(L::VT, L::VR, column, block);
+#pragma unroll
+            for (int ot = 0; ot < 4; ot++)
+#pragma unroll
+                for (int block = 0; block < 2; block++)
+                    if (REVERSE ? 32 * block + 31 >= 16 * ot : 32 * block <= 16 * ot + 15) {
+#pragma unroll
+                        for (int plane = 0; plane < L::PLANES; plane++) out[ot] = multiply(values[block], row_operand(L::P + plane * CHUNK * L::COLUMN, L::COLUMN, 16 * ot + l, block), out[ot]);
+                    }
+#pragma unroll
+            for (int ot = 0; ot < 4; ot++) {
+                const int i = 16 * ot + l, c0 = 16 * wave + 4 * quarter;
+                if (t0 + i < end) {
+                    O* to = at<O>(a.out, t0 + i, b, h) + c0;
+                    typedef typename Operand<O>::Quad OutQuad;
+                    rlt_f32x4 x = out[ot];
+                    if (i >= n) x = rlt_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                    if (a.out.vectors) { if (c0 < a.value) *reinterpret_cast<OutQuad*>(to) = __builtin_convertvector(x, OutQuad); }
+                    else {
+#pragma unroll
+                        for (int r = 0; r < 4; r++) if (c0 + r < a.value) to[r] = (O)x[r];
+                    }
+                }
+            }
+        }
+        // the state after the chunk
+        if (n > 0) {
+            const float f = resets ? 0.0f : power(log2_decay, REVERSE ? n - 1 : n);
+            counted += n; forgotten |= resets != 0;
+#pragma unroll
+            for (int k = 0; k < KEY_TILES; k++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    if constexpr (SLOPE) slope[k][r] = resets ? 0.0f : f * fmaf((float)n, state[k][r], slope[k][r]);
+                    state[k][r] = resets ? 0.0f : f * state[k][r];
+                }
+#pragma unroll
+            for (int block = 0; block < 2; block++) {
+                const Vector v = column_operand(L::VT, L::VR, column, block);
+                rlt_f32x8 weighted, lagged;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const int s = 32 * block + 8 * quarter + e;
+                    const bool stays = REVERSE ? s < first_reset : s >= last_reset;
+                    weighted[e] = stays ? (float)v[e] * added_weight[block][e] : 0.0f;
+                    if constexpr (SLOPE) lagged[e] = weighted[e] * (float)(n - 1 - s);
+                }
+                const Cut<T, ADDED_CUTS> x(weighted);
+#pragma unroll
+                for (int k = 0; k < KEY_TILES; k++) {
+                    const Vector key = column_operand(L::KT, L::KR, 16 * k + l, block);
+#pragma unroll
+                    for (int p = 0; p < ADDED_CUTS; p++) state[k] = multiply(key, x.part[p], state[k]);
+                }
+                if constexpr (SLOPE) {
+                    const Cut<T, ADDED_CUTS> y(lagged);
+#pragma unroll
+                    for (int k = 0; k < KEY_TILES; k++) {
+                        const Vector key = column_operand(L::KT, L::KR, 16 * k + l, block);
+#pragma unroll
+                        for (int p = 0; p < ADDED_CUTS; p++) slope[k] = multiply(key, y.part[p], slope[k]);
+                    }
+                }
+            }
+            if constexpr (REVERSE) {      // the power that all of them share: the cut operands keep their parts above the smallest numbers also where one step forgets nearly everything
+                const float once = power(log2_decay, 1);
+#pragma unroll
+                for (int k = 0; k < KEY_TILES; k++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) state[k][r] *= once;
+            }
+        }
+    }
+
+    if (a.exit)
+#pragma unroll
+        for (int k = 0; k < KEY_TILES; k++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int row = 16 * k + 4 * quarter + r;
+                if (row < a.key && column < a.value) {
+                    const size_t i = state_base + (size_t)row * a.state_key + (size_t)column * a.state_value;
+                    a.exit[i] = state[k][r];
+                    if constexpr (SLOPE && STATE) a.exit_slope[i] = slope[k][r];
+                }
+            }
+    if constexpr (STATE) { if (threadIdx.x == 0) a.factors[blockIdx.x] = make_float2(forgotten ? 0.0f : power(log2_decay, counted), (float)counted); }
+    if constexpr (SLOPE && !STATE) {
+        if (a.d_final && segment == a.segments - 1)
+#pragma unroll
+            for (int k = 0; k < KEY_TILES; k++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int row = 16 * k + 4 * quarter + r;
+                    if (row < a.key && column < a.value) total = fmaf(a.d_final[(size_t)pair * a.key * a.value + (size_t)row * a.state_key + (size_t)column * a.state_value], slope[k][r], total);
+                }
+        total = rlt_wave_sum(total);
+        float* sums = (float*)lds_bytes;
+        rlt_lds_barrier();
+        if (lane == 0) sums[wave] = total;
+        rlt_lds_barrier();
+        if (threadIdx.x == 0) {
+            float s = 0.0f;
+            for (int w = 0; w < WAVES; w++) s += sums[w];
+            a.partial[blockIdx.x] = s;
+        }
+    }
 }
 
-// Derivative by the decay's logarithm, of one row and head: the state's own derivative goes along with it.
-template <typename T> __global__ __launch_bounds__(MAX_WIDTH) void slope_kernel(Walk a, Part d_out, const float* d_final, float* partial) {
-    __shared__ float q[MAX_WIDTH], k[MAX_WIDTH], sum[2];
-    const int h = blockIdx.x % a.heads, b = blockIdx.x / a.heads, c = threadIdx.x;
-    const float decay = expf(a.log_decay[h]);
-    const size_t base = ((size_t)b * a.heads + h) * a.key * a.value;
-    float state[MAX_WIDTH], slope[MAX_WIDTH];
-#pragma unroll
-    for (int i = 0; i < MAX_WIDTH; i++) { state[i] = a.initial && c < a.value && i < a.key ? a.initial[base + i * a.value + c] : 0.0f; slope[i] = 0.0f; }
-    const int length = a.lengths ? min(max(a.lengths[b], 0), a.steps) : a.steps;
-    float total = 0.0f;
-    for (int t = 0; t < length; t++) {
-        __syncthreads();
-        q[c] = c < a.key ? (float)at<T>(a.q, t, b, h)[c] : 0.0f;
-        k[c] = c < a.key ? (float)at<T>(a.k, t, b, h)[c] : 0.0f;
-        const float v = c < a.value ? (float)at<T>(a.v, t, b, h)[c] : 0.0f, d = c < a.value ? (float)at<T>(d_out, t, b, h)[c] * a.scale_out : 0.0f;
-        __syncthreads();
-        const bool forget = a.reset && a.reset[(size_t)t * a.batch + b];
-        float out = 0.0f;
-#pragma unroll
-        for (int i = 0; i < MAX_WIDTH; i++) {
-            slope[i] = forget ? 0.0f : decay * (slope[i] + state[i]);
-            state[i] = fmaf(k[i], v, forget ? 0.0f : state[i] * decay);
-            out = fmaf(q[i], slope[i], out);
+// States that the segments start from, out of what each of them adds: element by element along the segments (REVERSE: from the last). locals become the entries.
+__global__ __launch_bounds__(256) void scan_kernel(const float* __restrict__ initial, float* __restrict__ locals, float* __restrict__ slopes, const float2* __restrict__ factors, float* __restrict__ final, int elements,
+                                                   int segments, int reverse) {
+    const int pair = blockIdx.y, e = blockIdx.x * 256 + threadIdx.x;
+    if (e >= elements) return;
+    float carry = initial ? initial[(size_t)pair * elements + e] : 0.0f, carry_slope = 0.0f;
+    for (int i = 0; i < segments; i++) {
+        const size_t p = (size_t)pair * segments + (reverse ? segments - 1 - i : i), at = p * elements + e;
+        const float2 f = factors[p];
+        const float local = locals[at];
+        if (slopes) {
+            const float local_slope = slopes[at];
+            slopes[at] = carry_slope;
+            carry_slope = f.x == 0.0f ? local_slope : fmaf(f.x, fmaf(f.y, carry, carry_slope), local_slope);
         }
-        total = fmaf(out, d, total);
+        locals[at] = carry;
+        carry = f.x == 0.0f ? local : fmaf(f.x, carry, local);
     }
-    if (d_final)
-#pragma unroll
-        for (int i = 0; i < MAX_WIDTH; i++)
-            if (c < a.value && i < a.key) total = fmaf(d_final[base + i * a.value + c], slope[i], total);
-    total = rlt_wave_sum(total);
-    if ((c & 63) == 0) sum[c >> 6] = total;
-    __syncthreads();
-    if (c == 0) partial[(size_t)b * a.heads + h] = sum[0] + sum[1];
+    if (final) final[(size_t)pair * elements + e] = carry;
 }
 
-// sums over the rows of a batch, in their order
-__global__ __launch_bounds__(64) void decay_sum_kernel(const float* __restrict__ partial, int batch, int heads, float* __restrict__ out, int accumulate) {
+// sums over the rows of a batch and their segments, in a fixed order
+__global__ __launch_bounds__(64) void decay_sum_kernel(const float* __restrict__ partial, int batch, int heads, int segments, float* __restrict__ out, int accumulate) {
     const int h = blockIdx.x;
     float s = 0.0f;
-    for (int b = threadIdx.x; b < batch; b += 64) s += partial[(size_t)b * heads + h];
+    for (int i = threadIdx.x; i < batch * segments; i += 64) s += partial[((size_t)(i / segments) * heads + h) * segments + i % segments];
     s = rlt_wave_sum(s);
     if (threadIdx.x == 0) out[h] = accumulate ? out[h] + s : s;
 }
@@ -133,61 +438,142 @@ template <typename T> __global__ __launch_bounds__(128) void step_kernel(Walk a)
     if (c >= a.value) return;
     float out = 0.0f;
     for (int i = 0; i < a.key; i++) {
-        const float s = fmaf(k[i], v, forget ? 0.0f : a.initial[base + i * a.value + c] * decay);
-        a.final[base + i * a.value + c] = s;
+        const float s = fmaf(k[i], v, forget ? 0.0f : a.entry[base + i * a.value + c] * decay);
+        a.exit[base + i * a.value + c] = s;
         out = fmaf(q[i], s, out);
     }
-    at<T>(a.out, 0, b, h)[c] = (T)(out * a.scale_out);
+    at<T>(a.out, 0, b, h)[c] = (T)(out * a.read_scale);
 }
 
-Part part(const rlt_head_view* v, int group) { return Part{v->data, v->step_stride, v->row_stride, v->head_stride, group}; }
+template <typename T> Part part(const rlt_head_view* v, int group, int width) {
+    const bool vectors = reinterpret_cast<uintptr_t>(v->data) % (4 * sizeof(T)) == 0 && v->step_stride % 4 == 0 && v->row_stride % 4 == 0 && v->head_stride % 4 == 0 && width % 4 == 0;
+    return Part{v->data, v->step_stride, v->row_stride, v->head_stride, group, vectors};
+}
 bool described(const rlt_linear_attention* p) {
     return p && (p->type == RLT_TYPE_F32 || p->type == RLT_TYPE_BF16) && p->batch > 0 && p->heads > 0 && p->kv_heads > 0 && p->heads % p->kv_heads == 0 && p->key_dim > 0 && p->value_dim > 0;
 }
-bool supported(const rlt_linear_attention* p) { return p->key_dim <= MAX_WIDTH && p->value_dim <= MAX_WIDTH && (int64_t)p->batch * p->heads <= INT32_MAX; }
+bool supported(const rlt_linear_attention* p) { return p->key_dim <= MAX_WIDTH && p->value_dim <= MAX_WIDTH && (int64_t)p->batch * p->heads <= INT32_MAX / 64; }
 bool given(const rlt_head_view* v) { return v && v->data; }
+size_t padded(size_t n) { return (n + 63) / 64 * 64; }
 
+// The steps of a row and head are cut into segments where rows and heads alone leave compute units without work: their states then cost a pass over keys and values ahead of the walk.
+struct Segments { int count, steps; };
+Segments segments_of(const rlt_linear_attention* p, int steps) {
+    const int chunks = (steps + CHUNK - 1) / CHUNK;
+    const int64_t pairs = (int64_t)p->batch * p->heads;
+    int64_t count = pairs >= 256 ? 1 : (256 + pairs - 1) / pairs;
+    if (count > (chunks + 3) / 4) count = (chunks + 3) / 4;      // at least four chunks each
+    const int per = (int)((chunks + count - 1) / count);
+    return {(chunks + per - 1) / per, per * CHUNK};
+}
+// scratch memory, in floats: [states of the segments][their slopes][factors][partial sums][gradients of the heads that share keys and values]
+struct Scratch { size_t states, slopes, factors, partial, shared, total; };
+Scratch scratch_of(const rlt_linear_attention* p, int steps, bool backward) {
+    const Segments g = segments_of(p, steps);
+    const size_t pairs = (size_t)p->batch * p->heads, state = padded(pairs * g.count * p->key_dim * p->value_dim);
+    Scratch s{};
+    size_t at = 0;
+    auto take = [&](size_t n) { const size_t here = at; at += padded(n); return here; };
+    if (g.count > 1) {
+        s.states = take(state);
+        if (backward) s.slopes = take(state);
+        s.factors = take(2 * pairs * g.count);
+    }
+    if (backward) {
+        s.partial = take(pairs * g.count);
+        if (p->heads != p->kv_heads) s.shared = take((size_t)steps * pairs * (p->key_dim > p->value_dim ? p->key_dim : p->value_dim));
+    }
+    s.total = at;
+    return s;
+}
+
+template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE> int launch_walk(rlt_rocm_device* device, const Walk& a) {
+    constexpr size_t bytes = Layout<T, D, SLOPE, STATE>::BYTES;
+    const auto kernel = walk_kernel<T, O, D, REVERSE, SLOPE, STATE>;
+    RLT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    hipLaunchKernelGGL(kernel, dim3((unsigned)a.batch * a.heads * a.segments), dim3(4 * D), bytes, device->stream, a);
+    return rlt_launch_status(device);
+}
+template <typename T, typename O, bool REVERSE, bool SLOPE, bool STATE> int walk(rlt_rocm_device* device, const Walk& a) {
+    const int width = a.key > a.value ? a.key : a.value;
+    return width <= 32 ? launch_walk<T, O, 32, REVERSE, SLOPE, STATE>(device, a) : width <= 64 ? launch_walk<T, O, 64, REVERSE, SLOPE, STATE>(device, a) : launch_walk<T, O, 128, REVERSE, SLOPE, STATE>(device, a);
+}
 Walk walk_of(const rlt_linear_attention* p, const uint8_t* reset, const int32_t* lengths, int steps) {
+    const Segments g = segments_of(p, steps);
     Walk a{};
-    a.log_decay = p->log_decay; a.reset = reset; a.lengths = lengths; a.scale_out = a.scale_added = 1.0f;
-    a.batch = p->batch; a.heads = p->heads; a.steps = steps; a.key = p->key_dim; a.value = p->value_dim;
+    a.log_decay = p->log_decay; a.reset = reset; a.lengths = lengths; a.score_scale = a.read_scale = p->scale; a.added_scale = 1.0f;
+    a.batch = p->batch; a.heads = p->heads; a.steps = steps; a.key = p->key_dim; a.value = p->value_dim; a.segments = g.count; a.segment_steps = g.steps;
+    a.state_key = p->value_dim; a.state_value = 1;
     return a;
 }
-template <typename T, typename O, bool REVERSE, bool TRANSPOSED> void walk(rlt_rocm_device* device, const Walk& a) {
-    hipLaunchKernelGGL((walk_kernel<T, O, REVERSE, TRANSPOSED>), dim3((unsigned)a.heads * a.batch), dim3(MAX_WIDTH), 0, device->stream, a);
+// states that the segments of `a` start from, in scratch memory
+template <typename T, bool REVERSE, bool SLOPE> int segment_states(rlt_rocm_device* device, const Walk& a, const float* initial, float* final, float* states, float* slopes, float2* factors) {
+    Walk s = a;
+    s.entry = nullptr; s.exit = states; s.exit_slope = slopes; s.factors = factors;
+    int rc = walk<T, T, REVERSE, SLOPE, true>(device, s);
+    if (rc) return rc;
+    const int elements = a.key * a.value, pairs = a.batch * a.heads;
+    hipLaunchKernelGGL(scan_kernel, dim3((elements + 255) / 256, pairs), dim3(256), 0, device->stream, initial, states, SLOPE ? slopes : nullptr, factors, final, elements, a.segments, (int)REVERSE);
+    return rlt_launch_status(device);
+}
+
+template <typename T> int forward(rlt_rocm_device* device, const rlt_linear_attention* p, const rlt_head_view* q, const rlt_head_view* k, const rlt_head_view* v, const rlt_head_view* output,
+                                  const float* initial_state, float* final_state, const uint8_t* reset, const int32_t* lengths, int steps, float* workspace) {
+    const int group = p->heads / p->kv_heads;
+    const Scratch s = scratch_of(p, steps, false);
+    Walk a = walk_of(p, reset, lengths, steps);
+    a.q = part<T>(q, 1, p->key_dim); a.k = part<T>(k, group, p->key_dim); a.v = part<T>(v, group, p->value_dim); a.out = part<T>(output, 1, p->value_dim);
+    a.entry = initial_state; a.exit = final_state;
+    if (a.segments > 1) {
+        const int rc = segment_states<T, false, false>(device, a, initial_state, final_state, workspace + s.states, nullptr, (float2*)(workspace + s.factors));
+        if (rc) return rc;
+        a.entry = workspace + s.states; a.exit = nullptr;
+    }
+    return walk<T, T, false, false, false>(device, a);
 }
 
 template <typename T> int backward(rlt_rocm_device* device, const rlt_linear_attention* p, const rlt_head_view* q, const rlt_head_view* k, const rlt_head_view* v, const rlt_head_view* d_output,
                                    const rlt_head_view* d_q, const rlt_head_view* d_k, const rlt_head_view* d_v, const float* initial_state, const float* d_final_state, float* d_initial_state,
-                                   float* d_log_decay, int accumulate, const uint8_t* reset, const int32_t* lengths, int steps, void* workspace) {
+                                   float* d_log_decay, int accumulate, const uint8_t* reset, const int32_t* lengths, int steps, float* workspace) {
     const int group = p->heads / p->kv_heads;
-    const Part Q = part(q, 1), K = part(k, group), V = part(v, group), D = part(d_output, 1);
-    float* partial = (float*)workspace;
-    float* shared = partial + (((size_t)p->batch * p->heads + 63) / 64) * 64;
-    Walk a = walk_of(p, reset, lengths, steps);      // d_q = scale * d_output S^T: the state, read across
-    a.q = D; a.k = V; a.v = K; a.out = part(d_q, 1); a.key = p->value_dim; a.value = p->key_dim; a.scale_out = p->scale; a.initial = initial_state;
-    walk<T, T, false, true>(device, a);
-    auto reverse = [&](const Part& reader, const Part& x, const Part& y, const rlt_head_view* to, bool transposed) {
-        Walk r = walk_of(p, reset, lengths, steps);
-        const int width = transposed ? p->key_dim : p->value_dim;
-        r.q = reader; r.k = x; r.v = y; r.scale_added = p->scale; r.initial = d_final_state; r.key = transposed ? p->value_dim : p->key_dim; r.value = width;
-        if (!transposed) r.final = d_initial_state;
-        r.out = group == 1 ? part(to, 1) : Part{shared, (int64_t)p->batch * p->heads * width, (int64_t)p->heads * width, width, 1};
-        if (group == 1) { if (transposed) walk<T, T, true, true>(device, r); else walk<T, T, true, false>(device, r); }
-        else {
-            if (transposed) walk<T, float, true, true>(device, r); else walk<T, float, true, false>(device, r);
-            hipLaunchKernelGGL((head_sum_kernel<T>), dim3(2048), dim3(128), 0, device->stream, shared, part(to, 1), steps, p->batch, p->kv_heads, group, width);
-        }
-    };
-    reverse(K, Q, D, d_v, false);
-    reverse(V, D, Q, d_k, true);
-    if (d_log_decay) {
-        Walk s = walk_of(p, reset, lengths, steps);
-        s.q = Q; s.k = K; s.v = V; s.initial = initial_state; s.scale_out = p->scale;
-        hipLaunchKernelGGL((slope_kernel<T>), dim3((unsigned)p->heads * p->batch), dim3(MAX_WIDTH), 0, device->stream, s, D, d_final_state, partial);
-        hipLaunchKernelGGL(decay_sum_kernel, dim3(p->heads), dim3(64), 0, device->stream, partial, p->batch, p->heads, d_log_decay, accumulate);
+    const Scratch s = scratch_of(p, steps, true);
+    const Part Q = part<T>(q, 1, p->key_dim), K = part<T>(k, group, p->key_dim), V = part<T>(v, group, p->value_dim), G = part<T>(d_output, 1, p->value_dim);
+    float* const states = workspace + s.states; float* const slopes = workspace + s.slopes; float2* const factors = (float2*)(workspace + s.factors);
+    int rc;
+    // d_q reads the state across: values are its keys
+    Walk a = walk_of(p, reset, lengths, steps);
+    const bool cut = a.segments > 1;
+    if (cut) {
+        a.k = K; a.v = V;
+        rc = d_log_decay ? segment_states<T, false, true>(device, a, initial_state, nullptr, states, slopes, factors) : segment_states<T, false, false>(device, a, initial_state, nullptr, states, nullptr, factors);
+        if (rc) return rc;
     }
-    return rlt_launch_status(device);
+    a.q = G; a.k = V; a.v = K; a.with = Q; a.out = part<T>(d_q, 1, p->key_dim); a.key = p->value_dim; a.value = p->key_dim; a.state_key = 1; a.state_value = p->value_dim;
+    a.entry = cut ? states : initial_state; a.entry_slope = cut ? slopes : nullptr; a.d_final = d_final_state; a.partial = workspace + s.partial;
+    rc = d_log_decay ? walk<T, T, false, true, false>(device, a) : walk<T, T, false, false, false>(device, a);
+    if (rc) return rc;
+    if (d_log_decay) hipLaunchKernelGGL(decay_sum_kernel, dim3(p->heads), dim3(64), 0, device->stream, a.partial, p->batch, p->heads, a.segments, d_log_decay, accumulate);
+    // the state's gradient, from the last step to the first; d_v reads it, d_k reads it across
+    Walk r = walk_of(p, reset, lengths, steps);
+    r.k = Q; r.v = G; r.read_scale = 1.0f; r.added_scale = p->scale;
+    if (cut && (rc = segment_states<T, true, false>(device, r, d_final_state, d_initial_state, states, nullptr, factors))) return rc;
+    r.entry = cut ? states : d_final_state;
+    auto gradient = [&](Walk w, const rlt_head_view* to, int width) {
+        if (group == 1) { w.out = part<T>(to, 1, width); return walk<T, T, true, false, false>(device, w); }
+        float* shared = workspace + s.shared;
+        w.out = Part{shared, (int64_t)p->batch * p->heads * width, (int64_t)p->heads * width, width, 1, width % 4 == 0};
+        const int code = walk<T, float, true, false, false>(device, w);
+        if (code) return code;
+        hipLaunchKernelGGL((head_sum_kernel<T>), dim3(2048), dim3(128), 0, device->stream, shared, part<T>(to, 1, width), steps, p->batch, p->kv_heads, group, width);
+        return rlt_launch_status(device);
+    };
+    Walk w = r;
+    w.q = K;
+    if (!cut) w.exit = d_initial_state;
+    if ((rc = gradient(w, d_v, p->value_dim))) return rc;
+    w = r;
+    w.q = V; w.k = G; w.v = Q; w.key = p->value_dim; w.value = p->key_dim; w.state_key = 1; w.state_value = p->value_dim;
+    return gradient(w, d_k, p->key_dim);
 }
 
 }  // namespace
@@ -195,10 +581,8 @@ template <typename T> int backward(rlt_rocm_device* device, const rlt_linear_att
 extern "C" {
 
 size_t rlt_rocm_linear_attention_workspace_bytes(const rlt_linear_attention* layer, int steps, int backward) {
-    if (!described(layer) || steps <= 0 || !backward) return 0;
-    const size_t partial = (((size_t)layer->batch * layer->heads + 63) / 64) * 64;
-    const size_t shared = layer->heads == layer->kv_heads ? 0 : (size_t)steps * layer->batch * layer->heads * (layer->key_dim > layer->value_dim ? layer->key_dim : layer->value_dim);
-    return (partial + shared) * sizeof(float);
+    if (!described(layer) || steps <= 0) return 0;
+    return scratch_of(layer, steps, backward != 0).total * sizeof(float);
 }
 
 int rlt_rocm_linear_attention_forward(rlt_rocm_device* device, const rlt_linear_attention* layer, const rlt_head_view* q, const rlt_head_view* k, const rlt_head_view* v,
@@ -207,13 +591,10 @@ int rlt_rocm_linear_attention_forward(rlt_rocm_device* device, const rlt_linear_
     if (!device) return RLT_E_NOT_INITIALISED;
     RLT_REQUIRE(described(layer) && layer->log_decay && steps > 0 && given(q) && given(k) && given(v) && given(output));
     const size_t need = rlt_rocm_linear_attention_workspace_bytes(layer, steps, 0);
-    RLT_REQUIRE(need == 0 || (workspace && workspace_bytes >= need));
+    RLT_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0));
     if (!supported(layer)) return RLT_E_UNSUPPORTED;
-    const int group = layer->heads / layer->kv_heads;
-    Walk a = walk_of(layer, reset, lengths, steps);
-    a.q = part(q, 1); a.k = part(k, group); a.v = part(v, group); a.out = part(output, 1); a.scale_out = layer->scale; a.initial = initial_state; a.final = final_state;
-    if (layer->type == RLT_TYPE_F32) walk<float, float, false, false>(device, a); else walk<rlt_bf16, rlt_bf16, false, false>(device, a);
-    return rlt_launch_status(device);
+    return layer->type == RLT_TYPE_F32 ? forward<float>(device, layer, q, k, v, output, initial_state, final_state, reset, lengths, steps, (float*)workspace)
+                                       : forward<rlt_bf16>(device, layer, q, k, v, output, initial_state, final_state, reset, lengths, steps, (float*)workspace);
 }
 
 int rlt_rocm_linear_attention_backward(rlt_rocm_device* device, const rlt_linear_attention* layer, const rlt_head_view* q, const rlt_head_view* k, const rlt_head_view* v,
@@ -223,10 +604,10 @@ int rlt_rocm_linear_attention_backward(rlt_rocm_device* device, const rlt_linear
     if (!device) return RLT_E_NOT_INITIALISED;
     RLT_REQUIRE(described(layer) && layer->log_decay && steps > 0 && given(q) && given(k) && given(v) && given(d_output) && given(d_q) && given(d_k) && given(d_v));
     const size_t need = rlt_rocm_linear_attention_workspace_bytes(layer, steps, 1);
-    RLT_REQUIRE(need == 0 || (workspace && workspace_bytes >= need));
+    RLT_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0));
     if (!supported(layer)) return RLT_E_UNSUPPORTED;
-    return layer->type == RLT_TYPE_F32 ? backward<float>(device, layer, q, k, v, d_output, d_q, d_k, d_v, initial_state, d_final_state, d_initial_state, d_log_decay, accumulate, reset, lengths, steps, workspace)
-                                       : backward<rlt_bf16>(device, layer, q, k, v, d_output, d_q, d_k, d_v, initial_state, d_final_state, d_initial_state, d_log_decay, accumulate, reset, lengths, steps, workspace);
+    return layer->type == RLT_TYPE_F32 ? backward<float>(device, layer, q, k, v, d_output, d_q, d_k, d_v, initial_state, d_final_state, d_initial_state, d_log_decay, accumulate, reset, lengths, steps, (float*)workspace)
+                                       : backward<rlt_bf16>(device, layer, q, k, v, d_output, d_q, d_k, d_v, initial_state, d_final_state, d_initial_state, d_log_decay, accumulate, reset, lengths, steps, (float*)workspace);
 }
 
 int rlt_rocm_linear_attention_step(rlt_rocm_device* device, const rlt_linear_attention* layer, const rlt_head_view* q, const rlt_head_view* k, const rlt_head_view* v,
@@ -236,9 +617,13 @@ int rlt_rocm_linear_attention_step(rlt_rocm_device* device, const rlt_linear_att
     if (!supported(layer)) return RLT_E_UNSUPPORTED;
     const int group = layer->heads / layer->kv_heads;
     Walk a = walk_of(layer, reset, nullptr, 1);
-    a.q = part(q, 1); a.k = part(k, group); a.v = part(v, group); a.out = part(output, 1); a.scale_out = layer->scale; a.initial = state; a.final = next_state;
-    if (layer->type == RLT_TYPE_F32) hipLaunchKernelGGL((step_kernel<float>), dim3((unsigned)a.heads * a.batch), dim3(MAX_WIDTH), 0, device->stream, a);
-    else hipLaunchKernelGGL((step_kernel<rlt_bf16>), dim3((unsigned)a.heads * a.batch), dim3(MAX_WIDTH), 0, device->stream, a);
+    a.entry = state; a.exit = next_state;
+    auto views = [&](auto type) {
+        typedef decltype(type) T;
+        a.q = part<T>(q, 1, layer->key_dim); a.k = part<T>(k, group, layer->key_dim); a.v = part<T>(v, group, layer->value_dim); a.out = part<T>(output, 1, layer->value_dim);
+        hipLaunchKernelGGL((step_kernel<T>), dim3((unsigned)a.heads * a.batch), dim3(MAX_WIDTH), 0, device->stream, a);
+    };
+    if (layer->type == RLT_TYPE_F32) views(0.0f); else views((rlt_bf16)0.0f);
     return rlt_launch_status(device);
 }
 
