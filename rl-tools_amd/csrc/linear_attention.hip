@@ -62,320 +62,401 @@ template <typename T, int PARTS> constexpr int CUTS = sizeof(T) == 4 ? 1 : PARTS
 // decay^n; n = 0 gives 1 also for a decay of zero
 __device__ __forceinline__ float power(float log2_decay, int n) { return n == 0 ? 1.0f : __builtin_amdgcn_exp2f(log2_decay * (float)n); }
 
+// Shape of a workgroup for heads of up to D channels: a wavefront owns TILES x 16 of the value columns.
 template <typename T, int D, bool SLOPE, bool STATE> struct Layout {
-    static constexpr bool NARROW = sizeof(T) == 2;
-    static constexpr int PAD = 16 / sizeof(T), ROW = D + PAD, COLUMN = CHUNK + PAD;      // rows start 4 (of 64) banks after each other: sixteen of them side by side in 16 bytes each meet no bank twice
-    static constexpr int PLANES = NARROW ? 2 : 1;
-    static constexpr int Q = 0, KR = Q + (STATE ? 0 : CHUNK * ROW), KT = KR + (STATE && NARROW ? 0 : CHUNK * ROW), VT = KT + (NARROW ? D * COLUMN : 0);      // narrow: keys and values also by columns
-    static constexpr int VR = VT + (NARROW ? D * COLUMN : 0), WR = VR + (!NARROW || (SLOPE && !STATE) ? CHUNK * ROW : 0), P = WR + (SLOPE && !STATE ? CHUNK * ROW : 0);
-    static constexpr int TOTAL = P + (STATE ? 0 : PLANES * CHUNK * COLUMN);
-    static constexpr size_t BYTES = TOTAL * sizeof(T);
+    static constexpr int TILES = D == 128 && sizeof(T) == 2 && !SLOPE ? 2 : 1, WAVES = D / (16 * TILES), THREADS = 64 * WAVES;
+    static constexpr int PAD = 16 / sizeof(T), ROW = D + PAD, SCORES = CHUNK + PAD;      // rows start 4 (of 64) banks after each other: sixteen of them side by side in 16 bytes each meet no bank twice
+    static constexpr int PLANES = sizeof(T) == 2 ? 2 : 1;
+    static constexpr int K = 0, V = K + CHUNK * ROW, Q = V + CHUNK * ROW, W = Q + (STATE ? 0 : CHUNK * ROW), P = W + (SLOPE && !STATE ? CHUNK * ROW : 0);
+    static constexpr int FLAGS = P + (STATE ? 0 : PLANES * CHUNK * SCORES);
+    static constexpr size_t BYTES = FLAGS * sizeof(T) + WAVES * sizeof(float);
+    // wavefronts that the registers of a SIMD are shared by: as many as LDS has room for workgroups
+    static constexpr int FIT = (int)(163840 / BYTES) * WAVES / 4, MOST = D == 128 ? 2 : 3, RESIDENT = FIT < 1 ? 1 : FIT > MOST ? MOST : FIT;
 };
 
-// Chunks of 64 steps. With i, s the steps of a chunk (n of them within the row's length), S the state before it and a the decay:
+// Chunks of up to 64 steps. With i, s the steps of a chunk (n of them within the row's length), S the state before it and a the decay:
 //     out_i = sum over s <= i of a^(i-s) (q_i k_s) v_s + a^(i+1) q_i S,     S <- a^n S + sum over s of a^(n-1-s) k_s^T v_s
 // where a reset between the two steps of a power makes it zero. REVERSE is the transposed recurrence of the gradients, from the last step to the first:
-//     out_i = sum over s >= i of a^(s-i) (q_i k_s) v_s + a^(n-1-i) q_i R,   R <- a^n R + sum over s of a^(s+1) k_s^T v_s.
-// A wavefront owns 16 of the value columns: their state stays in its accumulators from chunk to chunk, laid out as the matrix instruction leaves them, which is (with the summands in an order of their own) how the
-// product with the queries takes them. Scores of a chunk are shared out in tiles of 16 x 16, weighted, and exchanged through LDS.
-template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE> __global__ __launch_bounds__(4 * D) void walk_kernel(Walk a) {
+//     out_i = sum over s >= i of a^(s-i) (q_i k_s) v_s + a^(n-1-i) q_i R,   R <- a (a^(n-1) R + sum over s of a^s k_s^T v_s).
+// A wavefront owns some of the value columns: their state stays in its accumulators from chunk to chunk, laid out as the matrix instruction leaves them, which is (with the summands in an order of their own) how the
+// product with the queries takes them. Scores of a chunk are shared out in tiles of 16 x 16, weighted, and exchanged through LDS. SLOPE carries the state's derivative by the decay's logarithm along.
+// STATE: only the state, of a segment that starts from nothing. A launch may hold two walks over the same rows (gradients of keys and of values), whose workgroups take turns on an XCD and so find each other's inputs in its L2.
+struct Walks { Walk first, second; int items, two; };
+template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE> __global__ __launch_bounds__((Layout<T, D, SLOPE, STATE>::THREADS), (Layout<T, D, SLOPE, STATE>::RESIDENT)) void walk_kernel(Walks walks) {
     typedef typename Operand<T>::Vector Vector;
     typedef typename Operand<T>::Quad Quad;
     typedef Layout<T, D, SLOPE, STATE> L;
-    constexpr int KEY_TILES = D / 16, KEY_BLOCKS = D / 32, WAVES = D / 16, STATE_CUTS = CUTS<T, SLOPE ? 3 : 2>, ADDED_CUTS = CUTS<T, 3>;
+    constexpr int KEY_TILES = D / 16, KEY_BLOCKS = D / 32, TILES = L::TILES, ROUNDS = CHUNK * D / (16 * L::THREADS), STATE_CUTS = CUTS<T, SLOPE ? 3 : 2>, ADDED_CUTS = CUTS<T, 3>;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds_bytes[];
     T* const lds = (T*)lds_bytes;
-    const int pair = blockIdx.x / a.segments, segment = blockIdx.x % a.segments, b = pair / a.heads, h = pair % a.heads;
+    float* const flags = (float*)(lds_bytes + L::FLAGS * sizeof(T));
+    const bool other = walks.two && (blockIdx.x / 8) % 2;
+    const int item = walks.two ? blockIdx.x / 16 * 8 + blockIdx.x % 8 : blockIdx.x;
+    if (item >= walks.items) return;
+    const Walk& a = other ? walks.second : walks.first;
+    const int pair = item / a.segments, segment = item % a.segments, b = pair / a.heads, h = pair % a.heads;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, quarter = lane >> 4;
     const int length = a.lengths ? min(max(a.lengths[b], 0), a.steps) : a.steps;
     const float log2_decay = a.log_decay[h] * 1.44269504088896341f;
-    const int begin = segment * a.segment_steps, end = min(begin + a.segment_steps, a.steps), chunks = (end - begin + CHUNK - 1) / CHUNK;
+    const int begin = segment * a.segment_steps, end = min(begin + a.segment_steps, a.steps);
 
-    // state: tile k, element r of this lane is row 16 k + 4 quarter + r, column 16 wave + l
-    rlt_f32x4 state[KEY_TILES], slope[SLOPE ? KEY_TILES : 1];
-    const int column = 16 * wave + l;
-    const size_t state_base = ((size_t)pair * a.segments + segment) * a.key * a.value;
+    // state: tile k, element r of this lane is row 16 k + 4 quarter + r, column 16 (TILES wave + tile) + l
+    rlt_f32x4 state[TILES][KEY_TILES], slope[SLOPE ? TILES : 1][SLOPE ? KEY_TILES : 1];
+    const int column0 = 16 * TILES * wave;
+    const size_t state_base = (size_t)item * a.key * a.value;
+    auto over_state = [&](auto f) {
 #pragma unroll
-    for (int k = 0; k < KEY_TILES; k++)
+        for (int tile = 0; tile < TILES; tile++)
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const int row = 16 * k + 4 * quarter + r;
-            const bool there = row < a.key && column < a.value;
-            const size_t i = state_base + (size_t)row * a.state_key + (size_t)column * a.state_value;
-            state[k][r] = !STATE && a.entry && there ? a.entry[i] : 0.0f;
-            if constexpr (SLOPE) slope[k][r] = !STATE && a.entry_slope && there ? a.entry_slope[i] : 0.0f;
-        }
-
-    // what a thread carries from memory to LDS: four steps of four channels of each tensor
-    const int channel = (threadIdx.x % (D / 4)) * 4, first = (threadIdx.x / (D / 4)) * 4;
-    Quad next_q[4], next_k[4], next_v[4], next_with[4];
-    uint8_t next_reset = 0;
-    auto fetch = [&](const Part& p, int width, int t0, Quad (&to)[4]) {
-        const T* src = at<T>(p, t0 + first, b, h) + channel;
+            for (int k = 0; k < KEY_TILES; k++)
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-#pragma unroll
-            for (int c = 0; c < 4; c++) to[r][c] = (T)0.0f;
-            if (t0 + first + r < min(length, end)) {
-                if (p.vectors) { if (channel < width) to[r] = *reinterpret_cast<const Quad*>(src + (int64_t)r * p.step); }
-                else {
-#pragma unroll
-                    for (int c = 0; c < 4; c++) if (channel + c < width) to[r][c] = src[(int64_t)r * p.step + c];
+                for (int r = 0; r < 4; r++) {
+                    const int row = 16 * k + 4 * quarter + r, column = column0 + 16 * tile + l;
+                    f(tile, k, r, row < a.key && column < a.value, (size_t)row * a.state_key + (size_t)column * a.state_value);
                 }
-            }
+    };
+    over_state([&](int tile, int k, int r, bool there, size_t i) {
+        state[tile][k][r] = !STATE && a.entry && there ? a.entry[state_base + i] : 0.0f;
+        if constexpr (SLOPE) slope[tile][k][r] = !STATE && a.entry_slope && there ? a.entry_slope[state_base + i] : 0.0f;
+    });
+
+    // what a thread carries from memory to LDS, in rounds: four steps of four channels of each tensor
+    const int channel = (threadIdx.x % (D / 4)) * 4, first = (threadIdx.x / (D / 4)) * 4;
+    constexpr int ROUND_STEPS = 16 * L::THREADS / D;
+    Quad next_q[STATE ? 1 : ROUNDS][4], next_k[ROUNDS][4], next_v[ROUNDS][4], next_with[SLOPE && !STATE ? ROUNDS : 1][4];
+    uint8_t next_reset = 0;
+    auto fetch = [&](const Part& p, int width, int t0, int stop, Quad (&to)[ROUNDS][4]) {
+        const T* src = at<T>(p, t0, b, h) + (int64_t)first * p.step + channel;
+        if (p.vectors && stop - t0 == CHUNK) {
+#pragma unroll
+            for (int round = 0; round < ROUNDS; round++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    to[round][r] = Quad{};
+                    if (channel < width) to[round][r] = *reinterpret_cast<const Quad*>(src + (int64_t)(round * ROUND_STEPS + r) * p.step);
+                }
+        } else {
+#pragma unroll
+            for (int round = 0; round < ROUNDS; round++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    to[round][r] = Quad{};
+                    if (t0 + first + round * ROUND_STEPS + r < stop) {
+                        const T* from = src + (int64_t)(round * ROUND_STEPS + r) * p.step;
+                        if (p.vectors) { if (channel < width) to[round][r] = *reinterpret_cast<const Quad*>(from); }
+                        else {
+#pragma unroll
+                            for (int c = 0; c < 4; c++) if (channel + c < width) to[round][r][c] = from[c];
+                        }
+                    }
+                }
         }
     };
-    auto fetch_chunk = [&](int chunk) {
-        const int t0 = begin + chunk * CHUNK;
-        if constexpr (!STATE) fetch(a.q, a.key, t0, next_q);
-        fetch(a.k, a.key, t0, next_k);
-        fetch(a.v, a.value, t0, next_v);
-        if constexpr (SLOPE && !STATE) fetch(a.with, a.value, t0, next_with);
-        next_reset = a.reset && t0 + lane < min(length, end) ? a.reset[(size_t)(t0 + lane) * a.batch + b] : (uint8_t)0;
+    auto fetch_chunk = [&](int t0, int stop) {
+        stop = min(stop, length);
+        if constexpr (!STATE) fetch(a.q, a.key, t0, stop, next_q);
+        fetch(a.k, a.key, t0, stop, next_k);
+        fetch(a.v, a.value, t0, stop, next_v);
+        if constexpr (SLOPE && !STATE) fetch(a.with, a.value, t0, stop, next_with);
+        next_reset = a.reset && t0 + lane < stop ? a.reset[(size_t)(t0 + lane) * a.batch + b] : (uint8_t)0;
     };
-    auto put_rows = [&](int base, const Quad (&from)[4]) {
+    auto put = [&](int base, const Quad (&from)[ROUNDS][4]) {
 #pragma unroll
-        for (int r = 0; r < 4; r++) *reinterpret_cast<Quad*>(lds + base + (first + r) * L::ROW + channel) = from[r];
+        for (int round = 0; round < ROUNDS; round++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) *reinterpret_cast<Quad*>(lds + base + (first + round * ROUND_STEPS + r) * L::ROW + channel) = from[round][r];
     };
-    auto put_columns = [&](int base, const Quad (&from)[4]) {
-#pragma unroll
-        for (int c = 0; c < 4; c++) {
-            Quad x;
-#pragma unroll
-            for (int r = 0; r < 4; r++) x[r] = from[r][c];
-            *reinterpret_cast<Quad*>(lds + base + (channel + c) * L::COLUMN + first) = x;
-        }
-    };
-    // operands: eight summands 32 block + 8 quarter ... of a row; of a row in the order of the accumulators; of a column over the steps
+    // operands: eight summands 32 block + 8 quarter ... of a row; of a row in the order of the accumulators; of column 16 tile + l over the steps
     auto row_operand = [&](int base, int stride, int row, int block) { return *reinterpret_cast<const Vector*>(lds + base + row * stride + 32 * block + 8 * quarter); };
     auto tiled_operand = [&](int base, int row, int block) {
         const Quad x = *reinterpret_cast<const Quad*>(lds + base + row * L::ROW + 32 * block + 4 * quarter), y = *reinterpret_cast<const Quad*>(lds + base + row * L::ROW + 32 * block + 16 + 4 * quarter);
         return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
     };
-    auto column_operand = [&](int narrow_base, int rows_base, int col, int block) {
-        if constexpr (L::NARROW) return row_operand(narrow_base, L::COLUMN, col, block);
-        else {
+    auto column_operand = [&](int base, int tile, int block) {
+        if constexpr (sizeof(T) == 2) {      // the transposing load: of sixteen lanes, lane p names four channels 4 (p % 4) ... of step p / 4, and lane l receives channel l of the four steps
+            typedef short Raw __attribute__((ext_vector_type(4)));
+            typedef __attribute__((address_space(3))) Raw* Address;
+            T* const from = lds + base + (32 * block + 8 * quarter + l / 4) * L::ROW + 16 * tile + 4 * (l % 4);
+            const Raw x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Address)from), y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Address)(from + 4 * L::ROW));
+            return __builtin_bit_cast(Vector, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+        } else {
             Vector x;
 #pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = lds[rows_base + (32 * block + 8 * quarter + e) * L::ROW + col];
+            for (int e = 0; e < 8; e++) x[e] = lds[base + (32 * block + 8 * quarter + e) * L::ROW + 16 * tile + l];
             return x;
         }
     };
-    auto state_vector = [&](const rlt_f32x4 (&s)[KEY_TILES], int block) { return __builtin_shufflevector(s[2 * block], s[2 * block + 1], 0, 1, 2, 3, 4, 5, 6, 7); };
 
     if constexpr (!STATE) {      // score tiles that lie on the wrong side of the diagonal within a block of 32: zero for good
         constexpr int O0 = REVERSE ? 16 : 0, S0 = REVERSE ? 0 : 16;
-        for (int i = threadIdx.x; i < L::PLANES * 2 * 16 * 16; i += 4 * D) {
+        for (int i = threadIdx.x; i < L::PLANES * 2 * 16 * 16; i += L::THREADS) {
             const int plane = i / 512, which = (i / 256) % 2, row = (i / 16) % 16, col = i % 16;
-            lds[L::P + plane * CHUNK * L::COLUMN + (32 * which + O0 + row) * L::COLUMN + 32 * which + S0 + col] = (T)0.0f;
+            lds[L::P + plane * CHUNK * L::SCORES + (32 * which + O0 + row) * L::SCORES + 32 * which + S0 + col] = (T)0.0f;
         }
     }
-    float total = 0.0f;                       // SLOPE
-    float added_weight[2][8];                 // of the chunk's steps in the state after it
-    int weights_of = -1;                      // the number of steps that they are for
-    int counted = 0; bool forgotten = false;  // STATE
-    if (chunks > 0) fetch_chunk(REVERSE ? chunks - 1 : 0);
-    for (int c = 0; c < chunks; c++) {
-        const int chunk = REVERSE ? chunks - 1 - c : c, t0 = begin + chunk * CHUNK, n = min(max(min(length, end) - t0, 0), CHUNK);
-        const uint64_t resets = __ballot(next_reset != 0);
+    // weights of the scores of a tile: on the diagonal, and beside it (there a tile k further on has near * a^(16 (k - 1)))
+    float diagonal[4], near[4];
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        const int lag = REVERSE ? 4 * quarter + r - l : l - 4 * quarter - r;
+        diagonal[r] = lag >= 0 ? power(log2_decay, lag) * a.score_scale : 0.0f;
+        near[r] = power(log2_decay, 16 + lag) * a.score_scale;
+    }
+    float total = 0.0f;                                 // SLOPE
+    float read_weight[4], added_weight[2][8];           // of the state before the chunk in its steps' outputs, and of the steps in the state after it ...
+    int weights_n = -1; uint64_t weights_resets = 0;    // ... for so many steps and these resets
+    int counted = 0; bool forgotten = false;            // STATE
+    int t0 = REVERSE ? max(begin, end - CHUNK) : begin, stop = REVERSE ? end : min(begin + CHUNK, end);
+    fetch_chunk(t0, stop);
+    while (true) {
+        uint64_t resets = __ballot(next_reset != 0);
+        if (resets & ~1ull) {
+            // A step's weight of zero keeps other episodes out of sums of products as long as their values are finite. Where some are not, the chunk ends at its first reset (REVERSE: begins at its last).
+            bool finite = true;
+#pragma unroll
+            for (int round = 0; round < ROUNDS; round++)
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) finite = finite && __builtin_isfinite((float)next_k[round][r][c]) && __builtin_isfinite((float)next_v[round][r][c]);
+            const bool all = __all(finite);
+            if (lane == 0) flags[wave] = all ? 0.0f : 1.0f;
+        }
         rlt_lds_barrier();
-        if constexpr (!STATE) put_rows(L::Q, next_q);
-        if constexpr (!STATE || !L::NARROW) put_rows(L::KR, next_k);
-        if constexpr (L::NARROW) { put_columns(L::KT, next_k); put_columns(L::VT, next_v); }
-        if constexpr (!L::NARROW || (SLOPE && !STATE)) put_rows(L::VR, next_v);
-        if constexpr (SLOPE && !STATE) put_rows(L::WR, next_with);
+        if (resets & ~1ull) {
+            float any = 0.0f;
+            for (int w = 0; w < L::WAVES; w++) any += flags[w];
+            if (any != 0.0f) {
+                if (REVERSE) t0 += 63 - __builtin_clzll(resets); else stop = t0 + __builtin_ctzll(resets & ~1ull);
+                fetch_chunk(t0, stop);
+                resets = __ballot(next_reset != 0);
+            }
+        }
+        const int n = min(max(min(length, stop) - t0, 0), CHUNK);
+        put(L::K, next_k);
+        put(L::V, next_v);
+        if constexpr (!STATE) put(L::Q, next_q);
+        if constexpr (SLOPE && !STATE) put(L::W, next_with);
         rlt_lds_barrier();
-        if (c + 1 < chunks) fetch_chunk(REVERSE ? chunk - 1 : chunk + 1);
+        const bool done = REVERSE ? t0 <= begin : stop >= end;
+        const int next_t0 = REVERSE ? max(begin, t0 - CHUNK) : stop, next_stop = REVERSE ? t0 : min(stop + CHUNK, end);
+        if (!done) fetch_chunk(next_t0, next_stop);
 
-        if (n != weights_of) {
-            weights_of = n;
+        const int last_reset = resets ? 63 - __builtin_clzll(resets) : -1, first_reset = resets ? __builtin_ctzll(resets) : CHUNK;
+        if (n != weights_n || resets != weights_resets) {
+            weights_n = n; weights_resets = resets;
+#pragma unroll
+            for (int ot = 0; ot < 4; ot++) {
+                const int i = 16 * ot + l;
+                read_weight[ot] = i < n && (REVERSE ? last_reset <= i : first_reset > i) ? power(log2_decay, REVERSE ? n - 1 - i : i + 1) * a.read_scale : 0.0f;
+            }
 #pragma unroll
             for (int block = 0; block < 2; block++)
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
                     const int s = 32 * block + 8 * quarter + e;
-                    added_weight[block][e] = s < n ? power(log2_decay, REVERSE ? s : n - 1 - s) * a.added_scale : 0.0f;
+                    added_weight[block][e] = s < n && (REVERSE ? s < first_reset : s >= last_reset) ? power(log2_decay, REVERSE ? s : n - 1 - s) * a.added_scale : 0.0f;
                 }
         }
-        const int last_reset = resets ? 63 - __builtin_clzll(resets) : -1, first_reset = resets ? __builtin_ctzll(resets) : CHUNK;
         if constexpr (!STATE) {
             // scores, by tiles on and below (REVERSE: above) the diagonal: rows are the steps that are added, columns those that read
-            for (int tile = wave; tile < 10; tile += WAVES) {
-                int ot = tile < 1 ? 0 : tile < 3 ? 1 : tile < 6 ? 2 : 3, st = tile - ot * (ot + 1) / 2;
-                if (REVERSE) { ot = 3 - ot; st = 3 - st; }
+            for (int tile = wave; tile < 10; tile += L::WAVES) {
+                const int row = tile < 1 ? 0 : tile < 3 ? 1 : tile < 6 ? 2 : 3, col = tile - row * (row + 1) / 2, ot = REVERSE ? 3 - row : row, st = REVERSE ? 3 - col : col;
                 rlt_f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f}, y = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int block = 0; block < KEY_BLOCKS; block++) x = multiply(row_operand(L::KR, L::ROW, 16 * st + l, block), row_operand(L::Q, L::ROW, 16 * ot + l, block), x);
+                for (int block = 0; block < KEY_BLOCKS; block++) x = multiply(row_operand(L::K, L::ROW, 16 * st + l, block), row_operand(L::Q, L::ROW, 16 * ot + l, block), x);
                 if constexpr (SLOPE) {
 #pragma unroll
-                    for (int block = 0; block < KEY_BLOCKS; block++) y = multiply(row_operand(L::VR, L::ROW, 16 * st + l, block), row_operand(L::WR, L::ROW, 16 * ot + l, block), y);
+                    for (int block = 0; block < KEY_BLOCKS; block++) y = multiply(row_operand(L::V, L::ROW, 16 * st + l, block), row_operand(L::W, L::ROW, 16 * ot + l, block), y);
                 }
-                const int i = 16 * ot + l;      // the step that reads
-                const uint64_t before = resets & ((2ull << i) - 1), after = i < 63 ? resets & ~((2ull << i) - 1) : 0;
-                const int low = REVERSE ? i : before ? 63 - __builtin_clzll(before) : 0, high = REVERSE ? (after ? __builtin_ctzll(after) - 1 : 63) : i;      // steps that it sees
+                const int i = 16 * ot + l, apart = row - col;
+                if (apart == 0) {
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const int s = 16 * st + 4 * quarter + r, lag = REVERSE ? s - i : i - s;
-                    x[r] = s >= low && s <= high ? x[r] * (power(log2_decay, lag) * a.score_scale) : 0.0f;
-                    if constexpr (SLOPE) total += x[r] == 0.0f ? 0.0f : (float)lag * x[r] * y[r];
+                    for (int r = 0; r < 4; r++) x[r] = diagonal[r] != 0.0f ? x[r] * diagonal[r] : 0.0f;
+                } else {
+                    const float far = power(log2_decay, 16 * (apart - 1));
+#pragma unroll
+                    for (int r = 0; r < 4; r++) x[r] *= near[r] * far;
+                }
+                if (resets) {
+                    const uint64_t before = resets & ((2ull << i) - 1), after = i < 63 ? resets & ~((2ull << i) - 1) : 0;
+                    const int low = REVERSE ? 0 : before ? 63 - __builtin_clzll(before) : 0, high = REVERSE && after ? __builtin_ctzll(after) - 1 : 63;      // steps of the episode of step i
+#pragma unroll
+                    for (int r = 0; r < 4; r++) { const int s = 16 * st + 4 * quarter + r; x[r] = s >= low && s <= high ? x[r] : 0.0f; }
+                }
+                if constexpr (SLOPE) {
+#pragma unroll
+                    for (int r = 0; r < 4; r++) { const int s = 16 * st + 4 * quarter + r; total += x[r] == 0.0f ? 0.0f : (float)(REVERSE ? s - i : i - s) * x[r] * y[r]; }
                 }
 #pragma unroll
                 for (int plane = 0; plane < L::PLANES; plane++) {
                     const Quad part = __builtin_convertvector(x, Quad);
-                    *reinterpret_cast<Quad*>(lds + L::P + plane * CHUNK * L::COLUMN + i * L::COLUMN + 16 * st + 4 * quarter) = part;
+                    *reinterpret_cast<Quad*>(lds + L::P + plane * CHUNK * L::SCORES + i * L::SCORES + 16 * st + 4 * quarter) = part;
                     if (plane + 1 < L::PLANES) x -= __builtin_convertvector(part, rlt_f32x4);
                 }
             }
             // what the state before the chunk gives: columns of the result are the steps, rows the value columns
-            rlt_f32x4 out[4], out_slope[SLOPE ? 4 : 1];
+            rlt_f32x4 out[TILES][4], out_slope[SLOPE ? TILES : 1][SLOPE ? 4 : 1];
 #pragma unroll
-            for (int ot = 0; ot < 4; ot++) {
-                out[ot] = rlt_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                if constexpr (SLOPE) out_slope[ot] = rlt_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            }
-#pragma unroll
-            for (int block = 0; block < KEY_BLOCKS; block++) {
-                const Cut<T, STATE_CUTS> s(state_vector(state, block));
+            for (int tile = 0; tile < TILES; tile++)
 #pragma unroll
                 for (int ot = 0; ot < 4; ot++) {
-                    const Vector q = tiled_operand(L::Q, 16 * ot + l, block);
-#pragma unroll
-                    for (int p = 0; p < STATE_CUTS; p++) out[ot] = multiply(s.part[p], q, out[ot]);
+                    out[tile][ot] = rlt_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                    if constexpr (SLOPE) out_slope[tile][ot] = rlt_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
                 }
-                if constexpr (SLOPE) {
-                    const Cut<T, STATE_CUTS> d(state_vector(slope, block));
 #pragma unroll
-                    for (int ot = 0; ot < 4; ot++) {
-                        const Vector q = tiled_operand(L::Q, 16 * ot + l, block);
+            for (int block = 0; block < KEY_BLOCKS; block++) {
+                Vector q[4];
 #pragma unroll
-                        for (int p = 0; p < STATE_CUTS; p++) out_slope[ot] = multiply(d.part[p], q, out_slope[ot]);
+                for (int ot = 0; ot < 4; ot++) q[ot] = tiled_operand(L::Q, 16 * ot + l, block);
+#pragma unroll
+                for (int tile = 0; tile < TILES; tile++) {
+                    const Cut<T, STATE_CUTS> s(__builtin_shufflevector(state[tile][2 * block], state[tile][2 * block + 1], 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                    for (int ot = 0; ot < 4; ot++)
+#pragma unroll
+                        for (int p = 0; p < STATE_CUTS; p++) out[tile][ot] = multiply(s.part[p], q[ot], out[tile][ot]);
+                    if constexpr (SLOPE) {
+                        const Cut<T, STATE_CUTS> d(__builtin_shufflevector(slope[tile][2 * block], slope[tile][2 * block + 1], 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                        for (int ot = 0; ot < 4; ot++)
+#pragma unroll
+                            for (int p = 0; p < STATE_CUTS; p++) out_slope[tile][ot] = multiply(d.part[p], q[ot], out_slope[tile][ot]);
                     }
                 }
             }
+#pragma unroll
+            for (int tile = 0; tile < TILES; tile++)
+#pragma unroll
+                for (int ot = 0; ot < 4; ot++) {
+                    const int i = 16 * ot + l;
+                    if constexpr (SLOPE) {
+                        const Quad with = *reinterpret_cast<const Quad*>(lds + L::W + i * L::ROW + column0 + 16 * tile + 4 * quarter);
+                        float d = 0.0f;
+#pragma unroll
+                        for (int r = 0; r < 4; r++) d = fmaf((float)with[r], fmaf((float)(i + 1), out[tile][ot][r], out_slope[tile][ot][r]), d);
+                        if (read_weight[ot] != 0.0f) total = fmaf(read_weight[ot], d, total);
+                    }
+                    if (resets) {      // a state of another episode need not be finite
+#pragma unroll
+                        for (int r = 0; r < 4; r++) out[tile][ot][r] = read_weight[ot] != 0.0f ? out[tile][ot][r] * read_weight[ot] : 0.0f;
+                    } else out[tile][ot] *= read_weight[ot];
+                }
+            rlt_lds_barrier();
+            // what the chunk's own steps give
+#pragma unroll
+            for (int block = 0; block < 2; block++) {
+                Vector values[TILES];
+#pragma unroll
+                for (int tile = 0; tile < TILES; tile++) values[tile] = column_operand(L::V, TILES * wave + tile, block);
+#pragma unroll
+                for (int ot = 0; ot < 4; ot++)
+                    if (REVERSE ? 32 * block + 31 >= 16 * ot : 32 * block <= 16 * ot + 15) {
+#pragma unroll
+                        for (int plane = 0; plane < L::PLANES; plane++) {
+                            const Vector scores = row_operand(L::P + plane * CHUNK * L::SCORES, L::SCORES, 16 * ot + l, block);
+#pragma unroll
+                            for (int tile = 0; tile < TILES; tile++) out[tile][ot] = multiply(values[tile], scores, out[tile][ot]);
+                        }
+                    }
+            }
+            typedef typename Operand<O>::Quad OutQuad;
+            O* const to = at<O>(a.out, t0, b, h) + (int64_t)l * a.out.step + column0 + 4 * quarter;
 #pragma unroll
             for (int ot = 0; ot < 4; ot++) {
                 const int i = 16 * ot + l;
-                const bool sees = i < n && (REVERSE ? last_reset <= i : first_reset > i);
-                const float w = sees ? power(log2_decay, REVERSE ? n - 1 - i : i + 1) * a.read_scale : 0.0f;
-                if constexpr (SLOPE) {
-                    const Quad with = *reinterpret_cast<const Quad*>(lds + L::WR + i * L::ROW + 16 * wave + 4 * quarter);
-                    float d = 0.0f;
+                if (t0 + i < stop) {
 #pragma unroll
-                    for (int r = 0; r < 4; r++) d = fmaf((float)with[r], fmaf((float)(i + 1), out[ot][r], out_slope[ot][r]), d);
-                    if (sees) total = fmaf(w, d, total);
-                }
+                    for (int tile = 0; tile < TILES; tile++) {
+                        const int c0 = column0 + 16 * tile + 4 * quarter;
+                        rlt_f32x4 x = out[tile][ot];
+                        if (i >= n) x = rlt_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                        O* const here = to + (int64_t)(16 * ot) * a.out.step + 16 * tile;
+                        if (a.out.vectors) { if (c0 < a.value) *reinterpret_cast<OutQuad*>(here) = __builtin_convertvector(x, OutQuad); }
+                        else {
 #pragma unroll
-                for (int r = 0; r < 4; r++) out[ot][r] = sees ? out[ot][r] * w : 0.0f;
-            }
-            rlt_lds_barrier();
-            // what the chunk's own steps give
-            Vector values[2];
-#pragma unroll
-            for (int block = 0; block < 2; block++) values[block] = column_operand(L::VT, L::VR, column, block);
-#pragma unroll
-            for (int ot = 0; ot < 4; ot++)
-#pragma unroll
-                for (int block = 0; block < 2; block++)
-                    if (REVERSE ? 32 * block + 31 >= 16 * ot : 32 * block <= 16 * ot + 15) {
-#pragma unroll
-                        for (int plane = 0; plane < L::PLANES; plane++) out[ot] = multiply(values[block], row_operand(L::P + plane * CHUNK * L::COLUMN, L::COLUMN, 16 * ot + l, block), out[ot]);
-                    }
-#pragma unroll
-            for (int ot = 0; ot < 4; ot++) {
-                const int i = 16 * ot + l, c0 = 16 * wave + 4 * quarter;
-                if (t0 + i < end) {
-                    O* to = at<O>(a.out, t0 + i, b, h) + c0;
-                    typedef typename Operand<O>::Quad OutQuad;
-                    rlt_f32x4 x = out[ot];
-                    if (i >= n) x = rlt_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                    if (a.out.vectors) { if (c0 < a.value) *reinterpret_cast<OutQuad*>(to) = __builtin_convertvector(x, OutQuad); }
-                    else {
-#pragma unroll
-                        for (int r = 0; r < 4; r++) if (c0 + r < a.value) to[r] = (O)x[r];
+                            for (int r = 0; r < 4; r++) if (c0 + r < a.value) here[r] = (O)x[r];
+                        }
                     }
                 }
             }
         }
         // the state after the chunk
         if (n > 0) {
-            const float f = resets ? 0.0f : power(log2_decay, REVERSE ? n - 1 : n);
+            const float f = power(log2_decay, REVERSE ? n - 1 : n);
             counted += n; forgotten |= resets != 0;
 #pragma unroll
-            for (int k = 0; k < KEY_TILES; k++)
+            for (int tile = 0; tile < TILES; tile++)
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    if constexpr (SLOPE) slope[k][r] = resets ? 0.0f : f * fmaf((float)n, state[k][r], slope[k][r]);
-                    state[k][r] = resets ? 0.0f : f * state[k][r];
+                for (int k = 0; k < KEY_TILES; k++) {
+                    if (resets) {
+                        state[tile][k] = rlt_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                        if constexpr (SLOPE) slope[tile][k] = rlt_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                    } else {
+                        if constexpr (SLOPE) slope[tile][k] = f * (slope[tile][k] + (float)n * state[tile][k]);
+                        state[tile][k] *= f;
+                    }
                 }
 #pragma unroll
             for (int block = 0; block < 2; block++) {
-                const Vector v = column_operand(L::VT, L::VR, column, block);
-                rlt_f32x8 weighted, lagged;
+                rlt_f32x8 weight;
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const int s = 32 * block + 8 * quarter + e;
-                    const bool stays = REVERSE ? s < first_reset : s >= last_reset;
-                    weighted[e] = stays ? (float)v[e] * added_weight[block][e] : 0.0f;
-                    if constexpr (SLOPE) lagged[e] = weighted[e] * (float)(n - 1 - s);
-                }
-                const Cut<T, ADDED_CUTS> x(weighted);
+                for (int e = 0; e < 8; e++) weight[e] = added_weight[block][e];
+                Vector key[KEY_TILES];
 #pragma unroll
-                for (int k = 0; k < KEY_TILES; k++) {
-                    const Vector key = column_operand(L::KT, L::KR, 16 * k + l, block);
+                for (int k = 0; k < KEY_TILES; k++) key[k] = column_operand(L::K, k, block);
 #pragma unroll
-                    for (int p = 0; p < ADDED_CUTS; p++) state[k] = multiply(key, x.part[p], state[k]);
-                }
-                if constexpr (SLOPE) {
-                    const Cut<T, ADDED_CUTS> y(lagged);
+                for (int tile = 0; tile < TILES; tile++) {
+                    const Vector v = column_operand(L::V, TILES * wave + tile, block);
+                    const rlt_f32x8 weighted = __builtin_convertvector(v, rlt_f32x8) * weight;
+                    const Cut<T, ADDED_CUTS> x(weighted);
 #pragma unroll
-                    for (int k = 0; k < KEY_TILES; k++) {
-                        const Vector key = column_operand(L::KT, L::KR, 16 * k + l, block);
+                    for (int k = 0; k < KEY_TILES; k++)
 #pragma unroll
-                        for (int p = 0; p < ADDED_CUTS; p++) slope[k] = multiply(key, y.part[p], slope[k]);
+                        for (int p = 0; p < ADDED_CUTS; p++) state[tile][k] = multiply(key[k], x.part[p], state[tile][k]);
+                    if constexpr (SLOPE) {
+                        rlt_f32x8 lagged;
+#pragma unroll
+                        for (int e = 0; e < 8; e++) lagged[e] = weighted[e] * (float)(n - 1 - (32 * block + 8 * quarter + e));
+                        const Cut<T, ADDED_CUTS> y(lagged);
+#pragma unroll
+                        for (int k = 0; k < KEY_TILES; k++)
+#pragma unroll
+                            for (int p = 0; p < ADDED_CUTS; p++) slope[tile][k] = multiply(key[k], y.part[p], slope[tile][k]);
                     }
                 }
             }
             if constexpr (REVERSE) {      // the power that all of them share: the cut operands keep their parts above the smallest numbers also where one step forgets nearly everything
                 const float once = power(log2_decay, 1);
 #pragma unroll
-                for (int k = 0; k < KEY_TILES; k++)
+                for (int tile = 0; tile < TILES; tile++)
 #pragma unroll
-                    for (int r = 0; r < 4; r++) state[k][r] *= once;
+                    for (int k = 0; k < KEY_TILES; k++) state[tile][k] *= once;
             }
         }
+        if (done) break;
+        t0 = next_t0; stop = next_stop;
     }
 
-    if (a.exit)
-#pragma unroll
-        for (int k = 0; k < KEY_TILES; k++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int row = 16 * k + 4 * quarter + r;
-                if (row < a.key && column < a.value) {
-                    const size_t i = state_base + (size_t)row * a.state_key + (size_t)column * a.state_value;
-                    a.exit[i] = state[k][r];
-                    if constexpr (SLOPE && STATE) a.exit_slope[i] = slope[k][r];
-                }
-            }
-    if constexpr (STATE) { if (threadIdx.x == 0) a.factors[blockIdx.x] = make_float2(forgotten ? 0.0f : power(log2_decay, counted), (float)counted); }
+    if (a.exit) over_state([&](int tile, int k, int r, bool there, size_t i) {
+        if (there) {
+            a.exit[state_base + i] = state[tile][k][r];
+            if constexpr (SLOPE && STATE) a.exit_slope[state_base + i] = slope[tile][k][r];
+        }
+    });
+    if constexpr (STATE) { if (threadIdx.x == 0) a.factors[item] = make_float2(forgotten ? 0.0f : power(log2_decay, counted), (float)counted); }
     if constexpr (SLOPE && !STATE) {
-        if (a.d_final && segment == a.segments - 1)
-#pragma unroll
-            for (int k = 0; k < KEY_TILES; k++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const int row = 16 * k + 4 * quarter + r;
-                    if (row < a.key && column < a.value) total = fmaf(a.d_final[(size_t)pair * a.key * a.value + (size_t)row * a.state_key + (size_t)column * a.state_value], slope[k][r], total);
-                }
+        if (a.d_final && segment == a.segments - 1) over_state([&](int tile, int k, int r, bool there, size_t i) {
+            if (there) total = fmaf(a.d_final[(size_t)pair * a.key * a.value + i], slope[tile][k][r], total);
+        });
         total = rlt_wave_sum(total);
-        float* sums = (float*)lds_bytes;
         rlt_lds_barrier();
-        if (lane == 0) sums[wave] = total;
+        if (lane == 0) flags[wave] = total;
         rlt_lds_barrier();
         if (threadIdx.x == 0) {
             float s = 0.0f;
-            for (int w = 0; w < WAVES; w++) s += sums[w];
-            a.partial[blockIdx.x] = s;
+            for (int w = 0; w < L::WAVES; w++) s += flags[w];
+            a.partial[item] = s;
         }
     }
 }
@@ -481,22 +562,24 @@ Scratch scratch_of(const rlt_linear_attention* p, int steps, bool backward) {
     }
     if (backward) {
         s.partial = take(pairs * g.count);
-        if (p->heads != p->kv_heads) s.shared = take((size_t)steps * pairs * (p->key_dim > p->value_dim ? p->key_dim : p->value_dim));
+        if (p->heads != p->kv_heads) s.shared = take(padded((size_t)steps * pairs * p->value_dim) + (size_t)steps * pairs * p->key_dim);
     }
     s.total = at;
     return s;
 }
 
-template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE> int launch_walk(rlt_rocm_device* device, const Walk& a) {
-    constexpr size_t bytes = Layout<T, D, SLOPE, STATE>::BYTES;
+template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE> int launch_walk(rlt_rocm_device* device, const Walk& a, const Walk* second) {
+    typedef Layout<T, D, SLOPE, STATE> L;
     const auto kernel = walk_kernel<T, O, D, REVERSE, SLOPE, STATE>;
-    RLT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-    hipLaunchKernelGGL(kernel, dim3((unsigned)a.batch * a.heads * a.segments), dim3(4 * D), bytes, device->stream, a);
+    const unsigned items = (unsigned)a.batch * a.heads * a.segments;
+    RLT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)L::BYTES));
+    hipLaunchKernelGGL(kernel, dim3(second ? (items + 7) / 8 * 16 : items), dim3(L::THREADS), L::BYTES, device->stream, Walks{a, second ? *second : a, (int)items, second != nullptr});
     return rlt_launch_status(device);
 }
-template <typename T, typename O, bool REVERSE, bool SLOPE, bool STATE> int walk(rlt_rocm_device* device, const Walk& a) {
+template <typename T, typename O, bool REVERSE, bool SLOPE, bool STATE> int walk(rlt_rocm_device* device, const Walk& a, const Walk* second = nullptr) {
     const int width = a.key > a.value ? a.key : a.value;
-    return width <= 32 ? launch_walk<T, O, 32, REVERSE, SLOPE, STATE>(device, a) : width <= 64 ? launch_walk<T, O, 64, REVERSE, SLOPE, STATE>(device, a) : launch_walk<T, O, 128, REVERSE, SLOPE, STATE>(device, a);
+    return width <= 32 ? launch_walk<T, O, 32, REVERSE, SLOPE, STATE>(device, a, second) : width <= 64 ? launch_walk<T, O, 64, REVERSE, SLOPE, STATE>(device, a, second)
+                                                                                           : launch_walk<T, O, 128, REVERSE, SLOPE, STATE>(device, a, second);
 }
 Walk walk_of(const rlt_linear_attention* p, const uint8_t* reset, const int32_t* lengths, int steps) {
     const Segments g = segments_of(p, steps);
@@ -558,22 +641,23 @@ template <typename T> int backward(rlt_rocm_device* device, const rlt_linear_att
     r.k = Q; r.v = G; r.read_scale = 1.0f; r.added_scale = p->scale;
     if (cut && (rc = segment_states<T, true, false>(device, r, d_final_state, d_initial_state, states, nullptr, factors))) return rc;
     r.entry = cut ? states : d_final_state;
-    auto gradient = [&](Walk w, const rlt_head_view* to, int width) {
-        if (group == 1) { w.out = part<T>(to, 1, width); return walk<T, T, true, false, false>(device, w); }
-        float* shared = workspace + s.shared;
-        w.out = Part{shared, (int64_t)p->batch * p->heads * width, (int64_t)p->heads * width, width, 1, width % 4 == 0};
-        const int code = walk<T, float, true, false, false>(device, w);
-        if (code) return code;
-        hipLaunchKernelGGL((head_sum_kernel<T>), dim3(2048), dim3(128), 0, device->stream, shared, part<T>(to, 1, width), steps, p->batch, p->kv_heads, group, width);
-        return rlt_launch_status(device);
-    };
     Walk w = r;
-    w.q = K;
-    if (!cut) w.exit = d_initial_state;
-    if ((rc = gradient(w, d_v, p->value_dim))) return rc;
-    w = r;
+    r.q = K;
+    if (!cut) r.exit = d_initial_state;
     w.q = V; w.k = G; w.v = Q; w.key = p->value_dim; w.value = p->key_dim; w.state_key = 1; w.state_value = p->value_dim;
-    return gradient(w, d_k, p->key_dim);
+    if (group == 1) {
+        r.out = part<T>(d_v, 1, p->value_dim); w.out = part<T>(d_k, 1, p->key_dim);
+        return walk<T, T, true, false, false>(device, r, &w);
+    }
+    // shared keys and values: every head's share in fp32, then the sums over the heads
+    const size_t tokens = (size_t)steps * p->batch;
+    auto shares = [&](float* base, int width) { return Part{base, (int64_t)p->batch * p->heads * width, (int64_t)p->heads * width, width, 1, width % 4 == 0}; };
+    float* const shared_v = workspace + s.shared; float* const shared_k = shared_v + padded(tokens * p->heads * p->value_dim);
+    r.out = shares(shared_v, p->value_dim); w.out = shares(shared_k, p->key_dim);
+    if ((rc = walk<T, float, true, false, false>(device, r, &w))) return rc;
+    hipLaunchKernelGGL((head_sum_kernel<T>), dim3(2048), dim3(128), 0, device->stream, shared_v, part<T>(d_v, 1, p->value_dim), steps, p->batch, p->kv_heads, group, p->value_dim);
+    hipLaunchKernelGGL((head_sum_kernel<T>), dim3(2048), dim3(128), 0, device->stream, shared_k, part<T>(d_k, 1, p->key_dim), steps, p->batch, p->kv_heads, group, p->key_dim);
+    return rlt_launch_status(device);
 }
 
 }  // namespace

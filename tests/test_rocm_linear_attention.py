@@ -257,6 +257,25 @@ def test_a_reset_forgets_a_state_that_is_not_finite(rocm, dtype, steps):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("dk,dv", [(32, 32), (64, 48), (128, 128)])
+def test_an_episode_does_not_see_values_of_another_that_are_not_finite(rocm, dtype, dk, dv):
+    """row 0: a step of its first episode holds values that are not finite, in the chunk in which the second episode begins (and a third): from there on everything is as if they were"""
+    c, x = case(41, dtype, 200, 3, 2, 2, dk, dv)
+    x["reset"] = np.zeros((200, 3), np.uint8)
+    x["reset"][[75, 90, 140], 0] = 1
+    x["reset"][100, 1] = 1
+    want, size = reference(c, x), magnitudes(c, x)
+    b = bounds(c, want, size)
+    for i, n in enumerate(("q", "k", "v", "d_output")):
+        x[n][70, 0] = (np.nan, np.inf, np.nan, -np.inf)[i]
+    got = run(rocm, c, x)
+    for n in ("output", "d_q", "d_k", "d_v"):
+        assert np.all(np.abs(got[n][75:] - want[n][75:]) <= b[n][75:]) and np.all(np.abs(got[n][:, 1:] - want[n][:, 1:]) <= b[n][:, 1:]), n
+    assert np.all(np.abs(got["state"] - want["state"]) <= b["state"]) and np.all(np.abs(got["d_state"][1:] - want["d_state"][1:]) <= b["d_state"][1:])
+
+
+@gpu
 def test_the_decays_gradient_adds_up_and_runs_repeat_bit_for_bit(rocm):
     c, x = case(23, "float32", 200, 5, 4, 2, 32, 32, resets=0.02, ragged=True)
     first, second, onto = run(rocm, c, x), run(rocm, c, x), run(rocm, c, x, accumulate_onto=3.0)
