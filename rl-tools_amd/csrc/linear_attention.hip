@@ -5,8 +5,8 @@ namespace {
 
 constexpr int MAX_WIDTH = 128, CHUNK = 64;
 
-// a tensor as the kernels see it: heads / group of it; four channels side by side are one vector where `vectors` is set
-struct Part { void* data; int64_t step, row, head; int group, vectors; };
+// a tensor as the kernels see it: heads / group of it; channels side by side are read and written as vectors where `vectors` is set
+struct Part { void* data; int64_t step, row, head; int group, vectors; };      // vectors: of 16 bytes (inputs), of four channels (outputs)
 // One direction of the layer over segments of the steps. "key" and "value" are the two factors of what is added to the state [key x value], "query" what reads it.
 struct Walk {
     Part q, k, v, out;
@@ -32,8 +32,8 @@ template <typename T> __device__ __forceinline__ T* at(const Part& p, int t, int
 // 16x16x4 instructions, the e-th of which takes value e of every lane. Which summands a quarter has is free as long as both operands agree.
 typedef float rlt_f32x8 __attribute__((ext_vector_type(8)));
 template <typename T> struct Operand;
-template <> struct Operand<float> { typedef rlt_f32x8 Vector; typedef rlt_f32x4 Quad; };
-template <> struct Operand<rlt_bf16> { typedef rlt_bf16x8 Vector; typedef rlt_bf16x4 Quad; };
+template <> struct Operand<float> { typedef rlt_f32x8 Vector; typedef rlt_f32x4 Quad, Bytes16; };
+template <> struct Operand<rlt_bf16> { typedef rlt_bf16x8 Vector, Bytes16; typedef rlt_bf16x4 Quad; };
 __device__ __forceinline__ rlt_f32x4 multiply(rlt_f32x8 a, rlt_f32x8 b, rlt_f32x4 c) {
 #pragma unroll
     for (int e = 0; e < 8; e++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
@@ -82,11 +82,11 @@ template <typename T, int D, bool SLOPE, bool STATE> struct Layout {
 // product with the queries takes them. Scores of a chunk are shared out in tiles of 16 x 16, weighted, and exchanged through LDS. SLOPE carries the state's derivative by the decay's logarithm along.
 // STATE: only the state, of a segment that starts from nothing. A launch may hold two walks over the same rows (gradients of keys and of values), whose workgroups take turns on an XCD and so find each other's inputs in its L2.
 struct Walks { Walk first, second; int items, two; };
-template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE> __global__ __launch_bounds__((Layout<T, D, SLOPE, STATE>::THREADS), (Layout<T, D, SLOPE, STATE>::RESIDENT)) void walk_kernel(Walks walks) {
+template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, bool FULL> __global__ __launch_bounds__((Layout<T, D, SLOPE, STATE>::THREADS), (Layout<T, D, SLOPE, STATE>::RESIDENT)) void walk_kernel(Walks walks) {
     typedef typename Operand<T>::Vector Vector;
     typedef typename Operand<T>::Quad Quad;
     typedef Layout<T, D, SLOPE, STATE> L;
-    constexpr int KEY_TILES = D / 16, KEY_BLOCKS = D / 32, TILES = L::TILES, ROUNDS = CHUNK * D / (16 * L::THREADS), STATE_CUTS = CUTS<T, SLOPE ? 3 : 2>, ADDED_CUTS = CUTS<T, 3>;
+    constexpr int KEY_TILES = D / 16, KEY_BLOCKS = D / 32, TILES = L::TILES, STATE_CUTS = CUTS<T, SLOPE ? 3 : 2>, ADDED_CUTS = CUTS<T, 3>;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds_bytes[];
     T* const lds = (T*)lds_bytes;
     float* const flags = (float*)(lds_bytes + L::FLAGS * sizeof(T));
@@ -104,6 +104,7 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE> _
     rlt_f32x4 state[TILES][KEY_TILES], slope[SLOPE ? TILES : 1][SLOPE ? KEY_TILES : 1];
     const int column0 = 16 * TILES * wave;
     const size_t state_base = (size_t)item * a.key * a.value;
+    const int state_key = a.state_key, state_value = a.state_value;
     auto over_state = [&](auto f) {
 #pragma unroll
         for (int tile = 0; tile < TILES; tile++)
@@ -112,44 +113,48 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE> _
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     const int row = 16 * k + 4 * quarter + r, column = column0 + 16 * tile + l;
-                    f(tile, k, r, row < a.key && column < a.value, (size_t)row * a.state_key + (size_t)column * a.state_value);
+                    f(tile, k, r, FULL || (row < a.key && column < a.value), row * state_key + column * state_value);
                 }
     };
-    over_state([&](int tile, int k, int r, bool there, size_t i) {
-        state[tile][k][r] = !STATE && a.entry && there ? a.entry[state_base + i] : 0.0f;
-        if constexpr (SLOPE) slope[tile][k][r] = !STATE && a.entry_slope && there ? a.entry_slope[state_base + i] : 0.0f;
+    over_state([&](int tile, int k, int r, bool there, int i) {
+        state[tile][k][r] = 0.0f;
+        if constexpr (SLOPE) slope[tile][k][r] = 0.0f;
     });
+    if (const float* from = STATE ? nullptr : a.entry) {
+        from += state_base;
+        over_state([&](int tile, int k, int r, bool there, int i) { if (there) state[tile][k][r] = from[i]; });
+    }
+    if constexpr (SLOPE && !STATE)
+        if (const float* from = a.entry_slope) {
+            from += state_base;
+            over_state([&](int tile, int k, int r, bool there, int i) { if (there) slope[tile][k][r] = from[i]; });
+        }
 
-    // what a thread carries from memory to LDS, in rounds: four steps of four channels of each tensor
-    const int channel = (threadIdx.x % (D / 4)) * 4, first = (threadIdx.x / (D / 4)) * 4;
-    constexpr int ROUND_STEPS = 16 * L::THREADS / D;
-    Quad next_q[STATE ? 1 : ROUNDS][4], next_k[ROUNDS][4], next_v[ROUNDS][4], next_with[SLOPE && !STATE ? ROUNDS : 1][4];
+    // what a thread carries from memory to LDS, in rounds: 16 bytes of a step of each tensor
+    typedef typename Operand<T>::Bytes16 Bytes16;
+    constexpr int V = 16 / sizeof(T), ROUNDS = CHUNK * D / (V * L::THREADS), ROUND_STEPS = L::THREADS * V / D;
+    const int channel = (threadIdx.x % (D / V)) * V, first = threadIdx.x / (D / V);
+    Bytes16 next_q[STATE ? 1 : ROUNDS], next_k[ROUNDS], next_v[ROUNDS], next_with[SLOPE && !STATE ? ROUNDS : 1];
     uint8_t next_reset = 0;
-    auto fetch = [&](const Part& p, int width, int t0, int stop, Quad (&to)[ROUNDS][4]) {
+    auto fetch = [&](const Part& p, int width, int t0, int stop, Bytes16 (&to)[ROUNDS]) {
         const T* src = at<T>(p, t0, b, h) + (int64_t)first * p.step + channel;
-        if (p.vectors && stop - t0 == CHUNK) {
+        if (FULL && stop - t0 == CHUNK) {
 #pragma unroll
-            for (int round = 0; round < ROUNDS; round++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    to[round][r] = Quad{};
-                    if (channel < width) to[round][r] = *reinterpret_cast<const Quad*>(src + (int64_t)(round * ROUND_STEPS + r) * p.step);
-                }
+            for (int round = 0; round < ROUNDS; round++) to[round] = *reinterpret_cast<const Bytes16*>(src + (int64_t)(round * ROUND_STEPS) * p.step);
         } else {
 #pragma unroll
-            for (int round = 0; round < ROUNDS; round++)
+            for (int round = 0; round < ROUNDS; round++) {
+                to[round] = Bytes16{};
+                if (t0 + first + round * ROUND_STEPS < stop) {
+                    const T* from = src + (int64_t)(round * ROUND_STEPS) * p.step;
+                    if (FULL) to[round] = *reinterpret_cast<const Bytes16*>(from);
+                    else if (p.vectors) { if (channel < width) to[round] = *reinterpret_cast<const Bytes16*>(from); }
+                    else {
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    to[round][r] = Quad{};
-                    if (t0 + first + round * ROUND_STEPS + r < stop) {
-                        const T* from = src + (int64_t)(round * ROUND_STEPS + r) * p.step;
-                        if (p.vectors) { if (channel < width) to[round][r] = *reinterpret_cast<const Quad*>(from); }
-                        else {
-#pragma unroll
-                            for (int c = 0; c < 4; c++) if (channel + c < width) to[round][r][c] = from[c];
-                        }
+                        for (int c = 0; c < V; c++) if (channel + c < width) to[round][c] = from[c];
                     }
                 }
+            }
         }
     };
     auto fetch_chunk = [&](int t0, int stop) {
@@ -160,11 +165,9 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE> _
         if constexpr (SLOPE && !STATE) fetch(a.with, a.value, t0, stop, next_with);
         next_reset = a.reset && t0 + lane < stop ? a.reset[(size_t)(t0 + lane) * a.batch + b] : (uint8_t)0;
     };
-    auto put = [&](int base, const Quad (&from)[ROUNDS][4]) {
+    auto put = [&](int base, const Bytes16 (&from)[ROUNDS]) {
 #pragma unroll
-        for (int round = 0; round < ROUNDS; round++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) *reinterpret_cast<Quad*>(lds + base + (first + round * ROUND_STEPS + r) * L::ROW + channel) = from[round][r];
+        for (int round = 0; round < ROUNDS; round++) *reinterpret_cast<Bytes16*>(lds + base + (first + round * ROUND_STEPS) * L::ROW + channel) = from[round];
     };
     // operands: eight summands 32 block + 8 quarter ... of a row; of a row in the order of the accumulators; of column 16 tile + l over the steps
     auto row_operand = [&](int base, int stride, int row, int block) { return *reinterpret_cast<const Vector*>(lds + base + row * stride + 32 * block + 8 * quarter); };
@@ -212,14 +215,12 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE> _
         uint64_t resets = __ballot(next_reset != 0);
         if (resets & ~1ull) {
             // A step's weight of zero keeps other episodes out of sums of products as long as their values are finite. Where some are not, the chunk ends at its first reset (REVERSE: begins at its last).
-            bool finite = true;
+            float zero = 0.0f;
 #pragma unroll
             for (int round = 0; round < ROUNDS; round++)
 #pragma unroll
-                for (int r = 0; r < 4; r++)
-#pragma unroll
-                    for (int c = 0; c < 4; c++) finite = finite && __builtin_isfinite((float)next_k[round][r][c]) && __builtin_isfinite((float)next_v[round][r][c]);
-            const bool all = __all(finite);
+                for (int c = 0; c < V; c++) { zero = fmaf((float)next_k[round][c], 0.0f, zero); zero = fmaf((float)next_v[round][c], 0.0f, zero); }
+            const bool all = __all(zero == 0.0f);
             if (lane == 0) flags[wave] = all ? 0.0f : 1.0f;
         }
         rlt_lds_barrier();
@@ -372,7 +373,8 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE> _
                         rlt_f32x4 x = out[tile][ot];
                         if (i >= n) x = rlt_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
                         O* const here = to + (int64_t)(16 * ot) * a.out.step + 16 * tile;
-                        if (a.out.vectors) { if (c0 < a.value) *reinterpret_cast<OutQuad*>(here) = __builtin_convertvector(x, OutQuad); }
+                        if (FULL) *reinterpret_cast<OutQuad*>(here) = __builtin_convertvector(x, OutQuad);
+                        else if (a.out.vectors) { if (c0 < a.value) *reinterpret_cast<OutQuad*>(here) = __builtin_convertvector(x, OutQuad); }
                         else {
 #pragma unroll
                             for (int r = 0; r < 4; r++) if (c0 + r < a.value) here[r] = (O)x[r];
@@ -411,9 +413,11 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE> _
                     const rlt_f32x8 weighted = __builtin_convertvector(v, rlt_f32x8) * weight;
                     const Cut<T, ADDED_CUTS> x(weighted);
 #pragma unroll
-                    for (int k = 0; k < KEY_TILES; k++)
+                    for (int p = 0; p < ADDED_CUTS; p++) {
+                        if (!STATE && !SLOPE && p == 2 && !a.exit) break;      // a state that only goes into outputs of this type does with two parts
 #pragma unroll
-                        for (int p = 0; p < ADDED_CUTS; p++) state[tile][k] = multiply(key[k], x.part[p], state[tile][k]);
+                        for (int k = 0; k < KEY_TILES; k++) state[tile][k] = multiply(key[k], x.part[p], state[tile][k]);
+                    }
                     if constexpr (SLOPE) {
                         rlt_f32x8 lagged;
 #pragma unroll
@@ -438,17 +442,20 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE> _
         t0 = next_t0; stop = next_stop;
     }
 
-    if (a.exit) over_state([&](int tile, int k, int r, bool there, size_t i) {
-        if (there) {
-            a.exit[state_base + i] = state[tile][k][r];
-            if constexpr (SLOPE && STATE) a.exit_slope[state_base + i] = slope[tile][k][r];
-        }
-    });
+    if (float* to = a.exit) {
+        to += state_base;
+        over_state([&](int tile, int k, int r, bool there, int i) { if (there) to[i] = state[tile][k][r]; });
+    }
+    if constexpr (SLOPE && STATE) {
+        float* const to = a.exit_slope + state_base;
+        over_state([&](int tile, int k, int r, bool there, int i) { if (there) to[i] = slope[tile][k][r]; });
+    }
     if constexpr (STATE) { if (threadIdx.x == 0) a.factors[item] = make_float2(forgotten ? 0.0f : power(log2_decay, counted), (float)counted); }
     if constexpr (SLOPE && !STATE) {
-        if (a.d_final && segment == a.segments - 1) over_state([&](int tile, int k, int r, bool there, size_t i) {
-            if (there) total = fmaf(a.d_final[(size_t)pair * a.key * a.value + i], slope[tile][k][r], total);
-        });
+        if (a.d_final && segment == a.segments - 1) {
+            const float* const from = a.d_final + (size_t)pair * a.key * a.value;
+            over_state([&](int tile, int k, int r, bool there, int i) { if (there) total = fmaf(from[i], slope[tile][k][r], total); });
+        }
         total = rlt_wave_sum(total);
         rlt_lds_barrier();
         if (lane == 0) flags[wave] = total;
@@ -526,8 +533,8 @@ template <typename T> __global__ __launch_bounds__(128) void step_kernel(Walk a)
     at<T>(a.out, 0, b, h)[c] = (T)(out * a.read_scale);
 }
 
-template <typename T> Part part(const rlt_head_view* v, int group, int width) {
-    const bool vectors = reinterpret_cast<uintptr_t>(v->data) % (4 * sizeof(T)) == 0 && v->step_stride % 4 == 0 && v->row_stride % 4 == 0 && v->head_stride % 4 == 0 && width % 4 == 0;
+template <typename T, int V = 16 / sizeof(T)> Part part(const rlt_head_view* v, int group, int width) {
+    const bool vectors = reinterpret_cast<uintptr_t>(v->data) % (V * sizeof(T)) == 0 && v->step_stride % V == 0 && v->row_stride % V == 0 && v->head_stride % V == 0 && width % V == 0;
     return Part{v->data, v->step_stride, v->row_stride, v->head_stride, group, vectors};
 }
 bool described(const rlt_linear_attention* p) {
@@ -542,7 +549,7 @@ struct Segments { int count, steps; };
 Segments segments_of(const rlt_linear_attention* p, int steps) {
     const int chunks = (steps + CHUNK - 1) / CHUNK;
     const int64_t pairs = (int64_t)p->batch * p->heads;
-    int64_t count = pairs >= 256 ? 1 : (256 + pairs - 1) / pairs;
+    int64_t count = pairs >= 512 ? 1 : (512 + pairs - 1) / pairs;
     if (count > (chunks + 3) / 4) count = (chunks + 3) / 4;      // at least four chunks each
     const int per = (int)((chunks + count - 1) / count);
     return {(chunks + per - 1) / per, per * CHUNK};
@@ -568,18 +575,25 @@ Scratch scratch_of(const rlt_linear_attention* p, int steps, bool backward) {
     return s;
 }
 
-template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE> int launch_walk(rlt_rocm_device* device, const Walk& a, const Walk* second) {
+template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, bool FULL> int launch_walk(rlt_rocm_device* device, const Walk& a, const Walk* second) {
     typedef Layout<T, D, SLOPE, STATE> L;
-    const auto kernel = walk_kernel<T, O, D, REVERSE, SLOPE, STATE>;
+    const auto kernel = walk_kernel<T, O, D, REVERSE, SLOPE, STATE, FULL>;
     const unsigned items = (unsigned)a.batch * a.heads * a.segments;
     RLT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)L::BYTES));
     hipLaunchKernelGGL(kernel, dim3(second ? (items + 7) / 8 * 16 : items), dim3(L::THREADS), L::BYTES, device->stream, Walks{a, second ? *second : a, (int)items, second != nullptr});
     return rlt_launch_status(device);
 }
+// FULL: heads of exactly D channels, all of whose tensors may be read and written in vectors
+template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE> int walk_width(rlt_rocm_device* device, const Walk& a, const Walk* second) {
+    auto full = [&](const Walk& w) {
+        return w.key == D && w.value == D && w.k.vectors && w.v.vectors && (STATE || (w.q.vectors && w.out.vectors)) && (!SLOPE || STATE || w.with.vectors);
+    };
+    return full(a) && (!second || full(*second)) ? launch_walk<T, O, D, REVERSE, SLOPE, STATE, true>(device, a, second) : launch_walk<T, O, D, REVERSE, SLOPE, STATE, false>(device, a, second);
+}
 template <typename T, typename O, bool REVERSE, bool SLOPE, bool STATE> int walk(rlt_rocm_device* device, const Walk& a, const Walk* second = nullptr) {
     const int width = a.key > a.value ? a.key : a.value;
-    return width <= 32 ? launch_walk<T, O, 32, REVERSE, SLOPE, STATE>(device, a, second) : width <= 64 ? launch_walk<T, O, 64, REVERSE, SLOPE, STATE>(device, a, second)
-                                                                                           : launch_walk<T, O, 128, REVERSE, SLOPE, STATE>(device, a, second);
+    return width <= 32 ? walk_width<T, O, 32, REVERSE, SLOPE, STATE>(device, a, second) : width <= 64 ? walk_width<T, O, 64, REVERSE, SLOPE, STATE>(device, a, second)
+                                                                                           : walk_width<T, O, 128, REVERSE, SLOPE, STATE>(device, a, second);
 }
 Walk walk_of(const rlt_linear_attention* p, const uint8_t* reset, const int32_t* lengths, int steps) {
     const Segments g = segments_of(p, steps);
@@ -605,7 +619,7 @@ template <typename T> int forward(rlt_rocm_device* device, const rlt_linear_atte
     const int group = p->heads / p->kv_heads;
     const Scratch s = scratch_of(p, steps, false);
     Walk a = walk_of(p, reset, lengths, steps);
-    a.q = part<T>(q, 1, p->key_dim); a.k = part<T>(k, group, p->key_dim); a.v = part<T>(v, group, p->value_dim); a.out = part<T>(output, 1, p->value_dim);
+    a.q = part<T>(q, 1, p->key_dim); a.k = part<T>(k, group, p->key_dim); a.v = part<T>(v, group, p->value_dim); a.out = part<T, 4>(output, 1, p->value_dim);
     a.entry = initial_state; a.exit = final_state;
     if (a.segments > 1) {
         const int rc = segment_states<T, false, false>(device, a, initial_state, final_state, workspace + s.states, nullptr, (float2*)(workspace + s.factors));
@@ -631,7 +645,7 @@ template <typename T> int backward(rlt_rocm_device* device, const rlt_linear_att
         rc = d_log_decay ? segment_states<T, false, true>(device, a, initial_state, nullptr, states, slopes, factors) : segment_states<T, false, false>(device, a, initial_state, nullptr, states, nullptr, factors);
         if (rc) return rc;
     }
-    a.q = G; a.k = V; a.v = K; a.with = Q; a.out = part<T>(d_q, 1, p->key_dim); a.key = p->value_dim; a.value = p->key_dim; a.state_key = 1; a.state_value = p->value_dim;
+    a.q = G; a.k = V; a.v = K; a.with = Q; a.out = part<T, 4>(d_q, 1, p->key_dim); a.key = p->value_dim; a.value = p->key_dim; a.state_key = 1; a.state_value = p->value_dim;
     a.entry = cut ? states : initial_state; a.entry_slope = cut ? slopes : nullptr; a.d_final = d_final_state; a.partial = workspace + s.partial;
     rc = d_log_decay ? walk<T, T, false, true, false>(device, a) : walk<T, T, false, false, false>(device, a);
     if (rc) return rc;
@@ -646,7 +660,7 @@ template <typename T> int backward(rlt_rocm_device* device, const rlt_linear_att
     if (!cut) r.exit = d_initial_state;
     w.q = V; w.k = G; w.v = Q; w.key = p->value_dim; w.value = p->key_dim; w.state_key = 1; w.state_value = p->value_dim;
     if (group == 1) {
-        r.out = part<T>(d_v, 1, p->value_dim); w.out = part<T>(d_k, 1, p->key_dim);
+        r.out = part<T, 4>(d_v, 1, p->value_dim); w.out = part<T, 4>(d_k, 1, p->key_dim);
         return walk<T, T, true, false, false>(device, r, &w);
     }
     // shared keys and values: every head's share in fp32, then the sums over the heads
@@ -655,8 +669,8 @@ template <typename T> int backward(rlt_rocm_device* device, const rlt_linear_att
     float* const shared_v = workspace + s.shared; float* const shared_k = shared_v + padded(tokens * p->heads * p->value_dim);
     r.out = shares(shared_v, p->value_dim); w.out = shares(shared_k, p->key_dim);
     if ((rc = walk<T, float, true, false, false>(device, r, &w))) return rc;
-    hipLaunchKernelGGL((head_sum_kernel<T>), dim3(2048), dim3(128), 0, device->stream, shared_v, part<T>(d_v, 1, p->value_dim), steps, p->batch, p->kv_heads, group, p->value_dim);
-    hipLaunchKernelGGL((head_sum_kernel<T>), dim3(2048), dim3(128), 0, device->stream, shared_k, part<T>(d_k, 1, p->key_dim), steps, p->batch, p->kv_heads, group, p->key_dim);
+    hipLaunchKernelGGL((head_sum_kernel<T>), dim3(2048), dim3(128), 0, device->stream, shared_v, part<T, 4>(d_v, 1, p->value_dim), steps, p->batch, p->kv_heads, group, p->value_dim);
+    hipLaunchKernelGGL((head_sum_kernel<T>), dim3(2048), dim3(128), 0, device->stream, shared_k, part<T, 4>(d_k, 1, p->key_dim), steps, p->batch, p->kv_heads, group, p->key_dim);
     return rlt_launch_status(device);
 }
 
@@ -704,7 +718,7 @@ int rlt_rocm_linear_attention_step(rlt_rocm_device* device, const rlt_linear_att
     a.entry = state; a.exit = next_state;
     auto views = [&](auto type) {
         typedef decltype(type) T;
-        a.q = part<T>(q, 1, layer->key_dim); a.k = part<T>(k, group, layer->key_dim); a.v = part<T>(v, group, layer->value_dim); a.out = part<T>(output, 1, layer->value_dim);
+        a.q = part<T>(q, 1, layer->key_dim); a.k = part<T>(k, group, layer->key_dim); a.v = part<T>(v, group, layer->value_dim); a.out = part<T, 4>(output, 1, layer->value_dim);
         hipLaunchKernelGGL((step_kernel<T>), dim3((unsigned)a.heads * a.batch), dim3(MAX_WIDTH), 0, device->stream, a);
     };
     if (layer->type == RLT_TYPE_F32) views(0.0f); else views((rlt_bf16)0.0f);
