@@ -1,5 +1,6 @@
 // Linear attention with a decay for each head: sequences forward and backward, and single steps on a kept state.
 #include "typed.h"
+#include <type_traits>
 
 namespace {
 
@@ -62,14 +63,16 @@ template <typename T, int PARTS> constexpr int CUTS = sizeof(T) == 4 ? 1 : PARTS
 // decay^n; n = 0 gives 1 also for a decay of zero
 __device__ __forceinline__ float power(float log2_decay, int n) { return n == 0 ? 1.0f : __builtin_amdgcn_exp2f(log2_decay * (float)n); }
 
-// Shape of a workgroup for heads of up to D channels: a wavefront owns TILES x 16 of the value columns.
+// Shape of a workgroup for heads of up to D channels: a wavefront owns TILES x 16 of the value columns. SPLIT workgroups share a head's columns where two states would not fit the registers of one: the scores are then
+// formed in each of them.
 template <typename T, int D, bool SLOPE, bool STATE> struct Layout {
-    static constexpr int TILES = D == 128 && sizeof(T) == 2 && !SLOPE ? 2 : 1, WAVES = D / (16 * TILES), THREADS = 64 * WAVES;
-    static constexpr int PAD = 16 / sizeof(T), ROW = D + PAD, SCORES = CHUNK + PAD;      // rows start 4 (of 64) banks after each other: sixteen of them side by side in 16 bytes each meet no bank twice
+    static constexpr int SPLIT = SLOPE && D == 128 ? 2 : 1, COLUMNS = D / SPLIT;
+    static constexpr int TILES = D == 128 && sizeof(T) == 2 && !SLOPE ? 2 : 1, WAVES = COLUMNS / (16 * TILES), THREADS = 64 * WAVES;
+    static constexpr int PAD = 16 / sizeof(T), ROW = D + PAD, COLUMN_ROW = COLUMNS + PAD, SCORES = CHUNK + PAD;      // rows start 4 (of 64) banks after each other: sixteen of them side by side in 16 bytes each meet no bank twice
     static constexpr int PLANES = sizeof(T) == 2 ? 2 : 1;
-    static constexpr int K = 0, V = K + CHUNK * ROW, Q = V + CHUNK * ROW, W = Q + (STATE ? 0 : CHUNK * ROW), P = W + (SLOPE && !STATE ? CHUNK * ROW : 0);
+    static constexpr int K = 0, V = K + CHUNK * ROW, Q = V + CHUNK * COLUMN_ROW, W = Q + (STATE ? 0 : CHUNK * ROW), P = W + (SLOPE && !STATE ? CHUNK * COLUMN_ROW : 0);
     static constexpr int FLAGS = P + (STATE ? 0 : PLANES * CHUNK * SCORES);
-    static constexpr size_t BYTES = FLAGS * sizeof(T) + WAVES * sizeof(float);
+    static constexpr size_t BYTES = FLAGS * sizeof(T) + (4 * CHUNK + 16 + WAVES) * sizeof(float);
     // wavefronts that the registers of a SIMD are shared by: as many as LDS has room for workgroups
     static constexpr int FIT = (int)(163840 / BYTES) * WAVES / 4, MOST = D == 128 ? 2 : 3, RESIDENT = FIT < 1 ? 1 : FIT > MOST ? MOST : FIT;
 };
@@ -89,20 +92,22 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
     constexpr int KEY_TILES = D / 16, KEY_BLOCKS = D / 32, TILES = L::TILES, STATE_CUTS = CUTS<T, SLOPE ? 3 : 2>, ADDED_CUTS = CUTS<T, 3>;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds_bytes[];
     T* const lds = (T*)lds_bytes;
-    float* const flags = (float*)(lds_bytes + L::FLAGS * sizeof(T));
+    // weights of a chunk's steps: in the state after it, and of the state before it in their outputs
+    float* const added_weights = (float*)(lds_bytes + L::FLAGS * sizeof(T)); float* const read_weights = added_weights + CHUNK; float* const lagged_weights = read_weights + CHUNK;
+    float* const score_weights = lagged_weights + CHUNK + 16; float* const flags = score_weights + CHUNK;      // of scores by their lag, -16 ... 63 (zero below 0)
     const bool other = walks.two && (blockIdx.x / 8) % 2;
-    const int item = walks.two ? blockIdx.x / 16 * 8 + blockIdx.x % 8 : blockIdx.x;
+    const int item = (walks.two ? blockIdx.x / 16 * 8 + blockIdx.x % 8 : blockIdx.x) / L::SPLIT, half = L::SPLIT > 1 ? blockIdx.x % L::SPLIT : 0;
     if (item >= walks.items) return;
     const Walk& a = other ? walks.second : walks.first;
     const int pair = item / a.segments, segment = item % a.segments, b = pair / a.heads, h = pair % a.heads;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, quarter = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane & 15, quarter = lane >> 4;
     const int length = a.lengths ? min(max(a.lengths[b], 0), a.steps) : a.steps;
     const float log2_decay = a.log_decay[h] * 1.44269504088896341f;
     const int begin = segment * a.segment_steps, end = min(begin + a.segment_steps, a.steps);
 
     // state: tile k, element r of this lane is row 16 k + 4 quarter + r, column 16 (TILES wave + tile) + l
     rlt_f32x4 state[TILES][KEY_TILES], slope[SLOPE ? TILES : 1][SLOPE ? KEY_TILES : 1];
-    const int column0 = 16 * TILES * wave;
+    const int part0 = half * L::COLUMNS, inner0 = 16 * TILES * wave, column0 = part0 + inner0;      // first column of the workgroup, of the wavefront within it, of the wavefront
     const size_t state_base = (size_t)item * a.key * a.value;
     const int state_key = a.state_key, state_value = a.state_value;
     auto over_state = [&](auto f) {
@@ -130,44 +135,65 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
             over_state([&](int tile, int k, int r, bool there, int i) { if (there) slope[tile][k][r] = from[i]; });
         }
 
-    // what a thread carries from memory to LDS, in rounds: 16 bytes of a step of each tensor
+    // what a thread carries from memory to LDS, in rounds: 16 bytes of a step of each tensor, of all D channels or of the workgroup's columns
     typedef typename Operand<T>::Bytes16 Bytes16;
-    constexpr int V = 16 / sizeof(T), ROUNDS = CHUNK * D / (V * L::THREADS), ROUND_STEPS = L::THREADS * V / D;
-    const int channel = (threadIdx.x % (D / V)) * V, first = threadIdx.x / (D / V);
-    Bytes16 next_q[STATE ? 1 : ROUNDS], next_k[ROUNDS], next_v[ROUNDS], next_with[SLOPE && !STATE ? ROUNDS : 1];
+    constexpr int V = 16 / sizeof(T), ROUNDS = CHUNK * D / (V * L::THREADS), COLUMN_ROUNDS = CHUNK * L::COLUMNS / (V * L::THREADS);
+    Bytes16 next_q[STATE ? 1 : ROUNDS], next_k[ROUNDS], next_v[COLUMN_ROUNDS], next_with[SLOPE && !STATE ? COLUMN_ROUNDS : 1];
     uint8_t next_reset = 0;
-    auto fetch = [&](const Part& p, int width, int t0, int stop, Bytes16 (&to)[ROUNDS]) {
-        const T* src = at<T>(p, t0, b, h) + (int64_t)first * p.step + channel;
+    constexpr std::integral_constant<int, D> whole{};
+    constexpr std::integral_constant<int, L::COLUMNS> columns{};
+    // where a thread's vectors of step 0 lie, once for the walk
+    auto lane_of = [&](const Part& p, int from, auto across) {
+        constexpr int ACROSS = decltype(across)::value;
+        return at<T>(p, 0, b, h) + (int64_t)(threadIdx.x / (ACROSS / V)) * p.step + from + (threadIdx.x % (ACROSS / V)) * V;
+    };
+    const T* const lane_k = lane_of(a.k, 0, whole); const T* const lane_v = lane_of(a.v, part0, columns);
+    const T* const lane_q = STATE ? nullptr : lane_of(a.q, 0, whole); const T* const lane_with = SLOPE && !STATE ? lane_of(a.with, part0, columns) : nullptr;
+    auto fetch = [&](const T* lane_of_step_0, int64_t stride, int vectors, int from, int width, int t0, int stop, auto& to, auto across) {
+        constexpr int ACROSS = decltype(across)::value, N = CHUNK * ACROSS / (V * L::THREADS), STEPS = L::THREADS * V / ACROSS;
+        const T* const src = lane_of_step_0 + t0 * stride;
         if (FULL && stop - t0 == CHUNK) {
 #pragma unroll
-            for (int round = 0; round < ROUNDS; round++) to[round] = *reinterpret_cast<const Bytes16*>(src + (int64_t)(round * ROUND_STEPS) * p.step);
-        } else {
+            for (int round = 0; round < N; round++) to[round] = *reinterpret_cast<const Bytes16*>(src + (round * STEPS) * stride);
+        } else if (stop <= t0) {
 #pragma unroll
-            for (int round = 0; round < ROUNDS; round++) {
-                to[round] = Bytes16{};
-                if (t0 + first + round * ROUND_STEPS < stop) {
-                    const T* from = src + (int64_t)(round * ROUND_STEPS) * p.step;
-                    if (FULL) to[round] = *reinterpret_cast<const Bytes16*>(from);
-                    else if (p.vectors) { if (channel < width) to[round] = *reinterpret_cast<const Bytes16*>(from); }
-                    else {
+            for (int round = 0; round < N; round++) to[round] = Bytes16{};
+        } else {      // what lies outside is read from inside and dropped: no branch between the loads
+            const int channel = from + (threadIdx.x % (ACROSS / V)) * V, first = threadIdx.x / (ACROSS / V), most = stop - t0 - 1;
+            const T* const row0 = src - channel - first * stride;
+            if (FULL || vectors) {
 #pragma unroll
-                        for (int c = 0; c < V; c++) if (channel + c < width) to[round][c] = from[c];
-                    }
+                for (int round = 0; round < N; round++) {
+                    const int step = first + round * STEPS;
+                    to[round] = *reinterpret_cast<const Bytes16*>(row0 + min(step, most) * stride + (FULL ? channel : min(channel, width - V)));
+                    if (step > most || (!FULL && channel >= width)) to[round] = Bytes16{};
+                }
+            } else {
+#pragma unroll
+                for (int round = 0; round < N; round++) {
+                    const int step = first + round * STEPS;
+                    const T* const row = row0 + min(step, most) * stride;
+#pragma unroll
+                    for (int c = 0; c < V; c++) to[round][c] = row[min(channel + c, width - 1)];
+#pragma unroll
+                    for (int c = 0; c < V; c++) if (step > most || channel + c >= width) to[round][c] = (T)0.0f;
                 }
             }
         }
     };
     auto fetch_chunk = [&](int t0, int stop) {
         stop = min(stop, length);
-        if constexpr (!STATE) fetch(a.q, a.key, t0, stop, next_q);
-        fetch(a.k, a.key, t0, stop, next_k);
-        fetch(a.v, a.value, t0, stop, next_v);
-        if constexpr (SLOPE && !STATE) fetch(a.with, a.value, t0, stop, next_with);
+        if constexpr (!STATE) fetch(lane_q, a.q.step, a.q.vectors, 0, a.key, t0, stop, next_q, whole);
+        fetch(lane_k, a.k.step, a.k.vectors, 0, a.key, t0, stop, next_k, whole);
+        fetch(lane_v, a.v.step, a.v.vectors, part0, a.value, t0, stop, next_v, columns);
+        if constexpr (SLOPE && !STATE) fetch(lane_with, a.with.step, a.with.vectors, part0, a.value, t0, stop, next_with, columns);
         next_reset = a.reset && t0 + lane < stop ? a.reset[(size_t)(t0 + lane) * a.batch + b] : (uint8_t)0;
     };
-    auto put = [&](int base, const Bytes16 (&from)[ROUNDS]) {
+    auto put = [&](int base, const auto& from, auto across) {
+        constexpr int ACROSS = decltype(across)::value, N = CHUNK * ACROSS / (V * L::THREADS), STEPS = L::THREADS * V / ACROSS;
+        const int channel = (threadIdx.x % (ACROSS / V)) * V, first = threadIdx.x / (ACROSS / V);
 #pragma unroll
-        for (int round = 0; round < ROUNDS; round++) *reinterpret_cast<Bytes16*>(lds + base + (first + round * ROUND_STEPS) * L::ROW + channel) = from[round];
+        for (int round = 0; round < N; round++) *reinterpret_cast<Bytes16*>(lds + base + (first + round * STEPS) * (ACROSS + L::PAD) + channel) = from[round];
     };
     // operands: eight summands 32 block + 8 quarter ... of a row; of a row in the order of the accumulators; of column 16 tile + l over the steps
     auto row_operand = [&](int base, int stride, int row, int block) { return *reinterpret_cast<const Vector*>(lds + base + row * stride + 32 * block + 8 * quarter); };
@@ -175,17 +201,17 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
         const Quad x = *reinterpret_cast<const Quad*>(lds + base + row * L::ROW + 32 * block + 4 * quarter), y = *reinterpret_cast<const Quad*>(lds + base + row * L::ROW + 32 * block + 16 + 4 * quarter);
         return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
     };
-    auto column_operand = [&](int base, int tile, int block) {
+    auto column_operand = [&](int base, int stride, int tile, int block) {
         if constexpr (sizeof(T) == 2) {      // the transposing load: of sixteen lanes, lane p names four channels 4 (p % 4) ... of step p / 4, and lane l receives channel l of the four steps
             typedef short Raw __attribute__((ext_vector_type(4)));
             typedef __attribute__((address_space(3))) Raw* Address;
-            T* const from = lds + base + (32 * block + 8 * quarter + l / 4) * L::ROW + 16 * tile + 4 * (l % 4);
-            const Raw x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Address)from), y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Address)(from + 4 * L::ROW));
+            T* const from = lds + base + (32 * block + 8 * quarter + l / 4) * stride + 16 * tile + 4 * (l % 4);
+            const Raw x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Address)from), y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Address)(from + 4 * stride));
             return __builtin_bit_cast(Vector, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
         } else {
             Vector x;
 #pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = lds[base + (32 * block + 8 * quarter + e) * L::ROW + 16 * tile + l];
+            for (int e = 0; e < 8; e++) x[e] = lds[base + (32 * block + 8 * quarter + e) * stride + 16 * tile + l];
             return x;
         }
     };
@@ -197,17 +223,13 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
             lds[L::P + plane * CHUNK * L::SCORES + (32 * which + O0 + row) * L::SCORES + 32 * which + S0 + col] = (T)0.0f;
         }
     }
-    // weights of the scores of a tile: on the diagonal, and beside it (there a tile k further on has near * a^(16 (k - 1)))
-    float diagonal[4], near[4];
-#pragma unroll
-    for (int r = 0; r < 4; r++) {
-        const int lag = REVERSE ? 4 * quarter + r - l : l - 4 * quarter - r;
-        diagonal[r] = lag >= 0 ? power(log2_decay, lag) * a.score_scale : 0.0f;
-        near[r] = power(log2_decay, 16 + lag) * a.score_scale;
+    if (!STATE && wave == 0) {
+        if (lane < 16) score_weights[lane - 16] = 0.0f;
+        score_weights[lane] = power(log2_decay, lane) * a.score_scale;
     }
+    O* const lane_out = STATE ? nullptr : at<O>(a.out, 0, b, h) + l * a.out.step + column0 + 4 * quarter;
     float total = 0.0f;                                 // SLOPE
-    float read_weight[4], added_weight[2][8];           // of the state before the chunk in its steps' outputs, and of the steps in the state after it ...
-    int weights_n = -1; uint64_t weights_resets = 0;    // ... for so many steps and these resets
+    int weights_n = -1; uint64_t weights_resets = 0;    // the steps and the resets that the weights in LDS are for
     int counted = 0; bool forgotten = false;            // STATE
     int t0 = REVERSE ? max(begin, end - CHUNK) : begin, stop = REVERSE ? end : min(begin + CHUNK, end);
     fetch_chunk(t0, stop);
@@ -219,7 +241,11 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
 #pragma unroll
             for (int round = 0; round < ROUNDS; round++)
 #pragma unroll
-                for (int c = 0; c < V; c++) { zero = fmaf((float)next_k[round][c], 0.0f, zero); zero = fmaf((float)next_v[round][c], 0.0f, zero); }
+                for (int c = 0; c < V; c++) zero = fmaf((float)next_k[round][c], 0.0f, zero);
+#pragma unroll
+            for (int round = 0; round < COLUMN_ROUNDS; round++)
+#pragma unroll
+                for (int c = 0; c < V; c++) zero = fmaf((float)next_v[round][c], 0.0f, zero);
             const bool all = __all(zero == 0.0f);
             if (lane == 0) flags[wave] = all ? 0.0f : 1.0f;
         }
@@ -234,31 +260,25 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
             }
         }
         const int n = min(max(min(length, stop) - t0, 0), CHUNK);
-        put(L::K, next_k);
-        put(L::V, next_v);
-        if constexpr (!STATE) put(L::Q, next_q);
-        if constexpr (SLOPE && !STATE) put(L::W, next_with);
-        rlt_lds_barrier();
-        const bool done = REVERSE ? t0 <= begin : stop >= end;
-        const int next_t0 = REVERSE ? max(begin, t0 - CHUNK) : stop, next_stop = REVERSE ? t0 : min(stop + CHUNK, end);
-        if (!done) fetch_chunk(next_t0, next_stop);
-
         const int last_reset = resets ? 63 - __builtin_clzll(resets) : -1, first_reset = resets ? __builtin_ctzll(resets) : CHUNK;
         if (n != weights_n || resets != weights_resets) {
             weights_n = n; weights_resets = resets;
-#pragma unroll
-            for (int ot = 0; ot < 4; ot++) {
-                const int i = 16 * ot + l;
-                read_weight[ot] = i < n && (REVERSE ? last_reset <= i : first_reset > i) ? power(log2_decay, REVERSE ? n - 1 - i : i + 1) * a.read_scale : 0.0f;
+            if (wave == 0) {
+                const bool in = lane < n && (REVERSE ? lane < first_reset : lane >= last_reset), sees = lane < n && (REVERSE ? last_reset <= lane : first_reset > lane);
+                added_weights[lane] = in ? power(log2_decay, REVERSE ? lane : n - 1 - lane) * a.added_scale : 0.0f;
+                if constexpr (SLOPE) lagged_weights[lane] = added_weights[lane] * (float)(n - 1 - lane);
+                read_weights[lane] = sees ? power(log2_decay, REVERSE ? n - 1 - lane : lane + 1) * a.read_scale : 0.0f;
             }
-#pragma unroll
-            for (int block = 0; block < 2; block++)
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const int s = 32 * block + 8 * quarter + e;
-                    added_weight[block][e] = s < n && (REVERSE ? s < first_reset : s >= last_reset) ? power(log2_decay, REVERSE ? s : n - 1 - s) * a.added_scale : 0.0f;
-                }
         }
+        put(L::K, next_k, whole);
+        put(L::V, next_v, columns);
+        if constexpr (!STATE) put(L::Q, next_q, whole);
+        if constexpr (SLOPE && !STATE) put(L::W, next_with, columns);
+        rlt_lds_barrier();
+        const bool done = REVERSE ? t0 <= begin : stop >= end;
+        const int next_t0 = REVERSE ? max(begin, t0 - CHUNK) : stop, next_stop = REVERSE ? t0 : min(stop + CHUNK, end);
+        if constexpr (!SLOPE || STATE) { if (!done) fetch_chunk(next_t0, next_stop); }
+
         if constexpr (!STATE) {
             // scores, by tiles on and below (REVERSE: above) the diagonal: rows are the steps that are added, columns those that read
             for (int tile = wave; tile < 10; tile += L::WAVES) {
@@ -268,17 +288,12 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
                 for (int block = 0; block < KEY_BLOCKS; block++) x = multiply(row_operand(L::K, L::ROW, 16 * st + l, block), row_operand(L::Q, L::ROW, 16 * ot + l, block), x);
                 if constexpr (SLOPE) {
 #pragma unroll
-                    for (int block = 0; block < KEY_BLOCKS; block++) y = multiply(row_operand(L::V, L::ROW, 16 * st + l, block), row_operand(L::W, L::ROW, 16 * ot + l, block), y);
+                    for (int block = 0; block < L::COLUMNS / 32; block++) y = multiply(row_operand(L::V, L::COLUMN_ROW, 16 * st + l, block), row_operand(L::W, L::COLUMN_ROW, 16 * ot + l, block), y);
                 }
-                const int i = 16 * ot + l, apart = row - col;
-                if (apart == 0) {
+                const int i = 16 * ot + l;
+                const float* const weight = score_weights + (REVERSE ? 16 * (st - ot) + 4 * quarter - l : 16 * (ot - st) + l - 4 * quarter);
 #pragma unroll
-                    for (int r = 0; r < 4; r++) x[r] = diagonal[r] != 0.0f ? x[r] * diagonal[r] : 0.0f;
-                } else {
-                    const float far = power(log2_decay, 16 * (apart - 1));
-#pragma unroll
-                    for (int r = 0; r < 4; r++) x[r] *= near[r] * far;
-                }
+                for (int r = 0; r < 4; r++) { const float w = weight[REVERSE ? r : -r]; x[r] = w != 0.0f ? x[r] * w : 0.0f; }
                 if (resets) {
                     const uint64_t before = resets & ((2ull << i) - 1), after = i < 63 ? resets & ~((2ull << i) - 1) : 0;
                     const int low = REVERSE ? 0 : before ? 63 - __builtin_clzll(before) : 0, high = REVERSE && after ? __builtin_ctzll(after) - 1 : 63;      // steps of the episode of step i
@@ -314,42 +329,46 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
                 for (int tile = 0; tile < TILES; tile++) {
                     const Cut<T, STATE_CUTS> s(__builtin_shufflevector(state[tile][2 * block], state[tile][2 * block + 1], 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-                    for (int ot = 0; ot < 4; ot++)
+                    for (int p = 0; p < STATE_CUTS; p++)
 #pragma unroll
-                        for (int p = 0; p < STATE_CUTS; p++) out[tile][ot] = multiply(s.part[p], q[ot], out[tile][ot]);
+                        for (int ot = 0; ot < 4; ot++) out[tile][ot] = multiply(s.part[p], q[ot], out[tile][ot]);
                     if constexpr (SLOPE) {
                         const Cut<T, STATE_CUTS> d(__builtin_shufflevector(slope[tile][2 * block], slope[tile][2 * block + 1], 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-                        for (int ot = 0; ot < 4; ot++)
+                        for (int p = 0; p < STATE_CUTS; p++)
 #pragma unroll
-                            for (int p = 0; p < STATE_CUTS; p++) out_slope[tile][ot] = multiply(d.part[p], q[ot], out_slope[tile][ot]);
+                            for (int ot = 0; ot < 4; ot++) out_slope[tile][ot] = multiply(d.part[p], q[ot], out_slope[tile][ot]);
                     }
                 }
+                if constexpr (SLOPE) __builtin_amdgcn_sched_barrier(0);      // one block's operands in registers at a time
             }
 #pragma unroll
-            for (int tile = 0; tile < TILES; tile++)
+            for (int ot = 0; ot < 4; ot++) {
+                const int i = 16 * ot + l;
+                const float weight = read_weights[i];
 #pragma unroll
-                for (int ot = 0; ot < 4; ot++) {
-                    const int i = 16 * ot + l;
+                for (int tile = 0; tile < TILES; tile++) {
                     if constexpr (SLOPE) {
-                        const Quad with = *reinterpret_cast<const Quad*>(lds + L::W + i * L::ROW + column0 + 16 * tile + 4 * quarter);
+                        const Quad with = *reinterpret_cast<const Quad*>(lds + L::W + i * L::COLUMN_ROW + inner0 + 16 * tile + 4 * quarter);
                         float d = 0.0f;
 #pragma unroll
                         for (int r = 0; r < 4; r++) d = fmaf((float)with[r], fmaf((float)(i + 1), out[tile][ot][r], out_slope[tile][ot][r]), d);
-                        if (read_weight[ot] != 0.0f) total = fmaf(read_weight[ot], d, total);
+                        if (weight != 0.0f) total = fmaf(weight, d, total);
                     }
                     if (resets) {      // a state of another episode need not be finite
 #pragma unroll
-                        for (int r = 0; r < 4; r++) out[tile][ot][r] = read_weight[ot] != 0.0f ? out[tile][ot][r] * read_weight[ot] : 0.0f;
-                    } else out[tile][ot] *= read_weight[ot];
+                        for (int r = 0; r < 4; r++) out[tile][ot][r] = weight != 0.0f ? out[tile][ot][r] * weight : 0.0f;
+                    } else out[tile][ot] *= weight;
                 }
+            }
             rlt_lds_barrier();
+            if constexpr (SLOPE) { if (!done) fetch_chunk(next_t0, next_stop); }      // only here: the products with two states before leave no registers for it
             // what the chunk's own steps give
 #pragma unroll
             for (int block = 0; block < 2; block++) {
                 Vector values[TILES];
 #pragma unroll
-                for (int tile = 0; tile < TILES; tile++) values[tile] = column_operand(L::V, TILES * wave + tile, block);
+                for (int tile = 0; tile < TILES; tile++) values[tile] = column_operand(L::V, L::COLUMN_ROW, TILES * wave + tile, block);
 #pragma unroll
                 for (int ot = 0; ot < 4; ot++)
                     if (REVERSE ? 32 * block + 31 >= 16 * ot : 32 * block <= 16 * ot + 15) {
@@ -362,7 +381,7 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
                     }
             }
             typedef typename Operand<O>::Quad OutQuad;
-            O* const to = at<O>(a.out, t0, b, h) + (int64_t)l * a.out.step + column0 + 4 * quarter;
+            O* const to = lane_out + t0 * a.out.step;
 #pragma unroll
             for (int ot = 0; ot < 4; ot++) {
                 const int i = 16 * ot + l;
@@ -371,7 +390,7 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
                     for (int tile = 0; tile < TILES; tile++) {
                         const int c0 = column0 + 16 * tile + 4 * quarter;
                         rlt_f32x4 x = out[tile][ot];
-                        if (i >= n) x = rlt_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                        if (n < CHUNK && i >= n) x = rlt_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
                         O* const here = to + (int64_t)(16 * ot) * a.out.step + 16 * tile;
                         if (FULL) *reinterpret_cast<OutQuad*>(here) = __builtin_convertvector(x, OutQuad);
                         else if (a.out.vectors) { if (c0 < a.value) *reinterpret_cast<OutQuad*>(here) = __builtin_convertvector(x, OutQuad); }
@@ -401,34 +420,39 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
                 }
 #pragma unroll
             for (int block = 0; block < 2; block++) {
-                rlt_f32x8 weight;
+                const rlt_f32x8 weight = *reinterpret_cast<const rlt_f32x8*>(added_weights + 32 * block + 8 * quarter);
+                Vector key[SLOPE ? 1 : KEY_TILES];
+                if constexpr (!SLOPE) {
 #pragma unroll
-                for (int e = 0; e < 8; e++) weight[e] = added_weight[block][e];
-                Vector key[KEY_TILES];
-#pragma unroll
-                for (int k = 0; k < KEY_TILES; k++) key[k] = column_operand(L::K, k, block);
+                    for (int k = 0; k < KEY_TILES; k++) key[k] = column_operand(L::K, L::ROW, k, block);
+                }
 #pragma unroll
                 for (int tile = 0; tile < TILES; tile++) {
-                    const Vector v = column_operand(L::V, TILES * wave + tile, block);
+                    const Vector v = column_operand(L::V, L::COLUMN_ROW, TILES * wave + tile, block);
                     const rlt_f32x8 weighted = __builtin_convertvector(v, rlt_f32x8) * weight;
                     const Cut<T, ADDED_CUTS> x(weighted);
-#pragma unroll
-                    for (int p = 0; p < ADDED_CUTS; p++) {
-                        if (!STATE && !SLOPE && p == 2 && !a.exit) break;      // a state that only goes into outputs of this type does with two parts
-#pragma unroll
-                        for (int k = 0; k < KEY_TILES; k++) state[tile][k] = multiply(key[k], x.part[p], state[tile][k]);
-                    }
                     if constexpr (SLOPE) {
-                        rlt_f32x8 lagged;
-#pragma unroll
-                        for (int e = 0; e < 8; e++) lagged[e] = weighted[e] * (float)(n - 1 - (32 * block + 8 * quarter + e));
+                        const rlt_f32x8 lagged = __builtin_convertvector(v, rlt_f32x8) * *reinterpret_cast<const rlt_f32x8*>(lagged_weights + 32 * block + 8 * quarter);
                         const Cut<T, ADDED_CUTS> y(lagged);
 #pragma unroll
-                        for (int k = 0; k < KEY_TILES; k++)
+                        for (int k = 0; k < KEY_TILES; k++) {      // one key operand in registers at a time
+                            key[0] = column_operand(L::K, L::ROW, k, block);
 #pragma unroll
-                            for (int p = 0; p < ADDED_CUTS; p++) slope[tile][k] = multiply(key[k], y.part[p], slope[tile][k]);
+                            for (int p = 0; p < ADDED_CUTS; p++) {
+                                state[tile][k] = multiply(key[0], x.part[p], state[tile][k]);
+                                slope[tile][k] = multiply(key[0], y.part[p], slope[tile][k]);
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (int p = 0; p < ADDED_CUTS; p++) {
+                            if (!STATE && p == 2 && !a.exit) break;      // a state that only goes into outputs of this type does with two parts
+#pragma unroll
+                            for (int k = 0; k < KEY_TILES; k++) state[tile][k] = multiply(key[k], x.part[p], state[tile][k]);
+                        }
                     }
                 }
+                if constexpr (SLOPE) __builtin_amdgcn_sched_barrier(0);
             }
             if constexpr (REVERSE) {      // the power that all of them share: the cut operands keep their parts above the smallest numbers also where one step forgets nearly everything
                 const float once = power(log2_decay, 1);
@@ -450,7 +474,7 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
         float* const to = a.exit_slope + state_base;
         over_state([&](int tile, int k, int r, bool there, int i) { if (there) to[i] = slope[tile][k][r]; });
     }
-    if constexpr (STATE) { if (threadIdx.x == 0) a.factors[item] = make_float2(forgotten ? 0.0f : power(log2_decay, counted), (float)counted); }
+    if constexpr (STATE) { if (threadIdx.x == 0 && half == 0) a.factors[item] = make_float2(forgotten ? 0.0f : power(log2_decay, counted), (float)counted); }
     if constexpr (SLOPE && !STATE) {
         if (a.d_final && segment == a.segments - 1) {
             const float* const from = a.d_final + (size_t)pair * a.key * a.value;
@@ -463,33 +487,44 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
         if (threadIdx.x == 0) {
             float s = 0.0f;
             for (int w = 0; w < L::WAVES; w++) s += flags[w];
-            a.partial[item] = s;
+            a.partial[item * L::SPLIT + half] = s;
         }
     }
 }
 
-// States that the segments start from, out of what each of them adds: element by element along the segments (REVERSE: from the last). locals become the entries.
-__global__ __launch_bounds__(256) void scan_kernel(const float* __restrict__ initial, float* __restrict__ locals, float* __restrict__ slopes, const float2* __restrict__ factors, float* __restrict__ final, int elements,
-                                                   int segments, int reverse) {
+// States that the segments start from, out of what each of them adds: element by element along the segments (REVERSE: from the last). locals become the entries. The values of AHEAD segments are asked for at a time.
+template <bool SLOPES> __global__ __launch_bounds__(256) void scan_kernel(const float* __restrict__ initial, float* __restrict__ locals, float* __restrict__ slopes, const float2* __restrict__ factors,
+                                                                          float* __restrict__ final, int elements, int segments, int reverse) {
+    constexpr int AHEAD = 8;
     const int pair = blockIdx.y, e = blockIdx.x * 256 + threadIdx.x;
     if (e >= elements) return;
     float carry = initial ? initial[(size_t)pair * elements + e] : 0.0f, carry_slope = 0.0f;
-    for (int i = 0; i < segments; i++) {
-        const size_t p = (size_t)pair * segments + (reverse ? segments - 1 - i : i), at = p * elements + e;
-        const float2 f = factors[p];
-        const float local = locals[at];
-        if (slopes) {
-            const float local_slope = slopes[at];
-            slopes[at] = carry_slope;
-            carry_slope = f.x == 0.0f ? local_slope : fmaf(f.x, fmaf(f.y, carry, carry_slope), local_slope);
+    for (int i0 = 0; i0 < segments; i0 += AHEAD) {
+        float local[AHEAD], local_slope[AHEAD];
+#pragma unroll
+        for (int j = 0; j < AHEAD; j++) {
+            const int i = min(i0 + j, segments - 1);
+            const size_t at = ((size_t)pair * segments + (reverse ? segments - 1 - i : i)) * elements + e;
+            local[j] = locals[at];
+            if (SLOPES) local_slope[j] = slopes[at];
         }
-        locals[at] = carry;
-        carry = f.x == 0.0f ? local : fmaf(f.x, carry, local);
+#pragma unroll
+        for (int j = 0; j < AHEAD; j++)
+            if (i0 + j < segments) {
+                const size_t p = (size_t)pair * segments + (reverse ? segments - 1 - i0 - j : i0 + j), at = p * elements + e;
+                const float2 f = factors[p];
+                if (SLOPES) {
+                    slopes[at] = carry_slope;
+                    carry_slope = f.x == 0.0f ? local_slope[j] : fmaf(f.x, fmaf(f.y, carry, carry_slope), local_slope[j]);
+                }
+                locals[at] = carry;
+                carry = f.x == 0.0f ? local[j] : fmaf(f.x, carry, local[j]);
+            }
     }
     if (final) final[(size_t)pair * elements + e] = carry;
 }
 
-// sums over the rows of a batch and their segments, in a fixed order
+// sums over the rows of a batch and their segments (and the workgroups that share one), in a fixed order
 __global__ __launch_bounds__(64) void decay_sum_kernel(const float* __restrict__ partial, int batch, int heads, int segments, float* __restrict__ out, int accumulate) {
     const int h = blockIdx.x;
     float s = 0.0f;
@@ -568,7 +603,7 @@ Scratch scratch_of(const rlt_linear_attention* p, int steps, bool backward) {
         s.factors = take(2 * pairs * g.count);
     }
     if (backward) {
-        s.partial = take(pairs * g.count);
+        s.partial = take(2 * pairs * g.count);      // up to two workgroups share a head
         if (p->heads != p->kv_heads) s.shared = take(padded((size_t)steps * pairs * p->value_dim) + (size_t)steps * pairs * p->key_dim);
     }
     s.total = at;
@@ -580,7 +615,7 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
     const auto kernel = walk_kernel<T, O, D, REVERSE, SLOPE, STATE, FULL>;
     const unsigned items = (unsigned)a.batch * a.heads * a.segments;
     RLT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)L::BYTES));
-    hipLaunchKernelGGL(kernel, dim3(second ? (items + 7) / 8 * 16 : items), dim3(L::THREADS), L::BYTES, device->stream, Walks{a, second ? *second : a, (int)items, second != nullptr});
+    hipLaunchKernelGGL(kernel, dim3(second ? (items + 7) / 8 * 16 : items * L::SPLIT), dim3(L::THREADS), L::BYTES, device->stream, Walks{a, second ? *second : a, (int)items, second != nullptr});
     return rlt_launch_status(device);
 }
 // FULL: heads of exactly D channels, all of whose tensors may be read and written in vectors
@@ -610,7 +645,7 @@ template <typename T, bool REVERSE, bool SLOPE> int segment_states(rlt_rocm_devi
     int rc = walk<T, T, REVERSE, SLOPE, true>(device, s);
     if (rc) return rc;
     const int elements = a.key * a.value, pairs = a.batch * a.heads;
-    hipLaunchKernelGGL(scan_kernel, dim3((elements + 255) / 256, pairs), dim3(256), 0, device->stream, initial, states, SLOPE ? slopes : nullptr, factors, final, elements, a.segments, (int)REVERSE);
+    hipLaunchKernelGGL(scan_kernel<SLOPE>, dim3((elements + 255) / 256, pairs), dim3(256), 0, device->stream, initial, states, SLOPE ? slopes : nullptr, factors, final, elements, a.segments, (int)REVERSE);
     return rlt_launch_status(device);
 }
 
@@ -649,7 +684,7 @@ template <typename T> int backward(rlt_rocm_device* device, const rlt_linear_att
     a.entry = cut ? states : initial_state; a.entry_slope = cut ? slopes : nullptr; a.d_final = d_final_state; a.partial = workspace + s.partial;
     rc = d_log_decay ? walk<T, T, false, true, false>(device, a) : walk<T, T, false, false, false>(device, a);
     if (rc) return rc;
-    if (d_log_decay) hipLaunchKernelGGL(decay_sum_kernel, dim3(p->heads), dim3(64), 0, device->stream, a.partial, p->batch, p->heads, a.segments, d_log_decay, accumulate);
+    if (d_log_decay) hipLaunchKernelGGL(decay_sum_kernel, dim3(p->heads), dim3(64), 0, device->stream, a.partial, p->batch, p->heads, a.segments * (p->key_dim > 64 || p->value_dim > 64 ? 2 : 1), d_log_decay, accumulate);
     // the state's gradient, from the last step to the first; d_v reads it, d_k reads it across
     Walk r = walk_of(p, reset, lengths, steps);
     r.k = Q; r.v = G; r.read_scale = 1.0f; r.added_scale = p->scale;
