@@ -70,11 +70,14 @@ template <typename T, int D, bool SLOPE, bool STATE> struct Layout {
     static constexpr int TILES = D == 128 && sizeof(T) == 2 && !SLOPE ? 2 : 1, WAVES = COLUMNS / (16 * TILES), THREADS = 64 * WAVES;
     static constexpr int PAD = 16 / sizeof(T), ROW = D + PAD, COLUMN_ROW = COLUMNS + PAD, SCORES = CHUNK + PAD;      // rows start 4 (of 64) banks after each other: sixteen of them side by side in 16 bytes each meet no bank twice
     static constexpr int PLANES = sizeof(T) == 2 ? 2 : 1;
-    static constexpr int K = 0, V = K + CHUNK * ROW, Q = V + CHUNK * COLUMN_ROW, W = Q + (STATE ? 0 : CHUNK * ROW), P = W + (SLOPE && !STATE ? CHUNK * COLUMN_ROW : 0);
-    static constexpr int FLAGS = P + (STATE ? 0 : PLANES * CHUNK * SCORES);
+    // keys, values, what the slope is multiplied with, the queries, the scores: in the queries' place (for a barrier more) where that leaves room for another workgroup, which 128 channels of two bytes have no registers for
+    static constexpr bool OVER = !(D == 128 && sizeof(T) == 2 && !SLOPE);
+    static constexpr int K = 0, V = K + CHUNK * ROW, W = V + CHUNK * COLUMN_ROW, Q = W + (SLOPE && !STATE ? CHUNK * COLUMN_ROW : 0), P = OVER ? Q : Q + CHUNK * ROW;
+    static constexpr int FLAGS = STATE ? Q : OVER && ROW > PLANES * SCORES ? Q + CHUNK * ROW : P + CHUNK * PLANES * SCORES;
+    static constexpr int SCORE_TILES = (10 + WAVES - 1) / WAVES;      // of a wavefront
     static constexpr size_t BYTES = FLAGS * sizeof(T) + (4 * CHUNK + 16 + WAVES) * sizeof(float);
     // wavefronts that the registers of a SIMD are shared by: as many as LDS has room for workgroups
-    static constexpr int FIT = (int)(163840 / BYTES) * WAVES / 4, MOST = D == 128 ? 2 : 3, RESIDENT = FIT < 1 ? 1 : FIT > MOST ? MOST : FIT;
+    static constexpr int FIT = (int)(163840 / BYTES) * WAVES / 4, MOST = D == 128 || (SLOPE && !STATE) ? 2 : 3, RESIDENT = FIT < 1 ? 1 : FIT > MOST ? MOST : FIT;
 };
 
 // Chunks of up to 64 steps. With i, s the steps of a chunk (n of them within the row's length), S the state before it and a the decay:
@@ -100,7 +103,8 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
     if (item >= walks.items) return;
     const Walk& a = other ? walks.second : walks.first;
     const int pair = item / a.segments, segment = item % a.segments, b = pair / a.heads, h = pair % a.heads;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane & 15, quarter = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int l = lane & 15, quarter = lane >> 4;
     const int length = a.lengths ? min(max(a.lengths[b], 0), a.steps) : a.steps;
     const float log2_decay = a.log_decay[h] * 1.44269504088896341f;
     const int begin = segment * a.segment_steps, end = min(begin + a.segment_steps, a.steps);
@@ -142,37 +146,39 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
     uint8_t next_reset = 0;
     constexpr std::integral_constant<int, D> whole{};
     constexpr std::integral_constant<int, L::COLUMNS> columns{};
-    // where a thread's vectors of step 0 lie, once for the walk
-    auto lane_of = [&](const Part& p, int from, auto across) {
+    // Whole chunks of whole heads: a uniform address and a thread's offset in bytes (32 bits: the strides of FULL tensors leave room).
+    auto offset_of = [&](const Part& p, int from, auto across) {
         constexpr int ACROSS = decltype(across)::value;
-        return at<T>(p, 0, b, h) + (int64_t)(threadIdx.x / (ACROSS / V)) * p.step + from + (threadIdx.x % (ACROSS / V)) * V;
+        unsigned thread = threadIdx.x;
+        if constexpr (SLOPE && !STATE) asm volatile("" : "+v"(thread));      // formed anew for each chunk
+        return (thread / (ACROSS / V) * (unsigned)p.step + from + thread % (ACROSS / V) * V) * (unsigned)sizeof(T);
     };
-    const T* const lane_k = lane_of(a.k, 0, whole); const T* const lane_v = lane_of(a.v, part0, columns);
-    const T* const lane_q = STATE ? nullptr : lane_of(a.q, 0, whole); const T* const lane_with = SLOPE && !STATE ? lane_of(a.with, part0, columns) : nullptr;
-    auto fetch = [&](const T* lane_of_step_0, int64_t stride, int vectors, int from, int width, int t0, int stop, auto& to, auto across) {
+    auto fetch = [&](const Part& p, int from, int width, int t0, int stop, auto& to, auto across) {
         constexpr int ACROSS = decltype(across)::value, N = CHUNK * ACROSS / (V * L::THREADS), STEPS = L::THREADS * V / ACROSS;
-        const T* const src = lane_of_step_0 + t0 * stride;
+        const T* const row0 = at<T>(p, t0, b, h);
         if (FULL && stop - t0 == CHUNK) {
+            const unsigned offset = offset_of(p, from, across);
 #pragma unroll
-            for (int round = 0; round < N; round++) to[round] = *reinterpret_cast<const Bytes16*>(src + (round * STEPS) * stride);
+            for (int round = 0; round < N; round++) to[round] = *reinterpret_cast<const Bytes16*>(reinterpret_cast<const char*>(row0 + (round * STEPS) * p.step) + offset);
         } else if (stop <= t0) {
 #pragma unroll
             for (int round = 0; round < N; round++) to[round] = Bytes16{};
         } else {      // what lies outside is read from inside and dropped: no branch between the loads
-            const int channel = from + (threadIdx.x % (ACROSS / V)) * V, first = threadIdx.x / (ACROSS / V), most = stop - t0 - 1;
-            const T* const row0 = src - channel - first * stride;
-            if (FULL || vectors) {
+            int thread = threadIdx.x;
+            asm volatile("" : "+v"(thread));
+            const int channel = from + (thread % (ACROSS / V)) * V, first = thread / (ACROSS / V), most = stop - t0 - 1;
+            if (FULL || p.vectors) {
 #pragma unroll
                 for (int round = 0; round < N; round++) {
                     const int step = first + round * STEPS;
-                    to[round] = *reinterpret_cast<const Bytes16*>(row0 + min(step, most) * stride + (FULL ? channel : min(channel, width - V)));
+                    to[round] = *reinterpret_cast<const Bytes16*>(row0 + min(step, most) * p.step + (FULL ? channel : min(channel, width - V)));
                     if (step > most || (!FULL && channel >= width)) to[round] = Bytes16{};
                 }
             } else {
 #pragma unroll
                 for (int round = 0; round < N; round++) {
                     const int step = first + round * STEPS;
-                    const T* const row = row0 + min(step, most) * stride;
+                    const T* const row = row0 + min(step, most) * p.step;
 #pragma unroll
                     for (int c = 0; c < V; c++) to[round][c] = row[min(channel + c, width - 1)];
 #pragma unroll
@@ -183,10 +189,10 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
     };
     auto fetch_chunk = [&](int t0, int stop) {
         stop = min(stop, length);
-        if constexpr (!STATE) fetch(lane_q, a.q.step, a.q.vectors, 0, a.key, t0, stop, next_q, whole);
-        fetch(lane_k, a.k.step, a.k.vectors, 0, a.key, t0, stop, next_k, whole);
-        fetch(lane_v, a.v.step, a.v.vectors, part0, a.value, t0, stop, next_v, columns);
-        if constexpr (SLOPE && !STATE) fetch(lane_with, a.with.step, a.with.vectors, part0, a.value, t0, stop, next_with, columns);
+        if constexpr (!STATE) fetch(a.q, 0, a.key, t0, stop, next_q, whole);
+        fetch(a.k, 0, a.key, t0, stop, next_k, whole);
+        fetch(a.v, part0, a.value, t0, stop, next_v, columns);
+        if constexpr (SLOPE && !STATE) fetch(a.with, part0, a.value, t0, stop, next_with, columns);
         next_reset = a.reset && t0 + lane < stop ? a.reset[(size_t)(t0 + lane) * a.batch + b] : (uint8_t)0;
     };
     auto put = [&](int base, const auto& from, auto across) {
@@ -216,13 +222,6 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
         }
     };
 
-    if constexpr (!STATE) {      // score tiles that lie on the wrong side of the diagonal within a block of 32: zero for good
-        constexpr int O0 = REVERSE ? 16 : 0, S0 = REVERSE ? 0 : 16;
-        for (int i = threadIdx.x; i < L::PLANES * 2 * 16 * 16; i += L::THREADS) {
-            const int plane = i / 512, which = (i / 256) % 2, row = (i / 16) % 16, col = i % 16;
-            lds[L::P + plane * CHUNK * L::SCORES + (32 * which + O0 + row) * L::SCORES + 32 * which + S0 + col] = (T)0.0f;
-        }
-    }
     if (!STATE && wave == 0) {
         if (lane < 16) score_weights[lane - 16] = 0.0f;
         score_weights[lane] = power(log2_decay, lane) * a.score_scale;
@@ -234,6 +233,10 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
     int t0 = REVERSE ? max(begin, end - CHUNK) : begin, stop = REVERSE ? end : min(begin + CHUNK, end);
     fetch_chunk(t0, stop);
     while (true) {
+        if constexpr (SLOPE && !STATE) {      // two states leave no registers for addresses that hold from chunk to chunk: they are formed anew
+            asm volatile("" : "+v"(l));
+            asm volatile("" : "+v"(quarter));
+        }
         uint64_t resets = __ballot(next_reset != 0);
         if (resets & ~1ull) {
             // A step's weight of zero keeps other episodes out of sums of products as long as their values are finite. Where some are not, the chunk ends at its first reset (REVERSE: begins at its last).
@@ -281,8 +284,13 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
 
         if constexpr (!STATE) {
             // scores, by tiles on and below (REVERSE: above) the diagonal: rows are the steps that are added, columns those that read
-            for (int tile = wave; tile < 10; tile += L::WAVES) {
-                const int row = tile < 1 ? 0 : tile < 3 ? 1 : tile < 6 ? 2 : 3, col = tile - row * (row + 1) / 2, ot = REVERSE ? 3 - row : row, st = REVERSE ? 3 - col : col;
+            rlt_f32x4 score[L::SCORE_TILES];
+            int first_tile = wave;
+            asm volatile("" : "+s"(first_tile));      // the tiles' addresses are formed here, not kept in registers from chunk to chunk
+#pragma unroll
+            for (int j = 0; j < L::SCORE_TILES; j++) {
+                const int tile = first_tile + j * L::WAVES, row = tile < 1 ? 0 : tile < 3 ? 1 : tile < 6 ? 2 : 3, col = tile - row * (row + 1) / 2, ot = REVERSE ? 3 - row : row, st = REVERSE ? 3 - col : col;
+                if (tile >= 10) break;
                 rlt_f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f}, y = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int block = 0; block < KEY_BLOCKS; block++) x = multiply(row_operand(L::K, L::ROW, 16 * st + l, block), row_operand(L::Q, L::ROW, 16 * ot + l, block), x);
@@ -304,12 +312,8 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
 #pragma unroll
                     for (int r = 0; r < 4; r++) { const int s = 16 * st + 4 * quarter + r; total += x[r] == 0.0f ? 0.0f : (float)(REVERSE ? s - i : i - s) * x[r] * y[r]; }
                 }
-#pragma unroll
-                for (int plane = 0; plane < L::PLANES; plane++) {
-                    const Quad part = __builtin_convertvector(x, Quad);
-                    *reinterpret_cast<Quad*>(lds + L::P + plane * CHUNK * L::SCORES + i * L::SCORES + 16 * st + 4 * quarter) = part;
-                    if (plane + 1 < L::PLANES) x -= __builtin_convertvector(part, rlt_f32x4);
-                }
+                score[j] = x;
+                __builtin_amdgcn_sched_barrier(0);      // one tile in registers at a time
             }
             // what the state before the chunk gives: columns of the result are the steps, rows the value columns
             rlt_f32x4 out[TILES][4], out_slope[SLOPE ? TILES : 1][SLOPE ? 4 : 1];
@@ -361,6 +365,21 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
                     } else out[tile][ot] *= weight;
                 }
             }
+            if constexpr (L::OVER) rlt_lds_barrier();      // the queries have been read
+#pragma unroll
+            for (int j = 0; j < L::SCORE_TILES; j++) {
+                const int tile = first_tile + j * L::WAVES, row = tile < 1 ? 0 : tile < 3 ? 1 : tile < 6 ? 2 : 3, col = tile - row * (row + 1) / 2, ot = REVERSE ? 3 - row : row, st = REVERSE ? 3 - col : col;
+                if (tile >= 10) break;
+#pragma unroll
+                for (int plane = 0; plane < L::PLANES; plane++) {
+                    const Quad part = __builtin_convertvector(score[j], Quad);
+                    *reinterpret_cast<Quad*>(lds + L::P + plane * CHUNK * L::SCORES + (16 * ot + l) * L::SCORES + 16 * st + 4 * quarter) = part;
+                    if (plane + 1 < L::PLANES) score[j] -= __builtin_convertvector(part, rlt_f32x4);
+                }
+            }
+            // the tiles on the wrong side of the diagonal that are multiplied all the same, as halves of blocks of 32
+            for (int which = wave; which < 2 * L::PLANES; which += L::WAVES)
+                *reinterpret_cast<Quad*>(lds + L::P + which / 2 * CHUNK * L::SCORES + (32 * (which % 2) + (REVERSE ? 16 : 0) + l) * L::SCORES + 32 * (which % 2) + (REVERSE ? 0 : 16) + 4 * quarter) = Quad{};
             rlt_lds_barrier();
             if constexpr (SLOPE) { if (!done) fetch_chunk(next_t0, next_stop); }      // only here: the products with two states before leave no registers for it
             // what the chunk's own steps give
@@ -579,14 +598,27 @@ bool supported(const rlt_linear_attention* p) { return p->key_dim <= MAX_WIDTH &
 bool given(const rlt_head_view* v) { return v && v->data; }
 size_t padded(size_t n) { return (n + 63) / 64 * 64; }
 
-// The steps of a row and head are cut into segments where rows and heads alone leave compute units without work: their states then cost a pass over keys and values ahead of the walk.
+// The steps of a row and head are cut into segments where rows and heads alone leave compute units without work: their states then cost a pass over keys and values ahead of the walk, a quarter of a walk's time, and
+// launches worth about four chunks. Measured (us, by segments): 8 rows x 4 heads of 64, 1,024 steps, fp32: 103 with 1, 44 with 4, 30 with 8 and 16; 8 heads of 64, 2,048 steps, bf16: 104 with 1, 21 with 16 and 32;
+// 4 x 16 heads of 128, 8,192 steps: 498 with 2, 328 with 4, 297 with 8, 331 with 16; forward and backward of 16 x 8 heads of 128, 256 steps: 110 with 1, 188 with 2; of 37 x 6 heads of 41, 333 steps: 235 with 1, 252 to 280 with 2 to 6.
 struct Segments { int count, steps; };
 Segments segments_of(const rlt_linear_attention* p, int steps) {
     const int chunks = (steps + CHUNK - 1) / CHUNK;
-    const int64_t pairs = (int64_t)p->batch * p->heads;
-    int64_t count = pairs >= 512 ? 1 : (512 + pairs - 1) / pairs;
-    if (count > (chunks + 3) / 4) count = (chunks + 3) / 4;      // at least four chunks each
-    const int per = (int)((chunks + count - 1) / count);
+    const double pairs = (double)p->batch * p->heads;
+    int best = 1;
+    double least = chunks;      // with one segment, in chunks' walks, while every row and head has a place on the chip
+    if (pairs > 512) least *= pairs / 512;
+    auto try_count = [&](int count) {
+        if (count < 2 || count > chunks) return;
+        const int per = (chunks + count - 1) / count;
+        const double filled = pairs * ((chunks + per - 1) / per) / 512, cost = 1.25 * per * (filled > 1 ? filled : 1) + 4;
+        if (cost < least) { least = cost; best = count; }
+    };
+    if (pairs < 512) {
+        try_count((int)(512 / pairs));
+        for (int count = 2; count <= 512 / pairs; count *= 2) try_count(count);
+    }
+    const int per = (chunks + best - 1) / best;
     return {(chunks + per - 1) / per, per * CHUNK};
 }
 // scratch memory, in floats: [states of the segments][their slopes][factors][partial sums][gradients of the heads that share keys and values]
@@ -621,6 +653,8 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
 // FULL: heads of exactly D channels, all of whose tensors may be read and written in vectors
 template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE> int walk_width(rlt_rocm_device* device, const Walk& a, const Walk* second) {
     auto full = [&](const Walk& w) {
+        auto near = [](const Part& p) { return p.step > -(1 << 22) && p.step < 1 << 22; };      // a chunk's offsets in bytes fit 32 bits
+        if (!near(w.k) || !near(w.v) || (!STATE && !near(w.q)) || (SLOPE && !STATE && !near(w.with))) return false;
         return w.key == D && w.value == D && w.k.vectors && w.v.vectors && (STATE || (w.q.vectors && w.out.vectors)) && (!SLOPE || STATE || w.with.vectors);
     };
     return full(a) && (!second || full(*second)) ? launch_walk<T, O, D, REVERSE, SLOPE, STATE, true>(device, a, second) : launch_walk<T, O, D, REVERSE, SLOPE, STATE, false>(device, a, second);
