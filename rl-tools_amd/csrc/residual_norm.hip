@@ -1,9 +1,10 @@
 // The norm after a block, its gate and residual scale, and the norm before the next block: one pass over the rows forward, one backward.
 #include "typed.h"
+#include <type_traits>
 
 namespace {
 
-constexpr int MAX_DIM = 8192;
+constexpr int MAX_DIM = 8192, HELD_DIM = 4096;
 enum { BRANCH_W = 0, BRANCH_B, OUTPUT_W, OUTPUT_B, SCALE, SUMS };      // column sums of the backward pass
 
 struct NormForward {
@@ -20,6 +21,12 @@ struct NormBackward {
 
 // THREADS share a row: a part of a wavefront, a wavefront (several rows to a workgroup of 256 then, whose wavefronts do not wait for each other) or a workgroup.
 template <int THREADS> constexpr int WORKGROUP = THREADS <= 64 ? 256 : THREADS;
+
+// a thread's place in its row, and its row's in the workgroup (the same for all of a wavefront where a row has one or more: addresses of rows stay scalar)
+template <int THREADS> __device__ __forceinline__ int thread_of() { return WORKGROUP<THREADS> == THREADS ? (int)threadIdx.x : (int)(threadIdx.x % THREADS); }
+template <int THREADS> __device__ __forceinline__ int row_of() {
+    return WORKGROUP<THREADS> == THREADS ? 0 : THREADS == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / 64) : (int)(threadIdx.x / THREADS);
+}
 
 // Sums over the threads that share a row, every one of which receives them. Consecutive calls take turns with two halves of `lds`: a wavefront that writes one has passed the barrier
 // behind which everybody had read it.
@@ -53,7 +60,7 @@ template <int THREADS, int N> __device__ __forceinline__ void row_sums(float (&v
 template <int V, int K, int THREADS, typename T> __device__ __forceinline__ void load_row(const T* src, int dim, float (&v)[V * K]) {
 #pragma unroll
     for (int k = 0; k < K; k++) {
-        const int c = (k * THREADS + (int)(threadIdx.x % THREADS)) * V;
+        const int c = (k * THREADS + thread_of<THREADS>()) * V;
         if (c < dim) rlt_load<V>(src + c, v + k * V);
         else {
 #pragma unroll
@@ -61,31 +68,62 @@ template <int V, int K, int THREADS, typename T> __device__ __forceinline__ void
         }
     }
 }
+// the same without the conversion: rows that are asked for ahead wait in the type's own size
+template <typename T, int V, int K> struct Raw { typedef T Vector __attribute__((ext_vector_type(V))); Vector v[K]; };
+template <int V, int K, int THREADS, typename T> __device__ __forceinline__ void load_raw(const T* src, int dim, Raw<T, V, K>& to) {
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+        const int c = (k * THREADS + thread_of<THREADS>()) * V;
+        to.v[k] = typename Raw<T, V, K>::Vector{};
+        if (c < dim) to.v[k] = *reinterpret_cast<const typename Raw<T, V, K>::Vector*>(src + c);
+    }
+}
+template <typename T, int V, int K> __device__ __forceinline__ void unpack(const Raw<T, V, K>& from, float (&v)[V * K]) {
+#pragma unroll
+    for (int k = 0; k < K; k++)
+#pragma unroll
+        for (int i = 0; i < V; i++) v[k * V + i] = (float)from.v[k][i];
+}
 template <int V, int K, int THREADS, typename T> __device__ __forceinline__ void store_row(T* dst, int dim, const float (&v)[V * K]) {
 #pragma unroll
     for (int k = 0; k < K; k++) {
-        const int c = (k * THREADS + (int)(threadIdx.x % THREADS)) * V;
+        const int c = (k * THREADS + thread_of<THREADS>()) * V;
         if (c < dim) rlt_store<V>(dst + c, v + k * V);
     }
 }
 // parameters of this thread's columns; `otherwise` where there are none
 template <int V, int K, int THREADS> __device__ __forceinline__ void load_parameters(const float* src, float otherwise, int dim, float (&v)[V * K]) {
 #pragma unroll
-    for (int k = 0; k < K; k++)
+    for (int i = 0; i < V * K; i++) v[i] = otherwise;
+    if (!src) return;
 #pragma unroll
-        for (int i = 0; i < V; i++) {
-            const int c = (k * THREADS + (int)(threadIdx.x % THREADS)) * V + i;
-            v[k * V + i] = src && c < dim ? src[c] : otherwise;
+    for (int k = 0; k < K; k++) {
+        const int c = (k * THREADS + thread_of<THREADS>()) * V;
+        if (c < dim) {      // V columns or none
+#pragma unroll
+            for (int i = 0; i < V; i++) v[k * V + i] = src[c + i];
         }
+    }
 }
 // subtracts a row's mean; columns beyond dim stay zero
 template <int V, int K, int THREADS> __device__ __forceinline__ void subtract(float (&v)[V * K], float mean, int dim) {
 #pragma unroll
     for (int k = 0; k < K; k++) {
-        const int c = (k * THREADS + (int)(threadIdx.x % THREADS)) * V;
+        const int c = (k * THREADS + thread_of<THREADS>()) * V;
         if (c < dim) {
 #pragma unroll
             for (int i = 0; i < V; i++) v[k * V + i] -= mean;
+        }
+    }
+}
+
+template <int V, int K, int THREADS> __device__ __forceinline__ void zero_beyond(float (&v)[V * K], int dim) {
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+        const int c = (k * THREADS + thread_of<THREADS>()) * V;
+        if (c >= dim) {
+#pragma unroll
+            for (int i = 0; i < V; i++) v[k * V + i] = 0.0f;
         }
     }
 }
@@ -146,7 +184,7 @@ template <typename T, int V, int K, int THREADS> __global__ __launch_bounds__(WO
     load_parameters<V, K, THREADS>(a.p.branch_weights, 1.0f, dim, bw); load_parameters<V, K, THREADS>(a.p.branch_biases, 0.0f, dim, bb);
     load_parameters<V, K, THREADS>(a.p.output_weights, 1.0f, dim, ow); load_parameters<V, K, THREADS>(a.p.output_biases, 0.0f, dim, ob);
     load_parameters<V, K, THREADS>(a.p.residual_scale, 1.0f, dim, scale);
-    for (int row = blockIdx.x * ROWS + threadIdx.x / THREADS; row < a.rows; row += gridDim.x * ROWS) {
+    for (int row = blockIdx.x * ROWS + row_of<THREADS>(); row < a.rows; row += gridDim.x * ROWS) {
         float y[N], u[N], g[N];
         if (a.branch) load_row<V, K, THREADS>((const T*)a.branch + (size_t)row * a.ldb, dim, u);
         load_row<V, K, THREADS>((const T*)a.x + (size_t)row * a.ldx, dim, y);
@@ -169,82 +207,129 @@ template <typename T, int V, int K, int THREADS> __global__ __launch_bounds__(WO
     }
 }
 
-// d: gradient with respect to the normalised row; becomes the one with respect to the row
-template <int V, int K, int THREADS> __device__ __forceinline__ void norm_gradient(float (&d)[V * K], const float (&normalised)[V * K], float inverse, int kind, int dim, float* lds, int& turn) {
-    constexpr int N = V * K;
-    if (kind == RLT_NORM_NONE) return;
-    const float inverse_dim = 1.0f / dim;
-    float s[2] = {0.0f, 0.0f};
-#pragma unroll
-    for (int i = 0; i < N; i++) { s[0] = fmaf(d[i], normalised[i], s[0]); s[1] += d[i]; }
-    row_sums<THREADS>(s, lds, turn);
-    const float along = s[0] * inverse_dim, mean = kind == RLT_NORM_LAYER ? s[1] * inverse_dim : 0.0f;
-#pragma unroll
-    for (int k = 0; k < K; k++) {
-        const int c = (k * THREADS + (int)(threadIdx.x % THREADS)) * V;
-#pragma unroll
-        for (int i = k * V; i < k * V + V; i++) d[i] = c < dim ? inverse * (d[i] - normalised[i] * along - mean) : 0.0f;      // the sums that follow take no column beyond dim
-    }
-}
-
+// Memory bounds this pass: five rows in, three out. The next row's values are asked for before this row's sums, of which a row has two rounds (three with means): what the statistics and the output norm's gradient need
+// is added up together.
 template <typename T, int V, int K, int THREADS, bool BIASES> __global__ __launch_bounds__(WORKGROUP<THREADS>) void norm_backward_kernel(NormBackward a) {
     constexpr int N = V * K, ROWS = WORKGROUP<THREADS> / THREADS;
+    // Parameters and column sums stay in registers from row to row. Rows wider than 4,096 leave none for them: parameters are read again, from L2, and the sums are kept in LDS, each by its own thread (4,096 rows of 8,192 bfloat16
+    // values: 183 us; 536 with 1,024 threads of eight columns, whose registers spill. 16,384 rows of 4,096: 278 us with registers, 332 so).
+    constexpr bool HELD = N * THREADS <= HELD_DIM;
     __shared__ float lds[THREADS > 64 ? 2 * (THREADS / 64) * 4 : ROWS * THREADS * N];
+    extern __shared__ __attribute__((aligned(16))) float column_sums[];
     int turn = 0;
-    const int dim = a.p.dim;
+    const int dim = a.p.dim, stride = gridDim.x * ROWS;
+    const float inverse_dim = 1.0f / dim;
+    const bool output_layer = a.d_h && a.p.output_norm == RLT_NORM_LAYER, branch_layer = a.branch && a.p.branch_norm == RLT_NORM_LAYER;
     float bw[N], bb[N], ow[N], scale[N];
-    load_parameters<V, K, THREADS>(a.p.branch_weights, 1.0f, dim, bw);
-    load_parameters<V, K, THREADS>(BIASES ? a.p.branch_biases : nullptr, 0.0f, dim, bb);
-    load_parameters<V, K, THREADS>(a.p.output_weights, 1.0f, dim, ow); load_parameters<V, K, THREADS>(a.p.residual_scale, 1.0f, dim, scale);
-    float sums[SUMS][N];
+    auto output_parameters = [&] { load_parameters<V, K, THREADS>(a.p.output_weights, 1.0f, dim, ow); };
+    auto branch_parameters = [&] {
+        load_parameters<V, K, THREADS>(a.p.branch_weights, 1.0f, dim, bw); load_parameters<V, K, THREADS>(BIASES ? a.p.branch_biases : nullptr, 0.0f, dim, bb);
+        load_parameters<V, K, THREADS>(a.p.residual_scale, 1.0f, dim, scale);
+    };
+    if (HELD) { output_parameters(); branch_parameters(); }
+    // Sum j of this thread's columns: in a register, or in LDS, 16 bytes of every thread side by side. 160 KB hold four sums of the widest rows and not the fifth.
+    constexpr int SLOT[SUMS] = {0, 3, 1, 4, 2}, SLOTS = BIASES ? 4 : 3;
+    float sums[HELD ? SUMS : 1][N];
+    auto add = [&](auto which, const float (&v)[N]) {
+        constexpr int j = decltype(which)::value;
+        if constexpr (HELD || SLOT[j] >= SLOTS) {
 #pragma unroll
-    for (int j = 0; j < SUMS; j++)
+            for (int i = 0; i < N; i++) sums[HELD ? j : 0][i] += v[i];
+        } else {
+#pragma unroll
+            for (int k = 0; k < N; k += 4) {
+                __builtin_amdgcn_sched_barrier(0);
+                rlt_f32x4* const at = reinterpret_cast<rlt_f32x4*>(column_sums) + (SLOT[j] * (N / 4) + k / 4) * THREADS + threadIdx.x;
+                rlt_f32x4 x = *at;
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[i] += v[k + i];
+                *at = x;
+            }
+        }
+    };
+#pragma unroll
+    for (int j = 0; j < (HELD ? SUMS : 1); j++)
 #pragma unroll
         for (int i = 0; i < N; i++) sums[j][i] = 0.0f;
-    for (int row = blockIdx.x * ROWS + threadIdx.x / THREADS; row < a.rows; row += gridDim.x * ROWS) {
-        float d[N], e[N], y[N], u[N], g[N];      // d: the gradient that reaches the residual stream
-        if (a.d_h) {
-            load_row<V, K, THREADS>((const T*)a.d_h + (size_t)row * a.lddh, dim, e);
-            load_row<V, K, THREADS>((const T*)a.y + (size_t)row * a.ldy, dim, y);
-        }
-        if (a.d_y) load_row<V, K, THREADS>((const T*)a.d_y + (size_t)row * a.lddy, dim, d);
-        else {
+    if constexpr (!HELD) {
 #pragma unroll
-            for (int i = 0; i < N; i++) d[i] = 0.0f;
-        }
-        if (a.branch) load_row<V, K, THREADS>((const T*)a.branch + (size_t)row * a.ldb, dim, u);
-        if (a.branch && a.gate) load_row<V, K, THREADS>((const T*)a.gate + (size_t)row * a.ldg, dim, g);
+        for (int j = 0; j < SLOTS * (N / 4); j++) reinterpret_cast<rlt_f32x4*>(column_sums)[j * THREADS + threadIdx.x] = rlt_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+#define NORM_SUM(j) std::integral_constant<int, j>{}
+    Raw<T, V, K> next_e{}, next_y{}, next_d{}, next_u{}, next_g{};
+    auto ask = [&](int row) {
         if (a.d_h) {
-            const float inverse = normalise<V, K, THREADS>(y, a.p.output_norm, a.p.epsilon, dim, lds, turn);
+            load_raw<V, K, THREADS>((const T*)a.d_h + (size_t)row * a.lddh, dim, next_e);
+            load_raw<V, K, THREADS>((const T*)a.y + (size_t)row * a.ldy, dim, next_y);
+        }
+        if (a.d_y) load_raw<V, K, THREADS>((const T*)a.d_y + (size_t)row * a.lddy, dim, next_d);
+        if (a.branch) {
+            load_raw<V, K, THREADS>((const T*)a.branch + (size_t)row * a.ldb, dim, next_u);
+            if (a.gate) load_raw<V, K, THREADS>((const T*)a.gate + (size_t)row * a.ldg, dim, next_g);
+        }
+    };
+    const int first = blockIdx.x * ROWS + row_of<THREADS>();
+    if (first < a.rows) ask(first);
+    for (int row = first; row < a.rows; row += stride) {
+        float d[N], e[N], y[N], u[N], g[N];      // d: the gradient that reaches the residual stream
+        unpack<T, V, K>(next_e, e); unpack<T, V, K>(next_y, y); unpack<T, V, K>(next_d, d); unpack<T, V, K>(next_u, u); unpack<T, V, K>(next_g, g);
+        if (row + stride < a.rows) ask(row + stride);
+        if (output_layer || branch_layer) {
+            float s[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < N; i++) { s[0] += y[i]; s[1] += u[i]; }
+            row_sums<THREADS>(s, lds, turn);
+            if (output_layer) subtract<V, K, THREADS>(y, s[0] * inverse_dim, dim);
+            if (branch_layer) subtract<V, K, THREADS>(u, s[1] * inverse_dim, dim);
+        }
+        if (!HELD) { output_parameters(); __builtin_amdgcn_sched_barrier(0); }
+        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};      // of y^2, of the output norm's gradient times y, of that gradient, of branch^2
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const float w = e[i] * ow[i];
+            s[0] = fmaf(y[i], y[i], s[0]); s[1] = fmaf(w, y[i], s[1]); s[2] += w; s[3] = fmaf(u[i], u[i], s[3]);
+        }
+        row_sums<THREADS>(s, lds, turn);
+        if (a.d_h) {
+            const bool none = a.p.output_norm == RLT_NORM_NONE;
+            const float inverse = none ? 1.0f : 1.0f / sqrtf(s[0] * inverse_dim + a.p.epsilon), along = none ? 0.0f : inverse * s[1] * inverse_dim, mean = output_layer ? s[2] * inverse_dim : 0.0f;
 #pragma unroll
             for (int i = 0; i < N; i++) {
-                y[i] *= inverse;
-                sums[OUTPUT_W][i] = fmaf(e[i], y[i], sums[OUTPUT_W][i]);
-                if (BIASES) sums[OUTPUT_B][i] += e[i];
-                e[i] *= ow[i];
+                const float n = y[i] * inverse;
+                y[i] = e[i] * n;
+                d[i] = fmaf(inverse, fmaf(e[i], ow[i], -n * along) - mean, d[i]);
             }
-            norm_gradient<V, K, THREADS>(e, y, inverse, a.p.output_norm, dim, lds, turn);
-#pragma unroll
-            for (int i = 0; i < N; i++) d[i] += e[i];
+            if (!HELD) __builtin_amdgcn_sched_barrier(0);
+            add(NORM_SUM(OUTPUT_W), y);
+            if constexpr (BIASES) add(NORM_SUM(OUTPUT_B), e);
+            if (mean != 0.0f) zero_beyond<V, K, THREADS>(d, dim);      // the sums that follow take no column beyond dim
         }
         if (a.d_x) store_row<V, K, THREADS>((T*)a.d_x + (size_t)row * a.lddx, dim, d);
         if (a.branch) {
-            const float inverse = normalise<V, K, THREADS>(u, a.p.branch_norm, a.p.epsilon, dim, lds, turn);
-            float slope[N];
+            const bool none = a.p.branch_norm == RLT_NORM_NONE;
+            const float inverse = none ? 1.0f : 1.0f / sqrtf(s[3] * inverse_dim + a.p.epsilon);
+            if (!HELD) { __builtin_amdgcn_sched_barrier(0); branch_parameters(); }
+            float slope[N], t[2] = {0.0f, 0.0f};
             if (a.gate) gates_of<N, true>(g, slope, a.p.gate_activation);
 #pragma unroll
             for (int i = 0; i < N; i++) {
                 u[i] *= inverse;
-                const float n = BIASES ? fmaf(u[i], bw[i], bb[i]) : u[i] * bw[i], m = a.gate ? g[i] : 1.0f, dn = d[i] * scale[i] * m;
-                sums[SCALE][i] = fmaf(d[i] * m, n, sums[SCALE][i]);
-                sums[BRANCH_W][i] = fmaf(dn, u[i], sums[BRANCH_W][i]);
-                if (BIASES) sums[BRANCH_B][i] += dn;
-                if (a.gate) slope[i] *= d[i] * scale[i] * n;
+                const float n = BIASES ? fmaf(u[i], bw[i], bb[i]) : u[i] * bw[i], m = a.gate ? g[i] : 1.0f, ds = d[i] * scale[i], dn = ds * m;
+                if (a.gate) slope[i] *= ds * n;
+                y[i] = d[i] * m * n; d[i] = dn * u[i]; g[i] = dn;      // summands of the columns
                 e[i] = dn * bw[i];
+                t[0] = fmaf(e[i], u[i], t[0]); t[1] += e[i];
             }
+            add(NORM_SUM(SCALE), y); add(NORM_SUM(BRANCH_W), d);
+            if constexpr (BIASES) add(NORM_SUM(BRANCH_B), g);
             if (a.d_gate) store_row<V, K, THREADS>((T*)a.d_gate + (size_t)row * a.lddg, dim, slope);
             if (a.d_branch) {
-                norm_gradient<V, K, THREADS>(e, u, inverse, a.p.branch_norm, dim, lds, turn);
+                if (!none) {
+                    row_sums<THREADS>(t, lds, turn);
+                    const float along = t[0] * inverse_dim, mean = branch_layer ? t[1] * inverse_dim : 0.0f;
+#pragma unroll
+                    for (int i = 0; i < N; i++) e[i] = inverse * (e[i] - u[i] * along - mean);
+                }
                 store_row<V, K, THREADS>((T*)a.d_branch + (size_t)row * a.lddb, dim, e);
             }
         }
@@ -253,13 +338,13 @@ template <typename T, int V, int K, int THREADS, bool BIASES> __global__ __launc
     float* out = a.partial + (size_t)blockIdx.x * SUMS * dim;
 #pragma unroll
     for (int j = 0; j < SUMS; j++) {
-        if (!wanted[j]) continue;
+        if (!wanted[j] || (!BIASES && (j == BRANCH_B || j == OUTPUT_B))) continue;
         if constexpr (ROWS > 1) {      // the rows' threads side by side, then column by column in their order
             __syncthreads();
 #pragma unroll
             for (int k = 0; k < K; k++)
 #pragma unroll
-                for (int i = 0; i < V; i++) lds[(threadIdx.x / THREADS) * THREADS * N + (k * THREADS + threadIdx.x % THREADS) * V + i] = sums[j][k * V + i];
+                for (int i = 0; i < V; i++) lds[(threadIdx.x / THREADS) * THREADS * N + (k * THREADS + threadIdx.x % THREADS) * V + i] = sums[HELD ? j : 0][k * V + i];
             __syncthreads();
             for (int c = threadIdx.x; c < dim; c += WORKGROUP<THREADS>) {
                 float s = 0.0f;
@@ -272,12 +357,13 @@ template <typename T, int V, int K, int THREADS, bool BIASES> __global__ __launc
             for (int k = 0; k < K; k++)
 #pragma unroll
                 for (int i = 0; i < V; i++) {
-                    const int c = (k * THREADS + (int)threadIdx.x) * V + i;
-                    if (c < dim) out[(size_t)j * dim + c] = sums[j][k * V + i];
+                    const int c = (k * THREADS + (int)threadIdx.x) * V + i, n = k * V + i;
+                    if (c < dim) out[(size_t)j * dim + c] = HELD || SLOT[j] >= SLOTS ? sums[HELD ? j : 0][n] : column_sums[((SLOT[j] * (N / 4) + n / 4) * THREADS + threadIdx.x) * 4 + n % 4];
                 }
         }
     }
 }
+#undef NORM_SUM
 
 // adds up the workgroups' column sums, in a fixed order: 64 columns to a workgroup, whose wavefronts take every sixteenth block each
 __global__ __launch_bounds__(1024) void norm_sum_kernel(const float* __restrict__ partial, int blocks, int dim, rlt_residual_norm p, int accumulate) {
@@ -300,8 +386,8 @@ __global__ __launch_bounds__(1024) void norm_sum_kernel(const float* __restrict_
     }
 }
 
-// threads that share a row in the backward pass, eight columns each
-int backward_threads(int dim) { return dim <= 128 ? 16 : dim <= 512 ? 64 : dim <= 1024 ? 128 : dim <= 2048 ? 256 : dim <= 4096 ? 512 : 1024; }
+// threads that share a row in the backward pass, eight columns each, or sixteen
+int backward_threads(int dim) { return dim <= 128 ? 16 : dim <= 512 ? 64 : dim <= 1024 ? 128 : dim <= 2048 ? 256 : 512; }
 int backward_blocks(const rlt_residual_norm* p, int rows) {
     const int threads = backward_threads(p->dim), at_once = threads <= 64 ? 256 / threads : 1, blocks = (rows + at_once - 1) / at_once;
     return blocks < 512 ? blocks : 512;
@@ -320,15 +406,22 @@ template <typename T, int V> void launch_forward(rlt_rocm_device* device, const 
     else if (dim <= 4096) go(norm_forward_kernel<T, V, 8 / V, 512>, 512);
     else go(norm_forward_kernel<T, V, 8 / V, 1024>, 1024);
 }
-template <typename T, int V, bool BIASES> void launch_backward(rlt_rocm_device* device, const NormBackward& a) {
+template <typename T, int V, bool BIASES> int launch_backward(rlt_rocm_device* device, const NormBackward& a) {
     const int threads = backward_threads(a.p.dim);
-    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(backward_blocks(&a.p, a.rows)), dim3(threads <= 64 ? 256 : threads), 0, device->stream, a); };
+    const size_t bytes = a.p.dim > HELD_DIM ? (size_t)(BIASES ? 4 : 3) * MAX_DIM * sizeof(float) : 0;
+    hipError_t e = hipSuccess;
+    auto go = [&](auto kernel) {
+        if (bytes) e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        if (e == hipSuccess) hipLaunchKernelGGL(kernel, dim3(backward_blocks(&a.p, a.rows)), dim3(threads <= 64 ? 256 : threads), bytes, device->stream, a);
+    };
     if (threads == 16) go(norm_backward_kernel<T, V, 8 / V, 16, BIASES>);
     else if (threads == 64) go(norm_backward_kernel<T, V, 8 / V, 64, BIASES>);
     else if (threads == 128) go(norm_backward_kernel<T, V, 8 / V, 128, BIASES>);
     else if (threads == 256) go(norm_backward_kernel<T, V, 8 / V, 256, BIASES>);
-    else if (threads == 512) go(norm_backward_kernel<T, V, 8 / V, 512, BIASES>);
-    else go(norm_backward_kernel<T, V, 8 / V, 1024, BIASES>);
+    else if (a.p.dim <= HELD_DIM) go(norm_backward_kernel<T, V, 8 / V, 512, BIASES>);
+    else go(norm_backward_kernel<T, V, 16 / V, 512, BIASES>);
+    RLT_HIP(e);
+    return rlt_launch_status(device);
 }
 // vectors of 16 bytes where every tensor's rows start on such boundaries and hold whole vectors
 template <typename T> void forward(rlt_rocm_device* device, const NormForward& a) {
@@ -337,14 +430,14 @@ template <typename T> void forward(rlt_rocm_device* device, const NormForward& a
                          rlt_vectors<T>(a.y, a.y ? a.ldy : 0) && rlt_vectors<T>(a.h, a.h ? a.ldh : 0);
     if (vectors) launch_forward<T, V>(device, a); else launch_forward<T, 1>(device, a);
 }
-template <typename T> void backward(rlt_rocm_device* device, const NormBackward& a) {
+template <typename T> int backward(rlt_rocm_device* device, const NormBackward& a) {
     constexpr int V = 16 / sizeof(T);
     const bool vectors = a.p.dim % V == 0 && rlt_vectors<T>(a.branch, a.branch ? a.ldb : 0) && rlt_vectors<T>(a.gate, a.gate ? a.ldg : 0) && rlt_vectors<T>(a.y, a.d_h ? a.ldy : 0) &&
                          rlt_vectors<T>(a.d_y, a.d_y ? a.lddy : 0) && rlt_vectors<T>(a.d_h, a.d_h ? a.lddh : 0) && rlt_vectors<T>(a.d_x, a.d_x ? a.lddx : 0) &&
                          rlt_vectors<T>(a.d_branch, a.d_branch ? a.lddb : 0) && rlt_vectors<T>(a.d_gate, a.d_gate ? a.lddg : 0);
     const bool biases = a.p.branch_biases || a.p.d_branch_biases || a.p.d_output_biases;
-    if (vectors) { if (biases) launch_backward<T, V, true>(device, a); else launch_backward<T, V, false>(device, a); }
-    else { if (biases) launch_backward<T, 1, true>(device, a); else launch_backward<T, 1, false>(device, a); }
+    if (vectors) return biases ? launch_backward<T, V, true>(device, a) : launch_backward<T, V, false>(device, a);
+    return biases ? launch_backward<T, 1, true>(device, a) : launch_backward<T, 1, false>(device, a);
 }
 
 bool described(const rlt_residual_norm* p) {
@@ -387,8 +480,7 @@ int rlt_rocm_residual_norm_backward(rlt_rocm_device* device, const rlt_residual_
     const bool sums = layer->d_branch_weights || layer->d_branch_biases || layer->d_output_weights || layer->d_output_biases || layer->d_residual_scale;
     RLT_REQUIRE(!sums || (workspace && workspace_bytes >= rlt_rocm_residual_norm_workspace_bytes(layer, rows)));
     const NormBackward a = {*layer, branch, gate, y, d_y, d_h, d_x, d_branch, d_gate, ldb, ldg, ldy, lddy, lddh, lddx, lddb, lddg, rows, (float*)workspace};
-    if (layer->type == RLT_TYPE_F32) backward<float>(device, a); else backward<rlt_bf16>(device, a);
-    int rc = rlt_launch_status(device);
+    const int rc = layer->type == RLT_TYPE_F32 ? backward<float>(device, a) : backward<rlt_bf16>(device, a);
     if (rc || !sums) return rc;
     hipLaunchKernelGGL(norm_sum_kernel, dim3((dim + 63) / 64, SUMS), dim3(1024), 0, device->stream, (const float*)workspace, backward_blocks(layer, rows), dim, *layer, accumulate);
     return rlt_launch_status(device);
