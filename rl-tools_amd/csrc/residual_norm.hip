@@ -213,7 +213,7 @@ template <typename T, int V, int K, int THREADS, bool BIASES> __global__ __launc
     constexpr int N = V * K, ROWS = WORKGROUP<THREADS> / THREADS;
     // Parameters and column sums stay in registers from row to row. Rows wider than 4,096 leave none for them: parameters are read again, from L2, and the sums are kept in LDS, each by its own thread (4,096 rows of 8,192 bfloat16
     // values: 183 us; 536 with 1,024 threads of eight columns, whose registers spill. 16,384 rows of 4,096: 278 us with registers, 332 so).
-    constexpr bool HELD = N * THREADS <= HELD_DIM;
+    constexpr bool HELD = N * THREADS <= HELD_DIM, AHEAD = HELD || V == 8;
     __shared__ float lds[THREADS > 64 ? 2 * (THREADS / 64) * 4 : ROWS * THREADS * N];
     extern __shared__ __attribute__((aligned(16))) float column_sums[];
     int turn = 0;
@@ -269,11 +269,12 @@ template <typename T, int V, int K, int THREADS, bool BIASES> __global__ __launc
         }
     };
     const int first = blockIdx.x * ROWS + row_of<THREADS>();
-    if (first < a.rows) ask(first);
+    if (AHEAD && first < a.rows) ask(first);
     for (int row = first; row < a.rows; row += stride) {
         float d[N], e[N], y[N], u[N], g[N];      // d: the gradient that reaches the residual stream
+        if (!AHEAD) ask(row);
         unpack<T, V, K>(next_e, e); unpack<T, V, K>(next_y, y); unpack<T, V, K>(next_d, d); unpack<T, V, K>(next_u, u); unpack<T, V, K>(next_g, g);
-        if (row + stride < a.rows) ask(row + stride);
+        if (AHEAD && row + stride < a.rows) ask(row + stride);
         if (output_layer || branch_layer) {
             float s[2] = {0.0f, 0.0f};
 #pragma unroll

@@ -310,7 +310,8 @@ def test_optional_arguments(rocm):
 
 @gpu
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
-@pytest.mark.parametrize("rows,heads,kv_heads,dk,dv", [(1, 1, 1, 1, 1), (64, 2, 2, 32, 32), (3, 6, 2, 24, 41), (5, 4, 4, 64, 64), (2, 3, 1, 128, 128), (7, 2, 2, 128, 20), (2, 2, 2, 7, 128), (300, 8, 8, 16, 16)])
+@pytest.mark.parametrize("rows,heads,kv_heads,dk,dv", [(1, 1, 1, 1, 1), (64, 2, 2, 32, 32), (3, 6, 2, 24, 41), (5, 4, 4, 64, 64), (2, 3, 1, 128, 128), (7, 2, 2, 128, 20), (2, 2, 2, 7, 128), (300, 8, 8, 16, 16),
+                                                       (3, 2, 2, 128, 101), (5, 3, 1, 5, 64), (2, 3, 3, 100, 1), (3, 2, 1, 8, 101), (1, 5, 5, 8, 100), (9, 1, 1, 17, 3)])
 @pytest.mark.parametrize("in_place", [False, True])
 def test_steps_walk_a_sequence(rocm, rows, heads, kv_heads, dk, dv, dtype, in_place):
     """five steps one by one against the recurrence, states that a reset drops included; a state that is not finite is dropped too"""
