@@ -19,18 +19,19 @@ struct NormBackward {
     float* partial;               // [workgroups][SUMS][dim]
 };
 
-// THREADS share a row: a part of a wavefront, a wavefront (several rows to a workgroup of 256 then, whose wavefronts do not wait for each other) or a workgroup.
-template <int THREADS> constexpr int WORKGROUP = THREADS <= 64 ? 256 : THREADS;
+// THREADS share a row: a part of a wavefront, a wavefront, several or all of a workgroup of WIDTH threads.
+template <int THREADS> constexpr int FORWARD_WIDTH = THREADS <= 64 ? 256 : THREADS;
+template <int THREADS> constexpr int BACKWARD_WIDTH = THREADS < 256 ? 256 : THREADS;      // half the column sums to join that workgroups of 128 have, at as many wavefronts (4,001 x 1,000 fp32: 36 us, 40 with 128)
 
 // a thread's place in its row, and its row's in the workgroup (the same for all of a wavefront where a row has one or more: addresses of rows stay scalar)
-template <int THREADS> __device__ __forceinline__ int thread_of() { return WORKGROUP<THREADS> == THREADS ? (int)threadIdx.x : (int)(threadIdx.x % THREADS); }
-template <int THREADS> __device__ __forceinline__ int row_of() {
-    return WORKGROUP<THREADS> == THREADS ? 0 : THREADS == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / 64) : (int)(threadIdx.x / THREADS);
+template <int THREADS> __device__ __forceinline__ int thread_of() { return (int)(threadIdx.x % THREADS); }
+template <int THREADS, int WIDTH> __device__ __forceinline__ int row_of() {
+    return WIDTH == THREADS ? 0 : THREADS >= 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / THREADS) : (int)(threadIdx.x / THREADS);
 }
 
 // Sums over the threads that share a row, every one of which receives them. Consecutive calls take turns with two halves of `lds`: a wavefront that writes one has passed the barrier
 // behind which everybody had read it.
-template <int THREADS, int N> __device__ __forceinline__ void row_sums(float (&v)[N], float* lds, int& turn) {
+template <int THREADS, int WIDTH, int N> __device__ __forceinline__ void row_sums(float (&v)[N], float* lds, int& turn) {
 #pragma unroll
     for (int i = 0; i < N; i++) {
         asm volatile("" : "+v"(v[i]));      // no contraction into the first exchange: both sides of an exchange round alike (rlt_wave_sum)
@@ -39,12 +40,13 @@ template <int THREADS, int N> __device__ __forceinline__ void row_sums(float (&v
     }
     if constexpr (THREADS > 64) {
         constexpr int WAVES = THREADS / 64;
-        float* half = lds + turn * WAVES * 4;
+        float* half = lds + turn * (WIDTH / 64) * 4;
         turn ^= 1;
         if ((threadIdx.x & 63) == 0) {
 #pragma unroll
             for (int i = 0; i < N; i++) half[(threadIdx.x >> 6) * 4 + i] = v[i];
         }
+        if (WIDTH > THREADS) half += row_of<THREADS, WIDTH>() * WAVES * 4;
         rlt_lds_barrier();
 #pragma unroll
         for (int i = 0; i < N; i++) {
@@ -56,80 +58,124 @@ template <int THREADS, int N> __device__ __forceinline__ void row_sums(float (&v
     }
 }
 
-// Thread t of a row's THREADS has vectors t, t + THREADS, ... of V elements, K of them.
-template <int V, int K, int THREADS, typename T> __device__ __forceinline__ void load_row(const T* src, int dim, float (&v)[V * K]) {
-#pragma unroll
-    for (int k = 0; k < K; k++) {
-        const int c = (k * THREADS + thread_of<THREADS>()) * V;
-        if (c < dim) rlt_load<V>(src + c, v + k * V);
-        else {
-#pragma unroll
-            for (int i = 0; i < V; i++) v[k * V + i] = 0.0f;
-        }
-    }
-}
-// the same without the conversion: rows that are asked for ahead wait in the type's own size
+// Thread t of a row's THREADS has vectors t, t + THREADS, ... of V elements (16 bytes), K of them. WHOLE: rows start on 16-byte boundaries and hold whole vectors. Otherwise the same loads and stores start at any element, which the
+// memory instructions allow; a row's last vector is loaded where it ends with the row, and its elements move down when they are needed, so that no load waits for a branch. (8,192 rows of 1,001 bfloat16 values: 27 us
+// forward, 45 us backward; 52 and 71 with an element to a load.)
+template <typename T, int V, bool WHOLE> struct Row { typedef T Vector __attribute__((ext_vector_type(V))); };
+template <typename T, int V> struct Row<T, V, false> { typedef T Vector __attribute__((ext_vector_type(V), aligned(sizeof(T)))); };
 template <typename T, int V, int K> struct Raw { typedef T Vector __attribute__((ext_vector_type(V))); Vector v[K]; };
-template <int V, int K, int THREADS, typename T> __device__ __forceinline__ void load_raw(const T* src, int dim, Raw<T, V, K>& to) {
+template <int V, int K, int THREADS, bool WHOLE, typename T> __device__ __forceinline__ void load_raw(const T* src, int dim, Raw<T, V, K>& to) {
 #pragma unroll
     for (int k = 0; k < K; k++) {
         const int c = (k * THREADS + thread_of<THREADS>()) * V;
         to.v[k] = typename Raw<T, V, K>::Vector{};
-        if (c < dim) to.v[k] = *reinterpret_cast<const typename Raw<T, V, K>::Vector*>(src + c);
-    }
-}
-template <typename T, int V, int K> __device__ __forceinline__ void unpack(const Raw<T, V, K>& from, float (&v)[V * K]) {
+        if constexpr (WHOLE) {
+            if (c < dim) to.v[k] = *reinterpret_cast<const typename Row<T, V, WHOLE>::Vector*>(src + c);
+        } else if (dim >= V) {
+            if (c < dim) to.v[k] = *reinterpret_cast<const typename Row<T, V, WHOLE>::Vector*>(src + (c + V <= dim ? c : dim - V));
+        } else {
 #pragma unroll
-    for (int k = 0; k < K; k++)
-#pragma unroll
-        for (int i = 0; i < V; i++) v[k * V + i] = (float)from.v[k][i];
-}
-template <int V, int K, int THREADS, typename T> __device__ __forceinline__ void store_row(T* dst, int dim, const float (&v)[V * K]) {
-#pragma unroll
-    for (int k = 0; k < K; k++) {
-        const int c = (k * THREADS + thread_of<THREADS>()) * V;
-        if (c < dim) rlt_store<V>(dst + c, v + k * V);
-    }
-}
-// parameters of this thread's columns; `otherwise` where there are none
-template <int V, int K, int THREADS> __device__ __forceinline__ void load_parameters(const float* src, float otherwise, int dim, float (&v)[V * K]) {
-#pragma unroll
-    for (int i = 0; i < V * K; i++) v[i] = otherwise;
-    if (!src) return;
-#pragma unroll
-    for (int k = 0; k < K; k++) {
-        const int c = (k * THREADS + thread_of<THREADS>()) * V;
-        if (c < dim) {      // V columns or none
-#pragma unroll
-            for (int i = 0; i < V; i++) v[k * V + i] = src[c + i];
+            for (int i = 0; i < V; i++) to.v[k][i] = c + i < dim ? src[c + i] : (T)0.0f;
         }
     }
 }
+template <int V, int K, int THREADS, bool WHOLE, typename T> __device__ __forceinline__ void unpack(const Raw<T, V, K>& from, int dim, float (&v)[V * K]) {
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+#pragma unroll
+        for (int i = 0; i < V; i++) v[k * V + i] = (float)from.v[k][i];
+        const int c = (k * THREADS + thread_of<THREADS>()) * V, beyond = c + V - dim;
+        if (!WHOLE && beyond > 0 && c < dim && dim >= V) {
+#pragma unroll
+            for (int n = 1; n < V; n *= 2) {
+#pragma unroll
+                for (int i = 0; i < V; i++) v[k * V + i] = beyond & n ? (i + n < V ? v[k * V + (i + n) % V] : 0.0f) : v[k * V + i];
+            }
+        }
+    }
+}
+template <int V, int K, int THREADS, bool WHOLE, typename T> __device__ __forceinline__ void load_row(const T* src, int dim, float (&v)[V * K]) {
+    if constexpr (WHOLE && sizeof(T) == sizeof(float)) {
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            const int c = (k * THREADS + thread_of<THREADS>()) * V;
+            if (c < dim) rlt_load<V>(src + c, v + k * V);
+            else {
+#pragma unroll
+                for (int i = 0; i < V; i++) v[k * V + i] = 0.0f;
+            }
+        }
+    } else {
+        Raw<T, V, K> raw;
+        load_raw<V, K, THREADS, WHOLE>(src, dim, raw);
+        unpack<V, K, THREADS, WHOLE>(raw, dim, v);
+    }
+}
+// rounds to nearest, ties to even
+template <int V, int K, int THREADS, bool WHOLE, typename T> __device__ __forceinline__ void store_row(T* dst, int dim, const float (&v)[V * K]) {
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+        const int c = (k * THREADS + thread_of<THREADS>()) * V;
+        if (WHOLE ? c < dim : c + V <= dim) {
+            typename Raw<T, V, K>::Vector x;
+#pragma unroll
+            for (int i = 0; i < V; i++) x[i] = (T)v[k * V + i];
+            *reinterpret_cast<typename Row<T, V, WHOLE>::Vector*>(dst + c) = x;
+        } else if (!WHOLE && c < dim) {
+#pragma unroll
+            for (int i = 0; i < V - 1; i++) if (c + i < dim) dst[c + i] = (T)v[k * V + i];
+        }
+    }
+}
+// parameters of this thread's columns, zero beyond dim; `otherwise` where there are none
+template <int V, int K, int THREADS, bool WHOLE> __device__ __forceinline__ void load_parameters(const float* src, float otherwise, int dim, float (&v)[V * K]) {
+#pragma unroll
+    for (int i = 0; i < V * K; i++) v[i] = otherwise;
+    if (!src) return;
+    int t = thread_of<THREADS>();
+    asm volatile("" : "+v"(t));      // addresses are formed here, not ahead of a loop over rows, whose registers they would take
+#pragma unroll
+    for (int n = 0; n < V * K; n += 4) {
+        const int c = (n / V * THREADS + t) * V + n % V, beyond = c + 4 - dim;
+        rlt_f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (WHOLE || dim >= 4) {
+            if (c < dim) x = *reinterpret_cast<const Row<float, 4, false>::Vector*>(src + (WHOLE || beyond <= 0 ? c : dim - 4));
+            if (!WHOLE && beyond > 0) {
+                if (beyond & 1) x = rlt_f32x4{x[1], x[2], x[3], 0.0f};
+                if (beyond & 2) x = rlt_f32x4{x[2], x[3], 0.0f, 0.0f};
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) if (c + i < dim) x[i] = src[c + i];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[n + i] = x[i];
+    }
+}
 // subtracts a row's mean; columns beyond dim stay zero
-template <int V, int K, int THREADS> __device__ __forceinline__ void subtract(float (&v)[V * K], float mean, int dim) {
+template <int V, int K, int THREADS, bool WHOLE> __device__ __forceinline__ void subtract(float (&v)[V * K], float mean, int dim) {
 #pragma unroll
     for (int k = 0; k < K; k++) {
         const int c = (k * THREADS + thread_of<THREADS>()) * V;
         if (c < dim) {
 #pragma unroll
-            for (int i = 0; i < V; i++) v[k * V + i] -= mean;
+            for (int i = 0; i < V; i++) if (WHOLE || c + i < dim) v[k * V + i] -= mean;
         }
     }
 }
-
-template <int V, int K, int THREADS> __device__ __forceinline__ void zero_beyond(float (&v)[V * K], int dim) {
+template <int V, int K, int THREADS, bool WHOLE> __device__ __forceinline__ void zero_beyond(float (&v)[V * K], int dim) {
 #pragma unroll
     for (int k = 0; k < K; k++) {
         const int c = (k * THREADS + thread_of<THREADS>()) * V;
-        if (c >= dim) {
+        if (WHOLE ? c >= dim : c + V > dim) {
 #pragma unroll
-            for (int i = 0; i < V; i++) v[k * V + i] = 0.0f;
+            for (int i = 0; i < V; i++) if (WHOLE || c + i >= dim) v[k * V + i] = 0.0f;
         }
     }
 }
 
 // a row's values less their mean (RLT_NORM_LAYER), and 1 / deviation
-template <int V, int K, int THREADS> __device__ __forceinline__ float normalise(float (&v)[V * K], int kind, float epsilon, int dim, float* lds, int& turn) {
+template <int V, int K, int THREADS, bool WHOLE> __device__ __forceinline__ float normalise(float (&v)[V * K], int kind, float epsilon, int dim, float* lds, int& turn) {
     constexpr int N = V * K;
     if (kind == RLT_NORM_NONE) return 1.0f;
     const float inverse_dim = 1.0f / dim;
@@ -138,13 +184,13 @@ template <int V, int K, int THREADS> __device__ __forceinline__ float normalise(
         s[0] = 0.0f;
 #pragma unroll
         for (int i = 0; i < N; i++) s[0] += v[i];
-        row_sums<THREADS>(s, lds, turn);
-        subtract<V, K, THREADS>(v, s[0] * inverse_dim, dim);
+        row_sums<THREADS, FORWARD_WIDTH<THREADS>>(s, lds, turn);
+        subtract<V, K, THREADS, WHOLE>(v, s[0] * inverse_dim, dim);
     }
     s[0] = 0.0f;
 #pragma unroll
     for (int i = 0; i < N; i++) s[0] = fmaf(v[i], v[i], s[0]);
-    row_sums<THREADS>(s, lds, turn);
+    row_sums<THREADS, FORWARD_WIDTH<THREADS>>(s, lds, turn);
     return 1.0f / sqrtf(s[0] * inverse_dim + epsilon);
 }
 
@@ -175,56 +221,56 @@ template <int N, bool SLOPES> __device__ __forceinline__ void gates_of(float (&g
     }
 }
 
-template <typename T, int V, int K, int THREADS> __global__ __launch_bounds__(WORKGROUP<THREADS>) void norm_forward_kernel(NormForward a) {
-    constexpr int N = V * K, ROWS = WORKGROUP<THREADS> / THREADS;
+template <typename T, int V, int K, int THREADS, bool WHOLE> __global__ __launch_bounds__(FORWARD_WIDTH<THREADS>) void norm_forward_kernel(NormForward a) {
+    constexpr int N = V * K, ROWS = FORWARD_WIDTH<THREADS> / THREADS;
     __shared__ float lds[THREADS > 64 ? 2 * (THREADS / 64) * 4 : 1];
     int turn = 0;
     const int dim = a.p.dim;
     float bw[N], bb[N], ow[N], ob[N], scale[N];
-    load_parameters<V, K, THREADS>(a.p.branch_weights, 1.0f, dim, bw); load_parameters<V, K, THREADS>(a.p.branch_biases, 0.0f, dim, bb);
-    load_parameters<V, K, THREADS>(a.p.output_weights, 1.0f, dim, ow); load_parameters<V, K, THREADS>(a.p.output_biases, 0.0f, dim, ob);
-    load_parameters<V, K, THREADS>(a.p.residual_scale, 1.0f, dim, scale);
-    for (int row = blockIdx.x * ROWS + row_of<THREADS>(); row < a.rows; row += gridDim.x * ROWS) {
+    load_parameters<V, K, THREADS, WHOLE>(a.p.branch_weights, 1.0f, dim, bw); load_parameters<V, K, THREADS, WHOLE>(a.p.branch_biases, 0.0f, dim, bb);
+    load_parameters<V, K, THREADS, WHOLE>(a.p.output_weights, 1.0f, dim, ow); load_parameters<V, K, THREADS, WHOLE>(a.p.output_biases, 0.0f, dim, ob);
+    load_parameters<V, K, THREADS, WHOLE>(a.p.residual_scale, 1.0f, dim, scale);
+    for (int row = blockIdx.x * ROWS + row_of<THREADS, FORWARD_WIDTH<THREADS>>(); row < a.rows; row += gridDim.x * ROWS) {
         float y[N], u[N], g[N];
-        if (a.branch) load_row<V, K, THREADS>((const T*)a.branch + (size_t)row * a.ldb, dim, u);
-        load_row<V, K, THREADS>((const T*)a.x + (size_t)row * a.ldx, dim, y);
-        if (a.branch && a.gate) load_row<V, K, THREADS>((const T*)a.gate + (size_t)row * a.ldg, dim, g);
+        if (a.branch) load_row<V, K, THREADS, WHOLE>((const T*)a.branch + (size_t)row * a.ldb, dim, u);
+        load_row<V, K, THREADS, WHOLE>((const T*)a.x + (size_t)row * a.ldx, dim, y);
+        if (a.branch && a.gate) load_row<V, K, THREADS, WHOLE>((const T*)a.gate + (size_t)row * a.ldg, dim, g);
         if (a.branch) {
-            const float inverse = normalise<V, K, THREADS>(u, a.p.branch_norm, a.p.epsilon, dim, lds, turn);
+            const float inverse = normalise<V, K, THREADS, WHOLE>(u, a.p.branch_norm, a.p.epsilon, dim, lds, turn);
             float slope[N];
             if (a.gate) gates_of<N, false>(g, slope, a.p.gate_activation);
 #pragma unroll
             for (int i = 0; i < N; i++) y[i] = fmaf(a.gate ? scale[i] * g[i] : scale[i], fmaf(u[i] * inverse, bw[i], bb[i]), y[i]);
             // columns beyond dim: u, g and y are zero, a bias is too
         }
-        if (a.y) store_row<V, K, THREADS>((T*)a.y + (size_t)row * a.ldy, dim, y);
+        if (a.y) store_row<V, K, THREADS, WHOLE>((T*)a.y + (size_t)row * a.ldy, dim, y);
         if (a.h) {
-            const float inverse = normalise<V, K, THREADS>(y, a.p.output_norm, a.p.epsilon, dim, lds, turn);
+            const float inverse = normalise<V, K, THREADS, WHOLE>(y, a.p.output_norm, a.p.epsilon, dim, lds, turn);
 #pragma unroll
             for (int i = 0; i < N; i++) y[i] = fmaf(y[i] * inverse, ow[i], ob[i]);
-            store_row<V, K, THREADS>((T*)a.h + (size_t)row * a.ldh, dim, y);
+            store_row<V, K, THREADS, WHOLE>((T*)a.h + (size_t)row * a.ldh, dim, y);
         }
     }
 }
 
 // Memory bounds this pass: five rows in, three out. The next row's values are asked for before this row's sums, of which a row has two rounds (three with means): what the statistics and the output norm's gradient need
 // is added up together.
-template <typename T, int V, int K, int THREADS, bool BIASES> __global__ __launch_bounds__(WORKGROUP<THREADS>) void norm_backward_kernel(NormBackward a) {
-    constexpr int N = V * K, ROWS = WORKGROUP<THREADS> / THREADS;
+template <typename T, int V, int K, int THREADS, bool BIASES, bool WHOLE> __global__ __launch_bounds__(BACKWARD_WIDTH<THREADS>) void norm_backward_kernel(NormBackward a) {
+    constexpr int N = V * K, WIDTH = BACKWARD_WIDTH<THREADS>, ROWS = WIDTH / THREADS;
     // Parameters and column sums stay in registers from row to row. Rows wider than 4,096 leave none for them: parameters are read again, from L2, and the sums are kept in LDS, each by its own thread (4,096 rows of 8,192 bfloat16
     // values: 183 us; 536 with 1,024 threads of eight columns, whose registers spill. 16,384 rows of 4,096: 278 us with registers, 332 so).
-    constexpr bool HELD = N * THREADS <= HELD_DIM, AHEAD = HELD || V == 8;
-    __shared__ float lds[THREADS > 64 ? 2 * (THREADS / 64) * 4 : ROWS * THREADS * N];
+    constexpr bool HELD = N * THREADS <= HELD_DIM, AHEAD = HELD || (WHOLE && V == 8);
+    __shared__ float lds[ROWS == 1 ? 2 * (THREADS / 64) * 4 : WIDTH * N];
     extern __shared__ __attribute__((aligned(16))) float column_sums[];
     int turn = 0;
     const int dim = a.p.dim, stride = gridDim.x * ROWS;
     const float inverse_dim = 1.0f / dim;
     const bool output_layer = a.d_h && a.p.output_norm == RLT_NORM_LAYER, branch_layer = a.branch && a.p.branch_norm == RLT_NORM_LAYER;
     float bw[N], bb[N], ow[N], scale[N];
-    auto output_parameters = [&] { load_parameters<V, K, THREADS>(a.p.output_weights, 1.0f, dim, ow); };
+    auto output_parameters = [&] { load_parameters<V, K, THREADS, WHOLE>(a.p.output_weights, 1.0f, dim, ow); };
     auto branch_parameters = [&] {
-        load_parameters<V, K, THREADS>(a.p.branch_weights, 1.0f, dim, bw); load_parameters<V, K, THREADS>(BIASES ? a.p.branch_biases : nullptr, 0.0f, dim, bb);
-        load_parameters<V, K, THREADS>(a.p.residual_scale, 1.0f, dim, scale);
+        load_parameters<V, K, THREADS, WHOLE>(a.p.branch_weights, 1.0f, dim, bw); load_parameters<V, K, THREADS, WHOLE>(BIASES ? a.p.branch_biases : nullptr, 0.0f, dim, bb);
+        load_parameters<V, K, THREADS, WHOLE>(a.p.residual_scale, 1.0f, dim, scale);
     };
     if (HELD) { output_parameters(); branch_parameters(); }
     // Sum j of this thread's columns: in a register, or in LDS, 16 bytes of every thread side by side. 160 KB hold four sums of the widest rows and not the fifth.
@@ -258,30 +304,32 @@ template <typename T, int V, int K, int THREADS, bool BIASES> __global__ __launc
 #define NORM_SUM(j) std::integral_constant<int, j>{}
     Raw<T, V, K> next_e{}, next_y{}, next_d{}, next_u{}, next_g{};
     auto ask = [&](int row) {
+        const int dim = ROWS == 1 || row < a.rows ? a.p.dim : 0;      // rows that a workgroup has no more: zeros, which add nothing
         if (a.d_h) {
-            load_raw<V, K, THREADS>((const T*)a.d_h + (size_t)row * a.lddh, dim, next_e);
-            load_raw<V, K, THREADS>((const T*)a.y + (size_t)row * a.ldy, dim, next_y);
+            load_raw<V, K, THREADS, WHOLE>((const T*)a.d_h + (size_t)row * a.lddh, dim, next_e);
+            load_raw<V, K, THREADS, WHOLE>((const T*)a.y + (size_t)row * a.ldy, dim, next_y);
         }
-        if (a.d_y) load_raw<V, K, THREADS>((const T*)a.d_y + (size_t)row * a.lddy, dim, next_d);
+        if (a.d_y) load_raw<V, K, THREADS, WHOLE>((const T*)a.d_y + (size_t)row * a.lddy, dim, next_d);
         if (a.branch) {
-            load_raw<V, K, THREADS>((const T*)a.branch + (size_t)row * a.ldb, dim, next_u);
-            if (a.gate) load_raw<V, K, THREADS>((const T*)a.gate + (size_t)row * a.ldg, dim, next_g);
+            load_raw<V, K, THREADS, WHOLE>((const T*)a.branch + (size_t)row * a.ldb, dim, next_u);
+            if (a.gate) load_raw<V, K, THREADS, WHOLE>((const T*)a.gate + (size_t)row * a.ldg, dim, next_g);
         }
     };
-    const int first = blockIdx.x * ROWS + row_of<THREADS>();
-    if (AHEAD && first < a.rows) ask(first);
-    for (int row = first; row < a.rows; row += stride) {
+    if (AHEAD) ask(blockIdx.x * ROWS + row_of<THREADS, WIDTH>());
+    for (int first = blockIdx.x * ROWS; first < a.rows; first += stride) {      // all rows of a workgroup at once: they share its barriers
+        const int row = first + row_of<THREADS, WIDTH>();
+        const bool here = ROWS == 1 || row < a.rows;
         float d[N], e[N], y[N], u[N], g[N];      // d: the gradient that reaches the residual stream
         if (!AHEAD) ask(row);
-        unpack<T, V, K>(next_e, e); unpack<T, V, K>(next_y, y); unpack<T, V, K>(next_d, d); unpack<T, V, K>(next_u, u); unpack<T, V, K>(next_g, g);
-        if (AHEAD && row + stride < a.rows) ask(row + stride);
+        unpack<V, K, THREADS, WHOLE>(next_e, dim, e); unpack<V, K, THREADS, WHOLE>(next_y, dim, y); unpack<V, K, THREADS, WHOLE>(next_d, dim, d); unpack<V, K, THREADS, WHOLE>(next_u, dim, u); unpack<V, K, THREADS, WHOLE>(next_g, dim, g);
+        if (AHEAD && first + stride < a.rows) ask(row + stride);
         if (output_layer || branch_layer) {
             float s[2] = {0.0f, 0.0f};
 #pragma unroll
             for (int i = 0; i < N; i++) { s[0] += y[i]; s[1] += u[i]; }
-            row_sums<THREADS>(s, lds, turn);
-            if (output_layer) subtract<V, K, THREADS>(y, s[0] * inverse_dim, dim);
-            if (branch_layer) subtract<V, K, THREADS>(u, s[1] * inverse_dim, dim);
+            row_sums<THREADS, WIDTH>(s, lds, turn);
+            if (output_layer) subtract<V, K, THREADS, WHOLE>(y, s[0] * inverse_dim, dim);
+            if (branch_layer) subtract<V, K, THREADS, WHOLE>(u, s[1] * inverse_dim, dim);
         }
         if (!HELD) { output_parameters(); __builtin_amdgcn_sched_barrier(0); }
         float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};      // of y^2, of the output norm's gradient times y, of that gradient, of branch^2
@@ -290,7 +338,7 @@ template <typename T, int V, int K, int THREADS, bool BIASES> __global__ __launc
             const float w = e[i] * ow[i];
             s[0] = fmaf(y[i], y[i], s[0]); s[1] = fmaf(w, y[i], s[1]); s[2] += w; s[3] = fmaf(u[i], u[i], s[3]);
         }
-        row_sums<THREADS>(s, lds, turn);
+        row_sums<THREADS, WIDTH>(s, lds, turn);
         if (a.d_h) {
             const bool none = a.p.output_norm == RLT_NORM_NONE;
             const float inverse = none ? 1.0f : 1.0f / sqrtf(s[0] * inverse_dim + a.p.epsilon), along = none ? 0.0f : inverse * s[1] * inverse_dim, mean = output_layer ? s[2] * inverse_dim : 0.0f;
@@ -303,9 +351,9 @@ template <typename T, int V, int K, int THREADS, bool BIASES> __global__ __launc
             if (!HELD) __builtin_amdgcn_sched_barrier(0);
             add(NORM_SUM(OUTPUT_W), y);
             if constexpr (BIASES) add(NORM_SUM(OUTPUT_B), e);
-            if (mean != 0.0f) zero_beyond<V, K, THREADS>(d, dim);      // the sums that follow take no column beyond dim
+            if (mean != 0.0f) zero_beyond<V, K, THREADS, WHOLE>(d, dim);      // the sums that follow take no column beyond dim
         }
-        if (a.d_x) store_row<V, K, THREADS>((T*)a.d_x + (size_t)row * a.lddx, dim, d);
+        if (a.d_x && here) store_row<V, K, THREADS, WHOLE>((T*)a.d_x + (size_t)row * a.lddx, dim, d);
         if (a.branch) {
             const bool none = a.p.branch_norm == RLT_NORM_NONE;
             const float inverse = none ? 1.0f : 1.0f / sqrtf(s[3] * inverse_dim + a.p.epsilon);
@@ -323,15 +371,15 @@ template <typename T, int V, int K, int THREADS, bool BIASES> __global__ __launc
             }
             add(NORM_SUM(SCALE), y); add(NORM_SUM(BRANCH_W), d);
             if constexpr (BIASES) add(NORM_SUM(BRANCH_B), g);
-            if (a.d_gate) store_row<V, K, THREADS>((T*)a.d_gate + (size_t)row * a.lddg, dim, slope);
+            if (a.d_gate && here) store_row<V, K, THREADS, WHOLE>((T*)a.d_gate + (size_t)row * a.lddg, dim, slope);
             if (a.d_branch) {
                 if (!none) {
-                    row_sums<THREADS>(t, lds, turn);
+                    row_sums<THREADS, WIDTH>(t, lds, turn);
                     const float along = t[0] * inverse_dim, mean = branch_layer ? t[1] * inverse_dim : 0.0f;
 #pragma unroll
                     for (int i = 0; i < N; i++) e[i] = inverse * (e[i] - u[i] * along - mean);
                 }
-                store_row<V, K, THREADS>((T*)a.d_branch + (size_t)row * a.lddb, dim, e);
+                if (here) store_row<V, K, THREADS, WHOLE>((T*)a.d_branch + (size_t)row * a.lddb, dim, e);
             }
         }
     }
@@ -347,7 +395,7 @@ template <typename T, int V, int K, int THREADS, bool BIASES> __global__ __launc
 #pragma unroll
                 for (int i = 0; i < V; i++) lds[(threadIdx.x / THREADS) * THREADS * N + (k * THREADS + threadIdx.x % THREADS) * V + i] = sums[HELD ? j : 0][k * V + i];
             __syncthreads();
-            for (int c = threadIdx.x; c < dim; c += WORKGROUP<THREADS>) {
+            for (int c = threadIdx.x; c < dim; c += WIDTH) {
                 float s = 0.0f;
 #pragma unroll
                 for (int r = 0; r < ROWS; r++) s += lds[r * THREADS * N + c];
@@ -390,46 +438,46 @@ __global__ __launch_bounds__(1024) void norm_sum_kernel(const float* __restrict_
 // threads that share a row in the backward pass, eight columns each, or sixteen
 int backward_threads(int dim) { return dim <= 128 ? 16 : dim <= 512 ? 64 : dim <= 1024 ? 128 : dim <= 2048 ? 256 : 512; }
 int backward_blocks(const rlt_residual_norm* p, int rows) {
-    const int threads = backward_threads(p->dim), at_once = threads <= 64 ? 256 / threads : 1, blocks = (rows + at_once - 1) / at_once;
+    const int threads = backward_threads(p->dim), at_once = threads < 256 ? 256 / threads : 1, blocks = (rows + at_once - 1) / at_once;
     return blocks < 512 ? blocks : 512;
 }
 
-template <typename T, int V> void launch_forward(rlt_rocm_device* device, const NormForward& a) {
+template <typename T, int V, bool WHOLE> void launch_forward(rlt_rocm_device* device, const NormForward& a) {
     const int dim = a.p.dim;
     auto go = [&](auto kernel, int threads) {
         const int workgroup = threads <= 64 ? 256 : threads, at_once = workgroup / threads, blocks = (a.rows + at_once - 1) / at_once;
         hipLaunchKernelGGL(kernel, dim3(blocks < 2048 ? blocks : 2048), dim3(workgroup), 0, device->stream, a);
     };
-    if (dim <= 128) go(norm_forward_kernel<T, V, 8 / V, 16>, 16);
-    else if (dim <= 512) go(norm_forward_kernel<T, V, 8 / V, 64>, 64);
-    else if (dim <= 1024) go(norm_forward_kernel<T, V, 8 / V, 128>, 128);
-    else if (dim <= 2048) go(norm_forward_kernel<T, V, 8 / V, 256>, 256);
-    else if (dim <= 4096) go(norm_forward_kernel<T, V, 8 / V, 512>, 512);
-    else go(norm_forward_kernel<T, V, 8 / V, 1024>, 1024);
+    if (dim <= 128) go(norm_forward_kernel<T, V, 8 / V, 16, WHOLE>, 16);
+    else if (dim <= 512) go(norm_forward_kernel<T, V, 8 / V, 64, WHOLE>, 64);
+    else if (dim <= 1024) go(norm_forward_kernel<T, V, 8 / V, 128, WHOLE>, 128);
+    else if (dim <= 2048) go(norm_forward_kernel<T, V, 8 / V, 256, WHOLE>, 256);
+    else if (dim <= 4096) go(norm_forward_kernel<T, V, 8 / V, 512, WHOLE>, 512);
+    else go(norm_forward_kernel<T, V, 8 / V, 1024, WHOLE>, 1024);
 }
-template <typename T, int V, bool BIASES> int launch_backward(rlt_rocm_device* device, const NormBackward& a) {
+template <typename T, int V, bool BIASES, bool WHOLE> int launch_backward(rlt_rocm_device* device, const NormBackward& a) {
     const int threads = backward_threads(a.p.dim);
     const size_t bytes = a.p.dim > HELD_DIM ? (size_t)(BIASES ? 4 : 3) * MAX_DIM * sizeof(float) : 0;
     hipError_t e = hipSuccess;
     auto go = [&](auto kernel) {
         if (bytes) e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-        if (e == hipSuccess) hipLaunchKernelGGL(kernel, dim3(backward_blocks(&a.p, a.rows)), dim3(threads <= 64 ? 256 : threads), bytes, device->stream, a);
+        if (e == hipSuccess) hipLaunchKernelGGL(kernel, dim3(backward_blocks(&a.p, a.rows)), dim3(threads < 256 ? 256 : threads), bytes, device->stream, a);
     };
-    if (threads == 16) go(norm_backward_kernel<T, V, 8 / V, 16, BIASES>);
-    else if (threads == 64) go(norm_backward_kernel<T, V, 8 / V, 64, BIASES>);
-    else if (threads == 128) go(norm_backward_kernel<T, V, 8 / V, 128, BIASES>);
-    else if (threads == 256) go(norm_backward_kernel<T, V, 8 / V, 256, BIASES>);
-    else if (a.p.dim <= HELD_DIM) go(norm_backward_kernel<T, V, 8 / V, 512, BIASES>);
-    else go(norm_backward_kernel<T, V, 16 / V, 512, BIASES>);
+    if (threads == 16) go(norm_backward_kernel<T, V, 8 / V, 16, BIASES, WHOLE>);
+    else if (threads == 64) go(norm_backward_kernel<T, V, 8 / V, 64, BIASES, WHOLE>);
+    else if (threads == 128) go(norm_backward_kernel<T, V, 8 / V, 128, BIASES, WHOLE>);
+    else if (threads == 256) go(norm_backward_kernel<T, V, 8 / V, 256, BIASES, WHOLE>);
+    else if (a.p.dim <= HELD_DIM) go(norm_backward_kernel<T, V, 8 / V, 512, BIASES, WHOLE>);
+    else go(norm_backward_kernel<T, V, 16 / V, 512, BIASES, WHOLE>);
     RLT_HIP(e);
     return rlt_launch_status(device);
 }
-// vectors of 16 bytes where every tensor's rows start on such boundaries and hold whole vectors
+// whole vectors where every tensor's rows start on 16-byte boundaries and hold such
 template <typename T> void forward(rlt_rocm_device* device, const NormForward& a) {
     constexpr int V = 16 / sizeof(T);
     const bool vectors = a.p.dim % V == 0 && rlt_vectors<T>(a.x, a.ldx) && rlt_vectors<T>(a.branch, a.branch ? a.ldb : 0) && rlt_vectors<T>(a.gate, a.gate ? a.ldg : 0) &&
                          rlt_vectors<T>(a.y, a.y ? a.ldy : 0) && rlt_vectors<T>(a.h, a.h ? a.ldh : 0);
-    if (vectors) launch_forward<T, V>(device, a); else launch_forward<T, 1>(device, a);
+    if (vectors) launch_forward<T, V, true>(device, a); else launch_forward<T, V, false>(device, a);
 }
 template <typename T> int backward(rlt_rocm_device* device, const NormBackward& a) {
     constexpr int V = 16 / sizeof(T);
@@ -437,8 +485,8 @@ template <typename T> int backward(rlt_rocm_device* device, const NormBackward& 
                          rlt_vectors<T>(a.d_y, a.d_y ? a.lddy : 0) && rlt_vectors<T>(a.d_h, a.d_h ? a.lddh : 0) && rlt_vectors<T>(a.d_x, a.d_x ? a.lddx : 0) &&
                          rlt_vectors<T>(a.d_branch, a.d_branch ? a.lddb : 0) && rlt_vectors<T>(a.d_gate, a.d_gate ? a.lddg : 0);
     const bool biases = a.p.branch_biases || a.p.d_branch_biases || a.p.d_output_biases;
-    if (vectors) return biases ? launch_backward<T, V, true>(device, a) : launch_backward<T, V, false>(device, a);
-    return biases ? launch_backward<T, 1, true>(device, a) : launch_backward<T, 1, false>(device, a);
+    if (vectors) return biases ? launch_backward<T, V, true, true>(device, a) : launch_backward<T, V, false, true>(device, a);
+    return biases ? launch_backward<T, V, true, false>(device, a) : launch_backward<T, V, false, false>(device, a);
 }
 
 bool described(const rlt_residual_norm* p) {
