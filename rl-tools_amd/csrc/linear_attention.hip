@@ -23,6 +23,7 @@ struct Walk {
     float score_scale, read_scale, added_scale;
     int batch, heads, steps, key, value, segments, segment_steps;
     int state_key, state_value;   // strides of the state in memory
+    int last_wanted;              // STATE: the last segment's state too
 };
 
 template <typename T> __device__ __forceinline__ T* at(const Part& p, int t, int b, int h) {
@@ -107,6 +108,8 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
     int l = lane & 15, quarter = lane >> 4;
     const int length = a.lengths ? min(max(a.lengths[b], 0), a.steps) : a.steps;
     const float log2_decay = a.log_decay[h] * 1.44269504088896341f;
+    const bool last = segment == (REVERSE ? 0 : a.segments - 1);      // of the walk
+    if (STATE && last && !a.last_wanted) return;                      // no segment starts from the state after it
     const int begin = segment * a.segment_steps, end = min(begin + a.segment_steps, a.steps);
 
     // state: tile k, element r of this lane is row 16 k + 4 quarter + r, column 16 (TILES wave + tile) + l
@@ -230,6 +233,9 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
     float total = 0.0f;                                 // SLOPE
     int weights_n = -1; uint64_t weights_resets = 0;    // the steps and the resets that the weights in LDS are for
     int counted = 0; bool forgotten = false;            // STATE
+    // no state before the first steps, none asked for after the last: the products are left out
+    bool nothing = !STATE && !a.entry;
+    const bool last_unread = !STATE && !a.exit && !(SLOPE && a.d_final && last);
     int t0 = REVERSE ? max(begin, end - CHUNK) : begin, stop = REVERSE ? end : min(begin + CHUNK, end);
     fetch_chunk(t0, stop);
     while (true) {
@@ -324,6 +330,7 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
                     out[tile][ot] = rlt_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
                     if constexpr (SLOPE) out_slope[tile][ot] = rlt_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
                 }
+            if (!nothing) {
 #pragma unroll
             for (int block = 0; block < KEY_BLOCKS; block++) {
                 Vector q[4];
@@ -364,6 +371,7 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
                         for (int r = 0; r < 4; r++) out[tile][ot][r] = weight != 0.0f ? out[tile][ot][r] * weight : 0.0f;
                     } else out[tile][ot] *= weight;
                 }
+            }
             }
             if constexpr (L::OVER) rlt_lds_barrier();      // the queries have been read
 #pragma unroll
@@ -422,7 +430,8 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
             }
         }
         // the state after the chunk
-        if (n > 0) {
+        if (n > 0 && !(done && last_unread)) {
+            nothing = false;
             const float f = power(log2_decay, REVERSE ? n - 1 : n);
             counted += n; forgotten |= resets != 0;
 #pragma unroll
@@ -495,7 +504,7 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
     }
     if constexpr (STATE) { if (threadIdx.x == 0 && half == 0) a.factors[item] = make_float2(forgotten ? 0.0f : power(log2_decay, counted), (float)counted); }
     if constexpr (SLOPE && !STATE) {
-        if (a.d_final && segment == a.segments - 1) {
+        if (a.d_final && last) {
             const float* const from = a.d_final + (size_t)pair * a.key * a.value;
             over_state([&](int tile, int k, int r, bool there, int i) { if (there) total = fmaf(from[i], slope[tile][k][r], total); });
         }
@@ -518,11 +527,12 @@ template <bool SLOPES> __global__ __launch_bounds__(256) void scan_kernel(const 
     const int pair = blockIdx.y, e = blockIdx.x * 256 + threadIdx.x;
     if (e >= elements) return;
     float carry = initial ? initial[(size_t)pair * elements + e] : 0.0f, carry_slope = 0.0f;
+    const int added = final ? segments : segments - 1;      // segments whose own states are there
     for (int i0 = 0; i0 < segments; i0 += AHEAD) {
         float local[AHEAD], local_slope[AHEAD];
 #pragma unroll
         for (int j = 0; j < AHEAD; j++) {
-            const int i = min(i0 + j, segments - 1);
+            const int i = min(i0 + j, added - 1);
             const size_t at = ((size_t)pair * segments + (reverse ? segments - 1 - i : i)) * elements + e;
             local[j] = locals[at];
             if (SLOPES) local_slope[j] = slopes[at];
@@ -531,7 +541,7 @@ template <bool SLOPES> __global__ __launch_bounds__(256) void scan_kernel(const 
         for (int j = 0; j < AHEAD; j++)
             if (i0 + j < segments) {
                 const size_t p = (size_t)pair * segments + (reverse ? segments - 1 - i0 - j : i0 + j), at = p * elements + e;
-                const float2 f = factors[p];
+                const float2 f = i0 + j < added ? factors[p] : make_float2(0.0f, 0.0f);
                 if (SLOPES) {
                     slopes[at] = carry_slope;
                     carry_slope = f.x == 0.0f ? local_slope[j] : fmaf(f.x, fmaf(f.y, carry, carry_slope), local_slope[j]);
@@ -704,7 +714,7 @@ Walk walk_of(const rlt_linear_attention* p, const uint8_t* reset, const int32_t*
 // states that the segments of `a` start from, in scratch memory
 template <typename T, bool REVERSE, bool SLOPE> int segment_states(rlt_rocm_device* device, const Walk& a, const float* initial, float* final, float* states, float* slopes, float2* factors) {
     Walk s = a;
-    s.entry = nullptr; s.exit = states; s.exit_slope = slopes; s.factors = factors;
+    s.entry = nullptr; s.exit = states; s.exit_slope = slopes; s.factors = factors; s.last_wanted = final != nullptr;
     int rc = walk<T, T, REVERSE, SLOPE, true>(device, s);
     if (rc) return rc;
     const int elements = a.key * a.value, pairs = a.batch * a.heads;
