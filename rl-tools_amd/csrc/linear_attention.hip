@@ -170,26 +170,49 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
             int thread = threadIdx.x;
             asm volatile("" : "+v"(thread));
             const int channel = from + (thread % (ACROSS / V)) * V, first = thread / (ACROSS / V), most = stop - t0 - 1;
-            if (FULL || p.vectors) {
+            if (FULL) {
 #pragma unroll
                 for (int round = 0; round < N; round++) {
                     const int step = first + round * STEPS;
-                    to[round] = *reinterpret_cast<const Bytes16*>(row0 + min(step, most) * p.step + (FULL ? channel : min(channel, width - V)));
-                    if (step > most || (!FULL && channel >= width)) to[round] = Bytes16{};
+                    to[round] = *reinterpret_cast<const Bytes16*>(row0 + min(step, most) * p.step + channel);
+                    if (step > most) to[round] = Bytes16{};
                 }
+            } else if (width >= V) {      // dropped by settle, when it is needed: no load is waited for here. Vectors start at any element, which the memory instructions allow.
+                typedef T Anywhere __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+#pragma unroll
+                for (int round = 0; round < N; round++) to[round] = *reinterpret_cast<const Anywhere*>(row0 + min(first + round * STEPS, most) * p.step + min(channel, width - V));
             } else {
 #pragma unroll
                 for (int round = 0; round < N; round++) {
-                    const int step = first + round * STEPS;
-                    const T* const row = row0 + min(step, most) * p.step;
+                    const T* const row = row0 + min(first + round * STEPS, most) * p.step;
 #pragma unroll
-                    for (int c = 0; c < V; c++) to[round][c] = row[min(channel + c, width - 1)];
-#pragma unroll
-                    for (int c = 0; c < V; c++) if (step > most || channel + c >= width) to[round][c] = (T)0.0f;
+                    for (int c = 0; c < V; c++) to[round][c] = channel + c < width ? row[channel + c] : (T)0.0f;
                 }
             }
         }
     };
+    // !FULL: what fetch has read from elsewhere, steps beyond the chunk's n and channels beyond the width
+    auto settle = [&](int from, int width, int n, auto& to, auto across) {
+        constexpr int ACROSS = decltype(across)::value, N = CHUNK * ACROSS / (V * L::THREADS), STEPS = L::THREADS * V / ACROSS;
+        int thread = threadIdx.x;
+        asm volatile("" : "+v"(thread));
+        const int channel = from + (thread % (ACROSS / V)) * V, first = thread / (ACROSS / V), beyond = width >= V ? channel + V - width : 0;
+        if (beyond > 0 && beyond < V) {
+#pragma unroll
+            for (int round = 0; round < N; round++) to[round] = __builtin_bit_cast(Bytes16, __builtin_bit_cast(unsigned __int128, to[round]) >> (beyond * 8 * (int)sizeof(T)));      // elements move down to their channels, zeros behind them
+        }
+#pragma unroll
+        for (int round = 0; round < N; round++) if (first + round * STEPS >= n || beyond >= V) to[round] = Bytes16{};
+    };
+    auto settle_chunk = [&](int n) {
+        if constexpr (!FULL) {
+            if constexpr (!STATE) settle(0, a.key, n, next_q, whole);
+            settle(0, a.key, n, next_k, whole);
+            settle(part0, a.value, n, next_v, columns);
+            if constexpr (SLOPE && !STATE) settle(part0, a.value, n, next_with, columns);
+        }
+    };
+    auto steps_of = [&](int t0, int stop) { return min(max(min(length, stop) - t0, 0), CHUNK); };
     auto fetch_chunk = [&](int t0, int stop) {
         stop = min(stop, length);
         if constexpr (!STATE) fetch(a.q, 0, a.key, t0, stop, next_q, whole);
@@ -244,6 +267,8 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
             asm volatile("" : "+v"(quarter));
         }
         uint64_t resets = __ballot(next_reset != 0);
+        int n = steps_of(t0, stop);
+        settle_chunk(n);
         if (resets & ~1ull) {
             // A step's weight of zero keeps other episodes out of sums of products as long as their values are finite. Where some are not, the chunk ends at its first reset (REVERSE: begins at its last).
             float zero = 0.0f;
@@ -266,9 +291,10 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
                 if (REVERSE) t0 += 63 - __builtin_clzll(resets); else stop = t0 + __builtin_ctzll(resets & ~1ull);
                 fetch_chunk(t0, stop);
                 resets = __ballot(next_reset != 0);
+                n = steps_of(t0, stop);
+                settle_chunk(n);
             }
         }
-        const int n = min(max(min(length, stop) - t0, 0), CHUNK);
         const int last_reset = resets ? 63 - __builtin_clzll(resets) : -1, first_reset = resets ? __builtin_ctzll(resets) : CHUNK;
         if (n != weights_n || resets != weights_resets) {
             weights_n = n; weights_resets = resets;
@@ -299,10 +325,10 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
                 if (tile >= 10) break;
                 rlt_f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f}, y = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int block = 0; block < KEY_BLOCKS; block++) x = multiply(row_operand(L::K, L::ROW, 16 * st + l, block), row_operand(L::Q, L::ROW, 16 * ot + l, block), x);
+                for (int block = 0; block < KEY_BLOCKS; block++) if (FULL || 32 * block < a.key) x = multiply(row_operand(L::K, L::ROW, 16 * st + l, block), row_operand(L::Q, L::ROW, 16 * ot + l, block), x);
                 if constexpr (SLOPE) {
 #pragma unroll
-                    for (int block = 0; block < L::COLUMNS / 32; block++) y = multiply(row_operand(L::V, L::COLUMN_ROW, 16 * st + l, block), row_operand(L::W, L::COLUMN_ROW, 16 * ot + l, block), y);
+                    for (int block = 0; block < L::COLUMNS / 32; block++) if (FULL || part0 + 32 * block < a.value) y = multiply(row_operand(L::V, L::COLUMN_ROW, 16 * st + l, block), row_operand(L::W, L::COLUMN_ROW, 16 * ot + l, block), y);
                 }
                 const int i = 16 * ot + l;
                 const float* const weight = score_weights + (REVERSE ? 16 * (st - ot) + 4 * quarter - l : 16 * (ot - st) + l - 4 * quarter);
@@ -333,6 +359,7 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
             if (!nothing) {
 #pragma unroll
             for (int block = 0; block < KEY_BLOCKS; block++) {
+                if (!FULL && 32 * block >= a.key) break;
                 Vector q[4];
 #pragma unroll
                 for (int ot = 0; ot < 4; ot++) q[ot] = tiled_operand(L::Q, 16 * ot + l, block);
@@ -420,10 +447,12 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
                         if (n < CHUNK && i >= n) x = rlt_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
                         O* const here = to + (int64_t)(16 * ot) * a.out.step + 16 * tile;
                         if (FULL) *reinterpret_cast<OutQuad*>(here) = __builtin_convertvector(x, OutQuad);
-                        else if (a.out.vectors) { if (c0 < a.value) *reinterpret_cast<OutQuad*>(here) = __builtin_convertvector(x, OutQuad); }
-                        else {
+                        else if (c0 + 4 <= a.value) {
+                            typedef O Anywhere __attribute__((ext_vector_type(4), aligned(sizeof(O))));
+                            *reinterpret_cast<Anywhere*>(here) = __builtin_convertvector(x, Anywhere);
+                        } else {
 #pragma unroll
-                            for (int r = 0; r < 4; r++) if (c0 + r < a.value) here[r] = (O)x[r];
+                            for (int r = 0; r < 3; r++) if (c0 + r < a.value) here[r] = (O)x[r];
                         }
                     }
                 }
@@ -464,6 +493,7 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
                         const Cut<T, ADDED_CUTS> y(lagged);
 #pragma unroll
                         for (int k = 0; k < KEY_TILES; k++) {      // one key operand in registers at a time
+                            if (!FULL && 16 * k >= a.key) break;
                             key[0] = column_operand(L::K, L::ROW, k, block);
 #pragma unroll
                             for (int p = 0; p < ADDED_CUTS; p++) {
