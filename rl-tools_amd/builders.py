@@ -739,3 +739,140 @@ class Td3SequenceOnBackend:
 
     def ages(self):
         return [int(x.numpy()[0]) for x in (self.actor.age, self.critics[0].age, self.critics[1].age)]
+
+
+class SequenceBlocks:
+    """A stack of gated residual blocks over sequences [steps x batch x width], fp32: what takes a GRU's place between the dense layers of a recurrent policy or critic. Per block l
+        q, k, v, gate = W_in h + b_in (one product; the four are parts of its rows),   o = linear attention(q, k, v),   p = dropout(W_out o + b_out),
+        y = x + residual_scale * sigmoid(gate) * branch_norm(p),   the next block's h = output_norm(y);   h of the first block: input_norm(x).
+    Sequences train it (forward, backward, update); step() is one step of a rollout with the blocks' states, and gives what forward gives without dropout. Every device address is fixed when
+    the object is built, so that forward + backward + update can be captured into a graph."""
+
+    @staticmethod
+    def shapes(width, heads, kv_heads, blocks):
+        """name -> shape, in the order of the flat arenas"""
+        key = width // heads
+        s = {"input_weights": (width,), "input_biases": (width,)}
+        for l in range(blocks):
+            s.update({f"in_w{l}": (2 * width + 2 * kv_heads * key, width), f"in_b{l}": (2 * width + 2 * kv_heads * key,), f"log_decay{l}": (heads,), f"out_w{l}": (width, width), f"out_b{l}": (width,),
+                      f"branch_weights{l}": (width,), f"branch_biases{l}": (width,), f"output_weights{l}": (width,), f"output_biases{l}": (width,), f"residual_scale{l}": (width,)})
+        return s
+
+    @staticmethod
+    def random(rng, width, heads, kv_heads, blocks):
+        """parameters of a new stack: decays from a short to a long memory over the heads"""
+        p = {}
+        for name, shape in SequenceBlocks.shapes(width, heads, kv_heads, blocks).items():
+            if len(shape) == 2:
+                a = rng.uniform(-1, 1, shape) / np.sqrt(shape[1])
+            elif name.startswith("log_decay"):
+                a = np.log1p(-2.0 ** -np.linspace(2, 6, heads))
+            else:
+                a = np.ones(shape) if "weights" in name or "scale" in name else np.zeros(shape)
+            p[name] = a.astype(np.float32)
+        return p
+
+    def __init__(self, backend, params, steps, batch, width, heads, kv_heads, blocks, dropout=0.0, seed=0, norm="rms", epsilon=1e-5):
+        assert width % heads == 0 and heads % kv_heads == 0
+        self.backend, self.steps, self.batch, self.width, self.blocks, self.rate, self.seed = backend, steps, batch, width, blocks, dropout, seed
+        key, rows, z = width // heads, steps * batch, backend.zeros
+        parts, self.row = (0, width, width + kv_heads * key, width + 2 * kv_heads * key), 2 * width + 2 * kv_heads * key      # where q, k, v and the gate start in a row of the input product
+        shapes = self.shapes(width, heads, kv_heads, blocks)
+        self.offsets, total = {}, 0
+        for name, shape in shapes.items():
+            self.offsets[name] = total
+            total += (int(np.prod(shape)) + 3) // 4 * 4      # 16-byte boundaries
+        flat = np.zeros(total, np.float32)
+        for name, shape in shapes.items():
+            flat[self.offsets[name]:self.offsets[name] + int(np.prod(shape))] = np.asarray(params[name], np.float32).reshape(shape).ravel()
+        self.params, self.total = backend.array(flat), total
+        self.grads, self.m, self.v, self.age = z((total,)), z((total,)), z((total,)), backend.array(np.array([1], np.uint32))
+        self.grad_views = {name: ArenaView(self.grads, self.offsets[name], shape) for name, shape in shapes.items()}
+        self.param_views = {name: ArenaView(self.params, self.offsets[name], shape) for name, shape in shapes.items()}
+        P, G = (lambda name: self.params.offset(self.offsets[name])), (lambda name: self.grads.offset(self.offsets[name]))
+        adam = [capi.AdamTensor(P(n), G(n), self.m.offset(o), self.v.offset(o), None, int(np.prod(shapes[n])), 1 if len(shapes[n]) == 2 else 2) for n, o in self.offsets.items()]
+        self.adam, self.n_adam = (capi.AdamTensor * len(adam))(*adam), len(adam)
+
+        self.x, self.reset = z((steps, batch, width)), z((steps, batch), np.uint8)
+        self.h, self.y = [z((rows, width)) for _ in range(blocks + 1)], [z((rows, width)) for _ in range(blocks)]
+        self.projected, self.o, self.p = [z((rows, self.row)) for _ in range(blocks)], [z((rows, width)) for _ in range(blocks)], [z((rows, width)) for _ in range(blocks)]
+        self.d_h, self.d_stream, self.d_p, self.d_o, self.d_projected = z((rows, width)), z((rows, width)), z((rows, width)), z((rows, width)), z((rows, self.row))
+        self.states = [z((batch, heads, key, key)) for _ in range(blocks)]
+        state_rows = [z((batch, n)) for n in (width, self.row, width, width, width)]      # h, the input product, o, p, y of one step
+        self.step_x, self.step_reset = z((batch, width)), z((batch,), np.uint8)
+        self.step_h, self.step_projected, self.step_o, self.step_p, self.step_y = state_rows
+
+        def views(projected, step_stride):
+            return [capi.HeadView(projected.offset(start), step_stride, self.row, key) for start in parts[:3]]
+        self.in_layer, self.out_layer, self.attention, self.norm, self.gate_at = [], [], [], [], parts[3]
+        norm = capi.NORM[norm]
+        self.input_norm = capi.ResidualNorm(0, width, norm, norm, capi.ACT["sigmoid"], epsilon, None, None, P("input_weights"), P("input_biases"), None, None, None, G("input_weights"), G("input_biases"), None)
+        for l in range(blocks):
+            n = lambda name: f"{name}{l}"
+            self.in_layer.append(capi.DenseLayer(P(n("in_w")), P(n("in_b")), G(n("in_w")), G(n("in_b")), self.projected[l].ptr, None, width, self.row, capi.ACT["identity"], 0))
+            self.out_layer.append(capi.DenseLayer(P(n("out_w")), P(n("out_b")), G(n("out_w")), G(n("out_b")), self.p[l].ptr, None, width, width, capi.ACT["identity"], 0))
+            self.attention.append(capi.LinearAttention(P(n("log_decay")), key ** -0.5, 0, batch, heads, kv_heads, key, key, 0))
+            self.norm.append(capi.ResidualNorm(0, width, norm, norm, capi.ACT["sigmoid"], epsilon, *[P(n(a)) for a in ("branch_weights", "branch_biases", "output_weights", "output_biases", "residual_scale")],
+                                               *[G(n(a)) for a in ("branch_weights", "branch_biases", "output_weights", "output_biases", "residual_scale")]))
+        sequence = lambda a: capi.HeadView(a.ptr, batch * width, width, key)
+        self.qkv, self.d_qkv = [views(a, batch * self.row) for a in self.projected], views(self.d_projected, batch * self.row)
+        self.o_views, self.d_o_view = [sequence(a) for a in self.o], sequence(self.d_o)
+        self.step_qkv, self.step_o_view = views(self.step_projected, 0), capi.HeadView(self.step_o.ptr, 0, width, key)
+        lib = backend.device.lib
+        nbytes = max([lib.rlt_rocm_linear_attention_workspace_bytes(C.byref(a), steps, k) for a in self.attention for k in (0, 1)] + [lib.rlt_rocm_residual_norm_workspace_bytes(C.byref(a), rows) for a in self.norm])
+        self._workspace = backend.device.empty((max(int(nbytes), 16),), np.uint8)
+        self.workspace = (self._workspace.ptr, int(nbytes))
+
+    def zero_gradient(self):
+        self.backend.call("fill_f32", self.grads.ptr, 1, self.total, self.total, 0.0)
+
+    def _dropout(self, x, stream):
+        if self.rate > 0.0:
+            self.backend.call("dropout", 0, x.ptr, self.width, None, 0, x.ptr, self.width, self.steps * self.batch, self.width, self.rate, self.seed, stream)
+
+    def forward(self, stream=0, reset=True, dropout=True):
+        """x -> h[-1], over all steps from states of zeros; `reset` (of this object) ends episodes inside the sequences. stream: the first of `blocks` dropout streams, given to backward again."""
+        b, w, rows, call = self.backend, self.width, self.steps * self.batch, self.backend.call
+        r = self.reset.ptr if reset else None
+        x = self.x
+        call("residual_norm_forward", C.byref(self.input_norm), x.ptr, w, None, 0, None, 0, None, 0, self.h[0].ptr, w, rows)
+        for l in range(self.blocks):
+            call("dense_forward", C.byref(self.in_layer[l]), self.h[l].ptr, w, None, 0, rows)
+            call("linear_attention_forward", C.byref(self.attention[l]), *self.qkv[l], self.o_views[l], None, self.states[l].ptr, r, None, self.steps, *self.workspace)
+            call("dense_forward", C.byref(self.out_layer[l]), self.o[l].ptr, w, None, 0, rows)
+            if dropout:
+                self._dropout(self.p[l], stream + l)
+            call("residual_norm_forward", C.byref(self.norm[l]), x.ptr, w, self.p[l].ptr, w, self.projected[l].offset(self.gate_at), self.row, self.y[l].ptr, w, self.h[l + 1].ptr, w, rows)
+            x = self.y[l]
+        return self.h[-1]
+
+    def backward(self, d_output, stream=0, reset=True):
+        """From the gradient with respect to h[-1] (of the last forward call) to those of the parameters (added to `grads`) and of x (d_stream)."""
+        w, rows, call = self.width, self.steps * self.batch, self.backend.call
+        r = self.reset.ptr if reset else None
+        d_h, d_y = d_output, None
+        for l in reversed(range(self.blocks)):
+            call("residual_norm_backward", C.byref(self.norm[l]), self.p[l].ptr, w, self.projected[l].offset(self.gate_at), self.row, self.y[l].ptr, w, d_y.ptr if d_y else None, w, d_h.ptr, w,
+                 self.d_stream.ptr, w, self.d_p.ptr, w, self.d_projected.offset(self.gate_at), self.row, rows, 1, *self.workspace)
+            self._dropout(self.d_p, stream + l)
+            call("dense_backward_full", C.byref(self.out_layer[l]), self.o[l].ptr, w, self.d_p.ptr, w, self.d_o.ptr, w, rows)
+            call("linear_attention_backward", C.byref(self.attention[l]), *self.qkv[l], self.d_o_view, *self.d_qkv, None, None, None, self.grad_views[f"log_decay{l}"].ptr, 1, r, None, self.steps, *self.workspace)
+            call("dense_backward_full", C.byref(self.in_layer[l]), self.h[l].ptr, w, self.d_projected.ptr, self.row, self.d_h.ptr, w, rows)
+            d_h, d_y = self.d_h, self.d_stream
+        call("residual_norm_backward", C.byref(self.input_norm), None, 0, None, 0, self.x.ptr, w, d_y.ptr if d_y else None, w, d_h.ptr, w, self.d_stream.ptr, w, None, 0, None, 0, rows, 1, *self.workspace)
+
+    def update(self, adam):
+        self.backend.call("adam_step", self.adam, self.n_adam, C.byref(adam), self.age.ptr, 0.0, None)
+
+    def step(self):
+        """One step of every row: step_x -> step_h, the blocks' `states` in place; step_reset drops a row's states before it."""
+        w, n, call = self.width, self.batch, self.backend.call
+        x = self.step_x
+        call("residual_norm_forward", C.byref(self.input_norm), x.ptr, w, None, 0, None, 0, None, 0, self.step_h.ptr, w, n)
+        for l in range(self.blocks):
+            call("dense_evaluate", C.byref(self.in_layer[l]), self.step_h.ptr, w, self.step_projected.ptr, self.row, n)
+            call("linear_attention_step", C.byref(self.attention[l]), *self.step_qkv, self.step_o_view, self.states[l].ptr, self.states[l].ptr, self.step_reset.ptr)
+            call("dense_evaluate", C.byref(self.out_layer[l]), self.step_o.ptr, w, self.step_p.ptr, w, n)
+            call("residual_norm_forward", C.byref(self.norm[l]), x.ptr, w, self.step_p.ptr, w, self.step_projected.offset(self.gate_at), self.row, self.step_y.ptr, w, self.step_h.ptr, w, n)
+            x = self.step_y
+        return self.step_h
