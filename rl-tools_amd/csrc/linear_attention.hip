@@ -539,6 +539,7 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
             over_state([&](int tile, int k, int r, bool there, int i) { if (there) total = fmaf(from[i], slope[tile][k][r], total); });
         }
         total = rlt_wave_sum(total);
+        asm volatile("" : "+v"(total));      // the last exchange stays ahead of the barrier
         rlt_lds_barrier();
         if (lane == 0) flags[wave] = total;
         rlt_lds_barrier();
