@@ -17,7 +17,7 @@ struct Walk {
     float* exit;                  // state that it ends with (NULL: not wanted), the same
     const float* entry_slope; float* exit_slope;
     const float* d_final;         // SLOPE: gradient with respect to the final state (NULL: zeros)
-    float* partial;               // SLOPE: [rows x heads x segments]
+    double* partial;              // SLOPE: [rows x heads x segments]
     float2* factors;              // STATE: what a segment multiplies the state by (0: it forgets), and its steps
     const uint8_t* reset; const int32_t* lengths;
     float score_scale, read_scale, added_scale;
@@ -61,8 +61,15 @@ template <int PARTS> struct Cut<float, PARTS> {
 };
 template <typename T, int PARTS> constexpr int CUTS = sizeof(T) == 4 ? 1 : PARTS;
 
-// decay^n; n = 0 gives 1 also for a decay of zero
-__device__ __forceinline__ float power(float log2_decay, int n) { return n == 0 ? 1.0f : __builtin_amdgcn_exp2f(log2_decay * (float)n); }
+// decay^n; n = 0 gives 1 also for a decay of zero. The logarithm to the base of 2 is a sum of two numbers: one alone is off by 2^-24 of itself, its n-fold by that of n times as much, and every row and step would meet the same error.
+struct Log2 {
+    float high, low;
+    __device__ __forceinline__ explicit Log2(float log_decay) : high(log_decay * 1.44269504088896341f), low(fmaf(log_decay, 1.44269504088896341f, -high) + log_decay * 1.925963033500721e-8f) {}
+};
+__device__ __forceinline__ float power(const Log2& decay, int n) {
+    const float at = decay.high * (float)n, p = __builtin_amdgcn_exp2f(at), rest = fmaf(decay.high, (float)n, -at) + decay.low * (float)n;
+    return n == 0 ? 1.0f : at > -126.0f ? fmaf(p, rest * 0.6931471805599453f, p) : p;
+}
 
 // Shape of a workgroup for heads of up to D channels: a wavefront owns TILES x 16 of the value columns. SPLIT workgroups share a head's columns where two states would not fit the registers of one: the scores are then
 // formed in each of them.
@@ -107,7 +114,7 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int l = lane & 15, quarter = lane >> 4;
     const int length = a.lengths ? min(max(a.lengths[b], 0), a.steps) : a.steps;
-    const float log2_decay = a.log_decay[h] * 1.44269504088896341f;
+    const Log2 log2_decay(a.log_decay[h]);
     const bool last = segment == (REVERSE ? 0 : a.segments - 1);      // of the walk
     if (STATE && last && !a.last_wanted) return;                      // no segment starts from the state after it
     const int begin = segment * a.segment_steps, end = min(begin + a.segment_steps, a.steps);
@@ -253,7 +260,7 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
         score_weights[lane] = power(log2_decay, lane) * a.score_scale;
     }
     O* const lane_out = STATE ? nullptr : at<O>(a.out, 0, b, h) + l * a.out.step + column0 + 4 * quarter;
-    float total = 0.0f;                                 // SLOPE
+    double total = 0.0;                                 // SLOPE: of terms of either sign, which leave little of each other
     int weights_n = -1; uint64_t weights_resets = 0;    // the steps and the resets that the weights in LDS are for
     int counted = 0; bool forgotten = false;            // STATE
     // no state before the first steps, none asked for after the last: the products are left out
@@ -342,7 +349,7 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
                 }
                 if constexpr (SLOPE) {
 #pragma unroll
-                    for (int r = 0; r < 4; r++) { const int s = 16 * st + 4 * quarter + r; total += x[r] == 0.0f ? 0.0f : (float)(REVERSE ? s - i : i - s) * x[r] * y[r]; }
+                    for (int r = 0; r < 4; r++) { const int s = 16 * st + 4 * quarter + r; if (x[r] != 0.0f) total += (double)x[r] * ((float)(REVERSE ? s - i : i - s) * y[r]); }
                 }
                 score[j] = x;
                 __builtin_amdgcn_sched_barrier(0);      // one tile in registers at a time
@@ -391,7 +398,7 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
                         float d = 0.0f;
 #pragma unroll
                         for (int r = 0; r < 4; r++) d = fmaf((float)with[r], fmaf((float)(i + 1), out[tile][ot][r], out_slope[tile][ot][r]), d);
-                        if (weight != 0.0f) total = fmaf(weight, d, total);
+                        if (weight != 0.0f) total += (double)weight * d;
                     }
                     if (resets) {      // a state of another episode need not be finite
 #pragma unroll
@@ -536,16 +543,18 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
     if constexpr (SLOPE && !STATE) {
         if (a.d_final && last) {
             const float* const from = a.d_final + (size_t)pair * a.key * a.value;
-            over_state([&](int tile, int k, int r, bool there, int i) { if (there) total = fmaf(from[i], slope[tile][k][r], total); });
+            over_state([&](int tile, int k, int r, bool there, int i) { if (there) total += (double)from[i] * slope[tile][k][r]; });
         }
-        total = rlt_wave_sum(total);
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, 64);
         asm volatile("" : "+v"(total));      // the last exchange stays ahead of the barrier
+        double* const totals = (double*)added_weights;
         rlt_lds_barrier();
-        if (lane == 0) flags[wave] = total;
+        if (lane == 0) totals[wave] = total;
         rlt_lds_barrier();
         if (threadIdx.x == 0) {
-            float s = 0.0f;
-            for (int w = 0; w < L::WAVES; w++) s += flags[w];
+            double s = 0.0;
+            for (int w = 0; w < L::WAVES; w++) s += totals[w];
             a.partial[item * L::SPLIT + half] = s;
         }
     }
@@ -585,12 +594,13 @@ template <bool SLOPES> __global__ __launch_bounds__(256) void scan_kernel(const 
 }
 
 // sums over the rows of a batch and their segments (and the workgroups that share one), in a fixed order
-__global__ __launch_bounds__(64) void decay_sum_kernel(const float* __restrict__ partial, int batch, int heads, int segments, float* __restrict__ out, int accumulate) {
+__global__ __launch_bounds__(64) void decay_sum_kernel(const double* __restrict__ partial, int batch, int heads, int segments, float* __restrict__ out, int accumulate) {
     const int h = blockIdx.x;
-    float s = 0.0f;
+    double s = 0.0;
     for (int i = threadIdx.x; i < batch * segments; i += 64) s += partial[((size_t)(i / segments) * heads + h) * segments + i % segments];
-    s = rlt_wave_sum(s);
-    if (threadIdx.x == 0) out[h] = accumulate ? out[h] + s : s;
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
+    if (threadIdx.x == 0) out[h] = (float)(accumulate ? out[h] + s : s);
 }
 
 // gradients of shared keys and values: the sum over the heads that read them
@@ -705,7 +715,7 @@ Scratch scratch_of(const rlt_linear_attention* p, int steps, bool backward) {
         s.factors = take(2 * pairs * g.count);
     }
     if (backward) {
-        s.partial = take(2 * pairs * g.count);      // up to two workgroups share a head
+        s.partial = take(4 * pairs * g.count);      // doubles, of up to two workgroups that share a head
         if (p->heads != p->kv_heads) s.shared = take(padded((size_t)steps * pairs * p->value_dim) + (size_t)steps * pairs * p->key_dim);
     }
     s.total = at;
@@ -785,7 +795,7 @@ template <typename T> int backward(rlt_rocm_device* device, const rlt_linear_att
         if (rc) return rc;
     }
     a.q = G; a.k = V; a.v = K; a.with = Q; a.out = part<T, 4>(d_q, 1, p->key_dim); a.key = p->value_dim; a.value = p->key_dim; a.state_key = 1; a.state_value = p->value_dim;
-    a.entry = cut ? states : initial_state; a.entry_slope = cut ? slopes : nullptr; a.d_final = d_final_state; a.partial = workspace + s.partial;
+    a.entry = cut ? states : initial_state; a.entry_slope = cut ? slopes : nullptr; a.d_final = d_final_state; a.partial = (double*)(workspace + s.partial);
     rc = d_log_decay ? walk<T, T, false, true, false>(device, a) : walk<T, T, false, false, false>(device, a);
     if (rc) return rc;
     if (d_log_decay) hipLaunchKernelGGL(decay_sum_kernel, dim3(p->heads), dim3(64), 0, device->stream, a.partial, p->batch, p->heads, a.segments * (p->key_dim > 64 || p->value_dim > 64 ? 2 : 1), d_log_decay, accumulate);
