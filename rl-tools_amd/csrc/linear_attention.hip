@@ -593,27 +593,36 @@ template <bool SLOPES> __global__ __launch_bounds__(256) void scan_kernel(const 
     if (final) final[(size_t)pair * elements + e] = carry;
 }
 
-// sums over the rows of a batch and their segments (and the workgroups that share one), in a fixed order
-__global__ __launch_bounds__(64) void decay_sum_kernel(const double* __restrict__ partial, int batch, int heads, int segments, float* __restrict__ out, int accumulate) {
+// sums over the rows of a batch and their segments (and the workgroups that share one), in a fixed order: a workgroup per head
+__global__ __launch_bounds__(512) void decay_sum_kernel(const double* __restrict__ partial, int batch, int heads, int segments, float* __restrict__ out, int accumulate) {
+    __shared__ double sums[8];
     const int h = blockIdx.x;
     double s = 0.0;
-    for (int i = threadIdx.x; i < batch * segments; i += 64) s += partial[((size_t)(i / segments) * heads + h) * segments + i % segments];
+    for (int i = threadIdx.x; i < batch * segments; i += 512) s += partial[((size_t)(i / segments) * heads + h) * segments + i % segments];
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
-    if (threadIdx.x == 0) out[h] = (float)(accumulate ? out[h] + s : s);
+    if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < 8; w++) s += sums[w];
+        out[h] = (float)(accumulate ? out[h] + s : s);
+    }
 }
 
-// gradients of shared keys and values: the sum over the heads that read them
-template <typename T> __global__ __launch_bounds__(128) void head_sum_kernel(const float* __restrict__ parts, Part out, int steps, int batch, int kv_heads, int group, int width) {
-    const size_t total = (size_t)steps * batch * kv_heads * width;
-    for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (size_t)gridDim.x * blockDim.x) {
-        const int c = (int)(i % width);
-        const size_t r = i / width;
-        const int h = (int)(r % kv_heads);
-        const size_t tb = r / kv_heads;
-        float s = 0.0f;
-        for (int g = 0; g < group; g++) s += parts[((tb * kv_heads + h) * group + g) * width + c];
-        at<T>(out, (int)(tb / batch), (int)(tb % batch), h)[c] = (T)s;
+// gradients of shared keys and values: the sums over the heads that read them. A workgroup takes the elements of some tokens at a time; those of keys and of values are two rows of the grid.
+struct HeadSum { const float* parts; Part out; int width; };
+template <typename T> __global__ __launch_bounds__(256) void head_sum_kernel(HeadSum first, HeadSum second, size_t tokens, int batch, int kv_heads, int group) {
+    const HeadSum& a = blockIdx.y ? second : first;
+    const int elements = kv_heads * a.width, at_once = elements < 1024 ? 1024 / elements : 1;
+    for (size_t token0 = (size_t)blockIdx.x * at_once; token0 < tokens; token0 += (size_t)gridDim.x * at_once) {
+        const int there = tokens - token0 < (size_t)at_once ? (int)(tokens - token0) : at_once, t0 = (int)(token0 / batch), b0 = (int)(token0 % batch);
+        for (int i = threadIdx.x; i < there * elements; i += 256) {
+            const int token = i / elements, e = i - token * elements, h = e / a.width, c = e - h * a.width, steps = (b0 + token) / batch;
+            const float* const parts = a.parts + (((token0 + token) * kv_heads + h) * group) * a.width + c;
+            float s = 0.0f;
+            for (int g = 0; g < group; g++) s += parts[(size_t)g * a.width];
+            at<T>(a.out, t0 + steps, b0 + token - steps * batch, h)[c] = (T)s;
+        }
     }
 }
 
@@ -798,7 +807,7 @@ template <typename T> int backward(rlt_rocm_device* device, const rlt_linear_att
     a.entry = cut ? states : initial_state; a.entry_slope = cut ? slopes : nullptr; a.d_final = d_final_state; a.partial = (double*)(workspace + s.partial);
     rc = d_log_decay ? walk<T, T, false, true, false>(device, a) : walk<T, T, false, false, false>(device, a);
     if (rc) return rc;
-    if (d_log_decay) hipLaunchKernelGGL(decay_sum_kernel, dim3(p->heads), dim3(64), 0, device->stream, a.partial, p->batch, p->heads, a.segments * (p->key_dim > 64 || p->value_dim > 64 ? 2 : 1), d_log_decay, accumulate);
+    if (d_log_decay) hipLaunchKernelGGL(decay_sum_kernel, dim3(p->heads), dim3(512), 0, device->stream, a.partial, p->batch, p->heads, a.segments * (p->key_dim > 64 || p->value_dim > 64 ? 2 : 1), d_log_decay, accumulate);
     // the state's gradient, from the last step to the first; d_v reads it, d_k reads it across
     Walk r = walk_of(p, reset, lengths, steps);
     r.k = Q; r.v = G; r.read_scale = 1.0f; r.added_scale = p->scale;
@@ -818,8 +827,8 @@ template <typename T> int backward(rlt_rocm_device* device, const rlt_linear_att
     float* const shared_v = workspace + s.shared; float* const shared_k = shared_v + padded(tokens * p->heads * p->value_dim);
     r.out = shares(shared_v, p->value_dim); w.out = shares(shared_k, p->key_dim);
     if ((rc = walk<T, float, true, false, false>(device, r, &w))) return rc;
-    hipLaunchKernelGGL((head_sum_kernel<T>), dim3(2048), dim3(128), 0, device->stream, shared_v, part<T, 4>(d_v, 1, p->value_dim), steps, p->batch, p->kv_heads, group, p->value_dim);
-    hipLaunchKernelGGL((head_sum_kernel<T>), dim3(2048), dim3(128), 0, device->stream, shared_k, part<T, 4>(d_k, 1, p->key_dim), steps, p->batch, p->kv_heads, group, p->key_dim);
+    hipLaunchKernelGGL((head_sum_kernel<T>), dim3(2048, 2), dim3(256), 0, device->stream, HeadSum{shared_v, part<T, 4>(d_v, 1, p->value_dim), p->value_dim}, HeadSum{shared_k, part<T, 4>(d_k, 1, p->key_dim), p->key_dim},
+                       tokens, p->batch, p->kv_heads, group);
     return rlt_launch_status(device);
 }
 
