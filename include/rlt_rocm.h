@@ -1214,7 +1214,7 @@ typedef struct rlt_head_view {
 
 /* Linear attention with a decay for each head, a recurrent layer whose state is a matrix [key_dim x value_dim] per row and head:
  *     S_t = a_t S_{t-1} + k_t^T v_t,   output_t = scale * q_t S_t,   a_t = exp(log_decay[head]), or nothing at a reset.
- * Query head h reads key / value head h / (heads / kv_heads); every query head has its own decay and state. key_dim and value_dim up to 128. */
+ * Query head h reads key / value head h / (heads / kv_heads); every query head has its own decay and state. key_dim and value_dim up to 128, sequences up to 2^30 steps. */
 typedef struct rlt_linear_attention {
     const float* log_decay;      /* [heads], <= 0 for a state that forgets (-infinity: only the step itself) */
     float scale;
@@ -1253,7 +1253,7 @@ enum rlt_norm {
 
 /* What stands between two blocks of a residual stream, in one pass: the norm after a block, its gate and residual scale, and the norm before the next block,
  *     y = x + residual_scale * gate_activation(gate) * (branch_norm(branch) * branch_weights + branch_biases),   h = output_norm(y) * output_weights + output_biases,
- * row by row over dim columns (at most 8,192). Weights that are NULL are ones, biases that are NULL zeros. */
+ * row by row over dim columns (at most 8,192; at most 2^30 rows). Weights that are NULL are ones, biases that are NULL zeros. */
 typedef struct rlt_residual_norm {
     int32_t type;                /* enum rlt_type of the tensors [rows x dim] */
     int32_t dim;

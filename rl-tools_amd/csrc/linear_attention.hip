@@ -4,7 +4,7 @@
 
 namespace {
 
-constexpr int MAX_WIDTH = 128, CHUNK = 64, STEP_NARROW = 1024;
+constexpr int MAX_WIDTH = 128, CHUNK = 64, STEP_NARROW = 1024, MAX_STEPS = 1 << 30;
 
 // a tensor as the kernels see it: heads / group of it; channels side by side are read and written as vectors where `vectors` is set
 struct Part { void* data; int64_t step, row, head; int group, vectors; };      // vectors: of 16 bytes (inputs), of four channels (outputs)
@@ -95,6 +95,9 @@ template <typename T, int D, bool SLOPE, bool STATE> struct Layout {
 // A wavefront owns some of the value columns: their state stays in its accumulators from chunk to chunk, laid out as the matrix instruction leaves them, which is (with the summands in an order of their own) how the
 // product with the queries takes them. Scores of a chunk are shared out in tiles of 16 x 16, weighted, and exchanged through LDS. SLOPE carries the state's derivative by the decay's logarithm along.
 // STATE: only the state, of a segment that starts from nothing. A launch may hold two walks over the same rows (gradients of keys and of values), whose workgroups take turns on an XCD and so find each other's inputs in its L2.
+// What bounds it: whole heads of 128 bfloat16 channels, the vector and matrix instructions of two wavefronts a SIMD (81 % busy) beside 4 TB/s: 4 rows x 16 heads, 8,192 steps, a walk forward 165 us, d_q with the slope 418, d_k and d_v 325;
+// 16,384 steps of 16 heads forward 132 us in all. Short sequences in fp32, the parts of one chunk one after the other in eight wavefronts a compute unit, as many as LDS has room for (36 KB a workgroup of 32 channels): 64 steps,
+// 1,024 rows, 2 heads of 32: 32, 55 and 52 us, of which the matrix instructions take 8, 14 and 15. Fewer rows and heads than compute units leave a chunk's latency alone: 333 steps, 37 rows, 6 heads of 24 x 41: 47, 73 and 73 us.
 struct Walks { Walk first, second; int items, two; };
 template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, bool FULL> __global__ __launch_bounds__((Layout<T, D, SLOPE, STATE>::THREADS), (Layout<T, D, SLOPE, STATE>::RESIDENT)) void walk_kernel(Walks walks) {
     typedef typename Operand<T>::Vector Vector;
@@ -837,7 +840,7 @@ template <typename T> int backward(rlt_rocm_device* device, const rlt_linear_att
 extern "C" {
 
 size_t rlt_rocm_linear_attention_workspace_bytes(const rlt_linear_attention* layer, int steps, int backward) {
-    if (!described(layer) || steps <= 0) return 0;
+    if (!described(layer) || steps <= 0 || steps > MAX_STEPS) return 0;
     return scratch_of(layer, steps, backward != 0).total * sizeof(float);
 }
 
@@ -848,7 +851,7 @@ int rlt_rocm_linear_attention_forward(rlt_rocm_device* device, const rlt_linear_
     RLT_REQUIRE(described(layer) && layer->log_decay && steps > 0 && given(q) && given(k) && given(v) && given(output));
     const size_t need = rlt_rocm_linear_attention_workspace_bytes(layer, steps, 0);
     RLT_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0));
-    if (!supported(layer)) return RLT_E_UNSUPPORTED;
+    if (!supported(layer) || steps > MAX_STEPS) return RLT_E_UNSUPPORTED;
     return layer->type == RLT_TYPE_F32 ? forward<float>(device, layer, q, k, v, output, initial_state, final_state, reset, lengths, steps, (float*)workspace)
                                        : forward<rlt_bf16>(device, layer, q, k, v, output, initial_state, final_state, reset, lengths, steps, (float*)workspace);
 }
@@ -861,7 +864,7 @@ int rlt_rocm_linear_attention_backward(rlt_rocm_device* device, const rlt_linear
     RLT_REQUIRE(described(layer) && layer->log_decay && steps > 0 && given(q) && given(k) && given(v) && given(d_output) && given(d_q) && given(d_k) && given(d_v));
     const size_t need = rlt_rocm_linear_attention_workspace_bytes(layer, steps, 1);
     RLT_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0));
-    if (!supported(layer)) return RLT_E_UNSUPPORTED;
+    if (!supported(layer) || steps > MAX_STEPS) return RLT_E_UNSUPPORTED;
     return layer->type == RLT_TYPE_F32 ? backward<float>(device, layer, q, k, v, d_output, d_q, d_k, d_v, initial_state, d_final_state, d_initial_state, d_log_decay, accumulate, reset, lengths, steps, (float*)workspace)
                                        : backward<rlt_bf16>(device, layer, q, k, v, d_output, d_q, d_k, d_v, initial_state, d_final_state, d_initial_state, d_log_decay, accumulate, reset, lengths, steps, (float*)workspace);
 }

@@ -4,7 +4,7 @@
 
 namespace {
 
-constexpr int MAX_DIM = 8192, HELD_DIM = 4096;
+constexpr int MAX_DIM = 8192, HELD_DIM = 4096, MAX_ROWS = 1 << 30;      // a row's index and a step over the grid's rows fit 32 bits
 enum { BRANCH_W = 0, BRANCH_B, OUTPUT_W, OUTPUT_B, SCALE, SUMS };      // column sums of the backward pass
 
 struct NormForward {
@@ -221,6 +221,8 @@ template <int N, bool SLOPES> __device__ __forceinline__ void gates_of(float (&g
     }
 }
 
+// Memory bounds this pass: three rows in, two out, all of a row's elements in registers from its loads to its stores (16,384 x 4,096 bfloat16: 152 us, 4.4 TB/s; 65,536 x 256 fp32: 66 us, 5.0 TB/s; a launch at 256 x 256: 4.3 us).
+// bfloat16 rows are converted behind the last load: a conversion in a load's branch waits for it (163 us); fp32 rows need none and are faster without the copy (66 us, 74 with it).
 template <typename T, int V, int K, int THREADS, bool WHOLE> __global__ __launch_bounds__(FORWARD_WIDTH<THREADS>) void norm_forward_kernel(NormForward a) {
     constexpr int N = V * K, ROWS = FORWARD_WIDTH<THREADS> / THREADS;
     __shared__ float lds[THREADS > 64 ? 2 * (THREADS / 64) * 4 : 1];
@@ -253,12 +255,13 @@ template <typename T, int V, int K, int THREADS, bool WHOLE> __global__ __launch
     }
 }
 
-// Memory bounds this pass: five rows in, three out. The next row's values are asked for before this row's sums, of which a row has two rounds (three with means): what the statistics and the output norm's gradient need
+// Memory bounds this pass: five rows in, three out, 4.6 TB/s at 16,384 rows of 4,096 bfloat16 values (238 to 268 us), 4.8 at 16,384 of 2,048 fp32 values; few rows are bound by the trips to memory of the two or three that a workgroup
+// has (4,001 x 1,000 fp32: 36 us). The next row's values are asked for before this row's sums, of which a row has two rounds (three with means): what the statistics and the output norm's gradient need
 // is added up together.
 template <typename T, int V, int K, int THREADS, bool BIASES, bool WHOLE> __global__ __launch_bounds__(BACKWARD_WIDTH<THREADS>) void norm_backward_kernel(NormBackward a) {
     constexpr int N = V * K, WIDTH = BACKWARD_WIDTH<THREADS>, ROWS = WIDTH / THREADS;
     // Parameters and column sums stay in registers from row to row. Rows wider than 4,096 leave none for them: parameters are read again, from L2, and the sums are kept in LDS, each by its own thread (4,096 rows of 8,192 bfloat16
-    // values: 183 us; 536 with 1,024 threads of eight columns, whose registers spill. 16,384 rows of 4,096: 278 us with registers, 332 so).
+    // values: 183 us; 536 with 1,024 threads of eight columns, whose registers spill. 16,384 rows of 4,096: 266 us with registers, 332 so).
     constexpr bool HELD = N * THREADS <= HELD_DIM, AHEAD = HELD || (WHOLE && V == 8);
     __shared__ float lds[ROWS == 1 ? 2 * (THREADS / 64) * 4 : WIDTH * N];
     extern __shared__ __attribute__((aligned(16))) float column_sums[];
@@ -504,7 +507,7 @@ int rlt_rocm_residual_norm_forward(rlt_rocm_device* device, const rlt_residual_n
     RLT_REQUIRE(described(layer) && rows > 0);
     const int dim = layer->dim;
     RLT_REQUIRE(x && ldx >= dim && (!branch || ldb >= dim) && (!gate || ldg >= dim) && (!y || ldy >= dim) && (!h || ldh >= dim) && (y || h));
-    if (dim > MAX_DIM) return RLT_E_UNSUPPORTED;
+    if (dim > MAX_DIM || rows > MAX_ROWS) return RLT_E_UNSUPPORTED;
     const NormForward a = {*layer, x, branch, gate, y, h, ldx, ldb, ldg, ldy, ldh, rows};
     if (layer->type == RLT_TYPE_F32) forward<float>(device, a); else forward<rlt_bf16>(device, a);
     return rlt_launch_status(device);
@@ -525,7 +528,7 @@ int rlt_rocm_residual_norm_backward(rlt_rocm_device* device, const rlt_residual_
     RLT_REQUIRE((!d_x || lddx >= dim) && (!d_branch || (branch && lddb >= dim)) && (!d_gate || (branch && gate && lddg >= dim)));
     // gradients of parameters that nothing reaches
     RLT_REQUIRE((branch || !(layer->d_branch_weights || layer->d_branch_biases || layer->d_residual_scale)) && (d_h || !(layer->d_output_weights || layer->d_output_biases)));
-    if (dim > MAX_DIM) return RLT_E_UNSUPPORTED;
+    if (dim > MAX_DIM || rows > MAX_ROWS) return RLT_E_UNSUPPORTED;
     const bool sums = layer->d_branch_weights || layer->d_branch_biases || layer->d_output_weights || layer->d_output_biases || layer->d_residual_scale;
     RLT_REQUIRE(!sums || (workspace && workspace_bytes >= rlt_rocm_residual_norm_workspace_bytes(layer, rows)));
     const NormBackward a = {*layer, branch, gate, y, d_y, d_h, d_x, d_branch, d_gate, ldb, ldg, ldy, lddy, lddh, lddx, lddb, lddg, rows, (float*)workspace};

@@ -406,3 +406,16 @@ def test_refusals(rocm):
     assert lib.rlt_rocm_linear_attention_step(h, C.byref(good), t["q"].view, t["k"].view, t["v"].view, out.view, state.ptr, None, None) == capi.RLT_E_INVALID_ARGUMENT
     assert lib.rlt_rocm_linear_attention_workspace_bytes(None, 4, 1) == lib.rlt_rocm_linear_attention_workspace_bytes(C.byref(good), 0, 1) == 0
     rocm.sync()
+
+
+@gpu
+def test_longer_sequences_than_an_index_holds_are_refused(rocm):
+    c, x = case(2, "float32", 4, 2, 2, 2, 8, 8)
+    layer, t = layer_of(rocm, c, x), {n: Tensor(rocm, x[n], "float32") for n in ("q", "k", "v", "d_output")}
+    lib, h = rocm.device.lib, rocm.device.handle
+    w = rocm.zeros((1024,))
+    views = [t[n].view for n in ("q", "k", "v", "d_output")]
+    for steps in (2 ** 30 + 1, 2 ** 31 - 1):
+        assert lib.rlt_rocm_linear_attention_workspace_bytes(C.byref(layer), steps, 0) == lib.rlt_rocm_linear_attention_workspace_bytes(C.byref(layer), steps, 1) == 0
+        assert lib.rlt_rocm_linear_attention_forward(h, C.byref(layer), *views, None, None, None, None, steps, w.ptr, 4096) == capi.RLT_E_UNSUPPORTED
+        assert lib.rlt_rocm_linear_attention_backward(h, C.byref(layer), *views, *views[:3], None, None, None, None, 0, None, None, steps, w.ptr, 4096) == capi.RLT_E_UNSUPPORTED

@@ -330,3 +330,13 @@ def test_refusals(rocm):
     assert backward_code(summed, branch=None, w=w.ptr, n=need) == capi.RLT_E_INVALID_ARGUMENT      # nothing reaches the branch's weights
     assert backward_code(plain, d_y=None, d_h=None) == backward_code(plain, y=None) == backward_code(plain, d_gate=out.ptr) == backward_code(plain, branch=None, d_branch=out.ptr) == capi.RLT_E_INVALID_ARGUMENT
     rocm.sync()
+
+
+@gpu
+def test_more_rows_than_an_index_holds_are_refused(rocm):
+    a = rocm.zeros((4, 16))
+    layer = layer_of(rocm, dict(dtype="float32", dim=16, rows=4, branch_norm="rms", output_norm="rms", activation="sigmoid", epsilon=1e-5), {})
+    lib, h = rocm.device.lib, rocm.device.handle
+    for rows in (2 ** 30 + 1, 2 ** 31 - 1):
+        assert lib.rlt_rocm_residual_norm_forward(h, C.byref(layer), a.ptr, 16, None, 0, None, 0, a.ptr, 16, None, 0, rows) == capi.RLT_E_UNSUPPORTED
+        assert lib.rlt_rocm_residual_norm_backward(h, C.byref(layer), None, 0, None, 0, a.ptr, 16, a.ptr, 16, None, 0, a.ptr, 16, None, 0, None, 0, rows, 0, None, 0) == capi.RLT_E_UNSUPPORTED
