@@ -142,14 +142,17 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
         state[tile][k][r] = 0.0f;
         if constexpr (SLOPE) slope[tile][k][r] = 0.0f;
     });
+    // elements outside are read as the first one and dropped: a branch for each would wait for each
     if (const float* from = STATE ? nullptr : a.entry) {
         from += state_base;
-        over_state([&](int tile, int k, int r, bool there, int i) { if (there) state[tile][k][r] = from[i]; });
+        over_state([&](int tile, int k, int r, bool there, int i) { state[tile][k][r] = from[there ? i : 0]; });
+        if (!FULL) over_state([&](int tile, int k, int r, bool there, int i) { if (!there) state[tile][k][r] = 0.0f; });
     }
     if constexpr (SLOPE && !STATE)
         if (const float* from = a.entry_slope) {
             from += state_base;
-            over_state([&](int tile, int k, int r, bool there, int i) { if (there) slope[tile][k][r] = from[i]; });
+            over_state([&](int tile, int k, int r, bool there, int i) { slope[tile][k][r] = from[there ? i : 0]; });
+            if (!FULL) over_state([&](int tile, int k, int r, bool there, int i) { if (!there) slope[tile][k][r] = 0.0f; });
         }
 
     // what a thread carries from memory to LDS, in rounds: 16 bytes of a step of each tensor, of all D channels or of the workgroup's columns
@@ -546,7 +549,7 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
     if constexpr (SLOPE && !STATE) {
         if (a.d_final && last) {
             const float* const from = a.d_final + (size_t)pair * a.key * a.value;
-            over_state([&](int tile, int k, int r, bool there, int i) { if (there) total += (double)from[i] * slope[tile][k][r]; });
+            over_state([&](int tile, int k, int r, bool there, int i) { total += (double)from[there ? i : 0] * slope[tile][k][r]; });      // zero outside
         }
 #pragma unroll
         for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, 64);
