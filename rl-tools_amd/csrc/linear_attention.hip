@@ -225,6 +225,10 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
             if constexpr (SLOPE && !STATE) settle(part0, a.value, n, next_with, columns);
         }
     };
+    // products over a chunk's steps, sixteen to a tile: one, two or all four tiles
+    auto by_steps = [&](int n, auto f) {
+        if (n > 32) f(std::integral_constant<int, 4>{}); else if (n > 16) f(std::integral_constant<int, 2>{}); else if (n > 0) f(std::integral_constant<int, 1>{});
+    };
     auto steps_of = [&](int t0, int stop) { return min(max(min(length, stop) - t0, 0), CHUNK); };
     auto fetch_chunk = [&](int t0, int stop) {
         stop = min(stop, length);
@@ -336,6 +340,8 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
             for (int j = 0; j < L::SCORE_TILES; j++) {
                 const int tile = first_tile + j * L::WAVES, row = tile < 1 ? 0 : tile < 3 ? 1 : tile < 6 ? 2 : 3, col = tile - row * (row + 1) / 2, ot = REVERSE ? 3 - row : row, st = REVERSE ? 3 - col : col;
                 if (tile >= 10) break;
+                score[j] = rlt_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                if (16 * (REVERSE ? st : ot) >= n) continue;
                 rlt_f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f}, y = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int block = 0; block < KEY_BLOCKS; block++) if (FULL || 32 * block < a.key) x = multiply(row_operand(L::K, L::ROW, 16 * st + l, block), row_operand(L::Q, L::ROW, 16 * ot + l, block), x);
@@ -369,32 +375,33 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
                     out[tile][ot] = rlt_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
                     if constexpr (SLOPE) out_slope[tile][ot] = rlt_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
                 }
-            if (!nothing) {
+            auto before = [&](auto tiles) {
+                constexpr int STEP_TILES = decltype(tiles)::value;
 #pragma unroll
             for (int block = 0; block < KEY_BLOCKS; block++) {
                 if (!FULL && 32 * block >= a.key) break;
-                Vector q[4];
+                Vector q[STEP_TILES];
 #pragma unroll
-                for (int ot = 0; ot < 4; ot++) q[ot] = tiled_operand(L::Q, 16 * ot + l, block);
+                for (int ot = 0; ot < STEP_TILES; ot++) q[ot] = tiled_operand(L::Q, 16 * ot + l, block);
 #pragma unroll
                 for (int tile = 0; tile < TILES; tile++) {
                     const Cut<T, STATE_CUTS> s(__builtin_shufflevector(state[tile][2 * block], state[tile][2 * block + 1], 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
                     for (int p = 0; p < STATE_CUTS; p++)
 #pragma unroll
-                        for (int ot = 0; ot < 4; ot++) out[tile][ot] = multiply(s.part[p], q[ot], out[tile][ot]);
+                        for (int ot = 0; ot < STEP_TILES; ot++) out[tile][ot] = multiply(s.part[p], q[ot], out[tile][ot]);
                     if constexpr (SLOPE) {
                         const Cut<T, STATE_CUTS> d(__builtin_shufflevector(slope[tile][2 * block], slope[tile][2 * block + 1], 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
                         for (int p = 0; p < STATE_CUTS; p++)
 #pragma unroll
-                            for (int ot = 0; ot < 4; ot++) out_slope[tile][ot] = multiply(d.part[p], q[ot], out_slope[tile][ot]);
+                            for (int ot = 0; ot < STEP_TILES; ot++) out_slope[tile][ot] = multiply(d.part[p], q[ot], out_slope[tile][ot]);
                     }
                 }
                 if constexpr (SLOPE) __builtin_amdgcn_sched_barrier(0);      // one block's operands in registers at a time
             }
 #pragma unroll
-            for (int ot = 0; ot < 4; ot++) {
+            for (int ot = 0; ot < STEP_TILES; ot++) {
                 const int i = 16 * ot + l;
                 const float weight = read_weights[i];
 #pragma unroll
@@ -412,7 +419,8 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
                     } else out[tile][ot] *= weight;
                 }
             }
-            }
+            };
+            if (!nothing) by_steps(n, before);
             if constexpr (L::OVER) rlt_lds_barrier();      // the queries have been read
 #pragma unroll
             for (int j = 0; j < L::SCORE_TILES; j++) {
@@ -431,13 +439,15 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
             rlt_lds_barrier();
             if constexpr (SLOPE) { if (!done) fetch_chunk(next_t0, next_stop); }      // only here: the products with two states before leave no registers for it
             // what the chunk's own steps give
+            auto within = [&](auto tiles) {
+                constexpr int STEP_TILES = decltype(tiles)::value;
 #pragma unroll
-            for (int block = 0; block < 2; block++) {
+            for (int block = 0; block < (STEP_TILES + 1) / 2; block++) {
                 Vector values[TILES];
 #pragma unroll
                 for (int tile = 0; tile < TILES; tile++) values[tile] = column_operand(L::V, L::COLUMN_ROW, TILES * wave + tile, block);
 #pragma unroll
-                for (int ot = 0; ot < 4; ot++)
+                for (int ot = 0; ot < STEP_TILES; ot++)
                     if (REVERSE ? 32 * block + 31 >= 16 * ot : 32 * block <= 16 * ot + 15) {
 #pragma unroll
                         for (int plane = 0; plane < L::PLANES; plane++) {
@@ -447,6 +457,8 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
                         }
                     }
             }
+            };
+            by_steps(n, within);
             typedef typename Operand<O>::Quad OutQuad;
             O* const to = lane_out + t0 * a.out.step;
 #pragma unroll
@@ -490,6 +502,7 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
                 }
 #pragma unroll
             for (int block = 0; block < 2; block++) {
+                if (32 * block >= n) break;
                 const rlt_f32x8 weight = *reinterpret_cast<const rlt_f32x8*>(added_weights + 32 * block + 8 * quarter);
                 Vector key[SLOPE ? 1 : KEY_TILES];
                 if constexpr (!SLOPE) {
