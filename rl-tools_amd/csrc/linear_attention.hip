@@ -142,16 +142,32 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
         state[tile][k][r] = 0.0f;
         if constexpr (SLOPE) slope[tile][k][r] = 0.0f;
     });
-    // elements outside are read as the first one and dropped: a branch for each would wait for each
+    // f(tile, k, the four elements r = 0 ... 3 of a state in memory). Those of a state that is read across lie side by side: one load of 16 bytes. Elements outside are read as the first one and dropped when all have
+    // been asked for: a branch or a choice behind each would wait for each.
+    typedef float Four __attribute__((ext_vector_type(4), aligned(4)));
+    auto read_state = [&](const float* from, auto f) {
+        const bool across = state_key == 1 && (FULL || a.key % 4 == 0);
+#pragma unroll
+        for (int tile = 0; tile < TILES; tile++)
+#pragma unroll
+            for (int k = 0; k < KEY_TILES; k++) {
+                const int row = 16 * k + 4 * quarter, column = column0 + 16 * tile + l;
+                rlt_f32x4 x;
+                if (across) x = *reinterpret_cast<const Four*>(from + (FULL || (row < a.key && column < a.value) ? row + column * state_value : 0));
+                else {
+#pragma unroll
+                    for (int r = 0; r < 4; r++) x[r] = from[FULL || (row + r < a.key && column < a.value) ? (row + r) * state_key + column * state_value : 0];
+                }
+                f(tile, k, x);
+            }
+    };
     if (const float* from = STATE ? nullptr : a.entry) {
-        from += state_base;
-        over_state([&](int tile, int k, int r, bool there, int i) { state[tile][k][r] = from[there ? i : 0]; });
+        read_state(from + state_base, [&](int tile, int k, rlt_f32x4 x) { state[tile][k] = x; });
         if (!FULL) over_state([&](int tile, int k, int r, bool there, int i) { if (!there) state[tile][k][r] = 0.0f; });
     }
     if constexpr (SLOPE && !STATE)
         if (const float* from = a.entry_slope) {
-            from += state_base;
-            over_state([&](int tile, int k, int r, bool there, int i) { slope[tile][k][r] = from[there ? i : 0]; });
+            read_state(from + state_base, [&](int tile, int k, rlt_f32x4 x) { slope[tile][k] = x; });
             if (!FULL) over_state([&](int tile, int k, int r, bool there, int i) { if (!there) slope[tile][k][r] = 0.0f; });
         }
 
@@ -561,8 +577,10 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
     if constexpr (STATE) { if (threadIdx.x == 0 && half == 0) a.factors[item] = make_float2(forgotten ? 0.0f : power(log2_decay, counted), (float)counted); }
     if constexpr (SLOPE && !STATE) {
         if (a.d_final && last) {
-            const float* const from = a.d_final + (size_t)pair * a.key * a.value;
-            over_state([&](int tile, int k, int r, bool there, int i) { total += (double)from[there ? i : 0] * slope[tile][k][r]; });      // zero outside
+            read_state(a.d_final + (size_t)pair * a.key * a.value, [&](int tile, int k, rlt_f32x4 x) {
+#pragma unroll
+                for (int r = 0; r < 4; r++) total += (double)x[r] * slope[tile][k][r];      // zeros outside
+            });
         }
 #pragma unroll
         for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, 64);
