@@ -647,18 +647,21 @@ __global__ __launch_bounds__(512) void decay_sum_kernel(const double* __restrict
 }
 
 // gradients of shared keys and values: the sums over the heads that read them. A workgroup takes the elements of some tokens at a time; those of keys and of values are two rows of the grid.
+// V elements of a head at a time: four (16 bytes of each share) where the widths are multiples of four.
 struct HeadSum { const float* parts; Part out; int width; };
-template <typename T> __global__ __launch_bounds__(256) void head_sum_kernel(HeadSum first, HeadSum second, size_t tokens, int batch, int kv_heads, int group) {
+template <typename T, int V> __global__ __launch_bounds__(256) void head_sum_kernel(HeadSum first, HeadSum second, size_t tokens, int batch, int kv_heads, int group) {
+    typedef float vector __attribute__((ext_vector_type(V)));
+    typedef T OutVector __attribute__((ext_vector_type(V), aligned(sizeof(T))));
     const HeadSum& a = blockIdx.y ? second : first;
-    const int elements = kv_heads * a.width, at_once = elements < 1024 ? 1024 / elements : 1;
+    const int width = a.width / V, elements = kv_heads * width, at_once = elements < 1024 ? 1024 / elements : 1;
     for (size_t token0 = (size_t)blockIdx.x * at_once; token0 < tokens; token0 += (size_t)gridDim.x * at_once) {
         const int there = tokens - token0 < (size_t)at_once ? (int)(tokens - token0) : at_once, t0 = (int)(token0 / batch), b0 = (int)(token0 % batch);
         for (int i = threadIdx.x; i < there * elements; i += 256) {
-            const int token = i / elements, e = i - token * elements, h = e / a.width, c = e - h * a.width, steps = (b0 + token) / batch;
+            const int token = i / elements, e = i - token * elements, h = e / width, c = (e - h * width) * V, steps = (b0 + token) / batch;
             const float* const parts = a.parts + (((token0 + token) * kv_heads + h) * group) * a.width + c;
-            float s = 0.0f;
-            for (int g = 0; g < group; g++) s += parts[(size_t)g * a.width];
-            at<T>(a.out, t0 + steps, b0 + token - steps * batch, h)[c] = (T)s;
+            vector s = {};
+            for (int g = 0; g < group; g++) s += *reinterpret_cast<const vector*>(parts + (size_t)g * a.width);
+            *reinterpret_cast<OutVector*>(at<T>(a.out, t0 + steps, b0 + token - steps * batch, h) + c) = __builtin_convertvector(s, OutVector);
         }
     }
 }
@@ -864,8 +867,9 @@ template <typename T> int backward(rlt_rocm_device* device, const rlt_linear_att
     float* const shared_v = workspace + s.shared; float* const shared_k = shared_v + padded(tokens * p->heads * p->value_dim);
     r.out = shares(shared_v, p->value_dim); w.out = shares(shared_k, p->key_dim);
     if ((rc = walk<T, float, true, false, false>(device, r, &w))) return rc;
-    hipLaunchKernelGGL((head_sum_kernel<T>), dim3(2048, 2), dim3(256), 0, device->stream, HeadSum{shared_v, part<T, 4>(d_v, 1, p->value_dim), p->value_dim}, HeadSum{shared_k, part<T, 4>(d_k, 1, p->key_dim), p->key_dim},
-                       tokens, p->batch, p->kv_heads, group);
+    const HeadSum sum_v = {shared_v, part<T, 4>(d_v, 1, p->value_dim), p->value_dim}, sum_k = {shared_k, part<T, 4>(d_k, 1, p->key_dim), p->key_dim};
+    if (p->value_dim % 4 == 0 && p->key_dim % 4 == 0) hipLaunchKernelGGL((head_sum_kernel<T, 4>), dim3(2048, 2), dim3(256), 0, device->stream, sum_v, sum_k, tokens, p->batch, p->kv_heads, group);
+    else hipLaunchKernelGGL((head_sum_kernel<T, 1>), dim3(2048, 2), dim3(256), 0, device->stream, sum_v, sum_k, tokens, p->batch, p->kv_heads, group);
     return rlt_launch_status(device);
 }
 
