@@ -125,6 +125,11 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
     // state: tile k, element r of this lane is row 16 k + 4 quarter + r, column 16 (TILES wave + tile) + l
     rlt_f32x4 state[TILES][KEY_TILES], slope[SLOPE ? TILES : 1][SLOPE ? KEY_TILES : 1];
     const int part0 = half * L::COLUMNS, inner0 = 16 * TILES * wave, column0 = part0 + inner0;      // first column of the workgroup, of the wavefront within it, of the wavefront
+    const bool idle = !FULL && column0 >= a.value;      // a wavefront without columns, which takes part in loads and scores
+    if (L::SPLIT > 1 && !FULL && part0 >= a.value) {    // a workgroup without any
+        if (SLOPE && !STATE && threadIdx.x == 0) a.partial[item * L::SPLIT + half] = 0.0;
+        return;
+    }
     const size_t state_base = (size_t)item * a.key * a.value;
     const int state_key = a.state_key, state_value = a.state_value;
     auto over_state = [&](auto f) {
@@ -436,7 +441,7 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
                 }
             }
             };
-            if (!nothing) by_steps(n, before);
+            if (!nothing && !idle) by_steps(n, before);
             if constexpr (L::OVER) rlt_lds_barrier();      // the queries have been read
 #pragma unroll
             for (int j = 0; j < L::SCORE_TILES; j++) {
@@ -474,7 +479,7 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
                     }
             }
             };
-            by_steps(n, within);
+            if (!idle) by_steps(n, within);
             typedef typename Operand<O>::Quad OutQuad;
             O* const to = lane_out + t0 * a.out.step;
 #pragma unroll
@@ -500,7 +505,7 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
             }
         }
         // the state after the chunk
-        if (n > 0 && !(done && last_unread)) {
+        if (n > 0 && !(done && last_unread) && !idle) {
             nothing = false;
             const float f = power(log2_decay, REVERSE ? n - 1 : n);
             counted += n; forgotten |= resets != 0;
@@ -520,8 +525,9 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
             for (int block = 0; block < 2; block++) {
                 if (32 * block >= n) break;
                 const rlt_f32x8 weight = *reinterpret_cast<const rlt_f32x8*>(added_weights + 32 * block + 8 * quarter);
-                Vector key[SLOPE ? 1 : KEY_TILES];
-                if constexpr (!SLOPE) {
+                constexpr bool TOGETHER = !SLOPE && FULL;      // all key operands in registers, else one at a time, as far as there are keys
+                Vector key[TOGETHER ? KEY_TILES : 1];
+                if constexpr (TOGETHER) {
 #pragma unroll
                     for (int k = 0; k < KEY_TILES; k++) key[k] = column_operand(L::K, L::ROW, k, block);
                 }
@@ -534,7 +540,7 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
                         const rlt_f32x8 lagged = __builtin_convertvector(v, rlt_f32x8) * *reinterpret_cast<const rlt_f32x8*>(lagged_weights + 32 * block + 8 * quarter);
                         const Cut<T, ADDED_CUTS> y(lagged);
 #pragma unroll
-                        for (int k = 0; k < KEY_TILES; k++) {      // one key operand in registers at a time
+                        for (int k = 0; k < KEY_TILES; k++) {
                             if (!FULL && 16 * k >= a.key) break;
                             key[0] = column_operand(L::K, L::ROW, k, block);
 #pragma unroll
@@ -542,6 +548,14 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
                                 state[tile][k] = multiply(key[0], x.part[p], state[tile][k]);
                                 slope[tile][k] = multiply(key[0], y.part[p], slope[tile][k]);
                             }
+                        }
+                    } else if constexpr (!TOGETHER) {
+#pragma unroll
+                        for (int k = 0; k < KEY_TILES; k++) {
+                            if (16 * k >= a.key) break;
+                            key[0] = column_operand(L::K, L::ROW, k, block);
+#pragma unroll
+                            for (int p = 0; p < ADDED_CUTS; p++) state[tile][k] = multiply(key[0], x.part[p], state[tile][k]);
                         }
                     } else {
 #pragma unroll
