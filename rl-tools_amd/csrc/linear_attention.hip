@@ -97,7 +97,8 @@ template <typename T, int D, bool SLOPE, bool STATE> struct Layout {
 // STATE: only the state, of a segment that starts from nothing. A launch may hold two walks over the same rows (gradients of keys and of values), whose workgroups take turns on an XCD and so find each other's inputs in its L2.
 // What bounds it: whole heads of 128 bfloat16 channels, the vector and matrix instructions of two wavefronts a SIMD (81 % busy) beside 4 TB/s: 4 rows x 16 heads, 8,192 steps, a walk forward 165 us, d_q with the slope 418, d_k and d_v 325;
 // 16,384 steps of 16 heads forward 132 us in all. Short sequences in fp32, the parts of one chunk one after the other in eight wavefronts a compute unit, as many as LDS has room for (36 KB a workgroup of 32 channels): 64 steps,
-// 1,024 rows, 2 heads of 32: 32, 55 and 52 us, of which the matrix instructions take 8, 14 and 15. Fewer rows and heads than compute units leave a chunk's latency alone: 333 steps, 37 rows, 6 heads of 24 x 41: 47, 73 and 73 us.
+// 1,024 rows, 2 heads of 32: 32, 55 and 52 us, of which the matrix instructions take 8, 14 and 15. Fewer rows and heads than compute units leave a chunk's latency alone: 333 steps, 37 rows, 6 heads of 24 x 41: 46, 70 and 66 us.
+// Few steps on many rows: reading and writing the states, two wavefronts a SIMD: 20 steps, 2,240 rows, 8 heads of 64, bfloat16: 190, 346 and 340 us.
 struct Walks { Walk first, second; int items, two; };
 template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, bool FULL> __global__ __launch_bounds__((Layout<T, D, SLOPE, STATE>::THREADS), (Layout<T, D, SLOPE, STATE>::RESIDENT)) void walk_kernel(Walks walks) {
     typedef typename Operand<T>::Vector Vector;
@@ -696,17 +697,17 @@ template <typename T, int V, int THREADS> __global__ __launch_bounds__(256) void
         const T* const q = at<T>(a.q, 0, b, h); const T* const k = at<T>(a.k, 0, b, h); const T* const values = at<T>(a.v, 0, b, h) + c;
         const size_t base = ((size_t)b * a.heads + h) * a.key * a.value + c;
         const float decay = expf(a.log_decay[h]);
-        const bool forget = a.reset && a.reset[b];      // what the state holds then reaches nothing, values that are not finite either
+        const bool stay = a.lengths && a.lengths[b] <= 0, forget = !a.entry || (!stay && a.reset && a.reset[b]);      // what a forgotten state holds reaches nothing, values that are not finite either
         vector v;
 #pragma unroll
-        for (int n = 0; n < V; n++) v[n] = (float)values[n];
+        for (int n = 0; n < V; n++) v[n] = stay ? 0.0f : (float)values[n];
         for (int i = g; i < a.key; i += AHEAD * groups) {
             vector s[AHEAD] = {};
             float ks[AHEAD], qs[AHEAD];
 #pragma unroll
             for (int j = 0; j < AHEAD; j++) {
                 const int at_key = i + j * groups, key = at_key < a.key ? at_key : i;
-                ks[j] = (float)k[key]; qs[j] = (float)q[key];
+                ks[j] = stay ? 0.0f : (float)k[key]; qs[j] = stay ? 0.0f : (float)q[key];
                 if (!forget) s[j] = *reinterpret_cast<const vector*>(a.entry + base + key * a.value);
             }
 #pragma unroll
@@ -714,8 +715,8 @@ template <typename T, int V, int THREADS> __global__ __launch_bounds__(256) void
                 const int key = i + j * groups;
                 if (key < a.key) {
 #pragma unroll
-                    for (int n = 0; n < V; n++) { s[j][n] = fmaf(ks[j], v[n], s[j][n] * decay); out[n] = fmaf(qs[j], s[j][n], out[n]); }
-                    *reinterpret_cast<vector*>(a.exit + base + key * a.value) = s[j];
+                    for (int n = 0; n < V; n++) { s[j][n] = stay ? s[j][n] : fmaf(ks[j], v[n], s[j][n] * decay); out[n] = stay ? 0.0f : fmaf(qs[j], s[j][n], out[n]); }
+                    if (a.exit) *reinterpret_cast<vector*>(a.exit + base + key * a.value) = s[j];
                 }
             }
         }
@@ -826,6 +827,14 @@ template <typename T, bool REVERSE, bool SLOPE> int segment_states(rlt_rocm_devi
     return rlt_launch_status(device);
 }
 
+template <typename T> void launch_step(rlt_rocm_device* device, const Walk& a) {
+    const unsigned pairs = (unsigned)a.heads * a.batch;
+    const bool vectors = a.value % 4 == 0 && (reinterpret_cast<uintptr_t>(a.entry) | reinterpret_cast<uintptr_t>(a.exit)) % 16 == 0, narrow = a.key * a.value <= STEP_NARROW;
+    auto go = [&](auto kernel, unsigned at_once) { hipLaunchKernelGGL(kernel, dim3((pairs + at_once - 1) / at_once), dim3(256), 0, device->stream, a, pairs); };
+    if (vectors && narrow) go(step_kernel<T, 4, 64>, 4); else if (vectors) go(step_kernel<T, 4, 256>, 1);
+    else if (narrow && a.value <= 64) go(step_kernel<T, 1, 64>, 4); else go(step_kernel<T, 1, 256>, 1);
+}
+
 template <typename T> int forward(rlt_rocm_device* device, const rlt_linear_attention* p, const rlt_head_view* q, const rlt_head_view* k, const rlt_head_view* v, const rlt_head_view* output,
                                   const float* initial_state, float* final_state, const uint8_t* reset, const int32_t* lengths, int steps, float* workspace) {
     const int group = p->heads / p->kv_heads;
@@ -833,6 +842,10 @@ template <typename T> int forward(rlt_rocm_device* device, const rlt_linear_atte
     Walk a = walk_of(p, reset, lengths, steps);
     a.q = part<T>(q, 1, p->key_dim); a.k = part<T>(k, group, p->key_dim); a.v = part<T>(v, group, p->value_dim); a.out = part<T, 4>(output, 1, p->value_dim);
     a.entry = initial_state; a.exit = final_state;
+    if (steps == 1) {      // a pass over the states (9,639 rows, one head of 118, fp32: 235 us; 551 as a walk of one step)
+        launch_step<T>(device, a);
+        return rlt_launch_status(device);
+    }
     if (a.segments > 1) {
         const int rc = segment_states<T, false, false>(device, a, initial_state, final_state, workspace + s.states, nullptr, (float2*)(workspace + s.factors));
         if (rc) return rc;
@@ -932,11 +945,7 @@ int rlt_rocm_linear_attention_step(rlt_rocm_device* device, const rlt_linear_att
     auto views = [&](auto type) {
         typedef decltype(type) T;
         a.q = part<T>(q, 1, layer->key_dim); a.k = part<T>(k, group, layer->key_dim); a.v = part<T>(v, group, layer->value_dim); a.out = part<T, 4>(output, 1, layer->value_dim);
-        const unsigned pairs = (unsigned)a.heads * a.batch;
-        const bool vectors = a.value % 4 == 0 && (reinterpret_cast<uintptr_t>(state) | reinterpret_cast<uintptr_t>(next_state)) % 16 == 0, narrow = a.key * a.value <= STEP_NARROW;
-        auto go = [&](auto kernel, unsigned at_once) { hipLaunchKernelGGL(kernel, dim3((pairs + at_once - 1) / at_once), dim3(256), 0, device->stream, a, pairs); };
-        if (vectors && narrow) go(step_kernel<T, 4, 64>, 4); else if (vectors) go(step_kernel<T, 4, 256>, 1);
-        else if (narrow && a.value <= 64) go(step_kernel<T, 1, 64>, 4); else go(step_kernel<T, 1, 256>, 1);
+        launch_step<T>(device, a);
     };
     if (layer->type == RLT_TYPE_F32) views(0.0f); else views((rlt_bf16)0.0f);
     return rlt_launch_status(device);
