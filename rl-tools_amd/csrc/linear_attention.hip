@@ -693,21 +693,24 @@ template <typename T, int V, int THREADS> __global__ __launch_bounds__(256) void
     const bool work = pair < pairs;
     const int h = pair % a.heads, b = pair / a.heads, t = threadIdx.x % THREADS, columns = a.value / V, groups = THREADS / columns, g = t / columns, c = (t % columns) * V;
     vector out = {};
-    if (work && g < groups) {
+    if (work && a.lengths && a.lengths[b] <= 0) {      // a row without this step: its state stays, its output is zero
+        const size_t base = ((size_t)b * a.heads + h) * a.key * a.value;
+        for (int i = t; i < a.key * a.value; i += THREADS) a.exit[base + i] = a.entry ? a.entry[base + i] : 0.0f;
+    } else if (work && g < groups) {
         const T* const q = at<T>(a.q, 0, b, h); const T* const k = at<T>(a.k, 0, b, h); const T* const values = at<T>(a.v, 0, b, h) + c;
         const size_t base = ((size_t)b * a.heads + h) * a.key * a.value + c;
         const float decay = expf(a.log_decay[h]);
-        const bool stay = a.lengths && a.lengths[b] <= 0, forget = !a.entry || (!stay && a.reset && a.reset[b]);      // what a forgotten state holds reaches nothing, values that are not finite either
+        const bool forget = !a.entry || (a.reset && a.reset[b]);      // what a forgotten state holds reaches nothing, values that are not finite either
         vector v;
 #pragma unroll
-        for (int n = 0; n < V; n++) v[n] = stay ? 0.0f : (float)values[n];
+        for (int n = 0; n < V; n++) v[n] = (float)values[n];
         for (int i = g; i < a.key; i += AHEAD * groups) {
             vector s[AHEAD] = {};
             float ks[AHEAD], qs[AHEAD];
 #pragma unroll
             for (int j = 0; j < AHEAD; j++) {
                 const int at_key = i + j * groups, key = at_key < a.key ? at_key : i;
-                ks[j] = stay ? 0.0f : (float)k[key]; qs[j] = stay ? 0.0f : (float)q[key];
+                ks[j] = (float)k[key]; qs[j] = (float)q[key];
                 if (!forget) s[j] = *reinterpret_cast<const vector*>(a.entry + base + key * a.value);
             }
 #pragma unroll
@@ -715,8 +718,8 @@ template <typename T, int V, int THREADS> __global__ __launch_bounds__(256) void
                 const int key = i + j * groups;
                 if (key < a.key) {
 #pragma unroll
-                    for (int n = 0; n < V; n++) { s[j][n] = stay ? s[j][n] : fmaf(ks[j], v[n], s[j][n] * decay); out[n] = stay ? 0.0f : fmaf(qs[j], s[j][n], out[n]); }
-                    if (a.exit) *reinterpret_cast<vector*>(a.exit + base + key * a.value) = s[j];
+                    for (int n = 0; n < V; n++) { s[j][n] = fmaf(ks[j], v[n], s[j][n] * decay); out[n] = fmaf(qs[j], s[j][n], out[n]); }
+                    *reinterpret_cast<vector*>(a.exit + base + key * a.value) = s[j];
                 }
             }
         }
@@ -842,7 +845,7 @@ template <typename T> int forward(rlt_rocm_device* device, const rlt_linear_atte
     Walk a = walk_of(p, reset, lengths, steps);
     a.q = part<T>(q, 1, p->key_dim); a.k = part<T>(k, group, p->key_dim); a.v = part<T>(v, group, p->value_dim); a.out = part<T, 4>(output, 1, p->value_dim);
     a.entry = initial_state; a.exit = final_state;
-    if (steps == 1) {      // a pass over the states (9,639 rows, one head of 118, fp32: 235 us; 551 as a walk of one step)
+    if (steps == 1 && final_state) {      // a pass over the states (9,639 rows, one head of 118, fp32: 235 us; 551 as a walk of one step)
         launch_step<T>(device, a);
         return rlt_launch_status(device);
     }
