@@ -95,7 +95,7 @@ template <typename T, int D, bool SLOPE, bool STATE> struct Layout {
 // A wavefront owns some of the value columns: their state stays in its accumulators from chunk to chunk, laid out as the matrix instruction leaves them, which is (with the summands in an order of their own) how the
 // product with the queries takes them. Scores of a chunk are shared out in tiles of 16 x 16, weighted, and exchanged through LDS. SLOPE carries the state's derivative by the decay's logarithm along.
 // STATE: only the state, of a segment that starts from nothing. A launch may hold two walks over the same rows (gradients of keys and of values), whose workgroups take turns on an XCD and so find each other's inputs in its L2.
-// What bounds it: whole heads of 128 bfloat16 channels, the vector and matrix instructions of two wavefronts a SIMD (81 % busy) beside 4 TB/s: 4 rows x 16 heads, 8,192 steps, a walk forward 165 us, d_q with the slope 418, d_k and d_v 325;
+// What bounds it: whole heads of 128 bfloat16 channels, the vector and matrix instructions of two wavefronts a SIMD (81 % busy) beside 4 TB/s: 4 rows x 16 heads, 8,192 steps, a walk forward 165 us, d_q with the slope 397 to 420, d_k and d_v 320;
 // 16,384 steps of 16 heads forward 132 us in all. Short sequences in fp32, the parts of one chunk one after the other in eight wavefronts a compute unit, as many as LDS has room for (36 KB a workgroup of 32 channels): 64 steps,
 // 1,024 rows, 2 heads of 32: 32, 55 and 52 us, of which the matrix instructions take 8, 14 and 15. Fewer rows and heads than compute units leave a chunk's latency alone: 333 steps, 37 rows, 6 heads of 24 x 41: 46, 70 and 66 us.
 // Few steps on many rows: reading and writing the states, two wavefronts a SIMD: 20 steps, 2,240 rows, 8 heads of 64, bfloat16: 190, 346 and 340 us.
