@@ -72,9 +72,9 @@ __device__ __forceinline__ float power(const Log2& decay, int n) {
 }
 
 // Shape of a workgroup for heads of up to D channels: a wavefront owns TILES x 16 of the value columns. SPLIT workgroups share a head's columns where two states would not fit the registers of one: the scores are then
-// formed in each of them.
+// formed in each of them (bfloat16). fp32 takes one of eight wavefronts, which LDS has room for as it has for one of four (d_q of 2,846 heads of 64 x 127, 35 steps: 291 us, 524 with two workgroups a head).
 template <typename T, int D, bool SLOPE, bool STATE> struct Layout {
-    static constexpr int SPLIT = SLOPE && D == 128 ? 2 : 1, COLUMNS = D / SPLIT;
+    static constexpr int SPLIT = SLOPE && D == 128 && sizeof(T) == 2 ? 2 : 1, COLUMNS = D / SPLIT;
     static constexpr int TILES = D == 128 && sizeof(T) == 2 && !SLOPE ? 2 : 1, WAVES = COLUMNS / (16 * TILES), THREADS = 64 * WAVES;
     static constexpr int PAD = 16 / sizeof(T), ROW = D + PAD, COLUMN_ROW = COLUMNS + PAD, SCORES = CHUNK + PAD;      // rows start 4 (of 64) banks after each other: sixteen of them side by side in 16 bytes each meet no bank twice
     static constexpr int PLANES = sizeof(T) == 2 ? 2 : 1;
@@ -877,7 +877,7 @@ template <typename T> int backward(rlt_rocm_device* device, const rlt_linear_att
     a.entry = cut ? states : initial_state; a.entry_slope = cut ? slopes : nullptr; a.d_final = d_final_state; a.partial = (double*)(workspace + s.partial);
     rc = d_log_decay ? walk<T, T, false, true, false>(device, a) : walk<T, T, false, false, false>(device, a);
     if (rc) return rc;
-    if (d_log_decay) hipLaunchKernelGGL(decay_sum_kernel, dim3(p->heads), dim3(512), 0, device->stream, a.partial, p->batch, p->heads, a.segments * (p->key_dim > 64 || p->value_dim > 64 ? 2 : 1), d_log_decay, accumulate);
+    if (d_log_decay) hipLaunchKernelGGL(decay_sum_kernel, dim3(p->heads), dim3(512), 0, device->stream, a.partial, p->batch, p->heads, a.segments * (p->key_dim > 64 || p->value_dim > 64 ? Layout<T, 128, true, false>::SPLIT : 1), d_log_decay, accumulate);
     // the state's gradient, from the last step to the first; d_v reads it, d_k reads it across
     Walk r = walk_of(p, reset, lengths, steps);
     r.k = Q; r.v = G; r.read_scale = 1.0f; r.added_scale = p->scale;
