@@ -43,23 +43,23 @@ __device__ __forceinline__ rlt_f32x4 multiply(rlt_f32x8 a, rlt_f32x8 b, rlt_f32x
 }
 __device__ __forceinline__ rlt_f32x4 multiply(rlt_bf16x8 a, rlt_bf16x8 b, rlt_f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
-// fp32 values as operands. For bfloat16 kernels they are cut into parts whose sum they are to 2^-16 (two) or exactly to fp32 (three): what a product adds to the state, and what a gradient that stays in fp32 is made of, take three,
-// what only goes into an output that is rounded to bfloat16 takes two.
-template <typename T, int PARTS> struct Cut {
-    rlt_bf16x8 part[PARTS];
+// fp32 values (scores, states, weighted values) as operands. For bfloat16 kernels they are cut into three parts, whose sum they are exactly to fp32. (Two
+// leave 2^-18 of a value out, for which ten times as many outputs as with three are the second-nearest bfloat16 number.)
+template <typename T> constexpr int PARTS = sizeof(T) == 4 ? 1 : 3;
+template <typename T> struct Cut {
+    rlt_bf16x8 part[PARTS<T>];
     __device__ __forceinline__ explicit Cut(rlt_f32x8 x) {
 #pragma unroll
-        for (int p = 0; p < PARTS; p++) {
+        for (int p = 0; p < PARTS<T>; p++) {
             part[p] = __builtin_convertvector(x, rlt_bf16x8);
-            if (p + 1 < PARTS) x -= __builtin_convertvector(part[p], rlt_f32x8);
+            if (p + 1 < PARTS<T>) x -= __builtin_convertvector(part[p], rlt_f32x8);
         }
     }
 };
-template <int PARTS> struct Cut<float, PARTS> {
+template <> struct Cut<float> {
     rlt_f32x8 part[1];
     __device__ __forceinline__ explicit Cut(rlt_f32x8 x) { part[0] = x; }
 };
-template <typename T, int PARTS> constexpr int CUTS = sizeof(T) == 4 ? 1 : PARTS;
 
 // decay^n; n = 0 gives 1 also for a decay of zero. The logarithm to the base of 2 is a sum of two numbers: one alone is off by 2^-24 of itself, its n-fold by that of n times as much, and every row and step would meet the same error.
 struct Log2 {
@@ -77,7 +77,7 @@ template <typename T, int D, bool SLOPE, bool STATE> struct Layout {
     static constexpr int SPLIT = SLOPE && D == 128 && sizeof(T) == 2 ? 2 : 1, COLUMNS = D / SPLIT;
     static constexpr int TILES = D == 128 && sizeof(T) == 2 && !SLOPE ? 2 : 1, WAVES = COLUMNS / (16 * TILES), THREADS = 64 * WAVES;
     static constexpr int PAD = 16 / sizeof(T), ROW = D + PAD, COLUMN_ROW = COLUMNS + PAD, SCORES = CHUNK + PAD;      // rows start 4 (of 64) banks after each other: sixteen of them side by side in 16 bytes each meet no bank twice
-    static constexpr int PLANES = sizeof(T) == 2 ? 2 : 1;
+    static constexpr int PLANES = PARTS<T>;
     // keys, values, what the slope is multiplied with, the queries, the scores: in the queries' place (for a barrier more) where that leaves room for another workgroup, which 128 channels of two bytes have no registers for
     static constexpr bool OVER = !(D == 128 && sizeof(T) == 2 && !SLOPE);
     static constexpr int K = 0, V = K + CHUNK * ROW, W = V + CHUNK * COLUMN_ROW, Q = W + (SLOPE && !STATE ? CHUNK * COLUMN_ROW : 0), P = OVER ? Q : Q + CHUNK * ROW;
@@ -104,7 +104,7 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
     typedef typename Operand<T>::Vector Vector;
     typedef typename Operand<T>::Quad Quad;
     typedef Layout<T, D, SLOPE, STATE> L;
-    constexpr int KEY_TILES = D / 16, KEY_BLOCKS = D / 32, TILES = L::TILES, STATE_CUTS = CUTS<T, SLOPE ? 3 : 2>, ADDED_CUTS = CUTS<T, 3>;
+    constexpr int KEY_TILES = D / 16, KEY_BLOCKS = D / 32, TILES = L::TILES;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds_bytes[];
     T* const lds = (T*)lds_bytes;
     // weights of a chunk's steps: in the state after it, and of the state before it in their outputs
@@ -407,15 +407,15 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
                 for (int ot = 0; ot < STEP_TILES; ot++) q[ot] = tiled_operand(L::Q, 16 * ot + l, block);
 #pragma unroll
                 for (int tile = 0; tile < TILES; tile++) {
-                    const Cut<T, STATE_CUTS> s(__builtin_shufflevector(state[tile][2 * block], state[tile][2 * block + 1], 0, 1, 2, 3, 4, 5, 6, 7));
+                    const Cut<T> s(__builtin_shufflevector(state[tile][2 * block], state[tile][2 * block + 1], 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-                    for (int p = 0; p < STATE_CUTS; p++)
+                    for (int p = 0; p < PARTS<T>; p++)
 #pragma unroll
                         for (int ot = 0; ot < STEP_TILES; ot++) out[tile][ot] = multiply(s.part[p], q[ot], out[tile][ot]);
                     if constexpr (SLOPE) {
-                        const Cut<T, STATE_CUTS> d(__builtin_shufflevector(slope[tile][2 * block], slope[tile][2 * block + 1], 0, 1, 2, 3, 4, 5, 6, 7));
+                        const Cut<T> d(__builtin_shufflevector(slope[tile][2 * block], slope[tile][2 * block + 1], 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-                        for (int p = 0; p < STATE_CUTS; p++)
+                        for (int p = 0; p < PARTS<T>; p++)
 #pragma unroll
                             for (int ot = 0; ot < STEP_TILES; ot++) out_slope[tile][ot] = multiply(d.part[p], q[ot], out_slope[tile][ot]);
                     }
@@ -536,16 +536,16 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
                 for (int tile = 0; tile < TILES; tile++) {
                     const Vector v = column_operand(L::V, L::COLUMN_ROW, TILES * wave + tile, block);
                     const rlt_f32x8 weighted = __builtin_convertvector(v, rlt_f32x8) * weight;
-                    const Cut<T, ADDED_CUTS> x(weighted);
+                    const Cut<T> x(weighted);
                     if constexpr (SLOPE) {
                         const rlt_f32x8 lagged = __builtin_convertvector(v, rlt_f32x8) * *reinterpret_cast<const rlt_f32x8*>(lagged_weights + 32 * block + 8 * quarter);
-                        const Cut<T, ADDED_CUTS> y(lagged);
+                        const Cut<T> y(lagged);
 #pragma unroll
                         for (int k = 0; k < KEY_TILES; k++) {
                             if (!FULL && 16 * k >= a.key) break;
                             key[0] = column_operand(L::K, L::ROW, k, block);
 #pragma unroll
-                            for (int p = 0; p < ADDED_CUTS; p++) {
+                            for (int p = 0; p < PARTS<T>; p++) {
                                 state[tile][k] = multiply(key[0], x.part[p], state[tile][k]);
                                 slope[tile][k] = multiply(key[0], y.part[p], slope[tile][k]);
                             }
@@ -556,12 +556,11 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
                             if (16 * k >= a.key) break;
                             key[0] = column_operand(L::K, L::ROW, k, block);
 #pragma unroll
-                            for (int p = 0; p < ADDED_CUTS; p++) state[tile][k] = multiply(key[0], x.part[p], state[tile][k]);
+                            for (int p = 0; p < PARTS<T>; p++) state[tile][k] = multiply(key[0], x.part[p], state[tile][k]);
                         }
                     } else {
 #pragma unroll
-                        for (int p = 0; p < ADDED_CUTS; p++) {
-                            if (!STATE && p == 2 && !a.exit) break;      // a state that only goes into outputs of this type does with two parts
+                        for (int p = 0; p < PARTS<T>; p++) {
 #pragma unroll
                             for (int k = 0; k < KEY_TILES; k++) state[tile][k] = multiply(key[k], x.part[p], state[tile][k]);
                         }
