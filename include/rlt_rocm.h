@@ -1206,7 +1206,7 @@ enum rlt_type {
 
 /* A tensor [steps x rows x heads x channels]: element (t, b, h, c) is at data[t * step_stride + b * row_stride + h * head_stride + c], strides in elements, the channels
  * of a head side by side. Step-major sequences as the GRU's are step_stride = rows * heads * channels, row_stride = heads * channels, head_stride = channels; a part of a
- * wider tensor (queries, keys and values from one product) or another order of the axes differs in the strides alone. */
+ * wider tensor (queries, keys and values from one product) or another order of the axes differs in the strides alone. Strides may be negative (data is element (0, 0, 0, 0) all the same): a layer that runs from a sequence's end to its start. */
 typedef struct rlt_head_view {
     void* data;
     int64_t step_stride, row_stride, head_stride;

@@ -184,7 +184,7 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
     uint8_t next_reset = 0;
     constexpr std::integral_constant<int, D> whole{};
     constexpr std::integral_constant<int, L::COLUMNS> columns{};
-    // Whole chunks of whole heads: a uniform address and a thread's offset in bytes (32 bits: the strides of FULL tensors leave room).
+    // Whole chunks of whole heads: a uniform address and a thread's offset in bytes, which is added without a sign (32 bits: the steps of FULL tensors go forward in memory and leave room).
     auto offset_of = [&](const Part& p, int from, auto across) {
         constexpr int ACROSS = decltype(across)::value;
         unsigned thread = threadIdx.x;
@@ -799,7 +799,7 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
 // FULL: heads of exactly D channels, all of whose tensors may be read and written in vectors
 template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE> int walk_width(rlt_rocm_device* device, const Walk& a, const Walk* second) {
     auto full = [&](const Walk& w) {
-        auto near = [](const Part& p) { return p.step > -(1 << 22) && p.step < 1 << 22; };      // a chunk's offsets in bytes fit 32 bits
+        auto near = [](const Part& p) { return p.step >= 0 && p.step < 1 << 22; };      // a chunk's offsets in bytes fit 32 bits without a sign; steps that go back in memory take 64-bit addresses
         if (!near(w.k) || !near(w.v) || (!STATE && !near(w.q)) || (SLOPE && !STATE && !near(w.with))) return false;
         return w.key == D && w.value == D && w.k.vectors && w.v.vectors && (STATE || (w.q.vectors && w.out.vectors)) && (!SLOPE || STATE || w.with.vectors);
     };

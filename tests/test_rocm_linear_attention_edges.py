@@ -4,10 +4,25 @@ import ctypes as C
 import numpy as np
 import pytest
 
-from test_rocm_linear_attention import Tensor, case, layer_of, reference, workspace
-from typed_arrays import filled, rounded
+from test_rocm_linear_attention import Tensor, case, check, layer_of, reference, strides_of, view, workspace
+from typed_arrays import download, filled, rounded, upload
 
 gpu = pytest.mark.gpu
+
+
+class Backwards(Tensor):
+    """A tensor whose axes of `axes` lie in memory from the last index to the first: the view starts at element (0, 0, 0, 0) and its strides there are negative."""
+
+    def __init__(self, rocm, x, dtype, axes, value=None):
+        self.rocm, self.dtype, self.axes = rocm, dtype, axes
+        self.shape = self.padded = x.shape if value is None else x
+        host = np.full(self.shape, value, np.float32) if value is not None else x
+        self.array, strides = upload(rocm, np.flip(host, axes), dtype), strides_of(self.shape, (0, 1, 2))
+        first = sum((self.shape[a] - 1) * strides[a] for a in axes)
+        self.view = view(self.array, [-s if a in axes else s for a, s in enumerate(strides)], 4 if dtype == "float32" else 2, first)
+
+    def whole(self):
+        return np.flip(download(self.array, self.dtype).reshape(self.shape), self.axes)
 
 
 def run(rocm, c, x, tensor=None):
@@ -46,3 +61,18 @@ def test_bfloat16_outputs_are_rounded_once(rocm, steps, rows, heads, d):
         others = np.sum(got[n] != rounded(want[n], "bfloat16"))
         print(n, want[n].size, "elements", others, "elsewhere, at most", expected, flush=True)
         assert others <= expected + 5 * expected ** 0.5, n
+
+
+# ------------------------------------------------------------------ views
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("dk,dv", [(32, 32), (64, 64), (128, 128), (24, 41)])
+@pytest.mark.parametrize("steps,rows", [(130, 3), (900, 1)])
+def test_views_that_go_back_in_memory(rocm, dk, dv, steps, rows, dtype):
+    """steps, and steps, rows and heads, with strides below zero: heads of whole tiles and others, whole and cut chunks, one segment and several"""
+    print("case", steps, rows, dk, dv, dtype, flush=True)
+    c, x = case(43, dtype, steps, rows, 4, 2, dk, dv, resets=0.02, ragged=rows > 1)
+    for axes in ((0,), (0, 1, 2)):
+        check(c, x, run(rocm, c, x, lambda x, value=None: Backwards(rocm, x, dtype, axes, value)))
