@@ -1230,8 +1230,8 @@ typedef struct rlt_linear_attention {
 size_t rlt_rocm_linear_attention_workspace_bytes(const rlt_linear_attention* layer, int steps, int backward);
 /* All steps of a sequence. initial_state, final_state [batch x heads x key_dim x value_dim] (NULL: zeros / not wanted; they may be the same buffer); reset [steps x batch] (NULL: none): a row whose
  * flag is set at step t forgets its state (the initial one too) before that step; lengths [batch] (NULL: all of them): row b has lengths[b] steps (clamped to 0 ... steps), its
- * output beyond them is zero, its state stays, and what its inputs hold there is not looked at. Within a sequence a NaN or an infinity in an input may reach the outputs of up to 63 steps
- * before it, whatever the resets say. */
+ * output beyond them is zero, its state stays, and what its inputs hold there is not looked at. A NaN or an infinity in
+ * an input reaches the steps of its episode that see it and no others, as it does step by step (which of the two it is there is not said). */
 int rlt_rocm_linear_attention_forward(rlt_rocm_device* device, const rlt_linear_attention* layer, const rlt_head_view* q, const rlt_head_view* k, const rlt_head_view* v,
                                       const rlt_head_view* output, const float* initial_state, float* final_state, const uint8_t* reset, const int32_t* lengths, int steps,
                                       void* workspace, size_t workspace_bytes);

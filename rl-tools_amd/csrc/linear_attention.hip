@@ -61,6 +61,27 @@ template <> struct Cut<float> {
     __device__ __forceinline__ explicit Cut(rlt_f32x8 x) { part[0] = x; }
 };
 
+// whether some of 16-byte vectors' values are not finite (exponents of ones)
+template <int N> __device__ __forceinline__ bool not_finite(const rlt_f32x4 (&x)[N]) {
+    float zero = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) zero = fmaf(x[i][e], 0.0f, zero);
+    return zero != 0.0f;
+}
+template <int N> __device__ __forceinline__ bool not_finite(const rlt_bf16x8 (&x)[N]) {
+    typedef unsigned Words __attribute__((ext_vector_type(4)));
+    unsigned carried = 0;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const Words w = __builtin_bit_cast(Words, x[i]);
+#pragma unroll
+        for (int e = 0; e < 4; e++) carried |= (w[e] & 0x7f807f80u) + 0x00800080u;      // two to a word
+    }
+    return (carried & 0x80008000u) != 0;
+}
+
 // decay^n; n = 0 gives 1 also for a decay of zero. The logarithm to the base of 2 is a sum of two numbers: one alone is off by 2^-24 of itself, its n-fold by that of n times as much, and every row and step would meet the same error.
 struct Log2 {
     float high, low;
@@ -83,7 +104,7 @@ template <typename T, int D, bool SLOPE, bool STATE> struct Layout {
     static constexpr int K = 0, V = K + CHUNK * ROW, W = V + CHUNK * COLUMN_ROW, Q = W + (SLOPE && !STATE ? CHUNK * COLUMN_ROW : 0), P = OVER ? Q : Q + CHUNK * ROW;
     static constexpr int FLAGS = STATE ? Q : OVER && ROW > PLANES * SCORES ? Q + CHUNK * ROW : P + CHUNK * PLANES * SCORES;
     static constexpr int SCORE_TILES = (10 + WAVES - 1) / WAVES;      // of a wavefront
-    static constexpr size_t BYTES = FLAGS * sizeof(T) + (4 * CHUNK + 16 + WAVES) * sizeof(float);
+    static constexpr size_t BYTES = FLAGS * sizeof(T) + (4 * CHUNK + 16 + 2 * WAVES) * sizeof(float);
     // wavefronts that the registers of a SIMD are shared by: as many as LDS has room for workgroups
     static constexpr int FIT = (int)(163840 / BYTES) * WAVES / 4, MOST = D == 128 || (SLOPE && !STATE) ? 2 : 3, RESIDENT = FIT < 1 ? 1 : FIT > MOST ? MOST : FIT;
 };
@@ -310,17 +331,8 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
         settle_chunk(n);
         if (resets & ~1ull) {
             // A step's weight of zero keeps other episodes out of sums of products as long as their values are finite. Where some are not, the chunk ends at its first reset (REVERSE: begins at its last).
-            float zero = 0.0f;
-#pragma unroll
-            for (int round = 0; round < ROUNDS; round++)
-#pragma unroll
-                for (int c = 0; c < V; c++) zero = fmaf((float)next_k[round][c], 0.0f, zero);
-#pragma unroll
-            for (int round = 0; round < COLUMN_ROUNDS; round++)
-#pragma unroll
-                for (int c = 0; c < V; c++) zero = fmaf((float)next_v[round][c], 0.0f, zero);
-            const bool all = __all(zero == 0.0f);
-            if (lane == 0) flags[wave] = all ? 0.0f : 1.0f;
+            const bool some = __any(not_finite(next_k) || not_finite(next_v));
+            if (lane == 0) flags[wave] = some ? 1.0f : 0.0f;
         }
         rlt_lds_barrier();
         if (resets & ~1ull) {
@@ -346,6 +358,10 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
         }
         put(L::K, next_k, whole);
         put(L::V, next_v, columns);
+        if constexpr (!STATE) {
+            const bool some = __any(not_finite(next_v));
+            if (lane == 0) flags[L::WAVES + wave] = some ? 1.0f : 0.0f;
+        }
         if constexpr (!STATE) put(L::Q, next_q, whole);
         if constexpr (SLOPE && !STATE) put(L::W, next_with, columns);
         rlt_lds_barrier();
@@ -458,6 +474,9 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
             // the tiles on the wrong side of the diagonal that are multiplied all the same, as halves of blocks of 32
             for (int which = wave; which < 2 * L::PLANES; which += L::WAVES)
                 *reinterpret_cast<Quad*>(lds + L::P + which / 2 * CHUNK * L::SCORES + (32 * (which % 2) + (REVERSE ? 16 : 0) + l) * L::SCORES + 32 * (which % 2) + (REVERSE ? 0 : 16) + 4 * quarter) = Quad{};
+            float apart = 0.0f;
+#pragma unroll
+            for (int w = 0; w < L::WAVES; w++) apart += flags[L::WAVES + w];
             rlt_lds_barrier();
             if constexpr (SLOPE) { if (!done) fetch_chunk(next_t0, next_stop); }      // only here: the products with two states before leave no registers for it
             // what the chunk's own steps give
@@ -480,7 +499,24 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
                     }
             }
             };
-            if (!idle) by_steps(n, within);
+            if (__builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, apart)) == 0) { if (!idle) by_steps(n, within); }
+            else if (!idle) {      // zero times a value that is not finite is not zero: one step after the other goes to the steps that see it
+#pragma unroll 1
+                for (int s = 0; s < n; s++)
+#pragma unroll
+                    for (int ot = 0; ot < 4; ot++) {
+                        const int i = 16 * ot + l;
+                        float weight = 0.0f;
+#pragma unroll
+                        for (int plane = 0; plane < L::PLANES; plane++) weight += (float)lds[L::P + plane * CHUNK * L::SCORES + i * L::SCORES + s];
+#pragma unroll
+                        for (int tile = 0; tile < TILES; tile++) {
+                            const Quad v = *reinterpret_cast<const Quad*>(lds + L::V + s * L::COLUMN_ROW + inner0 + 16 * tile + 4 * quarter);
+#pragma unroll
+                            for (int r = 0; r < 4; r++) { const float x = fmaf(weight, (float)v[r], out[tile][ot][r]); out[tile][ot][r] = (REVERSE ? s >= i : s <= i) ? x : out[tile][ot][r]; }
+                        }
+                    }
+            }
             typedef typename Operand<O>::Quad OutQuad;
             O* const to = lane_out + t0 * a.out.step;
 #pragma unroll

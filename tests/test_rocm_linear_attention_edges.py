@@ -4,7 +4,7 @@ import ctypes as C
 import numpy as np
 import pytest
 
-from test_rocm_linear_attention import Tensor, case, check, layer_of, reference, strides_of, view, workspace
+from test_rocm_linear_attention import Tensor, bounds, case, check, layer_of, magnitudes, reference, strides_of, view, workspace
 from typed_arrays import download, filled, rounded, upload
 
 gpu = pytest.mark.gpu
@@ -76,3 +76,27 @@ def test_views_that_go_back_in_memory(rocm, dk, dv, steps, rows, dtype):
     c, x = case(43, dtype, steps, rows, 4, 2, dk, dv, resets=0.02, ragged=rows > 1)
     for axes in ((0,), (0, 1, 2)):
         check(c, x, run(rocm, c, x, lambda x, value=None: Backwards(rocm, x, dtype, axes, value)))
+
+
+# ------------------------------------------------------------------ values that are not finite
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("steps,rows,dk,dv", [(200, 3, 32, 32), (200, 2, 64, 48), (150, 2, 128, 128), (90, 3, 24, 41), (20, 2, 64, 64), (900, 1, 128, 128)])
+@pytest.mark.parametrize("name", ["q", "k", "v", "d_output"])
+def test_values_that_are_not_finite_reach_what_sees_them(rocm, steps, rows, dk, dv, name, dtype):
+    """One channel of one row and head at some steps, no resets: outputs of the steps before, gradients of the steps behind, and channels that the value has no part in are as if it were finite, the others are not finite. What
+    is finite in the recurrence itself, step by step in 64 bits, is what the formulas leave alone."""
+    print("case", steps, rows, dk, dv, name, dtype, flush=True)
+    c, x = case(53, dtype, steps, rows, 2, 2, dk, dv)
+    for at, value in ((0, np.inf), (steps // 2 + 3, np.nan), (min(63, steps - 1), -np.inf), (steps - 1, np.nan)):
+        y = {n: a.copy() for n, a in x.items()}
+        y[name][at, 0, 1, dv // 3 if name in ("v", "d_output") else dk // 3] = value
+        with np.errstate(invalid="ignore"):
+            want = reference(c, y)
+        b, got = bounds(c, reference(c, x), magnitudes(c, x)), run(rocm, c, y)
+        for n in ("output", "state", "d_q", "d_k", "d_v", "d_state"):
+            finite = np.isfinite(want[n])
+            assert np.array_equal(np.isfinite(got[n]), finite), (n, at, value)
+            assert np.all(np.abs(got[n][finite] - want[n][finite]) <= b[n][finite]), (n, at, value)
