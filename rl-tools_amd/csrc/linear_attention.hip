@@ -89,7 +89,7 @@ struct Log2 {
 };
 __device__ __forceinline__ float power(const Log2& decay, int n) {
     const float at = decay.high * (float)n, p = __builtin_amdgcn_exp2f(at), rest = fmaf(decay.high, (float)n, -at) + decay.low * (float)n;
-    return n == 0 ? 1.0f : at > -126.0f ? fmaf(p, rest * 0.6931471805599453f, p) : p;
+    return n == 0 ? 1.0f : fabsf(at) < 126.0f ? fmaf(p, rest * 0.6931471805599453f, p) : p;      // powers beyond fp32 are 0 or infinity as they are
 }
 
 // Shape of a workgroup for heads of up to D channels: a wavefront owns TILES x 16 of the value columns. SPLIT workgroups share a head's columns where two states would not fit the registers of one: the scores are then

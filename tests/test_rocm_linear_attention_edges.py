@@ -100,3 +100,18 @@ def test_values_that_are_not_finite_reach_what_sees_them(rocm, steps, rows, dk, 
             finite = np.isfinite(want[n])
             assert np.array_equal(np.isfinite(got[n]), finite), (n, at, value)
             assert np.all(np.abs(got[n][finite] - want[n][finite]) <= b[n][finite]), (n, at, value)
+
+
+@gpu
+@pytest.mark.parametrize("log_decay,steps", [(0.02, 200), (0.5, 300), (2.0, 70), (30.0, 40)])
+def test_states_that_grow_beyond_fp32_are_infinite(rocm, log_decay, steps):
+    """A logarithm above zero and sums of products of numbers from 1 on alone, which pass fp32's largest number on their way: what is beyond it by more than its bound is infinite, not a NaN."""
+    c, x = case(59, "float32", steps, 1, 2, 2, 32, 32, log_decay=[log_decay, log_decay / 2])
+    x = {n: (a if n == "log_decay" else (np.abs(a) + 1).astype(np.float32).astype(a.dtype)) for n, a in x.items()}
+    c["scale"] = 1.0
+    with np.errstate(over="ignore", invalid="ignore"):
+        want, got, largest = reference(c, x), run(rocm, c, x), float(np.finfo(np.float32).max)
+        b = bounds(c, want, want)
+        for n in ("output", "state", "d_q", "d_k", "d_v", "d_state"):
+            surely, within = (want[n] - b[n] > largest) | np.isinf(want[n]), want[n] + b[n] < largest
+            assert np.all(got[n][surely] == np.inf) and np.all(np.abs(got[n] - want[n])[within] <= b[n][within]), (n, log_decay)
