@@ -1216,7 +1216,8 @@ typedef struct rlt_head_view {
  *     S_t = a_t S_{t-1} + k_t^T v_t,   output_t = scale * q_t S_t,   a_t = exp(log_decay[head]), or nothing at a reset.
  * Query head h reads key / value head h / (heads / kv_heads); every query head has its own decay and state. key_dim and value_dim up to 128, sequences up to 2^30 steps. */
 typedef struct rlt_linear_attention {
-    const float* log_decay;      /* [heads], <= 0 for a state that forgets (-infinity: only the step itself) */
+    const float* log_decay;      /* [heads], <= 0 for a state that forgets (-infinity: only the step itself). Above 0 it grows, from 1.38 (exp(64 log_decay) beyond fp32) on perhaps to NaN
+                                  * where step by step it were infinite, or zero */
     float scale;
     int32_t type;                /* enum rlt_type of q, k, v, the output and their gradients */
     int32_t batch;               /* rows */

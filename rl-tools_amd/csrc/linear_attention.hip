@@ -140,6 +140,7 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
     int l = lane & 15, quarter = lane >> 4;
     const int length = a.lengths ? min(max(a.lengths[b], 0), a.steps) : a.steps;
     const Log2 log2_decay(a.log_decay[h]);
+    const bool grows = log2_decay.high >= 2.0f;      // weights of a chunk may be infinite: scores of zero (of steps beyond the chunk's n) are kept from them
     const bool last = segment == (REVERSE ? 0 : a.segments - 1);      // of the walk
     if (STATE && last && !a.last_wanted) return;                      // no segment starts from the state after it
     const int begin = segment * a.segment_steps, end = min(begin + a.segment_steps, a.steps);
@@ -389,8 +390,13 @@ template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, b
                 }
                 const int i = 16 * ot + l;
                 const float* const weight = score_weights + (REVERSE ? 16 * (st - ot) + 4 * quarter - l : 16 * (ot - st) + l - 4 * quarter);
+                if (grows) {
 #pragma unroll
-                for (int r = 0; r < 4; r++) { const float w = weight[REVERSE ? r : -r]; x[r] = w != 0.0f ? x[r] * w : 0.0f; }
+                    for (int r = 0; r < 4; r++) { const float w = weight[REVERSE ? r : -r]; x[r] = w != 0.0f && x[r] != 0.0f ? x[r] * w : 0.0f; }
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; r++) { const float w = weight[REVERSE ? r : -r]; x[r] = w != 0.0f ? x[r] * w : 0.0f; }
+                }
                 if (resets) {
                     const uint64_t before = resets & ((2ull << i) - 1), after = i < 63 ? resets & ~((2ull << i) - 1) : 0;
                     const int low = REVERSE ? 0 : before ? 63 - __builtin_clzll(before) : 0, high = REVERSE && after ? __builtin_ctzll(after) - 1 : 63;      // steps of the episode of step i
