@@ -1237,7 +1237,8 @@ int rlt_rocm_linear_attention_forward(rlt_rocm_device* device, const rlt_linear_
                                       const rlt_head_view* output, const float* initial_state, float* final_state, const uint8_t* reset, const int32_t* lengths, int steps,
                                       void* workspace, size_t workspace_bytes);
 /* Gradients through time, from the layer's inputs alone (the forward pass keeps nothing): d_q, d_k, d_v (zero beyond a row's length), d_initial_state (NULL: not wanted), d_log_decay [heads]
- * (NULL: not wanted; accumulate = 0 overwrites it, 1 adds to it). d_final_state is the gradient with respect to final_state (NULL: zeros). */
+ * (NULL: not wanted; accumulate = 0 overwrites it, 1 adds to it). d_final_state is the gradient with respect to final_state (NULL: zeros); d_initial_state may be
+ * the same buffer, as where the gradient goes on to the sequence before. Outputs overlap no other buffer of their call but where these comments say so. */
 int rlt_rocm_linear_attention_backward(rlt_rocm_device* device, const rlt_linear_attention* layer, const rlt_head_view* q, const rlt_head_view* k, const rlt_head_view* v,
                                        const rlt_head_view* d_output, const rlt_head_view* d_q, const rlt_head_view* d_k, const rlt_head_view* d_v,
                                        const float* initial_state, const float* d_final_state, float* d_initial_state, float* d_log_decay, int accumulate,

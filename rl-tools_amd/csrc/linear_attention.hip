@@ -928,16 +928,19 @@ template <typename T> int backward(rlt_rocm_device* device, const rlt_linear_att
     r.q = K;
     if (!cut) r.exit = d_initial_state;
     w.q = V; w.k = G; w.v = Q; w.key = p->value_dim; w.value = p->key_dim; w.state_key = 1; w.state_value = p->value_dim;
+    const bool in_place = r.exit && r.exit == r.entry;      // d_k's walk has read the state's gradient before d_v's overwrites it: one launch after the other
     if (group == 1) {
         r.out = part<T, 4>(d_v, 1, p->value_dim); w.out = part<T, 4>(d_k, 1, p->key_dim);
-        return walk<T, T, true, false, false>(device, r, &w);
+        if (in_place && (rc = walk<T, T, true, false, false>(device, w))) return rc;
+        return walk<T, T, true, false, false>(device, r, in_place ? nullptr : &w);
     }
     // shared keys and values: every head's share in fp32, then the sums over the heads
     const size_t tokens = (size_t)steps * p->batch;
     auto shares = [&](float* base, int width) { return Part{base, (int64_t)p->batch * p->heads * width, (int64_t)p->heads * width, width, 1, width % 4 == 0}; };
     float* const shared_v = workspace + s.shared; float* const shared_k = shared_v + padded(tokens * p->heads * p->value_dim);
     r.out = shares(shared_v, p->value_dim); w.out = shares(shared_k, p->key_dim);
-    if ((rc = walk<T, float, true, false, false>(device, r, &w))) return rc;
+    if (in_place && (rc = walk<T, float, true, false, false>(device, w))) return rc;
+    if ((rc = walk<T, float, true, false, false>(device, r, in_place ? nullptr : &w))) return rc;
     const HeadSum sum_v = {shared_v, part<T, 4>(d_v, 1, p->value_dim), p->value_dim}, sum_k = {shared_k, part<T, 4>(d_k, 1, p->key_dim), p->key_dim};
     if (p->value_dim % 4 == 0 && p->key_dim % 4 == 0) hipLaunchKernelGGL((head_sum_kernel<T, 4>), dim3(2048, 2), dim3(256), 0, device->stream, sum_v, sum_k, tokens, p->batch, p->kv_heads, group);
     else hipLaunchKernelGGL((head_sum_kernel<T, 1>), dim3(2048, 2), dim3(256), 0, device->stream, sum_v, sum_k, tokens, p->batch, p->kv_heads, group);

@@ -25,8 +25,8 @@ class Backwards(Tensor):
         return np.flip(download(self.array, self.dtype).reshape(self.shape), self.axes)
 
 
-def run(rocm, c, x, tensor=None):
-    """forward and backward, all outputs in 64 bits; tensor(x or shape, value) makes the tensors of heads"""
+def run(rocm, c, x, tensor=None, in_place=False):
+    """forward and backward, all outputs in 64 bits; tensor(x or shape, value) makes the tensors of heads; in_place: the states' gradients in one buffer"""
     tensor = tensor or (lambda x, value=None: Tensor(rocm, x, c["dtype"], value=value))
     layer, steps = layer_of(rocm, c, x), c["steps"]
     t = {n: tensor(x[n]) for n in ("q", "k", "v", "d_output")}
@@ -34,7 +34,7 @@ def run(rocm, c, x, tensor=None):
     state, d_state, reset, lengths = (rocm.array(x[n]) if x.get(n) is not None else None for n in ("state", "d_state", "reset", "lengths"))
     ptr = lambda a: a.ptr if a is not None else None
     shape = (c["rows"], c["heads"], c["dk"], c["dv"])
-    final, d_initial, d_rate = filled(rocm, shape, "float32"), filled(rocm, shape, "float32"), filled(rocm, (c["heads"],), "float32")
+    final, d_initial, d_rate = filled(rocm, shape, "float32"), d_state if in_place else filled(rocm, shape, "float32"), filled(rocm, (c["heads"],), "float32")
     w, n = workspace(rocm, layer, steps, 0)
     rocm.call("linear_attention_forward", C.byref(layer), t["q"].view, t["k"].view, t["v"].view, o["output"].view, ptr(state), final.ptr, ptr(reset), ptr(lengths), steps, w.ptr, n)
     w, n = workspace(rocm, layer, steps, 1)
@@ -115,3 +115,17 @@ def test_states_that_grow_beyond_fp32_are_infinite(rocm, log_decay, steps):
         for n in ("output", "state", "d_q", "d_k", "d_v", "d_state"):
             surely, within = (want[n] - b[n] > largest) | np.isinf(want[n]), want[n] + b[n] < largest
             assert np.all(got[n][surely] == np.inf) and np.all(np.abs(got[n] - want[n])[within] <= b[n][within]), (n, log_decay)
+
+
+# ------------------------------------------------------------------ buffers
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("steps,rows,heads,kv_heads,dk,dv", [(70, 300, 4, 4, 32, 32), (30, 200, 4, 2, 64, 48), (1, 900, 2, 2, 128, 128), (900, 1, 2, 2, 64, 64), (900, 1, 2, 1, 128, 96)])
+def test_the_states_gradient_in_place(rocm, steps, rows, heads, kv_heads, dk, dv, dtype):
+    """one buffer for the final and the initial state's gradient, bit for bit as two, in one segment and several"""
+    c, x = case(61, dtype, steps, rows, heads, kv_heads, dk, dv, resets=0.02, ragged=True)
+    two, one = run(rocm, c, x), run(rocm, c, x, in_place=True)
+    for n in two:
+        assert np.array_equal(two[n], one[n]), n
