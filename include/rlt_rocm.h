@@ -1214,7 +1214,9 @@ typedef struct rlt_head_view {
 
 /* Linear attention with a decay for each head, a recurrent layer whose state is a matrix [key_dim x value_dim] per row and head:
  *     S_t = a_t S_{t-1} + k_t^T v_t,   output_t = scale * q_t S_t,   a_t = exp(log_decay[head]), or nothing at a reset.
- * Query head h reads key / value head h / (heads / kv_heads); every query head has its own decay and state. key_dim and value_dim up to 128, sequences up to 2^30 steps. */
+ * Query head h reads key / value head h / (heads / kv_heads); every query head has its own decay and state. key_dim and value_dim up to 128, sequences up to 2^30 steps, and as many
+ * rows x heads as a launch of 2^32 threads takes: 4.19 million for gradients of fp32 heads wider than 64, twice as many for other heads wider than 32, 8.38 million forward for fp32 heads wider than 64, 16.7 million for others and for single steps, at the least.
+ * Anything beyond is RLT_E_UNSUPPORTED before anything is launched. */
 typedef struct rlt_linear_attention {
     const float* log_decay;      /* [heads], <= 0 for a state that forgets (-infinity: only the step itself). Above 0 it grows, from 1.38 (exp(64 log_decay) beyond fp32) on perhaps to NaN
                                   * where step by step it were infinite, or zero */
@@ -1226,7 +1228,7 @@ typedef struct rlt_linear_attention {
     int32_t reserved;
 } rlt_linear_attention;
 
-/* Scratch memory of a forward (backward = 0) or backward (1) call over `steps` steps; depends on the shapes alone. A workspace starts on
+/* Scratch memory of a forward (backward = 0) or backward (1) call over `steps` steps (0 for a call that is refused); depends on the shapes alone. A workspace starts on
  * a 16-byte boundary and belongs to one call at a time. */
 size_t rlt_rocm_linear_attention_workspace_bytes(const rlt_linear_attention* layer, int steps, int backward);
 /* All steps of a sequence. initial_state, final_state [batch x heads x key_dim x value_dim] (NULL: zeros / not wanted; they may be the same buffer); reset [steps x batch] (NULL: none): a row whose

@@ -871,13 +871,33 @@ template <typename T, bool REVERSE, bool SLOPE> int segment_states(rlt_rocm_devi
     return rlt_launch_status(device);
 }
 
-template <typename T> void launch_step(rlt_rocm_device* device, const Walk& a) {
+template <typename T> int launch_step(rlt_rocm_device* device, const Walk& a) {
     const unsigned pairs = (unsigned)a.heads * a.batch;
-    const bool vectors = a.value % 4 == 0 && (reinterpret_cast<uintptr_t>(a.entry) | reinterpret_cast<uintptr_t>(a.exit)) % 16 == 0, narrow = a.key * a.value <= STEP_NARROW;
-    auto go = [&](auto kernel, unsigned at_once) { hipLaunchKernelGGL(kernel, dim3((pairs + at_once - 1) / at_once), dim3(256), 0, device->stream, a, pairs); };
-    if (vectors && narrow) go(step_kernel<T, 4, 64>, 4); else if (vectors) go(step_kernel<T, 4, 256>, 1);
-    else if (narrow && a.value <= 64) go(step_kernel<T, 1, 64>, 4); else go(step_kernel<T, 1, 256>, 1);
+    const bool vectors = a.value % 4 == 0 && (reinterpret_cast<uintptr_t>(a.entry) | reinterpret_cast<uintptr_t>(a.exit)) % 16 == 0, narrow = a.key * a.value <= STEP_NARROW && (vectors || a.value <= 64);
+    const unsigned at_once = narrow ? 4 : 1, blocks = (pairs + at_once - 1) / at_once;
+    if (blocks > UINT32_MAX / 256) return RLT_E_UNSUPPORTED;
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 0, device->stream, a, pairs); };
+    if (vectors && narrow) go(step_kernel<T, 4, 64>); else if (vectors) go(step_kernel<T, 4, 256>);
+    else if (narrow) go(step_kernel<T, 1, 64>); else go(step_kernel<T, 1, 256>);
+    return rlt_launch_status(device);
 }
+
+// Whether a call's launches have fewer than 2^32 threads, which is what a dimension of a grid holds; asked before the first of them. `decays`: with the decays' gradient.
+enum Call { FORWARD, BACKWARD };
+template <typename T> bool launchable(const rlt_linear_attention* p, Call call, bool decays) {
+    const uint64_t pairs = (uint64_t)p->batch * p->heads;
+    auto of = [&](auto width) {
+        constexpr int D = decltype(width)::value;
+        typedef Layout<T, D, false, false> Plain;
+        typedef Layout<T, D, true, false> Sloped;
+        if (call == FORWARD) return pairs * Plain::THREADS;
+        const uint64_t both = (pairs + 7) / 8 * 16 * Plain::THREADS, sloped = decays ? pairs * Sloped::SPLIT * Sloped::THREADS : 0, sums = decays ? (uint64_t)p->heads * 512 : 0;
+        return both > sloped ? (both > sums ? both : sums) : (sloped > sums ? sloped : sums);
+    };
+    const int width = p->key_dim > p->value_dim ? p->key_dim : p->value_dim;
+    return (width <= 32 ? of(std::integral_constant<int, 32>{}) : width <= 64 ? of(std::integral_constant<int, 64>{}) : of(std::integral_constant<int, 128>{})) <= UINT32_MAX;
+}
+bool launchable(const rlt_linear_attention* p, Call call, bool decays) { return p->type == RLT_TYPE_F32 ? launchable<float>(p, call, decays) : launchable<rlt_bf16>(p, call, decays); }
 
 template <typename T> int forward(rlt_rocm_device* device, const rlt_linear_attention* p, const rlt_head_view* q, const rlt_head_view* k, const rlt_head_view* v, const rlt_head_view* output,
                                   const float* initial_state, float* final_state, const uint8_t* reset, const int32_t* lengths, int steps, float* workspace) {
@@ -886,10 +906,7 @@ template <typename T> int forward(rlt_rocm_device* device, const rlt_linear_atte
     Walk a = walk_of(p, reset, lengths, steps);
     a.q = part<T>(q, 1, p->key_dim); a.k = part<T>(k, group, p->key_dim); a.v = part<T>(v, group, p->value_dim); a.out = part<T, 4>(output, 1, p->value_dim);
     a.entry = initial_state; a.exit = final_state;
-    if (steps == 1 && final_state) {      // a pass over the states (9,639 rows, one head of 118, fp32: 235 us; 551 as a walk of one step)
-        launch_step<T>(device, a);
-        return rlt_launch_status(device);
-    }
+    if (steps == 1 && final_state) return launch_step<T>(device, a);      // a pass over the states (9,639 rows, one head of 118, fp32: 235 us; 551 as a walk of one step)
     if (a.segments > 1) {
         const int rc = segment_states<T, false, false>(device, a, initial_state, final_state, workspace + s.states, nullptr, (float2*)(workspace + s.factors));
         if (rc) return rc;
@@ -952,7 +969,7 @@ template <typename T> int backward(rlt_rocm_device* device, const rlt_linear_att
 extern "C" {
 
 size_t rlt_rocm_linear_attention_workspace_bytes(const rlt_linear_attention* layer, int steps, int backward) {
-    if (!described(layer) || steps <= 0 || steps > MAX_STEPS) return 0;
+    if (!described(layer) || !supported(layer) || steps <= 0 || steps > MAX_STEPS || !launchable(layer, backward ? BACKWARD : FORWARD, false)) return 0;
     return scratch_of(layer, steps, backward != 0).total * sizeof(float);
 }
 
@@ -961,9 +978,9 @@ int rlt_rocm_linear_attention_forward(rlt_rocm_device* device, const rlt_linear_
                                       void* workspace, size_t workspace_bytes) {
     if (!device) return RLT_E_NOT_INITIALISED;
     RLT_REQUIRE(described(layer) && layer->log_decay && steps > 0 && given(q) && given(k) && given(v) && given(output));
+    if (!supported(layer) || steps > MAX_STEPS || (!(steps == 1 && final_state) && !launchable(layer, FORWARD, false))) return RLT_E_UNSUPPORTED;
     const size_t need = rlt_rocm_linear_attention_workspace_bytes(layer, steps, 0);
     RLT_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0));
-    if (!supported(layer) || steps > MAX_STEPS) return RLT_E_UNSUPPORTED;
     return layer->type == RLT_TYPE_F32 ? forward<float>(device, layer, q, k, v, output, initial_state, final_state, reset, lengths, steps, (float*)workspace)
                                        : forward<rlt_bf16>(device, layer, q, k, v, output, initial_state, final_state, reset, lengths, steps, (float*)workspace);
 }
@@ -974,9 +991,9 @@ int rlt_rocm_linear_attention_backward(rlt_rocm_device* device, const rlt_linear
                                        const uint8_t* reset, const int32_t* lengths, int steps, void* workspace, size_t workspace_bytes) {
     if (!device) return RLT_E_NOT_INITIALISED;
     RLT_REQUIRE(described(layer) && layer->log_decay && steps > 0 && given(q) && given(k) && given(v) && given(d_output) && given(d_q) && given(d_k) && given(d_v));
+    if (!supported(layer) || steps > MAX_STEPS || !launchable(layer, BACKWARD, d_log_decay != nullptr)) return RLT_E_UNSUPPORTED;
     const size_t need = rlt_rocm_linear_attention_workspace_bytes(layer, steps, 1);
     RLT_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0));
-    if (!supported(layer) || steps > MAX_STEPS) return RLT_E_UNSUPPORTED;
     return layer->type == RLT_TYPE_F32 ? backward<float>(device, layer, q, k, v, d_output, d_q, d_k, d_v, initial_state, d_final_state, d_initial_state, d_log_decay, accumulate, reset, lengths, steps, (float*)workspace)
                                        : backward<rlt_bf16>(device, layer, q, k, v, d_output, d_q, d_k, d_v, initial_state, d_final_state, d_initial_state, d_log_decay, accumulate, reset, lengths, steps, (float*)workspace);
 }
@@ -992,10 +1009,9 @@ int rlt_rocm_linear_attention_step(rlt_rocm_device* device, const rlt_linear_att
     auto views = [&](auto type) {
         typedef decltype(type) T;
         a.q = part<T>(q, 1, layer->key_dim); a.k = part<T>(k, group, layer->key_dim); a.v = part<T>(v, group, layer->value_dim); a.out = part<T, 4>(output, 1, layer->value_dim);
-        launch_step<T>(device, a);
+        return launch_step<T>(device, a);
     };
-    if (layer->type == RLT_TYPE_F32) views(0.0f); else views((rlt_bf16)0.0f);
-    return rlt_launch_status(device);
+    return layer->type == RLT_TYPE_F32 ? views(0.0f) : views((rlt_bf16)0.0f);
 }
 
 }  // extern "C"

@@ -4,6 +4,8 @@ import ctypes as C
 import numpy as np
 import pytest
 
+import helpers
+from helpers import capi
 from test_rocm_linear_attention import Tensor, bounds, case, check, layer_of, magnitudes, reference, strides_of, view, workspace
 from typed_arrays import download, filled, rounded, upload
 
@@ -129,3 +131,41 @@ def test_the_states_gradient_in_place(rocm, steps, rows, heads, kv_heads, dk, dv
     two, one = run(rocm, c, x), run(rocm, c, x, in_place=True)
     for n in two:
         assert np.array_equal(two[n], one[n]), n
+
+
+# ------------------------------------------------------------------ more rows and heads than a launch holds
+
+
+MOST = [  # type, width, the most rows x heads: forward, backward, step
+    ("float32", 128, 8388607, 4194296, 16777215), ("float32", 64, 16777215, 8388600, 16777215), ("float32", 32, 33554431, 16777208, 33554431),
+    ("bfloat16", 128, 16777215, 8388600, 16777215), ("bfloat16", 64, 16777215, 8388600, 16777215), ("bfloat16", 32, 33554431, 16777208, 33554431)]
+
+
+@pytest.mark.parametrize("dtype,width,forward,backward,step", MOST)
+def test_scratch_memory_ends_where_launches_do(dtype, width, forward, backward, step):
+    """fewer than 2^32 threads: two walks of 512, 256 or 128 threads for each eight heads' gradients (no GPU is asked)"""
+    lib = helpers.package().load_library()
+    of = lambda batch: lib.rlt_rocm_linear_attention_workspace_bytes(C.byref(capi.LinearAttention(scale=1.0, type=capi.TYPE[dtype], batch=batch, heads=1, kv_heads=1, key_dim=width, value_dim=width)), 2, 1)
+    assert of(backward) > 0 and of(backward + 1) == 0 and of(33554432) == 0
+    threads = {128: 512 if dtype == "float32" else 256, 64: 256, 32: 128}[width]
+    assert -(-backward // 8) * 16 * threads < 2 ** 32 <= -(-(backward + 1) // 8) * 16 * threads
+
+
+@gpu
+@pytest.mark.parametrize("dtype,width,forward,backward,step", MOST)
+def test_more_rows_and_heads_than_a_launch_holds_are_refused(rocm, dtype, width, forward, backward, step):
+    """by the host, before the first launch: nothing is written"""
+    lib, h = rocm.device.lib, rocm.device.handle
+    decay, a = rocm.zeros((4,)), filled(rocm, (4096,), "float32")
+    view = C.byref(capi.HeadView(a.ptr, 0, 0, 0))
+    layer = lambda batch, heads=1: C.byref(capi.LinearAttention(log_decay=decay.ptr, scale=1.0, type=capi.TYPE[dtype], batch=batch, heads=heads, kv_heads=heads, key_dim=width, value_dim=width))
+    for one in (layer(forward + 1), layer(33554432), layer(1 << 16, 1 << 16)):
+        assert lib.rlt_rocm_linear_attention_forward(h, one, *[view] * 4, None, None, None, None, 2, a.ptr, 16384) == capi.RLT_E_UNSUPPORTED
+    assert lib.rlt_rocm_linear_attention_forward(h, layer(step + 1), *[view] * 4, None, a.ptr, None, None, 1, a.ptr, 16384) == capi.RLT_E_UNSUPPORTED
+    assert lib.rlt_rocm_linear_attention_step(h, layer(step + 1), *[view] * 4, a.ptr, a.ptr, None) == capi.RLT_E_UNSUPPORTED
+    for one in (layer(backward + 1), layer(1, backward + 1)):
+        for d_log_decay in (None, a.ptr):
+            assert lib.rlt_rocm_linear_attention_backward(h, one, *[view] * 7, None, None, None, d_log_decay, 1, None, None, 2, a.ptr, 1 << 62) == capi.RLT_E_UNSUPPORTED
+    assert lib.rlt_rocm_linear_attention_backward(h, layer(1, 8388608), *[view] * 7, None, None, None, a.ptr, 1, None, None, 2, a.ptr, 1 << 62) == capi.RLT_E_UNSUPPORTED      # a workgroup of 512 sums up a head's decay
+    rocm.sync()
+    assert np.all(a.numpy() == 7.0)
