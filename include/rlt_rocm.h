@@ -1282,7 +1282,8 @@ int rlt_rocm_residual_norm_backward(rlt_rocm_device* device, const rlt_residual_
 
 /* y = residual + (kept ? x / (1 - p) : 0) (residual NULL: zeros), rows x cols; y may be x or residual. Which elements stay is a function of (seed, stream) alone and stored nowhere: element
  * i = row * cols + column goes by 16 bits of the generator of rlt_rocm_rand_bits_u32, half i % 8 of group i / 8 (the low half of a word first), and stays where they reach
- * 65536 p, p being `rate` (0 ... 1) rounded to a multiple of 1 / 65536. The gradient with respect to x is the same call on the output's gradient, without a residual. */
+ * 65536 p, p being `rate` (0 ... 1) rounded to a multiple of 1 / 65536. The gradient with respect to x is the same call on the output's gradient, without a residual. More than 1.37e11 elements
+ * (2^32 threads) are RLT_E_UNSUPPORTED. */
 int rlt_rocm_dropout(rlt_rocm_device* device, int type, const void* x, int ldx, const void* residual, int ldr, void* y, int ldy, int rows, int cols, float rate,
                      uint64_t seed, uint64_t stream);
 

@@ -90,7 +90,7 @@ template <typename T, int LAYOUT> __global__ __launch_bounds__(256) void dropout
 
 template <typename T> int launch(rlt_rocm_device* device, const DropoutLaunch& a) {
     const size_t blocks = ((a.count + 7) / 8 + 256 * UNROLL - 1) / (256 * UNROLL);
-    if (blocks > INT32_MAX) return RLT_E_UNSUPPORTED;
+    if (blocks > UINT32_MAX / 256) return RLT_E_UNSUPPORTED;      // 2^32 threads are more than a dimension of a grid holds
     const bool aligned = rlt_vectors<T>(a.x, 0) && rlt_vectors<T>(a.y, 0) && (!a.residual || rlt_vectors<T>(a.residual, 0));
     const bool dense = a.ldx == a.cols && a.ldy == a.cols && (!a.residual || a.ldr == a.cols);
     const bool rows = a.cols % 8 == 0 && rlt_vectors<T>(a.x, a.ldx) && rlt_vectors<T>(a.y, a.ldy) && (!a.residual || rlt_vectors<T>(a.residual, a.ldr)) && a.count / 8 <= UINT32_MAX;
