@@ -219,9 +219,10 @@ template <typename T, int N, bool SLOPES> __device__ __forceinline__ void gates_
         const float a = 0.3989422804014327f, b = 0.044715f;
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            const float x = g[i], z = 2.0f * a * fmaf(b * x * x, x, x), e = expf(-fabsf(z)), large = 1.0f / (1.0f + e), small = e * large, p = z >= 0.0f ? large : small, q = z >= 0.0f ? small : large;
+            const float x = g[i] > 30.0f ? 30.0f : g[i] < -30.0f ? -30.0f : g[i];      // beyond, p and q are 0 and 1, and powers of x need not fit fp32
+            const float z = 2.0f * a * fmaf(b * x * x, x, x), e = expf(-fabsf(z)), large = 1.0f / (1.0f + e), small = e * large, p = z >= 0.0f ? large : small, q = z >= 0.0f ? small : large;
             if (SLOPES) slope[i] = p * fmaf(2.0f * x * q, a * fmaf(3.0f * b * x, x, 1.0f), 1.0f);
-            g[i] = x * p;
+            g[i] *= p;
         }
     } else {
 #pragma unroll

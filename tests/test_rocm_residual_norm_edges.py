@@ -2,7 +2,7 @@
 import numpy as np
 import pytest
 
-from test_rocm_residual_norm import Rows, act, layer_of, run_backward, run_forward
+from test_rocm_residual_norm import U, act, run_backward, run_forward
 
 gpu = pytest.mark.gpu
 
@@ -23,3 +23,23 @@ def test_sigmoid_gates_keep_their_relative_accuracy(rocm):
     want, want_slope = np.where(gates < 0, small, 1 - small), small * (1 - small)
     print("largest errors, units:", np.max(np.abs(value - want) / want) * 2 ** 24, np.max(np.abs(slope - want_slope) / want_slope) * 2 ** 24, flush=True)
     assert np.all(np.abs(value - want) <= 8 * 2.0 ** -24 * want) and np.all(np.abs(slope - want_slope) <= 8 * 2.0 ** -24 * want_slope)
+
+
+@gpu
+@pytest.mark.parametrize("activation", ["relu", "gelu", "tanh", "fast_tanh", "sigmoid"])
+def test_gates_of_any_size(rocm, activation):
+    """from the smallest numbers to the largest, of either sign: functions and derivatives as in 64 bits, to U = 128 units of the value and of one (the functions' own range)"""
+    gates = np.concatenate([2.0 ** np.arange(-126, 128), [float(np.finfo(np.float32).max)] * 2])
+    gates = np.stack([gates, -gates]).astype(np.float32).astype(np.float64)
+    value, slope = gates_alone(rocm, gates, activation)
+    with np.errstate(over="ignore"):
+        want, want_slope = act(gates, activation)
+    assert np.all(np.abs(value - want) <= U * (np.abs(want) + np.minimum(1, np.abs(gates))))
+    assert np.all(np.abs(slope - want_slope) <= U * (np.abs(want_slope) + 1))
+
+
+@gpu
+@pytest.mark.parametrize("activation", ["gelu", "sigmoid", "tanh"])
+def test_gates_that_are_not_numbers_stay_so(rocm, activation):
+    value, slope = gates_alone(rocm, np.full((3, 50), np.nan), activation)
+    assert np.isnan(value).all() and np.isnan(slope).all()
