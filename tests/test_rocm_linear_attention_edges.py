@@ -169,3 +169,15 @@ def test_more_rows_and_heads_than_a_launch_holds_are_refused(rocm, dtype, width,
     assert lib.rlt_rocm_linear_attention_backward(h, layer(1, 8388608), *[view] * 7, None, None, None, a.ptr, 1, None, None, 2, a.ptr, 1 << 62) == capi.RLT_E_UNSUPPORTED      # a workgroup of 512 sums up a head's decay
     rocm.sync()
     assert np.all(a.numpy() == 7.0)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("steps,rows,heads,kv_heads,dk,dv", [(66, 500, 128, 64, 4, 4), (33, 65, 64, 32, 33, 33)])
+def test_shared_heads_of_more_tokens_than_the_grid(rocm, steps, rows, heads, kv_heads, dk, dv, dtype):
+    """the sums over heads take 2,048 workgroups of 1,024 elements (or vectors of four) at a time"""
+    elements = kv_heads * (dk // 4 if dk % 4 == 0 else dk)
+    assert steps * rows > 2048 * max(1, 1024 // elements)
+    c, x = case(67, dtype, steps, rows, heads, kv_heads, dk, dv, resets=0.02, ragged=True)
+    got = run(rocm, c, x)
+    check(c, x, got, ["d_k", "d_v"])
