@@ -793,7 +793,7 @@ class SequenceBlocks:
         adam = [capi.AdamTensor(P(n), G(n), self.m.offset(o), self.v.offset(o), None, int(np.prod(shapes[n])), 1 if len(shapes[n]) == 2 else 2) for n, o in self.offsets.items()]
         self.adam, self.n_adam = (capi.AdamTensor * len(adam))(*adam), len(adam)
 
-        self.x, self.reset = z((steps, batch, width)), z((steps, batch), np.uint8)
+        self.x, self.reset, self.passed = z((steps, batch, width)), z((steps, batch), np.uint8), (0, True, True)
         self.h, self.y = [z((rows, width)) for _ in range(blocks + 1)], [z((rows, width)) for _ in range(blocks)]
         self.projected, self.o, self.p = [z((rows, self.row)) for _ in range(blocks)], [z((rows, width)) for _ in range(blocks)], [z((rows, width)) for _ in range(blocks)]
         self.d_h, self.d_stream, self.d_p, self.d_o, self.d_projected = z((rows, width)), z((rows, width)), z((rows, width)), z((rows, width)), z((rows, self.row))
@@ -831,8 +831,9 @@ class SequenceBlocks:
             self.backend.call("dropout", 0, x.ptr, self.width, None, 0, x.ptr, self.width, self.steps * self.batch, self.width, self.rate, self.seed, stream)
 
     def forward(self, stream=0, reset=True, dropout=True):
-        """x -> h[-1], over all steps from states of zeros; `reset` (of this object) ends episodes inside the sequences. stream: the first of `blocks` dropout streams, given to backward again."""
+        """x -> h[-1], over all steps from states of zeros; `reset` (of this object) ends episodes inside the sequences. stream: the first of `blocks` dropout streams."""
         b, w, rows, call = self.backend, self.width, self.steps * self.batch, self.backend.call
+        self.passed = stream, reset, dropout
         r = self.reset.ptr if reset else None
         x = self.x
         call("residual_norm_forward", C.byref(self.input_norm), x.ptr, w, None, 0, None, 0, None, 0, self.h[0].ptr, w, rows)
@@ -846,15 +847,17 @@ class SequenceBlocks:
             x = self.y[l]
         return self.h[-1]
 
-    def backward(self, d_output, stream=0, reset=True):
-        """From the gradient with respect to h[-1] (of the last forward call) to those of the parameters (added to `grads`) and of x (d_stream)."""
+    def backward(self, d_output, stream=None, reset=None, dropout=None):
+        """From the gradient with respect to h[-1] of the last forward call to those of the parameters (added to `grads`) and of x (d_stream). stream, reset, dropout: None for that call's own, whose function's gradients these are."""
         w, rows, call = self.width, self.steps * self.batch, self.backend.call
+        stream, reset, dropout = (last if given is None else given for given, last in zip((stream, reset, dropout), self.passed))
         r = self.reset.ptr if reset else None
         d_h, d_y = d_output, None
         for l in reversed(range(self.blocks)):
             call("residual_norm_backward", C.byref(self.norm[l]), self.p[l].ptr, w, self.projected[l].offset(self.gate_at), self.row, self.y[l].ptr, w, d_y.ptr if d_y else None, w, d_h.ptr, w,
                  self.d_stream.ptr, w, self.d_p.ptr, w, self.d_projected.offset(self.gate_at), self.row, rows, 1, *self.workspace)
-            self._dropout(self.d_p, stream + l)
+            if dropout:
+                self._dropout(self.d_p, stream + l)
             call("dense_backward_full", C.byref(self.out_layer[l]), self.o[l].ptr, w, self.d_p.ptr, w, self.d_o.ptr, w, rows)
             call("linear_attention_backward", C.byref(self.attention[l]), *self.qkv[l], self.d_o_view, *self.d_qkv, None, None, None, self.grad_views[f"log_decay{l}"].ptr, 1, r, None, self.steps, *self.workspace)
             call("dense_backward_full", C.byref(self.in_layer[l]), self.h[l].ptr, w, self.d_projected.ptr, self.row, self.d_h.ptr, w, rows)
