@@ -745,7 +745,7 @@ class SequenceBlocks:
     """A stack of gated residual blocks over sequences [steps x batch x width], fp32: what takes a GRU's place between the dense layers of a recurrent policy or critic. Per block l
         q, k, v, gate = W_in h + b_in (one product; the four are parts of its rows),   o = linear attention(q, k, v),   p = dropout(W_out o + b_out),
         y = x + residual_scale * sigmoid(gate) * branch_norm(p),   the next block's h = output_norm(y);   h of the first block: input_norm(x).
-    Sequences train it (forward, backward, update); step() is one step of a rollout with the blocks' states, and gives what forward gives without dropout. Every device address is fixed when
+    Sequences train it (forward, backward, update); step() is one step of a rollout with the blocks' `states`, which training leaves alone, and gives what forward gives without dropout. Every device address is fixed when
     the object is built, so that forward + backward + update can be captured into a graph."""
 
     @staticmethod
@@ -830,16 +830,18 @@ class SequenceBlocks:
         if self.rate > 0.0:
             self.backend.call("dropout", 0, x.ptr, self.width, None, 0, x.ptr, self.width, self.steps * self.batch, self.width, self.rate, self.seed, stream)
 
-    def forward(self, stream=0, reset=True, dropout=True):
-        """x -> h[-1], over all steps from states of zeros; `reset` (of this object) ends episodes inside the sequences. stream: the first of `blocks` dropout streams."""
+    def forward(self, stream=0, reset=True, dropout=True, keep_states=None):
+        """x -> h[-1], over all steps from states of zeros; `reset` (of this object) ends episodes inside the sequences. stream: the first of `blocks` dropout streams.
+        keep_states: whether the states after the last step replace `states`, which step() goes on from. None: those of a pass without dropout do, as of one that reads what step() is to continue; a training pass leaves the rollout's alone."""
         b, w, rows, call = self.backend, self.width, self.steps * self.batch, self.backend.call
         self.passed = stream, reset, dropout
+        keep_states = not dropout if keep_states is None else keep_states
         r = self.reset.ptr if reset else None
         x = self.x
         call("residual_norm_forward", C.byref(self.input_norm), x.ptr, w, None, 0, None, 0, None, 0, self.h[0].ptr, w, rows)
         for l in range(self.blocks):
             call("dense_forward", C.byref(self.in_layer[l]), self.h[l].ptr, w, None, 0, rows)
-            call("linear_attention_forward", C.byref(self.attention[l]), *self.qkv[l], self.o_views[l], None, self.states[l].ptr, r, None, self.steps, *self.workspace)
+            call("linear_attention_forward", C.byref(self.attention[l]), *self.qkv[l], self.o_views[l], None, self.states[l].ptr if keep_states else None, r, None, self.steps, *self.workspace)
             call("dense_forward", C.byref(self.out_layer[l]), self.o[l].ptr, w, None, 0, rows)
             if dropout:
                 self._dropout(self.p[l], stream + l)

@@ -28,3 +28,34 @@ def test_gradients_are_those_of_the_last_pass(rocm, dropout, reset):
         at = lambda s: np.sum(d * (of(p, x + s * along) if name == "x" else of({**p, name: p[name] + s * along}, x)))
         quotient = (at(step) - at(-step)) / (2 * step)
         assert abs(np.sum(g * along) - quotient) <= (3 * tolerance + 1e-6) * max(np.linalg.norm(g) * np.linalg.norm(along), abs(quotient)), name
+
+
+@gpu
+def test_training_leaves_the_rollouts_states_alone(rocm):
+    """steps with forward and backward passes between them against steps without, bit for bit; a pass without dropout leaves its own states, or not if it is asked so"""
+    c, p, x, resets, net, tolerance, rng = case(rocm, 6, 30, 4, 32, 2, 2, 2, dropout=0.2)
+    d = rocm.array(rng.standard_normal((30 * 4, 32)).astype(np.float32))
+
+    def act(between):
+        for s in net.states:
+            s.upload(np.zeros(s.shape, np.float32))
+        h = []
+        for t in range(6):
+            between()
+            net.step_x.upload(x[t].astype(np.float32))
+            net.step_reset.upload(resets[t])
+            h.append(net.step().numpy())
+        return np.stack(h)
+
+    def train():
+        net.forward(stream=2)
+        net.zero_gradient()
+        net.backward(d)
+    alone = act(lambda: None)
+    assert np.array_equal(alone, act(train)) and np.array_equal(alone, act(lambda: net.forward(dropout=False, keep_states=False)))
+    final = [s.numpy() for s in net.states]
+    net.forward(dropout=False)
+    kept = [s.numpy() for s in net.states]
+    assert all(not np.array_equal(a, b) for a, b in zip(final, kept))
+    net.forward(stream=2, keep_states=True)
+    assert all(not np.array_equal(a.numpy(), b) for a, b in zip(net.states[1:], kept[1:]))      # the second block's, behind a dropout
