@@ -786,6 +786,8 @@ class SequenceBlocks:
         for name, shape in shapes.items():
             flat[self.offsets[name]:self.offsets[name] + int(np.prod(shape))] = np.asarray(params[name], np.float32).reshape(shape).ravel()
         self.params, self.total = backend.array(flat), total
+        self.heads, self.decays = heads, z((blocks, heads))
+        self.decay_stride = self.offsets["log_decay1"] - self.offsets["log_decay0"] if blocks > 1 else heads      # every block's parameters take the same place
         self.grads, self.m, self.v, self.age = z((total,)), z((total,)), z((total,)), backend.array(np.array([1], np.uint32))
         self.grad_views = {name: ArenaView(self.grads, self.offsets[name], shape) for name, shape in shapes.items()}
         self.param_views = {name: ArenaView(self.params, self.offsets[name], shape) for name, shape in shapes.items()}
@@ -867,7 +869,13 @@ class SequenceBlocks:
         call("residual_norm_backward", C.byref(self.input_norm), None, 0, None, 0, self.x.ptr, w, d_y.ptr if d_y else None, w, d_h.ptr, w, self.d_stream.ptr, w, None, 0, None, 0, rows, 1, *self.workspace)
 
     def update(self, adam):
-        self.backend.call("adam_step", self.adam, self.n_adam, C.byref(adam), self.age.ptr, 0.0, None)
+        """One step of Adam; logarithms of decays that it takes above zero, where states grow without bound, are put back to zero: (x - |x|) / 2, exact for the others."""
+        call = self.backend.call
+        call("adam_step", self.adam, self.n_adam, C.byref(adam), self.age.ptr, 0.0, None)
+        at, ld, rows, cols = self.params.offset(self.offsets["log_decay0"]), self.decay_stride, self.blocks, self.heads      # the blocks' own, one row each
+        call("unary_f32", capi.UNARY["abs"], 0.0, at, ld, self.decays.ptr, cols, rows, cols)
+        call("binary_f32", capi.BINARY["subtract"], at, ld, self.decays.ptr, cols, at, ld, rows, cols)
+        call("unary_f32", capi.UNARY["scale"], 0.5, at, ld, at, ld, rows, cols)
 
     def step(self):
         """One step of every row: step_x -> step_h, the blocks' `states` in place; step_reset drops a row's states before it."""

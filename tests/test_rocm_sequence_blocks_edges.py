@@ -1,7 +1,10 @@
 """The stack of sequence blocks where training, acting and evaluation meet. Reference, cases and bounds are those of test_rocm_sequence_blocks."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
+from helpers import capi
 from test_rocm_sequence_blocks import case, reference
 
 gpu = pytest.mark.gpu
@@ -59,3 +62,36 @@ def test_training_leaves_the_rollouts_states_alone(rocm):
     assert all(not np.array_equal(a, b) for a, b in zip(final, kept))
     net.forward(stream=2, keep_states=True)
     assert all(not np.array_equal(a.numpy(), b) for a, b in zip(net.states[1:], kept[1:]))      # the second block's, behind a dropout
+
+
+@gpu
+@pytest.mark.parametrize("blocks,heads", [(1, 1), (2, 3), (3, 4)])
+def test_decays_stay_decays(rocm, blocks, heads):
+    """gradients that push every second logarithm up and the others down, in eager updates and in a graph's: none is above zero, the others are where Adam alone takes them"""
+    c, p, x, resets, net, tolerance, rng = case(rocm, 7, 4, 2, 12 * heads, heads, 1, blocks)
+    adam, names = capi.adam_parameters(alpha=3e-3), [f"log_decay{l}" for l in range(blocks)]
+    up = np.arange(heads) % 2 == 0
+    flat = np.zeros(net.total, np.float32)
+    for n in names:
+        flat[net.offsets[n]:net.offsets[n] + heads] = np.where(up, -1.0, 1.0)
+    net.grads.upload(flat)
+    before = {n: v.numpy() for n, v in net.param_views.items()}
+    lib, h = rocm.device.lib, rocm.device.handle
+    for i in range(20):
+        net.update(adam)
+    rocm.sync()
+    assert lib.rlt_rocm_graph_begin_capture(h) == 0
+    net.update(adam)
+    graph = C.c_void_p()
+    assert lib.rlt_rocm_graph_end_capture(h, C.byref(graph)) == 0
+    for i in range(5):
+        assert lib.rlt_rocm_graph_launch(h, graph) == 0
+        rocm.sync()
+        assert all(np.all(net.param_views[n].numpy() <= 0.0) for n in names)
+    lib.rlt_rocm_graph_destroy(h, graph)
+    for n in names:
+        after = net.param_views[n].numpy()
+        risen = before[n].astype(np.float64) + 25 * 3e-3      # a gradient of one sign and size moves a parameter by alpha an update, up to the epsilon beside its root
+        assert np.all(np.abs(after[up] - np.minimum(risen[up], 0.0)) <= 1e-4) and np.all(np.abs(after[~up] - (before[n][~up] - 25 * 3e-3)) <= 1e-4)
+        assert np.any(after[up] == 0.0) or heads == 1      # (a single head's decay starts too far below)
+    assert all(np.array_equal(net.param_views[n].numpy(), before[n]) for n in before if n not in names)
