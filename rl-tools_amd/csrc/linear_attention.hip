@@ -116,10 +116,11 @@ template <typename T, int D, bool SLOPE, bool STATE> struct Layout {
 // A wavefront owns some of the value columns: their state stays in its accumulators from chunk to chunk, laid out as the matrix instruction leaves them, which is (with the summands in an order of their own) how the
 // product with the queries takes them. Scores of a chunk are shared out in tiles of 16 x 16, weighted, and exchanged through LDS. SLOPE carries the state's derivative by the decay's logarithm along.
 // STATE: only the state, of a segment that starts from nothing. A launch may hold two walks over the same rows (gradients of keys and of values), whose workgroups take turns on an XCD and so find each other's inputs in its L2.
-// What bounds it: whole heads of 128 bfloat16 channels, the vector and matrix instructions of two wavefronts a SIMD (81 % busy) beside 4 TB/s: 4 rows x 16 heads, 8,192 steps, a walk forward 165 us, d_q with the slope 397 to 420, d_k and d_v 320;
-// 16,384 steps of 16 heads forward 132 us in all. Short sequences in fp32, the parts of one chunk one after the other in eight wavefronts a compute unit, as many as LDS has room for (36 KB a workgroup of 32 channels): 64 steps,
-// 1,024 rows, 2 heads of 32: 32, 55 and 52 us, of which the matrix instructions take 8, 14 and 15. Fewer rows and heads than compute units leave a chunk's latency alone: 333 steps, 37 rows, 6 heads of 24 x 41: 46, 70 and 66 us.
-// Few steps on many rows: reading and writing the states, two wavefronts a SIMD: 20 steps, 2,240 rows, 8 heads of 64, bfloat16: 190, 346 and 340 us.
+// What bounds it: whole heads of 128 bfloat16 channels, the vector and matrix instructions of two wavefronts a SIMD (81 to 83 % busy) beside 1.3 to 1.8 TB/s: 4 rows x 16 heads, 8,192 steps, a walk forward 206 us, d_q with the slope 439, d_k and d_v 382;
+// 16,384 steps of 16 heads forward 140 to 150 us in all. Short sequences in fp32, the parts of one chunk one after the other in eight wavefronts a compute unit, as many as LDS has room for (36 KB a workgroup of 32 channels): 64 steps,
+// 1,024 rows, 2 heads of 32: 34, 55 and 56 us, of which the matrix instructions take 8, 14 and 15. Fewer rows and heads than compute units leave a chunk's latency alone: 333 steps, 37 rows, 6 heads of 24 x 41: 47, 73 and 67 us.
+// Few steps on many rows: reading and writing the states, two wavefronts a SIMD: 20 steps, 2,240 rows, 8 heads of 64, bfloat16: 217, 382 and 386 us.
+// Steps that go back in memory take the kernel for any width: 1,024 steps, 64 rows, 8 heads of 64, fp32: 207 us, 190 with steps that go forward.
 struct Walks { Walk first, second; int items, two; };
 template <typename T, typename O, int D, bool REVERSE, bool SLOPE, bool STATE, bool FULL> __global__ __launch_bounds__((Layout<T, D, SLOPE, STATE>::THREADS), (Layout<T, D, SLOPE, STATE>::RESIDENT)) void walk_kernel(Walks walks) {
     typedef typename Operand<T>::Vector Vector;
@@ -787,8 +788,8 @@ bool given(const rlt_head_view* v) { return v && v->data; }
 size_t padded(size_t n) { return (n + 63) / 64 * 64; }
 
 // The steps of a row and head are cut into segments where rows and heads alone leave compute units without work: their states then cost a pass over keys and values ahead of the walk, a quarter of a walk's time, and
-// launches worth about four chunks. Measured (us, by segments): 8 rows x 4 heads of 64, 1,024 steps, fp32: 103 with 1, 44 with 4, 30 with 8 and 16; 8 heads of 64, 2,048 steps, bf16: 104 with 1, 21 with 16 and 32;
-// 4 x 16 heads of 128, 8,192 steps: 498 with 2, 328 with 4, 297 with 8, 331 with 16; forward and backward of 16 x 8 heads of 128, 256 steps: 110 with 1, 188 with 2; of 37 x 6 heads of 41, 333 steps: 235 with 1, 252 to 280 with 2 to 6.
+// launches worth about four chunks. Measured (us, by segments): 8 rows x 4 heads of 64, 1,024 steps, fp32: 77 with 2, 44 with 4, 30 with 8 and 16; 8 heads of 64, 2,048 steps, bf16: 133 with 1, 22 with 16, 21 with 32;
+// 4 x 16 heads of 128, 8,192 steps, bf16: 592 with 2, 317 with 4, 277 with 8, 309 with 16; forward and backward of 16 x 8 heads of 128, 256 steps, bf16: 111 with 1, 168 with 2, 197 with 4; of 37 x 6 heads of 24 x 41, 333 steps, fp32: 199 with 1, 190 to 222 with 2 to 6.
 struct Segments { int count, steps; };
 Segments segments_of(const rlt_linear_attention* p, int steps) {
     const int chunks = (steps + CHUNK - 1) / CHUNK;

@@ -59,8 +59,8 @@ template <int THREADS, int WIDTH, int N> __device__ __forceinline__ void row_sum
 }
 
 // Thread t of a row's THREADS has vectors t, t + THREADS, ... of V elements (16 bytes), K of them. WHOLE: rows start on 16-byte boundaries and hold whole vectors. Otherwise the same loads and stores start at any element, which the
-// memory instructions allow; a row's last vector is loaded where it ends with the row, and its elements move down when they are needed, so that no load waits for a branch. (8,192 rows of 1,001 bfloat16 values: 27 us
-// forward, 45 us backward; 52 and 71 with an element to a load.)
+// memory instructions allow; a row's last vector is loaded where it ends with the row, and its elements move down when they are needed, so that no load waits for a branch. (8,192 rows of 1,001 bfloat16 values: 22 to 27 us
+// forward, 43 to 45 us backward; 52 and 71 with an element to a load.)
 template <typename T, int V, bool WHOLE> struct Row { typedef T Vector __attribute__((ext_vector_type(V))); };
 template <typename T, int V> struct Row<T, V, false> { typedef T Vector __attribute__((ext_vector_type(V), aligned(sizeof(T)))); };
 template <typename T, int V, int K> struct Raw { typedef T Vector __attribute__((ext_vector_type(V))); Vector v[K]; };
@@ -264,13 +264,14 @@ template <typename T, int V, int K, int THREADS, bool WHOLE> __global__ __launch
     }
 }
 
-// Memory bounds this pass: five rows in, three out, 4.6 TB/s at 16,384 rows of 4,096 bfloat16 values (238 to 268 us), 4.8 at 16,384 of 2,048 fp32 values; few rows are bound by the trips to memory of the two or three that a workgroup
+// Memory bounds this pass: five rows in, three out, 4.6 TB/s at 16,384 rows of 4,096 bfloat16 values (236 to 268 us), 4.8 at 16,384 of 2,048 fp32 values; few rows are bound by the trips to memory of the two or three that a workgroup
 // has (4,001 x 1,000 fp32: 36 us). The next row's values are asked for before this row's sums, of which a row has two rounds (three with means): what the statistics and the output norm's gradient need
 // is added up together.
 template <typename T, int V, int K, int THREADS, bool BIASES, bool WHOLE> __global__ __launch_bounds__(BACKWARD_WIDTH<THREADS>) void norm_backward_kernel(NormBackward a) {
     constexpr int N = V * K, WIDTH = BACKWARD_WIDTH<THREADS>, ROWS = WIDTH / THREADS;
     // Parameters and column sums stay in registers from row to row. Rows wider than 4,096 leave none for them: parameters are read again, from L2, and the sums are kept in LDS, each by its own thread (4,096 rows of 8,192 bfloat16
-    // values: 183 us; 536 with 1,024 threads of eight columns, whose registers spill. 16,384 rows of 4,096: 266 us with registers, 332 so).
+    // values: 183 us; 536 with 1,024 threads of eight columns, whose registers spill. 16,384 rows of 4,096: 266 us with registers, 332 so). fp32 rows this wide spill all the same with biases, or where no vectors divide them (56 to 116 bytes of
+    // scratch memory a lane): 4,096 rows of 8,192 fp32 values 242 us, 334 with biases, of 8,191 with biases 536; bfloat16 184, 215 and 317.
     constexpr bool HELD = N * THREADS <= HELD_DIM, AHEAD = HELD || (WHOLE && V == 8);
     __shared__ float lds[ROWS == 1 ? 2 * (THREADS / 64) * 4 : WIDTH * N];
     extern __shared__ __attribute__((aligned(16))) float column_sums[];
