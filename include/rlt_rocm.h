@@ -1287,6 +1287,71 @@ int rlt_rocm_residual_norm_backward(rlt_rocm_device* device, const rlt_residual_
 int rlt_rocm_dropout(rlt_rocm_device* device, int type, const void* x, int ldx, const void* residual, int ldr, void* y, int ldy, int rows, int cols, float rate,
                      uint64_t seed, uint64_t stream);
 
+/* Short causal convolution over the steps, each channel with its own `width` (2 ... 8) weights, the step's own last:
+ *     output_t[c] = act(biases[c] + sum over j < width of weights[c][width - 1 - j] * x_{t-j}[c]),   act: the identity, or z / (1 + exp(-z)) where `silu` is set.
+ * Inputs of before the first step come from the state [batch x (width - 1) x channels] (fp32, the oldest first); inputs of before a reset are left out. Tensors are views whose channels lie
+ * side by side (head_stride is not read). Sequences up to 2^30 steps, up to 2^24 channels and rows, and as many rows x channels as 2^31 elements; anything beyond is RLT_E_UNSUPPORTED before anything is launched. */
+typedef struct rlt_causal_convolution {
+    const float* weights;        /* [channels x width] */
+    const float* biases;         /* [channels]; NULL: zeros */
+    float* d_weights; float* d_biases;      /* gradients; NULL: not wanted */
+    int32_t type;                /* enum rlt_type of x, the output and their gradients */
+    int32_t batch, channels, width;
+    int32_t silu;
+    int32_t reserved;
+} rlt_causal_convolution;
+
+/* All steps of a sequence. initial_state, final_state (NULL: zeros / not wanted; they may be the same buffer), reset [steps x batch] (NULL: none) and lengths [batch] (NULL: all of them) as
+ * rlt_rocm_linear_attention_forward has them: outputs beyond a row's length are zero, its state is that behind its last step, what its inputs hold there is not looked at. */
+int rlt_rocm_causal_convolution_forward(rlt_rocm_device* device, const rlt_causal_convolution* layer, const rlt_head_view* x, const rlt_head_view* output,
+                                        const float* initial_state, float* final_state, const uint8_t* reset, const int32_t* lengths, int steps);
+/* Scratch memory of the backward call (0 for a call that is refused, and where neither d_weights nor d_biases is wanted); starts on a 16-byte boundary and belongs to one call at a time. */
+size_t rlt_rocm_causal_convolution_workspace_bytes(const rlt_causal_convolution* layer, int steps);
+/* Gradients from the layer's inputs alone: d_x (zero beyond a row's length), d_initial_state (NULL: not wanted), the layer's d_weights and d_biases (accumulate = 0 overwrites them, 1 adds to
+ * them). d_final_state is the gradient with respect to final_state (NULL: zeros). Outputs overlap no other buffer of the call. */
+int rlt_rocm_causal_convolution_backward(rlt_rocm_device* device, const rlt_causal_convolution* layer, const rlt_head_view* x, const rlt_head_view* d_output, const rlt_head_view* d_x,
+                                         const float* initial_state, const float* d_final_state, float* d_initial_state, int accumulate, const uint8_t* reset, const int32_t* lengths, int steps,
+                                         void* workspace, size_t workspace_bytes);
+/* One step of every row: the output and next_state (which may be state itself). reset [batch] (NULL: none). The views' step_stride is not read. */
+int rlt_rocm_causal_convolution_step(rlt_rocm_device* device, const rlt_causal_convolution* layer, const rlt_head_view* x, const rlt_head_view* output, const float* state, float* next_state,
+                                     const uint8_t* reset);
+
+/* Selective scan, a recurrent layer of `states` numbers for each channel, whose decays, inputs and outputs depend on the step:
+ *     delta_t = log(1 + exp(raw_t + delta_biases)),   h_t[n] = exp(-exp(log_rates[n]) * delta_t) * h_{t-1}[n] + delta_t * x_t * b_t[n]   (nothing of h_{t-1} at a reset),
+ *     output_t = (sum over n of c_t[n] * h_t[n] + skip * x_t) * gate_t / (1 + exp(-gate_t)).
+ * x, raw (the view `delta`), gate and output are [steps x batch x heads x channels], b and c [steps x batch x heads x states], shared by a head's channels. States (at most 32) are fp32
+ * [batch x heads x channels x states]. Sequences up to 2^30 steps, batch x heads x channels x 32 up to 2^31 and steps x batch x heads up to 2^31; anything beyond is RLT_E_UNSUPPORTED before anything is launched. */
+typedef struct rlt_selective_scan {
+    const float* log_rates;      /* [heads x channels x states] */
+    const float* skip;           /* [heads x channels]; NULL: zeros */
+    const float* delta_biases;   /* [heads x channels]; NULL: zeros */
+    float* d_log_rates; float* d_skip; float* d_delta_biases;      /* gradients; NULL: not wanted */
+    int32_t type;                /* enum rlt_type of the tensors and their gradients */
+    int32_t batch;               /* rows */
+    int32_t heads, channels, states;
+    int32_t reserved;
+} rlt_selective_scan;
+
+/* Scratch memory of a forward (backward = 0) or backward (1) call, and what a forward call leaves for the backward call of the same inputs (its states every few steps); both depend on the shapes
+ * alone, are 0 for a call that is refused, start on 16-byte boundaries and belong to one call (one forward and its backward) at a time. */
+size_t rlt_rocm_selective_scan_workspace_bytes(const rlt_selective_scan* layer, int steps, int backward);
+size_t rlt_rocm_selective_scan_checkpoint_bytes(const rlt_selective_scan* layer, int steps);
+/* All steps of a sequence. gate NULL: no gate (the factor is 1). initial_state, final_state (NULL: zeros / not wanted; they may be the same buffer), reset and lengths as
+ * rlt_rocm_linear_attention_forward has them. checkpoints NULL: no backward call will follow. */
+int rlt_rocm_selective_scan_forward(rlt_rocm_device* device, const rlt_selective_scan* layer, const rlt_head_view* x, const rlt_head_view* delta, const rlt_head_view* b, const rlt_head_view* c,
+                                    const rlt_head_view* gate, const rlt_head_view* output, const float* initial_state, float* final_state, const uint8_t* reset, const int32_t* lengths, int steps,
+                                    void* checkpoints, void* workspace, size_t workspace_bytes);
+/* Gradients through time, from the inputs and the checkpoints of the forward call on them: d_x, d_delta (with respect to raw), d_b, d_c, d_gate (zero beyond a row's length; d_gate is not read where there is
+ * no gate), d_initial_state (NULL: not wanted), the layer's d_log_rates, d_skip and d_delta_biases (accumulate = 0 overwrites them, 1 adds to them). d_final_state is the gradient with respect to
+ * final_state (NULL: zeros); d_initial_state may be the same buffer. Outputs overlap no other buffer of the call but where these comments say so. */
+int rlt_rocm_selective_scan_backward(rlt_rocm_device* device, const rlt_selective_scan* layer, const rlt_head_view* x, const rlt_head_view* delta, const rlt_head_view* b, const rlt_head_view* c,
+                                     const rlt_head_view* gate, const rlt_head_view* d_output, const rlt_head_view* d_x, const rlt_head_view* d_delta, const rlt_head_view* d_b, const rlt_head_view* d_c,
+                                     const rlt_head_view* d_gate, const float* d_final_state, float* d_initial_state, int accumulate, const uint8_t* reset, const int32_t* lengths, int steps,
+                                     const void* checkpoints, void* workspace, size_t workspace_bytes);
+/* One step of every row: the output and next_state (which may be state itself). reset [batch] (NULL: none). The views' step_stride is not read. */
+int rlt_rocm_selective_scan_step(rlt_rocm_device* device, const rlt_selective_scan* layer, const rlt_head_view* x, const rlt_head_view* delta, const rlt_head_view* b, const rlt_head_view* c,
+                                 const rlt_head_view* gate, const rlt_head_view* output, const float* state, float* next_state, const uint8_t* reset);
+
 #ifdef __cplusplus
 }
 #endif

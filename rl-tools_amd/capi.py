@@ -264,6 +264,16 @@ class ResidualNorm(C.Structure):
                 ("d_branch_weights", C.c_void_p), ("d_branch_biases", C.c_void_p), ("d_output_weights", C.c_void_p), ("d_output_biases", C.c_void_p), ("d_residual_scale", C.c_void_p)]
 
 
+class CausalConvolution(C.Structure):
+    _fields_ = [("weights", C.c_void_p), ("biases", C.c_void_p), ("d_weights", C.c_void_p), ("d_biases", C.c_void_p), ("type", C.c_int32), ("batch", C.c_int32), ("channels", C.c_int32),
+                ("width", C.c_int32), ("silu", C.c_int32), ("reserved", C.c_int32)]
+
+
+class SelectiveScan(C.Structure):
+    _fields_ = [("log_rates", C.c_void_p), ("skip", C.c_void_p), ("delta_biases", C.c_void_p), ("d_log_rates", C.c_void_p), ("d_skip", C.c_void_p), ("d_delta_biases", C.c_void_p),
+                ("type", C.c_int32), ("batch", C.c_int32), ("heads", C.c_int32), ("channels", C.c_int32), ("states", C.c_int32), ("reserved", C.c_int32)]
+
+
 I, F, P, S, U64 = C.c_int, C.c_float, C.c_void_p, C.c_size_t, C.c_uint64
 LP = C.POINTER(DenseLayer)
 # return codes of the C ABI (include/rlt_rocm.h)
@@ -403,6 +413,15 @@ ROCM_ONLY = {
     "linear_attention_forward": ([P, C.POINTER(LinearAttention)] + [C.POINTER(HeadView)] * 4 + [P, P, P, P, I, P, S], I),
     "linear_attention_backward": ([P, C.POINTER(LinearAttention)] + [C.POINTER(HeadView)] * 7 + [P, P, P, P, I, P, P, I, P, S], I),
     "linear_attention_step": ([P, C.POINTER(LinearAttention)] + [C.POINTER(HeadView)] * 4 + [P, P, P], I),
+    "causal_convolution_forward": ([P, C.POINTER(CausalConvolution)] + [C.POINTER(HeadView)] * 2 + [P, P, P, P, I], I),
+    "causal_convolution_workspace_bytes": ([C.POINTER(CausalConvolution), I], S),
+    "causal_convolution_backward": ([P, C.POINTER(CausalConvolution)] + [C.POINTER(HeadView)] * 3 + [P, P, P, I, P, P, I, P, S], I),
+    "causal_convolution_step": ([P, C.POINTER(CausalConvolution)] + [C.POINTER(HeadView)] * 2 + [P, P, P], I),
+    "selective_scan_workspace_bytes": ([C.POINTER(SelectiveScan), I, I], S),
+    "selective_scan_checkpoint_bytes": ([C.POINTER(SelectiveScan), I], S),
+    "selective_scan_forward": ([P, C.POINTER(SelectiveScan)] + [C.POINTER(HeadView)] * 6 + [P, P, P, P, I, P, P, S], I),
+    "selective_scan_backward": ([P, C.POINTER(SelectiveScan)] + [C.POINTER(HeadView)] * 11 + [P, P, I, P, P, I, P, P, S], I),
+    "selective_scan_step": ([P, C.POINTER(SelectiveScan)] + [C.POINTER(HeadView)] * 6 + [P, P, P], I),
     "residual_norm_forward": ([P, C.POINTER(ResidualNorm), P, I, P, I, P, I, P, I, P, I, I], I),
     "residual_norm_workspace_bytes": ([C.POINTER(ResidualNorm), I], S),
     "residual_norm_backward": ([P, C.POINTER(ResidualNorm), P, I, P, I, P, I, P, I, P, I, P, I, P, I, P, I, I, I, P, S], I),

@@ -1,0 +1,790 @@
+// Selective scan: a few states for each channel, whose decays, inputs and readings depend on the step; forward, backward and single steps.
+#include "selective.h"
+#include <type_traits>
+
+namespace {
+
+constexpr int MAX_STEPS = 1 << 30, MAX_STATES = 32;
+constexpr int WAVES = 4, LANES = 64 * WAVES, TILE = 16 * WAVES;      // channels of a workgroup: four lanes share one, each with a quarter of its states
+constexpr float LOG2_E = 1.44269504088896341f, LN_2 = 0.69314718055994531f;
+
+// steps that a lane looks at together, and behind which the forward pass leaves the states for the backward pass; NPT states to a lane
+template <int NPT> constexpr int CHUNK = NPT == 8 ? 8 : 16;
+static int per_lane(int states) { return states <= 8 ? 2 : states <= 16 ? 4 : 8; }
+static int chunk_of(int states) { return states <= 16 ? 16 : 8; }
+
+struct Scan {
+    const float* log_rates; const float* skip; const float* delta_biases;
+    rlt_part x, delta, b, c, gate, out, d_out, d_x, d_delta, d_b, d_c, d_gate;
+    const float* entry; float* exit;         // states (backward: their gradients) before the first step walked and behind the last: [pairs][channels][states], or where there are segments [pairs][segments][channels][4 NPT]
+    float* sums;                  // of delta over a segment, [pairs][segments][channels]; below zero: the segment holds a reset, nothing passes it
+    float* checkpoints;           // [pairs][chunks][channels][4 NPT]: states before each chunk
+    float* d_shared;              // d_b, then d_c: [tiles][steps x batch x heads][4 NPT]
+    float* d_rates; float* d_skips; float* d_biases;      // [row groups x segments][heads][channels][4 NPT] and [...][channels]
+    const uint8_t* reset; const int32_t* lengths;
+    int batch, heads, channels, states, steps, segments, segment_steps, tiles, chunks, row_groups;
+    int entry_padded;             // entry is the segments'
+};
+
+template <typename T> __device__ __forceinline__ T* at(const rlt_part& p, int step, int row, int head) { return (T*)p.data + (int64_t)step * p.step + (int64_t)row * p.row + (int64_t)head * p.head; }
+
+// ---- exchanges between the four lanes of a channel
+template <int CTRL> __device__ __forceinline__ float lanes(float v) { return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true)); }
+template <int J> __device__ __forceinline__ float from_lane(float v) { return lanes<J * 0x55>(v); }
+// lane j receives the sum over its channel's lanes of v[j]
+__device__ __forceinline__ float sum_to_lane(const float (&v)[4], bool odd, bool upper) {
+    const float a = (odd ? v[1] : v[0]) + lanes<0xB1>(odd ? v[0] : v[1]), b = (odd ? v[3] : v[2]) + lanes<0xB1>(odd ? v[2] : v[3]);
+    return (upper ? b : a) + lanes<0x4E>(upper ? a : b);
+}
+__device__ __forceinline__ float sum_of_lanes(float v) {
+    v += lanes<0xB1>(v);
+    return v + lanes<0x4E>(v);
+}
+typedef unsigned rlt_u32x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ float add_halves(float a, float b) {      // lanes 0 to 31: a's sum over both halves of the wavefront, the others: b's
+    const auto s = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b), false, false);
+    return __builtin_bit_cast(float, (unsigned)s[0]) + __builtin_bit_cast(float, (unsigned)s[1]);
+}
+__device__ __forceinline__ float add_rows(float a, float b) {        // even rows of sixteen lanes: a's sum over both of a half, odd rows: b's
+    const auto s = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b), false, false);
+    return __builtin_bit_cast(float, (unsigned)s[0]) + __builtin_bit_cast(float, (unsigned)s[1]);
+}
+// Sums over the sixteen channels of a wavefront. A lane ends up with those of NPT / 4 of its states (of one where NPT < 4): state k + (NPT / 4) * (lane bit 4) + (NPT / 2) * (lane bit 5) of the lane's NPT.
+template <int NPT> __device__ __forceinline__ void sum_channels(const float (&v)[NPT], float (&s)[NPT > 4 ? NPT / 4 : 1]) {
+    if constexpr (NPT == 2) {
+        const float a = add_halves(v[0], v[1]);
+        s[0] = add_rows(a, a);
+    } else {
+        float h[NPT / 2];
+#pragma unroll
+        for (int i = 0; i < NPT / 2; i++) h[i] = add_halves(v[i], v[i + NPT / 2]);
+#pragma unroll
+        for (int i = 0; i < NPT / 4; i++) s[i] = add_rows(h[i], h[i + NPT / 4]);
+    }
+#pragma unroll
+    for (int i = 0; i < (NPT > 4 ? NPT / 4 : 1); i++) {
+        s[i] += lanes<0x124>(s[i]);      // four and eight lanes round the row
+        s[i] += lanes<0x128>(s[i]);
+    }
+}
+
+// log(1 + e^v), and e^-|v|: with s = e / (2 + e), e = e^-|v|, log(1 + e) = 2 artanh(s), whose series in s^2 <= 1/9 ends at s^15 (relative rest 1.4e-9); keeps its relative accuracy far below zero
+__device__ __forceinline__ float softplus(float v, float& e) {
+    e = rlt_exp_negative(-fabsf(v));
+    const float s = e * rlt_reciprocal(2.0f + e), z = s * s;
+    float p = fmaf(z, 1.0f / 15, 1.0f / 13);
+    p = fmaf(p, z, 1.0f / 11); p = fmaf(p, z, 1.0f / 9); p = fmaf(p, z, 1.0f / 7); p = fmaf(p, z, 1.0f / 5); p = fmaf(p, z, 1.0f / 3);
+    return fmaxf(v, 0.0f) + 2.0f * fmaf(s * z, p, s);
+}
+
+// ---- what a workgroup walks over
+struct Place { int tile, head, row, segment, first, end, length, live; };      // steps [first, end) of the segment; the row's steps; end or length
+__device__ __forceinline__ Place place_of(const Scan& a, unsigned item, int row_count) {
+    Place p;
+    p.tile = item % a.tiles; item /= a.tiles;
+    p.head = item % a.heads; item /= a.heads;
+    p.segment = item / row_count; p.row = item - p.segment * row_count;
+    p.first = p.segment * a.segment_steps; p.end = min(p.first + a.segment_steps, a.steps);
+    return p;
+}
+__device__ __forceinline__ void set_row(const Scan& a, Place& p, int row) {
+    p.row = row;
+    p.length = a.lengths ? min(max(a.lengths[row], 0), a.steps) : a.steps;
+    p.live = min(p.end, p.length);
+}
+__device__ __forceinline__ int pair_of(const Scan& a, const Place& p) { return p.row * a.heads + p.head; }
+// bit s: step t + s forgets its state
+template <int K> __device__ __forceinline__ unsigned resets_of(const Scan& a, const Place& p, int t) {
+    if (!a.reset) return 0;
+    const int s = threadIdx.x & 63;
+    return (unsigned)__ballot(s < K && t + s < p.live && a.reset[(size_t)min(t + s, a.steps - 1) * a.batch + p.row]);
+}
+
+// b and c of a chunk, zero beyond the row's length and the layer's states; a thread holds its elements while the chunk before is worked on
+template <typename T, int NPT> struct Shared {
+    static constexpr int K = CHUNK<NPT>, N = 4 * NPT, PER = (K * N + LANES - 1) / LANES;
+    float b[PER], c[PER];
+    __device__ __forceinline__ void ask(const Scan& a, const Place& p, int t, bool with_b) {
+#pragma unroll
+        for (int j = 0; j < PER; j++) {
+            const int e = threadIdx.x + j * LANES, s = e / N, n = e % N;
+            const bool there = e < K * N && t + s < p.live && n < a.states;
+            b[j] = there && with_b ? (float)at<T>(a.b, t + s, p.row, p.head)[n] : 0.0f;
+            c[j] = there && a.c.data ? (float)at<T>(a.c, t + s, p.row, p.head)[n] : 0.0f;
+        }
+    }
+    __device__ __forceinline__ void put(float (*to)[K * N]) const {
+#pragma unroll
+        for (int j = 0; j < PER; j++) {
+            const int e = threadIdx.x + j * LANES;
+            if (e < K * N) { to[0][e] = b[j]; to[1][e] = c[j]; }
+        }
+    }
+};
+template <int NPT> __device__ __forceinline__ void read(const float* from, float (&to)[NPT]) {
+    typedef float vector __attribute__((ext_vector_type(NPT < 4 ? NPT : 4)));
+#pragma unroll
+    for (int i = 0; i < NPT; i += NPT < 4 ? NPT : 4) {
+        const vector v = *reinterpret_cast<const vector*>(from + i);
+#pragma unroll
+        for (int j = 0; j < (NPT < 4 ? NPT : 4); j++) to[i + j] = v[j];
+    }
+}
+template <int NPT> __device__ __forceinline__ void write(float* to, const float (&from)[NPT]) {
+    typedef float vector __attribute__((ext_vector_type(NPT < 4 ? NPT : 4)));
+#pragma unroll
+    for (int i = 0; i < NPT; i += NPT < 4 ? NPT : 4) {
+        vector v;
+#pragma unroll
+        for (int j = 0; j < (NPT < 4 ? NPT : 4); j++) v[j] = from[i + j];
+        *reinterpret_cast<vector*>(to + i) = v;
+    }
+}
+// a lane's elements of its channel in the chunk's steps 4 i + (lane & 3)
+template <typename T, int OWN> __device__ __forceinline__ void ask(const Scan& a, const rlt_part& part, const Place& p, int channel, int t, T (&v)[OWN]) {
+    const int nq = threadIdx.x & 3;
+#pragma unroll
+    for (int i = 0; i < OWN; i++) v[i] = at<T>(part, min(t + 4 * i + nq, a.steps - 1), p.row, p.head)[channel];
+}
+template <int NPT> __device__ __forceinline__ void load_states(const float* from, int n0, int states, float (&h)[NPT]) {
+#pragma unroll
+    for (int n = 0; n < NPT; n++) h[n] = from && n0 + n < states ? from[n0 + n] : 0.0f;
+}
+template <int NPT> __device__ __forceinline__ void store_states(float* to, int n0, int states, const float (&h)[NPT]) {
+#pragma unroll
+    for (int n = 0; n < NPT; n++) if (n0 + n < states) to[n0 + n] = h[n];
+}
+// logarithms of the decays to base 2 for a delta of one; nothing where there is no state
+template <int NPT> __device__ __forceinline__ void load_rates(const Scan& a, int head, int channel, int n0, float (&rate)[NPT]) {
+    const float* const from = a.log_rates + ((size_t)head * a.channels + channel) * a.states;
+#pragma unroll
+    for (int n = 0; n < NPT; n++) rate[n] = n0 + n < a.states ? -expf(from[n0 + n]) * LOG2_E : 0.0f;
+}
+
+// Forward over a segment. STATES: only what the segment adds to the state, for states that segments start from.
+template <typename T, int NPT, bool STATES> __global__ __launch_bounds__(LANES) void forward_kernel(Scan a) {
+    constexpr int K = CHUNK<NPT>, OWN = K / 4, N = 4 * NPT;
+    __shared__ float shared[2][2][K * N];
+    Place p = place_of(a, blockIdx.x, a.batch);
+    set_row(a, p, p.row);
+    const int lane = threadIdx.x & 63, nq = lane & 3, n0 = nq * NPT, own_channel = p.tile * TILE + (int)(threadIdx.x >> 2), channel = min(own_channel, a.channels - 1);
+    const bool there = own_channel < a.channels, odd = nq & 1, upper = nq & 2;
+    const size_t pair = pair_of(a, p), at_channel = (size_t)p.head * a.channels + channel;
+    float rate[NPT], h[NPT];
+    load_rates<NPT>(a, p.head, channel, n0, rate);
+    const float bias = a.delta_biases ? a.delta_biases[at_channel] : 0.0f, skip = a.skip ? a.skip[at_channel] : 0.0f;
+    if (STATES || !a.entry) {
+#pragma unroll
+        for (int n = 0; n < NPT; n++) h[n] = 0.0f;
+    } else if (a.entry_padded) read<NPT>(a.entry + ((pair * a.segments + p.segment) * a.channels + channel) * N + n0, h);
+    else load_states<NPT>(a.entry + (pair * a.channels + channel) * a.states, n0, a.states, h);
+    float sum = 0.0f;
+    bool forgotten = false;
+
+    T x[OWN], raw[OWN], gate[OWN];
+    unsigned resets;
+    Shared<T, NPT> next;
+    auto ask_chunk = [&](int t) {
+        ask<T, OWN>(a, a.x, p, channel, t, x);
+        ask<T, OWN>(a, a.delta, p, channel, t, raw);
+        if (!STATES && a.gate.data) ask<T, OWN>(a, a.gate, p, channel, t, gate);
+        next.ask(a, p, t, true);
+        resets = resets_of<K>(a, p, t);
+    };
+    if (p.first < p.live) ask_chunk(p.first);
+    int turn = 0;
+    for (int t = p.first; t < p.live; t += K, turn ^= 1) {
+        float xs[OWN], delta[OWN], added[OWN], gates[OWN];
+#pragma unroll
+        for (int i = 0; i < OWN; i++) {
+            const bool in = t + 4 * i + nq < p.live;
+            float e;
+            xs[i] = in ? (float)x[i] : 0.0f;
+            delta[i] = in ? softplus((float)raw[i] + bias, e) : 0.0f;
+            added[i] = delta[i] * xs[i];
+            if (!STATES) gates[i] = a.gate.data ? (float)gate[i] : 0.0f;
+        }
+        const unsigned forget = resets;
+        next.put(shared[turn]);
+        if (t + K < p.live) ask_chunk(t + K);
+        rlt_lds_barrier();
+        const float* const bs = shared[turn][0] + n0; const float* const cs = shared[turn][1] + n0;
+        if (!STATES && a.checkpoints && there) write<NPT>(a.checkpoints + ((pair * a.chunks + t / K) * a.channels + channel) * N + n0, h);
+        float y[OWN];
+        auto walk = [&](auto with_resets) {
+#pragma unroll
+            for (int i = 0; i < OWN; i++) {
+                float part[4];
+                auto step = [&](auto which) {
+                    constexpr int j = decltype(which)::value;
+                    const float d = from_lane<j>(delta[i]), u = from_lane<j>(added[i]);
+                    float b[NPT], c[NPT];
+                    read<NPT>(bs + (4 * i + j) * N, b);
+                    if (!STATES) read<NPT>(cs + (4 * i + j) * N, c);
+                    if (decltype(with_resets)::value && (forget >> (4 * i + j) & 1)) {
+#pragma unroll
+                        for (int n = 0; n < NPT; n++) h[n] = 0.0f;
+                        if (STATES) forgotten = true;
+                    }
+                    part[j] = 0.0f;
+#pragma unroll
+                    for (int n = 0; n < NPT; n++) {
+                        h[n] = fmaf(__builtin_amdgcn_exp2f(d * rate[n]), h[n], u * b[n]);
+                        if (!STATES) part[j] = fmaf(c[n], h[n], part[j]);
+                    }
+                };
+                step(std::integral_constant<int, 0>{}); step(std::integral_constant<int, 1>{}); step(std::integral_constant<int, 2>{}); step(std::integral_constant<int, 3>{});
+                if (!STATES) y[i] = sum_to_lane(part, odd, upper);
+                else sum += delta[i];
+            }
+        };
+        if (forget) walk(std::true_type{}); else walk(std::false_type{});
+        if (!STATES) {
+#pragma unroll
+            for (int i = 0; i < OWN; i++) {
+                const int s = t + 4 * i + nq;
+                float v = fmaf(skip, xs[i], y[i]);
+                if (a.gate.data) {
+                    float one, other;
+                    rlt_sigmoids(gates[i], one, other);
+                    v *= gates[i] * one;
+                }
+                if (there && s < p.end) at<T>(a.out, s, p.row, p.head)[channel] = (T)(s < p.live ? v : 0.0f);
+            }
+        }
+    }
+    if constexpr (STATES) {
+        if (!there) return;
+        write<NPT>(a.exit + ((pair * a.segments + p.segment) * a.channels + channel) * N + n0, h);
+        sum = sum_of_lanes(sum);
+        if (nq == 0) a.sums[(pair * a.segments + p.segment) * a.channels + channel] = forgotten ? -1.0f : sum;
+    } else {
+        if (!there) return;
+        if (a.exit && p.segment == a.segments - 1) store_states<NPT>(a.exit + (pair * a.channels + channel) * a.states, n0, a.states, h);
+        // steps behind the last chunk that holds any of the row's
+        const int walked = p.live > p.first ? p.first + (p.live - p.first + K - 1) / K * K : p.first;
+        for (int s = walked + nq; s < p.end; s += 4) at<T>(a.out, s, p.row, p.head)[channel] = (T)0.0f;
+    }
+}
+
+// States that the segments start from, out of what each of them adds: element by element along the segments (REVERSE: from the last). locals become the entries.
+template <bool REVERSE> __global__ __launch_bounds__(256) void join_segments_kernel(Scan a, const float* __restrict__ initial, float* __restrict__ locals, int padded) {
+    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x, per_pair = (size_t)a.channels * padded, pair = i / per_pair;
+    if (pair >= (size_t)a.batch * a.heads) return;
+    const int e = (int)(i - pair * per_pair), channel = e / padded, n = e - channel * padded;
+    const bool there = n < a.states;
+    const size_t at_channel = (pair % a.heads) * a.channels + channel;
+    const float rate = there ? -expf(a.log_rates[at_channel * a.states + n]) * LOG2_E : 0.0f;
+    float carry = initial && there ? initial[(pair * a.channels + channel) * a.states + n] : 0.0f;
+    for (int k = 0; k < a.segments; k++) {
+        const int s = REVERSE ? a.segments - 1 - k : k;
+        float* const at_local = locals + (pair * a.segments + s) * per_pair + e;
+        if (k + 1 < a.segments) {
+            const float local = *at_local, sum = a.sums[(pair * a.segments + s) * a.channels + channel];
+            *at_local = carry;
+            carry = sum < 0.0f ? local : fmaf(__builtin_amdgcn_exp2f(sum * rate), carry, local);
+        } else *at_local = carry;
+    }
+}
+
+// Backward over a segment: from the last chunk to the first, the chunk's states again from its checkpoint, then its steps from the last to the first with the state's gradient G:
+//     G_t = c_t g_t + a_{t+1} G_{t+1},   g = d_output times the gate's factor;   d_c = sum over channels of g h,   d_b = sum over channels of delta x G,
+//     d_x = delta (G . b) + skip g,   d_delta = x (G . b) + rates . q,   d_rates += delta q   with q = G a h_{t-1}.
+template <typename T, int NPT> __global__ __launch_bounds__(LANES, 2) void backward_kernel(Scan a) {
+    constexpr int K = CHUNK<NPT>, OWN = K / 4, N = 4 * NPT, KEPT = NPT > 4 ? NPT / 4 : 1;
+    __shared__ float shared[2][2][K * N];
+    __shared__ float slabs[2][WAVES][2][K * N];
+    Place p = place_of(a, blockIdx.x, a.row_groups);
+    const int group = p.row, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nq = lane & 3, quad = lane >> 2 & 3, n0 = nq * NPT, own_channel = p.tile * TILE + (int)(threadIdx.x >> 2), channel = min(own_channel, a.channels - 1);
+    const int kept_state = n0 + (NPT >= 4 ? (lane >> 4 & 1) * (NPT / 4) : 0) + (lane >> 5) * (NPT / 2);      // the first state whose sums over channels this lane is left with
+    const bool there = own_channel < a.channels, odd = nq & 1, upper = nq & 2;
+    const size_t at_channel = (size_t)p.head * a.channels + channel;
+    float rate[NPT], d_rate[NPT];
+    load_rates<NPT>(a, p.head, channel, n0, rate);
+#pragma unroll
+    for (int n = 0; n < NPT; n++) d_rate[n] = 0.0f;
+    const float bias = a.delta_biases ? a.delta_biases[at_channel] : 0.0f, skip = a.skip ? a.skip[at_channel] : 0.0f;
+    float d_skip = 0.0f, d_bias = 0.0f;
+    const bool gated = a.gate.data != nullptr;
+    const size_t shared_size = (size_t)a.steps * a.batch * a.heads * N;
+    int turn = 0;
+    for (int row = group; row < a.batch; row += a.row_groups) {
+        set_row(a, p, row);
+        const size_t pair = pair_of(a, p);
+        float carry[NPT];
+        if (!a.entry) {
+#pragma unroll
+            for (int n = 0; n < NPT; n++) carry[n] = 0.0f;
+        } else if (a.entry_padded) read<NPT>(a.entry + ((pair * a.segments + p.segment) * a.channels + channel) * N + n0, carry);
+        else load_states<NPT>(a.entry + (pair * a.channels + channel) * a.states, n0, a.states, carry);
+
+        T x[OWN], raw[OWN], gate[OWN], d_out[OWN];
+        unsigned resets;
+        float first_state[NPT];
+        Shared<T, NPT> next;
+        auto ask_chunk = [&](int t) {
+            ask<T, OWN>(a, a.x, p, channel, t, x);
+            ask<T, OWN>(a, a.delta, p, channel, t, raw);
+            ask<T, OWN>(a, a.d_out, p, channel, t, d_out);
+            if (gated) ask<T, OWN>(a, a.gate, p, channel, t, gate);
+            next.ask(a, p, t, true);
+            resets = resets_of<K>(a, p, t);
+            read<NPT>(a.checkpoints + ((pair * a.chunks + t / K) * a.channels + channel) * N + n0, first_state);
+        };
+        const int chunks = p.live > p.first ? (p.live - p.first + K - 1) / K : 0;
+        // steps behind the last chunk that holds any of the row's
+        for (int s = p.first + chunks * K + nq; there && s < p.end; s += 4) {
+            at<T>(a.d_x, s, p.row, p.head)[channel] = (T)0.0f;
+            at<T>(a.d_delta, s, p.row, p.head)[channel] = (T)0.0f;
+            if (gated) at<T>(a.d_gate, s, p.row, p.head)[channel] = (T)0.0f;
+        }
+        auto store_shared = [&](int s, int n, float d_b, float d_c) {
+            if (a.tiles == 1) {
+                if (n < a.states) { at<T>(a.d_b, s, p.row, p.head)[n] = (T)d_b; at<T>(a.d_c, s, p.row, p.head)[n] = (T)d_c; }
+            } else {
+                float* const to = a.d_shared + (size_t)p.tile * 2 * shared_size + (((size_t)s * a.batch + p.row) * a.heads + p.head) * N + n;
+                to[0] = d_b; to[shared_size] = d_c;
+            }
+        };
+        for (int64_t e = threadIdx.x; e < ((int64_t)p.end - p.first - (int64_t)chunks * K) * N; e += LANES) store_shared(p.first + chunks * K + (int)(e / N), (int)(e % N), 0.0f, 0.0f);
+        if (chunks) ask_chunk(p.first + (chunks - 1) * K);
+        for (int k = chunks - 1; k >= 0; k--, turn ^= 1) {
+            const int t = p.first + k * K;
+            float xs[OWN], delta[OWN], added[OWN], slope[OWN], d[OWN], ups[OWN], factor[OWN], d_factor[OWN];
+#pragma unroll
+            for (int i = 0; i < OWN; i++) {
+                const bool in = there && t + 4 * i + nq < p.live;
+                float e;
+                const float v = (float)raw[i] + bias;
+                xs[i] = in ? (float)x[i] : 0.0f;
+                delta[i] = softplus(v, e);
+                const float large = rlt_reciprocal(1.0f + e);
+                slope[i] = in ? (v >= 0.0f ? large : e * large) : 0.0f;      // of softplus
+                delta[i] = in ? delta[i] : 0.0f;
+                added[i] = delta[i] * xs[i];
+                ups[i] = in ? (float)d_out[i] : 0.0f;
+                if (gated) {
+                    const float z = in ? (float)gate[i] : 0.0f;
+                    float one, other;
+                    rlt_sigmoids(z, one, other);
+                    factor[i] = z * one;
+                    d_factor[i] = one * fmaf(z, other, 1.0f);
+                    d[i] = ups[i] * factor[i];
+                } else d[i] = ups[i];
+            }
+            const unsigned forget = resets;
+            float h[K][NPT], decay[K][NPT], before[NPT];
+#pragma unroll
+            for (int n = 0; n < NPT; n++) before[n] = first_state[n];
+            next.put(shared[turn]);
+            if (k > 0) ask_chunk(t - K);
+            rlt_lds_barrier();
+            const float* const bs = shared[turn][0] + n0; const float* const cs = shared[turn][1] + n0;
+            float mixed[OWN], through[OWN], exponent[OWN];
+            auto walk = [&](auto with_resets) {
+                constexpr bool RESETS = decltype(with_resets)::value;
+#pragma unroll
+                for (int i = 0; i < OWN; i++) {
+                    auto step = [&](auto which) {
+                        constexpr int j = decltype(which)::value;
+                        const int s = 4 * i + j;
+                        const float dt = from_lane<j>(delta[i]), u = from_lane<j>(added[i]);
+                        const bool begins = RESETS && (forget >> s & 1);
+                        float b[NPT];
+                        read<NPT>(bs + s * N, b);
+#pragma unroll
+                        for (int n = 0; n < NPT; n++) {
+                            decay[s][n] = __builtin_amdgcn_exp2f(dt * rate[n]);
+                            const float old = s ? h[s ? s - 1 : 0][n] : before[n];
+                            h[s][n] = begins ? u * b[n] : fmaf(decay[s][n], old, u * b[n]);
+                        }
+                    };
+                    step(std::integral_constant<int, 0>{}); step(std::integral_constant<int, 1>{}); step(std::integral_constant<int, 2>{}); step(std::integral_constant<int, 3>{});
+                }
+#pragma unroll
+                for (int i = OWN - 1; i >= 0; i--) {
+                    float mixed_part[4], through_part[4], exponent_part[4], kept_b[KEPT], kept_c[KEPT];
+#pragma unroll
+                    for (int m = 0; m < KEPT; m++) kept_b[m] = kept_c[m] = 0.0f;
+                    auto step = [&](auto which) {
+                        constexpr int j = decltype(which)::value;
+                        const int s = 4 * i + j;
+                        const float dt = from_lane<j>(delta[i]), u = from_lane<j>(added[i]), g = from_lane<j>(d[i]);
+                        const bool begins = RESETS && (forget >> s & 1);
+                        float b[NPT], c[NPT], d_b[NPT], d_c[NPT];
+                        read<NPT>(bs + s * N, b);
+                        read<NPT>(cs + s * N, c);
+                        mixed_part[j] = through_part[j] = exponent_part[j] = 0.0f;
+#pragma unroll
+                        for (int n = 0; n < NPT; n++) {
+                            const float G = fmaf(c[n], g, carry[n]);
+                            d_c[n] = g * h[s][n];
+                            d_b[n] = u * G;
+                            mixed_part[j] = fmaf(c[n], h[s][n], mixed_part[j]);
+                            through_part[j] = fmaf(b[n], G, through_part[j]);
+                            carry[n] = begins ? 0.0f : decay[s][n] * G;
+                            const float old = s ? h[s ? s - 1 : 0][n] : before[n], q = begins ? 0.0f : carry[n] * old;
+                            exponent_part[j] = fmaf(rate[n], q, exponent_part[j]);
+                            d_rate[n] = fmaf(dt, q, d_rate[n]);
+                        }
+                        float sum_b[KEPT], sum_c[KEPT];
+                        sum_channels<NPT>(d_b, sum_b);
+                        sum_channels<NPT>(d_c, sum_c);
+#pragma unroll
+                        for (int m = 0; m < KEPT; m++) { kept_b[m] = quad == j ? sum_b[m] : kept_b[m]; kept_c[m] = quad == j ? sum_c[m] : kept_c[m]; }
+                    };
+                    step(std::integral_constant<int, 3>{}); step(std::integral_constant<int, 2>{}); step(std::integral_constant<int, 1>{}); step(std::integral_constant<int, 0>{});
+                    mixed[i] = sum_to_lane(mixed_part, odd, upper);
+                    through[i] = sum_to_lane(through_part, odd, upper);
+                    exponent[i] = sum_to_lane(exponent_part, odd, upper);
+#pragma unroll
+                    for (int m = 0; m < KEPT; m++) { slabs[turn][wave][0][(4 * i + quad) * N + kept_state + m] = kept_b[m]; slabs[turn][wave][1][(4 * i + quad) * N + kept_state + m] = kept_c[m]; }
+                }
+            };
+            if (forget) walk(std::true_type{}); else walk(std::false_type{});
+#pragma unroll
+            for (int i = 0; i < OWN; i++) {
+                const int s = t + 4 * i + nq;
+                const float d_delta = fmaf(exponent[i], LN_2, through[i] * xs[i]) * slope[i];
+                d_skip = fmaf(d[i], xs[i], d_skip);
+                d_bias += d_delta;
+                if (there && s < p.end) {
+                    at<T>(a.d_x, s, p.row, p.head)[channel] = (T)fmaf(through[i], delta[i], skip * d[i]);
+                    at<T>(a.d_delta, s, p.row, p.head)[channel] = (T)d_delta;
+                    if (gated) at<T>(a.d_gate, s, p.row, p.head)[channel] = (T)(ups[i] * d_factor[i] * fmaf(skip, xs[i], mixed[i]));
+                }
+            }
+            rlt_lds_barrier();
+            for (int e = threadIdx.x; e < K * N; e += LANES) {
+                const int s = t + e / N;
+                if (s < p.end) {
+                    float d_b = 0.0f, d_c = 0.0f;
+#pragma unroll
+                    for (int w = 0; w < WAVES; w++) { d_b += slabs[turn][w][0][e]; d_c += slabs[turn][w][1][e]; }
+                    store_shared(s, e % N, d_b, d_c);
+                }
+            }
+        }
+        if (there && a.exit && p.segment == 0) store_states<NPT>(a.exit + (pair * a.channels + channel) * a.states, n0, a.states, carry);
+    }
+    if (!there) return;
+    const size_t part = (size_t)p.segment * a.row_groups + group, of_channel = (part * a.heads + p.head) * a.channels + channel;
+    if (a.d_rates) write<NPT>(a.d_rates + of_channel * N + n0, d_rate);
+    d_skip = sum_of_lanes(d_skip); d_bias = sum_of_lanes(d_bias);
+    if (nq == 0 && a.d_skips) a.d_skips[of_channel] = d_skip;
+    if (nq == 0 && a.d_biases) a.d_biases[of_channel] = d_bias;
+}
+
+// What a segment adds to the state's gradient that reaches it from its end, for the gradients that segments start from.
+template <typename T, int NPT> __global__ __launch_bounds__(LANES) void backward_states_kernel(Scan a) {
+    constexpr int K = CHUNK<NPT>, OWN = K / 4, N = 4 * NPT;
+    __shared__ float shared[2][2][K * N];
+    Place p = place_of(a, blockIdx.x, a.batch);
+    set_row(a, p, p.row);
+    const int lane = threadIdx.x & 63, nq = lane & 3, n0 = nq * NPT, own_channel = p.tile * TILE + (int)(threadIdx.x >> 2), channel = min(own_channel, a.channels - 1);
+    const bool there = own_channel < a.channels;
+    const size_t pair = pair_of(a, p);
+    float rate[NPT], carry[NPT], sum = 0.0f;
+    load_rates<NPT>(a, p.head, channel, n0, rate);
+    const float bias = a.delta_biases ? a.delta_biases[(size_t)p.head * a.channels + channel] : 0.0f;
+    bool forgotten = false;
+#pragma unroll
+    for (int n = 0; n < NPT; n++) carry[n] = 0.0f;
+    T raw[OWN], gate[OWN], d_out[OWN];
+    unsigned resets;
+    Shared<T, NPT> next;
+    auto ask_chunk = [&](int t) {
+        ask<T, OWN>(a, a.delta, p, channel, t, raw);
+        ask<T, OWN>(a, a.d_out, p, channel, t, d_out);
+        if (a.gate.data) ask<T, OWN>(a, a.gate, p, channel, t, gate);
+        next.ask(a, p, t, false);
+        resets = resets_of<K>(a, p, t);
+    };
+    const int chunks = p.live > p.first ? (p.live - p.first + K - 1) / K : 0;
+    if (chunks) ask_chunk(p.first + (chunks - 1) * K);
+    int turn = 0;
+    for (int k = chunks - 1; k >= 0; k--, turn ^= 1) {
+        const int t = p.first + k * K;
+        float delta[OWN], d[OWN];
+#pragma unroll
+        for (int i = 0; i < OWN; i++) {
+            const bool in = t + 4 * i + nq < p.live;
+            float e;
+            delta[i] = in ? softplus((float)raw[i] + bias, e) : 0.0f;
+            d[i] = in ? (float)d_out[i] : 0.0f;
+            if (a.gate.data) {
+                float one, other;
+                rlt_sigmoids((float)gate[i], one, other);
+                d[i] = in ? d[i] * (float)gate[i] * one : 0.0f;
+            }
+            sum += delta[i];
+        }
+        const unsigned forget = resets;
+        next.put(shared[turn]);
+        if (k > 0) ask_chunk(t - K);
+        rlt_lds_barrier();
+        const float* const cs = shared[turn][1] + n0;
+#pragma unroll
+        for (int i = OWN - 1; i >= 0; i--) {
+            auto step = [&](auto which) {
+                constexpr int j = decltype(which)::value;
+                const float dt = from_lane<j>(delta[i]), g = from_lane<j>(d[i]);
+                float c[NPT];
+                read<NPT>(cs + (4 * i + j) * N, c);
+#pragma unroll
+                for (int n = 0; n < NPT; n++) carry[n] = __builtin_amdgcn_exp2f(dt * rate[n]) * fmaf(c[n], g, carry[n]);
+                if (forget >> (4 * i + j) & 1) {
+                    forgotten = true;
+#pragma unroll
+                    for (int n = 0; n < NPT; n++) carry[n] = 0.0f;
+                }
+            };
+            step(std::integral_constant<int, 3>{}); step(std::integral_constant<int, 2>{}); step(std::integral_constant<int, 1>{}); step(std::integral_constant<int, 0>{});
+        }
+    }
+    if (!there) return;
+    write<NPT>(a.exit + ((pair * a.segments + p.segment) * a.channels + channel) * N + n0, carry);
+    sum = sum_of_lanes(sum);
+    if (nq == 0) a.sums[(pair * a.segments + p.segment) * a.channels + channel] = forgotten ? -1.0f : sum;
+}
+
+// d_b and d_c out of the tiles' shares
+template <typename T> __global__ __launch_bounds__(256) void shared_sum_kernel(Scan a, int padded) {
+    const size_t tokens = (size_t)a.steps * a.batch * a.heads, size = tokens * padded;
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < 2 * size; i += (size_t)gridDim.x * 256) {
+        const bool second = i >= size;
+        const size_t e = second ? i - size : i, token = e / padded, line = token / a.heads;
+        const int n = (int)(e - token * padded), head = (int)(token - line * a.heads), step = (int)(line / a.batch), row = (int)(line - (size_t)step * a.batch);
+        if (n >= a.states) continue;
+        float s = 0.0f;
+        for (int tile = 0; tile < a.tiles; tile++) s += a.d_shared[(size_t)tile * 2 * size + i];
+        at<T>(second ? a.d_c : a.d_b, step, row, head)[n] = (T)s;
+    }
+}
+
+// the parameters' gradients out of the workgroups' shares, in a fixed order: sixteen threads an element, whose sums are added up in LDS
+__global__ __launch_bounds__(1024) void parameter_sum_kernel(Scan a, int parts, int padded, float* __restrict__ d_log_rates, float* __restrict__ d_skip, float* __restrict__ d_delta_biases, int accumulate) {
+    __shared__ float sums[16][64];
+    const int lane = threadIdx.x & 63, group = threadIdx.x >> 6;
+    const size_t channels = (size_t)a.heads * a.channels, rates = channels * padded;
+    size_t i = (size_t)blockIdx.x * 64 + lane;
+    const bool of_rates = i < rates, of_skips = !of_rates && i < rates + channels, there = i < rates + 2 * channels;
+    const size_t columns = of_rates ? rates : channels;
+    const float* const from = of_rates ? a.d_rates : of_skips ? a.d_skips : a.d_biases;
+    i -= of_rates ? 0 : of_skips ? rates : rates + channels;
+    float s = 0.0f;
+    if (there && from)
+        for (int p = group; p < parts; p += 16) s += from[(size_t)p * columns + i];
+    sums[group][lane] = s;
+    __syncthreads();
+    if (group || !there || !from) return;
+    for (int g = 1; g < 16; g++) s += sums[g][lane];
+    float* to = of_skips ? d_skip + i : d_delta_biases + i;
+    if (of_rates) {
+        const size_t channel = i / padded;
+        const int n = (int)(i - channel * padded);
+        if (n >= a.states) return;
+        to = d_log_rates + channel * a.states + n;
+        s *= -expf(a.log_rates[channel * a.states + n]);
+    }
+    *to = accumulate ? *to + s : s;
+}
+
+// One step of a row: a pass over the states, which are read and written once. Four lanes share a channel.
+template <typename T, int NPT> __global__ __launch_bounds__(256) void step_kernel(Scan a) {
+    const size_t i = (size_t)blockIdx.x * 64 + (threadIdx.x >> 2), pair = i / a.channels;
+    const int channel = (int)(i - pair * a.channels), row = (int)(pair / a.heads), head = (int)(pair - (size_t)row * a.heads), nq = threadIdx.x & 3, n0 = nq * NPT;
+    if (pair >= (size_t)a.batch * a.heads) return;
+    const size_t at_channel = (size_t)head * a.channels + channel;
+    float rate[NPT], h[NPT], e, sum = 0.0f;
+    const bool forget = a.reset && a.reset[row];
+    load_states<NPT>(forget ? nullptr : a.entry + (pair * a.channels + channel) * a.states, n0, a.states, h);
+    load_rates<NPT>(a, head, channel, n0, rate);
+    const T* const b = at<T>(a.b, 0, row, head); const T* const c = at<T>(a.c, 0, row, head);
+    const float x = (float)at<T>(a.x, 0, row, head)[channel], delta = softplus((float)at<T>(a.delta, 0, row, head)[channel] + (a.delta_biases ? a.delta_biases[at_channel] : 0.0f), e), u = delta * x;
+#pragma unroll
+    for (int n = 0; n < NPT; n++) {
+        const bool there = n0 + n < a.states;
+        h[n] = fmaf(__builtin_amdgcn_exp2f(delta * rate[n]), h[n], there ? u * (float)b[n0 + n] : 0.0f);
+        if (there) sum = fmaf((float)c[n0 + n], h[n], sum);
+    }
+    store_states<NPT>(a.exit + (pair * a.channels + channel) * a.states, n0, a.states, h);
+    sum = sum_of_lanes(sum);
+    if (nq == 0) {
+        float v = a.skip ? fmaf(a.skip[at_channel], x, sum) : sum;
+        if (a.gate.data) {
+            const float z = (float)at<T>(a.gate, 0, row, head)[channel];
+            float one, other;
+            rlt_sigmoids(z, one, other);
+            v *= z * one;
+        }
+        at<T>(a.out, 0, row, head)[channel] = (T)v;
+    }
+}
+
+bool described(const rlt_selective_scan* p) {
+    return p && (p->type == RLT_TYPE_F32 || p->type == RLT_TYPE_BF16) && p->batch > 0 && p->heads > 0 && p->channels > 0 && p->states > 0;
+}
+int tiles_of(const rlt_selective_scan* p) { return (p->channels + TILE - 1) / TILE; }
+
+// Steps are cut into segments where rows, heads and channels alone leave the chip without work.
+struct Segments { int count, steps, row_groups; };
+Segments segments_of(const rlt_selective_scan* p, int steps) {
+    const int chunk = chunk_of(p->states), chunks = (steps + chunk - 1) / chunk;
+    const int64_t blocks = (int64_t)p->batch * p->heads * tiles_of(p), wanted = 512;
+    int64_t count = blocks >= wanted ? 1 : (wanted + blocks - 1) / blocks;
+    if (count > chunks / 4) count = chunks / 4;
+    if (count < 1) count = 1;
+    const int per = (int)((chunks + count - 1) / count);
+    Segments g = {(chunks + per - 1) / per, per * chunk, 0};
+    int64_t groups = 2048 / ((int64_t)p->heads * tiles_of(p) * g.count);      // rows are walked one after the other where there are more than fill the chip
+    g.row_groups = (int)(groups < 1 ? 1 : groups < p->batch ? groups : p->batch);
+    return g;
+}
+bool supported(const rlt_selective_scan* p, int steps) {
+    if (p->states > MAX_STATES || steps > MAX_STEPS) return false;
+    const __int128 pairs = (__int128)p->batch * p->heads, limit = (__int128)1 << 31;
+    if (pairs * p->channels * MAX_STATES > limit || pairs * steps > limit) return false;
+    const __int128 blocks = pairs * tiles_of(p) * segments_of(p, steps).count;
+    return blocks * LANES <= UINT32_MAX;
+}
+size_t padded(size_t n) { return (n + 63) / 64 * 64; }
+// scratch memory, in floats
+struct Scratch { size_t states, sums, shared, rates, skips, biases, total; };
+Scratch scratch_of(const rlt_selective_scan* p, int steps, bool backward) {
+    const Segments g = segments_of(p, steps);
+    const size_t channels = (size_t)p->batch * p->heads * p->channels, wide = 4 * per_lane(p->states), parts = (size_t)g.row_groups * g.count * p->heads * p->channels;
+    Scratch s{};
+    size_t at = 0;
+    auto take = [&](size_t n) { const size_t here = at; at += padded(n); return here; };
+    if (g.count > 1) { s.states = take(channels * g.count * wide); s.sums = take(channels * g.count); }
+    if (backward) {
+        if (tiles_of(p) > 1) s.shared = take((size_t)tiles_of(p) * 2 * steps * p->batch * p->heads * wide);
+        s.rates = take(parts * wide); s.skips = take(parts); s.biases = take(parts);
+    }
+    s.total = at;
+    return s;
+}
+Scan scan_of(const rlt_selective_scan* p, const rlt_head_view* x, const rlt_head_view* delta, const rlt_head_view* b, const rlt_head_view* c, const rlt_head_view* gate, const uint8_t* reset,
+             const int32_t* lengths, int steps) {
+    const Segments g = segments_of(p, steps);
+    Scan a{};
+    a.log_rates = p->log_rates; a.skip = p->skip; a.delta_biases = p->delta_biases;
+    a.x = rlt_part_of(x); a.delta = rlt_part_of(delta); a.b = rlt_part_of(b); a.c = rlt_part_of(c); a.gate = rlt_part_of(gate);
+    a.reset = reset; a.lengths = lengths; a.batch = p->batch; a.heads = p->heads; a.channels = p->channels; a.states = p->states; a.steps = steps;
+    a.segments = g.count; a.segment_steps = g.steps; a.row_groups = g.row_groups; a.tiles = tiles_of(p); a.chunks = (steps + chunk_of(p->states) - 1) / chunk_of(p->states);
+    return a;
+}
+template <typename F> int by_kind(const rlt_selective_scan* p, F&& f) {
+    auto typed = [&](auto type) {
+        const int n = per_lane(p->states);
+        return n == 2 ? f(type, std::integral_constant<int, 2>{}) : n == 4 ? f(type, std::integral_constant<int, 4>{}) : f(type, std::integral_constant<int, 8>{});
+    };
+    return p->type == RLT_TYPE_F32 ? typed(0.0f) : typed((rlt_bf16)0.0f);
+}
+unsigned blocks_of(const Scan& a, int rows) { return (unsigned)a.tiles * a.heads * a.segments * rows; }
+template <bool REVERSE> int join_segments(rlt_rocm_device* device, const Scan& a, const float* initial, float* states, int wide) {
+    const size_t blocks = ((size_t)a.batch * a.heads * a.channels * wide + 255) / 256;
+    hipLaunchKernelGGL(join_segments_kernel<REVERSE>, dim3((unsigned)blocks), dim3(256), 0, device->stream, a, initial, states, wide);
+    return rlt_launch_status(device);
+}
+bool given(const rlt_selective_scan* p, const rlt_head_view* x, const rlt_head_view* delta, const rlt_head_view* b, const rlt_head_view* c, const rlt_head_view* gate) {
+    return described(p) && p->log_rates && rlt_given(x) && rlt_given(delta) && rlt_given(b) && rlt_given(c) && (!gate || gate->data);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t rlt_rocm_selective_scan_workspace_bytes(const rlt_selective_scan* layer, int steps, int backward) {
+    if (!described(layer) || steps <= 0 || !supported(layer, steps)) return 0;
+    return scratch_of(layer, steps, backward != 0).total * sizeof(float);
+}
+size_t rlt_rocm_selective_scan_checkpoint_bytes(const rlt_selective_scan* layer, int steps) {
+    if (!described(layer) || steps <= 0 || !supported(layer, steps)) return 0;
+    const int chunk = chunk_of(layer->states);
+    return (size_t)layer->batch * layer->heads * ((steps + chunk - 1) / chunk) * layer->channels * 4 * per_lane(layer->states) * sizeof(float);
+}
+
+int rlt_rocm_selective_scan_forward(rlt_rocm_device* device, const rlt_selective_scan* layer, const rlt_head_view* x, const rlt_head_view* delta, const rlt_head_view* b, const rlt_head_view* c,
+                                    const rlt_head_view* gate, const rlt_head_view* output, const float* initial_state, float* final_state, const uint8_t* reset, const int32_t* lengths, int steps,
+                                    void* checkpoints, void* workspace, size_t workspace_bytes) {
+    if (!device) return RLT_E_NOT_INITIALISED;
+    RLT_REQUIRE(given(layer, x, delta, b, c, gate) && rlt_given(output) && steps > 0 && reinterpret_cast<uintptr_t>(checkpoints) % 16 == 0);
+    if (!supported(layer, steps)) return RLT_E_UNSUPPORTED;
+    const Scratch s = scratch_of(layer, steps, false);
+    RLT_REQUIRE(s.total == 0 || (workspace && workspace_bytes >= s.total * sizeof(float) && reinterpret_cast<uintptr_t>(workspace) % 16 == 0));
+    Scan a = scan_of(layer, x, delta, b, c, gate, reset, lengths, steps);
+    a.out = rlt_part_of(output); a.checkpoints = (float*)checkpoints; a.entry = initial_state; a.exit = final_state;
+    return by_kind(layer, [&](auto type, auto n) {
+        typedef decltype(type) T;
+        constexpr int NPT = decltype(n)::value;
+        if (a.segments > 1) {
+            Scan f = a;
+            float* const states = (float*)workspace + s.states;
+            f.sums = (float*)workspace + s.sums; f.exit = states;
+            hipLaunchKernelGGL((forward_kernel<T, NPT, true>), dim3(blocks_of(a, a.batch)), dim3(LANES), 0, device->stream, f);
+            int rc = rlt_launch_status(device);
+            if (rc || (rc = join_segments<false>(device, f, initial_state, states, 4 * NPT))) return rc;
+            a.entry = states; a.entry_padded = 1;
+        }
+        hipLaunchKernelGGL((forward_kernel<T, NPT, false>), dim3(blocks_of(a, a.batch)), dim3(LANES), 0, device->stream, a);
+        return rlt_launch_status(device);
+    });
+}
+
+int rlt_rocm_selective_scan_backward(rlt_rocm_device* device, const rlt_selective_scan* layer, const rlt_head_view* x, const rlt_head_view* delta, const rlt_head_view* b, const rlt_head_view* c,
+                                     const rlt_head_view* gate, const rlt_head_view* d_output, const rlt_head_view* d_x, const rlt_head_view* d_delta, const rlt_head_view* d_b, const rlt_head_view* d_c,
+                                     const rlt_head_view* d_gate, const float* d_final_state, float* d_initial_state, int accumulate, const uint8_t* reset, const int32_t* lengths, int steps,
+                                     const void* checkpoints, void* workspace, size_t workspace_bytes) {
+    if (!device) return RLT_E_NOT_INITIALISED;
+    RLT_REQUIRE(given(layer, x, delta, b, c, gate) && rlt_given(d_output) && rlt_given(d_x) && rlt_given(d_delta) && rlt_given(d_b) && rlt_given(d_c) && (!gate || rlt_given(d_gate)) && steps > 0);
+    RLT_REQUIRE(checkpoints && reinterpret_cast<uintptr_t>(checkpoints) % 16 == 0);
+    if (!supported(layer, steps)) return RLT_E_UNSUPPORTED;
+    const Scratch s = scratch_of(layer, steps, true);
+    RLT_REQUIRE(workspace && workspace_bytes >= s.total * sizeof(float) && reinterpret_cast<uintptr_t>(workspace) % 16 == 0);
+    float* const w = (float*)workspace;
+    Scan a = scan_of(layer, x, delta, b, c, gate, reset, lengths, steps);
+    a.d_out = rlt_part_of(d_output); a.d_x = rlt_part_of(d_x); a.d_delta = rlt_part_of(d_delta); a.d_b = rlt_part_of(d_b); a.d_c = rlt_part_of(d_c); a.d_gate = rlt_part_of(d_gate);
+    a.checkpoints = (float*)const_cast<void*>(checkpoints); a.entry = d_final_state; a.exit = d_initial_state;
+    a.d_shared = w + s.shared; a.d_rates = layer->d_log_rates ? w + s.rates : nullptr; a.d_skips = layer->d_skip ? w + s.skips : nullptr; a.d_biases = layer->d_delta_biases ? w + s.biases : nullptr;
+    return by_kind(layer, [&](auto type, auto n) {
+        typedef decltype(type) T;
+        constexpr int NPT = decltype(n)::value;
+        int rc;
+        if (a.segments > 1) {
+            Scan f = a;
+            f.sums = w + s.sums; f.exit = w + s.states;
+            hipLaunchKernelGGL((backward_states_kernel<T, NPT>), dim3(blocks_of(a, a.batch)), dim3(LANES), 0, device->stream, f);
+            if ((rc = rlt_launch_status(device)) || (rc = join_segments<true>(device, f, d_final_state, f.exit, 4 * NPT))) return rc;
+            a.entry = f.exit; a.entry_padded = 1;
+        }
+        hipLaunchKernelGGL((backward_kernel<T, NPT>), dim3(blocks_of(a, a.row_groups)), dim3(LANES), 0, device->stream, a);
+        if ((rc = rlt_launch_status(device))) return rc;
+        if (a.tiles > 1) {
+            hipLaunchKernelGGL(shared_sum_kernel<T>, dim3(2048), dim3(256), 0, device->stream, a, 4 * NPT);
+            if ((rc = rlt_launch_status(device))) return rc;
+        }
+        if (!a.d_rates && !a.d_skips && !a.d_biases) return 0;
+        const size_t elements = (size_t)layer->heads * layer->channels * (4 * NPT + 2);
+        hipLaunchKernelGGL(parameter_sum_kernel, dim3((unsigned)((elements + 63) / 64)), dim3(1024), 0, device->stream, a, a.row_groups * a.segments, 4 * NPT, layer->d_log_rates, layer->d_skip,
+                           layer->d_delta_biases, accumulate);
+        return rlt_launch_status(device);
+    });
+}
+
+int rlt_rocm_selective_scan_step(rlt_rocm_device* device, const rlt_selective_scan* layer, const rlt_head_view* x, const rlt_head_view* delta, const rlt_head_view* b, const rlt_head_view* c,
+                                 const rlt_head_view* gate, const rlt_head_view* output, const float* state, float* next_state, const uint8_t* reset) {
+    if (!device) return RLT_E_NOT_INITIALISED;
+    RLT_REQUIRE(given(layer, x, delta, b, c, gate) && rlt_given(output) && state && next_state);
+    if (!supported(layer, 1)) return RLT_E_UNSUPPORTED;
+    Scan a = scan_of(layer, x, delta, b, c, gate, reset, nullptr, 1);
+    a.out = rlt_part_of(output); a.entry = state; a.exit = next_state;
+    return by_kind(layer, [&](auto type, auto n) {
+        const size_t blocks = ((size_t)a.batch * a.heads * a.channels + 63) / 64;
+        hipLaunchKernelGGL((step_kernel<decltype(type), decltype(n)::value>), dim3((unsigned)blocks), dim3(256), 0, device->stream, a);
+        return rlt_launch_status(device);
+    });
+}
+
+}  // extern "C"

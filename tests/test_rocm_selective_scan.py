@@ -1,0 +1,480 @@
+"""The selective scan, forward, backward and single steps, against the recurrence in 64 bits.
+
+Bounds, set before the first run; u = 2^-24. Every output is a sum of products; with the inputs, the gate's factors and the rates of the sums (not those of the exponents) replaced by their absolute values the reference gives the sum of the
+products' magnitudes, M. A product holds up to `steps` decays, exp(-rate delta): its argument is off by at most 16 u of itself (delta: an exponential with a first-order correction, a reciprocal, a polynomial, sums: eight; the rate: an
+exponential and its factor: four; the product and the power's own), the power itself by 2 u, and h's sum rounds once a step. With E the largest sum of rate * delta over a row's steps that is: (4 steps + 16 E) u, and the other factors (delta, the gate's
+sigmoid and its slope, delta's slope: at most 12 u each, of which a product has at most four), the sums over states and channels add (64 + channels + states) u. Sums over steps and rows round once more for each: (steps + rows) u.
+bfloat16 adds the output's own rounding, 2^-8 of the value."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from helpers import capi, package
+from test_rocm_linear_attention import Tensor, strides_of, view
+from typed_arrays import UNIT, download, filled, rounded, to_bits, upload
+
+gpu = pytest.mark.gpu
+U = 2.0 ** -24
+SEQUENCES = ("x", "delta", "b", "c", "gate", "d_output")
+PARAMETERS = ("log_rates", "skip", "delta_biases")
+
+
+def sigmoid(z):
+    e = np.exp(-np.abs(z))
+    return np.where(z >= 0, 1 / (1 + e), e / (1 + e))
+
+
+def factors(x):
+    """what the exponentials and the gate make of the inputs: delta and its slope, the gate's factor and its slope, the rates"""
+    raw = x["delta"] + (x["delta_biases"].astype(np.float64) if x.get("delta_biases") is not None else 0.0)
+    f = dict(delta=np.logaddexp(raw, 0.0), slope=sigmoid(raw), rates=np.exp(x["log_rates"].astype(np.float64)), factor=np.ones_like(raw), d_factor=np.zeros_like(raw))
+    if x.get("gate") is not None:
+        z = x["gate"]
+        f.update(factor=z * sigmoid(z), d_factor=sigmoid(z) * (1 + z * sigmoid(-z)))
+    return f
+
+
+def reference(c, x, f=None, sign=-1.0):
+    """All outputs by the recurrence in 64 bits. sign: of the rates in the sums (+1 for magnitudes)."""
+    f = factors(x) if f is None else f
+    steps, rows = c["steps"], c["rows"]
+    shape = (rows, c["heads"], c["channels"], c["states"])
+    rates, skip = f["rates"], x["skip"].astype(np.float64) if x.get("skip") is not None else np.zeros((c["heads"], c["channels"]))
+    lengths = np.clip(x["lengths"], 0, steps) if x.get("lengths") is not None else np.full(rows, steps)
+    h = np.zeros(shape) if x.get("state") is None else x["state"].astype(np.float64)
+    d = {n: np.zeros(s) for n, s in (("x", x["x"].shape), ("delta", x["x"].shape), ("gate", x["x"].shape), ("b", x["b"].shape), ("c", x["b"].shape), ("log_rates", rates.shape), ("skip", skip.shape), ("delta_biases", skip.shape))}
+    out, entries = np.zeros_like(x["x"]), []
+    flags = lambda t: ((t < lengths)[:, None, None, None], (x["reset"][t] != 0)[:, None, None, None] if x.get("reset") is not None else np.zeros((rows, 1, 1, 1), bool))
+    with np.errstate(invalid="ignore"):
+        for t in range(steps):
+            live, begins = flags(t)
+            entries.append(np.where(begins, 0.0, h))
+            after = np.exp(-rates * f["delta"][t][..., None]) * entries[-1] + (f["delta"][t] * x["x"][t])[..., None] * x["b"][t][:, :, None]
+            out[t] = np.where(live[..., 0], ((x["c"][t][:, :, None] * after).sum(-1) + skip * x["x"][t]) * f["factor"][t], 0.0)
+            h = np.where(live, after, h)
+        grad = np.zeros(shape) if x.get("d_state") is None else x["d_state"].astype(np.float64)
+        for t in reversed(range(steps)):
+            live, begins = flags(t)
+            decay, u = np.exp(-rates * f["delta"][t][..., None]), f["delta"][t] * x["x"][t]
+            after = np.where(live, decay * entries[t] + u[..., None] * x["b"][t][:, :, None], 0.0)
+            up = np.where(live[..., 0], x["d_output"][t], 0.0)
+            on = lambda a: np.where(live[..., 0], a, 0.0)
+            read, added, x_t = np.where(live, x["c"][t][:, :, None], 0.0), np.where(live, x["b"][t][:, :, None], 0.0), on(x["x"][t])
+            d["gate"][t] = on(up * ((read * after).sum(-1) + skip * x_t) * f["d_factor"][t])
+            g = on(up * f["factor"][t])
+            d["skip"] += (g * x_t).sum(0)
+            d["c"][t] = (g[..., None] * after).sum(2)
+            here = np.where(live, grad + g[..., None] * read, 0.0)
+            d["b"][t] = np.where(live, here * u[..., None], 0.0).sum(2)
+            through = (here * added).sum(-1)
+            d["x"][t] = on(through * f["delta"][t]) + skip * g
+            q = np.where(live, here * decay * entries[t], 0.0)
+            d["log_rates"] += sign * np.where(live, q * f["delta"][t][..., None] * rates, 0.0).sum(0)
+            d["delta"][t] = on((through * x_t + sign * (q * rates).sum(-1)) * f["slope"][t])
+            d["delta_biases"] += d["delta"][t].sum(0)
+            grad = np.where(live, np.where(begins, 0.0, decay * here), grad)
+    return dict({"d_" + n: a for n, a in d.items()}, output=out, state=h, d_state=grad)
+
+
+def case(seed, dtype, steps, rows, heads, channels, states, resets=0.0, ragged=False, with_state=True, gate=True, parameters=True, size=0.3):
+    rng = np.random.default_rng(seed)
+    n = lambda *shape: rounded(rng.standard_normal(shape), dtype)
+    wide, narrow = (steps, rows, heads, channels), (steps, rows, heads, states)
+    x = dict(x=n(*wide), delta=n(*wide), b=n(*narrow), c=n(*narrow), d_output=n(*wide), log_rates=(np.log(np.arange(1, states + 1)) + 0.1 * rng.standard_normal((heads, channels, states))).astype(np.float32))
+    if gate:
+        x["gate"] = n(*wide)
+    if parameters:
+        x["skip"], x["delta_biases"] = rng.standard_normal((heads, channels)).astype(np.float32), (np.log(size) + rng.uniform(-2, 0, (heads, channels))).astype(np.float32)
+    if with_state:
+        x["state"], x["d_state"] = (rng.standard_normal((rows, heads, channels, states)).astype(np.float32) for _ in range(2))
+    if resets:
+        x["reset"] = (rng.random((steps, rows)) < resets).astype(np.uint8)
+    if ragged:
+        x["lengths"] = rng.integers(0, steps + 1, rows).astype(np.int32)
+        x["lengths"][0], x["lengths"][-1] = 0, steps + 5      # an empty row; one that claims more than there is
+    return dict(dtype=dtype, steps=steps, rows=rows, heads=heads, channels=channels, states=states), x
+
+
+def magnitudes(c, x, f):
+    """The gate's slope, s (1 + z (1 - s)) with s = sigmoid(z), is a sum whose terms cancel near z = -1.28: what its roundings are relative to is s (1 + |z| (1 - s)) there, not the slope itself."""
+    sizes = {n: np.abs(a) for n, a in f.items()}
+    if x.get("gate") is not None:
+        sizes["d_factor"] = sigmoid(x["gate"]) * (1 + np.abs(x["gate"]) * sigmoid(-x["gate"]))
+    return reference(c, {n: (a if n in ("reset", "lengths") else np.abs(a)) for n, a in x.items()}, sizes, 1.0)
+
+
+def bounds(c, x, want):
+    f = factors(x)
+    size = magnitudes(c, x, f)
+    E = (f["rates"] * f["delta"][..., None]).sum(0).max()
+    unit = (4 * c["steps"] + 16 * E + 64 + c["channels"] + c["states"]) * U
+    b = {n: unit * m for n, m in size.items()}
+    for n in PARAMETERS:
+        b["d_" + n] = b["d_" + n] + (c["steps"] + c["rows"]) * U * size["d_" + n]
+    if c["dtype"] == "bfloat16":
+        for n in ("output", "d_x", "d_delta", "d_b", "d_c", "d_gate"):
+            b[n] = b[n] + UNIT["bfloat16"] * (np.abs(want[n]) + b[n])
+    return b
+
+
+def check(c, x, got, names=None):
+    want = reference(c, x)
+    b = bounds(c, x, want)
+    for n in names or got:
+        off = np.abs(got[n] - want[n]) - b[n]
+        assert np.all(off <= 0), (n, float(off.max()), float(np.abs(got[n] - want[n]).max()), float(np.abs(want[n]).max()))
+
+
+def layer_of(rocm, c, x, keep, onto=7.0, gradients=True):
+    for n in PARAMETERS:
+        keep[n] = rocm.array(x[n]) if x.get(n) is not None else None
+        keep["d_" + n] = rocm.array(np.full((c["heads"], c["channels"]) + ((c["states"],) if n == "log_rates" else ()), onto, np.float32))
+    ptr = lambda a: a.ptr if a is not None else None
+    return capi.SelectiveScan(*[ptr(keep[n]) for n in PARAMETERS], *[keep["d_" + n].ptr if gradients else None for n in PARAMETERS], capi.TYPE[c["dtype"]], c["rows"], c["heads"], c["channels"], c["states"], 0)
+
+
+class Buffers:
+    """a case's tensors, states and scratch memory on the device"""
+
+    def __init__(self, rocm, c, x, order=(0, 1, 2), gap=0, offset=0, onto=None):
+        self.rocm, self.c, self.x, self.keep, self.onto = rocm, c, x, {}, onto
+        self.layer = layer_of(rocm, c, x, self.keep, 7.0 if onto is None else onto)
+        dtype, steps = c["dtype"], c["steps"]
+        self.t = {n: Tensor(rocm, x[n], dtype, order, gap, offset=offset) for n in SEQUENCES if x.get(n) is not None}
+        shapes = {"output": "x", "d_x": "x", "d_delta": "x", "d_b": "b", "d_c": "c", "d_gate": "gate"}
+        self.o = {n: Tensor(rocm, x[like].shape, dtype, order, gap, value=7.0, offset=offset) for n, like in shapes.items() if x.get(like) is not None}
+        up = lambda n: rocm.array(x[n]) if x.get(n) is not None else None
+        self.state, self.d_state, self.reset, self.lengths = up("state"), up("d_state"), up("reset"), up("lengths")
+        shape = (c["rows"], c["heads"], c["channels"], c["states"])
+        self.final, self.d_initial = filled(rocm, shape, "float32"), filled(rocm, shape, "float32")
+        lib, layer = rocm.device.lib, C.byref(self.layer)
+        bytes_of = lambda n: rocm.device.empty((max(int(n), 16),), np.uint8)
+        self.sizes = [lib.rlt_rocm_selective_scan_workspace_bytes(layer, steps, k) for k in (0, 1)]
+        self.scratch = [bytes_of(n) for n in self.sizes]
+        self.checkpoints = bytes_of(lib.rlt_rocm_selective_scan_checkpoint_bytes(layer, steps))
+
+    def inputs(self):
+        return [self.t[n].view if n in self.t else None for n in SEQUENCES[:5]]
+
+    def tail(self, backward):
+        ptr = lambda a: a.ptr if a is not None else None
+        return ptr(self.reset), ptr(self.lengths), self.c["steps"], self.checkpoints.ptr, self.scratch[backward].ptr, self.sizes[backward]
+
+    def forward(self):
+        ptr = lambda a: a.ptr if a is not None else None
+        self.rocm.call("selective_scan_forward", C.byref(self.layer), *self.inputs(), self.o["output"].view, ptr(self.state), self.final.ptr, *self.tail(0))
+
+    def backward(self):
+        ptr = lambda a: a.ptr if a is not None else None
+        outs = [self.o[n].view if n in self.o else None for n in ("d_x", "d_delta", "d_b", "d_c", "d_gate")]
+        self.rocm.call("selective_scan_backward", C.byref(self.layer), *self.inputs(), self.t["d_output"].view, *outs, ptr(self.d_state), self.d_initial.ptr, int(self.onto is not None), *self.tail(1))
+
+    def results(self):
+        f = lambda a: a.numpy().astype(np.float64)
+        for a in self.o.values():
+            assert np.all(a.whole()[..., a.shape[3]:] == 7.0)      # nothing is written between the rows
+        return dict({n: a.numpy() for n, a in self.o.items()}, state=f(self.final), d_state=f(self.d_initial), **{"d_" + n: f(self.keep["d_" + n]) for n in PARAMETERS})
+
+
+def run(rocm, c, x, **layout):
+    b = Buffers(rocm, c, x, **layout)
+    b.forward()
+    b.backward()
+    rocm.sync()
+    return b.results()
+
+
+# ------------------------------------------------------------------ the reference itself (no GPU)
+
+
+def test_the_references_gradients_are_its_differences():
+    c, x = case(0, "float32", 7, 3, 2, 3, 4, resets=0.2, ragged=True)
+    x = {n: (a.astype(np.float64) if a.dtype.kind == "f" else a) for n, a in x.items()}
+
+    def loss(y):
+        r = reference(c, y)
+        return (r["output"] * x["d_output"]).sum() + (r["state"] * x["d_state"]).sum()
+    got, rng = reference(c, x), np.random.default_rng(2)
+    for name in ("x", "delta", "b", "c", "gate", "state", "log_rates", "skip", "delta_biases"):
+        direction, h = rng.standard_normal(x[name].shape), 1e-5
+        numeric = (loss(dict(x, **{name: x[name] + h * direction})) - loss(dict(x, **{name: x[name] - h * direction}))) / (2 * h)
+        assert abs(numeric - (got["d_" + name] * direction).sum()) <= 1e-7 * max(1.0, abs(numeric)), name
+
+
+# ------------------------------------------------------------------ sequences
+
+SHAPES = [  # steps, rows, heads, channels, states
+    (1, 1, 1, 1, 1), (1, 3, 2, 16, 16), (2, 2, 1, 17, 4), (15, 3, 1, 64, 16), (16, 2, 2, 65, 16), (17, 2, 1, 63, 15), (31, 2, 1, 48, 8), (33, 3, 2, 24, 32), (64, 2, 1, 130, 16), (65, 1, 3, 40, 31), (100, 2, 1, 33, 9),
+    (129, 1, 1, 16, 25), (300, 2, 1, 20, 16), (700, 1, 2, 16, 5), (900, 1, 1, 12, 20), (20, 300, 1, 8, 16), (3, 60, 40, 8, 4)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_forward_and_backward(rocm, shape, dtype):
+    print("case", shape, dtype, flush=True)
+    c, x = case(sum(shape), dtype, *shape)
+    check(c, x, run(rocm, c, x))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("shape", [(1, 5, 2, 16, 16), (40, 6, 1, 70, 16), (64, 9, 2, 16, 8), (200, 4, 1, 33, 32), (333, 5, 1, 24, 11), (600, 2, 1, 16, 16)])
+@pytest.mark.parametrize("resets", [0.02, 0.3, 1.0])
+def test_resets_and_lengths(rocm, shape, dtype, resets):
+    print("case", shape, dtype, resets, flush=True)
+    c, x = case(sum(shape), dtype, *shape, resets=resets, ragged=True)
+    check(c, x, run(rocm, c, x))
+
+
+@gpu
+@pytest.mark.parametrize("order,gap,offset", [((1, 2, 0), 0, 0), ((2, 1, 0), 0, 0), ((1, 0, 2), 8, 0), ((0, 1, 2), 5, 3), ((0, 2, 1), 1, 1)])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_orders_gaps_and_alignments(rocm, order, gap, offset, dtype):
+    print("case", order, gap, offset, dtype, flush=True)
+    c, x = case(7, dtype, 130, 3, 2, 80, 16, resets=0.05, ragged=True)
+    check(c, x, run(rocm, c, x, order=order, gap=gap, offset=offset))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_a_sequence_backwards_in_memory(rocm, dtype):
+    c, x = case(8, dtype, 150, 2, 1, 32, 16, ragged=True)
+    b = Buffers(rocm, c, x)
+    item, back = 4 if dtype == "float32" else 2, {}
+    for n, a in list(b.t.items()) + list(b.o.items()):
+        width = 2 * a.shape[3]
+        if n in b.t:
+            a.array.upload(x[n][::-1].astype(np.float32) if dtype == "float32" else to_bits(x[n][::-1].astype(np.float32)))
+        a.view = view(a.array, (-width, a.shape[3], a.shape[3]), item, 149 * width)
+    b.forward()
+    b.backward()
+    rocm.sync()
+    got = b.results()
+    check(c, x, {n: (a[::-1] if n in b.o else a) for n, a in got.items()})
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_without_states_gate_or_parameters(rocm, dtype):
+    for kinds in (dict(with_state=False), dict(gate=False), dict(parameters=False), dict(with_state=False, gate=False, parameters=False)):
+        c, x = case(11, dtype, 90, 3, 2, 48, 16, **kinds)
+        got = run(rocm, c, x)
+        check(c, x, got)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_steps_from_tiny_to_huge_and_rates_from_none_to_all(rocm, dtype):
+    """deltas whose exponentials leave the range of fp32 on either side, rates of zero and of infinity"""
+    c, x = case(13, dtype, 60, 2, 1, 16, 16)
+    x["delta"][:] = rounded(np.linspace(-120, 120, 16)[None, None, None] + np.zeros(x["delta"].shape), dtype)
+    x["log_rates"][0, :, 0] = -np.inf
+    x["log_rates"][0, :, 1] = 30.0
+    x["gate"][:] = rounded(np.linspace(-100, 100, 60)[:, None, None, None] + np.zeros(x["gate"].shape), dtype)
+    got, want = run(rocm, c, x), reference(c, x)
+    f = factors(x)
+    b = bounds(c, x, want)
+    # E counts what decays to nothing: a state of a product e^-E is off by E e^-E at most, 0.37 of a unit each; 64 units more than cover it, and numbers below fp32's smallest normal one are zero
+    unit = (4 * 60 + 16 * 60 + 64 + 32) * U
+    size = magnitudes(c, x, f)
+    for n in ("output", "state", "d_x", "d_b", "d_c", "d_gate", "d_state"):
+        limit = unit * size[n] + 1e-35 * (1 + size[n]) * 1e3 + (UNIT["bfloat16"] * np.abs(want[n]) + 1e-38 if dtype == "bfloat16" and n not in ("state", "d_state") else 0.0)
+        assert np.isfinite(got[n]).all() and np.all(np.abs(got[n] - want[n]) <= limit), n
+    assert np.isfinite(got["d_delta"]).all() and b is not None
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("steps", [150, 900])
+def test_what_lies_beyond_a_rows_length_is_not_looked_at(rocm, dtype, steps):
+    c, x = case(17, dtype, steps, 6, 1, 20, 16, resets=0.05, ragged=True)
+    beyond = np.arange(steps)[:, None] >= np.clip(x["lengths"], 0, steps)[None]
+    clean = {n: a.copy() for n, a in x.items()}
+    for i, n in enumerate(SEQUENCES):
+        x[n][beyond] = (np.nan, np.inf, -np.inf, np.nan, np.inf, -np.inf)[i]
+    x["reset"][beyond] = 1
+    got = run(rocm, c, x)
+    check(c, clean, got)
+    for n in ("output", "d_x", "d_delta", "d_b", "d_c", "d_gate"):
+        assert np.all(got[n][beyond] == 0.0), n
+    assert np.array_equal(got["state"][0], x["state"][0].astype(np.float64))      # the empty row's state, bit for bit
+    assert np.array_equal(got["d_state"][0], x["d_state"][0].astype(np.float64))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("steps", [1, 100, 700])
+def test_a_reset_forgets_a_state_that_is_not_finite(rocm, dtype, steps):
+    c, x = case(19, dtype, steps, 3, 1, 20, 16)
+    x["reset"] = np.zeros((steps, 3), np.uint8)
+    x["reset"][0] = 1
+    clean = {n: a.copy() for n, a in x.items()}
+    x["state"][0], x["state"][1], x["state"][2] = np.nan, np.inf, -np.inf
+    check(c, clean, run(rocm, c, x))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("steps", [200, 800])
+def test_an_episode_does_not_see_values_of_another_that_are_not_finite(rocm, dtype, steps):
+    """row 0: a step of its first episode holds values that are not finite, in the chunk in which the second episode begins: from there on everything is as if they were. A later episode's do not reach the one before either"""
+    c, x = case(41, dtype, steps, 3, 1, 24, 16)
+    x["reset"] = np.zeros((steps, 3), np.uint8)
+    x["reset"][[75, 90, 140], 0] = 1
+    x["reset"][75, 2] = 1
+    want = reference(c, x)
+    b = bounds(c, x, want)
+    for i, n in enumerate(SEQUENCES):
+        x[n][70, 0] = (np.nan, np.inf, np.nan, -np.inf, np.nan, np.inf)[i]
+        x[n][78, 2] = (np.nan, np.inf, np.nan, -np.inf, np.nan, np.inf)[i]
+    got = run(rocm, c, x)
+    for n in ("output", "d_x", "d_delta", "d_b", "d_c", "d_gate"):
+        off = np.abs(got[n] - want[n]) <= b[n]
+        assert np.all(off[75:, 0]) and np.all(off[:, 1]) and np.all(off[:75, 2]), n
+    assert np.all(np.abs(got["state"] - want["state"])[:2] <= b["state"][:2]) and np.all(np.abs(got["d_state"] - want["d_state"])[1:] <= b["d_state"][1:])
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(200, 5, 1, 70, 16), (700, 1, 1, 130, 16)])
+def test_gradients_add_up_and_runs_repeat_bit_for_bit(rocm, shape):
+    c, x = case(23, "float32", *shape, resets=0.02, ragged=shape[1] > 1)
+    first, second, onto = run(rocm, c, x), run(rocm, c, x), run(rocm, c, x, onto=3.0)
+    for n in first:
+        assert np.array_equal(first[n], second[n]), n
+    for n in PARAMETERS:
+        assert np.allclose(onto["d_" + n], first["d_" + n] + 3.0, rtol=2e-7, atol=0), n
+
+
+@gpu
+@pytest.mark.parametrize("steps", [40, 700])
+def test_optional_arguments_and_states_in_place(rocm, steps):
+    c, x = case(29, "float32", steps, 2, 1, 20, 16, resets=0.02)
+    want = run(rocm, c, x)
+    b = Buffers(rocm, c, x)
+    call, layer = rocm.device.lib, C.byref(b.layer)
+    h = rocm.device.handle
+    tail = list(b.tail(0))
+    tail[3] = None      # no checkpoints
+    assert call.rlt_rocm_selective_scan_forward(h, layer, *b.inputs(), b.o["output"].view, b.state.ptr, None, *tail) == 0
+    assert np.array_equal(b.o["output"].numpy(), want["output"])
+    assert call.rlt_rocm_selective_scan_forward(h, layer, *b.inputs(), b.o["output"].view, b.state.ptr, b.state.ptr, *b.tail(0)) == 0
+    assert np.array_equal(b.o["output"].numpy(), want["output"]) and np.array_equal(b.state.numpy().astype(np.float64), want["state"])
+    outs = [b.o[n].view for n in ("d_x", "d_delta", "d_b", "d_c", "d_gate")]
+    assert call.rlt_rocm_selective_scan_backward(h, layer, *b.inputs(), b.t["d_output"].view, *outs, b.d_state.ptr, b.d_state.ptr, 0, *b.tail(1)) == 0
+    assert np.array_equal(b.d_state.numpy().astype(np.float64), want["d_state"])
+    for n in ("d_x", "d_delta", "d_b", "d_c", "d_gate"):
+        assert np.array_equal(b.o[n].numpy(), want[n]), n
+    bare = layer_of(rocm, c, x, {}, gradients=False)
+    bare.log_rates, bare.skip, bare.delta_biases = b.layer.log_rates, b.layer.skip, b.layer.delta_biases
+    d_state = rocm.array(x["d_state"])
+    assert call.rlt_rocm_selective_scan_backward(h, C.byref(bare), *b.inputs(), b.t["d_output"].view, *outs, d_state.ptr, None, 0, *b.tail(1)) == 0
+    rocm.sync()
+    for n in ("d_x", "d_delta", "d_b", "d_c", "d_gate"):
+        assert np.array_equal(b.o[n].numpy(), want[n]), n
+
+
+# ------------------------------------------------------------------ single steps
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("rows,heads,channels,states", [(1, 1, 1, 1), (64, 1, 64, 16), (3, 2, 24, 11), (5, 1, 33, 32), (7, 3, 5, 7), (300, 1, 16, 16), (2, 1, 64, 4), (2, 2, 9, 8)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_steps_walk_a_sequence(rocm, rows, heads, channels, states, dtype, in_place):
+    print("case", rows, heads, channels, states, dtype, in_place, flush=True)
+    c, x = case(rows + states, dtype, 5, rows, heads, channels, states, resets=0.3)
+    x["reset"][0, 0] = 1
+    clean = {n: a.copy() for n, a in x.items()}
+    x["state"][0] = np.nan
+    want = reference(c, clean)
+    b, buffers = bounds(c, clean, want), Buffers(rocm, c, x)
+    state, other, item = buffers.state, filled(rocm, x["state"].shape, "float32"), 4 if dtype == "float32" else 2
+    for t in range(5):
+        at = lambda a: view(a.array, strides_of(a.padded, a.order), item, t * int(np.prod(a.padded[1:])))
+        to = state if in_place else other
+        rocm.call("selective_scan_step", C.byref(buffers.layer), *[at(buffers.t[n]) for n in SEQUENCES[:5]], at(buffers.o["output"]), state.ptr, to.ptr, buffers.reset.ptr + t * rows)
+        if not in_place:
+            state, other = other, state
+    rocm.sync()
+    assert np.all(np.abs(buffers.o["output"].numpy() - want["output"]) <= b["output"]) and np.all(np.abs(state.numpy() - want["state"]) <= b["state"])
+
+
+# ------------------------------------------------------------------ graphs, refusals
+
+
+@gpu
+@pytest.mark.parametrize("steps", [100, 700])
+def test_a_graph_replays_forward_and_backward(rocm, steps):
+    lib, h = rocm.device.lib, rocm.device.handle
+    c, x = case(31, "bfloat16", steps, 2, 1, 80, 16, resets=0.02, ragged=True)
+    want = run(rocm, c, x)
+    b = Buffers(rocm, c, x)
+    rocm.sync()
+    assert lib.rlt_rocm_graph_begin_capture(h) == 0
+    b.forward()
+    b.backward()
+    graph = C.c_void_p()
+    assert lib.rlt_rocm_graph_end_capture(h, C.byref(graph)) == 0
+    for _ in range(3):
+        for a in b.o.values():
+            a.array.upload(to_bits(np.full(a.array.shape, 7.0, np.float32)))      # eager work between the replays
+        assert lib.rlt_rocm_graph_launch(h, graph) == 0
+        rocm.sync()
+        for name, a in b.results().items():
+            assert np.array_equal(a, want[name]), name
+    lib.rlt_rocm_graph_destroy(h, graph)
+
+
+def changed(layer, **fields):
+    return C.byref(capi.SelectiveScan(**dict({n: getattr(layer, n) for n, _ in layer._fields_}, **fields)))
+
+
+def test_refusals_without_a_device():
+    lib = package().load_library()
+    good = capi.SelectiveScan(4096, None, None, None, None, None, 0, 2, 1, 100, 16, 0)
+    for size in (lambda layer, steps: lib.rlt_rocm_selective_scan_workspace_bytes(layer, steps, 1), lib.rlt_rocm_selective_scan_checkpoint_bytes):
+        assert size(C.byref(good), 40) > 0
+        for layer in (None, changed(good, states=33), changed(good, states=0), changed(good, channels=0), changed(good, type=2), changed(good, batch=2 ** 20, channels=2 ** 10), changed(good, batch=2 ** 30, heads=2 ** 30)):
+            assert size(layer, 40) == 0
+        assert size(C.byref(good), 0) == size(C.byref(good), 2 ** 30 + 1) == size(changed(good, batch=64), 2 ** 26) == 0
+    assert lib.rlt_rocm_selective_scan_forward(None, C.byref(good), *[None] * 6, None, None, None, None, 4, None, None, 0) == capi.RLT_E_NOT_INITIALISED
+
+
+@gpu
+def test_refusals(rocm):
+    lib, h = rocm.device.lib, rocm.device.handle
+    c, x = case(37, "float32", 4, 2, 1, 70, 16)
+    b = Buffers(rocm, c, x)
+    none, good = C.byref(capi.HeadView(None, 1, 1, 1)), C.byref(b.layer)
+    inputs, outs = b.inputs(), [b.o[n].view for n in ("d_x", "d_delta", "d_b", "d_c", "d_gate")]
+
+    def forward(layer=good, views=inputs + [b.o["output"].view], steps=4, checkpoints=b.checkpoints.ptr):
+        return lib.rlt_rocm_selective_scan_forward(h, layer, *views, None, None, None, None, steps, checkpoints, b.scratch[0].ptr, b.sizes[0])
+
+    def backward(layer=good, views=inputs + [b.t["d_output"].view] + outs, steps=4, checkpoints=b.checkpoints.ptr, ptr=b.scratch[1].ptr, size=b.sizes[1]):
+        return lib.rlt_rocm_selective_scan_backward(h, layer, *views, None, None, 0, None, None, steps, checkpoints, ptr, size)
+
+    def step(layer=good, views=inputs + [b.o["output"].view], state=b.state.ptr, to=b.state.ptr):
+        return lib.rlt_rocm_selective_scan_step(h, layer, *views, state, to, None)
+    assert forward() == backward() == step() == 0
+    for call, n in ((forward, 6), (backward, 11), (step, 6)):
+        for layer in (None, changed(b.layer, type=2), changed(b.layer, batch=0), changed(b.layer, heads=0), changed(b.layer, channels=-1), changed(b.layer, states=0), changed(b.layer, log_rates=None)):
+            assert call(layer) == capi.RLT_E_INVALID_ARGUMENT
+        assert call(changed(b.layer, states=33)) == call(changed(b.layer, batch=2 ** 20, channels=2 ** 10)) == capi.RLT_E_UNSUPPORTED
+        views = inputs + ([b.t["d_output"].view] + outs if n == 11 else [b.o["output"].view])
+        for i in range(n):
+            assert call(views=views[:i] + [none] + views[i + 1:]) == capi.RLT_E_INVALID_ARGUMENT
+            if i != 4:      # (no gate is no error)
+                assert call(views=views[:i] + [None] + views[i + 1:]) == capi.RLT_E_INVALID_ARGUMENT
+    for call in (forward, backward):
+        assert call(steps=0) == call(checkpoints=b.checkpoints.ptr + 4) == capi.RLT_E_INVALID_ARGUMENT
+        assert call(steps=2 ** 30 + 1) == capi.RLT_E_UNSUPPORTED
+    assert backward(checkpoints=None) == backward(ptr=None) == backward(size=b.sizes[1] - 1) == backward(ptr=b.scratch[1].ptr + 8) == capi.RLT_E_INVALID_ARGUMENT
+    assert step(state=None) == step(to=None) == capi.RLT_E_INVALID_ARGUMENT
+    long = case(38, "float32", 700, 1, 1, 16, 16)
+    b2 = Buffers(rocm, *long)
+    assert b2.sizes[0] > 0      # cut into segments: a forward call without its scratch memory is refused
+    assert lib.rlt_rocm_selective_scan_forward(h, C.byref(b2.layer), *b2.inputs(), b2.o["output"].view, None, None, None, None, 700, None, None, 0) == capi.RLT_E_INVALID_ARGUMENT
+    rocm.sync()
