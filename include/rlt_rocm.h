@@ -1352,6 +1352,31 @@ int rlt_rocm_selective_scan_backward(rlt_rocm_device* device, const rlt_selectiv
 int rlt_rocm_selective_scan_step(rlt_rocm_device* device, const rlt_selective_scan* layer, const rlt_head_view* x, const rlt_head_view* delta, const rlt_head_view* b, const rlt_head_view* c,
                                  const rlt_head_view* gate, const rlt_head_view* output, const float* state, float* next_state, const uint8_t* reset);
 
+/* A matrix that muon_step updates, row-major without gaps. next_parameters and next_momentum may be parameters and momentum themselves; otherwise no two buffers of a call overlap. */
+typedef struct rlt_muon_tensor {
+    const float* parameters; const float* gradient; const float* momentum;
+    float* next_parameters; float* next_momentum;
+    int32_t rows, cols;
+} rlt_muon_tensor;
+
+typedef struct rlt_muon_parameters {
+    float alpha;                 /* the step's size */
+    float momentum;
+    float weight_decay;
+    float epsilon;               /* >= 0, added to the update's norm */
+    int32_t nesterov;
+    int32_t iterations;          /* 1 ... 32; five bring singular values from 0.002 on to between 0.7 and 1.2 */
+} rlt_muon_parameters;
+
+/* One step of an optimiser for matrices, which makes the singular values of their updates alike, next to rlt_rocm_adam_step for vectors, of `n` matrices (`tensors` is a HOST array), fp32:
+ *     next_momentum = momentum_factor * momentum + gradient,   u = nesterov ? gradient + momentum_factor * next_momentum : next_momentum,   X = u / (|u| + epsilon) (Frobenius norm, in 64 bits),
+ *     `iterations` times   A = X X^T,   X = a X + (b A + c A A) X   with (a, b, c) = (3.4445, -4.775, 2.0315),
+ *     next_parameters = (1 - alpha * weight_decay) * parameters - alpha * sqrt(max(1, rows / cols)) * X.
+ * Up to 2^16 rows and columns and 2^30 elements to a matrix; anything beyond is RLT_E_UNSUPPORTED before anything is launched. The workspace starts on a 16-byte boundary and belongs to one call at a time;
+ * its size (0 for a call that is refused) depends on the shapes alone. */
+size_t rlt_rocm_muon_workspace_bytes(const rlt_muon_tensor* tensors, int n);
+int rlt_rocm_muon_step(rlt_rocm_device* device, const rlt_muon_tensor* tensors, int n, const rlt_muon_parameters* parameters, void* workspace, size_t workspace_bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -15,7 +15,7 @@ OBJ = os.path.join(HERE, "build")
 OUT = os.path.join(HERE, "librlt_rocm.so")
 SOURCES = ["device.hip", "tensor_ops.hip", "gemm.hip", "mlp.hip", "mlp_fused.hip", "mlp_small.hip", "mlp_rows.hip", "mlp_row.hip", "optim.hip", "sac.hip", "sac_fused.hip", "sac_update.hip", "sac_wide.hip", "batch_gradient.hip", "runner.hip",
            "ppo.hip", "pad.hip", "gru.hip", "td3.hip", "normalize.hip", "envs.hip", "seq.hip", "seq_stack.hip", "linear_attention.hip", "residual_norm.hip", "dropout.hip", "causal_convolution.hip",
-           "selective_scan.hip"]
+           "selective_scan.hip", "muon.hip"]
 FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fno-gpu-rdc",
     # keep the compiler from forming packed-fp32 VALU instructions

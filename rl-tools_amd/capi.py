@@ -274,6 +274,14 @@ class SelectiveScan(C.Structure):
                 ("type", C.c_int32), ("batch", C.c_int32), ("heads", C.c_int32), ("channels", C.c_int32), ("states", C.c_int32), ("reserved", C.c_int32)]
 
 
+class MuonTensor(C.Structure):
+    _fields_ = [("parameters", C.c_void_p), ("gradient", C.c_void_p), ("momentum", C.c_void_p), ("next_parameters", C.c_void_p), ("next_momentum", C.c_void_p), ("rows", C.c_int32), ("cols", C.c_int32)]
+
+
+class MuonParameters(C.Structure):
+    _fields_ = [("alpha", C.c_float), ("momentum", C.c_float), ("weight_decay", C.c_float), ("epsilon", C.c_float), ("nesterov", C.c_int32), ("iterations", C.c_int32)]
+
+
 I, F, P, S, U64 = C.c_int, C.c_float, C.c_void_p, C.c_size_t, C.c_uint64
 LP = C.POINTER(DenseLayer)
 # return codes of the C ABI (include/rlt_rocm.h)
@@ -422,6 +430,8 @@ ROCM_ONLY = {
     "selective_scan_forward": ([P, C.POINTER(SelectiveScan)] + [C.POINTER(HeadView)] * 6 + [P, P, P, P, I, P, P, S], I),
     "selective_scan_backward": ([P, C.POINTER(SelectiveScan)] + [C.POINTER(HeadView)] * 11 + [P, P, I, P, P, I, P, P, S], I),
     "selective_scan_step": ([P, C.POINTER(SelectiveScan)] + [C.POINTER(HeadView)] * 6 + [P, P, P], I),
+    "muon_workspace_bytes": ([C.POINTER(MuonTensor), I], S),
+    "muon_step": ([P, C.POINTER(MuonTensor), I, C.POINTER(MuonParameters), P, S], I),
     "residual_norm_forward": ([P, C.POINTER(ResidualNorm), P, I, P, I, P, I, P, I, P, I, I], I),
     "residual_norm_workspace_bytes": ([C.POINTER(ResidualNorm), I], S),
     "residual_norm_backward": ([P, C.POINTER(ResidualNorm), P, I, P, I, P, I, P, I, P, I, P, I, P, I, P, I, I, I, P, S], I),
