@@ -889,3 +889,169 @@ class SequenceBlocks:
             call("residual_norm_forward", C.byref(self.norm[l]), x.ptr, w, self.step_p.ptr, w, self.step_projected.offset(self.gate_at), self.row, self.step_y.ptr, w, self.step_h.ptr, w, n)
             x = self.step_y
         return self.step_h
+
+
+class SelectiveBlocks:
+    """A stack of selective blocks over sequences [steps x batch x width], fp32, beside SequenceBlocks, whose interface it has. Per block l, with inner = heads x channels
+        x, gate = W_in h + b_in (one product),   x = silu(causal convolution(x)),   low, b, c = W_x x + b_x (one product),   raw = W_dt low + b_dt,
+        o = selective scan(x, raw, b, c, gate),   p = dropout(W_out o + b_out),   y = residual stream + residual_scale * branch_norm(p),   the next block's h = output_norm(y);   h of the first block: input_norm(x).
+    Sequences train it (forward, backward, update); step() is one step of a rollout with the blocks' states (`windows` of the convolutions, `states` of the scans), which training leaves alone, and gives what forward gives
+    without dropout. Every device address is fixed when the object is built, so that forward + backward + update can be captured into a graph."""
+
+    MATRICES = ("in_w", "x_w", "dt_w", "out_w")      # what update() orthogonalises where it is asked to
+
+    @staticmethod
+    def shapes(width, inner, heads, states, rank, taps, blocks):
+        """name -> shape, in the order of the flat arenas"""
+        s = {"input_weights": (width,), "input_biases": (width,)}
+        for l in range(blocks):
+            s.update({f"in_w{l}": (2 * inner, width), f"in_b{l}": (2 * inner,), f"taps{l}": (inner, taps), f"tap_b{l}": (inner,), f"x_w{l}": (rank + 2 * heads * states, inner), f"x_b{l}": (rank + 2 * heads * states,),
+                      f"dt_w{l}": (inner, rank), f"dt_b{l}": (inner,), f"log_rates{l}": (inner, states), f"skip{l}": (inner,), f"out_w{l}": (width, inner), f"out_b{l}": (width,),
+                      f"branch_weights{l}": (width,), f"branch_biases{l}": (width,), f"output_weights{l}": (width,), f"output_biases{l}": (width,), f"residual_scale{l}": (width,)})
+        return s
+
+    @staticmethod
+    def random(rng, width, inner, heads, states, rank, taps, blocks):
+        """parameters of a new stack: rates 1 ... states, step sizes from 1e-3 to 1e-1"""
+        p = {}
+        for name, shape in SelectiveBlocks.shapes(width, inner, heads, states, rank, taps, blocks).items():
+            if name.startswith("log_rates"):
+                a = np.tile(np.log(np.arange(1, states + 1)), (inner, 1))
+            elif name.startswith("dt_b"):
+                a = np.log(np.expm1(np.exp(rng.uniform(np.log(1e-3), np.log(1e-1), shape))))
+            elif len(shape) == 2:
+                a = rng.uniform(-1, 1, shape) / np.sqrt(shape[1])
+            else:
+                a = np.ones(shape) if "weights" in name or "scale" in name or name.startswith("skip") else np.zeros(shape)
+            p[name] = a.astype(np.float32)
+        return p
+
+    def __init__(self, backend, params, steps, batch, width, inner, heads, states, rank, taps, blocks, dropout=0.0, seed=0, norm="rms", epsilon=1e-5):
+        assert inner % heads == 0
+        self.backend, self.steps, self.batch, self.width, self.inner, self.blocks, self.rate, self.seed = backend, steps, batch, width, inner, blocks, dropout, seed
+        channels, rows, z = inner // heads, steps * batch, backend.zeros
+        self.rank, self.b_at, self.c_at, self.row = rank, rank, rank + heads * states, rank + 2 * heads * states      # parts of a row of the product behind the convolution
+        shapes = self.shapes(width, inner, heads, states, rank, taps, blocks)
+        self.offsets, total = {}, 0
+        for name, shape in shapes.items():
+            self.offsets[name] = total
+            total += (int(np.prod(shape)) + 3) // 4 * 4      # 16-byte boundaries
+        flat = np.zeros(total, np.float32)
+        for name, shape in shapes.items():
+            flat[self.offsets[name]:self.offsets[name] + int(np.prod(shape))] = np.asarray(params[name], np.float32).reshape(shape).ravel()
+        self.params, self.total = backend.array(flat), total
+        self.grads, self.m, self.v, self.age = z((total,)), z((total,)), z((total,)), backend.array(np.array([1], np.uint32))
+        self.grad_views = {name: ArenaView(self.grads, self.offsets[name], shape) for name, shape in shapes.items()}
+        self.param_views = {name: ArenaView(self.params, self.offsets[name], shape) for name, shape in shapes.items()}
+        P, G = (lambda name: self.params.offset(self.offsets[name])), (lambda name: self.grads.offset(self.offsets[name]))
+        matrix = lambda n: n.rstrip("0123456789") in self.MATRICES
+        adam = [capi.AdamTensor(P(n), G(n), self.m.offset(o), self.v.offset(o), None, int(np.prod(shapes[n])), 1 if matrix(n) else 2) for n, o in sorted(self.offsets.items(), key=lambda e: matrix(e[0]))]
+        self.adam, self.n_adam, self.n_vectors = (capi.AdamTensor * len(adam))(*adam), len(adam), sum(not matrix(n) for n in shapes)      # the matrices last
+        matrices = [capi.MuonTensor(P(n), G(n), self.m.offset(self.offsets[n]), P(n), self.m.offset(self.offsets[n]), *shapes[n]) for n in shapes if matrix(n)]
+        self.matrices, self.n_matrices = (capi.MuonTensor * len(matrices))(*matrices), len(matrices)
+
+        self.x, self.reset, self.passed = z((steps, batch, width)), z((steps, batch), np.uint8), (0, True, True)
+        each = lambda shape: [z(shape) for _ in range(blocks)]
+        self.h, self.y, self.p = [z((rows, width)) for _ in range(blocks + 1)], each((rows, width)), each((rows, width))
+        self.projected, self.conv, self.parts, self.raw, self.o = each((rows, 2 * inner)), each((rows, inner)), each((rows, self.row)), each((rows, inner)), each((rows, inner))
+        self.d_h, self.d_stream, self.d_p = z((rows, width)), z((rows, width)), z((rows, width))
+        self.d_projected, self.d_conv, self.d_conv_parts, self.d_parts, self.d_raw, self.d_o = z((rows, 2 * inner)), z((rows, inner)), z((rows, inner)), z((rows, self.row)), z((rows, inner)), z((rows, inner))
+        self.windows, self.states = each((batch, taps - 1, inner)), each((batch, heads, channels, states))
+        self.step_x, self.step_reset = z((batch, width)), z((batch,), np.uint8)
+        self.step_h, self.step_projected, self.step_conv, self.step_parts, self.step_raw, self.step_o, self.step_p, self.step_y = (z((batch, n)) for n in (width, 2 * inner, inner, self.row, inner, inner, width, width))
+
+        norm = capi.NORM[norm]
+        self.input_norm = capi.ResidualNorm(0, width, norm, norm, 0, epsilon, None, None, P("input_weights"), P("input_biases"), None, None, None, G("input_weights"), G("input_biases"), None)
+        self.in_layer, self.x_layer, self.dt_layer, self.out_layer, self.convolution, self.scan, self.norm = [], [], [], [], [], [], []
+        for l in range(blocks):
+            n = lambda name: f"{name}{l}"
+            dense = lambda name, out, i, o: capi.DenseLayer(P(n(name + "_w")), P(n(name + "_b")), G(n(name + "_w")), G(n(name + "_b")), out.ptr, None, i, o, capi.ACT["identity"], 0)
+            self.in_layer.append(dense("in", self.projected[l], width, 2 * inner))
+            self.x_layer.append(dense("x", self.parts[l], inner, self.row))
+            self.dt_layer.append(dense("dt", self.raw[l], rank, inner))
+            self.out_layer.append(dense("out", self.p[l], inner, width))
+            self.convolution.append(capi.CausalConvolution(P(n("taps")), P(n("tap_b")), G(n("taps")), G(n("tap_b")), 0, batch, inner, taps, 1, 0))
+            self.scan.append(capi.SelectiveScan(P(n("log_rates")), P(n("skip")), None, G(n("log_rates")), G(n("skip")), None, 0, batch, heads, channels, states, 0))
+            self.norm.append(capi.ResidualNorm(0, width, norm, norm, 0, epsilon, *[P(n(a)) for a in ("branch_weights", "branch_biases", "output_weights", "output_biases", "residual_scale")],
+                                               *[G(n(a)) for a in ("branch_weights", "branch_biases", "output_weights", "output_biases", "residual_scale")]))
+        view = lambda a, at, row, head, step=None: capi.HeadView(a.offset(at), batch * row if step is None else step, row, head)
+        scan_views = lambda conv, raw, parts, projected, step=None: [view(conv, 0, inner, channels, step), view(raw, 0, inner, channels, step), view(parts, self.b_at, self.row, states, step),
+                                                                     view(parts, self.c_at, self.row, states, step), view(projected, inner, 2 * inner, channels, step)]
+        self.scan_views = [scan_views(*a) for a in zip(self.conv, self.raw, self.parts, self.projected)]
+        self.d_scan_views = scan_views(self.d_conv, self.d_raw, self.d_parts, self.d_projected)
+        self.o_views, self.d_o_view = [view(a, 0, inner, channels) for a in self.o], view(self.d_o, 0, inner, channels)
+        self.conv_views = [(view(p, 0, 2 * inner, 0), view(a, 0, inner, 0)) for p, a in zip(self.projected, self.conv)]
+        self.d_conv_views = view(self.d_conv, 0, inner, 0), view(self.d_projected, 0, 2 * inner, 0)
+        self.step_scan_views, self.step_o_view = scan_views(self.step_conv, self.step_raw, self.step_parts, self.step_projected, 0), view(self.step_o, 0, inner, channels, 0)
+        self.step_conv_views = view(self.step_projected, 0, 2 * inner, 0, 0), view(self.step_conv, 0, inner, 0, 0)
+        lib, ref = backend.device.lib, C.byref
+        nbytes = max([lib.rlt_rocm_selective_scan_workspace_bytes(ref(a), steps, k) for a in self.scan for k in (0, 1)] + [lib.rlt_rocm_causal_convolution_workspace_bytes(ref(a), steps) for a in self.convolution]
+                     + [lib.rlt_rocm_residual_norm_workspace_bytes(ref(a), rows) for a in self.norm] + [lib.rlt_rocm_muon_workspace_bytes(self.matrices, self.n_matrices)])
+        scratch = lambda n: backend.device.empty((max(int(n), 16),), np.uint8)
+        self._workspace, self.checkpoints = scratch(nbytes), [scratch(lib.rlt_rocm_selective_scan_checkpoint_bytes(ref(a), steps)) for a in self.scan]
+        self.workspace = (self._workspace.ptr, int(nbytes))
+
+    zero_gradient, _dropout = SequenceBlocks.zero_gradient, SequenceBlocks._dropout
+
+    def forward(self, stream=0, reset=True, dropout=True, keep_states=None):
+        """x -> h[-1], over all steps from states of zeros; arguments as SequenceBlocks.forward has them"""
+        b, w, rows, call = self.backend, self.width, self.steps * self.batch, self.backend.call
+        self.passed = stream, reset, dropout
+        keep_states = not dropout if keep_states is None else keep_states
+        r = self.reset.ptr if reset else None
+        x = self.x
+        call("residual_norm_forward", C.byref(self.input_norm), x.ptr, w, None, 0, None, 0, None, 0, self.h[0].ptr, w, rows)
+        for l in range(self.blocks):
+            call("dense_forward", C.byref(self.in_layer[l]), self.h[l].ptr, w, None, 0, rows)
+            call("causal_convolution_forward", C.byref(self.convolution[l]), *self.conv_views[l], None, self.windows[l].ptr if keep_states else None, r, None, self.steps)
+            call("dense_forward", C.byref(self.x_layer[l]), self.conv[l].ptr, self.inner, None, 0, rows)
+            call("dense_forward", C.byref(self.dt_layer[l]), self.parts[l].ptr, self.row, None, 0, rows)
+            call("selective_scan_forward", C.byref(self.scan[l]), *self.scan_views[l], self.o_views[l], None, self.states[l].ptr if keep_states else None, r, None, self.steps, self.checkpoints[l].ptr, *self.workspace)
+            call("dense_forward", C.byref(self.out_layer[l]), self.o[l].ptr, self.inner, None, 0, rows)
+            if dropout:
+                self._dropout(self.p[l], stream + l)
+            call("residual_norm_forward", C.byref(self.norm[l]), x.ptr, w, self.p[l].ptr, w, None, 0, self.y[l].ptr, w, self.h[l + 1].ptr, w, rows)
+            x = self.y[l]
+        return self.h[-1]
+
+    def backward(self, d_output, stream=None, reset=None, dropout=None):
+        """From the gradient with respect to h[-1] of the last forward call to those of the parameters (added to `grads`) and of x (d_stream); arguments as SequenceBlocks.backward has them"""
+        w, n, rows, call = self.width, self.inner, self.steps * self.batch, self.backend.call
+        stream, reset, dropout = (last if given is None else given for given, last in zip((stream, reset, dropout), self.passed))
+        r = self.reset.ptr if reset else None
+        d_h, d_y = d_output, None
+        for l in reversed(range(self.blocks)):
+            call("residual_norm_backward", C.byref(self.norm[l]), self.p[l].ptr, w, None, 0, self.y[l].ptr, w, d_y.ptr if d_y else None, w, d_h.ptr, w, self.d_stream.ptr, w, self.d_p.ptr, w, None, 0, rows, 1, *self.workspace)
+            if dropout:
+                self._dropout(self.d_p, stream + l)
+            call("dense_backward_full", C.byref(self.out_layer[l]), self.o[l].ptr, n, self.d_p.ptr, w, self.d_o.ptr, n, rows)
+            call("selective_scan_backward", C.byref(self.scan[l]), *self.scan_views[l], self.d_o_view, *self.d_scan_views, None, None, 1, r, None, self.steps, self.checkpoints[l].ptr, *self.workspace)
+            call("dense_backward_full", C.byref(self.dt_layer[l]), self.parts[l].ptr, self.row, self.d_raw.ptr, n, self.d_parts.ptr, self.row, rows)
+            call("dense_backward_full", C.byref(self.x_layer[l]), self.conv[l].ptr, n, self.d_parts.ptr, self.row, self.d_conv_parts.ptr, n, rows)
+            call("binary_f32", capi.BINARY["add"], self.d_conv.ptr, n, self.d_conv_parts.ptr, n, self.d_conv.ptr, n, rows, n)
+            call("causal_convolution_backward", C.byref(self.convolution[l]), self.conv_views[l][0], *self.d_conv_views, None, None, None, 1, r, None, self.steps, *self.workspace)
+            call("dense_backward_full", C.byref(self.in_layer[l]), self.h[l].ptr, w, self.d_projected.ptr, 2 * n, self.d_h.ptr, w, rows)
+            d_h, d_y = self.d_h, self.d_stream
+        call("residual_norm_backward", C.byref(self.input_norm), None, 0, None, 0, self.x.ptr, w, d_y.ptr if d_y else None, w, d_h.ptr, w, self.d_stream.ptr, w, None, 0, None, 0, rows, 1, *self.workspace)
+
+    def update(self, adam, muon=None):
+        """One step of Adam; with `muon` (capi.MuonParameters) of Adam for the vectors and of that for the matrices, whose first moments are its momenta."""
+        self.backend.call("adam_step", self.adam, self.n_adam if muon is None else self.n_vectors, C.byref(adam), self.age.ptr, 0.0, None)
+        if muon is not None:
+            self.backend.call("muon_step", self.matrices, self.n_matrices, C.byref(muon), *self.workspace)
+
+    def step(self):
+        """One step of every row: step_x -> step_h, the blocks' states in place; step_reset drops a row's states before it."""
+        w, n, call = self.width, self.batch, self.backend.call
+        x = self.step_x
+        call("residual_norm_forward", C.byref(self.input_norm), x.ptr, w, None, 0, None, 0, None, 0, self.step_h.ptr, w, n)
+        for l in range(self.blocks):
+            call("dense_evaluate", C.byref(self.in_layer[l]), self.step_h.ptr, w, self.step_projected.ptr, 2 * self.inner, n)
+            call("causal_convolution_step", C.byref(self.convolution[l]), *self.step_conv_views, self.windows[l].ptr, self.windows[l].ptr, self.step_reset.ptr)
+            call("dense_evaluate", C.byref(self.x_layer[l]), self.step_conv.ptr, self.inner, self.step_parts.ptr, self.row, n)
+            call("dense_evaluate", C.byref(self.dt_layer[l]), self.step_parts.ptr, self.row, self.step_raw.ptr, self.inner, n)
+            call("selective_scan_step", C.byref(self.scan[l]), *self.step_scan_views, self.step_o_view, self.states[l].ptr, self.states[l].ptr, self.step_reset.ptr)
+            call("dense_evaluate", C.byref(self.out_layer[l]), self.step_o.ptr, self.inner, self.step_p.ptr, w, n)
+            call("residual_norm_forward", C.byref(self.norm[l]), x.ptr, w, self.step_p.ptr, w, None, 0, self.step_y.ptr, w, self.step_h.ptr, w, n)
+            x = self.step_y
+        return self.step_h
