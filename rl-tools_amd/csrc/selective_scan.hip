@@ -5,7 +5,9 @@
 namespace {
 
 constexpr int MAX_STEPS = 1 << 30, MAX_STATES = 32;
+constexpr int64_t MAX_STRIDE = 1 << 27;      // elements between steps: three of them and a row of channels are an offset of 32 bits
 constexpr int WAVES = 4, LANES = 64 * WAVES, TILE = 16 * WAVES;      // channels of a workgroup: four lanes share one, each with a quarter of its states
+constexpr float NO_DELTA = -__builtin_huge_valf();      // what a delta of nothing comes of: a step that is not there leaves the state as it is
 constexpr float LOG2_E = 1.44269504088896341f, LN_2 = 0.69314718055994531f;
 
 // steps that a lane looks at together, and behind which the forward pass leaves the states for the backward pass; NPT states to a lane
@@ -19,7 +21,7 @@ struct Scan {
     const float* entry; float* exit;         // states (backward: their gradients) before the first step walked and behind the last: [pairs][channels][states], or where there are segments [pairs][segments][channels][4 NPT]
     float* sums;                  // of delta over a segment, [pairs][segments][channels]; below zero: the segment holds a reset, nothing passes it
     float* checkpoints;           // [pairs][chunks][channels][4 NPT]: states before each chunk
-    float* d_shared;              // d_b, then d_c: [tiles][steps x batch x heads][4 NPT]
+    float* d_shared;              // d_b, then d_c: [tiles][pairs][steps][4 NPT]
     float* d_rates; float* d_skips; float* d_biases;      // [row groups x segments][heads][channels][4 NPT] and [...][channels]
     const uint8_t* reset; const int32_t* lengths;
     int batch, heads, channels, states, steps, segments, segment_steps, tiles, chunks, row_groups;
@@ -27,6 +29,20 @@ struct Scan {
 };
 
 template <typename T> __device__ __forceinline__ T* at(const rlt_part& p, int step, int row, int head) { return (T*)p.data + (int64_t)step * p.step + (int64_t)row * p.row + (int64_t)head * p.head; }
+
+// The parts of a launch's arguments as they are needed, from where the launch left them: strides that a kernel needs once a row would otherwise hold scalar registers, of which there are too few, from its start to its end.
+struct Arguments {
+    const __attribute__((address_space(4))) char* at;
+    __device__ __forceinline__ Arguments() {
+        at = (const __attribute__((address_space(4))) char*)__builtin_amdgcn_kernarg_segment_ptr();
+        asm volatile("" : "+s"(at));
+    }
+    __device__ __forceinline__ rlt_part part(size_t offset) const {
+        const auto* const v = (const __attribute__((address_space(4))) int64_t*)(at + offset);
+        return {(void*)v[0], v[1], v[2], v[3]};
+    }
+};
+#define SCAN_PART(arguments, name) (arguments).part(offsetof(Scan, name))
 
 // ---- exchanges between the four lanes of a channel
 template <int CTRL> __device__ __forceinline__ float lanes(float v) { return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true)); }
@@ -40,7 +56,10 @@ __device__ __forceinline__ float sum_of_lanes(float v) {
     v += lanes<0xB1>(v);
     return v + lanes<0x4E>(v);
 }
-typedef unsigned rlt_u32x2 __attribute__((ext_vector_type(2)));
+// v in the lanes of quad J of each row of sixteen, `old` in the others
+template <int J> __device__ __forceinline__ float into_quad(float old, float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, old), __builtin_bit_cast(int, v), 0xE4, 0xF, 1 << J, false));
+}
 __device__ __forceinline__ float add_halves(float a, float b) {      // lanes 0 to 31: a's sum over both halves of the wavefront, the others: b's
     const auto s = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b), false, false);
     return __builtin_bit_cast(float, (unsigned)s[0]) + __builtin_bit_cast(float, (unsigned)s[1]);
@@ -93,6 +112,10 @@ __device__ __forceinline__ void set_row(const Scan& a, Place& p, int row) {
     p.live = min(p.end, p.length);
 }
 __device__ __forceinline__ int pair_of(const Scan& a, const Place& p) { return p.row * a.heads + p.head; }
+__device__ __forceinline__ bool bit(unsigned mask, int i) {
+    asm volatile("" : "+s"(mask));      // looked at where it is needed: sixteen answers held from a walk forward to the one back are 32 scalar registers
+    return mask >> i & 1;
+}
 // bit s: step t + s forgets its state
 template <int K> __device__ __forceinline__ unsigned resets_of(const Scan& a, const Place& p, int t) {
     if (!a.reset) return 0;
@@ -130,6 +153,15 @@ template <int NPT> __device__ __forceinline__ void read(const float* from, float
         for (int j = 0; j < (NPT < 4 ? NPT : 4); j++) to[i + j] = v[j];
     }
 }
+template <int NPT> __device__ __forceinline__ void read_global(const __attribute__((address_space(1))) char* from, float (&to)[NPT]) {
+    typedef float vector __attribute__((ext_vector_type(NPT < 4 ? NPT : 4)));
+#pragma unroll
+    for (int i = 0; i < NPT; i += NPT < 4 ? NPT : 4) {
+        const vector v = *(const __attribute__((address_space(1))) vector*)(from + i * sizeof(float));
+#pragma unroll
+        for (int j = 0; j < (NPT < 4 ? NPT : 4); j++) to[i + j] = v[j];
+    }
+}
 template <int NPT> __device__ __forceinline__ void write(float* to, const float (&from)[NPT]) {
     typedef float vector __attribute__((ext_vector_type(NPT < 4 ? NPT : 4)));
 #pragma unroll
@@ -140,12 +172,33 @@ template <int NPT> __device__ __forceinline__ void write(float* to, const float 
         *reinterpret_cast<vector*>(to + i) = v;
     }
 }
-// a lane's elements of its channel in the chunk's steps 4 i + (lane & 3)
-template <typename T, int OWN> __device__ __forceinline__ void ask(const Scan& a, const rlt_part& part, const Place& p, int channel, int t, T (&v)[OWN]) {
-    const int nq = threadIdx.x & 3;
+// A tensor of channels as a wavefront reads and writes it: lane l has the element of its channel in step t + 4 i + l % 4, at an address that all lanes share and an offset of its own, of 32 bits (MAX_STRIDE).
+#define GLOBAL __attribute__((address_space(1)))
+template <typename T> struct Lanes {
+    GLOBAL char* base; int stride; unsigned offset;      // of step 0; bytes to the next step; a lane's own
+    __device__ __forceinline__ Lanes(const rlt_part& part, const Place& p, int channel) {
+        stride = (int)(part.step * (int64_t)sizeof(T));
+        const int lowest = stride < 0 ? 3 * stride : 0;      // steps that go back in memory: from the last of four on
+        base = (GLOBAL char*)part.data + ((int64_t)p.row * part.row + (int64_t)p.head * part.head) * (int64_t)sizeof(T) + lowest;
+        offset = (unsigned)((int)(threadIdx.x & 3) * stride - lowest) + (unsigned)channel * (unsigned)sizeof(T);
+    }
+    // `whole`: all of the steps are there, and all lanes' channels; otherwise what is not there is `nothing`
+    template <int OWN> __device__ __forceinline__ void ask(bool whole, bool there, int t, int live, float nothing, T (&v)[OWN]) const {
+        const GLOBAL char* from = base + (int64_t)t * stride;
+        if (whole) {
 #pragma unroll
-    for (int i = 0; i < OWN; i++) v[i] = at<T>(part, min(t + 4 * i + nq, a.steps - 1), p.row, p.head)[channel];
-}
+            for (int i = 0; i < OWN; i++) { v[i] = *(const GLOBAL T*)(from + offset); from += 4 * (int64_t)stride; }
+        } else {
+#pragma unroll
+            for (int i = 0; i < OWN; i++) {
+                v[i] = (T)nothing;
+                if (there && t + 4 * i + (int)(threadIdx.x & 3) < live) v[i] = *(const GLOBAL T*)(from + offset);
+                from += 4 * (int64_t)stride;
+            }
+        }
+    }
+    __device__ __forceinline__ void put(int t, float v) const { *(GLOBAL T*)(base + (int64_t)t * stride + offset) = (T)v; }      // t: a multiple of four steps into a chunk
+};
 template <int NPT> __device__ __forceinline__ void load_states(const float* from, int n0, int states, float (&h)[NPT]) {
 #pragma unroll
     for (int n = 0; n < NPT; n++) h[n] = from && n0 + n < states ? from[n0 + n] : 0.0f;
@@ -168,7 +221,7 @@ template <typename T, int NPT, bool STATES> __global__ __launch_bounds__(LANES) 
     Place p = place_of(a, blockIdx.x, a.batch);
     set_row(a, p, p.row);
     const int lane = threadIdx.x & 63, nq = lane & 3, n0 = nq * NPT, own_channel = p.tile * TILE + (int)(threadIdx.x >> 2), channel = min(own_channel, a.channels - 1);
-    const bool there = own_channel < a.channels, odd = nq & 1, upper = nq & 2;
+    const bool there = own_channel < a.channels, all_there = (p.tile + 1) * TILE <= a.channels, gated = a.gate.data != nullptr, odd = nq & 1, upper = nq & 2;
     const size_t pair = pair_of(a, p), at_channel = (size_t)p.head * a.channels + channel;
     float rate[NPT], h[NPT];
     load_rates<NPT>(a, p.head, channel, n0, rate);
@@ -181,13 +234,16 @@ template <typename T, int NPT, bool STATES> __global__ __launch_bounds__(LANES) 
     float sum = 0.0f;
     bool forgotten = false;
 
+    const Arguments arguments;
+    const Lanes<T> x_lanes(SCAN_PART(arguments, x), p, channel), delta_lanes(SCAN_PART(arguments, delta), p, channel), gate_lanes(SCAN_PART(arguments, gate), p, channel), out_lanes(SCAN_PART(arguments, out), p, channel);
     T x[OWN], raw[OWN], gate[OWN];
     unsigned resets;
     Shared<T, NPT> next;
     auto ask_chunk = [&](int t) {
-        ask<T, OWN>(a, a.x, p, channel, t, x);
-        ask<T, OWN>(a, a.delta, p, channel, t, raw);
-        if (!STATES && a.gate.data) ask<T, OWN>(a, a.gate, p, channel, t, gate);
+        const bool whole = all_there && t + K <= p.live;
+        x_lanes.ask(whole, there, t, p.live, 0.0f, x);
+        delta_lanes.ask(whole, there, t, p.live, NO_DELTA, raw);
+        if (!STATES && gated) gate_lanes.ask(whole, there, t, p.live, 0.0f, gate);
         next.ask(a, p, t, true);
         resets = resets_of<K>(a, p, t);
     };
@@ -197,12 +253,11 @@ template <typename T, int NPT, bool STATES> __global__ __launch_bounds__(LANES) 
         float xs[OWN], delta[OWN], added[OWN], gates[OWN];
 #pragma unroll
         for (int i = 0; i < OWN; i++) {
-            const bool in = t + 4 * i + nq < p.live;
             float e;
-            xs[i] = in ? (float)x[i] : 0.0f;
-            delta[i] = in ? softplus((float)raw[i] + bias, e) : 0.0f;
+            xs[i] = (float)x[i];
+            delta[i] = softplus((float)raw[i] + bias, e);
             added[i] = delta[i] * xs[i];
-            if (!STATES) gates[i] = a.gate.data ? (float)gate[i] : 0.0f;
+            if (!STATES) gates[i] = gated ? (float)gate[i] : 0.0f;
         }
         const unsigned forget = resets;
         next.put(shared[turn]);
@@ -244,12 +299,12 @@ template <typename T, int NPT, bool STATES> __global__ __launch_bounds__(LANES) 
             for (int i = 0; i < OWN; i++) {
                 const int s = t + 4 * i + nq;
                 float v = fmaf(skip, xs[i], y[i]);
-                if (a.gate.data) {
+                if (gated) {
                     float one, other;
                     rlt_sigmoids(gates[i], one, other);
                     v *= gates[i] * one;
                 }
-                if (there && s < p.end) at<T>(a.out, s, p.row, p.head)[channel] = (T)(s < p.live ? v : 0.0f);
+                if (there && s < p.end) out_lanes.put(t + 4 * i, v);      // (steps beyond the row's length: no input and nothing read, zero)
             }
         }
     }
@@ -263,7 +318,7 @@ template <typename T, int NPT, bool STATES> __global__ __launch_bounds__(LANES) 
         if (a.exit && p.segment == a.segments - 1) store_states<NPT>(a.exit + (pair * a.channels + channel) * a.states, n0, a.states, h);
         // steps behind the last chunk that holds any of the row's
         const int walked = p.live > p.first ? p.first + (p.live - p.first + K - 1) / K * K : p.first;
-        for (int s = walked + nq; s < p.end; s += 4) at<T>(a.out, s, p.row, p.head)[channel] = (T)0.0f;
+        for (int s = walked; s + nq < p.end; s += 4) out_lanes.put(s, 0.0f);
     }
 }
 
@@ -290,14 +345,14 @@ template <bool REVERSE> __global__ __launch_bounds__(256) void join_segments_ker
 // Backward over a segment: from the last chunk to the first, the chunk's states again from its checkpoint, then its steps from the last to the first with the state's gradient G:
 //     G_t = c_t g_t + a_{t+1} G_{t+1},   g = d_output times the gate's factor;   d_c = sum over channels of g h,   d_b = sum over channels of delta x G,
 //     d_x = delta (G . b) + skip g,   d_delta = x (G . b) + rates . q,   d_rates += delta q   with q = G a h_{t-1}.
-template <typename T, int NPT> __global__ __launch_bounds__(LANES, 2) void backward_kernel(Scan a) {
-    constexpr int K = CHUNK<NPT>, OWN = K / 4, N = 4 * NPT, KEPT = NPT > 4 ? NPT / 4 : 1;
+template <typename T, int NPT, bool ONE_TILE> __global__ __launch_bounds__(LANES, 2) void backward_kernel(Scan a) {
+    constexpr int K = CHUNK<NPT>, OWN = K / 4, N = 4 * NPT, KEPT = NPT > 4 ? NPT / 4 : 1, PER = (K * N + LANES - 1) / LANES;
     __shared__ float shared[2][2][K * N];
     __shared__ float slabs[2][WAVES][2][K * N];
     Place p = place_of(a, blockIdx.x, a.row_groups);
     const int group = p.row, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nq = lane & 3, quad = lane >> 2 & 3, n0 = nq * NPT, own_channel = p.tile * TILE + (int)(threadIdx.x >> 2), channel = min(own_channel, a.channels - 1);
     const int kept_state = n0 + (NPT >= 4 ? (lane >> 4 & 1) * (NPT / 4) : 0) + (lane >> 5) * (NPT / 2);      // the first state whose sums over channels this lane is left with
-    const bool there = own_channel < a.channels, odd = nq & 1, upper = nq & 2;
+    const bool there = own_channel < a.channels, all_there = (p.tile + 1) * TILE <= a.channels, odd = nq & 1, upper = nq & 2;
     const size_t at_channel = (size_t)p.head * a.channels + channel;
     float rate[NPT], d_rate[NPT];
     load_rates<NPT>(a, p.head, channel, n0, rate);
@@ -306,7 +361,7 @@ template <typename T, int NPT> __global__ __launch_bounds__(LANES, 2) void backw
     const float bias = a.delta_biases ? a.delta_biases[at_channel] : 0.0f, skip = a.skip ? a.skip[at_channel] : 0.0f;
     float d_skip = 0.0f, d_bias = 0.0f;
     const bool gated = a.gate.data != nullptr;
-    const size_t shared_size = (size_t)a.steps * a.batch * a.heads * N;
+    const unsigned at_checkpoint = (unsigned)(channel * N + n0) * sizeof(float);
     int turn = 0;
     for (int row = group; row < a.batch; row += a.row_groups) {
         set_row(a, p, row);
@@ -317,70 +372,73 @@ template <typename T, int NPT> __global__ __launch_bounds__(LANES, 2) void backw
             for (int n = 0; n < NPT; n++) carry[n] = 0.0f;
         } else if (a.entry_padded) read<NPT>(a.entry + ((pair * a.segments + p.segment) * a.channels + channel) * N + n0, carry);
         else load_states<NPT>(a.entry + (pair * a.channels + channel) * a.states, n0, a.states, carry);
-
-        T x[OWN], raw[OWN], gate[OWN], d_out[OWN];
-        unsigned resets;
-        float first_state[NPT];
-        Shared<T, NPT> next;
-        auto ask_chunk = [&](int t) {
-            ask<T, OWN>(a, a.x, p, channel, t, x);
-            ask<T, OWN>(a, a.delta, p, channel, t, raw);
-            ask<T, OWN>(a, a.d_out, p, channel, t, d_out);
-            if (gated) ask<T, OWN>(a, a.gate, p, channel, t, gate);
-            next.ask(a, p, t, true);
-            resets = resets_of<K>(a, p, t);
-            read<NPT>(a.checkpoints + ((pair * a.chunks + t / K) * a.channels + channel) * N + n0, first_state);
+        const Arguments arguments;
+        const Lanes<T> x_lanes(SCAN_PART(arguments, x), p, channel), delta_lanes(SCAN_PART(arguments, delta), p, channel), gate_lanes(SCAN_PART(arguments, gate), p, channel), d_out_lanes(SCAN_PART(arguments, d_out), p, channel),
+            d_x_lanes(SCAN_PART(arguments, d_x), p, channel), d_delta_lanes(SCAN_PART(arguments, d_delta), p, channel), d_gate_lanes(SCAN_PART(arguments, d_gate), p, channel);
+        GLOBAL float* const d_shared = ONE_TILE ? nullptr : (GLOBAL float*)a.d_shared + ((size_t)p.tile * 2 * a.batch * a.heads + pair) * a.steps * N;
+        auto store_shared = [&](int t, int e, float d_b, float d_c) {      // of step t + e / N
+            if constexpr (ONE_TILE) {
+                if (e % N < a.states) {
+                    at<T>(a.d_b, t + e / N, p.row, p.head)[e % N] = (T)d_b;
+                    at<T>(a.d_c, t + e / N, p.row, p.head)[e % N] = (T)d_c;
+                }
+            } else {
+                GLOBAL float* const to = d_shared + (size_t)t * N;
+                to[e] = d_b;
+                (to + (size_t)a.batch * a.heads * a.steps * N)[e] = d_c;
+            }
         };
         const int chunks = p.live > p.first ? (p.live - p.first + K - 1) / K : 0;
         // steps behind the last chunk that holds any of the row's
-        for (int s = p.first + chunks * K + nq; there && s < p.end; s += 4) {
-            at<T>(a.d_x, s, p.row, p.head)[channel] = (T)0.0f;
-            at<T>(a.d_delta, s, p.row, p.head)[channel] = (T)0.0f;
-            if (gated) at<T>(a.d_gate, s, p.row, p.head)[channel] = (T)0.0f;
+        for (int t = p.first + chunks * K; t < p.end; t += K) {
+#pragma unroll 1
+            for (int i = 0; i < OWN; i++)
+                if (there && t + 4 * i + nq < p.end) {
+                    d_x_lanes.put(t + 4 * i, 0.0f);
+                    d_delta_lanes.put(t + 4 * i, 0.0f);
+                    if (gated) d_gate_lanes.put(t + 4 * i, 0.0f);
+                }
+            for (int e = threadIdx.x; e < K * N; e += LANES) if (t + e / N < p.end) store_shared(t, e, 0.0f, 0.0f);
         }
-        auto store_shared = [&](int s, int n, float d_b, float d_c) {
-            if (a.tiles == 1) {
-                if (n < a.states) { at<T>(a.d_b, s, p.row, p.head)[n] = (T)d_b; at<T>(a.d_c, s, p.row, p.head)[n] = (T)d_c; }
-            } else {
-                float* const to = a.d_shared + (size_t)p.tile * 2 * shared_size + (((size_t)s * a.batch + p.row) * a.heads + p.head) * N + n;
-                to[0] = d_b; to[shared_size] = d_c;
-            }
-        };
-        for (int64_t e = threadIdx.x; e < ((int64_t)p.end - p.first - (int64_t)chunks * K) * N; e += LANES) store_shared(p.first + chunks * K + (int)(e / N), (int)(e % N), 0.0f, 0.0f);
-        if (chunks) ask_chunk(p.first + (chunks - 1) * K);
         for (int k = chunks - 1; k >= 0; k--, turn ^= 1) {
             const int t = p.first + k * K;
-            float xs[OWN], delta[OWN], added[OWN], slope[OWN], d[OWN], ups[OWN], factor[OWN], d_factor[OWN];
-#pragma unroll
-            for (int i = 0; i < OWN; i++) {
-                const bool in = there && t + 4 * i + nq < p.live;
-                float e;
-                const float v = (float)raw[i] + bias;
-                xs[i] = in ? (float)x[i] : 0.0f;
-                delta[i] = softplus(v, e);
-                const float large = rlt_reciprocal(1.0f + e);
-                slope[i] = in ? (v >= 0.0f ? large : e * large) : 0.0f;      // of softplus
-                delta[i] = in ? delta[i] : 0.0f;
-                added[i] = delta[i] * xs[i];
-                ups[i] = in ? (float)d_out[i] : 0.0f;
-                if (gated) {
-                    const float z = in ? (float)gate[i] : 0.0f;
-                    float one, other;
-                    rlt_sigmoids(z, one, other);
-                    factor[i] = z * one;
-                    d_factor[i] = one * fmaf(z, other, 1.0f);
-                    d[i] = ups[i] * factor[i];
-                } else d[i] = ups[i];
-            }
-            const unsigned forget = resets;
+            const bool whole = all_there && t + K <= p.live;
+            float xs[OWN], delta[OWN], added[OWN], slope[OWN], d[OWN], by_gate[OWN];      // by_gate: the gate's gradient but for what it multiplies
             float h[K][NPT], decay[K][NPT], before[NPT];
+            unsigned forget;
+            {
+                T x[OWN], raw[OWN], gate[OWN], d_out[OWN];
+                Shared<T, NPT> next;
+                x_lanes.ask(whole, there, t, p.live, 0.0f, x);
+                delta_lanes.ask(whole, there, t, p.live, NO_DELTA, raw);
+                d_out_lanes.ask(whole, there, t, p.live, 0.0f, d_out);
+                if (gated) gate_lanes.ask(whole, there, t, p.live, 0.0f, gate);
+                next.ask(a, p, t, true);
+                forget = resets_of<K>(a, p, t);
+                read_global<NPT>((const GLOBAL char*)a.checkpoints + (pair * a.chunks + t / K) * a.channels * (N * sizeof(float)) + at_checkpoint, before);
+                next.put(shared[turn]);
 #pragma unroll
-            for (int n = 0; n < NPT; n++) before[n] = first_state[n];
-            next.put(shared[turn]);
-            if (k > 0) ask_chunk(t - K);
+                for (int i = 0; i < OWN; i++) {
+                    float e;
+                    const float v = (float)raw[i] + bias;
+                    xs[i] = (float)x[i];
+                    delta[i] = softplus(v, e);
+                    const float large = rlt_reciprocal(1.0f + e);
+                    slope[i] = v >= 0.0f ? large : e * large;      // of softplus
+                    added[i] = delta[i] * xs[i];
+                    d[i] = (float)d_out[i];
+                    by_gate[i] = 0.0f;
+                    if (gated) {
+                        const float z = (float)gate[i];
+                        float one, other;
+                        rlt_sigmoids(z, one, other);
+                        by_gate[i] = d[i] * one * fmaf(z, other, 1.0f);
+                        d[i] *= z * one;
+                    }
+                }
+            }
             rlt_lds_barrier();
             const float* const bs = shared[turn][0] + n0; const float* const cs = shared[turn][1] + n0;
-            float mixed[OWN], through[OWN], exponent[OWN];
             auto walk = [&](auto with_resets) {
                 constexpr bool RESETS = decltype(with_resets)::value;
 #pragma unroll
@@ -388,8 +446,9 @@ template <typename T, int NPT> __global__ __launch_bounds__(LANES, 2) void backw
                     auto step = [&](auto which) {
                         constexpr int j = decltype(which)::value;
                         const int s = 4 * i + j;
+                        __builtin_amdgcn_sched_barrier(0);
                         const float dt = from_lane<j>(delta[i]), u = from_lane<j>(added[i]);
-                        const bool begins = RESETS && (forget >> s & 1);
+                        const bool begins = RESETS && bit(forget, s);
                         float b[NPT];
                         read<NPT>(bs + s * N, b);
 #pragma unroll
@@ -401,6 +460,9 @@ template <typename T, int NPT> __global__ __launch_bounds__(LANES, 2) void backw
                     };
                     step(std::integral_constant<int, 0>{}); step(std::integral_constant<int, 1>{}); step(std::integral_constant<int, 2>{}); step(std::integral_constant<int, 3>{});
                 }
+                asm volatile("" ::: "memory");      // b is read again rather than held from the walk forward; what other lanes hold is fetched again too
+#pragma unroll
+                for (int i = 0; i < OWN; i++) asm volatile("" : "+v"(delta[i]), "+v"(added[i]));
 #pragma unroll
                 for (int i = OWN - 1; i >= 0; i--) {
                     float mixed_part[4], through_part[4], exponent_part[4], kept_b[KEPT], kept_c[KEPT];
@@ -409,8 +471,9 @@ template <typename T, int NPT> __global__ __launch_bounds__(LANES, 2) void backw
                     auto step = [&](auto which) {
                         constexpr int j = decltype(which)::value;
                         const int s = 4 * i + j;
+                        __builtin_amdgcn_sched_barrier(0);
                         const float dt = from_lane<j>(delta[i]), u = from_lane<j>(added[i]), g = from_lane<j>(d[i]);
-                        const bool begins = RESETS && (forget >> s & 1);
+                        const bool begins = RESETS && bit(forget, s);
                         float b[NPT], c[NPT], d_b[NPT], d_c[NPT];
                         read<NPT>(bs + s * N, b);
                         read<NPT>(cs + s * N, c);
@@ -431,37 +494,32 @@ template <typename T, int NPT> __global__ __launch_bounds__(LANES, 2) void backw
                         sum_channels<NPT>(d_b, sum_b);
                         sum_channels<NPT>(d_c, sum_c);
 #pragma unroll
-                        for (int m = 0; m < KEPT; m++) { kept_b[m] = quad == j ? sum_b[m] : kept_b[m]; kept_c[m] = quad == j ? sum_c[m] : kept_c[m]; }
+                        for (int m = 0; m < KEPT; m++) { kept_b[m] = into_quad<j>(kept_b[m], sum_b[m]); kept_c[m] = into_quad<j>(kept_c[m], sum_c[m]); }
                     };
                     step(std::integral_constant<int, 3>{}); step(std::integral_constant<int, 2>{}); step(std::integral_constant<int, 1>{}); step(std::integral_constant<int, 0>{});
-                    mixed[i] = sum_to_lane(mixed_part, odd, upper);
-                    through[i] = sum_to_lane(through_part, odd, upper);
-                    exponent[i] = sum_to_lane(exponent_part, odd, upper);
+                    const float mixed = sum_to_lane(mixed_part, odd, upper), through = sum_to_lane(through_part, odd, upper), exponent = sum_to_lane(exponent_part, odd, upper);
+                    const float d_delta = fmaf(exponent, LN_2, through * xs[i]) * slope[i];
+                    d_skip = fmaf(d[i], xs[i], d_skip);
+                    d_bias += d_delta;
+                    if (there && t + 4 * i + nq < p.end) {
+                        d_x_lanes.put(t + 4 * i, fmaf(through, delta[i], skip * d[i]));
+                        d_delta_lanes.put(t + 4 * i, d_delta);
+                        if (gated) d_gate_lanes.put(t + 4 * i, by_gate[i] * fmaf(skip, xs[i], mixed));
+                    }
 #pragma unroll
                     for (int m = 0; m < KEPT; m++) { slabs[turn][wave][0][(4 * i + quad) * N + kept_state + m] = kept_b[m]; slabs[turn][wave][1][(4 * i + quad) * N + kept_state + m] = kept_c[m]; }
                 }
             };
             if (forget) walk(std::true_type{}); else walk(std::false_type{});
-#pragma unroll
-            for (int i = 0; i < OWN; i++) {
-                const int s = t + 4 * i + nq;
-                const float d_delta = fmaf(exponent[i], LN_2, through[i] * xs[i]) * slope[i];
-                d_skip = fmaf(d[i], xs[i], d_skip);
-                d_bias += d_delta;
-                if (there && s < p.end) {
-                    at<T>(a.d_x, s, p.row, p.head)[channel] = (T)fmaf(through[i], delta[i], skip * d[i]);
-                    at<T>(a.d_delta, s, p.row, p.head)[channel] = (T)d_delta;
-                    if (gated) at<T>(a.d_gate, s, p.row, p.head)[channel] = (T)(ups[i] * d_factor[i] * fmaf(skip, xs[i], mixed[i]));
-                }
-            }
             rlt_lds_barrier();
-            for (int e = threadIdx.x; e < K * N; e += LANES) {
-                const int s = t + e / N;
-                if (s < p.end) {
+#pragma unroll
+            for (int j = 0; j < PER; j++) {
+                const int e = threadIdx.x + j * LANES;
+                if (e < K * N && t + e / N < p.end) {
                     float d_b = 0.0f, d_c = 0.0f;
 #pragma unroll
                     for (int w = 0; w < WAVES; w++) { d_b += slabs[turn][w][0][e]; d_c += slabs[turn][w][1][e]; }
-                    store_shared(s, e % N, d_b, d_c);
+                    store_shared(t, e, d_b, d_c);
                 }
             }
         }
@@ -482,7 +540,7 @@ template <typename T, int NPT> __global__ __launch_bounds__(LANES) void backward
     Place p = place_of(a, blockIdx.x, a.batch);
     set_row(a, p, p.row);
     const int lane = threadIdx.x & 63, nq = lane & 3, n0 = nq * NPT, own_channel = p.tile * TILE + (int)(threadIdx.x >> 2), channel = min(own_channel, a.channels - 1);
-    const bool there = own_channel < a.channels;
+    const bool there = own_channel < a.channels, all_there = (p.tile + 1) * TILE <= a.channels, gated = a.gate.data != nullptr;
     const size_t pair = pair_of(a, p);
     float rate[NPT], carry[NPT], sum = 0.0f;
     load_rates<NPT>(a, p.head, channel, n0, rate);
@@ -493,10 +551,13 @@ template <typename T, int NPT> __global__ __launch_bounds__(LANES) void backward
     T raw[OWN], gate[OWN], d_out[OWN];
     unsigned resets;
     Shared<T, NPT> next;
+    const Arguments arguments;
+    const Lanes<T> delta_lanes(SCAN_PART(arguments, delta), p, channel), gate_lanes(SCAN_PART(arguments, gate), p, channel), d_out_lanes(SCAN_PART(arguments, d_out), p, channel);
     auto ask_chunk = [&](int t) {
-        ask<T, OWN>(a, a.delta, p, channel, t, raw);
-        ask<T, OWN>(a, a.d_out, p, channel, t, d_out);
-        if (a.gate.data) ask<T, OWN>(a, a.gate, p, channel, t, gate);
+        const bool whole = all_there && t + K <= p.live;
+        delta_lanes.ask(whole, there, t, p.live, NO_DELTA, raw);
+        d_out_lanes.ask(whole, there, t, p.live, 0.0f, d_out);
+        if (gated) gate_lanes.ask(whole, there, t, p.live, 0.0f, gate);
         next.ask(a, p, t, false);
         resets = resets_of<K>(a, p, t);
     };
@@ -508,14 +569,13 @@ template <typename T, int NPT> __global__ __launch_bounds__(LANES) void backward
         float delta[OWN], d[OWN];
 #pragma unroll
         for (int i = 0; i < OWN; i++) {
-            const bool in = t + 4 * i + nq < p.live;
             float e;
-            delta[i] = in ? softplus((float)raw[i] + bias, e) : 0.0f;
-            d[i] = in ? (float)d_out[i] : 0.0f;
-            if (a.gate.data) {
+            delta[i] = softplus((float)raw[i] + bias, e);
+            d[i] = (float)d_out[i];
+            if (gated) {
                 float one, other;
                 rlt_sigmoids((float)gate[i], one, other);
-                d[i] = in ? d[i] * (float)gate[i] * one : 0.0f;
+                d[i] *= (float)gate[i] * one;
             }
             sum += delta[i];
         }
@@ -550,11 +610,11 @@ template <typename T, int NPT> __global__ __launch_bounds__(LANES) void backward
 
 // d_b and d_c out of the tiles' shares
 template <typename T> __global__ __launch_bounds__(256) void shared_sum_kernel(Scan a, int padded) {
-    const size_t tokens = (size_t)a.steps * a.batch * a.heads, size = tokens * padded;
+    const size_t size = (size_t)a.batch * a.heads * a.steps * padded;
     for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < 2 * size; i += (size_t)gridDim.x * 256) {
         const bool second = i >= size;
-        const size_t e = second ? i - size : i, token = e / padded, line = token / a.heads;
-        const int n = (int)(e - token * padded), head = (int)(token - line * a.heads), step = (int)(line / a.batch), row = (int)(line - (size_t)step * a.batch);
+        const size_t e = second ? i - size : i, line = e / padded, pair = line / a.steps;
+        const int n = (int)(e - line * padded), step = (int)(line - pair * a.steps), row = (int)(pair / a.heads), head = (int)(pair - (size_t)row * a.heads);
         if (n >= a.states) continue;
         float s = 0.0f;
         for (int tile = 0; tile < a.tiles; tile++) s += a.d_shared[(size_t)tile * 2 * size + i];
@@ -759,7 +819,9 @@ int rlt_rocm_selective_scan_backward(rlt_rocm_device* device, const rlt_selectiv
             if ((rc = rlt_launch_status(device)) || (rc = join_segments<true>(device, f, d_final_state, f.exit, 4 * NPT))) return rc;
             a.entry = f.exit; a.entry_padded = 1;
         }
-        hipLaunchKernelGGL((backward_kernel<T, NPT>), dim3(blocks_of(a, a.row_groups)), dim3(LANES), 0, device->stream, a);
+        const dim3 blocks(blocks_of(a, a.row_groups));
+        if (a.tiles == 1) hipLaunchKernelGGL((backward_kernel<T, NPT, true>), blocks, dim3(LANES), 0, device->stream, a);
+        else hipLaunchKernelGGL((backward_kernel<T, NPT, false>), blocks, dim3(LANES), 0, device->stream, a);
         if ((rc = rlt_launch_status(device))) return rc;
         if (a.tiles > 1) {
             hipLaunchKernelGGL(shared_sum_kernel<T>, dim3(2048), dim3(256), 0, device->stream, a, 4 * NPT);
