@@ -87,13 +87,31 @@ template <int NPT> __device__ __forceinline__ void sum_channels(const float (&v)
     }
 }
 
-// log(1 + e^v), and e^-|v|: with s = e / (2 + e), e = e^-|v|, log(1 + e) = 2 artanh(s), whose series in s^2 <= 1/9 ends at s^15 (relative rest 1.4e-9); keeps its relative accuracy far below zero
-__device__ __forceinline__ float softplus(float v, float& e) {
-    e = rlt_exp_negative(-fabsf(v));
-    const float s = e * rlt_reciprocal(2.0f + e), z = s * s;
-    float p = fmaf(z, 1.0f / 15, 1.0f / 13);
-    p = fmaf(p, z, 1.0f / 11); p = fmaf(p, z, 1.0f / 9); p = fmaf(p, z, 1.0f / 7); p = fmaf(p, z, 1.0f / 5); p = fmaf(p, z, 1.0f / 3);
-    return fmaxf(v, 0.0f) + 2.0f * fmaf(s * z, p, s);
+// The elements' own functions. fp32 tensors take what the rounding of an exponent drops along (rlt_exp_negative) and a step of Newton's method behind a reciprocal; bfloat16 ones do without: delta is off by |raw| 2^-25 of itself, a thousandth
+// of what the rounding of raw leaves, and it saves an eighth of the forward pass.
+template <typename T> __device__ __forceinline__ float exp_negative(float t) { return sizeof(T) == sizeof(float) ? rlt_exp_negative(t) : __builtin_amdgcn_exp2f(t * LOG2_E); }
+template <typename T> __device__ __forceinline__ float reciprocal(float d) { return sizeof(T) == sizeof(float) ? rlt_reciprocal(d) : __builtin_amdgcn_rcpf(d); }
+// log(1 + e^v), and e = e^-|v|. With u = 1 + e as it is rounded, log(1 + e) = log(u) + (e - (u - 1)), whose last part is exact and all there is of it far below zero; the instruction's logarithm to base 2 is within
+// 1.2e-7 of itself down to u's last bit (measured on all u in [1, 2)).
+template <typename T> __device__ __forceinline__ float softplus(float v, float& e) {
+    e = exp_negative<T>(-fabsf(v));
+    const float u = 1.0f + e;
+    return fmaxf(v, 0.0f) + fmaf(__builtin_amdgcn_logf(u), LN_2, e - (u - 1.0f));
+}
+// z / (1 + e^-z), and (PASSED) d times its slope
+template <typename T> __device__ __forceinline__ float gate_factor(float z) {
+    if constexpr (sizeof(T) == sizeof(float)) {
+        float one, other;
+        rlt_sigmoids(z, one, other);
+        return z * one;
+    } else return z * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -LOG2_E));
+}
+template <typename T> __device__ __forceinline__ float gate_factor(float z, float d, float& passed) {
+    float one, other;
+    if constexpr (sizeof(T) == sizeof(float)) rlt_sigmoids(z, one, other);
+    else { one = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -LOG2_E)); other = 1.0f - one; }
+    passed = d * one * fmaf(z, other, 1.0f);
+    return z * one;
 }
 
 // ---- what a workgroup walks over
@@ -113,6 +131,7 @@ __device__ __forceinline__ void set_row(const Scan& a, Place& p, int row) {
 }
 __device__ __forceinline__ int pair_of(const Scan& a, const Place& p) { return p.row * a.heads + p.head; }
 __device__ __forceinline__ bool bit(unsigned mask, int i) {
+    mask = __builtin_amdgcn_readfirstlane(mask);
     asm volatile("" : "+s"(mask));      // looked at where it is needed: sixteen answers held from a walk forward to the one back are 32 scalar registers
     return mask >> i & 1;
 }
@@ -255,7 +274,7 @@ template <typename T, int NPT, bool STATES> __global__ __launch_bounds__(LANES) 
         for (int i = 0; i < OWN; i++) {
             float e;
             xs[i] = (float)x[i];
-            delta[i] = softplus((float)raw[i] + bias, e);
+            delta[i] = softplus<T>((float)raw[i] + bias, e);
             added[i] = delta[i] * xs[i];
             if (!STATES) gates[i] = gated ? (float)gate[i] : 0.0f;
         }
@@ -299,11 +318,7 @@ template <typename T, int NPT, bool STATES> __global__ __launch_bounds__(LANES) 
             for (int i = 0; i < OWN; i++) {
                 const int s = t + 4 * i + nq;
                 float v = fmaf(skip, xs[i], y[i]);
-                if (gated) {
-                    float one, other;
-                    rlt_sigmoids(gates[i], one, other);
-                    v *= gates[i] * one;
-                }
+                if (gated) v *= gate_factor<T>(gates[i]);
                 if (there && s < p.end) out_lanes.put(t + 4 * i, v);      // (steps beyond the row's length: no input and nothing read, zero)
             }
         }
@@ -400,42 +415,41 @@ template <typename T, int NPT, bool ONE_TILE> __global__ __launch_bounds__(LANES
                 }
             for (int e = threadIdx.x; e < K * N; e += LANES) if (t + e / N < p.end) store_shared(t, e, 0.0f, 0.0f);
         }
+        T x[OWN], raw[OWN], gate[OWN], d_out[OWN];
+        Shared<T, NPT> next;
+        unsigned resets;
+        float first_state[NPT];
+        auto ask_chunk = [&](int t) {
+            const bool whole = all_there && t + K <= p.live;
+            x_lanes.ask(whole, there, t, p.live, 0.0f, x);
+            delta_lanes.ask(whole, there, t, p.live, NO_DELTA, raw);
+            d_out_lanes.ask(whole, there, t, p.live, 0.0f, d_out);
+            if (gated) gate_lanes.ask(whole, there, t, p.live, 0.0f, gate);
+            next.ask(a, p, t, true);
+            resets = resets_of<K>(a, p, t);
+            read_global<NPT>((const GLOBAL char*)a.checkpoints + (pair * a.chunks + t / K) * a.channels * (N * sizeof(float)) + at_checkpoint, first_state);
+        };
+        if (chunks) ask_chunk(p.first + (chunks - 1) * K);
         for (int k = chunks - 1; k >= 0; k--, turn ^= 1) {
             const int t = p.first + k * K;
-            const bool whole = all_there && t + K <= p.live;
             float xs[OWN], delta[OWN], added[OWN], slope[OWN], d[OWN], by_gate[OWN];      // by_gate: the gate's gradient but for what it multiplies
             float h[K][NPT], decay[K][NPT], before[NPT];
-            unsigned forget;
-            {
-                T x[OWN], raw[OWN], gate[OWN], d_out[OWN];
-                Shared<T, NPT> next;
-                x_lanes.ask(whole, there, t, p.live, 0.0f, x);
-                delta_lanes.ask(whole, there, t, p.live, NO_DELTA, raw);
-                d_out_lanes.ask(whole, there, t, p.live, 0.0f, d_out);
-                if (gated) gate_lanes.ask(whole, there, t, p.live, 0.0f, gate);
-                next.ask(a, p, t, true);
-                forget = resets_of<K>(a, p, t);
-                read_global<NPT>((const GLOBAL char*)a.checkpoints + (pair * a.chunks + t / K) * a.channels * (N * sizeof(float)) + at_checkpoint, before);
-                next.put(shared[turn]);
+            const unsigned forget = resets;
+            next.put(shared[turn]);
 #pragma unroll
-                for (int i = 0; i < OWN; i++) {
-                    float e;
-                    const float v = (float)raw[i] + bias;
-                    xs[i] = (float)x[i];
-                    delta[i] = softplus(v, e);
-                    const float large = rlt_reciprocal(1.0f + e);
-                    slope[i] = v >= 0.0f ? large : e * large;      // of softplus
-                    added[i] = delta[i] * xs[i];
-                    d[i] = (float)d_out[i];
-                    by_gate[i] = 0.0f;
-                    if (gated) {
-                        const float z = (float)gate[i];
-                        float one, other;
-                        rlt_sigmoids(z, one, other);
-                        by_gate[i] = d[i] * one * fmaf(z, other, 1.0f);
-                        d[i] *= z * one;
-                    }
-                }
+            for (int n = 0; n < NPT; n++) before[n] = first_state[n];
+#pragma unroll
+            for (int i = 0; i < OWN; i++) {
+                float e;
+                const float v = (float)raw[i] + bias;
+                xs[i] = (float)x[i];
+                delta[i] = softplus<T>(v, e);
+                const float large = reciprocal<T>(1.0f + e);
+                slope[i] = v >= 0.0f ? large : e * large;      // of softplus
+                added[i] = delta[i] * xs[i];
+                d[i] = (float)d_out[i];
+                by_gate[i] = 0.0f;
+                if (gated) d[i] *= gate_factor<T>((float)gate[i], (float)d_out[i], by_gate[i]);
             }
             rlt_lds_barrier();
             const float* const bs = shared[turn][0] + n0; const float* const cs = shared[turn][1] + n0;
@@ -465,6 +479,7 @@ template <typename T, int NPT, bool ONE_TILE> __global__ __launch_bounds__(LANES
                 for (int i = 0; i < OWN; i++) asm volatile("" : "+v"(delta[i]), "+v"(added[i]));
 #pragma unroll
                 for (int i = OWN - 1; i >= 0; i--) {
+                    if (i == 0 && k > 0) ask_chunk(t - K);      // the registers of states that are behind take what the next chunk needs
                     float mixed_part[4], through_part[4], exponent_part[4], kept_b[KEPT], kept_c[KEPT];
 #pragma unroll
                     for (int m = 0; m < KEPT; m++) kept_b[m] = kept_c[m] = 0.0f;
@@ -570,13 +585,9 @@ template <typename T, int NPT> __global__ __launch_bounds__(LANES) void backward
 #pragma unroll
         for (int i = 0; i < OWN; i++) {
             float e;
-            delta[i] = softplus((float)raw[i] + bias, e);
+            delta[i] = softplus<T>((float)raw[i] + bias, e);
             d[i] = (float)d_out[i];
-            if (gated) {
-                float one, other;
-                rlt_sigmoids((float)gate[i], one, other);
-                d[i] *= (float)gate[i] * one;
-            }
+            if (gated) d[i] *= gate_factor<T>((float)gate[i]);
             sum += delta[i];
         }
         const unsigned forget = resets;
@@ -661,7 +672,7 @@ template <typename T, int NPT> __global__ __launch_bounds__(256) void step_kerne
     load_states<NPT>(forget ? nullptr : a.entry + (pair * a.channels + channel) * a.states, n0, a.states, h);
     load_rates<NPT>(a, head, channel, n0, rate);
     const T* const b = at<T>(a.b, 0, row, head); const T* const c = at<T>(a.c, 0, row, head);
-    const float x = (float)at<T>(a.x, 0, row, head)[channel], delta = softplus((float)at<T>(a.delta, 0, row, head)[channel] + (a.delta_biases ? a.delta_biases[at_channel] : 0.0f), e), u = delta * x;
+    const float x = (float)at<T>(a.x, 0, row, head)[channel], delta = softplus<T>((float)at<T>(a.delta, 0, row, head)[channel] + (a.delta_biases ? a.delta_biases[at_channel] : 0.0f), e), u = delta * x;
 #pragma unroll
     for (int n = 0; n < NPT; n++) {
         const bool there = n0 + n < a.states;
@@ -689,9 +700,9 @@ int tiles_of(const rlt_selective_scan* p) { return (p->channels + TILE - 1) / TI
 
 // Steps are cut into segments where rows, heads and channels alone leave the chip without work.
 struct Segments { int count, steps, row_groups; };
-Segments segments_of(const rlt_selective_scan* p, int steps) {
+Segments segments_of(const rlt_selective_scan* p, int steps, bool backward) {
     const int chunk = chunk_of(p->states), chunks = (steps + chunk - 1) / chunk;
-    const int64_t blocks = (int64_t)p->batch * p->heads * tiles_of(p), wanted = 512;
+    const int64_t blocks = (int64_t)p->batch * p->heads * tiles_of(p), wanted = backward ? 512 : 1024;      // as many wavefronts as have registers: two to a SIMD, four
     int64_t count = blocks >= wanted ? 1 : (wanted + blocks - 1) / blocks;
     if (count > chunks / 4) count = chunks / 4;
     if (count < 1) count = 1;
@@ -705,14 +716,14 @@ bool supported(const rlt_selective_scan* p, int steps) {
     if (p->states > MAX_STATES || steps > MAX_STEPS) return false;
     const __int128 pairs = (__int128)p->batch * p->heads, limit = (__int128)1 << 31;
     if (pairs * p->channels * MAX_STATES > limit || pairs * steps > limit) return false;
-    const __int128 blocks = pairs * tiles_of(p) * segments_of(p, steps).count;
+    const __int128 blocks = pairs * tiles_of(p) * segments_of(p, steps, false).count;
     return blocks * LANES <= UINT32_MAX;
 }
 size_t padded(size_t n) { return (n + 63) / 64 * 64; }
 // scratch memory, in floats
 struct Scratch { size_t states, sums, shared, rates, skips, biases, total; };
 Scratch scratch_of(const rlt_selective_scan* p, int steps, bool backward) {
-    const Segments g = segments_of(p, steps);
+    const Segments g = segments_of(p, steps, backward);
     const size_t channels = (size_t)p->batch * p->heads * p->channels, wide = 4 * per_lane(p->states), parts = (size_t)g.row_groups * g.count * p->heads * p->channels;
     Scratch s{};
     size_t at = 0;
@@ -726,8 +737,8 @@ Scratch scratch_of(const rlt_selective_scan* p, int steps, bool backward) {
     return s;
 }
 Scan scan_of(const rlt_selective_scan* p, const rlt_head_view* x, const rlt_head_view* delta, const rlt_head_view* b, const rlt_head_view* c, const rlt_head_view* gate, const uint8_t* reset,
-             const int32_t* lengths, int steps) {
-    const Segments g = segments_of(p, steps);
+             const int32_t* lengths, int steps, bool backward) {
+    const Segments g = segments_of(p, steps, backward);
     Scan a{};
     a.log_rates = p->log_rates; a.skip = p->skip; a.delta_biases = p->delta_biases;
     a.x = rlt_part_of(x); a.delta = rlt_part_of(delta); a.b = rlt_part_of(b); a.c = rlt_part_of(c); a.gate = rlt_part_of(gate);
@@ -774,7 +785,7 @@ int rlt_rocm_selective_scan_forward(rlt_rocm_device* device, const rlt_selective
     if (!supported(layer, steps)) return RLT_E_UNSUPPORTED;
     const Scratch s = scratch_of(layer, steps, false);
     RLT_REQUIRE(s.total == 0 || (workspace && workspace_bytes >= s.total * sizeof(float) && reinterpret_cast<uintptr_t>(workspace) % 16 == 0));
-    Scan a = scan_of(layer, x, delta, b, c, gate, reset, lengths, steps);
+    Scan a = scan_of(layer, x, delta, b, c, gate, reset, lengths, steps, false);
     a.out = rlt_part_of(output); a.checkpoints = (float*)checkpoints; a.entry = initial_state; a.exit = final_state;
     return by_kind(layer, [&](auto type, auto n) {
         typedef decltype(type) T;
@@ -804,7 +815,7 @@ int rlt_rocm_selective_scan_backward(rlt_rocm_device* device, const rlt_selectiv
     const Scratch s = scratch_of(layer, steps, true);
     RLT_REQUIRE(workspace && workspace_bytes >= s.total * sizeof(float) && reinterpret_cast<uintptr_t>(workspace) % 16 == 0);
     float* const w = (float*)workspace;
-    Scan a = scan_of(layer, x, delta, b, c, gate, reset, lengths, steps);
+    Scan a = scan_of(layer, x, delta, b, c, gate, reset, lengths, steps, true);
     a.d_out = rlt_part_of(d_output); a.d_x = rlt_part_of(d_x); a.d_delta = rlt_part_of(d_delta); a.d_b = rlt_part_of(d_b); a.d_c = rlt_part_of(d_c); a.d_gate = rlt_part_of(d_gate);
     a.checkpoints = (float*)const_cast<void*>(checkpoints); a.entry = d_final_state; a.exit = d_initial_state;
     a.d_shared = w + s.shared; a.d_rates = layer->d_log_rates ? w + s.rates : nullptr; a.d_skips = layer->d_skip ? w + s.skips : nullptr; a.d_biases = layer->d_delta_biases ? w + s.biases : nullptr;
@@ -840,7 +851,7 @@ int rlt_rocm_selective_scan_step(rlt_rocm_device* device, const rlt_selective_sc
     if (!device) return RLT_E_NOT_INITIALISED;
     RLT_REQUIRE(given(layer, x, delta, b, c, gate) && rlt_given(output) && state && next_state);
     if (!supported(layer, 1)) return RLT_E_UNSUPPORTED;
-    Scan a = scan_of(layer, x, delta, b, c, gate, reset, nullptr, 1);
+    Scan a = scan_of(layer, x, delta, b, c, gate, reset, nullptr, 1, false);
     a.out = rlt_part_of(output); a.entry = state; a.exit = next_state;
     return by_kind(layer, [&](auto type, auto n) {
         const size_t blocks = ((size_t)a.batch * a.heads * a.channels + 63) / 64;
