@@ -56,6 +56,9 @@ __device__ __forceinline__ float sum_of_lanes(float v) {
     v += lanes<0xB1>(v);
     return v + lanes<0x4E>(v);
 }
+template <int FIRST, int LAST, typename F> __device__ __forceinline__ void each(F&& f) {
+    if constexpr (FIRST < LAST) { f(std::integral_constant<int, FIRST>{}); each<FIRST + 1, LAST>(f); }
+}
 // v in the lanes of quad J of each row of sixteen, `old` in the others
 template <int J> __device__ __forceinline__ float into_quad(float old, float v) {
     return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, old), __builtin_bit_cast(int, v), 0xE4, 0xF, 1 << J, false));
@@ -552,7 +555,7 @@ template <typename T, int NPT, bool ONE_TILE> __global__ __launch_bounds__(LANES
 template <typename T, int NPT> __global__ __launch_bounds__(LANES) void backward_states_kernel(Scan a) {
     constexpr int K = CHUNK<NPT>, OWN = K / 4, N = 4 * NPT;
     __shared__ float shared[2][2][K * N];
-    Place p = place_of(a, blockIdx.x, a.batch);
+    Place p = place_of(a, blockIdx.x + (unsigned)a.tiles * a.heads * a.batch, a.batch);      // the first segment's states reach none
     set_row(a, p, p.row);
     const int lane = threadIdx.x & 63, nq = lane & 3, n0 = nq * NPT, own_channel = p.tile * TILE + (int)(threadIdx.x >> 2), channel = min(own_channel, a.channels - 1);
     const bool there = own_channel < a.channels, all_there = (p.tile + 1) * TILE <= a.channels, gated = a.gate.data != nullptr;
@@ -661,36 +664,67 @@ __global__ __launch_bounds__(1024) void parameter_sum_kernel(Scan a, int parts, 
     *to = accumulate ? *to + s : s;
 }
 
-// One step of a row: a pass over the states, which are read and written once. Four lanes share a channel.
-template <typename T, int NPT> __global__ __launch_bounds__(256) void step_kernel(Scan a) {
-    const size_t i = (size_t)blockIdx.x * 64 + (threadIdx.x >> 2), pair = i / a.channels;
-    const int channel = (int)(i - pair * a.channels), row = (int)(pair / a.heads), head = (int)(pair - (size_t)row * a.heads), nq = threadIdx.x & 3, n0 = nq * NPT;
-    if (pair >= (size_t)a.batch * a.heads) return;
+// One step of four rows: a pass over the states, which are read and written once, and what bounds it. Four lanes share a channel, each with a quarter of its states of every row and all that depends on the step alone of one of them. WHOLE: a lane's
+// states are vectors of 16 bytes.
+template <typename T, int NPT, bool WHOLE> __global__ __launch_bounds__(LANES) void step_kernel(Scan a) {
+    constexpr int V = NPT < 4 ? NPT : 4;
+    typedef float vector __attribute__((ext_vector_type(V)));
+    const int nq = threadIdx.x & 3, n0 = nq * NPT;
+    unsigned item = blockIdx.x;
+    const int tile = item % a.tiles; item /= a.tiles;
+    const int head = item % a.heads, row0 = item / a.heads * 4, own_channel = tile * TILE + (int)(threadIdx.x >> 2), channel = min(own_channel, a.channels - 1), own_row = min(row0 + nq, a.batch - 1);
+    const bool there = own_channel < a.channels;
     const size_t at_channel = (size_t)head * a.channels + channel;
-    float rate[NPT], h[NPT], e, sum = 0.0f;
-    const bool forget = a.reset && a.reset[row];
-    load_states<NPT>(forget ? nullptr : a.entry + (pair * a.channels + channel) * a.states, n0, a.states, h);
-    load_rates<NPT>(a, head, channel, n0, rate);
-    const T* const b = at<T>(a.b, 0, row, head); const T* const c = at<T>(a.c, 0, row, head);
-    const float x = (float)at<T>(a.x, 0, row, head)[channel], delta = softplus<T>((float)at<T>(a.delta, 0, row, head)[channel] + (a.delta_biases ? a.delta_biases[at_channel] : 0.0f), e), u = delta * x;
+    float h[4][NPT], rate[NPT], sum[4];
 #pragma unroll
-    for (int n = 0; n < NPT; n++) {
-        const bool there = n0 + n < a.states;
-        h[n] = fmaf(__builtin_amdgcn_exp2f(delta * rate[n]), h[n], there ? u * (float)b[n0 + n] : 0.0f);
-        if (there) sum = fmaf((float)c[n0 + n], h[n], sum);
+    for (int r = 0; r < 4; r++) {
+        const int row = min(row0 + r, a.batch - 1);
+        const float* const from = a.entry + (((size_t)row * a.heads + head) * a.channels + channel) * a.states + n0;
+        if constexpr (WHOLE) {
+#pragma unroll
+            for (int n = 0; n < NPT; n += V) {
+                const vector v = *reinterpret_cast<const vector*>(from + n);
+#pragma unroll
+                for (int i = 0; i < V; i++) h[r][n + i] = v[i];
+            }
+        } else load_states<NPT>(from - n0, n0, a.states, h[r]);
     }
-    store_states<NPT>(a.exit + (pair * a.channels + channel) * a.states, n0, a.states, h);
-    sum = sum_of_lanes(sum);
-    if (nq == 0) {
-        float v = a.skip ? fmaf(a.skip[at_channel], x, sum) : sum;
-        if (a.gate.data) {
-            const float z = (float)at<T>(a.gate, 0, row, head)[channel];
-            float one, other;
-            rlt_sigmoids(z, one, other);
-            v *= z * one;
+    const float x = (float)at<T>(a.x, 0, own_row, head)[channel], raw = (float)at<T>(a.delta, 0, own_row, head)[channel], z = a.gate.data ? (float)at<T>(a.gate, 0, own_row, head)[channel] : 0.0f;
+    const bool forget = a.reset && a.reset[own_row];
+    load_rates<NPT>(a, head, channel, n0, rate);
+    float e;
+    const float delta = softplus<T>(raw + (a.delta_biases ? a.delta_biases[at_channel] : 0.0f), e), u = delta * x, forgets = forget ? 1.0f : 0.0f;
+    each<0, 4>([&](auto which) {
+        constexpr int r = decltype(which)::value;
+        const int row = min(row0 + r, a.batch - 1);
+        const float d = from_lane<r>(delta), added = from_lane<r>(u);
+        const bool begins = from_lane<r>(forgets) != 0.0f;
+        const T* const b = at<T>(a.b, 0, row, head); const T* const c = at<T>(a.c, 0, row, head);
+        sum[r] = 0.0f;
+#pragma unroll
+        for (int n = 0; n < NPT; n++) {
+            const bool in = WHOLE || n0 + n < a.states;
+            const float bn = in ? (float)b[n0 + n] : 0.0f, cn = in ? (float)c[n0 + n] : 0.0f;
+            h[r][n] = fmaf(__builtin_amdgcn_exp2f(d * rate[n]), begins ? 0.0f : h[r][n], added * bn);
+            sum[r] = fmaf(cn, h[r][n], sum[r]);
         }
-        at<T>(a.out, 0, row, head)[channel] = (T)v;
-    }
+        float* const to = a.exit + (((size_t)row * a.heads + head) * a.channels + channel) * a.states + n0;
+        if (there && row0 + r < a.batch) {
+            if constexpr (WHOLE) {
+#pragma unroll
+                for (int n = 0; n < NPT; n += V) {
+                    vector v;
+#pragma unroll
+                    for (int i = 0; i < V; i++) v[i] = h[r][n + i];
+                    *reinterpret_cast<vector*>(to + n) = v;
+                }
+            } else store_states<NPT>(to - n0, n0, a.states, h[r]);
+        }
+    });
+    float v = sum_to_lane(sum, nq & 1, nq & 2);
+    if (a.skip) v = fmaf(a.skip[at_channel], x, v);
+    if (a.gate.data) v *= gate_factor<T>(z);
+    if (there && row0 + nq < a.batch) at<T>(a.out, 0, own_row, head)[channel] = (T)v;
 }
 
 bool described(const rlt_selective_scan* p) {
@@ -702,7 +736,7 @@ int tiles_of(const rlt_selective_scan* p) { return (p->channels + TILE - 1) / TI
 struct Segments { int count, steps, row_groups; };
 Segments segments_of(const rlt_selective_scan* p, int steps, bool backward) {
     const int chunk = chunk_of(p->states), chunks = (steps + chunk - 1) / chunk;
-    const int64_t blocks = (int64_t)p->batch * p->heads * tiles_of(p), wanted = backward ? 512 : 1024;      // as many wavefronts as have registers: two to a SIMD, four
+    const int64_t blocks = (int64_t)p->batch * p->heads * tiles_of(p), wanted = 1024;      // four wavefronts to a SIMD
     int64_t count = blocks >= wanted ? 1 : (wanted + blocks - 1) / blocks;
     if (count > chunks / 4) count = chunks / 4;
     if (count < 1) count = 1;
@@ -759,6 +793,7 @@ template <bool REVERSE> int join_segments(rlt_rocm_device* device, const Scan& a
     hipLaunchKernelGGL(join_segments_kernel<REVERSE>, dim3((unsigned)blocks), dim3(256), 0, device->stream, a, initial, states, wide);
     return rlt_launch_status(device);
 }
+template <typename... V> bool near(const V*... views) { return ((!views || (views->step_stride >= -MAX_STRIDE && views->step_stride <= MAX_STRIDE)) && ...); }
 bool given(const rlt_selective_scan* p, const rlt_head_view* x, const rlt_head_view* delta, const rlt_head_view* b, const rlt_head_view* c, const rlt_head_view* gate) {
     return described(p) && p->log_rates && rlt_given(x) && rlt_given(delta) && rlt_given(b) && rlt_given(c) && (!gate || gate->data);
 }
@@ -782,7 +817,7 @@ int rlt_rocm_selective_scan_forward(rlt_rocm_device* device, const rlt_selective
                                     void* checkpoints, void* workspace, size_t workspace_bytes) {
     if (!device) return RLT_E_NOT_INITIALISED;
     RLT_REQUIRE(given(layer, x, delta, b, c, gate) && rlt_given(output) && steps > 0 && reinterpret_cast<uintptr_t>(checkpoints) % 16 == 0);
-    if (!supported(layer, steps)) return RLT_E_UNSUPPORTED;
+    if (!supported(layer, steps) || !near(x, delta, b, c, gate, output)) return RLT_E_UNSUPPORTED;
     const Scratch s = scratch_of(layer, steps, false);
     RLT_REQUIRE(s.total == 0 || (workspace && workspace_bytes >= s.total * sizeof(float) && reinterpret_cast<uintptr_t>(workspace) % 16 == 0));
     Scan a = scan_of(layer, x, delta, b, c, gate, reset, lengths, steps, false);
@@ -794,7 +829,7 @@ int rlt_rocm_selective_scan_forward(rlt_rocm_device* device, const rlt_selective
             Scan f = a;
             float* const states = (float*)workspace + s.states;
             f.sums = (float*)workspace + s.sums; f.exit = states;
-            hipLaunchKernelGGL((forward_kernel<T, NPT, true>), dim3(blocks_of(a, a.batch)), dim3(LANES), 0, device->stream, f);
+            hipLaunchKernelGGL((forward_kernel<T, NPT, true>), dim3(blocks_of(a, a.batch) / a.segments * (a.segments - 1)), dim3(LANES), 0, device->stream, f);      // (nothing starts from what the last segment adds)
             int rc = rlt_launch_status(device);
             if (rc || (rc = join_segments<false>(device, f, initial_state, states, 4 * NPT))) return rc;
             a.entry = states; a.entry_padded = 1;
@@ -811,7 +846,7 @@ int rlt_rocm_selective_scan_backward(rlt_rocm_device* device, const rlt_selectiv
     if (!device) return RLT_E_NOT_INITIALISED;
     RLT_REQUIRE(given(layer, x, delta, b, c, gate) && rlt_given(d_output) && rlt_given(d_x) && rlt_given(d_delta) && rlt_given(d_b) && rlt_given(d_c) && (!gate || rlt_given(d_gate)) && steps > 0);
     RLT_REQUIRE(checkpoints && reinterpret_cast<uintptr_t>(checkpoints) % 16 == 0);
-    if (!supported(layer, steps)) return RLT_E_UNSUPPORTED;
+    if (!supported(layer, steps) || !near(x, delta, b, c, gate, d_output, d_x, d_delta, d_b, d_c, gate ? d_gate : nullptr)) return RLT_E_UNSUPPORTED;
     const Scratch s = scratch_of(layer, steps, true);
     RLT_REQUIRE(workspace && workspace_bytes >= s.total * sizeof(float) && reinterpret_cast<uintptr_t>(workspace) % 16 == 0);
     float* const w = (float*)workspace;
@@ -826,7 +861,7 @@ int rlt_rocm_selective_scan_backward(rlt_rocm_device* device, const rlt_selectiv
         if (a.segments > 1) {
             Scan f = a;
             f.sums = w + s.sums; f.exit = w + s.states;
-            hipLaunchKernelGGL((backward_states_kernel<T, NPT>), dim3(blocks_of(a, a.batch)), dim3(LANES), 0, device->stream, f);
+            hipLaunchKernelGGL((backward_states_kernel<T, NPT>), dim3(blocks_of(a, a.batch) / a.segments * (a.segments - 1)), dim3(LANES), 0, device->stream, f);      // (nothing goes on from the first segment)
             if ((rc = rlt_launch_status(device)) || (rc = join_segments<true>(device, f, d_final_state, f.exit, 4 * NPT))) return rc;
             a.entry = f.exit; a.entry_padded = 1;
         }
@@ -854,8 +889,12 @@ int rlt_rocm_selective_scan_step(rlt_rocm_device* device, const rlt_selective_sc
     Scan a = scan_of(layer, x, delta, b, c, gate, reset, nullptr, 1, false);
     a.out = rlt_part_of(output); a.entry = state; a.exit = next_state;
     return by_kind(layer, [&](auto type, auto n) {
-        const size_t blocks = ((size_t)a.batch * a.heads * a.channels + 63) / 64;
-        hipLaunchKernelGGL((step_kernel<decltype(type), decltype(n)::value>), dim3((unsigned)blocks), dim3(256), 0, device->stream, a);
+        typedef decltype(type) T;
+        constexpr int NPT = decltype(n)::value;
+        const dim3 blocks((unsigned)a.tiles * a.heads * ((a.batch + 3) / 4));
+        const bool whole = a.states == 4 * NPT && (reinterpret_cast<uintptr_t>(state) | reinterpret_cast<uintptr_t>(next_state)) % 16 == 0;
+        if (whole) hipLaunchKernelGGL((step_kernel<T, NPT, true>), blocks, dim3(LANES), 0, device->stream, a);
+        else hipLaunchKernelGGL((step_kernel<T, NPT, false>), blocks, dim3(LANES), 0, device->stream, a);
         return rlt_launch_status(device);
     });
 }

@@ -229,6 +229,43 @@ def test_resets_and_lengths(rocm, shape, dtype, resets):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("shape", [(1, 700, 1, 4, 16), (17, 330, 2, 7, 16), (70, 650, 1, 3, 9), (150, 340, 1, 5, 16), (40, 330, 1, 8, 25), (70, 330, 2, 4, 32)])
+@pytest.mark.parametrize("resets", [0.0, 0.1])
+def test_many_rows(rocm, shape, dtype, resets):
+    """more channels and rows than segments are made for"""
+    print("case", shape, dtype, resets, flush=True)
+    c, x = case(sum(shape), dtype, *shape, resets=resets, ragged=resets > 0)
+    if resets:      # what lies beyond a row's length is not looked at
+        beyond = np.arange(shape[0])[:, None] >= np.clip(x["lengths"], 0, shape[0])[None]
+        clean = {n: a.copy() for n, a in x.items()}
+        for i, n in enumerate(SEQUENCES):
+            x[n][beyond] = (np.nan, np.inf, -np.inf, np.nan, np.inf, -np.inf)[i]
+        check(c, clean, run(rocm, c, x))
+    else:
+        check(c, x, run(rocm, c, x))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("states", [16, 20])
+def test_many_rows_in_another_order_and_episodes_that_are_not_finite(rocm, dtype, states):
+    c, x = case(43, dtype, 90, 330, 2, 4, states)
+    check(c, x, run(rocm, c, x, order=(2, 1, 0), gap=3, offset=1))
+    x["reset"] = np.zeros((90, 330), np.uint8)
+    x["reset"][40, 0] = x["reset"][40, 2] = 1
+    want = reference(c, x)
+    b = bounds(c, x, want)
+    for i, n in enumerate(SEQUENCES):
+        x[n][38, 0] = (np.nan, np.inf, np.nan, -np.inf, np.nan, np.inf)[i]
+        x[n][45, 2] = (np.nan, np.inf, np.nan, -np.inf, np.nan, np.inf)[i]
+    got = run(rocm, c, x)
+    for n in ("output", "d_x", "d_delta", "d_b", "d_c", "d_gate"):
+        off = np.abs(got[n] - want[n]) <= b[n]
+        assert np.all(off[40:, 0]) and np.all(off[:, 1]) and np.all(off[:40, 2]) and np.all(off[:, 3:]), n
+
+
+@gpu
 @pytest.mark.parametrize("order,gap,offset", [((1, 2, 0), 0, 0), ((2, 1, 0), 0, 0), ((1, 0, 2), 8, 0), ((0, 1, 2), 5, 3), ((0, 2, 1), 1, 1)])
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 def test_orders_gaps_and_alignments(rocm, order, gap, offset, dtype):
@@ -471,6 +508,9 @@ def test_refusals(rocm):
     for call in (forward, backward):
         assert call(steps=0) == call(checkpoints=b.checkpoints.ptr + 4) == capi.RLT_E_INVALID_ARGUMENT
         assert call(steps=2 ** 30 + 1) == capi.RLT_E_UNSUPPORTED
+        far = C.byref(capi.HeadView(b.t["x"].array.ptr, 2 ** 27 + 1, 1, 1))
+        views = inputs + ([b.t["d_output"].view] + outs if call is backward else [b.o["output"].view])
+        assert all(call(views=views[:i] + [far] + views[i + 1:]) == capi.RLT_E_UNSUPPORTED for i in range(len(views)))
     assert backward(checkpoints=None) == backward(ptr=None) == backward(size=b.sizes[1] - 1) == backward(ptr=b.scratch[1].ptr + 8) == capi.RLT_E_INVALID_ARGUMENT
     assert step(state=None) == step(to=None) == capi.RLT_E_INVALID_ARGUMENT
     long = case(38, "float32", 700, 1, 1, 16, 16)
