@@ -1,5 +1,7 @@
 // Optimiser step for matrices whose updates are orthogonalised by products: A = X X^T, X <- a X + (b A + c A A) X, a few times.
 #include "typed.h"
+#include <algorithm>
+#include <vector>
 
 namespace {
 
@@ -9,39 +11,64 @@ namespace {
 typedef _Float16 f16;
 typedef f16 f16x4 __attribute__((ext_vector_type(4)));
 typedef f16 f16x8 __attribute__((ext_vector_type(8)));
+typedef rlt_f32x4 f32x4;
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 constexpr float SCALE = 16384.0f, UNSCALE = 1.0f / 16384.0f, QA = 3.4445f, QB = -4.775f, QC = 2.0315f;
 constexpr int GROUP = 24, MAX_SIDE = 1 << 16, MAX_ITERATIONS = 32, PARTS = 256;      // matrices of a launch; partial sums of a norm
+constexpr int JOBS = 768;         // workgroups of a launch whose tiles are shared, at the most
 
-struct Matrix {
+// What a launch is told: 16 bytes for each of its matrices, which a wavefront reads in one trip to where the launch left them (a row of longer entries, found and then read, was two trips of a microsecond each, a sixth of a small call's time).
+struct Entry {
+    char* scratch;                // its part of the workspace, see Matrix
+    uint16_t M, N;                // in 64s: M <= N, rows and columns, or columns and rows where there are more rows, filled up
+    int first;                    // workgroups of the launch before this matrix's
+};
+static_assert(sizeof(Entry) == 16, "");
+struct Tensor {
     const float* w; const float* g; const float* m; float* next_w; float* next_m;
-    double* sums;                 // PARTS partial sums of u^2
-    f16* x; f16* t[2]; f16* a; f16* b;      // X [M x N], its transpose [N x M] (one that is read, one that is written), A and b A + c A A [M x M]; the low parts behind the high ones
-    int rows, cols, M, N;         // M <= N: rows and columns, or columns and rows where there are more rows, filled up to whole tiles
+    int rows, cols;
     float factor;                 // alpha * sqrt(max(1, rows / cols))
 };
-struct Matrices {
-    Matrix m[GROUP];
-    int first[GROUP];             // workgroups of a launch before each matrix's
+struct Entries {
+    Entry e[GROUP];
     int n, from;                  // from: which transpose is read
-    int blocks;
-    float momentum, epsilon, keep;      // keep: 1 - alpha * weight_decay
-    int nesterov;
+    int length;                   // symmetric products: k that a workgroup adds up, a tile's others go to others
+    float* parts;                 // their sums, by workgroups
 };
-__device__ __forceinline__ const Matrix& matrix_of(const Matrices& all, int& block) {
-    const int lane = threadIdx.x & 63, i = __builtin_amdgcn_readfirstlane(__popcll(__ballot(lane < all.n && all.first[lane < GROUP ? lane : 0] <= block)) - 1);
-    block -= all.first[i];
-    return all.m[i];
+struct Tensors { Tensor t[GROUP]; float momentum, epsilon, keep; int nesterov; };      // keep: 1 - alpha * weight_decay
+struct Phases { Entries entries; };
+struct Last { Entries entries; Tensors tensors; };
+
+// X [M x N], its transpose [N x M] (one that is read, one that is written), A and b A + c A A [M x M], the low parts behind the high ones; PARTS partial sums of u^2 ahead of them
+#define GLOBAL __attribute__((address_space(1)))
+struct Matrix {
+    GLOBAL char* scratch; int M, N, index;
+    __device__ __forceinline__ size_t plane() const { return (size_t)M * N; }
+    __device__ __forceinline__ size_t square() const { return (size_t)M * M; }
+    __device__ __forceinline__ const GLOBAL double* sums() const { return (const GLOBAL double*)scratch; }
+    __device__ __forceinline__ GLOBAL f16* x() const { return (GLOBAL f16*)(scratch + PARTS * sizeof(double)); }
+    __device__ __forceinline__ GLOBAL f16* t(int which) const { return x() + (which ? 4 : 2) * plane(); }
+    __device__ __forceinline__ GLOBAL f16* a() const { return x() + 6 * plane(); }
+    __device__ __forceinline__ GLOBAL f16* b() const { return a() + 2 * square(); }
+};
+__device__ __forceinline__ Matrix matrix_of(const Entries& all, int& block) {
+    typedef int i32x4 __attribute__((ext_vector_type(4)));
+    const int lane = threadIdx.x & 63;
+    const i32x4 mine = *reinterpret_cast<const i32x4*>(&all.e[lane < GROUP ? lane : 0]);
+    const int i = __builtin_amdgcn_readfirstlane(__popcll(__ballot(lane < all.n && mine[3] <= block)) - 1);
+    const unsigned low = __builtin_amdgcn_readlane(mine[0], i), high = __builtin_amdgcn_readlane(mine[1], i), sizes = __builtin_amdgcn_readlane(mine[2], i);
+    block -= __builtin_amdgcn_readlane(mine[3], i);
+    return {(GLOBAL char*)((uint64_t)high << 32 | low), (int)(sizes & 0xFFFF) * 64, (int)(sizes >> 16) * 64, i};
 }
-// consecutive workgroups go round the XCDs: those that read the same rows to one XCD, whose L2 they share. Beyond the last: -1
-__device__ __forceinline__ int block_of(const Matrices& all) {
-    const int per = (all.blocks + 7) / 8, block = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
-    return block < all.blocks ? block : -1;
+// A matrix's tiles, of which a launch has workgroups for a multiple of eight: consecutive workgroups go round the XCDs, those that read the same rows to one XCD, whose L2 they share. Beyond the last: -1
+__device__ __forceinline__ int tile_of(int block, int tiles) {
+    const int tile = (block & 7) * ((tiles + 7) / 8) + (block >> 3);
+    return block >> 3 < (tiles + 7) / 8 && tile < tiles ? tile : -1;
 }
 __device__ __forceinline__ void split(float v, f16& high, f16& low) { high = (f16)v; low = (f16)(v - (float)high); }
 
 // The momentum, and the sum of the update's squares in 64 bits (no square of an fp32 number leaves their range). VECTORS: four elements at a time, where all buffers start on 16-byte boundaries.
-template <bool VECTORS> __device__ __forceinline__ double momentum(const Matrices& all, const Matrix& a, int part) {
+template <bool VECTORS> __device__ __forceinline__ double momentum(const Tensors& all, const Tensor& a, int part) {
     constexpr int V = VECTORS ? 4 : 1, AHEAD = 4;
     typedef float vector __attribute__((ext_vector_type(V)));
     const size_t size = (size_t)a.rows * a.cols / V, step = (size_t)PARTS * 256;
@@ -67,97 +94,272 @@ template <bool VECTORS> __device__ __forceinline__ double momentum(const Matrice
     for (; i < size; i += step) one(reinterpret_cast<const vector*>(a.g)[i], reinterpret_cast<const vector*>(a.m)[i], i);
     return s;
 }
-__global__ __launch_bounds__(256) void momentum_kernel(Matrices all) {
+__global__ __launch_bounds__(256) void momentum_kernel(Last launch) {
     __shared__ double sums[4];
-    int block = blockIdx.x;
-    const Matrix& a = matrix_of(all, block);
+    const Tensors& all = launch.tensors;
+    const int block = blockIdx.x % PARTS, matrix = blockIdx.x / PARTS;
+    const Tensor& a = all.t[matrix];
     const bool vectors = ((reinterpret_cast<uintptr_t>(a.g) | reinterpret_cast<uintptr_t>(a.m) | reinterpret_cast<uintptr_t>(a.next_m)) & 15) == 0 && (size_t)a.rows * a.cols % 4 == 0;
     double s = vectors ? momentum<true>(all, a, block) : momentum<false>(all, a, block);
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
     if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = s;
     __syncthreads();
-    if (threadIdx.x == 0) a.sums[block] = ((sums[0] + sums[1]) + sums[2]) + sums[3];
+    if (threadIdx.x == 0) ((double*)launch.entries.e[matrix].scratch)[block] = ((sums[0] + sums[1]) + sums[2]) + sums[3];
 }
 
 // X and its transpose, tiles of 64 x 64, zeros beyond the matrix
-__global__ __launch_bounds__(256) void normalise_kernel(Matrices all) {
+__global__ __launch_bounds__(256) void normalise_kernel(Last launch) {
     __shared__ float tile[64][65];
-    __shared__ double norm;
+    __shared__ double norms[4];
     int block = blockIdx.x;
-    const Matrix& a = matrix_of(all, block);
+    const Tensors& all = launch.tensors;
+    const Matrix mat = matrix_of(launch.entries, block);
+    const Tensor& a = all.t[mat.index];
     const bool tall = a.rows > a.cols;
-    const int wide = tall ? a.M : a.N, across = wide / 64, r0 = block / across * 64, c0 = block % across * 64, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    if (wave == 0) {
-        double s = 0.0;
-        for (int i = lane; i < PARTS; i += 64) s += a.sums[i];
+    const int wide = tall ? mat.M : mat.N, high = tall ? mat.N : mat.M, across = wide / 64, r0 = block / across * 64, c0 = block % across * 64, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    float g[16], m[16];
 #pragma unroll
-        for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
-        if (lane == 0) norm = sqrt(s) + (double)all.epsilon;
+    for (int i = 0; i < 16; i++) {
+        const int r = r0 + i * 4 + wave, c = c0 + lane;
+        g[i] = m[i] = 0.0f;
+        if (r < a.rows && c < a.cols) { g[i] = a.g[(size_t)r * a.cols + c]; m[i] = a.next_m[(size_t)r * a.cols + c]; }
     }
+    double s = mat.sums()[threadIdx.x];
+    static_assert(PARTS == 256, "");
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
+    if (lane == 0) norms[wave] = s;
     __syncthreads();
-    const double inverse = (double)SCALE / norm;
-    f16* const rows = tall ? a.t[0] : a.x; f16* const columns = tall ? a.x : a.t[0];
-    const size_t plane = (size_t)a.M * a.N;
-    const int high = tall ? a.N : a.M;
-#pragma unroll 4
-    for (int i = wave; i < 64; i += 4) {
-        const int r = r0 + i, c = c0 + lane;
-        float v = 0.0f;
-        if (r < a.rows && c < a.cols) {
-            const size_t e = (size_t)r * a.cols + c;
-            const float g = a.g[e], m = a.next_m[e];
-            v = (float)((double)(all.nesterov ? fmaf(all.momentum, m, g) : m) * inverse);
-        }
-        tile[i][lane] = v;
+    const double inverse = (double)SCALE / (sqrt(((norms[0] + norms[1]) + norms[2]) + norms[3]) + (double)all.epsilon);
+    GLOBAL f16* const rows = tall ? mat.t(0) : mat.x(); GLOBAL f16* const columns = tall ? mat.x() : mat.t(0);
+    const size_t plane = mat.plane();
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+        const int r = r0 + i * 4 + wave, c = c0 + lane;
+        const float v = (float)((double)(all.nesterov ? fmaf(all.momentum, m[i], g[i]) : m[i]) * inverse);
+        tile[i * 4 + wave][lane] = v;
         f16 h, l;
         split(v, h, l);
         rows[(size_t)r * wide + c] = h; rows[plane + (size_t)r * wide + c] = l;
     }
     __syncthreads();
-#pragma unroll 4
-    for (int i = wave; i < 64; i += 4) {
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
         f16 h, l;
-        split(tile[lane][i], h, l);
-        columns[(size_t)(c0 + i) * high + r0 + lane] = h; columns[plane + (size_t)(c0 + i) * high + r0 + lane] = l;
+        split(tile[lane][i * 4 + wave], h, l);
+        columns[(size_t)(c0 + i * 4 + wave) * high + r0 + lane] = h; columns[plane + (size_t)(c0 + i * 4 + wave) * high + r0 + lane] = l;
     }
 }
 
-// C[i][j] = sum over k of P[i][k] Q[j][k], both with k side by side. Four wavefronts share a tile of 64 W x 64 W, each has W x W tiles of 32 x 32. GRAM: A = X X^T; SQUARE: b A + c A A (both symmetric: tiles on and below the
-// diagonal, written twice); UPDATE: a X + (b A + c A A) X; LAST: the same, straight into the parameters. What comes from memory waits in registers for DEPTH stages of 32 k.
+// C[i][j] = sum over k of P[i][k] Q[j][k], both with k side by side. GRAM: A = X X^T; SQUARE: b A + c A A (both symmetric: tiles on and below the diagonal, written twice); UPDATE: a X + (b A + c A A) X; LAST: the same,
+// straight into the parameters.
 enum Phase { GRAM, SQUARE, UPDATE, LAST };
-template <int W> constexpr int DEPTH = W == 1 ? 4 : W == 2 ? 2 : 1;
-template <int W, int PHASE> __global__ __launch_bounds__(256, W < 3 ? 2 : 1) void product_kernel(Matrices all) {
-    constexpr int T = 64 * W, BK = 32, ROWS = 4 * T, LOADS = ROWS * 4 / 256;      // rows of the tile in LDS: P high, P low, Q high, Q low
-    extern __shared__ __attribute__((aligned(16))) f16 lds[];      // [2][ROWS][BK], chunks of eight changed about within a row so that the rows that are read together lie in different banks
-    int block = block_of(all);
-    if (block < 0) return;
-    const Matrix& a = matrix_of(all, block);
-    const bool symmetric = PHASE == GRAM || PHASE == SQUARE;
-    int ti, tj;
-    if (symmetric) {
-        ti = (int)((sqrtf(8.0f * block + 1.0f) - 1.0f) * 0.5f);
-        while (ti * (ti + 1) / 2 > block) ti--;
-        while ((ti + 1) * (ti + 2) / 2 <= block) ti++;
-        tj = block - ti * (ti + 1) / 2;
-    } else {      // eight rows of tiles at a time, column by column
-        const int down = (a.M + T - 1) / T, across = (a.N + T - 1) / T, band = block / (8 * across), rows = min(8, down - band * 8), within = block - band * 8 * across;
-        tj = within / rows; ti = band * 8 + within - tj * rows;
+template <int PHASE> constexpr bool SYMMETRIC = PHASE == GRAM || PHASE == SQUARE;
+struct Product {
+    const GLOBAL f16* P; const GLOBAL f16* Q; size_t p_plane, q_plane, square, plane;
+    int depth, q_rows, ti, tj;
+    int from, to, parts, job;     // the k of this workgroup; how many share the tile, and which of all jobs of the launch this is
+};
+template <int PHASE> struct ArgumentsOf { typedef Phases type; };
+template <> struct ArgumentsOf<LAST> { typedef Last type; };
+template <int PHASE, int T> __device__ __forceinline__ bool product_of(const Entries& all, const Matrix& a, int block, Product& p) {
+    const int down = (a.M + T - 1) / T, across = (a.N + T - 1) / T;
+    p.depth = PHASE == GRAM ? a.N : a.M;
+    p.parts = SYMMETRIC<PHASE> && T <= 128 ? (p.depth + all.length - 1) / all.length : 1;
+    int tile = tile_of(block, (SYMMETRIC<PHASE> ? down * (down + 1) / 2 : down * across) * p.parts);
+    if (tile < 0) return false;
+    p.from = 0; p.to = p.depth; p.job = (int)blockIdx.x - block + tile;
+    if (p.parts > 1) {
+        const int part = tile % p.parts;
+        tile /= p.parts;
+        p.from = part * all.length; p.to = min(p.from + all.length, p.depth);
     }
-    const int depth = PHASE == GRAM ? a.N : a.M;
-    const f16* const P = PHASE == GRAM ? a.x : PHASE == SQUARE ? a.a : a.b; const f16* const Q = PHASE == GRAM ? a.x : PHASE == SQUARE ? a.a : a.t[all.from];
-    const size_t square = (size_t)a.M * a.M, plane = (size_t)a.M * a.N, p_plane = PHASE == GRAM ? plane : square, q_plane = PHASE == SQUARE ? square : plane;
-    const int q_rows = symmetric ? a.M : a.N;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave >> 1, wj = wave & 1;
-    const int row = threadIdx.x >> 2, chunk = threadIdx.x & 3;
-    const unsigned own = (unsigned)row * depth + chunk * 8;
-    f16x8 held[DEPTH<W>][LOADS];
+    if (SYMMETRIC<PHASE>) {
+        p.ti = (int)((sqrtf(8.0f * tile + 1.0f) - 1.0f) * 0.5f);
+        while (p.ti * (p.ti + 1) / 2 > tile) p.ti--;
+        while ((p.ti + 1) * (p.ti + 2) / 2 <= tile) p.ti++;
+        p.tj = tile - p.ti * (p.ti + 1) / 2;
+    } else {      // eight rows of tiles at a time, column by column
+        const int band = tile / (8 * across), rows = min(8, down - band * 8), within = tile - band * 8 * across;
+        p.tj = within / rows; p.ti = band * 8 + within - p.tj * rows;
+    }
+    p.square = a.square(); p.plane = a.plane();
+    p.P = PHASE == GRAM ? a.x() : PHASE == SQUARE ? a.a() : a.b(); p.Q = PHASE == GRAM ? a.x() : PHASE == SQUARE ? a.a() : a.t(all.from);
+    p.p_plane = PHASE == GRAM ? p.plane : p.square; p.q_plane = PHASE == SQUARE ? p.square : p.plane;
+    p.q_rows = SYMMETRIC<PHASE> ? a.M : a.N;
+    return true;
+}
+// What the sums of a tile of 32 x 32 are added to, and where they go. A lane has column lane % 32 and, four by four, rows of it.
+template <int PHASE> __device__ __forceinline__ void addends(const Matrix& a, const Product& p, int r0, int c0, float (&v)[16]) {
+    const int lane = threadIdx.x & 63, c = c0 + (lane & 31);
+    if constexpr (PHASE != GRAM) {
+        const GLOBAL f16* const from = PHASE == SQUARE ? a.a() : a.x();
+        const unsigned width = PHASE == SQUARE ? a.M : a.N, at = ((r0 + (lane >> 5) * 4) * width + c) * sizeof(f16);      // (a plane has at most 2^30 elements: offsets of 32 bits)
+        const GLOBAL f16* const low = from + (PHASE == SQUARE ? p.square : p.plane);
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+            const unsigned row = ((e >> 2) * 8 + (e & 3)) * width * (unsigned)sizeof(f16);
+            v[e] = (float)*(const GLOBAL f16*)((const GLOBAL char*)from + (at + row)) + (float)*(const GLOBAL f16*)((const GLOBAL char*)low + (at + row));
+        }
+    }
+}
+template <int PHASE> __device__ __forceinline__ void finish(const typename ArgumentsOf<PHASE>::type& launch, const Matrix& a, const Product& p, int r0, int c0, const f32x16& sum, const float (&added)[16]) {
+    const int lane = threadIdx.x & 63, c = c0 + (lane & 31);
+#pragma unroll
+    for (int g = 0; g < 4; g++) {
+        const int r = r0 + g * 8 + (lane >> 5) * 4;
+        f16x4 high, low;
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            v[e] = sum[g * 4 + e] * UNSCALE;
+            if (PHASE == SQUARE) v[e] = fmaf(QC, v[e], QB * added[g * 4 + e]);
+            if (PHASE == UPDATE || PHASE == LAST) v[e] = fmaf(QA, added[g * 4 + e], v[e]);
+            f16 h, l;
+            split(v[e], h, l);
+            high[e] = h; low[e] = l;
+        }
+        if constexpr (PHASE == LAST) {
+            v *= UNSCALE;
+            const Tensor& t = launch.tensors.t[a.index];
+            const float keep = launch.tensors.keep;
+            if (t.rows <= t.cols) {
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (r + e < t.rows && c < t.cols) t.next_w[(size_t)(r + e) * t.cols + c] = fmaf(-t.factor, v[e], keep * t.w[(size_t)(r + e) * t.cols + c]);
+            } else if (c < t.rows) {
+                const size_t at = (size_t)c * t.cols + r;
+                typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+                if (r + 4 <= t.cols) {
+                    const f32x4 w = *reinterpret_cast<const f32x4_any*>(t.w + at);
+                    f32x4 next;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) next[e] = fmaf(-t.factor, v[e], keep * w[e]);
+                    *reinterpret_cast<f32x4_any*>(t.next_w + at) = next;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) if (r + e < t.cols) t.next_w[at + e] = fmaf(-t.factor, v[e], keep * t.w[at + e]);
+                }
+            }
+        } else {
+            GLOBAL f16* const out = PHASE == GRAM ? a.a() : PHASE == SQUARE ? a.b() : a.x();
+            const size_t behind = PHASE == UPDATE ? p.plane : p.square;
+            const unsigned width = PHASE == UPDATE ? a.N : a.M, at = (r * width + c) * (unsigned)sizeof(f16);
+            GLOBAL char* const highs = (GLOBAL char*)out; GLOBAL char* const lows = (GLOBAL char*)(out + behind);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                *(GLOBAL f16*)(highs + (at + e * width * (unsigned)sizeof(f16))) = high[e];
+                *(GLOBAL f16*)(lows + (at + e * width * (unsigned)sizeof(f16))) = low[e];
+            }
+            if (PHASE == UPDATE || p.ti != p.tj) {
+                GLOBAL f16* const t = PHASE == UPDATE ? a.t(launch.entries.from ^ 1) : out;
+                const unsigned across = (c * (unsigned)a.M + r) * (unsigned)sizeof(f16);
+                *(GLOBAL f16x4*)((GLOBAL char*)t + across) = high; *(GLOBAL f16x4*)((GLOBAL char*)(t + behind) + across) = low;
+            }
+        }
+    }
+}
+
+// A tile whose k several workgroups share: each leaves its sums, and a launch behind adds them up, in the order of k. (The last workgroup of a tile to arrive did, which a ticket told it: the releases and acquires around the tickets write back and
+// invalidate the XCDs' L2s, 30 us at 350 workgroups, where the launch costs 6.)
+template <int W> __device__ __forceinline__ float* parts_of(const Entries& all, int job) { return all.parts + (size_t)job * (64 * W) * (64 * W) + threadIdx.x * 4; }      // tiles of 32 x 32 of the wavefronts, four sums of a lane at a time
+template <int W> __device__ __forceinline__ void leave(const Entries& all, const Product& p, int i, const f32x16& v) {
+    float* const to = parts_of<W>(all, p.job) + i * 4096;
+#pragma unroll
+    for (int e = 0; e < 4; e++) *reinterpret_cast<f32x4*>(to + e * 1024) = f32x4{v[e * 4], v[e * 4 + 1], v[e * 4 + 2], v[e * 4 + 3]};
+}
+template <int W> __device__ __forceinline__ f32x16 joined(const Entries& all, const Product& p, int i) {
+    const float* from = parts_of<W>(all, p.job) + i * 4096;
+    f32x16 total;
+#pragma unroll
+    for (int e = 0; e < 16; e++) total[e] = 0.0f;
+    for (int part = 0; part < p.parts; part++, from += (64 * W) * (64 * W)) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const f32x4 v = *reinterpret_cast<const f32x4*>(from + e * 1024);
+#pragma unroll
+            for (int n = 0; n < 4; n++) total[e * 4 + n] += v[n];
+        }
+    }
+    return total;
+}
+
+// Tiles of 64 x 64, for few of them: a launch is bound by trips to memory then. What 128 k need is on its way ahead, what the sums are added to with it; four wavefronts have 32 x 32 of the tile each, factors come through LDS in stages of
+// 64 k, and the three kinds of products have sums of their own, which are joined at the end: a chain of dependent matrix instructions is a third as long.
+template <int PHASE> __global__ __launch_bounds__(256, SYMMETRIC<PHASE> ? 2 : 1) void product_small_kernel(typename ArgumentsOf<PHASE>::type launch) {
+    constexpr int BK = 64, LOADS = 8, DEPTH = 2;
+    __shared__ __attribute__((aligned(16))) f16 lds[2][256 * BK];      // rows of P high, P low, Q high, Q low; chunks of eight changed about within a row
+    int block = blockIdx.x;
+    const Matrix a = matrix_of(launch.entries, block);
+    Product p;
+    if (!product_of<PHASE, 64>(launch.entries, a, block, p)) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = threadIdx.x >> 3, chunk = threadIdx.x & 7, r0 = p.ti * 64 + (wave >> 1) * 32, c0 = p.tj * 64 + (wave & 1) * 32;
+    const GLOBAL char* const p0 = (const GLOBAL char*)(p.P + (size_t)p.ti * 64 * p.depth); const GLOBAL char* const q0 = (const GLOBAL char*)(p.Q + (size_t)p.tj * 64 * p.depth);
+    const unsigned own = (row * p.depth + chunk * 8) * (unsigned)sizeof(f16);
+    f16x8 held[DEPTH][LOADS];
     auto ask = [&](int k, f16x8 (&to)[LOADS]) {
 #pragma unroll
+        for (int i = 0; i < LOADS; i++)
+            to[i] = *(const GLOBAL f16x8*)((i < 4 ? p0 + (i >> 1 & 1) * p.p_plane * sizeof(f16) : q0 + (i >> 1 & 1) * p.q_plane * sizeof(f16)) + ((size_t)(i & 1) * 32 * p.depth + k) * sizeof(f16) + own);
+    };
+#pragma unroll
+    for (int d = 0; d < DEPTH; d++) ask(min(p.from + d * BK, p.to - BK), held[d]);      // (the last stage again where there are no more: a branch around a load waits for it)
+    float added[16];
+    addends<PHASE>(a, p, r0, c0, added);
+    f32x16 sum[3];
+#pragma unroll
+    for (int i = 0; i < 3; i++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) sum[i][e] = 0.0f;
+#pragma unroll 1
+    for (int k0 = p.from; k0 < p.to; k0 += DEPTH * BK) {
+#pragma unroll
+        for (int d = 0; d < DEPTH; d++) {
+            const int k = k0 + d * BK;
+            if (k >= p.to) break;
+            f16* const to = lds[d & 1];
+#pragma unroll
+            for (int i = 0; i < LOADS; i++) *reinterpret_cast<f16x8*>(to + (i * 32 + row) * BK + (chunk ^ (row & 7)) * 8) = held[d][i];
+            ask(min(k + DEPTH * BK, p.to - BK), held[d]);
+            rlt_lds_barrier();
+#pragma unroll
+            for (int kk = 0; kk < BK / 16; kk++) {
+                auto fragment = [&](int part, int half) {
+                    const int r = part * 64 + half * 32 + (lane & 31);
+                    return *reinterpret_cast<const f16x8*>(to + r * BK + ((kk * 2 + (lane >> 5)) ^ (r & 7)) * 8);
+                };
+                const f16x8 ph = fragment(0, wave >> 1), pl = fragment(1, wave >> 1), qh = fragment(2, wave & 1), ql = fragment(3, wave & 1);
+                sum[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, qh, sum[0], 0, 0, 0);
+                sum[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, ql, sum[1], 0, 0, 0);
+                sum[2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl, qh, sum[2], 0, 0, 0);
+            }
+        }
+    }
+    f32x16 total = sum[0] + (sum[1] + sum[2]);
+    if (p.parts > 1) { leave<1>(launch.entries, p, 0, total); return; }
+    finish<PHASE>(launch, a, p, r0, c0, total, added);
+}
+
+// Tiles of 64 W x 64 W: four wavefronts share one, each has W x W tiles of 32 x 32, factors come through LDS in stages of 32 k. Half a stage ahead: while the products of one half run, the other half's factors come from LDS, the next stage's go there
+// and the one after that is asked for, dealt out between the matrix instructions. 256 x 256: 1,054 TFLOP/s of 16-bit products at 4,096 x 20,480 x 4,096 (the clock is down to 1.7 GHz by then; a large library product: 1,080), 867 without that order.
+template <int W, int PHASE> __global__ __launch_bounds__(256, W < 3 ? 2 : 1) void product_kernel(typename ArgumentsOf<PHASE>::type launch) {
+    constexpr int T = 64 * W, BK = 32, ROWS = 4 * T, LOADS = ROWS * 4 / 256, PRODUCTS = 3 * W * W, READS = 4 * W;      // rows of the tile in LDS: P high, P low, Q high, Q low
+    extern __shared__ __attribute__((aligned(16))) f16 lds[];      // [2][ROWS][BK], chunks of eight changed about within a row so that the rows that are read together lie in different banks
+    int block = blockIdx.x;
+    const Matrix a = matrix_of(launch.entries, block);
+    Product p;
+    if (!product_of<PHASE, T>(launch.entries, a, block, p)) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave >> 1, wj = wave & 1;
+    const int row = threadIdx.x >> 2, chunk = threadIdx.x & 3;
+    const unsigned own = (row * p.depth + chunk * 8) * (unsigned)sizeof(f16);
+    f16x8 held[LOADS];
+    auto ask = [&](int k) {
+#pragma unroll
         for (int i = 0; i < LOADS; i++) {
-            const int part = i / W, down = (part < 2 ? ti : tj) * T + i % W * 64, at_row = down < (part < 2 ? a.M : q_rows) ? down : 0;      // rows beyond the matrix: any that are there, nobody reads their sums
-            const f16* const from = (part < 2 ? P + (part & 1) * p_plane : Q + (part & 1) * q_plane) + (size_t)at_row * depth + k;
-            to[i] = *reinterpret_cast<const f16x8*>(from + own);
+            const int part = i / W, down = (part < 2 ? p.ti : p.tj) * T + i % W * 64, at_row = down < (part < 2 ? a.M : p.q_rows) ? down : 0;      // rows beyond the matrix: any that are there, nobody reads their sums
+            const GLOBAL f16* const from = (part < 2 ? p.P + (part & 1) * p.p_plane : p.Q + (part & 1) * p.q_plane) + (size_t)at_row * p.depth + k;
+            held[i] = *(const GLOBAL f16x8*)((const GLOBAL char*)from + own);
         }
     };
     f32x16 sum[W][W];
@@ -167,90 +369,112 @@ template <int W, int PHASE> __global__ __launch_bounds__(256, W < 3 ? 2 : 1) voi
         for (int j = 0; j < W; j++)
 #pragma unroll
             for (int e = 0; e < 16; e++) sum[i][j][e] = 0.0f;
-    auto multiply = [&](const f16* from) {
+    struct Fragments { f16x8 ph[W], pl[W], qh[W], ql[W]; };
+    auto read = [&](const f16* from, int kk, Fragments& f) {
+        auto fragment = [&](int part, int tile) {
+            const int r = part * T + tile * 32 + (lane & 31);
+            return *reinterpret_cast<const f16x8*>(from + r * BK + ((kk * 2 + (lane >> 5)) ^ (r >> 1 & 3)) * 8);
+        };
 #pragma unroll
-        for (int kk = 0; kk < BK / 16; kk++) {
-            auto fragment = [&](int part, int tile) {
-                const int r = part * T + tile * 32 + (lane & 31);
-                return *reinterpret_cast<const f16x8*>(from + r * BK + ((kk * 2 + (lane >> 5)) ^ (r >> 1 & 3)) * 8);
-            };
-            f16x8 ph[W], pl[W], qh[W], ql[W];
+        for (int i = 0; i < W; i++) {
+            f.ph[i] = fragment(0, wi * W + i); f.pl[i] = fragment(1, wi * W + i);
+            f.qh[i] = fragment(2, wj * W + i); f.ql[i] = fragment(3, wj * W + i);
+        }
+    };
+    auto multiply = [&](const Fragments& f) {      // sums that follow each other in the matrix pipeline are not the same
 #pragma unroll
-            for (int i = 0; i < W; i++) {
-                ph[i] = fragment(0, wi * W + i); pl[i] = fragment(1, wi * W + i);
-                qh[i] = fragment(2, wj * W + i); ql[i] = fragment(3, wj * W + i);
-            }
+        for (int term = 0; term < 3; term++)
 #pragma unroll
             for (int i = 0; i < W; i++)
 #pragma unroll
-                for (int j = 0; j < W; j++) {
-                    sum[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl[i], qh[j], sum[i][j], 0, 0, 0);
-                    sum[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[i], ql[j], sum[i][j], 0, 0, 0);
-                    sum[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[i], qh[j], sum[i][j], 0, 0, 0);
-                }
+                for (int j = 0; j < W; j++) sum[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(term == 0 ? f.pl[i] : f.ph[i], term == 1 ? f.ql[j] : f.qh[j], sum[i][j], 0, 0, 0);
+    };
+    auto put = [&](f16* to) {
+#pragma unroll
+        for (int i = 0; i < LOADS; i++) {
+            const int r = i * 64 + row;
+            *reinterpret_cast<f16x8*>(to + r * BK + (chunk ^ (r >> 1 & 3)) * 8) = held[i];
         }
     };
+    f16* here = lds; f16* there = lds + ROWS * BK;
+    Fragments first, second;
+    ask(p.from);
+    put(here);
+    ask(p.from + BK);
+    rlt_lds_barrier();
+    read(here, 0, first);
+    const int stages = (p.to - p.from) / BK;      // two at the least
+    for (int s = 0; s + 1 < stages; s++) {
+        read(here, 1, second);
+        multiply(first);
+        put(there);
+        ask(p.from + min(s + 2, stages - 1) * BK);
 #pragma unroll
-    for (int d = 0; d < DEPTH<W>; d++) if (d * BK < depth) ask(d * BK, held[d]);
-    int turn = 0;
-    for (int k0 = 0; k0 < depth; k0 += DEPTH<W> * BK) {
+        for (int i = 0; i < READS; i++) { __builtin_amdgcn_sched_group_barrier(0x100, 1, 0); __builtin_amdgcn_sched_group_barrier(0x8, 1, 0); }
+        constexpr int LEFT = PRODUCTS > READS ? (PRODUCTS - READS) / LOADS : 0;
 #pragma unroll
-        for (int d = 0; d < DEPTH<W>; d++) {
-            const int k = k0 + d * BK;
-            if (k >= depth) break;
-            f16* const to = lds + turn * ROWS * BK;
+        for (int i = 0; i < LOADS; i++) {
+            __builtin_amdgcn_sched_group_barrier(0x200, 1, 0); __builtin_amdgcn_sched_group_barrier(0x20, 1, 0);
+            if (LEFT) __builtin_amdgcn_sched_group_barrier(0x8, LEFT, 0);
+        }
+        rlt_lds_barrier();
+        read(there, 0, first);
+        multiply(second);
 #pragma unroll
-            for (int i = 0; i < LOADS; i++) {
-                const int r = i * 64 + row;
-                *reinterpret_cast<f16x8*>(to + r * BK + (chunk ^ (r >> 1 & 3)) * 8) = held[d][i];
-            }
-            if (k + DEPTH<W> * BK < depth) ask(k + DEPTH<W> * BK, held[d]);
-            rlt_lds_barrier();
-            multiply(to);
-            turn ^= 1;
+        for (int i = 0; i < READS; i++) { __builtin_amdgcn_sched_group_barrier(0x8, 1, 0); __builtin_amdgcn_sched_group_barrier(0x100, 1, 0); }
+        f16* const t = here; here = there; there = t;
+    }
+    read(here, 1, second);
+    multiply(first);
+    multiply(second);
+    if constexpr (W == 2 && SYMMETRIC<PHASE>) {
+        if (p.parts > 1) {
+#pragma unroll
+            for (int i = 0; i < W * W; i++) leave<W>(launch.entries, p, i, sum[i / W][i % W]);
+            return;
         }
     }
-    // a lane has column lane % 32 and, four by four, rows of its tiles
+    // sums go through LDS, a row of tiles at a time: one copy of what is done with a tile, whose needs are no more than a tile's
+    rlt_lds_barrier();
+    f32x4* const kept = reinterpret_cast<f32x4*>(lds) + wave * W * 256 + lane;
 #pragma unroll
-    for (int i = 0; i < W; i++)
+    for (int i = 0; i < W; i++) {
 #pragma unroll
+        for (int j = 0; j < W; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) kept[j * 256 + e * 64] = f32x4{sum[i][j][e * 4], sum[i][j][e * 4 + 1], sum[i][j][e * 4 + 2], sum[i][j][e * 4 + 3]};
+#pragma unroll 1
         for (int j = 0; j < W; j++) {
-            const int c = tj * T + (wj * W + j) * 32 + (lane & 31);
-            if (ti * T + (wi * W + i) * 32 >= a.M || tj * T + (wj * W + j) * 32 >= q_rows) continue;
+            const int r0 = p.ti * T + (wi * W + i) * 32, c0 = p.tj * T + (wj * W + j) * 32;
+            if (r0 >= a.M || c0 >= p.q_rows) continue;
+            f32x16 total;
+            float added[16];
+            addends<PHASE>(a, p, r0, c0, added);
 #pragma unroll
-            for (int g = 0; g < 4; g++) {
-                const int r = ti * T + (wi * W + i) * 32 + g * 8 + (lane >> 5) * 4;
-                f16x4 high, low;
-                float v[4];
+            for (int e = 0; e < 4; e++) {
+                const f32x4 v = kept[j * 256 + e * 64];
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    v[e] = sum[i][j][g * 4 + e] * UNSCALE;
-                    if (PHASE == SQUARE) v[e] = fmaf(QC, v[e], QB * ((float)a.a[(size_t)(r + e) * a.M + c] + (float)a.a[square + (size_t)(r + e) * a.M + c]));
-                    if (PHASE == UPDATE || PHASE == LAST) v[e] = fmaf(QA, (float)a.x[(size_t)(r + e) * a.N + c] + (float)a.x[plane + (size_t)(r + e) * a.N + c], v[e]);
-                    f16 h, l;
-                    split(v[e], h, l);
-                    high[e] = h; low[e] = l;
-                }
-                if (PHASE == LAST) {
-                    const bool tall = a.rows > a.cols;
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const int wr = tall ? c : r + e, wc = tall ? r + e : c;
-                        if (wr < a.rows && wc < a.cols) a.next_w[(size_t)wr * a.cols + wc] = fmaf(-a.factor, v[e] * UNSCALE, all.keep * a.w[(size_t)wr * a.cols + wc]);
-                    }
-                } else if (PHASE == UPDATE) {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) { a.x[(size_t)(r + e) * a.N + c] = high[e]; a.x[plane + (size_t)(r + e) * a.N + c] = low[e]; }
-                    f16* const t = a.t[all.from ^ 1] + (size_t)c * a.M + r;
-                    *reinterpret_cast<f16x4*>(t) = high; *reinterpret_cast<f16x4*>(t + plane) = low;
-                } else {
-                    f16* const out = PHASE == GRAM ? a.a : a.b;
-#pragma unroll
-                    for (int e = 0; e < 4; e++) { out[(size_t)(r + e) * a.M + c] = high[e]; out[square + (size_t)(r + e) * a.M + c] = low[e]; }
-                    if (ti != tj) { *reinterpret_cast<f16x4*>(out + (size_t)c * a.M + r) = high; *reinterpret_cast<f16x4*>(out + square + (size_t)c * a.M + r) = low; }
-                }
+                for (int n = 0; n < 4; n++) total[e * 4 + n] = v[n];
             }
+            finish<PHASE>(launch, a, p, r0, c0, total, added);
         }
+    }
+}
+
+// the sums of tiles that workgroups shared: a workgroup for every tile of 32 x 32 of each wavefront
+template <int W, int PHASE> __global__ __launch_bounds__(256) void join_kernel(Phases launch) {
+    int block = blockIdx.x / (W * W);
+    const int i = blockIdx.x % (W * W), job = block, wave = threadIdx.x >> 6;
+    const Matrix a = matrix_of(launch.entries, block);
+    Product p;
+    if (!product_of<PHASE, 64 * W>(launch.entries, a, block, p) || p.parts == 1 || p.from) return;      // (the job of a tile's first k stands for the tile)
+    const int r0 = p.ti * 64 * W + ((wave >> 1) * W + i / W) * 32, c0 = p.tj * 64 * W + ((wave & 1) * W + i % W) * 32;
+    if (r0 >= a.M || c0 >= p.q_rows) return;
+    p.job += job - (int)blockIdx.x;
+    float added[16];
+    addends<PHASE>(a, p, r0, c0, added);
+    const f32x16 total = joined<W>(launch.entries, p, i);
+    finish<PHASE>(launch, a, p, r0, c0, total, added);
 }
 
 bool described(const rlt_muon_tensor* t, int n) {
@@ -262,52 +486,105 @@ bool supported(const rlt_muon_tensor* t, int n) {
     for (int i = 0; i < n; i++) if (t[i].rows > MAX_SIDE || t[i].cols > MAX_SIDE || (int64_t)t[i].rows * t[i].cols > 1 << 30) return false;
     return true;
 }
+constexpr size_t SHARED_BYTES = (size_t)JOBS / 2 * 128 * 128 * sizeof(float);      // of jobs that share tiles: half of JOBS of 128 x 128, or JOBS of 64 x 64
 int filled(int n) { return (n + 63) / 64 * 64; }
 size_t bytes_of(const rlt_muon_tensor& t) {
     const size_t M = filled(t.rows < t.cols ? t.rows : t.cols), N = filled(t.rows < t.cols ? t.cols : t.rows);
     return PARTS * sizeof(double) + (6 * M * N + 4 * M * M) * sizeof(f16);
 }
-template <int W, int PHASE> size_t tiles_of(const Matrix& m) {
-    const size_t down = (m.M + 64 * W - 1) / (64 * W), across = (m.N + 64 * W - 1) / (64 * W);
-    return PHASE == GRAM || PHASE == SQUARE ? down * (down + 1) / 2 : down * across;
+template <int W, int PHASE> size_t tiles_of(const Entry& m) {
+    const size_t down = (m.M + W - 1) / W, across = (m.N + W - 1) / W;
+    return SYMMETRIC<PHASE> ? down * (down + 1) / 2 : down * across;
 }
-template <int W, int PHASE> size_t tiles_of(const Matrices& all) {
+template <int W, int PHASE> size_t tiles_of(const Entries& all) {
     size_t n = 0;
-    for (int i = 0; i < all.n; i++) n += tiles_of<W, PHASE>(all.m[i]);
+    for (int i = 0; i < all.n; i++) n += tiles_of<W, PHASE>(all.e[i]);
     return n;
 }
-template <int W, int PHASE> int launch_width(rlt_rocm_device* device, Matrices& all) {
+int depth_of(const Entry& m, int phase) { return 64 * (phase == GRAM ? m.N : m.M); }
+// Jobs of a launch whose tiles are shared out in lengths of `length` k. Lengths are 512 at the least, where a launch more is worth it, and leave no more than JOBS jobs (GRAM of 88 tiles of 128 x 128, up to 2,048 k: 49 us as they are, 22 shared)
+template <int W, int PHASE> size_t jobs_of(const Entries& all, int length) {
+    size_t n = 0;
+    for (int i = 0; i < all.n; i++) n += (tiles_of<W, PHASE>(all.e[i]) * ((depth_of(all.e[i], PHASE) + length - 1) / length) + 7) / 8 * 8;
+    return n;
+}
+int deepest_of(const Entries& all, int phase) {
+    int deepest = 0;
+    for (int i = 0; i < all.n; i++) deepest = std::max(deepest, depth_of(all.e[i], phase));
+    return deepest;
+}
+constexpr int WHOLE = 1 << 30;
+template <int W, int PHASE> int length_of(const Entries& all) {
+    if (W > 2 || !SYMMETRIC<PHASE>) return WHOLE;
+    const int deepest = deepest_of(all, PHASE);
+    for (int length = 512; length < deepest; length *= 2)
+        if (jobs_of<W, PHASE>(all, length) <= (W == 1 ? JOBS : JOBS / 2)) return length;
+    return WHOLE;
+}
+// Microseconds that a launch takes, round by round of 256 tiles: for 512 k of a tile with few others, with one on every compute unit, and for its sums' way out.
+template <int W, int PHASE> double cost_of(const Entries& all) {
+    constexpr double few[5] = {0, 5.5, 12, 15, 24}, full[5] = {0, 6.5, 14, 27, 46}, out[5] = {0, 3, 6, 28, 23};
+    const int length = length_of<W, PHASE>(all);
+    double cost = length == WHOLE ? 0.0 : 6.0;
+    size_t jobs = 0, in_round = 0;
+    int deepest = 0;
+    auto round = [&] { cost += deepest / 512.0 * (few[W] + (full[W] - few[W]) * in_round / 256.0) + out[W]; in_round = 0; deepest = 0; };
+    for (int i = 0; i < all.n; i++) {
+        const int depth = depth_of(all.e[i], PHASE);
+        for (jobs = tiles_of<W, PHASE>(all.e[i]) * ((depth + length - 1) / length); jobs; ) {
+            const size_t taken = std::min(jobs, 256 - in_round);
+            jobs -= taken; in_round += taken; deepest = std::max(deepest, std::min(depth, length));
+            if (in_round == 256) round();
+        }
+    }
+    if (in_round) round();
+    return cost;
+}
+template <int W, int PHASE> int launch_width(rlt_rocm_device* device, typename ArgumentsOf<PHASE>::type all) {
     size_t blocks = 0;
-    for (int i = 0; i < all.n; i++) { all.first[i] = (int)blocks; blocks += tiles_of<W, PHASE>(all.m[i]); }
-    all.blocks = (int)blocks;
-    const auto kernel = product_kernel<W, PHASE>;
-    const int bytes = 2 * 4 * 64 * W * 32 * (int)sizeof(f16);
-    RLT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(blocks + 7) / 8 * 8), dim3(256), bytes, device->stream, all);
+    Entries& entries = all.entries;
+    entries.length = length_of<W, PHASE>(entries);
+    for (int i = 0; i < entries.n; i++) {
+        const size_t parts = SYMMETRIC<PHASE> ? (depth_of(entries.e[i], PHASE) + entries.length - 1) / entries.length : 1;
+        entries.e[i].first = (int)blocks;
+        blocks += (tiles_of<W, PHASE>(entries.e[i]) * parts + 7) / 8 * 8;
+    }
+    if constexpr (W == 1) hipLaunchKernelGGL((product_small_kernel<PHASE>), dim3((unsigned)blocks), dim3(256), 0, device->stream, all);
+    else {
+        const auto kernel = product_kernel<W, PHASE>;
+        const int bytes = 2 * 4 * 64 * W * 32 * (int)sizeof(f16);
+        RLT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), bytes, device->stream, all);
+    }
+    if constexpr (W <= 2 && SYMMETRIC<PHASE>) {
+        if (entries.length != WHOLE) {
+            const int rc = rlt_launch_status(device);
+            if (rc) return rc;
+            hipLaunchKernelGGL((join_kernel<W, PHASE>), dim3((unsigned)blocks * W * W), dim3(256), 0, device->stream, all);
+        }
+    }
     return rlt_launch_status(device);
 }
-// Tiles as wide as leave the fewest rounds over the compute units, a round's time as measured per tile.
-template <int PHASE> int launch(rlt_rocm_device* device, Matrices& all) {
-    const size_t units = device->compute_units > 0 ? device->compute_units : 256;
-    auto rounds = [&](size_t tiles) { return (double)((tiles + units - 1) / units); };
-    const double cost[4] = {rounds(tiles_of<1, PHASE>(all)) * 2.5, rounds(tiles_of<2, PHASE>(all)) * 6.2, rounds(tiles_of<3, PHASE>(all)) * 11.3, rounds(tiles_of<4, PHASE>(all)) * 18.8};
-    int best = 0;
-    for (int i = 1; i < 4; i++) if (cost[i] < cost[best]) best = i;
+template <int PHASE> int launch(rlt_rocm_device* device, const typename ArgumentsOf<PHASE>::type& all) {
+    const Entries& e = all.entries;
+    const double cost[4] = {cost_of<1, PHASE>(e), cost_of<2, PHASE>(e), cost_of<3, PHASE>(e), cost_of<4, PHASE>(e)};
+    const int best = (int)(std::min_element(cost, cost + 4) - cost);
     return best == 0 ? launch_width<1, PHASE>(device, all) : best == 1 ? launch_width<2, PHASE>(device, all) : best == 2 ? launch_width<3, PHASE>(device, all) : launch_width<4, PHASE>(device, all);
 }
-int run(rlt_rocm_device* device, Matrices& all, int iterations) {
+int run(rlt_rocm_device* device, Last& all, int iterations) {
     size_t tiles = 0;
-    for (int i = 0; i < all.n; i++) all.first[i] = i * PARTS;
-    hipLaunchKernelGGL(momentum_kernel, dim3(all.n * PARTS), dim3(256), 0, device->stream, all);
+    Entries& e = all.entries;
+    hipLaunchKernelGGL(momentum_kernel, dim3(e.n * PARTS), dim3(256), 0, device->stream, all);
     int rc = rlt_launch_status(device);
     if (rc) return rc;
-    for (int i = 0; i < all.n; i++) { all.first[i] = (int)tiles; tiles += (size_t)all.m[i].M / 64 * (all.m[i].N / 64); }
+    for (int i = 0; i < e.n; i++) { e.e[i].first = (int)tiles; tiles += (size_t)e.e[i].M * e.e[i].N; }
     hipLaunchKernelGGL(normalise_kernel, dim3((unsigned)tiles), dim3(256), 0, device->stream, all);
     if ((rc = rlt_launch_status(device))) return rc;
-    all.from = 0;
-    for (int k = 0; k < iterations; k++, all.from ^= 1) {
-        if ((rc = launch<GRAM>(device, all)) || (rc = launch<SQUARE>(device, all))) return rc;
-        if ((rc = k + 1 < iterations ? launch<UPDATE>(device, all) : launch<LAST>(device, all))) return rc;
+    e.from = 0;
+    for (int k = 0; k < iterations; k++, e.from ^= 1) {
+        const Phases phases = {e};
+        if ((rc = launch<GRAM>(device, phases)) || (rc = launch<SQUARE>(device, phases))) return rc;
+        if ((rc = k + 1 < iterations ? launch<UPDATE>(device, phases) : launch<LAST>(device, all))) return rc;
     }
     return 0;
 }
@@ -320,7 +597,7 @@ size_t rlt_rocm_muon_workspace_bytes(const rlt_muon_tensor* tensors, int n) {
     if (!described(tensors, n) || !supported(tensors, n)) return 0;
     size_t bytes = 0;
     for (int i = 0; i < n; i++) bytes += bytes_of(tensors[i]);
-    return bytes;
+    return bytes + SHARED_BYTES;
 }
 
 int rlt_rocm_muon_step(rlt_rocm_device* device, const rlt_muon_tensor* tensors, int n, const rlt_muon_parameters* parameters, void* workspace, size_t workspace_bytes) {
@@ -335,23 +612,24 @@ int rlt_rocm_muon_step(rlt_rocm_device* device, const rlt_muon_tensor* tensors, 
     if (!supported(tensors, n)) return RLT_E_UNSUPPORTED;
     RLT_REQUIRE(workspace && workspace_bytes >= rlt_rocm_muon_workspace_bytes(tensors, n) && reinterpret_cast<uintptr_t>(workspace) % 16 == 0);
     char* at = (char*)workspace;
-    Matrices all{};
-    all.momentum = parameters->momentum; all.epsilon = parameters->epsilon; all.keep = 1.0f - parameters->alpha * parameters->weight_decay; all.nesterov = parameters->nesterov;
+    std::vector<int> order(n);
+    for (int i = 0; i < n; i++) order[i] = i;
+    auto size = [&](int i) { return (int64_t)tensors[i].rows * tensors[i].cols; };
+    std::stable_sort(order.begin(), order.end(), [&](int i, int j) { return size(i) > size(j); });      // the longest products of a launch first
+    Last all{};
+    all.entries.parts = (float*)at;
+    at += SHARED_BYTES;
+    all.tensors.momentum = parameters->momentum; all.tensors.epsilon = parameters->epsilon; all.tensors.keep = 1.0f - parameters->alpha * parameters->weight_decay; all.tensors.nesterov = parameters->nesterov;
     for (int i = 0; i < n; i++) {
-        const rlt_muon_tensor& t = tensors[i];
-        Matrix& m = all.m[all.n++];
-        m.w = t.parameters; m.g = t.gradient; m.m = t.momentum; m.next_w = t.next_parameters; m.next_m = t.next_momentum;
-        m.rows = t.rows; m.cols = t.cols; m.M = filled(t.rows < t.cols ? t.rows : t.cols); m.N = filled(t.rows < t.cols ? t.cols : t.rows);
-        m.factor = parameters->alpha * sqrtf(t.rows > t.cols ? (float)t.rows / t.cols : 1.0f);
-        const size_t plane = (size_t)m.M * m.N, square = (size_t)m.M * m.M;
-        m.sums = (double*)at; at += PARTS * sizeof(double);
-        f16* const p = (f16*)at;
-        m.x = p; m.t[0] = p + 2 * plane; m.t[1] = p + 4 * plane; m.a = p + 6 * plane; m.b = m.a + 2 * square;
-        at = (char*)(m.b + 2 * square);
-        if (all.n == GROUP || i == n - 1) {
+        const rlt_muon_tensor& t = tensors[order[i]];
+        const int low = t.rows < t.cols ? t.rows : t.cols, high = t.rows < t.cols ? t.cols : t.rows;
+        all.entries.e[all.entries.n] = {at, (uint16_t)(filled(low) / 64), (uint16_t)(filled(high) / 64), 0};
+        all.tensors.t[all.entries.n++] = {t.parameters, t.gradient, t.momentum, t.next_parameters, t.next_momentum, t.rows, t.cols, parameters->alpha * sqrtf(t.rows > t.cols ? (float)t.rows / t.cols : 1.0f)};
+        at += bytes_of(t);
+        if (all.entries.n == GROUP || i == n - 1) {
             const int rc = run(device, all, parameters->iterations);
             if (rc) return rc;
-            all.n = 0;
+            all.entries.n = 0;
         }
     }
     return 0;
