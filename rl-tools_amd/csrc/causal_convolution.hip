@@ -5,7 +5,6 @@
 namespace {
 
 constexpr int MAX_STEPS = 1 << 30, MAX_SIDE = 1 << 24, MIN_WIDTH = 2, MAX_WIDTH = 8;
-constexpr int UNROLL = 8;         // steps whose inputs are asked for together
 
 struct Convolution {
     const float* weights; const float* biases;
@@ -59,15 +58,42 @@ template <int W, int V> __device__ __forceinline__ void load_weights(const Convo
     }
 }
 // sum over the taps that the episode has
-template <int W, int V> __device__ __forceinline__ void taps(const float (&w)[W][V], const float (&bias)[V], const float (&x)[V], const float (&window)[W - 1][V], int age, float (&z)[V]) {
+template <int W, int V, bool RESETS> __device__ __forceinline__ void taps(const float (&w)[W][V], const float (&bias)[V], const float (&x)[V], const float (&window)[W - 1][V], int age, float (&z)[V]) {
 #pragma unroll
     for (int i = 0; i < V; i++) {
         z[i] = bias[i];
 #pragma unroll
-        for (int j = W - 1; j > 0; j--) z[i] = age >= j ? fmaf(w[j][i], window[j - 1][i], z[i]) : z[i];
+        for (int j = W - 1; j > 0; j--) z[i] = !RESETS || age >= j ? fmaf(w[j][i], window[j - 1][i], z[i]) : z[i];
         z[i] = fmaf(w[0][i], x[i], z[i]);
     }
 }
+// 1 / (1 + e^-z), and what it leaves to one. bfloat16 tensors do without what the rounding of the exponent drops, |z| 2^-25 of the sigmoid, a thousandth of their own rounding at z = -64; the instructions' own
+// errors are 2^-23 of it (the forward pass at 8,192 x 4 x 2,048: 72 us with them, 61 without)
+template <typename T> __device__ __forceinline__ void sigmoids(float z, float& s, float& other) {
+    if constexpr (sizeof(T) == sizeof(float)) rlt_sigmoids(z, s, other);
+    else {
+        s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504088896341f));
+        other = 1.0f - s;
+    }
+}
+template <typename T, int V> __device__ __forceinline__ void activate(float (&z)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        float s, other;
+        sigmoids<T>(z[i], s, other);
+        z[i] *= s;
+    }
+}
+// V elements as they lie in memory
+template <typename T, int V> struct Raw {
+    typedef T vector __attribute__((ext_vector_type(V)));
+    vector v;
+    __device__ __forceinline__ void load(const T* from) { if constexpr (V == 1) v = vector(*from); else v = *reinterpret_cast<const vector*>(from); }
+    __device__ __forceinline__ void unpack(float (&to)[V]) const {
+#pragma unroll
+        for (int i = 0; i < V; i++) to[i] = (float)v[i];
+    }
+};
 template <int W, int V> __device__ __forceinline__ void shift(float (&window)[W - 1][V], const float (&x)[V]) {
 #pragma unroll
     for (int i = 0; i < V; i++) {
@@ -83,8 +109,9 @@ template <int W, int V> __device__ __forceinline__ void store_state(float* state
         for (int i = 0; i < V; i++) state[((size_t)row * (W - 1) + W - 2 - j) * channels + channel + i] = age > j ? window[j][i] : 0.0f;
 }
 
-// Memory bounds it: each input once (and the window ahead of a segment again), each output once.
-template <typename T, int W, int V> __global__ __launch_bounds__(256) void forward_kernel(Convolution a) {
+// Memory bounds it: each input once (and the window ahead of a segment again), each output once. Eight steps' inputs are on their way while those of the eight before them are worked on.
+template <typename T, int W, int V, bool RESETS> __global__ __launch_bounds__(256) void forward_kernel(Convolution a) {
+    constexpr int U = 8;
     const Place p = place_of<V>(a);
     if (!p.there) return;
     const int first = p.segment * a.segment_steps, end = min(first + a.segment_steps, a.steps), length = a.lengths ? min(max(a.lengths[p.row], 0), a.steps) : a.steps, live = min(end, length);
@@ -92,44 +119,56 @@ template <typename T, int W, int V> __global__ __launch_bounds__(256) void forwa
     load_weights<W, V>(a, p.channel, w, bias);
     int age = W - 1;
     if (first <= length) {
-        age = age_of<W>(a, first, p.row);
+        if (RESETS) age = age_of<W>(a, first, p.row);
         load_window<T, W, V>(a, first, p.row, p.channel, window);
     }
+    const T* from = at<T>(a.x, first, p.row, p.channel); T* to = at<T>(a.out, first, p.row, p.channel);
+    const uint8_t* flags = RESETS ? a.reset + (size_t)first * a.batch + p.row : nullptr;
+    auto step = [&](const Raw<T, V>& raw, bool begins) {
+        float x[V], z[V];
+        raw.unpack(x);
+        if (RESETS && begins) age = 0;
+        taps<W, V, RESETS>(w, bias, x, window, age, z);
+        if (a.silu) activate<T, V>(z);
+        rlt_store<V>(to, z);
+        to += a.out.step;
+        shift<W, V>(window, x);
+        if (RESETS) age = min(age + 1, W - 1);
+    };
+    Raw<T, V> next[U];
+    bool begins[U];
+    auto ask = [&] {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            next[u].load(from);
+            from += a.x.step;
+            if (RESETS) { begins[u] = *flags; flags += a.batch; }
+        }
+    };
     int t = first;
-    for (; t < live; t += UNROLL) {
-        float x[UNROLL][V];
-        bool begins[UNROLL];
+    if (t + U <= live) ask();
+    for (; t + U <= live; t += U) {
+        Raw<T, V> x[U];
+        bool now[U];
 #pragma unroll
-        for (int u = 0; u < UNROLL; u++) {
-            const int s = min(t + u, live - 1);
-            rlt_load<V>(at<T>(a.x, s, p.row, p.channel), x[u]);
-            begins[u] = a.reset && a.reset[(size_t)s * a.batch + p.row];
-        }
+        for (int u = 0; u < U; u++) { x[u] = next[u]; if (RESETS) now[u] = begins[u]; }
+        if (t + 2 * U <= live) ask();
 #pragma unroll
-        for (int u = 0; u < UNROLL; u++) {
-            if (t + u < live) {
-                float z[V];
-                if (begins[u]) age = 0;
-                taps<W, V>(w, bias, x[u], window, age, z);
-                if (a.silu) {
-#pragma unroll
-                    for (int i = 0; i < V; i++) {
-                        float s, other;
-                        rlt_sigmoids(z[i], s, other);
-                        z[i] *= s;
-                    }
-                }
-                rlt_store<V>(at<T>(a.out, t + u, p.row, p.channel), z);
-                shift<W, V>(window, x[u]);
-                age = min(age + 1, W - 1);
-            }
-        }
+        for (int u = 0; u < U; u++) step(x[u], RESETS && now[u]);
+    }
+    for (; t < live; t++) {
+        Raw<T, V> x;
+        x.load(from);
+        from += a.x.step;
+        bool now = false;
+        if (RESETS) { now = *flags; flags += a.batch; }
+        step(x, now);
     }
     if (a.final && (length > first ? length <= end : length == 0 && first == 0)) store_state<W, V>(a.final, a.channels, p.row, p.channel, window, age);
     float zeros[V];
 #pragma unroll
     for (int i = 0; i < V; i++) zeros[i] = 0.0f;
-    for (t = max(live, first); t < end; t++) rlt_store<V>(at<T>(a.out, t, p.row, p.channel), zeros);
+    for (t = max(live, first); t < end; t++, to += a.out.step) rlt_store<V>(to, zeros);
 }
 
 // The state behind the last steps alone, where it takes the initial state's place: a launch behind the one that reads it. A thread reads what it writes over before it does.
@@ -146,7 +185,8 @@ template <typename T, int W> __global__ __launch_bounds__(256) void final_state_
 
 // One walk with the steps: step t's gradient before the activation needs the inputs up to t, and is added to those of the W inputs that it read; the oldest of them is then whole and is written. A segment goes W - 1 steps beyond
 // its end for the sake of its last inputs. Memory bounds it: inputs and the output's gradient in, the input's gradient out.
-template <typename T, int W, int V> __global__ __launch_bounds__(256) void backward_kernel(Convolution a) {
+template <typename T, int W, int V, bool RESETS> __global__ __launch_bounds__(256) void backward_kernel(Convolution a) {
+    constexpr int U = 4;
     Place p = place_of<V>(a);
     if (!p.there) return;
     float w[W][V], bias[V], d_w[W][V], d_bias[V];
@@ -169,64 +209,88 @@ template <typename T, int W, int V> __global__ __launch_bounds__(256) void backw
             for (int i = 0; i < V; i++) d[j][i] = 0.0f;
         int age = W - 1;
         if (first <= length) {
-            age = age_of<W>(a, first, p.row);
+            if (RESETS) age = age_of<W>(a, first, p.row);
             load_window<T, W, V>(a, first, p.row, p.channel, window);
         }
+        T* const d_x0 = at<T>(a.d_x, 0, p.row, p.channel);
         auto emit = [&](int s, const float (&v)[V]) {      // the gradient of the input of step s
-            if (s >= first) { if (s < own) rlt_store<V>(at<T>(a.d_x, s, p.row, p.channel), v); }
+            if (s >= first) { if (s < own) rlt_store<V>(d_x0 + (int64_t)s * a.d_x.step, v); }
             else if (s < 0 && first == 0 && a.d_initial) {
 #pragma unroll
                 for (int i = 0; i < V; i++) a.d_initial[((size_t)p.row * (W - 1) + W - 1 + s) * a.channels + p.channel + i] = v[i];
             }
         };
-        constexpr int U = UNROLL / 2;
-        for (int t = first; t < stop; t += U) {
-            float x[U][V], g[U][V];
-            bool begins[U];
+        // INNER: a step of the segment whose oldest input is one, too
+        auto step = [&](int t, const Raw<T, V>& x_raw, const Raw<T, V>& d_raw, bool begins, auto inner) {
+            constexpr bool INNER = decltype(inner)::value;
+            float x[V], g[V], now[V];
+            x_raw.unpack(x);
+            d_raw.unpack(g);
+            if (RESETS && begins) age = 0;
+            if (a.silu) {
+                float z[V];
+                taps<W, V, RESETS>(w, bias, x, window, age, z);
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                const int s = min(t + u, stop - 1);
-                rlt_load<V>(at<T>(a.x, s, p.row, p.channel), x[u]);
-                rlt_load<V>(at<T>(a.d_out, s, p.row, p.channel), g[u]);
-                begins[u] = a.reset && a.reset[(size_t)s * a.batch + p.row];
-            }
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                if (t + u < stop) {
-                    if (begins[u]) age = 0;
-                    if (a.silu) {
-                        float z[V];
-                        taps<W, V>(w, bias, x[u], window, age, z);
-#pragma unroll
-                        for (int i = 0; i < V; i++) {
-                            float s, other;
-                            rlt_sigmoids(z[i], s, other);
-                            g[u][i] *= s * fmaf(z[i], other, 1.0f);
-                        }
-                    }
-                    if (t + u < end) {
-#pragma unroll
-                        for (int i = 0; i < V; i++) {
-                            d_bias[i] += g[u][i];
-                            d_w[0][i] = fmaf(g[u][i], x[u][i], d_w[0][i]);
-#pragma unroll
-                            for (int j = 1; j < W; j++) d_w[j][i] = age >= j ? fmaf(g[u][i], window[j - 1][i], d_w[j][i]) : d_w[j][i];
-                        }
-                    }
-                    float now[V];
-#pragma unroll
-                    for (int i = 0; i < V; i++) {
-                        now[i] = w[0][i] * g[u][i];
-#pragma unroll
-                        for (int j = 1; j < W; j++) d[j - 1][i] = age >= j ? fmaf(w[j][i], g[u][i], d[j - 1][i]) : d[j - 1][i];
-                    }
-                    emit(t + u - (W - 1), d[W - 2]);
-                    shift<W, V>(d, now);
-                    shift<W, V>(window, x[u]);
-                    age = min(age + 1, W - 1);
+                for (int i = 0; i < V; i++) {
+                    float s, other;
+                    sigmoids<T>(z[i], s, other);
+                    g[i] *= s * fmaf(z[i], other, 1.0f);
                 }
             }
+            if (INNER || t < end) {
+#pragma unroll
+                for (int i = 0; i < V; i++) {
+                    d_bias[i] += g[i];
+                    d_w[0][i] = fmaf(g[i], x[i], d_w[0][i]);
+#pragma unroll
+                    for (int j = 1; j < W; j++) d_w[j][i] = !RESETS || age >= j ? fmaf(g[i], window[j - 1][i], d_w[j][i]) : d_w[j][i];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                now[i] = w[0][i] * g[i];
+#pragma unroll
+                for (int j = 1; j < W; j++) d[j - 1][i] = !RESETS || age >= j ? fmaf(w[j][i], g[i], d[j - 1][i]) : d[j - 1][i];
+            }
+            if (INNER) rlt_store<V>(d_x0 + (int64_t)(t - (W - 1)) * a.d_x.step, d[W - 2]);
+            else emit(t - (W - 1), d[W - 2]);
+            shift<W, V>(d, now);
+            shift<W, V>(window, x);
+            if (RESETS) age = min(age + 1, W - 1);
+        };
+        const T* from = at<T>(a.x, first, p.row, p.channel); const T* d_from = at<T>(a.d_out, first, p.row, p.channel);
+        const uint8_t* flags = RESETS ? a.reset + (size_t)first * a.batch + p.row : nullptr;
+        auto one = [&](int t) {
+            Raw<T, V> x, g;
+            x.load(from); g.load(d_from);
+            from += a.x.step; d_from += a.d_out.step;
+            bool begins = false;
+            if (RESETS) { begins = *flags; flags += a.batch; }
+            step(t, x, g, begins, std::false_type{});
+        };
+        int t = first;
+        for (; t < min(first + W - 1, stop); t++) one(t);
+        Raw<T, V> next_x[U], next_d[U];
+        bool next_begins[U];
+        auto ask = [&] {
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                next_x[u].load(from); next_d[u].load(d_from);
+                from += a.x.step; d_from += a.d_out.step;
+                if (RESETS) { next_begins[u] = *flags; flags += a.batch; }
+            }
+        };
+        if (t + U <= own) ask();
+        for (; t + U <= own; t += U) {
+            Raw<T, V> x[U], g[U];
+            bool begins[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) { x[u] = next_x[u]; g[u] = next_d[u]; if (RESETS) begins[u] = next_begins[u]; }
+            if (t + 2 * U <= own) ask();
+#pragma unroll
+            for (int u = 0; u < U; u++) step(t + u, x[u], g[u], RESETS && begins[u], std::true_type{});
         }
+        for (; t < stop; t++) one(t);
         // a row that ends here: the gradient of the state behind it, then what waits
         if (length >= first && length < end + W - 1 && (length > 0 || first == 0)) {
             if (a.d_final) {
@@ -234,7 +298,7 @@ template <typename T, int W, int V> __global__ __launch_bounds__(256) void backw
                 for (int j = 1; j < W; j++)
 #pragma unroll
                     for (int i = 0; i < V; i++)
-                        if (age >= j) d[j - 1][i] += a.d_final[((size_t)p.row * (W - 1) + W - 1 - j) * a.channels + p.channel + i];
+                        if (!RESETS || age >= j) d[j - 1][i] += a.d_final[((size_t)p.row * (W - 1) + W - 1 - j) * a.channels + p.channel + i];
             }
 #pragma unroll
             for (int j = W - 1; j > 0; j--) emit(length - j, d[j - 1]);
@@ -242,7 +306,7 @@ template <typename T, int W, int V> __global__ __launch_bounds__(256) void backw
         float zeros[V];
 #pragma unroll
         for (int i = 0; i < V; i++) zeros[i] = 0.0f;
-        for (int t = max(own, first); t < end; t++) rlt_store<V>(at<T>(a.d_x, t, p.row, p.channel), zeros);
+        for (t = max(own, first); t < end; t++) rlt_store<V>(d_x0 + (int64_t)t * a.d_x.step, zeros);
     }
     if (a.partial) {
         float* const to = a.partial + group * (W + 1) * a.channels + p.channel;
@@ -255,44 +319,44 @@ template <typename T, int W, int V> __global__ __launch_bounds__(256) void backw
     }
 }
 
-// sums over rows and segments, in a fixed order: sixteen threads a column, whose sums are added up in LDS
+// sums over rows and segments
 __global__ __launch_bounds__(1024) void join_kernel(const float* __restrict__ partial, int parts, int width, int channels, float* __restrict__ d_weights, float* __restrict__ d_biases, int accumulate) {
-    __shared__ float sums[16][64];
-    const int lane = threadIdx.x & 63, group = threadIdx.x >> 6, column = blockIdx.x * 64 + lane, columns = (width + 1) * channels;
-    float s = 0.0f;
-    if (column < columns)
-        for (int p = group; p < parts; p += 16) s += partial[(size_t)p * columns + column];
-    sums[group][lane] = s;
-    __syncthreads();
-    if (group == 0 && column < columns) {
-        for (int g = 1; g < 16; g++) s += sums[g][lane];
+    const int column = blockIdx.x * RLT_JOIN_COLUMNS + threadIdx.x % RLT_JOIN_COLUMNS, columns = (width + 1) * channels;
+    const float s = rlt_join_column(partial, parts, columns, column, column < columns);
+    if (threadIdx.x < RLT_JOIN_COLUMNS && column < columns) {
         const int tap = column / channels, channel = column - tap * channels;
         float* const to = tap < width ? (d_weights ? d_weights + (size_t)channel * width + tap : nullptr) : (d_biases ? d_biases + channel : nullptr);
         if (to) *to = accumulate ? *to + s : s;
     }
 }
 
-// A pass over the states, which are read and written once.
+// A pass over the states, which are read and written once: a thread has its channels of ROWS rows, whose loads are all on their way before the first of them is worked on, and their weights once.
+constexpr int STEP_ROWS = 4;
 template <typename T, int W, int V> __global__ __launch_bounds__(256) void step_kernel(Convolution a) {
-    const Place p = place_of<V>(a);
-    if (!p.there) return;
-    float w[W][V], bias[V], window[W - 1][V], x[V], z[V];
-    rlt_load<V>(at<T>(a.x, 0, p.row, p.channel), x);
-    load_window<T, W, V>(a, 0, p.row, p.channel, window);
-    load_weights<W, V>(a, p.channel, w, bias);
-    int age = a.reset && a.reset[p.row] ? 0 : W - 1;
-    taps<W, V>(w, bias, x, window, age, z);
-    if (a.silu) {
+    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x, rows = i / a.vectors;
+    const int row0 = (int)rows * STEP_ROWS, channel = (int)(i - rows * a.vectors) * V;
+    if (rows * STEP_ROWS >= (size_t)a.batch) return;
+    float window[STEP_ROWS][W - 1][V], x[STEP_ROWS][V], w[W][V], bias[V];
+    bool begins[STEP_ROWS];
 #pragma unroll
-        for (int i = 0; i < V; i++) {
-            float s, other;
-            rlt_sigmoids(z[i], s, other);
-            z[i] *= s;
-        }
+    for (int r = 0; r < STEP_ROWS; r++) {
+        const int row = min(row0 + r, a.batch - 1);
+        rlt_load<V>(at<T>(a.x, 0, row, channel), x[r]);
+        load_window<T, W, V>(a, 0, row, channel, window[r]);
+        begins[r] = a.reset && a.reset[row];
     }
-    rlt_store<V>(at<T>(a.out, 0, p.row, p.channel), z);
-    shift<W, V>(window, x);
-    store_state<W, V>(a.final, a.channels, p.row, p.channel, window, min(age + 1, W - 1));
+    load_weights<W, V>(a, channel, w, bias);
+#pragma unroll
+    for (int r = 0; r < STEP_ROWS; r++) {
+        if (row0 + r >= a.batch) break;
+        float z[V];
+        const int age = begins[r] ? 0 : W - 1;
+        taps<W, V, true>(w, bias, x[r], window[r], age, z);
+        if (a.silu) activate<T, V>(z);
+        rlt_store<V>(at<T>(a.out, 0, row0 + r, channel), z);
+        shift<W, V>(window[r], x[r]);
+        store_state<W, V>(a.final, a.channels, row0 + r, channel, window[r], min(age + 1, W - 1));
+    }
 }
 
 bool described(const rlt_causal_convolution* p) {
@@ -323,20 +387,28 @@ Convolution convolution_of(const rlt_causal_convolution* p, const uint8_t* reset
     return a;
 }
 enum Pass { FORWARD, BACKWARD, STEP };
-template <typename T, int W, int V> int launch_vectors(rlt_rocm_device* device, Convolution a, Pass pass) {
+template <typename T, int W, int V, int PASS> int launch_vectors(rlt_rocm_device* device, Convolution a) {
     a.vectors = a.channels / V;
-    const size_t blocks = ((size_t)a.vectors * a.groups + 255) / 256;
+    const size_t blocks = ((size_t)a.vectors * (PASS == STEP ? (a.batch + STEP_ROWS - 1) / STEP_ROWS : a.groups) + 255) / 256;
     if (blocks > UINT32_MAX / 256) return RLT_E_UNSUPPORTED;
     const dim3 grid((unsigned)blocks), block(256);
-    if (pass == FORWARD) hipLaunchKernelGGL((forward_kernel<T, W, V>), grid, block, 0, device->stream, a);
-    else if (pass == BACKWARD) hipLaunchKernelGGL((backward_kernel<T, W, V>), grid, block, 0, device->stream, a);
-    else hipLaunchKernelGGL((step_kernel<T, W, V>), grid, block, 0, device->stream, a);
+    if constexpr (PASS == STEP) hipLaunchKernelGGL((step_kernel<T, W, V>), grid, block, 0, device->stream, a);
+    else if constexpr (PASS == FORWARD) {
+        if (a.reset) hipLaunchKernelGGL((forward_kernel<T, W, V, true>), grid, block, 0, device->stream, a);
+        else hipLaunchKernelGGL((forward_kernel<T, W, V, false>), grid, block, 0, device->stream, a);
+    } else {
+        if (a.reset) hipLaunchKernelGGL((backward_kernel<T, W, V, true>), grid, block, 0, device->stream, a);
+        else hipLaunchKernelGGL((backward_kernel<T, W, V, false>), grid, block, 0, device->stream, a);
+    }
     return rlt_launch_status(device);
 }
+// Vectors of 16 bytes, in the backward pass of bfloat16 of 8: what it holds for eight channels leaves a SIMD two wavefronts.
 template <typename T, int W> int launch_width(rlt_rocm_device* device, const Convolution& a, Pass pass) {
     constexpr int V = 16 / sizeof(T);
-    if (a.channels % V == 0 && whole(a.x, V, sizeof(T)) && whole(a.out, V, sizeof(T)) && whole(a.d_out, V, sizeof(T)) && whole(a.d_x, V, sizeof(T))) return launch_vectors<T, W, V>(device, a, pass);
-    return launch_vectors<T, W, 1>(device, a, pass);
+    const bool vectors = a.channels % V == 0 && whole(a.x, V, sizeof(T)) && whole(a.out, V, sizeof(T)) && whole(a.d_out, V, sizeof(T)) && whole(a.d_x, V, sizeof(T));
+    if (pass == FORWARD) return vectors ? launch_vectors<T, W, V, FORWARD>(device, a) : launch_vectors<T, W, 1, FORWARD>(device, a);
+    if (pass == BACKWARD) return vectors ? launch_vectors<T, W, 4, BACKWARD>(device, a) : launch_vectors<T, W, 1, BACKWARD>(device, a);
+    return vectors ? launch_vectors<T, W, V, STEP>(device, a) : launch_vectors<T, W, 1, STEP>(device, a);
 }
 template <typename F> int by_width(int width, F&& f) {
     switch (width) {
@@ -402,7 +474,7 @@ int rlt_rocm_causal_convolution_backward(rlt_rocm_device* device, const rlt_caus
     const int rc = launch(device, layer, a, BACKWARD);
     if (rc || !need) return rc;
     const size_t columns = (size_t)(layer->width + 1) * layer->channels;
-    hipLaunchKernelGGL(join_kernel, dim3((unsigned)((columns + 63) / 64)), dim3(1024), 0, device->stream, (const float*)workspace, (int)a.groups, layer->width, layer->channels, layer->d_weights,
+    hipLaunchKernelGGL(join_kernel, dim3((unsigned)((columns + RLT_JOIN_COLUMNS - 1) / RLT_JOIN_COLUMNS)), dim3(1024), 0, device->stream, (const float*)workspace, (int)a.groups, layer->width, layer->channels, layer->d_weights,
                        layer->d_biases, accumulate);
     return rlt_launch_status(device);
 }

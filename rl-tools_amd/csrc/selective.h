@@ -23,3 +23,38 @@ __device__ __forceinline__ void rlt_sigmoids(float x, float& s, float& other) {
     s = x >= 0.0f ? large : small;
     other = x >= 0.0f ? small : large;
 }
+
+// Sums over `parts` rows of a matrix of `columns` columns, in a fixed order, by a workgroup of 1,024 for sixteen columns: the sum of column `column` in the first sixteen threads. Sixty-four threads share a column, eight rows of each on their way
+// at a time (777 parts of 804 columns: 5 us; 15 with sixteen threads to a column, which follow one row with the next).
+constexpr int RLT_JOIN_COLUMNS = 16;
+__device__ __forceinline__ float rlt_join_column(const float* __restrict__ from, int parts, size_t columns, size_t column, bool there) {
+    __shared__ float sums[16][RLT_JOIN_COLUMNS];
+    constexpr int AHEAD = 8, GROUPS = 1024 / RLT_JOIN_COLUMNS;
+    const int group = threadIdx.x / RLT_JOIN_COLUMNS, lane = threadIdx.x & 63;
+    float s = 0.0f;
+    if (there) {
+        int p = group;
+        for (; p + (AHEAD - 1) * GROUPS < parts; p += AHEAD * GROUPS) {
+            float v[AHEAD];
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++) v[i] = from[(size_t)(p + i * GROUPS) * columns + column];
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++) s += v[i];
+        }
+        float v[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) v[i] = p + i * GROUPS < parts ? from[(size_t)(p + i * GROUPS) * columns + column] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) s += v[i];
+    }
+    s += __shfl_xor(s, 16, 64);
+    s += __shfl_xor(s, 32, 64);
+    if (lane < 16) sums[threadIdx.x >> 6][lane] = s;
+    __syncthreads();
+    if (threadIdx.x < 16) {
+        s = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 16; w++) s += sums[w][threadIdx.x];
+    }
+    return s;
+}

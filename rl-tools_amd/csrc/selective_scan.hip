@@ -636,25 +636,18 @@ template <typename T> __global__ __launch_bounds__(256) void shared_sum_kernel(S
     }
 }
 
-// the parameters' gradients out of the workgroups' shares, in a fixed order: sixteen threads an element, whose sums are added up in LDS
+// the parameters' gradients out of the workgroups' shares; sixteen elements of one of the three to a workgroup
 __global__ __launch_bounds__(1024) void parameter_sum_kernel(Scan a, int parts, int padded, float* __restrict__ d_log_rates, float* __restrict__ d_skip, float* __restrict__ d_delta_biases, int accumulate) {
-    __shared__ float sums[16][64];
-    const int lane = threadIdx.x & 63, group = threadIdx.x >> 6;
     const size_t channels = (size_t)a.heads * a.channels, rates = channels * padded;
-    size_t i = (size_t)blockIdx.x * 64 + lane;
-    const bool of_rates = i < rates, of_skips = !of_rates && i < rates + channels, there = i < rates + 2 * channels;
-    const size_t columns = of_rates ? rates : channels;
-    const float* const from = of_rates ? a.d_rates : of_skips ? a.d_skips : a.d_biases;
-    i -= of_rates ? 0 : of_skips ? rates : rates + channels;
-    float s = 0.0f;
-    if (there && from)
-        for (int p = group; p < parts; p += 16) s += from[(size_t)p * columns + i];
-    sums[group][lane] = s;
-    __syncthreads();
-    if (group || !there || !from) return;
-    for (int g = 1; g < 16; g++) s += sums[g][lane];
-    float* to = of_skips ? d_skip + i : d_delta_biases + i;
-    if (of_rates) {
+    const unsigned of_rates = (unsigned)((rates + RLT_JOIN_COLUMNS - 1) / RLT_JOIN_COLUMNS), of_channels = (unsigned)((channels + RLT_JOIN_COLUMNS - 1) / RLT_JOIN_COLUMNS);
+    const int which = blockIdx.x < of_rates ? 0 : blockIdx.x < of_rates + of_channels ? 1 : 2;
+    const size_t columns = which ? channels : rates, i = (size_t)(blockIdx.x - (which ? of_rates : 0) - (which == 2 ? of_channels : 0)) * RLT_JOIN_COLUMNS + threadIdx.x % RLT_JOIN_COLUMNS;
+    const float* const from = which == 0 ? a.d_rates : which == 1 ? a.d_skips : a.d_biases;
+    if (!from) return;
+    float s = rlt_join_column(from, parts, columns, i, i < columns);
+    if (threadIdx.x >= RLT_JOIN_COLUMNS || i >= columns) return;
+    float* to = which == 1 ? d_skip + i : d_delta_biases + i;
+    if (which == 0) {
         const size_t channel = i / padded;
         const int n = (int)(i - channel * padded);
         if (n >= a.states) return;
@@ -874,8 +867,9 @@ int rlt_rocm_selective_scan_backward(rlt_rocm_device* device, const rlt_selectiv
             if ((rc = rlt_launch_status(device))) return rc;
         }
         if (!a.d_rates && !a.d_skips && !a.d_biases) return 0;
-        const size_t elements = (size_t)layer->heads * layer->channels * (4 * NPT + 2);
-        hipLaunchKernelGGL(parameter_sum_kernel, dim3((unsigned)((elements + 63) / 64)), dim3(1024), 0, device->stream, a, a.row_groups * a.segments, 4 * NPT, layer->d_log_rates, layer->d_skip,
+        const size_t channels = (size_t)layer->heads * layer->channels;
+        auto blocks_for = [](size_t columns) { return (columns + RLT_JOIN_COLUMNS - 1) / RLT_JOIN_COLUMNS; };
+        hipLaunchKernelGGL(parameter_sum_kernel, dim3((unsigned)(blocks_for(channels * 4 * NPT) + 2 * blocks_for(channels))), dim3(1024), 0, device->stream, a, a.row_groups * a.segments, 4 * NPT, layer->d_log_rates, layer->d_skip,
                            layer->d_delta_biases, accumulate);
         return rlt_launch_status(device);
     });
