@@ -138,32 +138,50 @@ __device__ __forceinline__ bool bit(unsigned mask, int i) {
     asm volatile("" : "+s"(mask));      // looked at where it is needed: sixteen answers held from a walk forward to the one back are 32 scalar registers
     return mask >> i & 1;
 }
-// bit s: step t + s forgets its state
-template <int K> __device__ __forceinline__ unsigned resets_of(const Scan& a, const Place& p, int t) {
-    if (!a.reset) return 0;
-    const int s = threadIdx.x & 63;
-    return (unsigned)__ballot(s < K && t + s < p.live && a.reset[(size_t)min(t + s, a.steps - 1) * a.batch + p.row]);
-}
+// What a chunk needs is asked for without a branch and without looking at it, so that all of it is under way at once and nothing waits before the chunk is worked on: what is not there is read from where something is, and taken out then.
+// WHOLE: all of the chunk's steps are there, which is known of every chunk but a row's last.
+// Resets: a lane holds step t + lane's; bit s of the answer: step t + s forgets its state.
+template <int K> struct Resets {
+    uint8_t own;
+    template <bool WHOLE> __device__ __forceinline__ void ask(const Scan& a, const Place& p, int t) {
+        own = 0;
+        const int step = t + (int)(threadIdx.x & (K - 1));
+        if (a.reset) own = a.reset[(size_t)(WHOLE ? step : min(step, p.live - 1)) * a.batch + p.row];
+    }
+    __device__ __forceinline__ unsigned get(const Place& p, int t) const {
+        const int s = threadIdx.x & 63;
+        return (unsigned)__ballot(s < K && t + s < p.live && own);
+    }
+};
 
 // b and c of a chunk, zero beyond the row's length and the layer's states; a thread holds its elements while the chunk before is worked on
-template <typename T, int NPT> struct Shared {
-    static constexpr int K = CHUNK<NPT>, N = 4 * NPT, PER = (K * N + LANES - 1) / LANES;
-    float b[PER], c[PER];
-    __device__ __forceinline__ void ask(const Scan& a, const Place& p, int t, bool with_b) {
+template <typename T, int NPT, int K = CHUNK<NPT>> struct Shared {
+    static constexpr int N = 4 * NPT, PER = (K * N + LANES - 1) / LANES;
+    T b[PER], c[PER];
+    template <bool WHOLE, bool B, bool C> __device__ __forceinline__ void ask(const Scan& a, const Place& p, int t) {
 #pragma unroll
         for (int j = 0; j < PER; j++) {
-            const int e = threadIdx.x + j * LANES, s = e / N, n = e % N;
-            const bool there = e < K * N && t + s < p.live && n < a.states;
-            b[j] = there && with_b ? (float)at<T>(a.b, t + s, p.row, p.head)[n] : 0.0f;
-            c[j] = there && a.c.data ? (float)at<T>(a.c, t + s, p.row, p.head)[n] : 0.0f;
+            int e = threadIdx.x + j * LANES;
+            asm volatile("" : "+v"(e));      // addresses are worked out for each chunk rather than held from one to the next
+            const int step = WHOLE ? t + e / N : min(t + e / N, p.live - 1), n = min(e % N, a.states - 1);
+            if (K * N % LANES && e >= K * N) continue;
+            if (B) b[j] = at<T>(a.b, step, p.row, p.head)[n];
+            if (C) c[j] = at<T>(a.c, step, p.row, p.head)[n];
         }
     }
-    __device__ __forceinline__ void put(float (*to)[K * N]) const {
+    template <bool WHOLE, bool B, bool C> __device__ __forceinline__ void put(const Scan& a, const Place& p, int t, float (*to)[K * N]) const {
 #pragma unroll
         for (int j = 0; j < PER; j++) {
             const int e = threadIdx.x + j * LANES;
-            if (e < K * N) { to[0][e] = b[j]; to[1][e] = c[j]; }
+            const bool there = (WHOLE || t + e / N < p.live) && e % N < a.states;
+            if (K * N % LANES && e >= K * N) continue;
+            if (B) to[0][e] = there ? (float)b[j] : 0.0f;
+            if (C) to[1][e] = there ? (float)c[j] : 0.0f;
         }
+    }
+    __device__ __forceinline__ void cut(const Place& p, int t) {
+#pragma unroll
+        for (int j = 0; j < PER; j++) if (t + (int)(threadIdx.x + j * LANES) / N >= p.live) b[j] = c[j] = (T)0.0f;
     }
 };
 template <int NPT> __device__ __forceinline__ void read(const float* from, float (&to)[NPT]) {
@@ -204,30 +222,53 @@ template <typename T> struct Lanes {
         base = (GLOBAL char*)part.data + ((int64_t)p.row * part.row + (int64_t)p.head * part.head) * (int64_t)sizeof(T) + lowest;
         offset = (unsigned)((int)(threadIdx.x & 3) * stride - lowest) + (unsigned)channel * (unsigned)sizeof(T);
     }
-    // `whole`: all of the steps are there, and all lanes' channels; otherwise what is not there is `nothing`
-    template <int OWN> __device__ __forceinline__ void ask(bool whole, bool there, int t, int live, float nothing, T (&v)[OWN]) const {
+    template <bool WHOLE, int OWN> __device__ __forceinline__ void ask(int t, int live, T (&v)[OWN]) const {
         const GLOBAL char* from = base + (int64_t)t * stride;
-        if (whole) {
+        if (WHOLE || t + 4 * OWN <= live) {
 #pragma unroll
             for (int i = 0; i < OWN; i++) { v[i] = *(const GLOBAL T*)(from + offset); from += 4 * (int64_t)stride; }
         } else {
+            const int last = live - 1 - t, last_four = last & ~3;      // lanes beyond the last step read the last one's
+            const unsigned cut = offset - (unsigned)(max(last_four + (int)(threadIdx.x & 3) - last, 0) * stride);
 #pragma unroll
-            for (int i = 0; i < OWN; i++) {
-                v[i] = (T)nothing;
-                if (there && t + 4 * i + (int)(threadIdx.x & 3) < live) v[i] = *(const GLOBAL T*)(from + offset);
-                from += 4 * (int64_t)stride;
-            }
+            for (int i = 0; i < OWN; i++) v[i] = *(const GLOBAL T*)(from + (int64_t)min(4 * i, last_four) * stride + (4 * i < last_four ? offset : cut));
         }
     }
     __device__ __forceinline__ void put(int t, float v) const { *(GLOBAL T*)(base + (int64_t)t * stride + offset) = (T)v; }      // t: a multiple of four steps into a chunk
 };
+// a channel's states in the caller's memory; together where the lanes' shares come out even, from any element on
 template <int NPT> __device__ __forceinline__ void load_states(const float* from, int n0, int states, float (&h)[NPT]) {
+    constexpr int V = NPT < 4 ? NPT : 4;
+    typedef float vector __attribute__((ext_vector_type(V), aligned(4)));
+    if (states % NPT == 0) {
 #pragma unroll
-    for (int n = 0; n < NPT; n++) h[n] = from && n0 + n < states ? from[n0 + n] : 0.0f;
+        for (int n = 0; n < NPT; n += V) {
+            vector v = (vector)0.0f;
+            if (n0 < states) v = *reinterpret_cast<const vector*>(from + n0 + n);
+#pragma unroll
+            for (int i = 0; i < V; i++) h[n + i] = v[i];
+        }
+    } else {
+#pragma unroll
+        for (int n = 0; n < NPT; n++) h[n] = n0 + n < states ? from[n0 + n] : 0.0f;
+    }
 }
 template <int NPT> __device__ __forceinline__ void store_states(float* to, int n0, int states, const float (&h)[NPT]) {
+    constexpr int V = NPT < 4 ? NPT : 4;
+    typedef float vector __attribute__((ext_vector_type(V), aligned(4)));
+    if (states % NPT == 0) {
+        if (n0 >= states) return;
 #pragma unroll
-    for (int n = 0; n < NPT; n++) if (n0 + n < states) to[n0 + n] = h[n];
+        for (int n = 0; n < NPT; n += V) {
+            vector v;
+#pragma unroll
+            for (int i = 0; i < V; i++) v[i] = h[n + i];
+            *reinterpret_cast<vector*>(to + n0 + n) = v;
+        }
+    } else {
+#pragma unroll
+        for (int n = 0; n < NPT; n++) if (n0 + n < states) to[n0 + n] = h[n];
+    }
 }
 // logarithms of the decays to base 2 for a delta of one; nothing where there is no state
 template <int NPT> __device__ __forceinline__ void load_rates(const Scan& a, int head, int channel, int n0, float (&rate)[NPT]) {
@@ -237,42 +278,45 @@ template <int NPT> __device__ __forceinline__ void load_rates(const Scan& a, int
 }
 
 // Forward over a segment. STATES: only what the segment adds to the state, for states that segments start from.
-template <typename T, int NPT, bool STATES> __global__ __launch_bounds__(LANES) void forward_kernel(Scan a) {
-    constexpr int K = CHUNK<NPT>, OWN = K / 4, N = 4 * NPT;
+template <typename T, int NPT, bool STATES, int K> __global__ __launch_bounds__(LANES) void forward_kernel(Scan a) {
+    constexpr int OWN = K / 4, N = 4 * NPT;
     __shared__ float shared[2][2][K * N];
     Place p = place_of(a, blockIdx.x, a.batch);
     set_row(a, p, p.row);
     const int lane = threadIdx.x & 63, nq = lane & 3, n0 = nq * NPT, own_channel = p.tile * TILE + (int)(threadIdx.x >> 2), channel = min(own_channel, a.channels - 1);
     const bool there = own_channel < a.channels, all_there = (p.tile + 1) * TILE <= a.channels, gated = a.gate.data != nullptr, odd = nq & 1, upper = nq & 2;
     const size_t pair = pair_of(a, p), at_channel = (size_t)p.head * a.channels + channel;
+    T x[OWN], raw[OWN], gate[OWN];
+    Resets<K> resets;
+    Shared<T, NPT, K> next;
+    const Arguments arguments;
+    const Lanes<T> x_lanes(SCAN_PART(arguments, x), p, channel), delta_lanes(SCAN_PART(arguments, delta), p, channel), gate_lanes(SCAN_PART(arguments, gate), p, channel), out_lanes(SCAN_PART(arguments, out), p, channel);
+    auto ask_chunk = [&](int t) {
+        x_lanes.template ask<false>(t, p.live, x);
+        delta_lanes.template ask<false>(t, p.live, raw);
+        if (!STATES && gated) gate_lanes.template ask<false>(t, p.live, gate);
+        next.template ask<false, true, !STATES>(a, p, t);
+        resets.template ask<false>(a, p, t);
+    };
+    if (p.first < p.live) ask_chunk(p.first);
     float rate[NPT], h[NPT];
-    load_rates<NPT>(a, p.head, channel, n0, rate);
-    const float bias = a.delta_biases ? a.delta_biases[at_channel] : 0.0f, skip = a.skip ? a.skip[at_channel] : 0.0f;
     if (STATES || !a.entry) {
 #pragma unroll
         for (int n = 0; n < NPT; n++) h[n] = 0.0f;
     } else if (a.entry_padded) read<NPT>(a.entry + ((pair * a.segments + p.segment) * a.channels + channel) * N + n0, h);
     else load_states<NPT>(a.entry + (pair * a.channels + channel) * a.states, n0, a.states, h);
+    const float bias = a.delta_biases ? a.delta_biases[at_channel] : 0.0f, skip = a.skip ? a.skip[at_channel] : 0.0f;
+    load_rates<NPT>(a, p.head, channel, n0, rate);
     float sum = 0.0f;
     bool forgotten = false;
 
-    const Arguments arguments;
-    const Lanes<T> x_lanes(SCAN_PART(arguments, x), p, channel), delta_lanes(SCAN_PART(arguments, delta), p, channel), gate_lanes(SCAN_PART(arguments, gate), p, channel), out_lanes(SCAN_PART(arguments, out), p, channel);
-    T x[OWN], raw[OWN], gate[OWN];
-    unsigned resets;
-    Shared<T, NPT> next;
-    auto ask_chunk = [&](int t) {
-        const bool whole = all_there && t + K <= p.live;
-        x_lanes.ask(whole, there, t, p.live, 0.0f, x);
-        delta_lanes.ask(whole, there, t, p.live, NO_DELTA, raw);
-        if (!STATES && gated) gate_lanes.ask(whole, there, t, p.live, 0.0f, gate);
-        next.ask(a, p, t, true);
-        resets = resets_of<K>(a, p, t);
-    };
-    if (p.first < p.live) ask_chunk(p.first);
     int turn = 0;
     for (int t = p.first; t < p.live; t += K, turn ^= 1) {
         float xs[OWN], delta[OWN], added[OWN], gates[OWN];
+        if (!all_there || t + K > p.live) {
+#pragma unroll
+            for (int i = 0; i < OWN; i++) if (!there || t + 4 * i + nq >= p.live) { x[i] = gate[i] = (T)0.0f; raw[i] = (T)NO_DELTA; }
+        }
 #pragma unroll
         for (int i = 0; i < OWN; i++) {
             float e;
@@ -281,16 +325,17 @@ template <typename T, int NPT, bool STATES> __global__ __launch_bounds__(LANES) 
             added[i] = delta[i] * xs[i];
             if (!STATES) gates[i] = gated ? (float)gate[i] : 0.0f;
         }
-        const unsigned forget = resets;
-        next.put(shared[turn]);
+        const unsigned forget = resets.get(p, t);
+        next.template put<false, true, !STATES>(a, p, t, shared[turn]);
         if (t + K < p.live) ask_chunk(t + K);
         rlt_lds_barrier();
         const float* const bs = shared[turn][0] + n0; const float* const cs = shared[turn][1] + n0;
         if (!STATES && a.checkpoints && there) write<NPT>(a.checkpoints + ((pair * a.chunks + t / K) * a.channels + channel) * N + n0, h);
         float y[OWN];
-        auto walk = [&](auto with_resets) {
+        auto walk = [&](auto with_resets, auto whole) {
 #pragma unroll
             for (int i = 0; i < OWN; i++) {
+                if (!decltype(whole)::value && t + 4 * i >= p.live) { y[i] = 0.0f; continue; }
                 float part[4];
                 auto step = [&](auto which) {
                     constexpr int j = decltype(which)::value;
@@ -315,7 +360,9 @@ template <typename T, int NPT, bool STATES> __global__ __launch_bounds__(LANES) 
                 else sum += delta[i];
             }
         };
-        if (forget) walk(std::true_type{}); else walk(std::false_type{});
+        if (t + K > p.live) walk(std::true_type{}, std::false_type{});
+        else if (forget) walk(std::true_type{}, std::true_type{});
+        else walk(std::false_type{}, std::true_type{});
         if (!STATES) {
 #pragma unroll
             for (int i = 0; i < OWN; i++) {
@@ -363,8 +410,9 @@ template <bool REVERSE> __global__ __launch_bounds__(256) void join_segments_ker
 // Backward over a segment: from the last chunk to the first, the chunk's states again from its checkpoint, then its steps from the last to the first with the state's gradient G:
 //     G_t = c_t g_t + a_{t+1} G_{t+1},   g = d_output times the gate's factor;   d_c = sum over channels of g h,   d_b = sum over channels of delta x G,
 //     d_x = delta (G . b) + skip g,   d_delta = x (G . b) + rates . q,   d_rates += delta q   with q = G a h_{t-1}.
-template <typename T, int NPT, bool ONE_TILE> __global__ __launch_bounds__(LANES, 2) void backward_kernel(Scan a) {
-    constexpr int K = CHUNK<NPT>, OWN = K / 4, N = 4 * NPT, KEPT = NPT > 4 ? NPT / 4 : 1, PER = (K * N + LANES - 1) / LANES;
+// K: the chunk, or four, where no sequence is longer: then nothing is computed for steps that are not there, and the registers leave room for more wavefronts.
+template <typename T, int NPT, bool ONE_TILE, int K> __global__ __launch_bounds__(LANES, K > 4 || NPT > 4 ? 2 : 3) void backward_kernel(Scan a) {
+    constexpr int OWN = K / 4, N = 4 * NPT, KEPT = NPT > 4 ? NPT / 4 : 1, PER = (K * N + LANES - 1) / LANES;
     __shared__ float shared[2][2][K * N];
     __shared__ float slabs[2][WAVES][2][K * N];
     Place p = place_of(a, blockIdx.x, a.row_groups);
@@ -419,26 +467,38 @@ template <typename T, int NPT, bool ONE_TILE> __global__ __launch_bounds__(LANES
             for (int e = threadIdx.x; e < K * N; e += LANES) if (t + e / N < p.end) store_shared(t, e, 0.0f, 0.0f);
         }
         T x[OWN], raw[OWN], gate[OWN], d_out[OWN];
-        Shared<T, NPT> next;
-        unsigned resets;
+        Shared<T, NPT, K> next;
+        Resets<K> resets;
         float first_state[NPT];
-        auto ask_chunk = [&](int t) {
-            const bool whole = all_there && t + K <= p.live;
-            x_lanes.ask(whole, there, t, p.live, 0.0f, x);
-            delta_lanes.ask(whole, there, t, p.live, NO_DELTA, raw);
-            d_out_lanes.ask(whole, there, t, p.live, 0.0f, d_out);
-            if (gated) gate_lanes.ask(whole, there, t, p.live, 0.0f, gate);
-            next.ask(a, p, t, true);
-            resets = resets_of<K>(a, p, t);
+        auto ask_chunk = [&](int t, auto whole) {
+            constexpr bool WHOLE = decltype(whole)::value;
+            x_lanes.template ask<WHOLE>(t, p.live, x);
+            delta_lanes.template ask<WHOLE>(t, p.live, raw);
+            d_out_lanes.template ask<WHOLE>(t, p.live, d_out);
+            if (gated) gate_lanes.template ask<WHOLE>(t, p.live, gate);
+            next.template ask<WHOLE, true, true>(a, p, t);
+            resets.template ask<WHOLE>(a, p, t);
             read_global<NPT>((const GLOBAL char*)a.checkpoints + (pair * a.chunks + t / K) * a.channels * (N * sizeof(float)) + at_checkpoint, first_state);
         };
-        if (chunks) ask_chunk(p.first + (chunks - 1) * K);
+        if (chunks) {
+            const int t = p.first + (chunks - 1) * K;
+            ask_chunk(t, std::false_type{});
+            if (t + K > p.live) {
+                next.cut(p, t);
+#pragma unroll
+                for (int i = 0; i < OWN; i++) if (t + 4 * i + nq >= p.live) { x[i] = gate[i] = d_out[i] = (T)0.0f; raw[i] = (T)NO_DELTA; }
+            }
+        }
         for (int k = chunks - 1; k >= 0; k--, turn ^= 1) {
             const int t = p.first + k * K;
             float xs[OWN], delta[OWN], added[OWN], slope[OWN], d[OWN], by_gate[OWN];      // by_gate: the gate's gradient but for what it multiplies
             float h[K][NPT], decay[K][NPT], before[NPT];
-            const unsigned forget = resets;
-            next.put(shared[turn]);
+            const unsigned forget = resets.get(p, t);
+            next.template put<true, true, true>(a, p, t, shared[turn]);
+            if (!all_there) {
+#pragma unroll
+                for (int i = 0; i < OWN; i++) if (!there) { x[i] = gate[i] = d_out[i] = (T)0.0f; raw[i] = (T)NO_DELTA; }
+            }
 #pragma unroll
             for (int n = 0; n < NPT; n++) before[n] = first_state[n];
 #pragma unroll
@@ -482,7 +542,7 @@ template <typename T, int NPT, bool ONE_TILE> __global__ __launch_bounds__(LANES
                 for (int i = 0; i < OWN; i++) asm volatile("" : "+v"(delta[i]), "+v"(added[i]));
 #pragma unroll
                 for (int i = OWN - 1; i >= 0; i--) {
-                    if (i == 0 && k > 0) ask_chunk(t - K);      // the registers of states that are behind take what the next chunk needs
+                    if (i == 0 && k > 0) ask_chunk(t - K, std::true_type{});      // the registers of states that are behind take what the next chunk needs
                     float mixed_part[4], through_part[4], exponent_part[4], kept_b[KEPT], kept_c[KEPT];
 #pragma unroll
                     for (int m = 0; m < KEPT; m++) kept_b[m] = kept_c[m] = 0.0f;
@@ -567,17 +627,16 @@ template <typename T, int NPT> __global__ __launch_bounds__(LANES) void backward
 #pragma unroll
     for (int n = 0; n < NPT; n++) carry[n] = 0.0f;
     T raw[OWN], gate[OWN], d_out[OWN];
-    unsigned resets;
+    Resets<K> resets;
     Shared<T, NPT> next;
     const Arguments arguments;
     const Lanes<T> delta_lanes(SCAN_PART(arguments, delta), p, channel), gate_lanes(SCAN_PART(arguments, gate), p, channel), d_out_lanes(SCAN_PART(arguments, d_out), p, channel);
     auto ask_chunk = [&](int t) {
-        const bool whole = all_there && t + K <= p.live;
-        delta_lanes.ask(whole, there, t, p.live, NO_DELTA, raw);
-        d_out_lanes.ask(whole, there, t, p.live, 0.0f, d_out);
-        if (gated) gate_lanes.ask(whole, there, t, p.live, 0.0f, gate);
-        next.ask(a, p, t, false);
-        resets = resets_of<K>(a, p, t);
+        delta_lanes.template ask<false>(t, p.live, raw);
+        d_out_lanes.template ask<false>(t, p.live, d_out);
+        if (gated) gate_lanes.template ask<false>(t, p.live, gate);
+        next.template ask<false, false, true>(a, p, t);
+        resets.template ask<false>(a, p, t);
     };
     const int chunks = p.live > p.first ? (p.live - p.first + K - 1) / K : 0;
     if (chunks) ask_chunk(p.first + (chunks - 1) * K);
@@ -585,6 +644,10 @@ template <typename T, int NPT> __global__ __launch_bounds__(LANES) void backward
     for (int k = chunks - 1; k >= 0; k--, turn ^= 1) {
         const int t = p.first + k * K;
         float delta[OWN], d[OWN];
+        if (!all_there || t + K > p.live) {
+#pragma unroll
+            for (int i = 0; i < OWN; i++) if (!there || t + 4 * i + nq >= p.live) { gate[i] = d_out[i] = (T)0.0f; raw[i] = (T)NO_DELTA; }
+        }
 #pragma unroll
         for (int i = 0; i < OWN; i++) {
             float e;
@@ -593,8 +656,8 @@ template <typename T, int NPT> __global__ __launch_bounds__(LANES) void backward
             if (gated) d[i] *= gate_factor<T>((float)gate[i]);
             sum += delta[i];
         }
-        const unsigned forget = resets;
-        next.put(shared[turn]);
+        const unsigned forget = resets.get(p, t);
+        next.template put<false, false, true>(a, p, t, shared[turn]);
         if (k > 0) ask_chunk(t - K);
         rlt_lds_barrier();
         const float* const cs = shared[turn][1] + n0;
@@ -824,12 +887,14 @@ int rlt_rocm_selective_scan_forward(rlt_rocm_device* device, const rlt_selective
             Scan f = a;
             float* const states = (float*)workspace + s.states;
             f.sums = (float*)workspace + s.sums; f.exit = states;
-            hipLaunchKernelGGL((forward_kernel<T, NPT, true>), dim3(blocks_of(a, a.batch) / a.segments * (a.segments - 1)), dim3(LANES), 0, device->stream, f);      // (nothing starts from what the last segment adds)
+            hipLaunchKernelGGL((forward_kernel<T, NPT, true, CHUNK<NPT>>), dim3(blocks_of(a, a.batch) / a.segments * (a.segments - 1)), dim3(LANES), 0, device->stream, f);      // (nothing starts from what the last segment adds)
             int rc = rlt_launch_status(device);
             if (rc || (rc = join_segments<false>(device, f, initial_state, states, 4 * NPT))) return rc;
             a.entry = states; a.entry_padded = 1;
         }
-        hipLaunchKernelGGL((forward_kernel<T, NPT, false>), dim3(blocks_of(a, a.batch)), dim3(LANES), 0, device->stream, a);
+        const dim3 blocks(blocks_of(a, a.batch));
+        if (steps <= 4) hipLaunchKernelGGL((forward_kernel<T, NPT, false, 4>), blocks, dim3(LANES), 0, device->stream, a);
+        else hipLaunchKernelGGL((forward_kernel<T, NPT, false, CHUNK<NPT>>), blocks, dim3(LANES), 0, device->stream, a);
         return rlt_launch_status(device);
     });
 }
@@ -861,8 +926,10 @@ int rlt_rocm_selective_scan_backward(rlt_rocm_device* device, const rlt_selectiv
             a.entry = f.exit; a.entry_padded = 1;
         }
         const dim3 blocks(blocks_of(a, a.row_groups));
-        if (a.tiles == 1) hipLaunchKernelGGL((backward_kernel<T, NPT, true>), blocks, dim3(LANES), 0, device->stream, a);
-        else hipLaunchKernelGGL((backward_kernel<T, NPT, false>), blocks, dim3(LANES), 0, device->stream, a);
+        if (a.tiles == 1 && steps <= 4) hipLaunchKernelGGL((backward_kernel<T, NPT, true, 4>), blocks, dim3(LANES), 0, device->stream, a);
+        else if (a.tiles == 1) hipLaunchKernelGGL((backward_kernel<T, NPT, true, CHUNK<NPT>>), blocks, dim3(LANES), 0, device->stream, a);
+        else if (steps <= 4) hipLaunchKernelGGL((backward_kernel<T, NPT, false, 4>), blocks, dim3(LANES), 0, device->stream, a);
+        else hipLaunchKernelGGL((backward_kernel<T, NPT, false, CHUNK<NPT>>), blocks, dim3(LANES), 0, device->stream, a);
         if ((rc = rlt_launch_status(device))) return rc;
         if (a.tiles > 1) {
             hipLaunchKernelGGL(shared_sum_kernel<T>, dim3(2048), dim3(256), 0, device->stream, a, 4 * NPT);
