@@ -4,7 +4,7 @@
 
 namespace {
 
-constexpr int MAX_STEPS = 1 << 30, MAX_SIDE = 1 << 24, MIN_WIDTH = 2, MAX_WIDTH = 8;
+constexpr int MAX_STEPS = 1 << 30, MAX_ROWS = 1 << 24, MAX_CHANNELS = 1 << 22, MIN_WIDTH = 2, MAX_WIDTH = 8;
 
 struct Convolution {
     const float* weights; const float* biases;
@@ -363,7 +363,7 @@ bool described(const rlt_causal_convolution* p) {
     return p && (p->type == RLT_TYPE_F32 || p->type == RLT_TYPE_BF16) && p->batch > 0 && p->channels > 0 && p->width > 0;
 }
 bool supported(const rlt_causal_convolution* p) {
-    return p->width >= MIN_WIDTH && p->width <= MAX_WIDTH && p->batch <= MAX_SIDE && p->channels <= MAX_SIDE && (int64_t)p->batch * p->channels <= INT32_MAX;
+    return p->width >= MIN_WIDTH && p->width <= MAX_WIDTH && p->batch <= MAX_ROWS && p->channels <= MAX_CHANNELS && (int64_t)p->batch * p->channels <= INT32_MAX;
 }
 bool whole(const rlt_part& p, int64_t vector, int64_t size) { return !p.data || (reinterpret_cast<uintptr_t>(p.data) % 16 == 0 && p.step % vector == 0 && p.row % vector == 0 && 16 / size == vector); }
 
