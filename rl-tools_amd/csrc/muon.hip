@@ -1,7 +1,6 @@
 // Optimiser step for matrices whose updates are orthogonalised by products: A = X X^T, X <- a X + (b A + c A A) X, a few times.
 #include "typed.h"
 #include <algorithm>
-#include <vector>
 
 namespace {
 
@@ -9,7 +8,6 @@ namespace {
 // what is dropped, low x low and the rounding of the low part, is 2^-24.6 of a product in the mean (fp32's own rounding of a factor: 2^-25.3), at a third of the 16-bit rate, where fp32 instructions have a sixteenth.
 // Values are held times SCALE. Singular values stay below 1.21, those of A below 1.47, those of b A + c A A above -2.81 and below 0, so that no element leaves the range of 16 bits.
 typedef _Float16 f16;
-typedef f16 f16x4 __attribute__((ext_vector_type(4)));
 typedef f16 f16x8 __attribute__((ext_vector_type(8)));
 typedef rlt_f32x4 f32x4;
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -17,7 +15,7 @@ constexpr float SCALE = 16384.0f, UNSCALE = 1.0f / 16384.0f, QA = 3.4445f, QB = 
 constexpr int GROUP = 24, MAX_SIDE = 1 << 16, MAX_ITERATIONS = 32, PARTS = 256;      // matrices of a launch; partial sums of a norm
 constexpr int JOBS = 768;         // workgroups of a launch whose tiles are shared, at the most
 
-// What a launch is told: 16 bytes for each of its matrices, which a wavefront reads in one trip to where the launch left them (a row of longer entries, found and then read, was two trips of a microsecond each, a sixth of a small call's time).
+// What a launch is told: 16 bytes for each of its matrices, which a wavefront reads in one trip to where the launch left them (a row of longer entries, found and then read, was two trips).
 struct Entry {
     char* scratch;                // its part of the workspace, see Matrix
     uint16_t M, N;                // in 64s: M <= N, rows and columns, or columns and rows where there are more rows, filled up
@@ -163,6 +161,24 @@ struct Product {
 };
 template <int PHASE> struct ArgumentsOf { typedef Phases type; };
 template <> struct ArgumentsOf<LAST> { typedef Last type; };
+__device__ __forceinline__ const Tensors* tensors_of(const Phases&) { return nullptr; }
+__device__ __forceinline__ const Tensors* tensors_of(const Last& launch) { return &launch.tensors; }
+// which tile of `down` rows and `across` columns of tiles this is, and where its factors lie
+template <int PHASE> __device__ __forceinline__ void place(const Matrix& a, int tile, int down, int across, int from, Product& p) {
+    if (SYMMETRIC<PHASE>) {
+        p.ti = (int)((sqrtf(8.0f * tile + 1.0f) - 1.0f) * 0.5f);
+        while (p.ti * (p.ti + 1) / 2 > tile) p.ti--;
+        while ((p.ti + 1) * (p.ti + 2) / 2 <= tile) p.ti++;
+        p.tj = tile - p.ti * (p.ti + 1) / 2;
+    } else {      // eight rows of tiles at a time, column by column
+        const int band = tile / (8 * across), rows = min(8, down - band * 8), within = tile - band * 8 * across;
+        p.tj = within / rows; p.ti = band * 8 + within - p.tj * rows;
+    }
+    p.square = a.square(); p.plane = a.plane();
+    p.P = PHASE == GRAM ? a.x() : PHASE == SQUARE ? a.a() : a.b(); p.Q = PHASE == GRAM ? a.x() : PHASE == SQUARE ? a.a() : a.t(from);
+    p.p_plane = PHASE == GRAM ? p.plane : p.square; p.q_plane = PHASE == SQUARE ? p.square : p.plane;
+    p.q_rows = SYMMETRIC<PHASE> ? a.M : a.N;
+}
 template <int PHASE, int T> __device__ __forceinline__ bool product_of(const Entries& all, const Matrix& a, int block, Product& p) {
     const int down = (a.M + T - 1) / T, across = (a.N + T - 1) / T;
     p.depth = PHASE == GRAM ? a.N : a.M;
@@ -175,94 +191,105 @@ template <int PHASE, int T> __device__ __forceinline__ bool product_of(const Ent
         tile /= p.parts;
         p.from = part * all.length; p.to = min(p.from + all.length, p.depth);
     }
-    if (SYMMETRIC<PHASE>) {
-        p.ti = (int)((sqrtf(8.0f * tile + 1.0f) - 1.0f) * 0.5f);
-        while (p.ti * (p.ti + 1) / 2 > tile) p.ti--;
-        while ((p.ti + 1) * (p.ti + 2) / 2 <= tile) p.ti++;
-        p.tj = tile - p.ti * (p.ti + 1) / 2;
-    } else {      // eight rows of tiles at a time, column by column
-        const int band = tile / (8 * across), rows = min(8, down - band * 8), within = tile - band * 8 * across;
-        p.tj = within / rows; p.ti = band * 8 + within - p.tj * rows;
-    }
-    p.square = a.square(); p.plane = a.plane();
-    p.P = PHASE == GRAM ? a.x() : PHASE == SQUARE ? a.a() : a.b(); p.Q = PHASE == GRAM ? a.x() : PHASE == SQUARE ? a.a() : a.t(all.from);
-    p.p_plane = PHASE == GRAM ? p.plane : p.square; p.q_plane = PHASE == SQUARE ? p.square : p.plane;
-    p.q_rows = SYMMETRIC<PHASE> ? a.M : a.N;
+    place<PHASE>(a, tile, down, across, all.from, p);
     return true;
 }
-// What the sums of a tile of 32 x 32 are added to, and where they go. A lane has column lane % 32 and, four by four, rows of it.
-template <int PHASE> __device__ __forceinline__ void addends(const Matrix& a, const Product& p, int r0, int c0, float (&v)[16]) {
-    const int lane = threadIdx.x & 63, c = c0 + (lane & 31);
+// What becomes of a tile of 32 x 32. The sums come as the matrix instructions leave them, a column to a lane, and go through a square of LDS that belongs to the wavefront, so that memory sees eight elements of a row, or of a column, at a time
+// (stores of single elements and of four, as they come: a launch over sixteen block matrices of 256 to 2,048 columns 46 us, so 38).
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+constexpr int PITCH = 33;
+typedef float Square[32 * PITCH];
+struct Added { f16x8 high[2], low[2]; };      // of rows lane / 4 and lane / 4 + 16, columns lane % 4 * 8 and on: what the sums are added to
+template <int PHASE> __device__ __forceinline__ void addends(const Matrix& a, const Product& p, int r0, int c0, Added& v) {
     if constexpr (PHASE != GRAM) {
+        const int lane = threadIdx.x & 63;
         const GLOBAL f16* const from = PHASE == SQUARE ? a.a() : a.x();
-        const unsigned width = PHASE == SQUARE ? a.M : a.N, at = ((r0 + (lane >> 5) * 4) * width + c) * sizeof(f16);      // (a plane has at most 2^30 elements: offsets of 32 bits)
-        const GLOBAL f16* const low = from + (PHASE == SQUARE ? p.square : p.plane);
+        const size_t width = PHASE == SQUARE ? a.M : a.N, behind = PHASE == SQUARE ? p.square : p.plane;
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-            const unsigned row = ((e >> 2) * 8 + (e & 3)) * width * (unsigned)sizeof(f16);
-            v[e] = (float)*(const GLOBAL f16*)((const GLOBAL char*)from + (at + row)) + (float)*(const GLOBAL f16*)((const GLOBAL char*)low + (at + row));
+        for (int h = 0; h < 2; h++) {
+            const GLOBAL f16* const at = from + (size_t)(r0 + h * 16 + (lane >> 2)) * width + c0 + (lane & 3) * 8;
+            v.high[h] = *(const GLOBAL f16x8*)at; v.low[h] = *(const GLOBAL f16x8*)(at + behind);
         }
     }
 }
-template <int PHASE> __device__ __forceinline__ void finish(const typename ArgumentsOf<PHASE>::type& launch, const Matrix& a, const Product& p, int r0, int c0, const f32x16& sum, const float (&added)[16]) {
-    const int lane = threadIdx.x & 63, c = c0 + (lane & 31);
+__device__ __forceinline__ void keep(const f32x16& sum, float* square) {
+    const int lane = threadIdx.x & 63;
 #pragma unroll
-    for (int g = 0; g < 4; g++) {
-        const int r = r0 + g * 8 + (lane >> 5) * 4;
-        f16x4 high, low;
-        f32x4 v;
+    for (int e = 0; e < 16; e++) square[((e >> 2) * 8 + (lane >> 5) * 4 + (e & 3)) * PITCH + (lane & 31)] = sum[e];
+}
+// eight parameters from element `at` of a row on, of which `left` are there
+__device__ __forceinline__ void step_parameters(const Tensors& all, const Tensor& t, size_t at, int left, const float (&v)[8]) {
+    typedef float vector __attribute__((ext_vector_type(4), aligned(4)));
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            v[e] = sum[g * 4 + e] * UNSCALE;
-            if (PHASE == SQUARE) v[e] = fmaf(QC, v[e], QB * added[g * 4 + e]);
-            if (PHASE == UPDATE || PHASE == LAST) v[e] = fmaf(QA, added[g * 4 + e], v[e]);
+    for (int half = 0; half < 2; half++, at += 4, left -= 4) {
+        if (left >= 4) {
+            const vector w = *reinterpret_cast<const vector*>(t.w + at);
+            vector next;
+#pragma unroll
+            for (int e = 0; e < 4; e++) next[e] = fmaf(-t.factor, v[half * 4 + e] * UNSCALE, all.keep * w[e]);
+            *reinterpret_cast<vector*>(t.next_w + at) = next;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++) if (e < left) t.next_w[at + e] = fmaf(-t.factor, v[half * 4 + e] * UNSCALE, all.keep * t.w[at + e]);
+        }
+    }
+}
+template <int PHASE> __device__ __forceinline__ void finish(const Tensors* tensors, int from, const Matrix& a, const Product& p, int r0, int c0, float* square, const Added& added) {
+    const int lane = threadIdx.x & 63, line = lane >> 2, chunk = (lane & 3) * 8;
+    const bool tall = PHASE == LAST && tensors->t[a.index].rows > tensors->t[a.index].cols, turned = PHASE == UPDATE || (PHASE == LAST ? tall : p.ti != p.tj);
+    GLOBAL f16* const out = PHASE == GRAM ? a.a() : PHASE == SQUARE ? a.b() : a.x();
+    GLOBAL f16* const across = PHASE == UPDATE ? a.t(from ^ 1) : out;
+    const size_t behind = PHASE == UPDATE ? p.plane : p.square, width = PHASE == UPDATE ? a.N : a.M;
+    auto store = [&](GLOBAL f16* to, const float (&v)[8]) {
+        f16x8 high, low;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
             f16 h, l;
             split(v[e], h, l);
             high[e] = h; low[e] = l;
         }
-        if constexpr (PHASE == LAST) {
-            v *= UNSCALE;
-            const Tensor& t = launch.tensors.t[a.index];
-            const float keep = launch.tensors.keep;
-            if (t.rows <= t.cols) {
+        *(GLOBAL f16x8*)to = high; *(GLOBAL f16x8*)(to + behind) = low;
+    };
+    wave_sync();
 #pragma unroll
-                for (int e = 0; e < 4; e++)
-                    if (r + e < t.rows && c < t.cols) t.next_w[(size_t)(r + e) * t.cols + c] = fmaf(-t.factor, v[e], keep * t.w[(size_t)(r + e) * t.cols + c]);
-            } else if (c < t.rows) {
-                const size_t at = (size_t)c * t.cols + r;
-                typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
-                if (r + 4 <= t.cols) {
-                    const f32x4 w = *reinterpret_cast<const f32x4_any*>(t.w + at);
-                    f32x4 next;
+    for (int h = 0; h < 2; h++) {
+        const int r = r0 + h * 16 + line, c = c0 + chunk;
+        float* const own = square + (h * 16 + line) * PITCH + chunk;
+        float v[8];
 #pragma unroll
-                    for (int e = 0; e < 4; e++) next[e] = fmaf(-t.factor, v[e], keep * w[e]);
-                    *reinterpret_cast<f32x4_any*>(t.next_w + at) = next;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) if (r + e < t.cols) t.next_w[at + e] = fmaf(-t.factor, v[e], keep * t.w[at + e]);
-                }
-            }
-        } else {
-            GLOBAL f16* const out = PHASE == GRAM ? a.a() : PHASE == SQUARE ? a.b() : a.x();
-            const size_t behind = PHASE == UPDATE ? p.plane : p.square;
-            const unsigned width = PHASE == UPDATE ? a.N : a.M, at = (r * width + c) * (unsigned)sizeof(f16);
-            GLOBAL char* const highs = (GLOBAL char*)out; GLOBAL char* const lows = (GLOBAL char*)(out + behind);
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                *(GLOBAL f16*)(highs + (at + e * width * (unsigned)sizeof(f16))) = high[e];
-                *(GLOBAL f16*)(lows + (at + e * width * (unsigned)sizeof(f16))) = low[e];
-            }
-            if (PHASE == UPDATE || p.ti != p.tj) {
-                GLOBAL f16* const t = PHASE == UPDATE ? a.t(launch.entries.from ^ 1) : out;
-                const unsigned across = (c * (unsigned)a.M + r) * (unsigned)sizeof(f16);
-                *(GLOBAL f16x4*)((GLOBAL char*)t + across) = high; *(GLOBAL f16x4*)((GLOBAL char*)(t + behind) + across) = low;
-            }
+        for (int e = 0; e < 8; e++) {
+            v[e] = own[e] * UNSCALE;
+            const float add = PHASE == GRAM ? 0.0f : (float)added.high[h][e] + (float)added.low[h][e];
+            if (PHASE == SQUARE) v[e] = fmaf(QC, v[e], QB * add);
+            if (PHASE == UPDATE || PHASE == LAST) v[e] = fmaf(QA, add, v[e]);
+            if (turned) own[e] = v[e];
         }
+        if constexpr (PHASE == LAST) {
+            const Tensor& t = tensors->t[a.index];
+            if (!tall && r < t.rows) step_parameters(*tensors, t, (size_t)r * t.cols + c, t.cols - c, v);
+        } else store(out + (size_t)r * width + c, v);
+    }
+    if (!turned) return;
+    wave_sync();
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const int c = c0 + h * 16 + line, r = r0 + chunk;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = square[(chunk + e) * PITCH + h * 16 + line];
+        if constexpr (PHASE == LAST) {
+            const Tensor& t = tensors->t[a.index];
+            if (c < t.rows) step_parameters(*tensors, t, (size_t)c * t.cols + r, t.cols - r, v);
+        } else store(across + (size_t)c * a.M + r, v);
     }
 }
 
 // A tile whose k several workgroups share: each leaves its sums, and a launch behind adds them up, in the order of k. (The last workgroup of a tile to arrive did, which a ticket told it: the releases and acquires around the tickets write back and
-// invalidate the XCDs' L2s, 30 us at 350 workgroups, where the launch costs 6.)
+// invalidate the XCDs' L2s, 25 us at 350 workgroups, where the launch costs 7.)
 template <int W> __device__ __forceinline__ float* parts_of(const Entries& all, int job) { return all.parts + (size_t)job * (64 * W) * (64 * W) + threadIdx.x * 4; }      // tiles of 32 x 32 of the wavefronts, four sums of a lane at a time
 template <int W> __device__ __forceinline__ void leave(const Entries& all, const Product& p, int i, const f32x16& v) {
     float* const to = parts_of<W>(all, p.job) + i * 4096;
@@ -287,14 +314,10 @@ template <int W> __device__ __forceinline__ f32x16 joined(const Entries& all, co
 
 // Tiles of 64 x 64, for few of them: a launch is bound by trips to memory then. What 128 k need is on its way ahead, what the sums are added to with it; four wavefronts have 32 x 32 of the tile each, factors come through LDS in stages of
 // 64 k, and the three kinds of products have sums of their own, which are joined at the end: a chain of dependent matrix instructions is a third as long.
-template <int PHASE> __global__ __launch_bounds__(256, SYMMETRIC<PHASE> ? 2 : 1) void product_small_kernel(typename ArgumentsOf<PHASE>::type launch) {
+typedef f16 SmallStage[256 * 64];      // rows of P high, P low, Q high, Q low; chunks of eight changed about within a row
+template <int PHASE> __device__ __forceinline__ f32x16 small_sums(SmallStage* lds, const Matrix& a, const Product& p, int r0, int c0, Added& added) {
     constexpr int BK = 64, LOADS = 8, DEPTH = 2;
-    __shared__ __attribute__((aligned(16))) f16 lds[2][256 * BK];      // rows of P high, P low, Q high, Q low; chunks of eight changed about within a row
-    int block = blockIdx.x;
-    const Matrix a = matrix_of(launch.entries, block);
-    Product p;
-    if (!product_of<PHASE, 64>(launch.entries, a, block, p)) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = threadIdx.x >> 3, chunk = threadIdx.x & 7, r0 = p.ti * 64 + (wave >> 1) * 32, c0 = p.tj * 64 + (wave & 1) * 32;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = threadIdx.x >> 3, chunk = threadIdx.x & 7;
     const GLOBAL char* const p0 = (const GLOBAL char*)(p.P + (size_t)p.ti * 64 * p.depth); const GLOBAL char* const q0 = (const GLOBAL char*)(p.Q + (size_t)p.tj * 64 * p.depth);
     const unsigned own = (row * p.depth + chunk * 8) * (unsigned)sizeof(f16);
     f16x8 held[DEPTH][LOADS];
@@ -305,7 +328,6 @@ template <int PHASE> __global__ __launch_bounds__(256, SYMMETRIC<PHASE> ? 2 : 1)
     };
 #pragma unroll
     for (int d = 0; d < DEPTH; d++) ask(min(p.from + d * BK, p.to - BK), held[d]);      // (the last stage again where there are no more: a branch around a load waits for it)
-    float added[16];
     addends<PHASE>(a, p, r0, c0, added);
     f32x16 sum[3];
 #pragma unroll
@@ -336,13 +358,26 @@ template <int PHASE> __global__ __launch_bounds__(256, SYMMETRIC<PHASE> ? 2 : 1)
             }
         }
     }
-    f32x16 total = sum[0] + (sum[1] + sum[2]);
+    return sum[0] + (sum[1] + sum[2]);
+}
+template <int PHASE> __global__ __launch_bounds__(256, SYMMETRIC<PHASE> ? 2 : 1) void product_small_kernel(typename ArgumentsOf<PHASE>::type launch) {
+    __shared__ __attribute__((aligned(16))) SmallStage lds[2];
+    int block = blockIdx.x;
+    const Matrix a = matrix_of(launch.entries, block);
+    Product p;
+    if (!product_of<PHASE, 64>(launch.entries, a, block, p)) return;
+    const int wave = threadIdx.x >> 6, r0 = p.ti * 64 + (wave >> 1) * 32, c0 = p.tj * 64 + (wave & 1) * 32;
+    Added added;
+    const f32x16 total = small_sums<PHASE>(lds, a, p, r0, c0, added);
     if (p.parts > 1) { leave<1>(launch.entries, p, 0, total); return; }
-    finish<PHASE>(launch, a, p, r0, c0, total, added);
+    float* const square = reinterpret_cast<Square*>(lds)[wave];
+    rlt_lds_barrier();      // the stages are read
+    keep(total, square);
+    finish<PHASE>(tensors_of(launch), launch.entries.from, a, p, r0, c0, square, added);
 }
 
 // Tiles of 64 W x 64 W: four wavefronts share one, each has W x W tiles of 32 x 32, factors come through LDS in stages of 32 k. Half a stage ahead: while the products of one half run, the other half's factors come from LDS, the next stage's go there
-// and the one after that is asked for, dealt out between the matrix instructions. 256 x 256: 1,054 TFLOP/s of 16-bit products at 4,096 x 20,480 x 4,096 (the clock is down to 1.7 GHz by then; a large library product: 1,080), 867 without that order.
+// and the one after that is asked for, dealt out between the matrix instructions. 256 x 256: 1,138 TFLOP/s of 16-bit products at 4,096 x 20,480 x 4,096 (the clock is down to 1.7 GHz by then; a large library product: 1,080 to 1,135); the order brought 867 to 1,054 of it.
 template <int W, int PHASE> __global__ __launch_bounds__(256, W < 3 ? 2 : 1) void product_kernel(typename ArgumentsOf<PHASE>::type launch) {
     constexpr int T = 64 * W, BK = 32, ROWS = 4 * T, LOADS = ROWS * 4 / 256, PRODUCTS = 3 * W * W, READS = 4 * W;      // rows of the tile in LDS: P high, P low, Q high, Q low
     extern __shared__ __attribute__((aligned(16))) f16 lds[];      // [2][ROWS][BK], chunks of eight changed about within a row so that the rows that are read together lie in different banks
@@ -436,33 +471,26 @@ template <int W, int PHASE> __global__ __launch_bounds__(256, W < 3 ? 2 : 1) voi
     }
     // sums go through LDS, a row of tiles at a time: one copy of what is done with a tile, whose needs are no more than a tile's
     rlt_lds_barrier();
-    f32x4* const kept = reinterpret_cast<f32x4*>(lds) + wave * W * 256 + lane;
+    Square* const squares = reinterpret_cast<Square*>(lds) + wave * W;
 #pragma unroll
     for (int i = 0; i < W; i++) {
 #pragma unroll
-        for (int j = 0; j < W; j++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) kept[j * 256 + e * 64] = f32x4{sum[i][j][e * 4], sum[i][j][e * 4 + 1], sum[i][j][e * 4 + 2], sum[i][j][e * 4 + 3]};
+        for (int j = 0; j < W; j++) keep(sum[i][j], squares[j]);
 #pragma unroll 1
         for (int j = 0; j < W; j++) {
             const int r0 = p.ti * T + (wi * W + i) * 32, c0 = p.tj * T + (wj * W + j) * 32;
             if (r0 >= a.M || c0 >= p.q_rows) continue;
-            f32x16 total;
-            float added[16];
+            Added added;
             addends<PHASE>(a, p, r0, c0, added);
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const f32x4 v = kept[j * 256 + e * 64];
-#pragma unroll
-                for (int n = 0; n < 4; n++) total[e * 4 + n] = v[n];
-            }
-            finish<PHASE>(launch, a, p, r0, c0, total, added);
+            finish<PHASE>(tensors_of(launch), launch.entries.from, a, p, r0, c0, squares[j], added);
         }
+        wave_sync();
     }
 }
 
 // the sums of tiles that workgroups shared: a workgroup for every tile of 32 x 32 of each wavefront
 template <int W, int PHASE> __global__ __launch_bounds__(256) void join_kernel(Phases launch) {
+    __shared__ Square squares[4];
     int block = blockIdx.x / (W * W);
     const int i = blockIdx.x % (W * W), job = block, wave = threadIdx.x >> 6;
     const Matrix a = matrix_of(launch.entries, block);
@@ -471,10 +499,10 @@ template <int W, int PHASE> __global__ __launch_bounds__(256) void join_kernel(P
     const int r0 = p.ti * 64 * W + ((wave >> 1) * W + i / W) * 32, c0 = p.tj * 64 * W + ((wave & 1) * W + i % W) * 32;
     if (r0 >= a.M || c0 >= p.q_rows) return;
     p.job += job - (int)blockIdx.x;
-    float added[16];
+    Added added;
     addends<PHASE>(a, p, r0, c0, added);
-    const f32x16 total = joined<W>(launch.entries, p, i);
-    finish<PHASE>(launch, a, p, r0, c0, total, added);
+    keep(joined<W>(launch.entries, p, i), squares[wave]);
+    finish<PHASE>(tensors_of(launch), launch.entries.from, a, p, r0, c0, squares[wave], added);
 }
 
 bool described(const rlt_muon_tensor* t, int n) {
@@ -502,7 +530,7 @@ template <int W, int PHASE> size_t tiles_of(const Entries& all) {
     return n;
 }
 int depth_of(const Entry& m, int phase) { return 64 * (phase == GRAM ? m.N : m.M); }
-// Jobs of a launch whose tiles are shared out in lengths of `length` k. Lengths are 512 at the least, where a launch more is worth it, and leave no more than JOBS jobs (GRAM of 88 tiles of 128 x 128, up to 2,048 k: 49 us as they are, 22 shared)
+// Jobs of a launch whose tiles are shared out in lengths of `length` k. Lengths are 512 at the least, where a launch more is worth it, and leave no more than JOBS jobs (GRAM of 88 tiles of 128 x 128, up to 2,048 k: 49 us as they are, 35 shared)
 template <int W, int PHASE> size_t jobs_of(const Entries& all, int length) {
     size_t n = 0;
     for (int i = 0; i < all.n; i++) n += (tiles_of<W, PHASE>(all.e[i]) * ((depth_of(all.e[i], PHASE) + length - 1) / length) + 7) / 8 * 8;
@@ -523,7 +551,7 @@ template <int W, int PHASE> int length_of(const Entries& all) {
 }
 // Microseconds that a launch takes, round by round of 256 tiles: for 512 k of a tile with few others, with one on every compute unit, and for its sums' way out.
 template <int W, int PHASE> double cost_of(const Entries& all) {
-    constexpr double few[5] = {0, 5.5, 12, 15, 24}, full[5] = {0, 6.5, 14, 27, 46}, out[5] = {0, 3, 6, 28, 23};
+    constexpr double few[5] = {0, 5.5, 12, 15, 26}, full[5] = {0, 6.5, 14, 27, 46}, out[5] = {0, 3, 6, 18, 23};
     const int length = length_of<W, PHASE>(all);
     double cost = length == WHOLE ? 0.0 : 6.0;
     size_t jobs = 0, in_round = 0;
@@ -612,16 +640,24 @@ int rlt_rocm_muon_step(rlt_rocm_device* device, const rlt_muon_tensor* tensors, 
     if (!supported(tensors, n)) return RLT_E_UNSUPPORTED;
     RLT_REQUIRE(workspace && workspace_bytes >= rlt_rocm_muon_workspace_bytes(tensors, n) && reinterpret_cast<uintptr_t>(workspace) % 16 == 0);
     char* at = (char*)workspace;
-    std::vector<int> order(n);
-    for (int i = 0; i < n; i++) order[i] = i;
-    auto size = [&](int i) { return (int64_t)tensors[i].rows * tensors[i].cols; };
-    std::stable_sort(order.begin(), order.end(), [&](int i, int j) { return size(i) > size(j); });      // the longest products of a launch first
+    // the longest products of a launch first: behind each matrix the largest of those that are no larger, in the caller's order where they are alike
+    auto before = [&](int i, int j) {
+        const int64_t a = (int64_t)tensors[i].rows * tensors[i].cols, b = (int64_t)tensors[j].rows * tensors[j].cols;
+        return a != b ? a > b : i < j;
+    };
+    auto behind = [&](int last) {
+        int next = -1;
+        for (int i = 0; i < n; i++) if ((last < 0 || before(last, i)) && (next < 0 || before(i, next))) next = i;
+        return next;
+    };
     Last all{};
     all.entries.parts = (float*)at;
     at += SHARED_BYTES;
     all.tensors.momentum = parameters->momentum; all.tensors.epsilon = parameters->epsilon; all.tensors.keep = 1.0f - parameters->alpha * parameters->weight_decay; all.tensors.nesterov = parameters->nesterov;
+    int last = -1;
     for (int i = 0; i < n; i++) {
-        const rlt_muon_tensor& t = tensors[order[i]];
+        last = behind(last);
+        const rlt_muon_tensor& t = tensors[last];
         const int low = t.rows < t.cols ? t.rows : t.cols, high = t.rows < t.cols ? t.cols : t.rows;
         all.entries.e[all.entries.n] = {at, (uint16_t)(filled(low) / 64), (uint16_t)(filled(high) / 64), 0};
         all.tensors.t[all.entries.n++] = {t.parameters, t.gradient, t.momentum, t.next_parameters, t.next_momentum, t.rows, t.cols, parameters->alpha * sqrtf(t.rows > t.cols ? (float)t.rows / t.cols : 1.0f)};
