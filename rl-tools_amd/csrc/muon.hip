@@ -35,7 +35,7 @@ struct Entries {
 };
 struct Tensors { Tensor t[GROUP]; float momentum, epsilon, keep; int nesterov; };      // keep: 1 - alpha * weight_decay
 struct Phases { Entries entries; };
-struct Last { Entries entries; Tensors tensors; };
+struct Last { Entries entries; Tensors tensors; int iterations; };
 
 // X [M x N], its transpose [N x M] (one that is read, one that is written), A and b A + c A A [M x M], the low parts behind the high ones; PARTS partial sums of u^2 ahead of them
 #define GLOBAL __attribute__((address_space(1)))
@@ -505,6 +505,154 @@ template <int W, int PHASE> __global__ __launch_bounds__(256) void join_kernel(P
     finish<PHASE>(tensors_of(launch), launch.entries.from, a, p, r0, c0, squares[wave], added);
 }
 
+// The whole step of matrices with a side of up to 64 and another of up to 256, a workgroup each: X, its transpose and A, or b A + c A A in A's place, stay in LDS, and a kind of products costs two barriers where it would be a launch (64 x 64: 20 us
+// where the launches take 72; 64 x 256: 52, and 128 x 128 in launches 84). Where a larger matrix is in the call, the launches are there all the same and take the small ones along.
+constexpr int LOCAL_COLUMNS = 4;      // in 64s
+int local_bytes(int columns) { return (4 * 64 * columns * 64 + 2 * 64 * 64) * (int)sizeof(f16); }
+__global__ __launch_bounds__(1024) void local_kernel(Last launch) {
+    extern __shared__ __attribute__((aligned(16))) f16 lds[];
+    __shared__ double norms[16];
+    const Tensors& all = launch.tensors;
+    const Tensor& a = all.t[blockIdx.x];
+    const int N = launch.entries.e[blockIdx.x].N * 64, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    f16* const x = lds; f16* const t = x + 128 * N; f16* const square = t + 128 * N;      // [64][N], [N][64] and [64][64], the low parts behind the high ones; chunks of eight changed about within a row
+    auto at = [](int row, int k, int width) { return row * width + ((k >> 3) ^ (row >> 1 & 7)) * 8 + (k & 7); };
+    const bool tall = a.rows > a.cols;
+    const int across = tall ? 1 : N / 64, units = (tall ? N : 64) * across;      // 64 elements of a row, filled up
+    constexpr int AHEAD = 4;
+    float held[AHEAD];      // the first of a wavefront's updates; those behind them are worked out twice
+    double s = 0.0;
+    auto updates = [&](int u0, bool first) {
+        float g[AHEAD], m[AHEAD];
+#pragma unroll
+        for (int j = 0; j < AHEAD; j++) {
+            const int u = u0 + 16 * j, r = u / across, c = u % across * 64 + lane;
+            const bool there = r < a.rows && c < a.cols;
+            const size_t i = (size_t)r * a.cols + c;
+            g[j] = there ? a.g[i] : 0.0f;
+            m[j] = there ? (first ? a.m : a.next_m)[i] : 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < AHEAD; j++) {
+            const int u = u0 + 16 * j, r = u / across, c = u % across * 64 + lane;
+            const float next = first ? fmaf(all.momentum, m[j], g[j]) : m[j];
+            if (first && r < a.rows && c < a.cols) a.next_m[(size_t)r * a.cols + c] = next;
+            g[j] = all.nesterov ? fmaf(all.momentum, next, g[j]) : next;
+            if (first) s = fma((double)g[j], (double)g[j], s);
+        }
+        if (!first || u0 == wave) {
+#pragma unroll
+            for (int j = 0; j < AHEAD; j++) held[j] = g[j];
+        }
+    };
+    for (int u0 = wave; u0 < units; u0 += 16 * AHEAD) updates(u0, true);
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
+    if (lane == 0) norms[wave] = s;
+    __syncthreads();
+    double sum_of_norms = 0.0;
+#pragma unroll
+    for (int w = 0; w < 16; w++) sum_of_norms += norms[w];
+    const double inverse = (double)SCALE / (sqrt(sum_of_norms) + (double)all.epsilon);
+    for (int u0 = wave; u0 < units; u0 += 16 * AHEAD) {
+        if (u0 != wave) updates(u0, false);
+#pragma unroll
+        for (int j = 0; j < AHEAD; j++) {
+            const int u = u0 + 16 * j, pr = u / across, pc = u % across * 64 + lane, r = tall ? pc : pr, c = tall ? pr : pc;
+            f16 h, l;
+            split((float)((double)held[j] * inverse), h, l);
+            x[at(r, c, N)] = h; x[64 * N + at(r, c, N)] = l;
+            t[at(c, r, 64)] = h; t[64 * N + at(c, r, 64)] = l;
+        }
+    }
+    __syncthreads();
+
+    // sums over k of 16 rows of P and 16 of Q, in three kinds
+    auto product = [&](const f16* P, int p_low, int p_row, const f16* Q, int q_low, int q_row, int depth) {
+        f32x4 sum[3];
+#pragma unroll
+        for (int i = 0; i < 3; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) sum[i][e] = 0.0f;
+        const f16* const ps = P + (p_row + (lane & 15)) * depth; const f16* const qs = Q + (q_row + (lane & 15)) * depth;
+#pragma unroll 2
+        for (int k = 0; k < depth / 8; k += 4) {
+            const int chunk = ((k + (lane >> 4)) ^ (lane >> 1 & 7)) * 8;
+            const f16x8 ph = *reinterpret_cast<const f16x8*>(ps + chunk), pl = *reinterpret_cast<const f16x8*>(ps + p_low + chunk);
+            const f16x8 qh = *reinterpret_cast<const f16x8*>(qs + chunk), ql = *reinterpret_cast<const f16x8*>(qs + q_low + chunk);
+            sum[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, qh, sum[0], 0, 0, 0);
+            sum[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, ql, sum[1], 0, 0, 0);
+            sum[2] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl, qh, sum[2], 0, 0, 0);
+        }
+        return sum[0] + (sum[1] + sum[2]);
+    };
+    // A lane has a column and, four by four, rows of it: column c of the sums as row c of what is written, which for A and b A + c A A is the same (sums are alike on both sides of the diagonal, bit by bit).
+    typedef f16 f16x4 __attribute__((ext_vector_type(4)));
+    auto get = [&](const f16* from, int low, int r, int c, float (&v)[4]) {
+        const f16x4 h = *reinterpret_cast<const f16x4*>(from + at(c, r, 64)), l = *reinterpret_cast<const f16x4*>(from + low + at(c, r, 64));
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = (float)h[e] + (float)l[e];
+    };
+    auto put = [&](f16* to, int low, int r, int c, const float (&v)[4], f16x4& high, f16x4& rest) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            f16 h, l;
+            split(v[e], h, l);
+            high[e] = h; rest[e] = l;
+        }
+        *reinterpret_cast<f16x4*>(to + at(c, r, 64)) = high; *reinterpret_cast<f16x4*>(to + low + at(c, r, 64)) = rest;
+    };
+    const int r0 = (wave >> 2) * 16, c0 = (wave & 3) * 16, r = r0 + (lane >> 4) * 4, c = c0 + (lane & 15);
+    for (int k = 0; k < launch.iterations; k++) {
+        f16x4 high, rest;
+        f32x4 total = product(x, 64 * N, r0, x, 64 * N, c0, N);
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = total[e] * UNSCALE;
+        put(square, 4096, r, c, v, high, rest);
+        __syncthreads();
+        total = product(square, 4096, r0, square, 4096, c0, 64);
+        get(square, 4096, r, c, v);
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = fmaf(QC, total[e] * UNSCALE, QB * v[e]);
+        __syncthreads();
+        put(square, 4096, r, c, v, high, rest);
+        __syncthreads();
+        // a wavefront has a tile of 16 x 16 in each 64 columns
+        float next[LOCAL_COLUMNS][4];
+#pragma unroll
+        for (int i = 0; i < LOCAL_COLUMNS; i++)
+            if (i * 64 < N) {
+                total = product(square, 4096, r0, t, 64 * N, i * 64 + c0, 64);
+                get(t, 64 * N, r, i * 64 + c, next[i]);
+#pragma unroll
+                for (int e = 0; e < 4; e++) next[i][e] = fmaf(QA, next[i][e], total[e] * UNSCALE);
+            }
+        __syncthreads();
+        if (k + 1 < launch.iterations) {
+#pragma unroll
+            for (int i = 0; i < LOCAL_COLUMNS; i++)
+                if (i * 64 < N) {
+                    put(t, 64 * N, r, i * 64 + c, next[i], high, rest);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) { x[at(r + e, i * 64 + c, N)] = high[e]; x[64 * N + at(r + e, i * 64 + c, N)] = rest[e]; }
+                }
+            __syncthreads();
+            continue;
+        }
+#pragma unroll
+        for (int i = 0; i < LOCAL_COLUMNS; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int row = tall ? i * 64 + c : r + e, column = tall ? r + e : i * 64 + c;
+                if (i * 64 < N && row < a.rows && column < a.cols) {
+                    const size_t j = (size_t)row * a.cols + column;
+                    a.next_w[j] = fmaf(-a.factor, next[i][e] * UNSCALE, all.keep * a.w[j]);
+                }
+            }
+    }
+}
+
 bool described(const rlt_muon_tensor* t, int n) {
     if (!t || n <= 0) return false;
     for (int i = 0; i < n; i++) if (t[i].rows <= 0 || t[i].cols <= 0) return false;
@@ -599,9 +747,17 @@ template <int PHASE> int launch(rlt_rocm_device* device, const typename Argument
     const int best = (int)(std::min_element(cost, cost + 4) - cost);
     return best == 0 ? launch_width<1, PHASE>(device, all) : best == 1 ? launch_width<2, PHASE>(device, all) : best == 2 ? launch_width<3, PHASE>(device, all) : launch_width<4, PHASE>(device, all);
 }
-int run(rlt_rocm_device* device, Last& all, int iterations) {
+int run(rlt_rocm_device* device, Last& all, int iterations, bool local) {
     size_t tiles = 0;
     Entries& e = all.entries;
+    all.iterations = iterations;
+    if (local) {
+        int columns = 1;
+        for (int i = 0; i < e.n; i++) columns = std::max(columns, (int)e.e[i].N);
+        RLT_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(local_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, local_bytes(LOCAL_COLUMNS)));
+        hipLaunchKernelGGL(local_kernel, dim3(e.n), dim3(1024), local_bytes(columns), device->stream, all);
+        return rlt_launch_status(device);
+    }
     hipLaunchKernelGGL(momentum_kernel, dim3(e.n * PARTS), dim3(256), 0, device->stream, all);
     int rc = rlt_launch_status(device);
     if (rc) return rc;
@@ -654,6 +810,8 @@ int rlt_rocm_muon_step(rlt_rocm_device* device, const rlt_muon_tensor* tensors, 
     all.entries.parts = (float*)at;
     at += SHARED_BYTES;
     all.tensors.momentum = parameters->momentum; all.tensors.epsilon = parameters->epsilon; all.tensors.keep = 1.0f - parameters->alpha * parameters->weight_decay; all.tensors.nesterov = parameters->nesterov;
+    bool local = true;
+    for (int i = 0; i < n; i++) local = local && std::min(tensors[i].rows, tensors[i].cols) <= 64 && std::max(tensors[i].rows, tensors[i].cols) <= 64 * LOCAL_COLUMNS;
     int last = -1;
     for (int i = 0; i < n; i++) {
         last = behind(last);
@@ -663,7 +821,7 @@ int rlt_rocm_muon_step(rlt_rocm_device* device, const rlt_muon_tensor* tensors, 
         all.tensors.t[all.entries.n++] = {t.parameters, t.gradient, t.momentum, t.next_parameters, t.next_momentum, t.rows, t.cols, parameters->alpha * sqrtf(t.rows > t.cols ? (float)t.rows / t.cols : 1.0f)};
         at += bytes_of(t);
         if (all.entries.n == GROUP || i == n - 1) {
-            const int rc = run(device, all, parameters->iterations);
+            const int rc = run(device, all, parameters->iterations, local);
             if (rc) return rc;
             all.entries.n = 0;
         }
