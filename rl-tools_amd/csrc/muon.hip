@@ -791,7 +791,11 @@ int rlt_rocm_muon_step(rlt_rocm_device* device, const rlt_muon_tensor* tensors, 
         const rlt_muon_tensor& t = tensors[i];
         RLT_REQUIRE(t.parameters && t.gradient && t.momentum && t.next_parameters && t.next_momentum && t.next_momentum != t.gradient && t.next_parameters != t.gradient && t.next_parameters != t.next_momentum &&
                     t.next_parameters != t.momentum && t.next_momentum != t.parameters);
-        for (int j = 0; j < i; j++) RLT_REQUIRE(t.next_parameters != tensors[j].next_parameters && t.next_momentum != tensors[j].next_momentum);      // a matrix twice
+        for (int j = 0; j < n; j++) {      // a matrix twice, or one that another reads
+            const rlt_muon_tensor& o = tensors[j];
+            RLT_REQUIRE(j == i || (t.next_parameters != o.next_parameters && t.next_momentum != o.next_momentum && t.next_parameters != o.parameters && t.next_parameters != o.gradient && t.next_parameters != o.momentum &&
+                                   t.next_parameters != o.next_momentum && t.next_momentum != o.parameters && t.next_momentum != o.gradient && t.next_momentum != o.momentum));
+        }
     }
     if (!supported(tensors, n)) return RLT_E_UNSUPPORTED;
     RLT_REQUIRE(workspace && workspace_bytes >= rlt_rocm_muon_workspace_bytes(tensors, n) && reinterpret_cast<uintptr_t>(workspace) % 16 == 0);

@@ -113,6 +113,62 @@ def test_in_place_and_again_bit_for_bit(rocm, shapes):
         assert all(np.array_equal(a[n], b[n]) for n in a)
 
 
+# matrices that a workgroup holds (sides of up to 64 and 256), by themselves; just beyond; and beside larger ones
+HELD = [[(64, 256)], [(256, 64)], [(64, 192)], [(1, 256), (256, 1)], [(17, 200), (200, 17), (64, 64), (1, 1), (63, 255), (255, 63), (33, 129)], [(64, 257)], [(257, 64)], [(65, 64)], [(64, 256), (65, 256)]]
+
+
+@gpu
+@pytest.mark.parametrize("shapes", HELD)
+def test_matrices_that_a_workgroup_holds(rocm, shapes):
+    print("case", shapes, flush=True)
+    tensors, p = tensors_of(21, shapes), settings()
+    first, second = run(rocm, tensors, p), run(rocm, tensors, p, in_place=True)
+    check(tensors, p, first)
+    for a, b in zip(first, second):
+        assert all(np.array_equal(a[n], b[n]) for n in a)
+
+
+@gpu
+@pytest.mark.parametrize("changes", [dict(nesterov=0), dict(iterations=1), dict(iterations=2), dict(iterations=6), dict(weight_decay=0.0), dict(momentum=0.0), dict(epsilon=0.0)])
+def test_settings_of_matrices_that_a_workgroup_holds(rocm, changes):
+    tensors, p = tensors_of(23, [(60, 64), (250, 30), (40, 100)]), settings(**changes)
+    check(tensors, p, run(rocm, tensors, p))
+
+
+@gpu
+@pytest.mark.parametrize("size", [1e-30, 1e30])
+def test_small_matrices_of_any_size_of_none_and_of_what_is_not_finite(rocm, size):
+    tensors, p = tensors_of(25, [(60, 64), (64, 200), (200, 10), (30, 30)] * 8), settings(epsilon=2.0 ** -149)
+    for t in tensors:
+        t["gradient"], t["momentum"] = (t["gradient"] * np.float32(size)).astype(np.float32), (t["momentum"] * np.float32(size)).astype(np.float32)
+    clean = run(rocm, tensors, p)
+    check(tensors, p, clean)
+    tensors[1]["gradient"][3, 4] = np.nan
+    tensors[2]["gradient"][:] = tensors[2]["momentum"][:] = 0
+    got = run(rocm, tensors, p)
+    assert np.isnan(got[1]["next_parameters"]).any() and np.isnan(got[1]["next_momentum"]).sum() == 1
+    assert np.allclose(got[2]["next_parameters"], (1 - p["alpha"] * p["weight_decay"]) * tensors[2]["parameters"], rtol=2e-7, atol=0)
+    for i in range(3, len(got)):
+        assert all(np.array_equal(got[i][n], clean[i][n]) for n in got[i])
+
+
+# tiles of 128, 192 and 256, and lengths of k that workgroups share: by the sizes that come to them
+@gpu
+@pytest.mark.parametrize("shapes", [[(2048, 512), (64, 1024), (1024, 32), (512, 1024)] * 4, [(64, 8192)], [(1000, 1030)], [(2880, 2870)], [(2048, 8190)], [(8190, 2048)], [(5600, 5632)]])
+def test_large_matrices(rocm, shapes):
+    """no element is further off than the bound on the spectral norm of the errors, and their root mean square is as in check"""
+    print("case", shapes, flush=True)
+    tensors, p = tensors_of(27, shapes), settings(iterations=2)
+    for t, r in zip(tensors, run(rocm, tensors, p)):
+        m, scale, x, x32, kept = reference(t, p)
+        assert np.all(np.abs(r["next_momentum"] - m) <= 2 * U * (np.abs(p["momentum"] * t["momentum"]) + np.abs(m)) + 1e-45)
+        off = (r["next_parameters"].astype(np.float64) - (kept - p["alpha"] * scale * x)) / (p["alpha"] * scale)
+        own = 3 * U * (np.abs(kept) + p["alpha"] * scale * np.abs(x)) / (p["alpha"] * scale)
+        error = np.maximum(np.abs(off) - own, 0.0)
+        assert error.max() <= 960 * U * (np.sqrt(x.shape[0]) + np.sqrt(x.shape[1])) * (1 + 3.4445)
+        assert np.sqrt((error ** 2).mean()) <= 4 * np.sqrt(((x32 - x) ** 2).mean()) + U * np.sqrt((x ** 2).mean()), x.shape
+
+
 @gpu
 @pytest.mark.parametrize("size", [1e-30, 1e-12, 1e12, 1e30])
 def test_gradients_of_any_size(rocm, size):
@@ -206,5 +262,9 @@ def test_refusals(rocm):
     assert step(p=settings(iterations=0)) == step(p=settings(iterations=33)) == step(p=settings(epsilon=-1.0)) == step(p=settings(epsilon=float("nan"))) == bad
     assert step((first, first)) == step((first, second[:3] + (first[3], second[4], 8, 8))) == step((first, second[:4] + (first[4], 8, 8))) == bad      # a matrix twice
     assert step((first[:3] + (first[1], first[4], 8, 8),)) == step((first[:4] + (first[3], 8, 8),)) == step((first[:4] + (first[0], 8, 8),)) == bad      # buffers that overlap
+    for i in range(5):      # what one matrix writes and another reads
+        for written in (3, 4):
+            assert step((first, second[:i] + (first[written],) + second[i + 1:])) == bad
+    assert step((first, second[:1] + (first[1],) + second[2:])) == 0      # a gradient that two read
     assert step((first[:5] + (2 ** 16 + 1, 1),)) == step((first[:5] + (2 ** 16, 2 ** 15),)) == capi.RLT_E_UNSUPPORTED
     rocm.sync()
