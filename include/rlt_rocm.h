@@ -1302,7 +1302,7 @@ typedef struct rlt_causal_convolution {
 } rlt_causal_convolution;
 
 /* All steps of a sequence. initial_state, final_state (NULL: zeros / not wanted; they may be the same buffer), reset [steps x batch] (NULL: none) and lengths [batch] (NULL: all of them) as
- * rlt_rocm_linear_attention_forward has them: outputs beyond a row's length are zero, its state is that behind its last step, what its inputs hold there is not looked at. */
+ * rlt_rocm_linear_attention_forward has them: outputs beyond a row's length are zero, its state is that behind its last step, what its inputs hold there is not looked at. The output overlaps no input. */
 int rlt_rocm_causal_convolution_forward(rlt_rocm_device* device, const rlt_causal_convolution* layer, const rlt_head_view* x, const rlt_head_view* output,
                                         const float* initial_state, float* final_state, const uint8_t* reset, const int32_t* lengths, int steps);
 /* Scratch memory of the backward call (0 for a call that is refused, and where neither d_weights nor d_biases is wanted); starts on a 16-byte boundary and belongs to one call at a time. */
@@ -1337,7 +1337,7 @@ typedef struct rlt_selective_scan {
 size_t rlt_rocm_selective_scan_workspace_bytes(const rlt_selective_scan* layer, int steps, int backward);
 size_t rlt_rocm_selective_scan_checkpoint_bytes(const rlt_selective_scan* layer, int steps);
 /* All steps of a sequence. gate NULL: no gate (the factor is 1). initial_state, final_state (NULL: zeros / not wanted; they may be the same buffer), reset and lengths as
- * rlt_rocm_linear_attention_forward has them. checkpoints NULL: no backward call will follow. */
+ * rlt_rocm_linear_attention_forward has them. checkpoints NULL: no backward call will follow. The output overlaps no input. */
 int rlt_rocm_selective_scan_forward(rlt_rocm_device* device, const rlt_selective_scan* layer, const rlt_head_view* x, const rlt_head_view* delta, const rlt_head_view* b, const rlt_head_view* c,
                                     const rlt_head_view* gate, const rlt_head_view* output, const float* initial_state, float* final_state, const uint8_t* reset, const int32_t* lengths, int steps,
                                     void* checkpoints, void* workspace, size_t workspace_bytes);
@@ -1352,7 +1352,7 @@ int rlt_rocm_selective_scan_backward(rlt_rocm_device* device, const rlt_selectiv
 int rlt_rocm_selective_scan_step(rlt_rocm_device* device, const rlt_selective_scan* layer, const rlt_head_view* x, const rlt_head_view* delta, const rlt_head_view* b, const rlt_head_view* c,
                                  const rlt_head_view* gate, const rlt_head_view* output, const float* state, float* next_state, const uint8_t* reset);
 
-/* A matrix that muon_step updates, row-major without gaps. next_parameters and next_momentum may be parameters and momentum themselves; otherwise no two buffers of a call overlap. */
+/* A matrix that muon_step updates, row-major without gaps. next_parameters and next_momentum may be parameters and momentum themselves; otherwise nothing that a call writes overlaps anything else of it. */
 typedef struct rlt_muon_tensor {
     const float* parameters; const float* gradient; const float* momentum;
     float* next_parameters; float* next_momentum;

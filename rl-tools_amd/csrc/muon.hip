@@ -506,7 +506,7 @@ template <int W, int PHASE> __global__ __launch_bounds__(256) void join_kernel(P
 }
 
 // The whole step of matrices with a side of up to 64 and another of up to 256, a workgroup each: X, its transpose and A, or b A + c A A in A's place, stay in LDS, and a kind of products costs two barriers where it would be a launch (64 x 64: 20 us
-// where the launches take 72; 64 x 256: 52, and 128 x 128 in launches 84). Where a larger matrix is in the call, the launches are there all the same and take the small ones along.
+// where the launches take 66; 64 x 256: 52 and 78). Where a larger matrix is in the call, the launches are there all the same and take the small ones along.
 constexpr int LOCAL_COLUMNS = 4;      // in 64s
 int local_bytes(int columns) { return (4 * 64 * columns * 64 + 2 * 64 * 64) * (int)sizeof(f16); }
 __global__ __launch_bounds__(1024) void local_kernel(Last launch) {
