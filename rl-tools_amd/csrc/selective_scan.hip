@@ -280,8 +280,8 @@ template <int NPT> __device__ __forceinline__ void load_rates(const Scan& a, int
 }
 
 // Forward over a segment. STATES: only what the segment adds to the state, for states that segments start from.
-template <typename T, int NPT, bool STATES, int K> __global__ __launch_bounds__(LANES) void forward_kernel(Scan a) {
-    constexpr int OWN = K / 4, N = 4 * NPT;
+template <typename T, int NPT, bool STATES> __global__ __launch_bounds__(LANES) void forward_kernel(Scan a) {
+    constexpr int K = CHUNK<NPT>, OWN = K / 4, N = 4 * NPT;
     __shared__ float shared[2][2][K * N];
     Place p = place_of(a, blockIdx.x, a.batch);
     set_row(a, p, p.row);
@@ -386,6 +386,79 @@ template <typename T, int NPT, bool STATES, int K> __global__ __launch_bounds__(
         // steps behind the last chunk that holds any of the row's
         const int walked = p.live > p.first ? p.first + (p.live - p.first + K - 1) / K * K : p.first;
         for (int s = walked; s + nq < p.end; s += 4) out_lanes.put(s, 0.0f);
+    }
+}
+
+// Forward over sequences of four steps at most: a workgroup goes from one row to the next, whose inputs and state are on their way while it works.
+template <typename T, int NPT> __global__ __launch_bounds__(LANES) void short_forward_kernel(Scan a) {
+    constexpr int K = 4, N = 4 * NPT;
+    __shared__ float shared[2][2][K * N];
+    Place p = place_of(a, blockIdx.x, a.row_groups);
+    const int group = p.row, nq = threadIdx.x & 3, n0 = nq * NPT, own_channel = p.tile * TILE + (int)(threadIdx.x >> 2), channel = min(own_channel, a.channels - 1);
+    const bool there = own_channel < a.channels, gated = a.gate.data != nullptr, odd = nq & 1, upper = nq & 2;
+    const size_t at_channel = (size_t)p.head * a.channels + channel;
+    T x[1], raw[1], gate[1] = {(T)0.0f};
+    Resets<K> resets;
+    Shared<T, NPT, K> next;
+    float entry[NPT];
+    int live;
+    auto ask = [&](int row) {
+        const Arguments arguments;
+        set_row(a, p, row);
+        live = p.live;
+        p.live = max(live, 1);      // (a row without steps reads its first one all the same, and looks at none)
+        const Lanes<T> x_lanes(SCAN_PART(arguments, x), p, channel), delta_lanes(SCAN_PART(arguments, delta), p, channel), gate_lanes(SCAN_PART(arguments, gate), p, channel);
+        x_lanes.template ask<false>(0, p.live, x);
+        delta_lanes.template ask<false>(0, p.live, raw);
+        if (gated) gate_lanes.template ask<false>(0, p.live, gate);
+        next.template ask<false, true, true>(a, p, 0);
+        resets.template ask<false>(a, p, 0);
+        if (a.entry) load_states<NPT>(a.entry + ((size_t)pair_of(a, p) * a.channels + channel) * a.states, n0, a.states, entry);
+        p.live = live;
+    };
+#pragma unroll
+    for (int n = 0; n < NPT; n++) entry[n] = 0.0f;
+    ask(group);
+    const float bias = a.delta_biases ? a.delta_biases[at_channel] : 0.0f, skip = a.skip ? a.skip[at_channel] : 0.0f;
+    float rate[NPT];
+    load_rates<NPT>(a, p.head, channel, n0, rate);
+    int turn = 0;
+    for (int row = group; row < a.batch; row += a.row_groups, turn ^= 1) {
+        const size_t pair = (size_t)row * a.heads + p.head;
+        const int steps = live;
+        const bool whole = there && nq < steps;
+        float e, h[NPT];
+        const float xs = whole ? (float)x[0] : 0.0f, delta = softplus<T>(whole ? (float)raw[0] + bias : NO_DELTA, e), added = delta * xs, z = (float)gate[0];
+        const unsigned forget = resets.get(p, 0);
+        next.template put<false, true, true>(a, p, 0, shared[turn]);
+#pragma unroll
+        for (int n = 0; n < NPT; n++) h[n] = entry[n];
+        const Arguments arguments;
+        const Lanes<T> out_lanes(SCAN_PART(arguments, out), p, channel);
+        ask(min(row + a.row_groups, a.batch - 1));
+        rlt_lds_barrier();
+        if (a.checkpoints && there && steps > 0) write<NPT>(a.checkpoints + (pair * a.channels + channel) * N + n0, h);
+        float part[4];
+        each<0, K>([&](auto which) {
+            constexpr int j = decltype(which)::value;
+            part[j] = 0.0f;
+            if (j < steps) {
+                const float d = from_lane<j>(delta), u = from_lane<j>(added);
+                float b[NPT], c[NPT];
+                read<NPT>(shared[turn][0] + n0 + j * N, b);
+                read<NPT>(shared[turn][1] + n0 + j * N, c);
+                const bool begins = forget >> j & 1;
+#pragma unroll
+                for (int n = 0; n < NPT; n++) {
+                    h[n] = fmaf(__builtin_amdgcn_exp2f(d * rate[n]), begins ? 0.0f : h[n], u * b[n]);
+                    part[j] = fmaf(c[n], h[n], part[j]);
+                }
+            }
+        });
+        float v = fmaf(skip, xs, sum_to_lane(part, odd, upper));
+        if (gated && whole) v *= gate_factor<T>(z);
+        if (there && nq < a.steps) out_lanes.put(0, v);
+        if (there && a.exit) store_states<NPT>(a.exit + (pair * a.channels + channel) * a.states, n0, a.states, h);
     }
 }
 
@@ -902,14 +975,14 @@ int rlt_rocm_selective_scan_forward(rlt_rocm_device* device, const rlt_selective
             Scan f = a;
             float* const states = (float*)workspace + s.states;
             f.sums = (float*)workspace + s.sums; f.exit = states;
-            hipLaunchKernelGGL((forward_kernel<T, NPT, true, CHUNK<NPT>>), dim3(blocks_of(a, a.batch) / a.segments * (a.segments - 1)), dim3(LANES), 0, device->stream, f);      // (nothing starts from what the last segment adds)
+            hipLaunchKernelGGL((forward_kernel<T, NPT, true>), dim3(blocks_of(a, a.batch) / a.segments * (a.segments - 1)), dim3(LANES), 0, device->stream, f);      // (nothing starts from what the last segment adds)
             int rc = rlt_launch_status(device);
             if (rc || (rc = join_segments<false>(device, f, initial_state, states, 4 * NPT))) return rc;
             a.entry = states; a.entry_padded = 1;
         }
         const dim3 blocks(blocks_of(a, a.batch));
-        if (steps <= 4) hipLaunchKernelGGL((forward_kernel<T, NPT, false, 4>), blocks, dim3(LANES), 0, device->stream, a);
-        else hipLaunchKernelGGL((forward_kernel<T, NPT, false, CHUNK<NPT>>), blocks, dim3(LANES), 0, device->stream, a);
+        if (steps <= 4) hipLaunchKernelGGL((short_forward_kernel<T, NPT>), dim3(blocks_of(a, a.row_groups)), dim3(LANES), 0, device->stream, a);
+        else hipLaunchKernelGGL((forward_kernel<T, NPT, false>), blocks, dim3(LANES), 0, device->stream, a);
         return rlt_launch_status(device);
     });
 }
