@@ -493,9 +493,8 @@ template <bool REVERSE> __global__ __launch_bounds__(256) void join_segments_ker
 // Backward over a segment: from the last chunk to the first, the chunk's states again from its checkpoint, then its steps from the last to the first with the state's gradient G:
 //     G_t = c_t g_t + a_{t+1} G_{t+1},   g = d_output times the gate's factor;   d_c = sum over channels of g h,   d_b = sum over channels of delta x G,
 //     d_x = delta (G . b) + skip g,   d_delta = x (G . b) + rates . q,   d_rates += delta q   with q = G a h_{t-1}.
-// K: the chunk, or four, where no sequence is longer: then nothing is computed for steps that are not there, and the registers leave room for more wavefronts.
-template <typename T, int NPT, bool ONE_TILE, int K> __global__ __launch_bounds__(LANES, K > 4 || NPT > 4 ? 2 : 3) void backward_kernel(Scan a) {
-    constexpr int OWN = K / 4, N = 4 * NPT, KEPT = NPT > 4 ? NPT / 4 : 1, PER = (K * N + LANES - 1) / LANES;
+template <typename T, int NPT, bool ONE_TILE> __global__ __launch_bounds__(LANES, 2) void backward_kernel(Scan a) {
+    constexpr int K = CHUNK<NPT>, OWN = K / 4, N = 4 * NPT, KEPT = NPT > 4 ? NPT / 4 : 1, PER = (K * N + LANES - 1) / LANES;
     __shared__ float shared[2][2][K * N];
     __shared__ float slabs[2][WAVES][2][K * N];
     Place p = place_of(a, blockIdx.x, a.row_groups);
@@ -688,6 +687,150 @@ template <typename T, int NPT, bool ONE_TILE, int K> __global__ __launch_bounds_
     }
     if (!there) return;
     const size_t part = (size_t)p.segment * a.row_groups + group, of_channel = (part * a.heads + p.head) * a.channels + channel;
+    if (a.d_rates) write<NPT>(a.d_rates + of_channel * N + n0, d_rate);
+    d_skip = sum_of_lanes(d_skip); d_bias = sum_of_lanes(d_bias);
+    if (nq == 0 && a.d_skips) a.d_skips[of_channel] = d_skip;
+    if (nq == 0 && a.d_biases) a.d_biases[of_channel] = d_bias;
+}
+
+// Backward over sequences of four steps at most, as backward_kernel, from one row to the next like short_forward_kernel.
+template <typename T, int NPT, bool ONE_TILE> __global__ __launch_bounds__(LANES, NPT > 4 ? 2 : 3) void short_backward_kernel(Scan a) {
+    constexpr int K = 4, N = 4 * NPT, KEPT = NPT > 4 ? NPT / 4 : 1;
+    static_assert(K * N <= LANES, "");
+    __shared__ float shared[2][2][K * N];
+    __shared__ float slabs[2][WAVES][2][K * N];
+    Place p = place_of(a, blockIdx.x, a.row_groups);
+    const int group = p.row, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nq = lane & 3, quad = lane >> 2 & 3, n0 = nq * NPT, own_channel = p.tile * TILE + (int)(threadIdx.x >> 2), channel = min(own_channel, a.channels - 1);
+    const int kept_state = n0 + (NPT >= 4 ? (lane >> 4 & 1) * (NPT / 4) : 0) + (lane >> 5) * (NPT / 2);
+    const bool there = own_channel < a.channels, gated = a.gate.data != nullptr, odd = nq & 1, upper = nq & 2;
+    const size_t at_channel = (size_t)p.head * a.channels + channel;
+    T x[1], raw[1], gate[1] = {(T)0.0f}, d_out[1];
+    Resets<K> resets;
+    Shared<T, NPT, K> next;
+    float first_state[NPT], entry[NPT];
+    int live;
+    auto ask = [&](int row) {
+        const Arguments arguments;
+        set_row(a, p, row);
+        live = p.live;
+        p.live = max(live, 1);      // (a row without steps reads its first one all the same, and looks at none)
+        const Lanes<T> x_lanes(SCAN_PART(arguments, x), p, channel), delta_lanes(SCAN_PART(arguments, delta), p, channel), gate_lanes(SCAN_PART(arguments, gate), p, channel), d_out_lanes(SCAN_PART(arguments, d_out), p, channel);
+        x_lanes.template ask<false>(0, p.live, x);
+        delta_lanes.template ask<false>(0, p.live, raw);
+        d_out_lanes.template ask<false>(0, p.live, d_out);
+        if (gated) gate_lanes.template ask<false>(0, p.live, gate);
+        next.template ask<false, true, true>(a, p, 0);
+        resets.template ask<false>(a, p, 0);
+        const size_t pair = pair_of(a, p);
+        read_global<NPT>((const GLOBAL char*)a.checkpoints + pair * a.channels * (N * sizeof(float)) + (unsigned)(channel * N + n0) * sizeof(float), first_state);
+        if (a.entry) load_states<NPT>(a.entry + (pair * a.channels + channel) * a.states, n0, a.states, entry);
+        p.live = live;
+    };
+#pragma unroll
+    for (int n = 0; n < NPT; n++) entry[n] = 0.0f;
+    ask(group);
+    const float bias = a.delta_biases ? a.delta_biases[at_channel] : 0.0f, skip = a.skip ? a.skip[at_channel] : 0.0f;
+    float rate[NPT], d_rate[NPT], d_skip = 0.0f, d_bias = 0.0f;
+    load_rates<NPT>(a, p.head, channel, n0, rate);
+#pragma unroll
+    for (int n = 0; n < NPT; n++) d_rate[n] = 0.0f;
+    int turn = 0;
+    for (int row = group; row < a.batch; row += a.row_groups, turn ^= 1) {
+        const size_t pair = (size_t)row * a.heads + p.head;
+        const int steps = live;
+        const bool whole = there && nq < steps;
+        float e, by_gate = 0.0f, h[K][NPT], decay[K][NPT], before[NPT], carry[NPT];
+        const float v = whole ? (float)raw[0] + bias : NO_DELTA, xs = whole ? (float)x[0] : 0.0f, delta = softplus<T>(v, e), large = reciprocal<T>(1.0f + e), slope = v >= 0.0f ? large : e * large, added = delta * xs;
+        float d = whole ? (float)d_out[0] : 0.0f;
+        if (gated) {
+            const float g = d;
+            d *= gate_factor<T>(whole ? (float)gate[0] : 0.0f, g, by_gate);
+        }
+        const unsigned forget = resets.get(p, 0);
+        next.template put<false, true, true>(a, p, 0, shared[turn]);
+#pragma unroll
+        for (int n = 0; n < NPT; n++) { before[n] = first_state[n]; carry[n] = entry[n]; }
+        const Arguments arguments;
+        const Lanes<T> d_x_lanes(SCAN_PART(arguments, d_x), p, channel), d_delta_lanes(SCAN_PART(arguments, d_delta), p, channel), d_gate_lanes(SCAN_PART(arguments, d_gate), p, channel);
+        ask(min(row + a.row_groups, a.batch - 1));
+        rlt_lds_barrier();
+        each<0, K>([&](auto which) {
+            constexpr int j = decltype(which)::value;
+            if (j < steps) {
+                const float dt = from_lane<j>(delta), u = from_lane<j>(added);
+                const bool begins = forget >> j & 1;
+                float b[NPT];
+                read<NPT>(shared[turn][0] + n0 + j * N, b);
+#pragma unroll
+                for (int n = 0; n < NPT; n++) {
+                    decay[j][n] = __builtin_amdgcn_exp2f(dt * rate[n]);
+                    h[j][n] = begins ? u * b[n] : fmaf(decay[j][n], j ? h[j ? j - 1 : 0][n] : before[n], u * b[n]);
+                }
+            }
+        });
+        float mixed_part[4], through_part[4], exponent_part[4], kept_b[KEPT], kept_c[KEPT];
+#pragma unroll
+        for (int m = 0; m < KEPT; m++) kept_b[m] = kept_c[m] = 0.0f;
+        each<0, K>([&](auto which) {
+            constexpr int j = K - 1 - decltype(which)::value;
+            mixed_part[j] = through_part[j] = exponent_part[j] = 0.0f;
+            if (j < steps) {
+                const float dt = from_lane<j>(delta), u = from_lane<j>(added), g = from_lane<j>(d);
+                const bool begins = forget >> j & 1;
+                float b[NPT], c[NPT], d_b[NPT], d_c[NPT];
+                read<NPT>(shared[turn][0] + n0 + j * N, b);
+                read<NPT>(shared[turn][1] + n0 + j * N, c);
+#pragma unroll
+                for (int n = 0; n < NPT; n++) {
+                    const float G = fmaf(c[n], g, carry[n]);
+                    d_c[n] = g * h[j][n];
+                    d_b[n] = u * G;
+                    mixed_part[j] = fmaf(c[n], h[j][n], mixed_part[j]);
+                    through_part[j] = fmaf(b[n], G, through_part[j]);
+                    carry[n] = begins ? 0.0f : decay[j][n] * G;
+                    const float old = j ? h[j ? j - 1 : 0][n] : before[n], q = begins ? 0.0f : carry[n] * old;
+                    exponent_part[j] = fmaf(rate[n], q, exponent_part[j]);
+                    d_rate[n] = fmaf(dt, q, d_rate[n]);
+                }
+                float sum_b[KEPT], sum_c[KEPT];
+                sum_channels<NPT>(d_b, sum_b);
+                sum_channels<NPT>(d_c, sum_c);
+#pragma unroll
+                for (int m = 0; m < KEPT; m++) { kept_b[m] = into_quad<j>(kept_b[m], sum_b[m]); kept_c[m] = into_quad<j>(kept_c[m], sum_c[m]); }
+            }
+        });
+        const float mixed = sum_to_lane(mixed_part, odd, upper), through = sum_to_lane(through_part, odd, upper), exponent = sum_to_lane(exponent_part, odd, upper);
+        const float d_delta = fmaf(exponent, LN_2, through * xs) * slope;
+        d_skip = fmaf(d, xs, d_skip);
+        d_bias += d_delta;
+        if (there && nq < a.steps) {
+            d_x_lanes.put(0, fmaf(through, delta, skip * d));
+            d_delta_lanes.put(0, d_delta);
+            if (gated) d_gate_lanes.put(0, by_gate * fmaf(skip, xs, mixed));
+        }
+#pragma unroll
+        for (int m = 0; m < KEPT; m++) { slabs[turn][wave][0][quad * N + kept_state + m] = kept_b[m]; slabs[turn][wave][1][quad * N + kept_state + m] = kept_c[m]; }
+        rlt_lds_barrier();
+        const int element = threadIdx.x, step = element / N, n = element % N;
+        if (step < a.steps && element < K * N) {
+            float d_b = 0.0f, d_c = 0.0f;
+#pragma unroll
+            for (int w = 0; w < WAVES; w++) { d_b += slabs[turn][w][0][element]; d_c += slabs[turn][w][1][element]; }
+            if constexpr (ONE_TILE) {
+                if (n < a.states) {
+                    at<T>(a.d_b, step, row, p.head)[n] = (T)d_b;
+                    at<T>(a.d_c, step, row, p.head)[n] = (T)d_c;
+                }
+            } else {
+                float* const to = a.d_shared + ((size_t)p.tile * 2 * a.batch * a.heads + pair) * a.steps * N + element;
+                to[0] = d_b;
+                to[(size_t)a.batch * a.heads * a.steps * N] = d_c;
+            }
+        }
+        if (there && a.exit) store_states<NPT>(a.exit + (pair * a.channels + channel) * a.states, n0, a.states, carry);
+    }
+    if (!there) return;
+    const size_t of_channel = ((size_t)group * a.heads + p.head) * a.channels + channel;
     if (a.d_rates) write<NPT>(a.d_rates + of_channel * N + n0, d_rate);
     d_skip = sum_of_lanes(d_skip); d_bias = sum_of_lanes(d_bias);
     if (nq == 0 && a.d_skips) a.d_skips[of_channel] = d_skip;
@@ -1014,10 +1157,10 @@ int rlt_rocm_selective_scan_backward(rlt_rocm_device* device, const rlt_selectiv
             a.entry = f.exit; a.entry_padded = 1;
         }
         const dim3 blocks(blocks_of(a, a.row_groups));
-        if (a.tiles == 1 && steps <= 4) hipLaunchKernelGGL((backward_kernel<T, NPT, true, 4>), blocks, dim3(LANES), 0, device->stream, a);
-        else if (a.tiles == 1) hipLaunchKernelGGL((backward_kernel<T, NPT, true, CHUNK<NPT>>), blocks, dim3(LANES), 0, device->stream, a);
-        else if (steps <= 4) hipLaunchKernelGGL((backward_kernel<T, NPT, false, 4>), blocks, dim3(LANES), 0, device->stream, a);
-        else hipLaunchKernelGGL((backward_kernel<T, NPT, false, CHUNK<NPT>>), blocks, dim3(LANES), 0, device->stream, a);
+        if (a.tiles == 1 && steps <= 4) hipLaunchKernelGGL((short_backward_kernel<T, NPT, true>), blocks, dim3(LANES), 0, device->stream, a);
+        else if (a.tiles == 1) hipLaunchKernelGGL((backward_kernel<T, NPT, true>), blocks, dim3(LANES), 0, device->stream, a);
+        else if (steps <= 4) hipLaunchKernelGGL((short_backward_kernel<T, NPT, false>), blocks, dim3(LANES), 0, device->stream, a);
+        else hipLaunchKernelGGL((backward_kernel<T, NPT, false>), blocks, dim3(LANES), 0, device->stream, a);
         if ((rc = rlt_launch_status(device))) return rc;
         const size_t channels = (size_t)layer->heads * layer->channels, shared = a.tiles > 1 ? (size_t)2 * a.batch * a.heads * steps * 4 * NPT : 0;
         auto blocks_for = [](size_t columns) { return (columns + RLT_JOIN_COLUMNS - 1) / RLT_JOIN_COLUMNS; };
