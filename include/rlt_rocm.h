@@ -1319,6 +1319,7 @@ int rlt_rocm_causal_convolution_step(rlt_rocm_device* device, const rlt_causal_c
 /* Selective scan, a recurrent layer of `states` numbers for each channel, whose decays, inputs and outputs depend on the step:
  *     delta_t = log(1 + exp(raw_t + delta_biases)),   h_t[n] = exp(-exp(log_rates[n]) * delta_t) * h_{t-1}[n] + delta_t * x_t * b_t[n]   (nothing of h_{t-1} at a reset),
  *     output_t = (sum over n of c_t[n] * h_t[n] + skip * x_t) * gate_t / (1 + exp(-gate_t)).
+ * with exp(log_rates) as 1e30 where it is more.
  * x, raw (the view `delta`), gate and output are [steps x batch x heads x channels], b and c [steps x batch x heads x states], shared by a head's channels. States (at most 32) are fp32
  * [batch x heads x channels x states]. Sequences up to 2^30 steps, 2^27 elements between them at the most, heads x channels up to 2^20, batch x heads x channels x 32 up to 2^31 and steps x batch x heads up to 2^31; anything beyond is RLT_E_UNSUPPORTED before anything is launched. */
 typedef struct rlt_selective_scan {

@@ -272,11 +272,16 @@ template <int NPT> __device__ __forceinline__ void store_states(float* to, int n
         for (int n = 0; n < NPT; n++) if (n0 + n < states) to[n0 + n] = h[n];
     }
 }
+// exp(log_rate), 1e30 at the most: a delta of zero, of a step that is not there, decays nothing then, whatever the rate, and what such a step would give a gradient, rate times a state and its gradient times zero, is zero
+__device__ __forceinline__ float rate_of(float log_rate) {
+    const float r = expf(log_rate);
+    return r > 1e30f ? 1e30f : r;
+}
 // logarithms of the decays to base 2 for a delta of one; nothing where there is no state
 template <int NPT> __device__ __forceinline__ void load_rates(const Scan& a, int head, int channel, int n0, float (&rate)[NPT]) {
     const float* const from = a.log_rates + ((size_t)head * a.channels + channel) * a.states;
 #pragma unroll
-    for (int n = 0; n < NPT; n++) rate[n] = n0 + n < a.states ? -expf(from[n0 + n]) * LOG2_E : 0.0f;
+    for (int n = 0; n < NPT; n++) rate[n] = n0 + n < a.states ? -rate_of(from[n0 + n]) * LOG2_E : 0.0f;
 }
 
 // Forward over a segment. STATES: only what the segment adds to the state, for states that segments start from.
@@ -469,7 +474,7 @@ template <bool REVERSE> __global__ __launch_bounds__(256) void join_segments_ker
     const int e = (int)(i - pair * per_pair), channel = e / padded, n = e - channel * padded;
     const bool there = n < a.states;
     const size_t at_channel = (pair % a.heads) * a.channels + channel;
-    const float rate = there ? -expf(a.log_rates[at_channel * a.states + n]) * LOG2_E : 0.0f;
+    const float rate = there ? -rate_of(a.log_rates[at_channel * a.states + n]) * LOG2_E : 0.0f;
     float carry = initial && there ? initial[(pair * a.channels + channel) * a.states + n] : 0.0f;
     constexpr int AHEAD = 8;      // segments whose shares are asked for before the first of them is used
     for (int k0 = 0; k0 < a.segments; k0 += AHEAD) {
@@ -946,7 +951,7 @@ template <typename T> __global__ __launch_bounds__(1024) void sum_kernel(Scan a,
         const int n = (int)(i - channel * padded);
         if (n >= a.states) return;
         to = d_log_rates + channel * a.states + n;
-        s *= -expf(a.log_rates[channel * a.states + n]);
+        s *= -rate_of(a.log_rates[channel * a.states + n]);
     }
     *to = accumulate ? *to + s : s;
 }

@@ -118,11 +118,11 @@ def bounds(c, x, want):
     return b
 
 
-def check(c, x, got, names=None):
+def check(c, x, got, names=None, underflow=0.0):
     want = reference(c, x)
     b = bounds(c, x, want)
     for n in names or got:
-        off = np.abs(got[n] - want[n]) - b[n]
+        off = np.abs(got[n] - want[n]) - b[n] - underflow
         assert np.all(off <= 0), (n, float(off.max()), float(np.abs(got[n] - want[n]).max()), float(np.abs(want[n]).max()))
 
 
@@ -263,6 +263,64 @@ def test_many_rows_in_another_order_and_episodes_that_are_not_finite(rocm, dtype
     for n in ("output", "d_x", "d_delta", "d_b", "d_c", "d_gate"):
         off = np.abs(got[n] - want[n]) <= b[n]
         assert np.all(off[40:, 0]) and np.all(off[:, 1]) and np.all(off[:40, 2]) and np.all(off[:, 3:]), n
+
+
+SHORT = [(1, 600, 8, 40, 8), (1, 700, 4, 130, 16), (2, 300, 8, 65, 16), (3, 150, 16, 130, 16), (4, 120, 8, 300, 32), (4, 500, 16, 9, 5), (3, 330, 16, 64, 27), (2, 3, 1, 1, 1)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("shape", SHORT)
+@pytest.mark.parametrize("kind", [dict(), dict(resets=0.3, ragged=True), dict(gate=False, with_state=False), dict(parameters=False, ragged=True)])
+def test_few_steps_of_many_rows(rocm, shape, dtype, kind):
+    """rows that a workgroup goes through one after the other, some of them empty; what lies beyond a row's length is not looked at"""
+    print("case", shape, dtype, kind, flush=True)
+    c, x = case(sum(shape), dtype, *shape, **kind)
+    clean = {n: a.copy() for n, a in x.items()}
+    if kind.get("ragged"):
+        beyond = np.arange(shape[0])[:, None] >= np.clip(x["lengths"], 0, shape[0])[None]
+        for i, n in enumerate(SEQUENCES):
+            if n in x:
+                x[n][beyond] = (np.nan, np.inf, -np.inf, np.nan, np.inf, -np.inf)[i]
+    first, second = run(rocm, c, x), run(rocm, c, x)
+    # Relative bounds end where fp32 does: states of rates up to 32 and deltas of three pass on e^-96 of a gradient a step, below 2^-126, where an operation's result may be zero instead, off by 2^-126 at most. On its way to an output such an error meets
+    # decays, which are at most one, at most two of the inputs (m is the largest) and a rate, and as many of its kind as there are operations: eight for each step and state or channel of the sum.
+    m, rate = max(np.abs(a).max() for n, a in clean.items() if n not in ("reset", "lengths", "log_rates")), np.exp(clean["log_rates"].max())
+    check(c, clean, first, underflow=2.0 ** -126 * 8 * shape[0] * (shape[1] + shape[3] + shape[4]) * (1 + m) ** 2 * (1 + rate))
+    assert all(np.array_equal(a, second[n]) for n, a in first.items())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("steps", [1, 3, 4])
+def test_few_steps_in_other_orders_and_states_that_a_reset_forgets(rocm, dtype, steps):
+    c, x = case(47 + steps, dtype, steps, 300, 8, 24, 16, resets=0.1)
+    check(c, x, run(rocm, c, x, order=(2, 1, 0), gap=3, offset=1))
+    x["reset"][0, 5] = 1
+    clean = run(rocm, c, x)
+    x["state"][5] = np.inf
+    got = run(rocm, c, x)
+    assert all(np.array_equal(got[n], clean[n]) for n in got)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("shape", [(3, 40, 1, 70, 16), (20, 5, 2, 70, 16), (300, 3, 1, 20, 12), (700, 1, 1, 70, 20)])
+def test_rates_that_leave_the_range(rocm, shape, dtype):
+    """a state that forgets all at every step that is there, and nothing at those that are not: exp(100) is infinite in 32 bits"""
+    c, x = case(51, dtype, *shape, ragged=True)
+    if shape[1] == 1:
+        x["lengths"][:] = shape[0] - 9
+    x["log_rates"][:, ::2, 1] = 100.0
+    got, want, f = run(rocm, c, x), reference(c, x), factors(x)
+    size = magnitudes(c, x, f)
+    E = np.where(f["rates"] < 1e30, f["rates"] * f["delta"][..., None], 0.0).sum(0).max()
+    unit = (4 * c["steps"] + 16 * E + 64 + c["channels"] + c["states"] + c["steps"] + c["rows"]) * U
+    for n in got:
+        limit = unit * size[n]
+        if dtype == "bfloat16" and n in ("output", "d_x", "d_delta", "d_b", "d_c", "d_gate"):
+            limit = limit + UNIT["bfloat16"] * (np.abs(want[n]) + limit)
+        assert np.isfinite(got[n]).all() and np.all(np.abs(got[n] - want[n]) <= limit), n
 
 
 @gpu
