@@ -238,15 +238,14 @@ template <typename T> struct Lanes {
     }
     __device__ __forceinline__ void put(int t, float v) const { *(GLOBAL T*)(base + (int64_t)t * stride + offset) = (T)v; }      // t: a multiple of four steps into a chunk
 };
-// a channel's states in the caller's memory; together where the lanes' shares come out even, from any element on
+// a channel's states in the caller's memory: a lane's together, from any element on, but for what is left to the last lane that has any
 template <int NPT> __device__ __forceinline__ void load_states(const float* from, int n0, int states, float (&h)[NPT]) {
     constexpr int V = NPT < 4 ? NPT : 4;
     typedef float vector __attribute__((ext_vector_type(V), aligned(4)));
-    if (states % NPT == 0) {
+    if (n0 + NPT <= states) {
 #pragma unroll
         for (int n = 0; n < NPT; n += V) {
-            vector v = (vector)0.0f;
-            if (n0 < states) v = *reinterpret_cast<const vector*>(from + n0 + n);
+            const vector v = *reinterpret_cast<const vector*>(from + n0 + n);
 #pragma unroll
             for (int i = 0; i < V; i++) h[n + i] = v[i];
         }
@@ -258,8 +257,7 @@ template <int NPT> __device__ __forceinline__ void load_states(const float* from
 template <int NPT> __device__ __forceinline__ void store_states(float* to, int n0, int states, const float (&h)[NPT]) {
     constexpr int V = NPT < 4 ? NPT : 4;
     typedef float vector __attribute__((ext_vector_type(V), aligned(4)));
-    if (states % NPT == 0) {
-        if (n0 >= states) return;
+    if (n0 + NPT <= states) {
 #pragma unroll
         for (int n = 0; n < NPT; n += V) {
             vector v;
@@ -394,15 +392,16 @@ template <typename T, int NPT, bool STATES> __global__ __launch_bounds__(LANES) 
     }
 }
 
-// Forward over sequences of four steps at most: a workgroup goes from one row to the next, whose inputs and state are on their way while it works.
-template <typename T, int NPT> __global__ __launch_bounds__(LANES) void short_forward_kernel(Scan a) {
-    constexpr int K = 4, N = 4 * NPT;
+// Forward over sequences of K steps at most, four or eight: a workgroup goes from one row to the next, whose inputs and state are on their way while it works (8 steps x 4,096 rows x 1,024 channels, bfloat16: 246 us, a workgroup for each row 458;
+// one step x 4,096 rows x 256 channels 40 and 54).
+template <typename T, int NPT, int K> __global__ __launch_bounds__(LANES) void short_forward_kernel(Scan a) {
+    constexpr int OWN = K / 4, N = 4 * NPT;
     __shared__ float shared[2][2][K * N];
     Place p = place_of(a, blockIdx.x, a.row_groups);
     const int group = p.row, nq = threadIdx.x & 3, n0 = nq * NPT, own_channel = p.tile * TILE + (int)(threadIdx.x >> 2), channel = min(own_channel, a.channels - 1);
     const bool there = own_channel < a.channels, gated = a.gate.data != nullptr, odd = nq & 1, upper = nq & 2;
     const size_t at_channel = (size_t)p.head * a.channels + channel;
-    T x[1], raw[1], gate[1] = {(T)0.0f};
+    T x[OWN], raw[OWN], gate[OWN];
     Resets<K> resets;
     Shared<T, NPT, K> next;
     float entry[NPT];
@@ -431,9 +430,16 @@ template <typename T, int NPT> __global__ __launch_bounds__(LANES) void short_fo
     for (int row = group; row < a.batch; row += a.row_groups, turn ^= 1) {
         const size_t pair = (size_t)row * a.heads + p.head;
         const int steps = live;
-        const bool whole = there && nq < steps;
-        float e, h[NPT];
-        const float xs = whole ? (float)x[0] : 0.0f, delta = softplus<T>(whole ? (float)raw[0] + bias : NO_DELTA, e), added = delta * xs, z = (float)gate[0];
+        float h[NPT], xs[OWN], delta[OWN], added[OWN], z[OWN];
+#pragma unroll
+        for (int i = 0; i < OWN; i++) {
+            const bool whole = there && 4 * i + nq < steps;
+            float e;
+            xs[i] = whole ? (float)x[i] : 0.0f;
+            delta[i] = softplus<T>(whole ? (float)raw[i] + bias : NO_DELTA, e);
+            added[i] = delta[i] * xs[i];
+            z[i] = gated && whole ? (float)gate[i] : 0.0f;
+        }
         const unsigned forget = resets.get(p, 0);
         next.template put<false, true, true>(a, p, 0, shared[turn]);
 #pragma unroll
@@ -443,12 +449,12 @@ template <typename T, int NPT> __global__ __launch_bounds__(LANES) void short_fo
         ask(min(row + a.row_groups, a.batch - 1));
         rlt_lds_barrier();
         if (a.checkpoints && there && steps > 0) write<NPT>(a.checkpoints + (pair * a.channels + channel) * N + n0, h);
-        float part[4];
+        float part[OWN][4];
         each<0, K>([&](auto which) {
             constexpr int j = decltype(which)::value;
-            part[j] = 0.0f;
+            part[j / 4][j % 4] = 0.0f;
             if (j < steps) {
-                const float d = from_lane<j>(delta), u = from_lane<j>(added);
+                const float d = from_lane<j % 4>(delta[j / 4]), u = from_lane<j % 4>(added[j / 4]);
                 float b[NPT], c[NPT];
                 read<NPT>(shared[turn][0] + n0 + j * N, b);
                 read<NPT>(shared[turn][1] + n0 + j * N, c);
@@ -456,13 +462,16 @@ template <typename T, int NPT> __global__ __launch_bounds__(LANES) void short_fo
 #pragma unroll
                 for (int n = 0; n < NPT; n++) {
                     h[n] = fmaf(__builtin_amdgcn_exp2f(d * rate[n]), begins ? 0.0f : h[n], u * b[n]);
-                    part[j] = fmaf(c[n], h[n], part[j]);
+                    part[j / 4][j % 4] = fmaf(c[n], h[n], part[j / 4][j % 4]);
                 }
             }
         });
-        float v = fmaf(skip, xs, sum_to_lane(part, odd, upper));
-        if (gated && whole) v *= gate_factor<T>(z);
-        if (there && nq < a.steps) out_lanes.put(0, v);
+#pragma unroll
+        for (int i = 0; i < OWN; i++) {
+            float v = fmaf(skip, xs[i], sum_to_lane(part[i], odd, upper));
+            if (gated) v *= gate_factor<T>(z[i]);
+            if (there && 4 * i + nq < a.steps) out_lanes.put(4 * i, v);
+        }
         if (there && a.exit) store_states<NPT>(a.exit + (pair * a.channels + channel) * a.states, n0, a.states, h);
     }
 }
@@ -698,9 +707,10 @@ template <typename T, int NPT, bool ONE_TILE> __global__ __launch_bounds__(LANES
     if (nq == 0 && a.d_biases) a.d_biases[of_channel] = d_bias;
 }
 
-// Backward over sequences of four steps at most, as backward_kernel, from one row to the next like short_forward_kernel.
-template <typename T, int NPT, bool ONE_TILE> __global__ __launch_bounds__(LANES, NPT > 4 ? 2 : 3) void short_backward_kernel(Scan a) {
-    constexpr int K = 4, N = 4 * NPT, KEPT = NPT > 4 ? NPT / 4 : 1;
+// Backward over sequences of K steps at most, as backward_kernel, from one row to the next like short_forward_kernel; nothing is computed for steps that are not there (both passes, 8 steps x 1,024 rows x 1,024 channels, fp32: 290 us, by whole
+// chunks 433; one step x 8,192 rows x 4 heads of 256: 770 and 1,760). Registers for three wavefronts a SIMD where the states of its steps leave them.
+template <typename T, int NPT, bool ONE_TILE, int K> __global__ __launch_bounds__(LANES, NPT * K > 16 ? 2 : 3) void short_backward_kernel(Scan a) {
+    constexpr int OWN = K / 4, N = 4 * NPT, KEPT = NPT > 4 ? NPT / 4 : 1;
     static_assert(K * N <= LANES, "");
     __shared__ float shared[2][2][K * N];
     __shared__ float slabs[2][WAVES][2][K * N];
@@ -709,7 +719,7 @@ template <typename T, int NPT, bool ONE_TILE> __global__ __launch_bounds__(LANES
     const int kept_state = n0 + (NPT >= 4 ? (lane >> 4 & 1) * (NPT / 4) : 0) + (lane >> 5) * (NPT / 2);
     const bool there = own_channel < a.channels, gated = a.gate.data != nullptr, odd = nq & 1, upper = nq & 2;
     const size_t at_channel = (size_t)p.head * a.channels + channel;
-    T x[1], raw[1], gate[1] = {(T)0.0f}, d_out[1];
+    T x[OWN], raw[OWN], gate[OWN], d_out[OWN];
     Resets<K> resets;
     Shared<T, NPT, K> next;
     float first_state[NPT], entry[NPT];
@@ -743,13 +753,23 @@ template <typename T, int NPT, bool ONE_TILE> __global__ __launch_bounds__(LANES
     for (int row = group; row < a.batch; row += a.row_groups, turn ^= 1) {
         const size_t pair = (size_t)row * a.heads + p.head;
         const int steps = live;
-        const bool whole = there && nq < steps;
-        float e, by_gate = 0.0f, h[K][NPT], decay[K][NPT], before[NPT], carry[NPT];
-        const float v = whole ? (float)raw[0] + bias : NO_DELTA, xs = whole ? (float)x[0] : 0.0f, delta = softplus<T>(v, e), large = reciprocal<T>(1.0f + e), slope = v >= 0.0f ? large : e * large, added = delta * xs;
-        float d = whole ? (float)d_out[0] : 0.0f;
-        if (gated) {
-            const float g = d;
-            d *= gate_factor<T>(whole ? (float)gate[0] : 0.0f, g, by_gate);
+        float by_gate[OWN], h[K][NPT], decay[K][NPT], before[NPT], carry[NPT], xs[OWN], delta[OWN], added[OWN], slope[OWN], d[OWN];
+#pragma unroll
+        for (int i = 0; i < OWN; i++) {
+            const bool whole = there && 4 * i + nq < steps;
+            float e;
+            const float v = whole ? (float)raw[i] + bias : NO_DELTA;
+            xs[i] = whole ? (float)x[i] : 0.0f;
+            delta[i] = softplus<T>(v, e);
+            const float large = reciprocal<T>(1.0f + e);
+            slope[i] = v >= 0.0f ? large : e * large;
+            added[i] = delta[i] * xs[i];
+            d[i] = whole ? (float)d_out[i] : 0.0f;
+            by_gate[i] = 0.0f;
+            if (gated) {
+                const float g = d[i];
+                d[i] *= gate_factor<T>(whole ? (float)gate[i] : 0.0f, g, by_gate[i]);
+            }
         }
         const unsigned forget = resets.get(p, 0);
         next.template put<false, true, true>(a, p, 0, shared[turn]);
@@ -762,7 +782,7 @@ template <typename T, int NPT, bool ONE_TILE> __global__ __launch_bounds__(LANES
         each<0, K>([&](auto which) {
             constexpr int j = decltype(which)::value;
             if (j < steps) {
-                const float dt = from_lane<j>(delta), u = from_lane<j>(added);
+                const float dt = from_lane<j % 4>(delta[j / 4]), u = from_lane<j % 4>(added[j / 4]);
                 const bool begins = forget >> j & 1;
                 float b[NPT];
                 read<NPT>(shared[turn][0] + n0 + j * N, b);
@@ -773,48 +793,51 @@ template <typename T, int NPT, bool ONE_TILE> __global__ __launch_bounds__(LANES
                 }
             }
         });
-        float mixed_part[4], through_part[4], exponent_part[4], kept_b[KEPT], kept_c[KEPT];
+        each<0, OWN>([&](auto group_of_four) {
+            constexpr int i = OWN - 1 - decltype(group_of_four)::value;
+            float mixed_part[4], through_part[4], exponent_part[4], kept_b[KEPT], kept_c[KEPT];
 #pragma unroll
-        for (int m = 0; m < KEPT; m++) kept_b[m] = kept_c[m] = 0.0f;
-        each<0, K>([&](auto which) {
-            constexpr int j = K - 1 - decltype(which)::value;
-            mixed_part[j] = through_part[j] = exponent_part[j] = 0.0f;
-            if (j < steps) {
-                const float dt = from_lane<j>(delta), u = from_lane<j>(added), g = from_lane<j>(d);
-                const bool begins = forget >> j & 1;
-                float b[NPT], c[NPT], d_b[NPT], d_c[NPT];
-                read<NPT>(shared[turn][0] + n0 + j * N, b);
-                read<NPT>(shared[turn][1] + n0 + j * N, c);
+            for (int m = 0; m < KEPT; m++) kept_b[m] = kept_c[m] = 0.0f;
+            each<0, 4>([&](auto which) {
+                constexpr int j = 3 - decltype(which)::value, s = 4 * i + j;
+                mixed_part[j] = through_part[j] = exponent_part[j] = 0.0f;
+                if (s < steps) {
+                    const float dt = from_lane<j>(delta[i]), u = from_lane<j>(added[i]), g = from_lane<j>(d[i]);
+                    const bool begins = forget >> s & 1;
+                    float b[NPT], c[NPT], d_b[NPT], d_c[NPT];
+                    read<NPT>(shared[turn][0] + n0 + s * N, b);
+                    read<NPT>(shared[turn][1] + n0 + s * N, c);
 #pragma unroll
-                for (int n = 0; n < NPT; n++) {
-                    const float G = fmaf(c[n], g, carry[n]);
-                    d_c[n] = g * h[j][n];
-                    d_b[n] = u * G;
-                    mixed_part[j] = fmaf(c[n], h[j][n], mixed_part[j]);
-                    through_part[j] = fmaf(b[n], G, through_part[j]);
-                    carry[n] = begins ? 0.0f : decay[j][n] * G;
-                    const float old = j ? h[j ? j - 1 : 0][n] : before[n], q = begins ? 0.0f : carry[n] * old;
-                    exponent_part[j] = fmaf(rate[n], q, exponent_part[j]);
-                    d_rate[n] = fmaf(dt, q, d_rate[n]);
+                    for (int n = 0; n < NPT; n++) {
+                        const float G = fmaf(c[n], g, carry[n]);
+                        d_c[n] = g * h[s][n];
+                        d_b[n] = u * G;
+                        mixed_part[j] = fmaf(c[n], h[s][n], mixed_part[j]);
+                        through_part[j] = fmaf(b[n], G, through_part[j]);
+                        carry[n] = begins ? 0.0f : decay[s][n] * G;
+                        const float old = s ? h[s ? s - 1 : 0][n] : before[n], q = begins ? 0.0f : carry[n] * old;
+                        exponent_part[j] = fmaf(rate[n], q, exponent_part[j]);
+                        d_rate[n] = fmaf(dt, q, d_rate[n]);
+                    }
+                    float sum_b[KEPT], sum_c[KEPT];
+                    sum_channels<NPT>(d_b, sum_b);
+                    sum_channels<NPT>(d_c, sum_c);
+#pragma unroll
+                    for (int m = 0; m < KEPT; m++) { kept_b[m] = into_quad<j>(kept_b[m], sum_b[m]); kept_c[m] = into_quad<j>(kept_c[m], sum_c[m]); }
                 }
-                float sum_b[KEPT], sum_c[KEPT];
-                sum_channels<NPT>(d_b, sum_b);
-                sum_channels<NPT>(d_c, sum_c);
-#pragma unroll
-                for (int m = 0; m < KEPT; m++) { kept_b[m] = into_quad<j>(kept_b[m], sum_b[m]); kept_c[m] = into_quad<j>(kept_c[m], sum_c[m]); }
+            });
+            const float mixed = sum_to_lane(mixed_part, odd, upper), through = sum_to_lane(through_part, odd, upper), exponent = sum_to_lane(exponent_part, odd, upper);
+            const float d_delta = fmaf(exponent, LN_2, through * xs[i]) * slope[i];
+            d_skip = fmaf(d[i], xs[i], d_skip);
+            d_bias += d_delta;
+            if (there && 4 * i + nq < a.steps) {
+                d_x_lanes.put(4 * i, fmaf(through, delta[i], skip * d[i]));
+                d_delta_lanes.put(4 * i, d_delta);
+                if (gated) d_gate_lanes.put(4 * i, by_gate[i] * fmaf(skip, xs[i], mixed));
             }
-        });
-        const float mixed = sum_to_lane(mixed_part, odd, upper), through = sum_to_lane(through_part, odd, upper), exponent = sum_to_lane(exponent_part, odd, upper);
-        const float d_delta = fmaf(exponent, LN_2, through * xs) * slope;
-        d_skip = fmaf(d, xs, d_skip);
-        d_bias += d_delta;
-        if (there && nq < a.steps) {
-            d_x_lanes.put(0, fmaf(through, delta, skip * d));
-            d_delta_lanes.put(0, d_delta);
-            if (gated) d_gate_lanes.put(0, by_gate * fmaf(skip, xs, mixed));
-        }
 #pragma unroll
-        for (int m = 0; m < KEPT; m++) { slabs[turn][wave][0][quad * N + kept_state + m] = kept_b[m]; slabs[turn][wave][1][quad * N + kept_state + m] = kept_c[m]; }
+            for (int m = 0; m < KEPT; m++) { slabs[turn][wave][0][(4 * i + quad) * N + kept_state + m] = kept_b[m]; slabs[turn][wave][1][(4 * i + quad) * N + kept_state + m] = kept_c[m]; }
+        });
         rlt_lds_barrier();
         const int element = threadIdx.x, step = element / N, n = element % N;
         if (step < a.steps && element < K * N) {
@@ -1129,7 +1152,8 @@ int rlt_rocm_selective_scan_forward(rlt_rocm_device* device, const rlt_selective
             a.entry = states; a.entry_padded = 1;
         }
         const dim3 blocks(blocks_of(a, a.batch));
-        if (steps <= 4) hipLaunchKernelGGL((short_forward_kernel<T, NPT>), dim3(blocks_of(a, a.row_groups)), dim3(LANES), 0, device->stream, a);
+        if (steps <= 4) hipLaunchKernelGGL((short_forward_kernel<T, NPT, 4>), dim3(blocks_of(a, a.row_groups)), dim3(LANES), 0, device->stream, a);
+        else if (steps <= 8) hipLaunchKernelGGL((short_forward_kernel<T, NPT, 8>), dim3(blocks_of(a, a.row_groups)), dim3(LANES), 0, device->stream, a);
         else hipLaunchKernelGGL((forward_kernel<T, NPT, false>), blocks, dim3(LANES), 0, device->stream, a);
         return rlt_launch_status(device);
     });
@@ -1162,10 +1186,14 @@ int rlt_rocm_selective_scan_backward(rlt_rocm_device* device, const rlt_selectiv
             a.entry = f.exit; a.entry_padded = 1;
         }
         const dim3 blocks(blocks_of(a, a.row_groups));
-        if (a.tiles == 1 && steps <= 4) hipLaunchKernelGGL((short_backward_kernel<T, NPT, true>), blocks, dim3(LANES), 0, device->stream, a);
-        else if (a.tiles == 1) hipLaunchKernelGGL((backward_kernel<T, NPT, true>), blocks, dim3(LANES), 0, device->stream, a);
-        else if (steps <= 4) hipLaunchKernelGGL((short_backward_kernel<T, NPT, false>), blocks, dim3(LANES), 0, device->stream, a);
-        else hipLaunchKernelGGL((backward_kernel<T, NPT, false>), blocks, dim3(LANES), 0, device->stream, a);
+        auto walk = [&](auto one_tile) {
+            constexpr bool ONE_TILE = decltype(one_tile)::value;
+            if (steps <= 4) hipLaunchKernelGGL((short_backward_kernel<T, NPT, ONE_TILE, 4>), blocks, dim3(LANES), 0, device->stream, a);
+            else if (steps <= 8) hipLaunchKernelGGL((short_backward_kernel<T, NPT, ONE_TILE, 8>), blocks, dim3(LANES), 0, device->stream, a);
+            else hipLaunchKernelGGL((backward_kernel<T, NPT, ONE_TILE>), blocks, dim3(LANES), 0, device->stream, a);
+        };
+        if (a.tiles == 1) walk(std::true_type{});
+        else walk(std::false_type{});
         if ((rc = rlt_launch_status(device))) return rc;
         const size_t channels = (size_t)layer->heads * layer->channels, shared = a.tiles > 1 ? (size_t)2 * a.batch * a.heads * steps * 4 * NPT : 0;
         auto blocks_for = [](size_t columns) { return (columns + RLT_JOIN_COLUMNS - 1) / RLT_JOIN_COLUMNS; };

@@ -314,7 +314,7 @@ def test_refusals_without_a_device():
     good = capi.CausalConvolution(4096, None, 4096, None, 0, 2, 8, 4, 1, 0)
     size = lambda steps=10, **fields: lib.rlt_rocm_causal_convolution_workspace_bytes(C.byref(capi.CausalConvolution(**dict({n: getattr(good, n) for n, _ in good._fields_}, **fields))), steps)
     assert size() > 0
-    assert size(d_weights=None) == size(0) == size(2 ** 30 + 1) == size(width=1) == size(width=9) == size(channels=0) == size(batch=-1) == size(type=2) == size(batch=2 ** 24, channels=2 ** 8) == 0
+    assert size(d_weights=None) == size(0) == size(2 ** 30 + 1) == size(width=1) == size(width=9) == size(channels=0) == size(batch=-1) == size(type=2) == size(batch=2 ** 24, channels=2 ** 8) == size(batch=1, channels=2 ** 22 + 1) == size(batch=2 ** 24 + 1, channels=1) == 0
     assert lib.rlt_rocm_causal_convolution_forward(None, C.byref(good), None, None, None, None, None, None, 4) == capi.RLT_E_NOT_INITIALISED
 
 

@@ -265,13 +265,12 @@ def test_many_rows_in_another_order_and_episodes_that_are_not_finite(rocm, dtype
         assert np.all(off[40:, 0]) and np.all(off[:, 1]) and np.all(off[:40, 2]) and np.all(off[:, 3:]), n
 
 
-SHORT = [(1, 600, 8, 40, 8), (1, 700, 4, 130, 16), (2, 300, 8, 65, 16), (3, 150, 16, 130, 16), (4, 120, 8, 300, 32), (4, 500, 16, 9, 5), (3, 330, 16, 64, 27), (2, 3, 1, 1, 1)]
+SHORT = [(5, 300, 8, 65, 16), (8, 150, 16, 130, 16), (7, 130, 16, 64, 27), (6, 400, 8, 20, 8), (1, 600, 8, 40, 8), (1, 700, 4, 130, 16), (2, 300, 8, 65, 16), (3, 150, 16, 130, 16), (4, 120, 8, 300, 32), (4, 500, 16, 9, 5), (3, 330, 16, 64, 27), (2, 3, 1, 1, 1)]
 
 
 @gpu
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
-@pytest.mark.parametrize("shape", SHORT)
-@pytest.mark.parametrize("kind", [dict(), dict(resets=0.3, ragged=True), dict(gate=False, with_state=False), dict(parameters=False, ragged=True)])
+@pytest.mark.parametrize("shape,kind", [(s, dict(resets=0.3, ragged=True)) for s in SHORT] + [(s, dict()) for s in SHORT[::3]] + [(s, k) for s in SHORT[:2] + SHORT[-2:] for k in (dict(gate=False, with_state=False), dict(parameters=False, ragged=True))])
 def test_few_steps_of_many_rows(rocm, shape, dtype, kind):
     """rows that a workgroup goes through one after the other, some of them empty; what lies beyond a row's length is not looked at"""
     print("case", shape, dtype, kind, flush=True)
@@ -292,7 +291,7 @@ def test_few_steps_of_many_rows(rocm, shape, dtype, kind):
 
 @gpu
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
-@pytest.mark.parametrize("steps", [1, 3, 4])
+@pytest.mark.parametrize("steps", [1, 3, 4, 6, 8])
 def test_few_steps_in_other_orders_and_states_that_a_reset_forgets(rocm, dtype, steps):
     c, x = case(47 + steps, dtype, steps, 300, 8, 24, 16, resets=0.1)
     check(c, x, run(rocm, c, x, order=(2, 1, 0), gap=3, offset=1))
@@ -531,7 +530,7 @@ def test_refusals_without_a_device():
     good = capi.SelectiveScan(4096, None, None, None, None, None, 0, 2, 1, 100, 16, 0)
     for size in (lambda layer, steps: lib.rlt_rocm_selective_scan_workspace_bytes(layer, steps, 1), lib.rlt_rocm_selective_scan_checkpoint_bytes):
         assert size(C.byref(good), 40) > 0
-        for layer in (None, changed(good, states=33), changed(good, states=0), changed(good, channels=0), changed(good, type=2), changed(good, batch=2 ** 20, channels=2 ** 10), changed(good, batch=2 ** 30, heads=2 ** 30)):
+        for layer in (None, changed(good, heads=2, channels=2 ** 20), changed(good, batch=1, heads=1, channels=2 ** 20 + 1), changed(good, states=33), changed(good, states=0), changed(good, channels=0), changed(good, type=2), changed(good, batch=2 ** 20, channels=2 ** 10), changed(good, batch=2 ** 30, heads=2 ** 30)):
             assert size(layer, 40) == 0
         assert size(C.byref(good), 0) == size(C.byref(good), 2 ** 30 + 1) == size(changed(good, batch=64), 2 ** 26) == 0
     assert lib.rlt_rocm_selective_scan_forward(None, C.byref(good), *[None] * 6, None, None, None, None, 4, None, None, 0) == capi.RLT_E_NOT_INITIALISED
