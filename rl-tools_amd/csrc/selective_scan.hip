@@ -392,8 +392,8 @@ template <typename T, int NPT, bool STATES> __global__ __launch_bounds__(LANES) 
     }
 }
 
-// Forward over sequences of K steps at most, four or eight: a workgroup goes from one row to the next, whose inputs and state are on their way while it works (8 steps x 4,096 rows x 1,024 channels, bfloat16: 246 us, a workgroup for each row 458;
-// one step x 4,096 rows x 256 channels 40 and 54).
+// Forward over sequences of K steps at most, four or eight: a workgroup goes from one row to the next, whose inputs and state are on their way while it works (8 steps x 4,096 rows x 1,024 channels, bfloat16: 240 us, a workgroup for each row 458;
+// one step x 4,096 rows x 256 channels 40 and 54; two rows on their way: no faster).
 template <typename T, int NPT, int K> __global__ __launch_bounds__(LANES) void short_forward_kernel(Scan a) {
     constexpr int OWN = K / 4, N = 4 * NPT;
     __shared__ float shared[2][2][K * N];
@@ -707,8 +707,8 @@ template <typename T, int NPT, bool ONE_TILE> __global__ __launch_bounds__(LANES
     if (nq == 0 && a.d_biases) a.d_biases[of_channel] = d_bias;
 }
 
-// Backward over sequences of K steps at most, as backward_kernel, from one row to the next like short_forward_kernel; nothing is computed for steps that are not there (both passes, 8 steps x 1,024 rows x 1,024 channels, fp32: 290 us, by whole
-// chunks 433; one step x 8,192 rows x 4 heads of 256: 770 and 1,760). Registers for three wavefronts a SIMD where the states of its steps leave them.
+// Backward over sequences of K steps at most, as backward_kernel, from one row to the next like short_forward_kernel; nothing is computed for steps that are not there (both passes, 8 steps x 1,024 rows x 1,024 channels, fp32: 280 us, by whole
+// chunks 433; one step x 8,192 rows x 4 heads of 256: 700 and 1,760). Registers for three wavefronts a SIMD where the states of its steps leave them.
 template <typename T, int NPT, bool ONE_TILE, int K> __global__ __launch_bounds__(LANES, NPT * K > 16 ? 2 : 3) void short_backward_kernel(Scan a) {
     constexpr int OWN = K / 4, N = 4 * NPT, KEPT = NPT > 4 ? NPT / 4 : 1;
     static_assert(K * N <= LANES, "");
