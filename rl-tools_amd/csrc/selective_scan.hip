@@ -270,7 +270,7 @@ template <int NPT> __device__ __forceinline__ void store_states(float* to, int n
         for (int n = 0; n < NPT; n++) if (n0 + n < states) to[n0 + n] = h[n];
     }
 }
-// exp(log_rate), 1e30 at the most: a delta of zero, of a step that is not there, decays nothing then, whatever the rate, and what such a step would give a gradient, rate times a state and its gradient times zero, is zero
+// exp(log_rate), 1e30 at the most: a delta of zero, of a step that is not there, decays nothing then, whatever the rate (infinity times zero would be no number)
 __device__ __forceinline__ float rate_of(float log_rate) {
     const float r = expf(log_rate);
     return r > 1e30f ? 1e30f : r;
@@ -375,7 +375,7 @@ template <typename T, int NPT, bool STATES> __global__ __launch_bounds__(LANES) 
                 const int s = t + 4 * i + nq;
                 float v = fmaf(skip, xs[i], y[i]);
                 if (gated) v *= gate_factor<T>(gates[i]);
-                if (there && s < p.end) out_lanes.put(t + 4 * i, v);      // (steps beyond the row's length: no input and nothing read, zero)
+                if (there && s < p.end) out_lanes.put(t + 4 * i, s < p.live ? v : 0.0f);      // (nothing read times a state that is infinite is no zero)
             }
         }
     }
@@ -591,11 +591,13 @@ template <typename T, int NPT, bool ONE_TILE> __global__ __launch_bounds__(LANES
             const int t = p.first + k * K;
             float xs[OWN], delta[OWN], added[OWN], slope[OWN], d[OWN], by_gate[OWN];      // by_gate: the gate's gradient but for what it multiplies
             float h[K][NPT], decay[K][NPT], before[NPT];
-            const unsigned forget = resets.get(p, t);
+            const unsigned forget = resets.get(p, t), passed = forget | (t + K > p.live ? ~0u << (p.live - t) : 0u);      // steps that add nothing to the rates' gradients: of another episode before them, or not there
             next.template put<true, true, true>(a, p, t, shared[turn]);
-            if (!all_there) {
+            if (!all_there && !there) {      // (lanes beyond the channels have another's state, which may be infinite)
 #pragma unroll
-                for (int i = 0; i < OWN; i++) if (!there) { x[i] = gate[i] = d_out[i] = (T)0.0f; raw[i] = (T)NO_DELTA; }
+                for (int i = 0; i < OWN; i++) { x[i] = gate[i] = d_out[i] = (T)0.0f; raw[i] = (T)NO_DELTA; }
+#pragma unroll
+                for (int n = 0; n < NPT; n++) first_state[n] = carry[n] = 0.0f;
             }
 #pragma unroll
             for (int n = 0; n < NPT; n++) before[n] = first_state[n];
@@ -649,7 +651,7 @@ template <typename T, int NPT, bool ONE_TILE> __global__ __launch_bounds__(LANES
                         const int s = 4 * i + j;
                         __builtin_amdgcn_sched_barrier(0);
                         const float dt = from_lane<j>(delta[i]), u = from_lane<j>(added[i]), g = from_lane<j>(d[i]);
-                        const bool begins = RESETS && bit(forget, s);
+                        const bool begins = RESETS && bit(forget, s), adds_nothing = RESETS && bit(passed, s);
                         float b[NPT], c[NPT], d_b[NPT], d_c[NPT];
                         read<NPT>(bs + s * N, b);
                         read<NPT>(cs + s * N, c);
@@ -662,7 +664,7 @@ template <typename T, int NPT, bool ONE_TILE> __global__ __launch_bounds__(LANES
                             mixed_part[j] = fmaf(c[n], h[s][n], mixed_part[j]);
                             through_part[j] = fmaf(b[n], G, through_part[j]);
                             carry[n] = begins ? 0.0f : decay[s][n] * G;
-                            const float old = s ? h[s ? s - 1 : 0][n] : before[n], q = begins ? 0.0f : carry[n] * old;
+                            const float old = s ? h[s ? s - 1 : 0][n] : before[n], q = adds_nothing ? 0.0f : carry[n] * old;
                             exponent_part[j] = fmaf(rate[n], q, exponent_part[j]);
                             d_rate[n] = fmaf(dt, q, d_rate[n]);
                         }
@@ -674,19 +676,20 @@ template <typename T, int NPT, bool ONE_TILE> __global__ __launch_bounds__(LANES
                     };
                     step(std::integral_constant<int, 3>{}); step(std::integral_constant<int, 2>{}); step(std::integral_constant<int, 1>{}); step(std::integral_constant<int, 0>{});
                     const float mixed = sum_to_lane(mixed_part, odd, upper), through = sum_to_lane(through_part, odd, upper), exponent = sum_to_lane(exponent_part, odd, upper);
-                    const float d_delta = fmaf(exponent, LN_2, through * xs[i]) * slope[i];
+                    const bool live = !RESETS || t + 4 * i + nq < p.live;      // (nothing times a state or a gradient that is infinite is no zero)
+                    const float d_delta = live ? fmaf(exponent, LN_2, through * xs[i]) * slope[i] : 0.0f;
                     d_skip = fmaf(d[i], xs[i], d_skip);
                     d_bias += d_delta;
                     if (there && t + 4 * i + nq < p.end) {
-                        d_x_lanes.put(t + 4 * i, fmaf(through, delta[i], skip * d[i]));
+                        d_x_lanes.put(t + 4 * i, live ? fmaf(through, delta[i], skip * d[i]) : 0.0f);
                         d_delta_lanes.put(t + 4 * i, d_delta);
-                        if (gated) d_gate_lanes.put(t + 4 * i, by_gate[i] * fmaf(skip, xs[i], mixed));
+                        if (gated) d_gate_lanes.put(t + 4 * i, live ? by_gate[i] * fmaf(skip, xs[i], mixed) : 0.0f);
                     }
 #pragma unroll
                     for (int m = 0; m < KEPT; m++) { slabs[turn][wave][0][(4 * i + quad) * N + kept_state + m] = kept_b[m]; slabs[turn][wave][1][(4 * i + quad) * N + kept_state + m] = kept_c[m]; }
                 }
             };
-            if (forget) walk(std::true_type{}); else walk(std::false_type{});
+            if (passed) walk(std::true_type{}); else walk(std::false_type{});
             rlt_lds_barrier();
 #pragma unroll
             for (int j = 0; j < PER; j++) {
@@ -695,7 +698,8 @@ template <typename T, int NPT, bool ONE_TILE> __global__ __launch_bounds__(LANES
                     float d_b = 0.0f, d_c = 0.0f;
 #pragma unroll
                     for (int w = 0; w < WAVES; w++) { d_b += slabs[turn][w][0][e]; d_c += slabs[turn][w][1][e]; }
-                    store_shared(t, e, d_b, d_c);
+                    const bool live = t + e / N < p.live;
+                    store_shared(t, e, live ? d_b : 0.0f, live ? d_c : 0.0f);
                 }
             }
         }
@@ -751,6 +755,7 @@ template <typename T, int NPT, bool ONE_TILE, int K> __global__ __launch_bounds_
     load_rates<NPT>(a, p.head, channel, n0, rate);
 #pragma unroll
     for (int n = 0; n < NPT; n++) d_rate[n] = 0.0f;
+    const unsigned own = there ? ~0u : 0u;
     int turn = 0;
     for (int row = group; row < a.batch; row += a.row_groups, turn ^= 1) {
         const size_t pair = (size_t)row * a.heads + p.head;
@@ -776,7 +781,10 @@ template <typename T, int NPT, bool ONE_TILE, int K> __global__ __launch_bounds_
         const unsigned forget = resets.get(p, 0);
         next.template put<false, true, true>(a, p, 0, shared[turn]);
 #pragma unroll
-        for (int n = 0; n < NPT; n++) { before[n] = first_state[n]; carry[n] = entry[n]; }
+        for (int n = 0; n < NPT; n++) {      // (lanes beyond the channels have another's state, which may be infinite: none)
+            before[n] = __builtin_bit_cast(float, __builtin_bit_cast(unsigned, first_state[n]) & own);
+            carry[n] = __builtin_bit_cast(float, __builtin_bit_cast(unsigned, entry[n]) & own);
+        }
         const Arguments arguments;
         const Lanes<T> d_x_lanes(SCAN_PART(arguments, d_x), p, channel), d_delta_lanes(SCAN_PART(arguments, d_delta), p, channel), d_gate_lanes(SCAN_PART(arguments, d_gate), p, channel);
         ask(min(row + a.row_groups, a.batch - 1));

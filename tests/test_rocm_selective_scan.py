@@ -322,6 +322,87 @@ def test_rates_that_leave_the_range(rocm, shape, dtype):
         assert np.isfinite(got[n]).all() and np.all(np.abs(got[n] - want[n]) <= limit), n
 
 
+ENDS = [(21, 12, 1, 20, 8), (21, 12, 2, 70, 16), (45, 12, 1, 16, 16), (22, 12, 1, 20, 20), (30, 12, 1, 70, 27), (700, 2, 1, 20, 16), (900, 2, 1, 70, 12), (6, 12, 2, 70, 16), (3, 12, 1, 20, 25)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("shape", ENDS)
+@pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
+def test_rows_that_end_in_a_state_or_a_gradient_that_is_not_finite(rocm, shape, dtype, bad):
+    """steps behind a row's last are exact zeros then too, and so is what they add to the parameters' gradients"""
+    print("case", shape, dtype, bad, flush=True)
+    steps, rows = shape[:2]
+    c, x = case(61 + sum(shape), dtype, *shape)
+    x["lengths"] = np.maximum(steps - 1 - np.arange(rows) % 11, 1).astype(np.int32)
+    beyond = np.arange(steps)[:, None] >= x["lengths"][None]
+    # a state that is not finite from a row's last step on, by an input of that step: what it gives the rates is finite, as the state before it is
+    clean = {n: a for n, a in x.items() if n != "d_state"}
+    by_input = dict(clean, b=x["b"].copy())
+    for r in range(rows):
+        by_input["b"][x["lengths"][r] - 1, r, 0, 0] = bad
+    want = reference(c, clean)
+    limit = bounds(c, clean, want)
+    got = run(rocm, c, by_input)
+    for n in ("output", "d_x", "d_delta", "d_b", "d_c", "d_gate"):
+        assert np.all(got[n][beyond] == 0.0), n
+    for n in ("d_log_rates", "d_skip"):
+        assert np.all(np.abs(got[n] - want[n]) <= limit[n]), n
+    # the gradient of the state behind the last step is not finite
+    by_gradient = dict(x, d_state=x["d_state"].copy())
+    by_gradient["d_state"][:, 0, 0, 0] = bad
+    got = run(rocm, c, by_gradient)
+    for n in ("output", "d_x", "d_delta", "d_b", "d_c", "d_gate"):
+        assert np.all(got[n][beyond] == 0.0), n
+    # channels whose states are finite keep their outputs and gradients
+    want = reference(c, x)
+    limit = bounds(c, x, want)
+    for n in ("output", "d_gate", "d_c"):      # (that need no gradient of the state)
+        assert np.all(np.abs(got[n] - want[n]) <= limit[n]), n
+    for n in ("d_x", "d_delta", "d_log_rates", "d_skip", "d_delta_biases"):
+        others = np.ones(want[n].shape, bool)
+        others[(Ellipsis, slice(0, 1), slice(0, 1), slice(None)) if n == "d_log_rates" else (Ellipsis, slice(0, 1), slice(0, 1))] = False
+        assert np.all(np.abs(got[n] - want[n])[others] <= limit[n][others]), n
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("shape", ENDS)
+def test_an_infinite_state_of_the_last_channel_is_infinite_in_the_sums_over_channels(rocm, shape, dtype):
+    """and no number where it is summed up with what lanes beyond the channels have"""
+    print("case", shape, dtype, flush=True)
+    c, x = case(63 + sum(shape), dtype, *shape)
+    x["log_rates"][:], x["delta"][:] = np.log(0.1), rounded(np.full(x["delta"].shape, -2.0), dtype)      # nothing is forgotten that counts: infinite states stay so
+    x["state"][:, :, -1, 0] = np.inf
+    got, want = run(rocm, c, x), reference(c, x)
+    assert np.isinf(want["d_c"][..., 0]).all() and np.array_equal(got["d_c"][..., 0], want["d_c"][..., 0])
+    x["state"][:, :, -1, 0] = 1.0
+    x["d_state"][:, :, -1, 0] = np.inf
+    got, want = run(rocm, c, x), reference(c, x)
+    assert np.isinf(want["d_b"][..., 0]).all() and np.array_equal(got["d_b"][..., 0], want["d_b"][..., 0])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("shape", ENDS)
+def test_rates_that_leave_the_range_with_large_states_and_gradients(rocm, shape, dtype):
+    """states and gradients of 1e5, whose product times the largest rate, 1e30, is beyond fp32: steps that are not there give nothing all the same"""
+    print("case", shape, dtype, flush=True)
+    c, x = case(67 + sum(shape), dtype, *shape)
+    x["lengths"] = np.maximum(c["steps"] - 1 - np.arange(c["rows"]) % 11, 1).astype(np.int32)
+    x["log_rates"][:, ::2, 1] = 100.0
+    x["b"], x["d_state"] = rounded(1e5 * x["b"], dtype), 1e5 * x["d_state"]
+    got, want, f = run(rocm, c, x), reference(c, x), factors(x)
+    size = magnitudes(c, x, f)
+    E = np.where(f["rates"] < 1e30, f["rates"] * f["delta"][..., None], 0.0).sum(0).max()
+    unit = (4 * c["steps"] + 16 * E + 64 + c["channels"] + c["states"] + c["steps"] + c["rows"]) * U
+    for n in got:
+        limit = unit * size[n]
+        if dtype == "bfloat16" and n in ("output", "d_x", "d_delta", "d_b", "d_c", "d_gate"):
+            limit = limit + UNIT["bfloat16"] * (np.abs(want[n]) + limit)
+        assert np.isfinite(got[n]).all() and np.all(np.abs(got[n] - want[n]) <= limit), n
+
+
 @gpu
 @pytest.mark.parametrize("order,gap,offset", [((1, 2, 0), 0, 0), ((2, 1, 0), 0, 0), ((1, 0, 2), 8, 0), ((0, 1, 2), 5, 3), ((0, 2, 1), 1, 1)])
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
