@@ -1373,6 +1373,8 @@ typedef struct rlt_muon_parameters {
  *     next_momentum = momentum_factor * momentum + gradient,   u = nesterov ? gradient + momentum_factor * next_momentum : next_momentum,   X = u / (|u| + epsilon) (Frobenius norm, in 64 bits),
  *     `iterations` times   A = X X^T,   X = a X + (b A + c A A) X   with (a, b, c) = (3.4445, -4.775, 2.0315),
  *     next_parameters = (1 - alpha * weight_decay) * parameters - alpha * sqrt(max(1, rows / cols)) * X.
+ * The products' factors have 22 bits: over the whole of X the error is that of fp32 products. Elements below 2^-25 of |u| keep fewer, one for each factor of two, so that rows and columns far below the others are further off relative to themselves: some 1e-6 to
+ * 6e-6 where they are a millionth of the others, 1e-4 to 6e-4 at 1e-8.
  * Up to 2^16 rows and columns and 2^30 elements to a matrix; anything beyond is RLT_E_UNSUPPORTED before anything is launched. The workspace starts on a 16-byte boundary and belongs to one call at a time;
  * its size (0 for a call that is refused) depends on the shapes alone. */
 size_t rlt_rocm_muon_workspace_bytes(const rlt_muon_tensor* tensors, int n);

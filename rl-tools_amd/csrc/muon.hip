@@ -4,13 +4,18 @@
 
 namespace {
 
-// Factors are held as two numbers of 16 bits, the value's nearest and what it leaves: 22 bits and a sign, whose products in the matrix instructions (high x high, high x low, low x high, summed up in fp32) are as good as fp32's own:
-// what is dropped, low x low and the rounding of the low part, is 2^-24.6 of a product in the mean (fp32's own rounding of a factor: 2^-25.3), at a third of the 16-bit rate, where fp32 instructions have a sixteenth.
-// Values are held times SCALE. Singular values stay below 1.21, those of A below 1.47, those of b A + c A A above -2.81 and below 0, so that no element leaves the range of 16 bits.
+// Factors are held as two numbers of 16 bits, the value's nearest and LOW times what it leaves: 22 bits and a sign, where fp32 has 24, for a third of the 16-bit rate in the matrix instructions; fp32 instructions have a sixteenth. Products are
+// high x high, high x low and low x high, summed up in fp32; what is dropped, low x low and the rounding of the low part, is 2^-24.6 of a product in the mean (fp32's own rounding of a factor: 2^-25.3). Over the whole update the error is fp32's, most of
+// it from the sums (512 x 1,024: 1.3e-6 of it, 2.0e-6 with fp32 products).
+// Values are held times SCALE. Singular values stay below 1.21, those of A below 1.47, those of b A + c A A above -2.81 and below 0, so that no element leaves the range of 16 bits. At its lower end the two parts do: elements keep their 22 bits down to
+// 2^-25 of the update's norm and lose one for each factor of two below. LOW moves that end: 2^9 is where rows and columns far below the others are best (as they are, 2^0, 2^-16 of the norm; half of the rows of 512 x 1,024 times 1e-6 of the others: 5.6e-4 of
+// theirs then, 1.1e-6 now, 4e-7 with fp32 products; times 1e-8: 5.6e-2 and 1.1e-4). Tiles whose registers hold one sum alone take the high parts times 2^-9 to the low ones, which costs such a product bits below 2^-20 of the factor's norm; more than 2^9
+// loses more there than the low parts gain. With sums apart 2^11 would be better still, in a second walk over k, as the registers do not hold both: two matrices of 4,096 columns 21.0 ms, 17.2 with the factors (16.8 without).
 typedef _Float16 f16;
 typedef f16 f16x8 __attribute__((ext_vector_type(8)));
 typedef rlt_f32x4 f32x4;
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+constexpr float LOW = 512.0f, UNLOW = 1.0f / LOW;
 constexpr float SCALE = 16384.0f, UNSCALE = 1.0f / 16384.0f, QA = 3.4445f, QB = -4.775f, QC = 2.0315f;
 constexpr int GROUP = 24, MAX_SIDE = 1 << 16, MAX_ITERATIONS = 32, PARTS = 256;      // matrices of a launch; partial sums of a norm
 constexpr int JOBS = 768;         // workgroups of a launch whose tiles are shared, at the most
@@ -63,7 +68,8 @@ __device__ __forceinline__ int tile_of(int block, int tiles) {
     const int tile = (block & 7) * ((tiles + 7) / 8) + (block >> 3);
     return block >> 3 < (tiles + 7) / 8 && tile < tiles ? tile : -1;
 }
-__device__ __forceinline__ void split(float v, f16& high, f16& low) { high = (f16)v; low = (f16)(v - (float)high); }
+__device__ __forceinline__ void split(float v, f16& high, f16& low) { high = (f16)v; low = (f16)((v - (float)high) * LOW); }
+__device__ __forceinline__ float whole(f16 high, f16 low) { return fmaf((float)low, UNLOW, (float)high); }
 
 // The momentum, and the sum of the update's squares in 64 bits (no square of an fp32 number leaves their range). VECTORS: four elements at a time, where all buffers start on 16-byte boundaries. Memory bounds it (84 million
 // elements: 172 us, 5.9 TB/s).
@@ -264,7 +270,7 @@ template <int PHASE> __device__ __forceinline__ void finish(const Tensors* tenso
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             v[e] = own[e] * UNSCALE;
-            const float add = PHASE == GRAM ? 0.0f : (float)added.high[h][e] + (float)added.low[h][e];
+            const float add = PHASE == GRAM ? 0.0f : whole(added.high[h][e], added.low[h][e]);
             if (PHASE == SQUARE) v[e] = fmaf(QC, v[e], QB * add);
             if (PHASE == UPDATE || PHASE == LAST) v[e] = fmaf(QA, add, v[e]);
             if (turned) own[e] = v[e];
@@ -359,7 +365,7 @@ template <int PHASE> __device__ __forceinline__ f32x16 small_sums(SmallStage* ld
             }
         }
     }
-    return sum[0] + (sum[1] + sum[2]);
+    return sum[0] + (sum[1] + sum[2]) * UNLOW;
 }
 template <int PHASE> __global__ __launch_bounds__(256, SYMMETRIC<PHASE> ? 2 : 1) void product_small_kernel(typename ArgumentsOf<PHASE>::type launch) {
     __shared__ __attribute__((aligned(16))) SmallStage lds[2];
@@ -417,13 +423,17 @@ template <int W, int PHASE> __global__ __launch_bounds__(256, W < 3 ? 2 : 1) voi
             f.qh[i] = fragment(2, wj * W + i); f.ql[i] = fragment(3, wj * W + i);
         }
     };
-    auto multiply = [&](const Fragments& f) {      // sums that follow each other in the matrix pipeline are not the same
+    auto multiply = [&](const Fragments& f) {      // the high parts of products with low ones by 1 / LOW; sums that follow each other in the matrix pipeline are not the same
+        f16x8 p[W], q[W];
 #pragma unroll
-        for (int term = 0; term < 3; term++)
+        for (int term = 0; term < 3; term++) {
+#pragma unroll
+            for (int i = 0; i < W; i++) { p[i] = term == 0 ? f.pl[i] : term == 1 ? f.ph[i] * (f16)UNLOW : f.ph[i]; q[i] = term == 0 ? f.qh[i] * (f16)UNLOW : term == 1 ? f.ql[i] : f.qh[i]; }
 #pragma unroll
             for (int i = 0; i < W; i++)
 #pragma unroll
-                for (int j = 0; j < W; j++) sum[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(term == 0 ? f.pl[i] : f.ph[i], term == 1 ? f.ql[j] : f.qh[j], sum[i][j], 0, 0, 0);
+                for (int j = 0; j < W; j++) sum[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[i], q[j], sum[i][j], 0, 0, 0);
+        }
     };
     auto put = [&](f16* to) {
 #pragma unroll
@@ -585,14 +595,14 @@ __global__ __launch_bounds__(1024) void local_kernel(Last launch) {
             sum[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, ql, sum[1], 0, 0, 0);
             sum[2] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl, qh, sum[2], 0, 0, 0);
         }
-        return sum[0] + (sum[1] + sum[2]);
+        return sum[0] + (sum[1] + sum[2]) * UNLOW;
     };
     // A lane has a column and, four by four, rows of it: column c of the sums as row c of what is written, which for A and b A + c A A is the same (sums are alike on both sides of the diagonal, bit by bit).
     typedef f16 f16x4 __attribute__((ext_vector_type(4)));
     auto get = [&](const f16* from, int low, int r, int c, float (&v)[4]) {
         const f16x4 h = *reinterpret_cast<const f16x4*>(from + at(c, r, 64)), l = *reinterpret_cast<const f16x4*>(from + low + at(c, r, 64));
 #pragma unroll
-        for (int e = 0; e < 4; e++) v[e] = (float)h[e] + (float)l[e];
+        for (int e = 0; e < 4; e++) v[e] = whole(h[e], l[e]);
     };
     auto put = [&](f16* to, int low, int r, int c, const float (&v)[4], f16x4& high, f16x4& rest) {
 #pragma unroll

@@ -169,6 +169,30 @@ def test_large_matrices(rocm, shapes):
         assert np.sqrt((error ** 2).mean()) <= 4 * np.sqrt(((x32 - x) ** 2).mean()) + U * np.sqrt((x ** 2).mean()), x.shape
 
 
+# Rows or columns far below the others. What is held, two parts of 16 bits, has a quantum of 2^-47 of the update's norm where the low part leaves its normal range: a root mean square of 2^-49 an element, sqrt(n) 2^-49 of a row of n. In tiles of 128
+# and more a product takes a factor's high part times 2^-9 with the other's low part, of at most 2^-11: 2^-15 (times 0.29) of 2^-14 there, by 2^-11 times 0.29 of the other factor: 2^-44 of that one's norm, which is as large as X's or, for A and
+# b A + c A A, ten times that with their coefficients. Both relative to the row as it is at the start (it grows as fast as the errors do); four as a factor of safety, and on top of four times what the same products in fp32 are off.
+WEAK = [((40, 200), 5), ((128, 256), 5), ((256, 128), 5), ((512, 1024), 5), ((1030, 1000), 5), ((2048, 2050), 2), ((8190, 2048), 2), ((2048, 8190), 2)]
+
+
+@gpu
+@pytest.mark.parametrize("shape,iterations", WEAK)
+@pytest.mark.parametrize("size", [2.0 ** -17, 2.0 ** -27])
+@pytest.mark.parametrize("side", [0, 1])
+def test_rows_and_columns_far_below_the_others(rocm, shape, iterations, size, side):
+    print("case", shape, size, side, flush=True)
+    t, p = tensors_of(29, [shape])[0], settings(alpha=1.0, momentum=0.0, weight_decay=0.0, nesterov=0, iterations=iterations, epsilon=0.0)
+    weak = (slice(None),) * side + (slice(shape[side] // 2, None),)
+    t["parameters"][:] = t["momentum"][:] = 0
+    t["gradient"][weak] *= np.float32(size)
+    got = run(rocm, [t], p)[0]
+    _, scale, x, x32, _ = reference(t, p)
+    error = np.linalg.norm((got["next_parameters"].astype(np.float64) / -scale - x)[weak]) / np.linalg.norm(x[weak])
+    plain = np.linalg.norm((x32 - x)[weak]) / np.linalg.norm(x[weak])
+    start = size / np.sqrt(shape[side] / 2)      # the norm of a weak row (or column) at the start
+    assert error <= 4 * plain + U + 4 * (np.sqrt(shape[1 - side]) * 2.0 ** -49 + 10 * 2.0 ** -44) / start, (error, plain)
+
+
 @gpu
 @pytest.mark.parametrize("size", [1e-30, 1e-12, 1e12, 1e30])
 def test_gradients_of_any_size(rocm, size):
