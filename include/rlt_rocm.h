@@ -1290,7 +1290,7 @@ int rlt_rocm_dropout(rlt_rocm_device* device, int type, const void* x, int ldx, 
 /* Short causal convolution over the steps, each channel with its own `width` (2 ... 8) weights, the step's own last:
  *     output_t[c] = act(biases[c] + sum over j < width of weights[c][width - 1 - j] * x_{t-j}[c]),   act: the identity, or z / (1 + exp(-z)) where `silu` is set.
  * Inputs of before the first step come from the state [batch x (width - 1) x channels] (fp32, the oldest first); inputs of before a reset are left out. Tensors are views whose channels lie
- * side by side (head_stride is not read). Sequences up to 2^30 steps, up to 2^22 channels and 2^24 rows, and as many rows x channels as 2^31 elements; anything beyond is RLT_E_UNSUPPORTED before anything is launched. */
+ * side by side (head_stride is not read). Sequences up to 2^30 steps, up to 2^22 channels and 2^24 rows, and fewer than 2^31 rows x channels; anything beyond is RLT_E_UNSUPPORTED before anything is launched. */
 typedef struct rlt_causal_convolution {
     const float* weights;        /* [channels x width] */
     const float* biases;         /* [channels]; NULL: zeros */
@@ -1321,7 +1321,7 @@ int rlt_rocm_causal_convolution_step(rlt_rocm_device* device, const rlt_causal_c
  *     output_t = (sum over n of c_t[n] * h_t[n] + skip * x_t) * gate_t / (1 + exp(-gate_t)).
  * with exp(log_rates) as 1e30 where it is more.
  * x, raw (the view `delta`), gate and output are [steps x batch x heads x channels], b and c [steps x batch x heads x states], shared by a head's channels. States (at most 32) are fp32
- * [batch x heads x channels x states]. Sequences up to 2^30 steps, 2^27 elements between them at the most, heads x channels up to 2^20, batch x heads x channels x 32 up to 2^31 and steps x batch x heads up to 2^31; anything beyond is RLT_E_UNSUPPORTED before anything is launched. */
+ * [batch x heads x channels x states]. Sequences up to 2^30 steps, 2^27 elements between them at the most, heads x channels up to 2^20, batch x heads below 2^24, batch x heads x channels x 32 up to 2^31 and steps x batch x heads up to 2^31; anything beyond is RLT_E_UNSUPPORTED before anything is launched. */
 typedef struct rlt_selective_scan {
     const float* log_rates;      /* [heads x channels x states] */
     const float* skip;           /* [heads x channels]; NULL: zeros */

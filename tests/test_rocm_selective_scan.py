@@ -460,6 +460,84 @@ def test_steps_from_tiny_to_huge_and_rates_from_none_to_all(rocm, dtype):
     assert np.isfinite(got["d_delta"]).all() and b is not None
 
 
+def underflow_of(c, x):
+    """Relative bounds end where fp32 does: what decays below 2^-126 may be zero instead, off by 2^-126 at most. On its way to an output such an error meets decays, which are at most one, at most two of the inputs (m is the largest) and a rate, and as many of
+    its kind as there are operations: eight for each step and state or channel of the sum."""
+    m, rate = max(np.abs(a).max() for n, a in x.items() if n not in ("reset", "lengths", "log_rates")), np.exp(x["log_rates"].max())
+    return 2.0 ** -126 * 8 * c["steps"] * (c["rows"] + c["channels"] + c["states"]) * (1 + m) ** 2 * (1 + rate)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("shape", [(20, 330, 8, 5, 16), (17, 300, 8, 9, 27), (33, 400, 8, 9, 8), (20, 150, 8, 65, 16), (9, 150, 8, 66, 20), (25, 280, 8, 7, 3), (100, 260, 8, 3, 16)])
+@pytest.mark.parametrize("kind", [dict(resets=0.1, ragged=True), dict(gate=False, with_state=False)])
+def test_long_rows_that_a_workgroup_goes_through_one_after_the_other(rocm, shape, dtype, kind):
+    """more rows than gradients' workgroups are made for, empty ones between full ones; what lies beyond a row's length is not looked at"""
+    print("case", shape, dtype, kind, flush=True)
+    steps, rows, heads, channels, states = shape
+    groups = 2048 // (heads * ((channels + 63) // 64))
+    assert groups < rows
+    c, x = case(71 + sum(shape), dtype, *shape, **kind)
+    if kind.get("ragged"):
+        x["lengths"][groups::7], x["lengths"][3::groups] = 0, steps
+    clean = {n: a.copy() for n, a in x.items()}
+    if kind.get("ragged"):
+        beyond = np.arange(steps)[:, None] >= np.clip(x["lengths"], 0, steps)[None]
+        for i, n in enumerate(SEQUENCES):
+            x[n][beyond] = (np.nan, np.inf, -np.inf, np.nan, np.inf, -np.inf)[i]
+        x["reset"][beyond] = 1
+    buffers = Buffers(rocm, c, x)
+    wide = 8 if states <= 8 else 16 if states <= 16 else 32
+    if channels <= 64:      # the workspace is for the workgroups' shares: fewer than there are rows
+        assert buffers.sizes[1] < rows * heads * channels * (wide + 2) * 4
+    first, second = run(rocm, c, x), run(rocm, c, x)
+    check(c, clean, first, underflow=underflow_of(c, clean))
+    assert all(np.array_equal(a, second[n]) for n, a in first.items())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("shape", [(40, 3, 1, 580, 16), (6, 5, 1, 1100, 9), (300, 1, 2, 520, 20)])
+def test_more_tiles_of_channels_than_are_added_up_at_a_time(rocm, shape, dtype):
+    print("case", shape, dtype, flush=True)
+    c, x = case(73 + sum(shape), dtype, *shape, resets=0.05, ragged=shape[1] > 1)
+    check(c, x, run(rocm, c, x), underflow=underflow_of(c, x))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_gradients_of_steps_from_tiny_to_huge_and_of_rates_from_none_to_all(rocm, dtype):
+    """as test_steps_from_tiny_to_huge_and_rates_from_none_to_all: what exponentials that leave the range of fp32 give delta and the parameters"""
+    c, x = case(13, dtype, 60, 2, 1, 16, 16)
+    x["delta"][:] = rounded(np.linspace(-120, 120, 16)[None, None, None] + np.zeros(x["delta"].shape), dtype)
+    x["log_rates"][0, :, 0] = -np.inf
+    x["log_rates"][0, :, 1] = 30.0
+    x["gate"][:] = rounded(np.linspace(-100, 100, 60)[:, None, None, None] + np.zeros(x["gate"].shape), dtype)
+    got, want, f = run(rocm, c, x), reference(c, x), factors(x)
+    unit, size = (4 * 60 + 16 * 60 + 64 + 32 + 62) * U, magnitudes(c, x, f)
+    # What is below fp32's smallest normal number, 2^-126, may be zero: a slope, off by 2^-126 at most, times what it is multiplied by, which are the magnitudes for a slope of one; a decay, in the product q = G decay h, and products with it on their way into the
+    # sums. G is a sum over steps of c, d_output and the gate's factor and of the last state's gradient, h of delta, x and b and of the first state, whose decays are at most one; q is multiplied by the rate and, in the rates' gradient, by delta (in delta's by a
+    # slope, at most one, and over the states). Four such roundings for each of 120 steps of rows.
+    m = {n: np.abs(a).max() for n, a in list(x.items()) + [("factor", f["factor"]), ("step", f["delta"])]}
+    G, h = 60 * m["c"] * m["d_output"] * m["factor"] + m["d_state"], 60 * m["step"] * m["x"] * m["b"] + m["state"]
+    of_decays = 4 * G * h * (1 + m["step"]) * f["rates"][0]      # [channels, states]
+    steep = magnitudes(c, x, dict(f, slope=np.ones_like(f["slope"])))["d_delta"] + of_decays.sum(-1)
+    lost = dict(d_delta=steep, d_delta_biases=steep.sum((0, 1)), d_log_rates=120 * of_decays, d_skip=np.abs(x["d_output"] * x["gate"] * x["x"]).sum((0, 1)))
+    for n, m in lost.items():
+        limit = unit * size[n] + 2.0 ** -125 * m
+        if dtype == "bfloat16" and n == "d_delta":
+            limit = limit + UNIT["bfloat16"] * (np.abs(want[n]) + limit) + 2.0 ** -126      # (below the smallest normal number of that type, too)
+        assert np.isfinite(got[n]).all() and np.all(np.abs(got[n] - want[n]) <= limit), (n, float((np.abs(got[n] - want[n]) - limit).max()))
+
+
+def test_the_rows_that_a_launch_holds():
+    """rows x heads below 2^24, beside the limits on elements"""
+    lib = package().load_library()
+    size = lambda *shape: lib.rlt_rocm_selective_scan_checkpoint_bytes(C.byref(capi.SelectiveScan(4096, None, None, None, None, None, 0, *shape, 0)), 4)
+    assert size(2 ** 24 - 1, 1, 1, 1) == (2 ** 24 - 1) * 8 * 4 and size(2 ** 23 - 1, 2, 4, 2) == (2 ** 23 - 1) * 2 * 4 * 8 * 4
+    assert size(2 ** 24, 1, 1, 1) == size(2 ** 23, 2, 4, 2) == 0
+
+
 @gpu
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 @pytest.mark.parametrize("steps", [150, 900])
