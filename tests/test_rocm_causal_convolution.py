@@ -174,6 +174,19 @@ def test_resets_and_lengths(rocm, shape, dtype, resets):
 
 
 @gpu
+@pytest.mark.parametrize("shape,dtype", [((24, 140, 4096, 4), "float32"), ((24, 140, 4095, 4), "float32"), ((20, 140, 8192, 3), "bfloat16"), ((17, 140, 8191, 2), "bfloat16"), ((100, 34, 4096, 3), "float32")])
+def test_rows_and_segments_that_a_thread_goes_through_one_after_the_other(rocm, shape, dtype):
+    """more of them than lanes, and segments of more steps than are on their way at a time; what lies beyond a row's length is not looked at"""
+    print("case", shape, dtype, flush=True)
+    c, x = case(sum(shape), dtype, *shape, resets=0.05, ragged=True)
+    beyond = np.arange(shape[0])[:, None] >= np.clip(x["lengths"], 0, shape[0])[None]
+    layer = layer_of(rocm, c, x, {})
+    assert workspace(rocm, layer, shape[0])[1] < shape[1] * (-(-shape[0] // 25)) * (shape[3] + 1) * shape[2] * 4      # fewer threads share a channel than there are rows and segments (of 25 steps at the most here)
+    got = run(rocm, c, dict(x, x=np.where(beyond[..., None], np.nan, x["x"]), d_output=np.where(beyond[..., None], np.inf, x["d_output"]), reset=np.where(beyond, 1, x["reset"]).astype(np.uint8)))
+    check(c, x, got)
+
+
+@gpu
 @pytest.mark.parametrize("gap,offset,order", [(5, 3, (0, 1, 2)), (8, 0, (0, 1, 2)), (1, 1, (1, 0, 2)), (0, 0, (1, 0, 2)), (16, 8, (1, 0, 2))])
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 def test_orders_gaps_and_alignments(rocm, gap, offset, order, dtype):
