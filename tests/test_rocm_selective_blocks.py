@@ -180,3 +180,33 @@ def test_training_runs(rocm, with_muon):
         net.backward(d)
         net.update(adam, muon if with_muon else None)
     assert np.isfinite(net.params.numpy()).all() and not np.array_equal(net.params.numpy(), np.concatenate([a.ravel() for a in p.values()]).astype(np.float32)[:net.total])
+
+
+@gpu
+@pytest.mark.parametrize("with_muon", [False, True])
+def test_every_tensor_moves_as_its_optimiser_says(rocm, with_muon):
+    """Two updates in a row by the definitions in 64 bits. Adam: what its bias corrections lose, 2 u / (1 - beta_2) of them, and some ten roundings of the update; Muon: as in test_rocm_muon"""
+    c, p, x, reset, net, tolerance, rng = case(rocm, 15, 24, 6, 32, 64, 1, 16, 4, 4, 2)
+    adam, muon = capi.adam_parameters(alpha=1e-3), capi.MuonParameters(alpha=1 / 64, momentum=15 / 16, weight_decay=1 / 8, epsilon=2.0 ** -23, nesterov=1, iterations=5)
+    u, one, two = 2.0 ** -24, np.float64(np.float32(0.9)), np.float64(np.float32(0.999))
+    m, v = {n: np.zeros(a.shape) for n, a in p.items()}, {n: np.zeros(a.shape) for n, a in p.items()}
+    for age in (1, 2):
+        out = net.forward(stream=0).numpy()
+        net.zero_gradient()
+        net.backward(rocm.array((out - 0.5 * x.reshape(out.shape)).astype(np.float32)))
+        before = {n: a.numpy().astype(np.float64) for n, a in net.param_views.items()}
+        net.update(adam, muon if with_muon else None)
+        for n, a in net.param_views.items():
+            g, after = net.grad_views[n].numpy().astype(np.float64), a.numpy().astype(np.float64)
+            assert np.any(after != before[n]), n
+            if with_muon and n.rstrip("0123456789") in SelectiveBlocks.MATRICES:
+                rows, cols = g.shape
+                m[n] = 15 / 16 * m[n] + g
+                scale = np.sqrt(max(1.0, rows / cols)) / 64
+                want = (1 - 1 / 512) * before[n] - scale * orthogonalised(g + 15 / 16 * m[n], 2.0 ** -23, 5)
+                assert np.linalg.norm((after - want) / scale, 2) <= 960 * u * (rows ** 0.5 + cols ** 0.5) * 200 + 3 * u / scale * np.linalg.norm(before[n]), n
+            else:
+                m[n], v[n] = one * m[n] + (1 - one) * g, two * v[n] + (1 - two) * g * g
+                step = 1e-3 * m[n] / (1 - one ** age) / (np.sqrt(np.maximum(v[n] / (1 - two ** age), 1e-7)) + 1e-7)
+                slack = 1e-3 * (np.abs(one * m[n]) + np.abs(g)) / (1 - one ** age) / (np.sqrt(np.maximum(v[n] / (1 - two ** age), 1e-7)) + 1e-7)
+                assert np.all(np.abs(after - (before[n] - step)) <= (2 * u / (1 - two) + 2 * u / (1 - one) + 16 * u) * slack + 2 * u * np.abs(before[n])), n
