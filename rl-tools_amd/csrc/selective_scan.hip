@@ -1059,11 +1059,11 @@ bool described(const rlt_selective_scan* p) {
 }
 int tiles_of(const rlt_selective_scan* p) { return (p->channels + TILE - 1) / TILE; }
 
-// Steps are cut into segments where rows, heads and channels alone leave the chip without work: up to four wavefronts to a SIMD, where they have fewer than two (a pass more over the steps is not worth less: 104 steps x 37 rows x 1,024 channels,
+// Steps are cut into segments, the same for both passes, where rows, heads and channels alone leave the chip without work: up to four wavefronts to a SIMD, where they have fewer than two (a pass more over the steps is not worth less: 104 steps x 37 rows x 1,024 channels,
 // forward and backward, 125 us whole, 146 in three segments). A chunk takes the passes over a segment some 6 us, and a segment the launches that chain them 0.6, one after the other: their sum is least, and flat, around four times the root of the
 // chunks (16,000 steps x 1 row x 64 channels: 172 us in 126 segments, 205 in 250, 620 in 1,000; 203 steps x 4 rows x 256 channels: 44 in 13, 75 in three).
 struct Segments { int count, steps, row_groups; };
-Segments segments_of(const rlt_selective_scan* p, int steps, bool backward) {
+Segments segments_of(const rlt_selective_scan* p, int steps) {
     const int chunk = chunk_of(p->states), chunks = (steps + chunk - 1) / chunk;
     const int64_t blocks = (int64_t)p->batch * p->heads * tiles_of(p), most = std::min((int64_t)(4.0 * std::sqrt((double)chunks)), (int64_t)chunks);
     const int64_t count = std::max(std::min(blocks >= 512 ? 1 : (1024 + blocks - 1) / blocks, most), (int64_t)1);
@@ -1077,14 +1077,14 @@ bool supported(const rlt_selective_scan* p, int steps) {
     if (p->states > MAX_STATES || steps > MAX_STEPS) return false;
     const __int128 pairs = (__int128)p->batch * p->heads, limit = (__int128)1 << 31;
     if (pairs * p->channels * MAX_STATES > limit || pairs * steps > limit || (int64_t)p->heads * p->channels > MAX_CHANNELS) return false;
-    const __int128 blocks = pairs * tiles_of(p) * segments_of(p, steps, false).count;
+    const __int128 blocks = pairs * tiles_of(p) * segments_of(p, steps).count;
     return blocks * LANES <= UINT32_MAX;
 }
 size_t padded(size_t n) { return (n + 63) / 64 * 64; }
 // scratch memory, in floats
 struct Scratch { size_t states, sums, shared, rates, skips, biases, total; };
 Scratch scratch_of(const rlt_selective_scan* p, int steps, bool backward) {
-    const Segments g = segments_of(p, steps, backward);
+    const Segments g = segments_of(p, steps);
     const size_t channels = (size_t)p->batch * p->heads * p->channels, wide = 4 * per_lane(p->states), parts = (size_t)g.row_groups * g.count * p->heads * p->channels;
     Scratch s{};
     size_t at = 0;
@@ -1098,8 +1098,8 @@ Scratch scratch_of(const rlt_selective_scan* p, int steps, bool backward) {
     return s;
 }
 Scan scan_of(const rlt_selective_scan* p, const rlt_head_view* x, const rlt_head_view* delta, const rlt_head_view* b, const rlt_head_view* c, const rlt_head_view* gate, const uint8_t* reset,
-             const int32_t* lengths, int steps, bool backward) {
-    const Segments g = segments_of(p, steps, backward);
+             const int32_t* lengths, int steps) {
+    const Segments g = segments_of(p, steps);
     Scan a{};
     a.log_rates = p->log_rates; a.skip = p->skip; a.delta_biases = p->delta_biases;
     a.x = rlt_part_of(x); a.delta = rlt_part_of(delta); a.b = rlt_part_of(b); a.c = rlt_part_of(c); a.gate = rlt_part_of(gate);
@@ -1147,7 +1147,7 @@ int rlt_rocm_selective_scan_forward(rlt_rocm_device* device, const rlt_selective
     if (!supported(layer, steps) || !near(x, delta, b, c, gate, output)) return RLT_E_UNSUPPORTED;
     const Scratch s = scratch_of(layer, steps, false);
     RLT_REQUIRE(s.total == 0 || (workspace && workspace_bytes >= s.total * sizeof(float) && reinterpret_cast<uintptr_t>(workspace) % 16 == 0));
-    Scan a = scan_of(layer, x, delta, b, c, gate, reset, lengths, steps, false);
+    Scan a = scan_of(layer, x, delta, b, c, gate, reset, lengths, steps);
     a.out = rlt_part_of(output); a.checkpoints = (float*)checkpoints; a.entry = initial_state; a.exit = final_state;
     return by_kind(layer, [&](auto type, auto n) {
         typedef decltype(type) T;
@@ -1180,7 +1180,7 @@ int rlt_rocm_selective_scan_backward(rlt_rocm_device* device, const rlt_selectiv
     const Scratch s = scratch_of(layer, steps, true);
     RLT_REQUIRE(workspace && workspace_bytes >= s.total * sizeof(float) && reinterpret_cast<uintptr_t>(workspace) % 16 == 0);
     float* const w = (float*)workspace;
-    Scan a = scan_of(layer, x, delta, b, c, gate, reset, lengths, steps, true);
+    Scan a = scan_of(layer, x, delta, b, c, gate, reset, lengths, steps);
     a.d_out = rlt_part_of(d_output); a.d_x = rlt_part_of(d_x); a.d_delta = rlt_part_of(d_delta); a.d_b = rlt_part_of(d_b); a.d_c = rlt_part_of(d_c); a.d_gate = rlt_part_of(d_gate);
     a.checkpoints = (float*)const_cast<void*>(checkpoints); a.entry = d_final_state; a.exit = d_initial_state;
     a.d_shared = w + s.shared; a.d_rates = layer->d_log_rates ? w + s.rates : nullptr; a.d_skips = layer->d_skip ? w + s.skips : nullptr; a.d_biases = layer->d_delta_biases ? w + s.biases : nullptr;
@@ -1220,7 +1220,7 @@ int rlt_rocm_selective_scan_step(rlt_rocm_device* device, const rlt_selective_sc
     if (!device) return RLT_E_NOT_INITIALISED;
     RLT_REQUIRE(given(layer, x, delta, b, c, gate) && rlt_given(output) && state && next_state);
     if (!supported(layer, 1)) return RLT_E_UNSUPPORTED;
-    Scan a = scan_of(layer, x, delta, b, c, gate, reset, nullptr, 1, false);
+    Scan a = scan_of(layer, x, delta, b, c, gate, reset, nullptr, 1);
     a.out = rlt_part_of(output); a.entry = state; a.exit = next_state;
     return by_kind(layer, [&](auto type, auto n) {
         typedef decltype(type) T;
