@@ -687,6 +687,10 @@ template <typename T, int NPT, bool ONE_TILE> __global__ __launch_bounds__(LANES
                         d_delta_lanes.put(t + 4 * i, d_delta);
                         if (gated) d_gate_lanes.put(t + 4 * i, live ? by_gate[i] * fmaf(skip, xs[i], mixed) : 0.0f);
                     }
+                    if (RESETS && t + 4 * i + quad >= p.live) {
+#pragma unroll
+                        for (int m = 0; m < KEPT; m++) kept_b[m] = kept_c[m] = 0.0f;
+                    }
 #pragma unroll
                     for (int m = 0; m < KEPT; m++) { slabs[turn][wave][0][(4 * i + quad) * N + kept_state + m] = kept_b[m]; slabs[turn][wave][1][(4 * i + quad) * N + kept_state + m] = kept_c[m]; }
                 }
@@ -700,8 +704,7 @@ template <typename T, int NPT, bool ONE_TILE> __global__ __launch_bounds__(LANES
                     float d_b = 0.0f, d_c = 0.0f;
 #pragma unroll
                     for (int w = 0; w < WAVES; w++) { d_b += slabs[turn][w][0][e]; d_c += slabs[turn][w][1][e]; }
-                    const bool live = t + e / N < p.live;
-                    store_shared(t, e, live ? d_b : 0.0f, live ? d_c : 0.0f);
+                    store_shared(t, e, d_b, d_c);
                 }
             }
         }
