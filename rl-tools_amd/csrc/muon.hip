@@ -384,7 +384,8 @@ template <int PHASE> __global__ __launch_bounds__(256, SYMMETRIC<PHASE> ? 2 : 1)
 }
 
 // Tiles of 64 W x 64 W: four wavefronts share one, each has W x W tiles of 32 x 32, factors come through LDS in stages of 32 k. Half a stage ahead: while the products of one half run, the other half's factors come from LDS, the next stage's go there
-// and the one after that is asked for, dealt out between the matrix instructions. 256 x 256: 1,138 TFLOP/s of 16-bit products at 4,096 x 20,480 x 4,096 (the clock is down to 1.7 GHz by then; a large library product: 1,080 to 1,135); the order brought 867 to 1,054 of it.
+// and the one after that is asked for, dealt out between the matrix instructions. 256 x 256: 1,100 to 1,126 TFLOP/s of 16-bit products at 4,096 x 20,480 x 4,096 (the clock is down to 1.6 GHz by then; a large library product: 1,080 to 1,135); the order brought 867 to 1,054 of
+// it, before high parts were scaled for the low ones (1,138 without). 65 registers a lane wait in scratch memory for what comes behind the loop; none is read within it.
 template <int W, int PHASE> __global__ __launch_bounds__(256, W < 3 ? 2 : 1) void product_kernel(typename ArgumentsOf<PHASE>::type launch) {
     constexpr int T = 64 * W, BK = 32, ROWS = 4 * T, LOADS = ROWS * 4 / 256, PRODUCTS = 3 * W * W, READS = 4 * W;      // rows of the tile in LDS: P high, P low, Q high, Q low
     extern __shared__ __attribute__((aligned(16))) f16 lds[];      // [2][ROWS][BK], chunks of eight changed about within a row so that the rows that are read together lie in different banks
@@ -708,7 +709,8 @@ template <int W, int PHASE> int length_of(const Entries& all) {
         if (jobs_of<W, PHASE>(all, length) <= (W == 1 ? JOBS : JOBS / 2)) return length;
     return WHOLE;
 }
-// Microseconds that a launch takes, round by round of 256 tiles: for 512 k of a tile with few others, with one on every compute unit, and for its sums' way out.
+// Microseconds that a launch takes, round by round of 256 tiles: for 512 k of a tile with few others, with one on every compute unit, and for its sums' way out. Against all four sizes measured, from one matrix of 256 x 256 to two of 4,096 columns, the size
+// that costs least is the fastest one or within 4 us of it (profiles/muon_tiles.txt).
 template <int W, int PHASE> double cost_of(const Entries& all) {
     constexpr double few[5] = {0, 5.5, 12, 15, 26}, full[5] = {0, 6.5, 14, 27, 46}, out[5] = {0, 3, 6, 18, 23};
     const int length = length_of<W, PHASE>(all);

@@ -284,8 +284,8 @@ template <int NPT> __device__ __forceinline__ void load_rates(const Scan& a, int
     for (int n = 0; n < NPT; n++) rate[n] = n0 + n < a.states ? -rate_of(from[n0 + n]) * LOG2_E : 0.0f;
 }
 
-// Forward over a segment. STATES: only what the segment adds to the state, for states that segments start from. The vector units bound it, 83 % busy with four wavefronts to a SIMD (16,384 steps x 4,096 channels x 16 states, bfloat16: 340 us,
-// 3.2e12 steps of a state a second; STATES 235).
+// Forward over a segment. STATES: only what the segment adds to the state, for states that segments start from. The vector units bound it, 83 % busy with four wavefronts to a SIMD (16,384 steps x 4,096 channels x 16 states, bfloat16: 350 us,
+// 3.1e12 steps of a state a second; STATES 237, 78 % busy).
 template <typename T, int NPT, bool STATES> __global__ __launch_bounds__(LANES) void forward_kernel(Scan a) {
     constexpr int K = CHUNK<NPT>, OWN = K / 4, N = 4 * NPT;
     __shared__ float shared[2][2][K * N];
@@ -510,7 +510,9 @@ template <bool REVERSE> __global__ __launch_bounds__(256) void join_segments_ker
 // Backward over a segment: from the last chunk to the first, the chunk's states again from its checkpoint, then its steps from the last to the first with the state's gradient G:
 //     G_t = c_t g_t + a_{t+1} G_{t+1},   g = d_output times the gate's factor;   d_c = sum over channels of g h,   d_b = sum over channels of delta x G,
 //     d_x = delta (G . b) + skip g,   d_delta = x (G . b) + rates . q,   d_rates += delta q   with q = G a h_{t-1}.
-// The vector units bound it, 77 % busy with two wavefronts to a SIMD, whose registers hold a chunk's states and decays (8,192 steps x 2 rows x 2,048 channels x 16 states, bfloat16: 525 us, 1.0e12 steps of a state a second).
+// The vector units bound it, 78 % busy with two wavefronts to a SIMD, whose registers hold a chunk's states and decays (8,192 steps x 2 rows x 2,048 channels x 16 states, bfloat16: 510 to 543 us, 1.0e12 steps of a state a second). What a row or a
+// chunk needs once goes to scratch memory, 12 to 68 bytes a lane with more than eight states; the steps read none of it. Steps that fill up a row's last chunk are taken out by selection: a branch around each sends a chunk's states to scratch memory
+// (944 bytes a lane, 3,455 us for both passes where they take 899).
 template <typename T, int NPT, bool ONE_TILE> __global__ __launch_bounds__(LANES, 2) void backward_kernel(Scan a) {
     constexpr int K = CHUNK<NPT>, OWN = K / 4, N = 4 * NPT, KEPT = NPT > 4 ? NPT / 4 : 1, PER = (K * N + LANES - 1) / LANES;
     __shared__ float shared[2][2][K * N];
