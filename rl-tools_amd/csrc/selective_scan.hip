@@ -721,7 +721,8 @@ template <typename T, int NPT, bool ONE_TILE> __global__ __launch_bounds__(LANES
 }
 
 // Backward over sequences of K steps at most, as backward_kernel, from one row to the next like short_forward_kernel; nothing is computed for steps that are not there (both passes, 8 steps x 1,024 rows x 1,024 channels, fp32: 280 us, by whole
-// chunks 433; one step x 8,192 rows x 4 heads of 256: 700 and 1,760). Registers for three wavefronts a SIMD where the states of its steps leave them.
+// chunks 433; one step x 8,192 rows x 4 heads of 256: 700 and 1,760). Registers for three wavefronts a SIMD where the states of its steps leave them (eight steps of more than
+// sixteen states send 8 to 12 a lane to scratch memory, 36 to 52 bytes).
 template <typename T, int NPT, bool ONE_TILE, int K> __global__ __launch_bounds__(LANES, NPT * K > 16 ? 2 : 3) void short_backward_kernel(Scan a) {
     constexpr int OWN = K / 4, N = 4 * NPT, KEPT = NPT > 4 ? NPT / 4 : 1;
     static_assert(K * N <= LANES, "");
